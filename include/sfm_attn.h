@@ -325,6 +325,76 @@ typedef struct sfm_linear_desc {
 int sfm_linear(const sfm_linear_desc* desc, const void* x, const void* w, const void* bias, const void* res, const void* gate,
                void* out, void* stream);
 
+/* Rows and weights in 8-bit blocks, the products that read them, and the gradients of the block's rows.  No counterpart in
+ * the reference, whose linear layers are 16 bits and whose gradients are autograd's.
+ *
+ * A block is 128 consecutive values of a row (of a weight: 128 x 128).  It has the smallest power of two 2^s with max |v| <= 448 *
+ * 2^s over its finite values (s = 0 for a block of zeros; s >= -126); a value is kept as e4m3 (OCP) of v * 2^-s, ties to even, one
+ * that is not finite as NaN.
+ *   rows     data: rows x SFM_PAD8(K) bytes, zeros past K.  scale: SFM_ROWS8_SCALE_BYTES(rows, K) bytes of s + 127; row r, block
+ *            column kb at ((kb * ceil(rows / 128) + r / 128) * 32 + r % 32) * 4 + r % 128 / 32.
+ *   weights  data: N x SFM_PAD8(K) bytes, scale: ceil(N / 128) rows of SFM_PITCH8(K) bytes; data_t, scale_t: the same of the
+ *            transposed weight [K, N] (the same values), for the product with the output's gradient.
+ * data and scale are 16-byte aligned.
+ *
+ * sfm_quantize8: data / scale of x [rows, K] (rows x_stride apart, any alignment).  colsum (NULL or float [ceil(rows / 128)][K])
+ *   receives the column sums of each 128 rows; y (NULL or [rows, K]): GELU (tanh) of x, rounded once.
+ *   data NULL: nothing is quantised.
+ * sfm_dequantize8: the values, rounded to the dtype (exact in bf16 and fp32 but for fp32-subnormal ones; fp16 saturates at 65504).
+ * sfm_pack8: a weight's data and scale, and data_t and scale_t unless both are NULL. */
+#define SFM_PAD8(n) (((int64_t)(n) + 127) / 128 * 128)
+#define SFM_PITCH8(n) (((int64_t)(n) + 511) / 512 * 4)
+#define SFM_ROWS8_SCALE_BYTES(rows, K) (((int64_t)(rows) + 127) / 128 * SFM_PAD8(K))
+int sfm_quantize8(int32_t dtype, int64_t rows, int32_t K, const void* x, int64_t x_stride, void* data, void* scale, void* y,
+                  int64_t y_stride, float* colsum, void* stream);
+int sfm_dequantize8(int32_t dtype, int64_t rows, int32_t K, const void* data, const void* scale, void* y, int64_t y_stride, void* stream);
+int sfm_pack8(int32_t dtype, int32_t N, int32_t K, const void* w, int64_t w_stride, void* data, void* scale, void* data_t,
+              void* scale_t, void* stream);
+
+/* out = x8 w8^T + bias with the epilogues of sfm_linear, on the 8-bit values of both operands with fp32 sums; bias, GELU and the
+ * gated residual follow on the fp32 sum, and the result is rounded once (sfm_linear rounds after each step).  Any N and K;
+ * rows of out, res, gate and bias may have any alignment.  x8 has M rows of K, w8 is a weight [N, K]; the input gradient of a
+ * layer is this product of the quantised output gradient with data_t, scale_t.  out must not overlap x8 or w8; res may be out. */
+typedef struct sfm_linear8_desc {
+    int32_t dtype;            /* SFM_BF16 | SFM_F16 : type of bias, res, gate and out */
+    int32_t epilogue;         /* SFM_EPI_* */
+    int64_t M;
+    int32_t N, K;
+    int64_t out_stride, res_stride, gate_stride;   /* elements */
+    int32_t rows_per_frame;   /* rows sharing one gate row */
+    int32_t reserved;
+} sfm_linear8_desc;
+int sfm_linear8(const sfm_linear8_desc* desc, const void* x8, const void* xscale, const void* w8, const void* wscale, const void* bias,
+                const void* res, const void* gate, void* out, void* stream);
+
+/* Gradients of a linear layer's weight and bias: dw[n][k] = sum_m dy[m][n] x[m][k] from the rows that the forward kept in 8 bits
+ * (dy as it is; [N, K] contiguous), dbias[n] = sum_m dy[m][n]; either may be NULL.  16-bit tensors, fp32 sums in a fixed order, one
+ * rounding.  colsum: dy's column sums where sfm_quantize8 has formed them (NULL: formed here, in the workspace). */
+int sfm_linear8_wgrad_workspace_bytes(int64_t M, int32_t N, int32_t K, size_t* bytes);
+int sfm_linear8_wgrad(int32_t dtype, int64_t M, int32_t N, int32_t K, const void* dy, int64_t dy_stride, const void* x8,
+                      const void* xscale, void* dw, void* dbias, const float* colsum, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/* dx = dy * gelu_tanh'(x) from x, or (x NULL) from the 8-bit blocks that sfm_quantize8 kept of it. */
+int sfm_gelu_bwd(int32_t dtype, int64_t rows, int32_t C, const void* x, int64_t x_stride, const void* data, const void* scale,
+                 const void* dy, int64_t dy_stride, void* dx, int64_t dx_stride, void* stream);
+
+/* sfm_ln_modulate (the same y, bit for bit) that keeps what its backward needs in 8 bits: the normalised rows (x - mean) r as
+ * 8-bit blocks, and r = 1 / sqrt(var + eps), fp32 [rows]. */
+int sfm_ln_keep8(int32_t dtype, int64_t rows, int32_t C, float eps, const void* x, int64_t x_stride, void* y, int64_t y_stride,
+                 const void* scale, const void* shift, int64_t mod_stride, int32_t rows_per_frame, const void* weight, const void* bias,
+                 void* data, void* scale8, float* rstd, void* stream);
+
+/* Backward of sfm_ln_modulate.  Rows in groups of rows_per_group (affine form: all of them; modulated: the rows of a frame); dw, db:
+ * [rows / rows_per_group][C], for the affine form the gradients of weight and bias, for the modulated one of scale and shift.
+ * Exactly one of weight ([C]) and scale (rows mod_stride apart) is given; dx may be NULL.  From x, or (x NULL) from the blocks and
+ * rstd of sfm_ln_keep8.  Statistics and sums in fp32, in a fixed order; one rounding. */
+int sfm_ln_bwd_workspace_bytes(int64_t rows, int32_t C, int64_t rows_per_group, size_t* bytes);
+int sfm_ln_bwd(int32_t dtype, int64_t rows, int32_t C, float eps, const void* x, int64_t x_stride, const void* data, const void* scale8,
+               const float* rstd, const void* dy, int64_t dy_stride, const void* weight, const void* scale, int64_t mod_stride,
+               int64_t rows_per_group, void* dx, int64_t dx_stride, void* dw, void* db, void* workspace, size_t workspace_bytes,
+               void* stream);
+
 typedef struct sfm_conv_desc {
     int32_t dtype;            /* SFM_BF16 | SFM_F16 */
     int32_t T, H, W;          /* output frames, rows, columns */

@@ -8,8 +8,10 @@ reference's module names:
     attention.attention / attention.full_attention_with_kv_cache
     prologue.qk_prologue / prologue.rope_table
     causal_model.CausalWanModel (+ self-attention, block, head), pipeline.CausalInferencePipeline
+    linear8.linear8 / linear8.pack / linear8.quantize (linear layers in 8-bit blocks and their gradients),
+    block_ops.ln_affine / ln_modulate / gelu_tanh (forward and backward, with 8-bit checkpoints)
     vae_decode.WanVAEDecoder (streaming latent -> pixel decode; channels-last HIP convolutions and norms, conv_ops)
 """
-from . import lib, monarch_attn, attention, prologue, causal_model, pipeline, vae_decode, linear, block_ops  # noqa: F401
+from . import lib, monarch_attn, attention, prologue, causal_model, pipeline, vae_decode, linear, block_ops, linear8  # noqa: F401
 
-__all__ = ["lib", "monarch_attn", "attention", "prologue", "causal_model", "pipeline", "vae_decode", "linear"]
+__all__ = ["lib", "monarch_attn", "attention", "prologue", "causal_model", "pipeline", "vae_decode", "linear", "linear8"]

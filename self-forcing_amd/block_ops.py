@@ -1,10 +1,25 @@
 """Fused element-wise operators of the causal Wan block (LayerNorm + adaLN modulation, gated residual,
-RMSNorm); counterparts of the eager chains in wan/modules/causal_model.py:1176-1205 and
+RMSNorm, GELU); counterparts of the eager chains in wan/modules/causal_model.py:1176-1205 and
 wan/modules/model.py:462-478.  [B, L, C] tensors, modulation rows [B, F, 1, C] (one per latent frame)."""
+import ctypes
+
 import torch
 
 from . import lib as _l
 from .monarch_attn import _DT, _stream
+
+_HALF = (torch.float16, torch.bfloat16)
+
+
+def _row_stride(x):
+    """Elements between the rows of a [B, L, C] tensor with contiguous channels; None where they are not evenly strided.  The
+    stride of a dimension of one says nothing."""
+    if x.dim() != 3 or (x.stride(2) != 1 and x.shape[2] > 1):
+        return None
+    B, L, C = x.shape
+    if B == 1 or L == 1:
+        return x.stride(1) if L > 1 else x.stride(0) if B > 1 else C
+    return x.stride(1) if x.stride(0) == L * x.stride(1) else None
 
 
 def _rows(x):
@@ -12,9 +27,10 @@ def _rows(x):
         raise ValueError("the block operators run on the GPU")
     if x.dtype not in _DT:
         raise ValueError(f"unsupported dtype {x.dtype}")
-    if x.dim() != 3 or x.stride(2) != 1 or x.stride(0) != x.shape[1] * x.stride(1):
+    xs = _row_stride(x)
+    if xs is None:
         raise ValueError("expected a [B, L, C] tensor with contiguous channels and evenly strided rows")
-    return x.shape[0] * x.shape[1], x.shape[2], x.stride(1)
+    return x.shape[0] * x.shape[1], x.shape[2], xs
 
 
 def _like(name, t, x):
@@ -35,6 +51,8 @@ def _mod(e, x):
     """[B, F, 1, C] (or [B, F, C]) modulation tensor -> (tensor, frame stride, rows per frame)."""
     B, L, C = x.shape
     _like("modulation", e, x)
+    if e.numel() == 0 or e.numel() % (B * C):
+        raise ValueError("modulation: expected [B, F, 1, C] rows")
     e = e.reshape(B, -1, C)
     if e.stride(2) != 1 or (B > 1 and e.stride(0) != e.shape[1] * e.stride(1)):
         e = e.contiguous()
@@ -43,29 +61,196 @@ def _mod(e, x):
     return e, e.stride(1), L // e.shape[1]
 
 
-def ln_modulate(x, scale, shift, eps=1e-6):
-    """LayerNorm(x) (no affine) * (1 + scale) + shift with per-frame scale/shift."""
-    rows, C, xs = _rows(x)
+def _pairs(scale, shift, x):
+    """The two modulation tensors as (tensor, tensor, frame stride, rows per frame); they share their frames."""
     sc, ms, rpf = _mod(scale, x)
-    sh, ms2, _ = _mod(shift, x)
+    sh, ms2, rpf2 = _mod(shift, x)
+    if rpf2 != rpf:
+        raise ValueError("scale and shift must have the same number of modulation frames")
     if ms2 != ms:
         sc, sh = sc.contiguous(), sh.contiguous()
         ms = sc.stride(1)
-    y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    with torch.cuda.device(x.device):
-        _l.check(_l.load().sfm_ln_modulate(_DT[x.dtype], rows, C, eps, x.data_ptr(), xs, y.data_ptr(), C, sc.data_ptr(),
-                                           sh.data_ptr(), ms, rpf, None, None, _stream(x)))
-    return y
+    return sc, sh, ms, rpf
 
 
-def ln_affine(x, weight, bias, eps=1e-6):
+def _needs_grad(*ts):
+    return torch.is_grad_enabled() and any(t.requires_grad for t in ts)
+
+
+def _written(t):
+    """A tensor written in place through its address: autograd is told, so that a graph that has saved it does not use it."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
+def _even(dy):
+    """Gradients come in any layout (expanded from a sum, transposed): rows of contiguous channels, evenly strided and 16-byte
+    aligned."""
+    s = _row_stride(dy)
+    ok = s is not None and s >= dy.shape[2] and dy.data_ptr() % 16 == 0 and s * dy.element_size() % 16 == 0
+    return dy if ok else dy.clone(memory_format=torch.contiguous_format)
+
+
+def _ln(x, mod, eps):
     rows, C, xs = _rows(x)
-    weight, bias = _vec("weight", weight, x), _vec("bias", bias, x)
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     with torch.cuda.device(x.device):
-        _l.check(_l.load().sfm_ln_modulate(_DT[x.dtype], rows, C, eps, x.data_ptr(), xs, y.data_ptr(), C, None, None, 0, 1,
-                                           weight.data_ptr(), bias.data_ptr(), _stream(x)))
+        _l.check(_l.load().sfm_ln_modulate(_DT[x.dtype], rows, C, eps, x.data_ptr(), xs, y.data_ptr(), C, *mod, _stream(x)))
     return y
+
+
+def _ln_keep8(x, mod, eps):
+    """(y, normalised rows' 8-bit data, their scales, 1 / standard deviation of each row)."""
+    rows, C, xs = _rows(x)
+    kp = -(-C // 128) * 128
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    data = torch.empty((rows, kp), dtype=torch.uint8, device=x.device)
+    scale = torch.empty(-(-rows // 128) * kp, dtype=torch.uint8, device=x.device)
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
+    with torch.cuda.device(x.device):
+        _l.check(_l.load().sfm_ln_keep8(_DT[x.dtype], rows, C, eps, x.data_ptr(), xs, y.data_ptr(), C, *mod, data.data_ptr(),
+                                        scale.data_ptr(), rstd.data_ptr(), _stream(x)))
+    return y, data, scale, rstd
+
+
+def _ln_bwd(dy, x, kept, weight, scale, ms, group, eps, want_dx=True):
+    """(dx, dw, db): dw, db [groups of rows, C].  From x, or from `kept` = (data, scales, 1 / standard deviations)."""
+    dy = _even(dy)
+    B, L, C = dy.shape
+    rows, xs = B * L, 0 if x is None else _rows(x)[2]
+    dx = torch.empty((B, L, C), dtype=dy.dtype, device=dy.device) if want_dx else None
+    dw, db = (torch.empty((rows // group, C), dtype=dy.dtype, device=dy.device) for _ in range(2))
+    n = ctypes.c_size_t(0)
+    _l.check(_l.load().sfm_ln_bwd_workspace_bytes(rows, C, group, ctypes.byref(n)))
+    ws = torch.empty(n.value, dtype=torch.uint8, device=dy.device)
+    data, sc8, rstd = (None, None, None) if kept is None else (t.data_ptr() for t in kept)
+    with torch.cuda.device(dy.device):
+        _l.check(_l.load().sfm_ln_bwd(_DT[dy.dtype], rows, C, eps, None if x is None else x.data_ptr(), xs, data, sc8, rstd, dy.data_ptr(),
+                                      _row_stride(dy), None if weight is None else weight.data_ptr(), None if scale is None else scale.data_ptr(),
+                                      ms, group, None if dx is None else dx.data_ptr(), C, dw.data_ptr(), db.data_ptr(), ws.data_ptr(),
+                                      n.value, _stream(dy)))
+    return dx, dw, db
+
+
+class _LnFn(torch.autograd.Function):
+    """LayerNorm with `a`, `b` = weight, bias ([C]) or scale, shift (per frame).  Keeps x, or with `checkpoint8` the normalised rows
+    in 8 bits and a float per row."""
+
+    @staticmethod
+    def forward(ctx, x, a, b, modulate, eps, checkpoint8):
+        if modulate:
+            sc, sh, ms, rpf = _pairs(a, b, x)
+            mod = (sc.data_ptr(), sh.data_ptr(), ms, rpf, None, None)
+        else:
+            sc, sh, ms, rpf = _vec("weight", a, x), _vec("bias", b, x), 0, x.shape[0] * x.shape[1]
+            mod = (None, None, 0, 1, sc.data_ptr(), sh.data_ptr())
+        ctx.cfg = (modulate, eps, checkpoint8, ms, rpf, a.shape, b.shape)
+        if checkpoint8:
+            y, *kept = _ln_keep8(x, mod, eps)
+            ctx.save_for_backward(sc, *kept)
+        else:
+            y = _ln(x, mod, eps)
+            ctx.save_for_backward(sc, x)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        modulate, eps, checkpoint8, ms, rpf, a_shape, b_shape = ctx.cfg
+        sc, *rest = ctx.saved_tensors
+        x, kept = (None, rest) if checkpoint8 else (rest[0], None)
+        dx, dw, db = _ln_bwd(dy, x, kept, None if modulate else sc, sc if modulate else None, ms, rpf, eps, ctx.needs_input_grad[0])
+        return dx, dw.view(a_shape), db.view(b_shape), None, None, None
+
+
+def ln_modulate(x, scale, shift, eps=1e-6, checkpoint8=False):
+    """LayerNorm(x) (no affine) * (1 + scale) + shift with per-frame scale/shift.  Differentiable in all three; with `checkpoint8`
+    the normalised rows are kept for the backward in 8-bit blocks (see linear8) instead of x."""
+    if _needs_grad(x, scale, shift):
+        return _LnFn.apply(x, scale, shift, True, eps, checkpoint8)
+    sc, sh, ms, rpf = _pairs(scale, shift, x)
+    return _ln(x, (sc.data_ptr(), sh.data_ptr(), ms, rpf, None, None), eps)
+
+
+def ln_affine(x, weight, bias, eps=1e-6, checkpoint8=False):
+    """LayerNorm(x) * weight + bias.  Differentiable in all three; `checkpoint8` as in ln_modulate."""
+    if _needs_grad(x, weight, bias):
+        return _LnFn.apply(x, weight, bias, False, eps, checkpoint8)
+    weight, bias = _vec("weight", weight, x), _vec("bias", bias, x)
+    return _ln(x, (None, None, 0, 1, weight.data_ptr(), bias.data_ptr()), eps)
+
+
+def _check_dy(dy, x):
+    _like("dy", dy, x)
+    if dy.shape != x.shape:
+        raise ValueError("dy and x must have the same shape")
+
+
+def ln_affine_backward(dy, x, weight, eps=1e-6):
+    """(dx, dweight, dbias) of ln_affine from its output's gradient."""
+    _rows(x)
+    _check_dy(dy, x)
+    dx, dw, db = _ln_bwd(dy, x, None, _vec("weight", weight, x), None, 0, x.shape[0] * x.shape[1], eps)
+    return dx, dw[0], db[0]
+
+
+def ln_modulate_backward(dy, x, scale, eps=1e-6):
+    """(dx, dscale, dshift) of ln_modulate from its output's gradient; dscale and dshift in scale's shape."""
+    _rows(x)
+    _check_dy(dy, x)
+    sc, ms, rpf = _mod(scale, x)
+    dx, dw, db = _ln_bwd(dy, x, None, None, sc, ms, rpf, eps)
+    return dx, dw.view(scale.shape), db.view(scale.shape)
+
+
+def _gelu(x, keep8):
+    rows, C, xs = _rows(x)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    data = scale = None
+    if keep8:
+        kp = -(-C // 128) * 128
+        data = torch.empty((rows, kp), dtype=torch.uint8, device=x.device)
+        scale = torch.empty(-(-rows // 128) * kp, dtype=torch.uint8, device=x.device)
+    with torch.cuda.device(x.device):
+        _l.check(_l.load().sfm_quantize8(_DT[x.dtype], rows, C, x.data_ptr(), xs, data.data_ptr() if keep8 else None,
+                                         scale.data_ptr() if keep8 else None, y.data_ptr(), C, None, _stream(x)))
+    return y, data, scale
+
+
+class _GeluFn(torch.autograd.Function):
+    """Keeps x, or with `checkpoint8` x in 8-bit blocks."""
+
+    @staticmethod
+    def forward(ctx, x, checkpoint8):
+        y, data, scale = _gelu(x, checkpoint8)
+        ctx.checkpoint8 = checkpoint8
+        ctx.save_for_backward(*((data, scale) if checkpoint8 else (x,)))
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        dy = _even(dy)
+        B, L, C = dy.shape
+        x, xs, data, scale = None, 0, None, None
+        if ctx.checkpoint8:
+            data, scale = (t.data_ptr() for t in ctx.saved_tensors)
+        else:
+            x, = ctx.saved_tensors
+            xs, x = _row_stride(x), x.data_ptr()
+        dx = torch.empty((B, L, C), dtype=dy.dtype, device=dy.device)
+        with torch.cuda.device(dy.device):
+            _l.check(_l.load().sfm_gelu_bwd(_DT[dy.dtype], B * L, C, x, xs, data, scale, dy.data_ptr(), _row_stride(dy), dx.data_ptr(), C,
+                                            _stream(dy)))
+        return dx, None
+
+
+def gelu_tanh(x, checkpoint8=False):
+    """GELU in its tanh form (wan/modules/model.py:648-650) of [B, L, C] rows.  Differentiable; with `checkpoint8` x is kept for the
+    backward in 8-bit blocks (see linear8)."""
+    if _needs_grad(x):
+        return _GeluFn.apply(x, checkpoint8)
+    return _gelu(x, False)[0]
 
 
 def gate_residual_(x, y, gate=None):
@@ -75,6 +260,7 @@ def gate_residual_(x, y, gate=None):
     if y.shape != x.shape:
         raise ValueError("x and y must have the same shape")
     g, ms, rpf = (None, 0, 1) if gate is None else _mod(gate, x)
+    _written(x)
     with torch.cuda.device(x.device):
         _l.check(_l.load().sfm_gate_residual(_DT[x.dtype], rows, C, x.data_ptr(), xs, y.data_ptr(), ys,
                                              None if g is None else g.data_ptr(), ms, rpf, _stream(x)))
@@ -91,15 +277,12 @@ def gate_residual_ln_(x, y, gate=None, scale=None, shift=None, weight=None, bias
     g, gms, grpf = (None, 0, 1) if gate is None else _mod(gate, x)
     out = torch.empty_like(x, memory_format=torch.contiguous_format)
     if weight is None:
-        sc, ms, rpf = _mod(scale, x)
-        sh, ms2, _ = _mod(shift, x)
-        if ms2 != ms:
-            sc, sh = sc.contiguous(), sh.contiguous()
-            ms = sc.stride(1)
+        sc, sh, ms, rpf = _pairs(scale, shift, x)
         mod = (sc.data_ptr(), sh.data_ptr(), ms, rpf, None, None)
     else:
         weight, bias = _vec("weight", weight, x), _vec("bias", bias, x)
         mod = (None, None, 0, 1, weight.data_ptr(), bias.data_ptr())
+    _written(x)
     with torch.cuda.device(x.device):
         _l.check(_l.load().sfm_gate_residual_ln(_DT[x.dtype], rows, C, eps, x.data_ptr(), xs, y.data_ptr(), ys,
                                                 None if g is None else g.data_ptr(), gms, grpf, out.data_ptr(), C, *mod,

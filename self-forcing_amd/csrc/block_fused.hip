@@ -12,49 +12,9 @@
 // every eager op of the reference rounds to the tensor dtype, so the kernels round after the same steps
 // (LayerNorm output, 1 + scale, the product, the sum; y * gate, x + ...).
 
-#include "sfm_common.hpp"
+#include "rows8.hpp"
 
 namespace sfm {
-
-template <typename T> struct V8;   // 8 consecutive elements <-> 8 floats
-template <> struct V8<float> {
-    static __device__ __forceinline__ void load(const void* p, int64_t e, float* x) {
-        const f32x4* s = (const f32x4*)((const float*)p + e);
-        f32x4 a = s[0], b = s[1];
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    }
-    static __device__ __forceinline__ void store(void* p, int64_t e, const float* x) {
-        f32x4* d = (f32x4*)((float*)p + e);
-        f32x4 a = {x[0], x[1], x[2], x[3]}, b = {x[4], x[5], x[6], x[7]};
-        d[0] = a; d[1] = b;
-    }
-    static __device__ __forceinline__ float rnd(float x) { return x; }
-};
-template <class E> struct V8_16 {
-    static __device__ __forceinline__ void load(const void* p, int64_t e, float* x) {
-        u32x4 w = *(const u32x4*)((const uint16_t*)p + e);
-        uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = E::to_float((uint16_t)(ww[i] & 0xffffu));
-            x[2 * i + 1] = E::to_float((uint16_t)(ww[i] >> 16));
-        }
-    }
-    static __device__ __forceinline__ void store(void* p, int64_t e, const float* x) {
-        u32x4 w;
-        w.x = pack2<E>(x[0], x[1]); w.y = pack2<E>(x[2], x[3]); w.z = pack2<E>(x[4], x[5]); w.w = pack2<E>(x[6], x[7]);
-        *(u32x4*)((uint16_t*)p + e) = w;
-    }
-    static __device__ __forceinline__ float rnd(float x) { return E::to_float(E::from_float(x)); }
-};
-template <> struct V8<BF16> : V8_16<BF16> {};
-template <> struct V8<F16> : V8_16<F16> {};
-
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
 
 // x [rows, C] (row stride xs), scale/shift [B, F, C] addressed through (row -> frame) = row / rows_per_frame,
 // with element strides ms (between frames); weight/bias [C] or nullptr.  NT = 8-element chunks per lane.

@@ -1,0 +1,186 @@
+// Rows of channels in registers: eight elements at a time for the three tensor types, sums over a wave, and the 8-bit
+// blocks that rows and weights are kept in.
+//
+// 8-bit blocks: 128 consecutive values of a row share a power of two 2^s, the smallest with max |v| <= 448 * 2^s over the
+// finite values (s = 0 for a block of zeros, never below -126); a value is kept as e4m3 of v * 2^-s, ties to even, one
+// that is not finite as NaN.  Powers of two cost up to one bit of the e4m3 range against a free scale and nothing of its
+// relative precision (half a step is 2^-4 either way), and the scaled matrix instructions apply them: no product needs a
+// multiplication of its own per block, and the 8-bit value times its scale is exact in bf16.
+//
+// Memory: `data` [rows][round_up(K, 128)] bytes, zeros past K; `scale` bytes s + 127, one word of four for the rows
+// 128 g + m + 32 t (t = byte) of block column kb at word (kb * groups + g) * 32 + m, groups = ceil(rows / 128): a lane of a
+// 32-row matrix instruction finds the scales of its row in four row blocks in one word.
+#pragma once
+
+#include <type_traits>
+
+#include "sfm_common.hpp"
+
+namespace sfm {
+
+template <typename T> struct V8;   // 8 consecutive elements <-> 8 floats
+template <> struct V8<float> {
+    static __device__ __forceinline__ void load(const void* p, int64_t e, float* x) {
+        const f32x4* s = (const f32x4*)((const float*)p + e);
+        f32x4 a = s[0], b = s[1];
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    }
+    static __device__ __forceinline__ void store(void* p, int64_t e, const float* x) {
+        f32x4* d = (f32x4*)((float*)p + e);
+        f32x4 a = {x[0], x[1], x[2], x[3]}, b = {x[4], x[5], x[6], x[7]};
+        d[0] = a; d[1] = b;
+    }
+    static __device__ __forceinline__ float rnd(float x) { return x; }
+};
+template <class E> struct V8_16 {
+    static __device__ __forceinline__ void load(const void* p, int64_t e, float* x) {
+        u32x4 w = *(const u32x4*)((const uint16_t*)p + e);
+        uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = E::to_float((uint16_t)(ww[i] & 0xffffu));
+            x[2 * i + 1] = E::to_float((uint16_t)(ww[i] >> 16));
+        }
+    }
+    static __device__ __forceinline__ void store(void* p, int64_t e, const float* x) {
+        u32x4 w;
+        w.x = pack2<E>(x[0], x[1]); w.y = pack2<E>(x[2], x[3]); w.z = pack2<E>(x[4], x[5]); w.w = pack2<E>(x[6], x[7]);
+        *(u32x4*)((uint16_t*)p + e) = w;
+    }
+    static __device__ __forceinline__ float rnd(float x) { return E::to_float(E::from_float(x)); }
+};
+template <> struct V8<BF16> : V8_16<BF16> {};
+template <> struct V8<F16> : V8_16<F16> {};
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+
+typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
+
+template <typename T> constexpr bool kWide = std::is_same<T, float>::value;      // 4-byte elements
+
+constexpr int kBlock8 = 128;
+
+__host__ __device__ inline int blocks8(int64_t k) { return (int)((k + kBlock8 - 1) / kBlock8); }
+__host__ __device__ inline int64_t pad8(int64_t k) { return (k + kBlock8 - 1) / kBlock8 * kBlock8; }
+__host__ __device__ inline int64_t scale_bytes8(int64_t rows, int64_t k) { return (int64_t)blocks8(k) * blocks8(rows) * kBlock8; }
+// bytes between the scales of two block rows of a weight: whole words, which a wave reads through the scalar cache
+__host__ __device__ inline int pitch8(int64_t k) { return (blocks8(k) + 3) & ~3; }
+// byte of row r in block column kb
+__device__ __forceinline__ int64_t scale_at8(int64_t r, int kb, int64_t groups) {
+    return ((kb * groups + (r >> 7)) << 7) + ((r & 31) << 2) + ((r & 127) >> 5);
+}
+
+// exponent s of a block from the largest finite magnitude
+__device__ __forceinline__ int block_exp8(float amax) {
+    const uint32_t u = __float_as_uint(amax);
+    const int s = (int)(u >> 23) - 135 + ((u & 0x7fffffu) > 0x600000u);      // 448 = 1.75 * 2^8
+    return u == 0 ? 0 : max(s, -126);
+}
+__device__ __forceinline__ float two_to(int s) { return __uint_as_float((uint32_t)(s + 127) << 23); }      // -126 <= s <= 127
+// |v| where it counts for a block's scale
+__device__ __forceinline__ float finite_mag(float v) {
+    const float a = fabsf(v);
+    return a <= 3.402823466e38f ? a : 0.f;
+}
+// four values, already divided by the block's scale, to e4m3
+__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
+    auto fit = [](float v) { return fabsf(v) <= 448.f ? v : __uint_as_float(0x7fc00000u); };
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(fit(a), fit(b), 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(fit(c), fit(d), w, true);
+    return (uint32_t)w;
+}
+__device__ __forceinline__ void unpack_e4m3(uint32_t w, float* v) {
+    auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+    auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    v[0] = lo[0]; v[1] = lo[1]; v[2] = hi[0]; v[3] = hi[1];
+}
+
+// eight elements of a row of n that may end inside them or start off a 16-byte boundary; zeros past the end
+template <typename T> struct Elem {
+    static __device__ __forceinline__ float get(const void* p, int64_t e) { return T::to_float(((const uint16_t*)p)[e]); }
+    static __device__ __forceinline__ void put(void* p, int64_t e, float v) { ((uint16_t*)p)[e] = T::from_float(v); }
+};
+template <> struct Elem<float> {
+    static __device__ __forceinline__ float get(const void* p, int64_t e) { return ((const float*)p)[e]; }
+    static __device__ __forceinline__ void put(void* p, int64_t e, float v) { ((float*)p)[e] = v; }
+};
+template <typename T>
+__device__ __forceinline__ void load_part8(const void* p, int64_t row_off, int c, int n, bool vec, float* v) {
+    if (vec && c + 8 <= n) {
+        V8<T>::load(p, row_off + c, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < n ? Elem<T>::get(p, row_off + c + i) : 0.f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store_part8(void* p, int64_t row_off, int c, int n, bool vec, const float* v) {
+    if (vec && c + 8 <= n) {
+        V8<T>::store(p, row_off + c, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c + i < n) Elem<T>::put(p, row_off + c + i, v[i]);
+    }
+}
+
+// maximum over the 16 lanes that share a block of 128 values (8 a lane)
+__device__ __forceinline__ float max16(float a) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o));
+    return a;
+}
+
+// GELU in its tanh form, 0.5 x (1 + tanh(u)) with u = sqrt(2/pi) (x + 0.044715 x^3), as x p with p = 1 / (1 + exp(-2u)): no
+// cancellation where tanh approaches -1.  FULL: expf instead of the hardware's exponential (fp32 tensors).
+template <bool FULL>
+__device__ __forceinline__ float gelu_gate(float x) {
+    const float u2 = -1.5957691216057308f * (x + 0.044715f * x * x * x);
+    return 1.f / (1.f + (FULL ? expf(u2) : __expf(u2)));
+}
+// d gelu / dx = p + x p (1 - p) 2 u'(x); past |x| = 16 p is 0 or 1 to fp32
+template <bool FULL>
+__device__ __forceinline__ float gelu_slope(float x) {
+    if (fabsf(x) > 16.f) return x > 0.f ? 1.f : 0.f;
+    const float p = gelu_gate<FULL>(x);
+    return p + x * p * (1.f - p) * (1.5957691216057308f + 0.21406445f * x * x);
+}
+
+// the launch that precedes: SFM_OK, or SFM_ERR_HIP with the runtime's message
+inline int launched8(const char* what) {
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess) return SFM_OK;
+    set_error("%s: launch failed: %s", what, hipGetErrorString(e));
+    return SFM_ERR_HIP;
+}
+
+// quant8.hip
+int launch_quantize8(int dtype, int64_t rows, int K, const void* x, int64_t xs, void* data, void* scale, void* y, int64_t ys, float* colsum,
+                     hipStream_t st);
+int launch_dequantize8(int dtype, int64_t rows, int K, const void* data, const void* scale, void* y, int64_t ys, hipStream_t st);
+int launch_gelu_bwd(int dtype, int64_t rows, int K, const void* x, int64_t xs, const void* data, const void* scale, const void* dy,
+                    int64_t dys, void* dx, int64_t dxs, hipStream_t st);
+int launch_pack8(int dtype, int N, int K, const void* w, int64_t ws, void* data, void* scale, void* data_t, void* scale_t, hipStream_t st);
+// linear8.hip
+int launch_linear8(const sfm_linear8_desc& d, const void* x8, const void* xscale, const void* w8, const void* wscale, const void* bias,
+                   const void* res, const void* gate, void* out, hipStream_t stream);
+// linear8_wgrad.hip; `colsum`: column sums of dy by groups of 128 rows where a quantisation has formed them, else null
+size_t wgrad8_workspace_bytes(int64_t M, int N, int K, bool bias);
+int launch_wgrad8(int dtype, int64_t M, int N, int K, const void* dy, int64_t dy_stride, const void* x8, const void* xscale, void* dw,
+                  void* dbias, const float* colsum, void* workspace, hipStream_t st);
+// ln_train.hip; launch_sum_parts: out[g][c] = sum over s of part[g][s][c], two halves of the columns to out1 and out2 if that is given
+int launch_sum_parts(int dtype, int64_t parts, int64_t n, int64_t groups, const float* part, void* out1, void* out2, hipStream_t st);
+size_t ln_bwd_workspace_bytes(int64_t rows, int C, int64_t rows_per_group);
+int launch_ln_bwd(int dtype, int64_t rows, int C, float eps, const void* x, int64_t xs, const void* data, const void* scale8,
+                  const float* rstd, const void* dy, int64_t dys, const void* weight, int64_t ms, int64_t rows_per_group, bool mod, void* dx,
+                  int64_t dxs, void* dw, void* db, void* workspace, hipStream_t st);
+int launch_ln_keep8(int dtype, int64_t rows, int C, float eps, const void* x, int64_t xs, void* y, int64_t ys, const void* scale,
+                    const void* shift, int64_t ms, int rows_per_frame, const void* weight, const void* bias, void* data, void* scale8,
+                    float* rstd, hipStream_t st);
+
+}  // namespace sfm

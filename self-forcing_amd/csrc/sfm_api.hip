@@ -6,7 +6,7 @@
 #include <stdlib.h>
 #include <string.h>
 
-#include "sfm_common.hpp"
+#include "rows8.hpp"
 
 namespace sfm {
 
@@ -1397,6 +1397,242 @@ int sfm_rms_norm(int32_t dtype, int64_t rows, int32_t C, float eps, const void* 
         return SFM_ERR_ALIGN;
     }
     return launch_rms_norm(dtype, rows, C, eps, x, x_stride, y, y_stride, weight, (hipStream_t)stream);
+}
+
+static int check_rows8(int dtype, int64_t rows, int64_t K, bool f32) {
+    if (dtype != SFM_BF16 && dtype != SFM_F16 && !(f32 && dtype == SFM_F32)) {
+        set_error("unsupported dtype %d", dtype);
+        return SFM_ERR_DTYPE;
+    }
+    if (rows < 1 || rows > 0x7fffffff || K < 1 || K > (1 << 22)) {
+        set_error("rows=%lld, K=%lld: need 1 <= rows < 2^31 and 1 <= K <= 4194304", (long long)rows, (long long)K);
+        return SFM_ERR_SHAPE;
+    }
+    return SFM_OK;
+}
+static int check_elem(const char* name, const void* p, int64_t stride, int64_t n, int esz) {
+    if (stride < n) {
+        set_error("%s: rows of %lld elements, %lld apart", name, (long long)n, (long long)stride);
+        return SFM_ERR_STRIDE;
+    }
+    if (((uintptr_t)p) % esz) {
+        set_error("%s is not aligned to its elements", name);
+        return SFM_ERR_ALIGN;
+    }
+    return SFM_OK;
+}
+static int check_blocks(const char* name, const void* data, const void* scale) {
+    if (!data || !scale) {
+        set_error("%s: data and scale must be non-NULL", name);
+        return SFM_ERR_NULL;
+    }
+    if (!aligned16(data) || !aligned16(scale)) {
+        set_error("%s: data and scale must be 16-byte aligned", name);
+        return SFM_ERR_ALIGN;
+    }
+    return SFM_OK;
+}
+static bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+    const char *pa = (const char*)a, *pb = (const char*)b;
+    return pa < pb + nb && pb < pa + na;
+}
+
+int sfm_quantize8(int32_t dtype, int64_t rows, int32_t K, const void* x, int64_t x_stride, void* data, void* scale, void* y,
+                  int64_t y_stride, float* colsum, void* stream) {
+    int rc = check_rows8(dtype, rows, K, true);
+    if (rc) return rc;
+    if (!x || (!data && !colsum && !y)) {
+        set_error("x and one of data, colsum and y must be non-NULL");
+        return SFM_ERR_NULL;
+    }
+    const int esz = elem_size(dtype);
+    if ((rc = check_elem("x", x, x_stride, K, esz))) return rc;
+    if (data && (rc = check_blocks("quantize8", data, scale))) return rc;
+    if (y && (rc = check_elem("y", y, y_stride, K, esz))) return rc;
+    if (((uintptr_t)colsum) & 3) {
+        set_error("colsum is not 4-byte aligned");
+        return SFM_ERR_ALIGN;
+    }
+    return launch_quantize8(dtype, rows, K, x, x_stride, data, scale, y, y_stride, colsum, (hipStream_t)stream);
+}
+
+int sfm_dequantize8(int32_t dtype, int64_t rows, int32_t K, const void* data, const void* scale, void* y, int64_t y_stride, void* stream) {
+    int rc = check_rows8(dtype, rows, K, true);
+    if (rc) return rc;
+    if ((rc = check_blocks("dequantize8", data, scale))) return rc;
+    if (!y) {
+        set_error("y must be non-NULL");
+        return SFM_ERR_NULL;
+    }
+    if ((rc = check_elem("y", y, y_stride, K, elem_size(dtype)))) return rc;
+    return launch_dequantize8(dtype, rows, K, data, scale, y, y_stride, (hipStream_t)stream);
+}
+
+int sfm_pack8(int32_t dtype, int32_t N, int32_t K, const void* w, int64_t w_stride, void* data, void* scale, void* data_t,
+              void* scale_t, void* stream) {
+    int rc = check_rows8(dtype, N, K, true);
+    if (!rc) rc = check_rows8(dtype, K, N, true);
+    if (rc) return rc;
+    if (!w) {
+        set_error("w must be non-NULL");
+        return SFM_ERR_NULL;
+    }
+    if ((rc = check_elem("w", w, w_stride, K, elem_size(dtype)))) return rc;
+    if ((rc = check_blocks("pack8", data, scale))) return rc;
+    if ((data_t || scale_t) && (rc = check_blocks("pack8 (transposed)", data_t, scale_t))) return rc;
+    return launch_pack8(dtype, N, K, w, w_stride, data, scale, data_t, scale_t, (hipStream_t)stream);
+}
+
+int sfm_linear8(const sfm_linear8_desc* d, const void* x8, const void* xscale, const void* w8, const void* wscale, const void* bias,
+                const void* res, const void* gate, void* out, void* stream) {
+    if (!d || !out) {
+        set_error("desc and out must be non-NULL");
+        return SFM_ERR_NULL;
+    }
+    int rc = check_rows8(d->dtype, d->M, d->K, false);
+    if (!rc) rc = check_rows8(d->dtype, d->M, d->N, false);
+    if (rc) return rc;
+    if (d->epilogue < SFM_EPI_NONE || d->epilogue > SFM_EPI_GATE_RESIDUAL) {
+        set_error("unknown epilogue %d", d->epilogue);
+        return SFM_ERR_SHAPE;
+    }
+    if ((rc = check_blocks("x8", x8, xscale)) || (rc = check_blocks("w8", w8, wscale))) return rc;
+    const bool gr = d->epilogue == SFM_EPI_GATE_RESIDUAL;
+    if (gr && !res) {
+        set_error("the gated-residual epilogue needs res");
+        return SFM_ERR_NULL;
+    }
+    if ((rc = check_elem("out", out, d->out_stride, d->N, 2)) || (bias && (rc = check_elem("bias", bias, d->N, d->N, 2)))) return rc;
+    if (gr && ((rc = check_elem("res", res, d->res_stride, d->N, 2)) || (gate && (rc = check_elem("gate", gate, d->N, d->N, 2))))) return rc;
+    if (gr && gate && (d->rows_per_frame < 1 || d->gate_stride < 0)) {
+        set_error("rows_per_frame >= 1 and gate_stride >= 0 are needed");
+        return SFM_ERR_STRIDE;
+    }
+    const size_t ob = ((size_t)(d->M - 1) * d->out_stride + d->N) * 2;
+    if (overlap(out, ob, x8, (size_t)d->M * SFM_PAD8(d->K)) || overlap(out, ob, w8, (size_t)d->N * SFM_PAD8(d->K))) {
+        set_error("out overlaps x8 or w8");
+        return SFM_ERR_RANGE;
+    }
+    return launch_linear8(*d, x8, xscale, w8, wscale, bias, gr ? res : nullptr, gr ? gate : nullptr, out, (hipStream_t)stream);
+}
+
+int sfm_linear8_wgrad_workspace_bytes(int64_t M, int32_t N, int32_t K, size_t* bytes) {
+    if (!bytes) {
+        set_error("bytes must be non-NULL");
+        return SFM_ERR_NULL;
+    }
+    int rc = check_rows8(SFM_BF16, M, K, false);
+    if (!rc) rc = check_rows8(SFM_BF16, M, N, false);
+    if (rc) return rc;
+    *bytes = wgrad8_workspace_bytes(M, N, K, true);
+    return SFM_OK;
+}
+
+int sfm_linear8_wgrad(int32_t dtype, int64_t M, int32_t N, int32_t K, const void* dy, int64_t dy_stride, const void* x8,
+                      const void* xscale, void* dw, void* dbias, const float* colsum, void* workspace, size_t workspace_bytes,
+                      void* stream) {
+    int rc = check_rows8(dtype, M, K, false);
+    if (!rc) rc = check_rows8(dtype, M, N, false);
+    if (rc) return rc;
+    if (!dy || (!dw && !dbias)) {
+        set_error("dy and dw or dbias must be non-NULL");
+        return SFM_ERR_NULL;
+    }
+    if ((rc = check_elem("dy", dy, dy_stride, N, 2)) || (dw && (rc = check_blocks("x8", x8, xscale)))) return rc;
+    if ((dw && (rc = check_elem("dw", dw, K, K, 2))) || (dbias && (rc = check_elem("dbias", dbias, N, N, 2)))) return rc;
+    const size_t need = wgrad8_workspace_bytes(M, N, K, dbias != nullptr && colsum == nullptr);
+    if (need && (!workspace || (((uintptr_t)workspace) & 255) || workspace_bytes < need)) {
+        set_error("workspace must be non-NULL, 256-byte aligned and hold %zu bytes", need);
+        return SFM_ERR_WORKSPACE;
+    }
+    return launch_wgrad8(dtype, M, N, K, dy, dy_stride, x8, xscale, dw, dbias, colsum, workspace, (hipStream_t)stream);
+}
+
+int sfm_gelu_bwd(int32_t dtype, int64_t rows, int32_t C, const void* x, int64_t x_stride, const void* data, const void* scale,
+                 const void* dy, int64_t dy_stride, void* dx, int64_t dx_stride, void* stream) {
+    int rc = check_rows8(dtype, rows, C, true);
+    if (rc) return rc;
+    if (!dy || !dx) {
+        set_error("dy and dx must be non-NULL");
+        return SFM_ERR_NULL;
+    }
+    const int esz = elem_size(dtype);
+    rc = x ? check_elem("x", x, x_stride, C, esz) : check_blocks("gelu_bwd", data, scale);
+    if (rc || (rc = check_elem("dy", dy, dy_stride, C, esz)) || (rc = check_elem("dx", dx, dx_stride, C, esz))) return rc;
+    return launch_gelu_bwd(dtype, rows, C, x, x_stride, x ? nullptr : data, scale, dy, dy_stride, dx, dx_stride, (hipStream_t)stream);
+}
+
+int sfm_ln_keep8(int32_t dtype, int64_t rows, int32_t C, float eps, const void* x, int64_t x_stride, void* y, int64_t y_stride,
+                 const void* scale, const void* shift, int64_t mod_stride, int32_t rows_per_frame, const void* weight, const void* bias,
+                 void* data, void* scale8, float* rstd, void* stream) {
+    int rc = check_rows(dtype, rows, C, x_stride, y_stride);
+    if (rc) return rc;
+    const bool affine = weight != nullptr || bias != nullptr;
+    if (!x || !y || !rstd || (affine && (!weight || !bias)) || (!affine && (!scale || !shift))) {
+        set_error("x, y, rstd and either (scale, shift) or (weight, bias) must be non-NULL");
+        return SFM_ERR_NULL;
+    }
+    if (!affine && (rows_per_frame < 1 || mod_stride < 0 || (mod_stride * elem_size(dtype)) % 16)) {
+        set_error("rows_per_frame must be >= 1 and mod_stride a multiple of 16 bytes");
+        return SFM_ERR_STRIDE;
+    }
+    if (!aligned16(x) || !aligned16(y) || !aligned16(scale) || !aligned16(shift) || !aligned16(weight) || !aligned16(bias) ||
+        (((uintptr_t)rstd) & 3)) {
+        set_error("tensors must be 16-byte aligned (rstd: 4-byte)");
+        return SFM_ERR_ALIGN;
+    }
+    if ((rc = check_blocks("ln_keep8", data, scale8))) return rc;
+    return launch_ln_keep8(dtype, rows, C, eps, x, x_stride, y, y_stride, scale, shift, mod_stride, affine ? 1 : rows_per_frame, weight,
+                           bias, data, scale8, rstd, (hipStream_t)stream);
+}
+
+static int check_groups(int64_t rows, int64_t rows_per_group) {
+    if (rows_per_group < 1 || rows % rows_per_group) {
+        set_error("%lld rows are not groups of %lld", (long long)rows, (long long)rows_per_group);
+        return SFM_ERR_SHAPE;
+    }
+    return SFM_OK;
+}
+
+int sfm_ln_bwd_workspace_bytes(int64_t rows, int32_t C, int64_t rows_per_group, size_t* bytes) {
+    if (!bytes) {
+        set_error("bytes must be non-NULL");
+        return SFM_ERR_NULL;
+    }
+    int rc = check_rows(SFM_F32, rows, C, C, C);
+    if (rc || (rc = check_groups(rows, rows_per_group))) return rc;
+    *bytes = ln_bwd_workspace_bytes(rows, C, rows_per_group);
+    return SFM_OK;
+}
+
+int sfm_ln_bwd(int32_t dtype, int64_t rows, int32_t C, float eps, const void* x, int64_t x_stride, const void* data, const void* scale8,
+               const float* rstd, const void* dy, int64_t dy_stride, const void* weight, const void* scale, int64_t mod_stride,
+               int64_t rows_per_group, void* dx, int64_t dx_stride, void* dw, void* db, void* workspace, size_t workspace_bytes,
+               void* stream) {
+    int rc = check_rows(dtype, rows, C, x ? x_stride : dy_stride, dy_stride);
+    if (!rc && dx) rc = check_rows(dtype, rows, C, dx_stride, dy_stride);
+    if (rc || (rc = check_groups(rows, rows_per_group))) return rc;
+    if (!dy || !dw || !db || (!weight) == (!scale) || (!x && !rstd)) {
+        set_error("dy, dw, db, one of weight and scale, and x or rstd must be non-NULL");
+        return SFM_ERR_NULL;
+    }
+    if (!x && (rc = check_blocks("ln_bwd", data, scale8))) return rc;
+    if (scale && (mod_stride < 0 || (mod_stride * elem_size(dtype)) % 16)) {
+        set_error("mod_stride must be a multiple of 16 bytes");
+        return SFM_ERR_STRIDE;
+    }
+    if (!aligned16(x) || !aligned16(dy) || !aligned16(dx) || !aligned16(weight) || !aligned16(scale) || !aligned16(dw) || !aligned16(db) ||
+        (((uintptr_t)rstd) & 3)) {
+        set_error("tensors must be 16-byte aligned (rstd: 4-byte)");
+        return SFM_ERR_ALIGN;
+    }
+    const size_t need = ln_bwd_workspace_bytes(rows, C, rows_per_group);
+    if (!workspace || (((uintptr_t)workspace) & 255) || workspace_bytes < need) {
+        set_error("workspace must be non-NULL, 256-byte aligned and hold %zu bytes", need);
+        return SFM_ERR_WORKSPACE;
+    }
+    return launch_ln_bwd(dtype, rows, C, eps, x, x_stride, x ? nullptr : data, scale8, rstd, dy, dy_stride, weight ? weight : scale, mod_stride,
+                         rows_per_group, scale != nullptr, dx, dx_stride, dw, db, workspace, (hipStream_t)stream);
 }
 
 }  // extern "C"

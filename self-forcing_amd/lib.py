@@ -30,7 +30,9 @@ SYMBOLS = [
     "sfm_rms_norm", "sfm_gate_residual_ln", "sfm_linear", "sfm_monarch_bwd_workspace_bytes", "sfm_monarch_bwd", "sfm_monarch_bwd_uses_gemm",
     "sfm_monarch_stats_bytes", "sfm_monarch_fwd_stats", "sfm_monarch_bwd_saved",
     "sfm_monarch_kept_bytes", "sfm_monarch_fwd_kept", "sfm_monarch_bwd_kept_workspace_bytes", "sfm_monarch_bwd_kept",
-    "sfm_monarch_attn_with_kv_cache_kept", "sfm_dense_bwd_workspace_bytes", "sfm_dense_bwd", "sfm_probe_mfma_bf16", "sfm_probe_tile_traffic", "sfm_probe_row_stream", "sfm_probe_l2_read", "sfm_conv3d_cl", "sfm_vae_norm_act", "sfm_set_switches", "sfm_get_switches", "sfm_last_error", "sfm_version",
+    "sfm_monarch_attn_with_kv_cache_kept", "sfm_dense_bwd_workspace_bytes", "sfm_dense_bwd", "sfm_probe_mfma_bf16", "sfm_probe_tile_traffic", "sfm_probe_row_stream", "sfm_probe_l2_read", "sfm_conv3d_cl", "sfm_vae_norm_act",
+    "sfm_quantize8", "sfm_dequantize8", "sfm_pack8", "sfm_linear8", "sfm_linear8_wgrad_workspace_bytes", "sfm_linear8_wgrad",
+    "sfm_gelu_bwd", "sfm_ln_keep8", "sfm_ln_bwd_workspace_bytes", "sfm_ln_bwd", "sfm_set_switches", "sfm_get_switches", "sfm_last_error", "sfm_version",
 ]
 
 
@@ -44,6 +46,12 @@ class LinearDesc(C.Structure):
     _fields_ = [("dtype", C.c_int32), ("epilogue", C.c_int32), ("M", C.c_int64), ("N", C.c_int32), ("K", C.c_int32),
                 ("x_stride", C.c_int64), ("out_stride", C.c_int64), ("res_stride", C.c_int64), ("gate_stride", C.c_int64),
                 ("rows_per_frame", C.c_int32), ("tile_rows", C.c_int32)]
+
+
+class Linear8Desc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("epilogue", C.c_int32), ("M", C.c_int64), ("N", C.c_int32), ("K", C.c_int32),
+                ("out_stride", C.c_int64), ("res_stride", C.c_int64), ("gate_stride", C.c_int64), ("rows_per_frame", C.c_int32),
+                ("reserved", C.c_int32)]
 
 
 EPI_NONE, EPI_GELU_TANH, EPI_GATE_RESIDUAL = 0, 1, 2
@@ -143,6 +151,17 @@ def load():
     lib.sfm_linear.argtypes = [C.POINTER(LinearDesc), P, P, P, P, P, P, P]
     lib.sfm_rms_norm.argtypes = [C.c_int32, I64, C.c_int32, C.c_float, P, I64, P, I64, P, P]
     lib.sfm_conv3d_cl.argtypes = [C.POINTER(ConvDesc), P, P, P, P, P, P]
+    I32 = C.c_int32
+    lib.sfm_quantize8.argtypes = [I32, I64, I32, P, I64, P, P, P, I64, P, P]
+    lib.sfm_dequantize8.argtypes = [I32, I64, I32, P, P, P, I64, P]
+    lib.sfm_pack8.argtypes = [I32, I32, I32, P, I64, P, P, P, P, P]
+    lib.sfm_linear8.argtypes = [C.POINTER(Linear8Desc), P, P, P, P, P, P, P, P, P]
+    lib.sfm_linear8_wgrad_workspace_bytes.argtypes = [I64, I32, I32, C.POINTER(C.c_size_t)]
+    lib.sfm_linear8_wgrad.argtypes = [I32, I64, I32, I32, P, I64, P, P, P, P, P, P, C.c_size_t, P]
+    lib.sfm_gelu_bwd.argtypes = [I32, I64, I32, P, I64, P, P, P, I64, P, I64, P]
+    lib.sfm_ln_keep8.argtypes = [I32, I64, I32, C.c_float, P, I64, P, I64, P, P, I64, I32, P, P, P, P, P, P]
+    lib.sfm_ln_bwd_workspace_bytes.argtypes = [I64, I32, I64, C.POINTER(C.c_size_t)]
+    lib.sfm_ln_bwd.argtypes = [I32, I64, I32, C.c_float, P, I64, P, P, P, P, I64, P, P, I64, I64, P, I64, P, P, P, C.c_size_t, P]
     lib.sfm_vae_norm_act.argtypes = [C.c_int32] * 6 + [P, S3, P, P, S3, P]
     lib.sfm_probe_mfma_bf16.argtypes = [C.c_int32, P, C.POINTER(C.c_float)]
     lib.sfm_probe_tile_traffic.argtypes = [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, P, C.c_size_t, P, C.POINTER(C.c_float)]

@@ -4,7 +4,7 @@ of nn.Linear + nn.GELU(approximate='tanh') (wan/modules/model.py:648-650) and of
 import torch
 
 from . import lib as _l
-from .block_ops import _like, _mod, _rows
+from .block_ops import _like, _mod, _rows, _written
 from .monarch_attn import _DT, _stream
 
 _EPI = {"none": _l.EPI_NONE, "gelu_tanh": _l.EPI_GELU_TANH, "gate_residual": _l.EPI_GATE_RESIDUAL}
@@ -56,12 +56,15 @@ def linear(x, weight, bias=None, epilogue="none", res=None, gate=None, out=None,
             g, d.gate_stride, d.rows_per_frame = _mod(gate, res)
     elif res is not None or gate is not None:
         raise ValueError("res / gate belong to the gate_residual epilogue")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty((B, L, N), dtype=x.dtype, device=x.device)
     _like("out", out, x)
     if out.shape != (B, L, N):
         raise ValueError("out must be [B, L, N]")
     _, _, d.out_stride = _rows(out)
+    if given:
+        _written(out)
     with torch.cuda.device(x.device):
         _l.check(_l.load().sfm_linear(d, x.data_ptr(), weight.data_ptr(), None if bias is None else bias.data_ptr(),
                                       None if res is None else res.data_ptr(), None if g is None else g.data_ptr(),

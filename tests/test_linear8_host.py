@@ -1,0 +1,144 @@
+"""Refusals of the 8-bit block operators at the C boundary and in Python: nothing touches a device."""
+import ctypes as C
+import os
+import re
+
+import pytest
+import torch
+
+import self_forcing_amd as sfa
+from self_forcing_amd import lib as L
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+P = 1 << 20          # a 16-byte aligned address that no refused call reads
+
+
+def _rc(rc, code, text):
+    assert rc == code and text in L.load().sfm_last_error().decode()
+
+
+def test_struct_size_matches_the_header():
+    assert C.sizeof(L.Linear8Desc) == 2 * 4 + 8 + 2 * 4 + 3 * 8 + 2 * 4
+
+
+def test_header_macros_are_what_the_host_allocates():
+    text = open(os.path.join(ROOT, "include", "sfm_attn.h")).read()
+    assert re.search(r"SFM_PAD8\(n\) \(\(\(int64_t\)\(n\) \+ 127\) / 128 \* 128\)", text)
+    assert re.search(r"SFM_PITCH8\(n\) \(\(\(int64_t\)\(n\) \+ 511\) / 512 \* 4\)", text)
+
+
+def test_quantize_dequantize_pack_refusals():
+    lib = L.load()
+    q = lambda dt=0, r=4, K=128, x=P, xs=128, d=2 * P, s=3 * P, y=None, ys=0, cs=None: lib.sfm_quantize8(dt, r, K, x, xs, d, s, y, ys, cs, None)
+    _rc(q(dt=7), -2, "dtype")
+    for r, K in ((0, 128), (4, 0), (1 << 31, 128), (4, 1 << 23)):
+        _rc(q(r=r, K=K, xs=1 << 24), -3, "rows=")
+    _rc(q(x=None), -1, "non-NULL")
+    _rc(q(d=None, s=None), -1, "non-NULL")
+    _rc(q(s=None), -1, "scale")
+    _rc(q(xs=127), -5, "x: rows")
+    _rc(q(x=P + 1), -7, "x is not aligned")
+    _rc(q(d=2 * P + 8), -7, "16-byte")
+    _rc(q(y=P, ys=100), -5, "y: rows")
+    _rc(q(cs=P + 2), -7, "colsum")
+    _rc(lib.sfm_dequantize8(0, 4, 128, P, 2 * P, None, 128, None), -1, "y must")
+    _rc(lib.sfm_dequantize8(0, 4, 128, P, None, 3 * P, 128, None), -1, "scale")
+    _rc(lib.sfm_dequantize8(2, 4, 128, P, 2 * P, 3 * P, 127, None), -5, "y: rows")
+    _rc(lib.sfm_pack8(0, 4, 128, None, 128, P, P, None, None, None), -1, "w must")
+    _rc(lib.sfm_pack8(0, 4, 128, P, 100, P, P, None, None, None), -5, "w: rows")
+    _rc(lib.sfm_pack8(0, 4, 128, P, 128, P, P, P, None, None), -1, "transposed")
+
+
+def _desc(**kw):
+    d = L.Linear8Desc(0, L.EPI_NONE, 16, 64, 128, 64, 64, 64, 1, 0)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def test_product_refusals():
+    lib = L.load()
+
+    def f(d=None, x=P, xs=2 * P, w=3 * P, ws=4 * P, b=None, res=None, gate=None, out=5 * P):
+        return lib.sfm_linear8(C.byref(_desc() if d is None else d), x, xs, w, ws, b, res, gate, out, None)
+    _rc(f(_desc(dtype=2)), -2, "dtype")
+    for kw in (dict(M=0), dict(N=0), dict(K=0), dict(M=1 << 31)):
+        _rc(f(_desc(**kw)), -3, "rows=")
+    _rc(f(_desc(epilogue=9)), -3, "epilogue")
+    _rc(f(out=None), -1, "out")
+    _rc(f(xs=None), -1, "x8")
+    _rc(f(ws=None), -1, "w8")
+    _rc(f(w=3 * P + 4), -7, "w8")
+    _rc(f(_desc(out_stride=63)), -5, "out")
+    _rc(f(out=5 * P + 1), -7, "out")
+    _rc(f(b=P + 1), -7, "bias")
+    _rc(f(_desc(epilogue=L.EPI_GATE_RESIDUAL)), -1, "res")
+    _rc(f(_desc(epilogue=L.EPI_GATE_RESIDUAL, res_stride=1), res=6 * P), -5, "res")
+    _rc(f(_desc(epilogue=L.EPI_GATE_RESIDUAL, rows_per_frame=0), res=6 * P, gate=7 * P), -5, "rows_per_frame")
+    _rc(f(out=P + 2), -6 + 2, "overlaps")
+    _rc(f(out=3 * P + 64 * 128 - 2), -4, "overlaps")
+
+
+def test_gradient_refusals():
+    lib = L.load()
+    n = C.c_size_t(0)
+    assert lib.sfm_linear8_wgrad_workspace_bytes(300, 64, 128, C.byref(n)) == 0 and n.value >= 3 * 64 * 4
+    need = n.value
+    _rc(lib.sfm_linear8_wgrad_workspace_bytes(300, 64, 128, None), -1, "bytes")
+    _rc(lib.sfm_linear8_wgrad_workspace_bytes(0, 64, 128, C.byref(n)), -3, "rows=")
+
+    def f(dt=0, M=300, dy=P, dys=64, x=2 * P, xs=3 * P, dw=4 * P, db=5 * P, cs=None, ws=6 * P, wb=need):
+        return lib.sfm_linear8_wgrad(dt, M, 64, 128, dy, dys, x, xs, dw, db, cs, ws, wb, None)
+    _rc(f(dt=2), -2, "dtype")
+    _rc(f(M=0), -3, "rows=")
+    _rc(f(dy=None), -1, "dy")
+    _rc(f(dw=None, db=None), -1, "dy")
+    _rc(f(dys=63), -5, "dy")
+    _rc(f(x=None), -1, "x8")
+    _rc(f(dw=4 * P + 1), -7, "dw")
+    _rc(f(ws=None), -6, "workspace")
+    _rc(f(ws=6 * P + 16), -6, "workspace")
+    _rc(f(wb=need - 1), -6, "workspace")
+    _rc(lib.sfm_gelu_bwd(0, 4, 128, None, 0, None, P, P, 128, P, 128, None), -1, "gelu_bwd")
+    _rc(lib.sfm_gelu_bwd(0, 4, 128, P, 128, None, None, None, 128, P, 128, None), -1, "dy")
+    _rc(lib.sfm_gelu_bwd(0, 4, 128, P, 127, None, None, P, 128, P, 128, None), -5, "x: rows")
+
+
+def test_layer_norm_refusals():
+    lib = L.load()
+    n = C.c_size_t(0)
+    assert lib.sfm_ln_bwd_workspace_bytes(60, 64, 20, C.byref(n)) == 0 and n.value >= 3 * 2 * 64 * 4
+    need = n.value
+    for rows, Cc, g in ((60, 12, 20), (60, 8200, 20), (0, 64, 1), (60, 64, 7), (60, 64, 0)):
+        assert lib.sfm_ln_bwd_workspace_bytes(rows, Cc, g, C.byref(n)) == -3
+
+    def f(dt=0, x=P, xs=64, data=None, sc8=None, rstd=None, dy=P, dys=64, w=None, sc=2 * P, ms=64, g=20, dx=3 * P, dxs=64, dw=4 * P, db=5 * P,
+          ws=6 * P, wb=need):
+        return lib.sfm_ln_bwd(dt, 60, 64, 1e-6, x, xs, data, sc8, rstd, dy, dys, w, sc, ms, g, dx, dxs, dw, db, ws, wb, None)
+    _rc(f(dt=5), -2, "dtype")
+    _rc(f(g=7), -3, "groups")
+    _rc(f(sc=None), -1, "one of weight and scale")
+    _rc(f(w=P), -1, "one of weight and scale")
+    _rc(f(x=None), -1, "rstd")
+    _rc(f(x=None, rstd=P), -1, "ln_bwd")
+    _rc(f(ms=4), -5, "mod_stride")
+    _rc(f(dys=63), -5, "strides")
+    _rc(f(dx=3 * P + 2), -7, "16-byte")
+    _rc(f(ws=None), -6, "workspace")
+    _rc(f(wb=need - 1), -6, "workspace")
+    k = lambda data=P, rstd=P, y=P, sc=P: lib.sfm_ln_keep8(0, 60, 64, 1e-6, P, 64, y, 64, sc, P, 64, 20, None, None, data, P, rstd, None)
+    _rc(k(rstd=None), -1, "rstd")
+    _rc(k(sc=None), -1, "scale")
+    _rc(k(data=None), -1, "ln_keep8")
+    _rc(k(data=P + 4), -7, "ln_keep8")
+
+
+def test_python_entry_points_refuse_before_any_call():
+    x, w = torch.zeros((1, 4, 128), dtype=torch.bfloat16), torch.zeros((64, 128), dtype=torch.bfloat16)
+    l8, blk = sfa.linear8, sfa.block_ops
+    for call in (lambda: l8.quantize(x), lambda: l8.pack(w), lambda: l8.linear8(x, w), lambda: blk.gelu_tanh(x),
+                 lambda: blk.ln_affine(x, w[0], w[0], checkpoint8=True), lambda: blk.ln_affine_backward(x, x, w[0]),
+                 lambda: l8.linear8(x, w, epilogue="relu"), lambda: l8.linear8(x.float(), w.float()), lambda: l8.linear8(x, w.half()),
+                 lambda: l8.linear8(x, w[0])):
+        with pytest.raises(ValueError):
+            call()
