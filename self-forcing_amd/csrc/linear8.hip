@@ -32,11 +32,22 @@ struct L8Args {
     int N, nkb, pitch;
     int64_t out_stride, res_stride, gate_stride;
     int rows_per_frame;
-    int tn;                  // tiles along N
+    int tm, tn;              // tiles along M and N
     bool vec;                // rows of out, res, gate and bias allow 8-byte accesses
 };
 
-// the tail of four neighbouring channels c.. of a row: bias, epilogue, one rounding, store
+template <class E>
+__device__ __forceinline__ void l8_unpack4(u32x2 w, float* d) {
+    d[0] = E::to_float((uint16_t)(w.x & 0xffffu)); d[1] = E::to_float((uint16_t)(w.x >> 16));
+    d[2] = E::to_float((uint16_t)(w.y & 0xffffu)); d[3] = E::to_float((uint16_t)(w.y >> 16));
+}
+template <class E, int EPI>
+__device__ __forceinline__ float l8_tail(float sum, float bias, float res, float gate) {
+    const float v = sum + bias;
+    return EPI == SFM_EPI_GELU_TANH ? v * gelu_gate<false>(v) : EPI == SFM_EPI_GATE_RESIDUAL ? res + v * gate : v;
+}
+
+// four neighbouring channels c.. of a row: bias and epilogue on the fp32 sums, rounded once and stored
 template <class E, int EPI>
 __device__ __forceinline__ void l8_finish4(const L8Args& p, int64_t row, int c, const float* acc) {
     if (row >= p.M || c >= p.N) return;
@@ -44,9 +55,7 @@ __device__ __forceinline__ void l8_finish4(const L8Args& p, int64_t row, int c, 
     float v[4], r[4] = {0.f, 0.f, 0.f, 0.f}, g[4] = {1.f, 1.f, 1.f, 1.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
     auto get4 = [&](const uint16_t* s, float* d) {
         if (full) {
-            const u32x2 w = *(const u32x2*)s;
-            d[0] = E::to_float((uint16_t)(w.x & 0xffffu)); d[1] = E::to_float((uint16_t)(w.x >> 16));
-            d[2] = E::to_float((uint16_t)(w.y & 0xffffu)); d[3] = E::to_float((uint16_t)(w.y >> 16));
+            l8_unpack4<E>(*(const u32x2*)s, d);
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -59,11 +68,7 @@ __device__ __forceinline__ void l8_finish4(const L8Args& p, int64_t row, int c, 
         if (p.gate != nullptr) get4(p.gate + (row / p.rows_per_frame) * p.gate_stride + c, g);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[i] = acc[i] + b[i];
-        if (EPI == SFM_EPI_GELU_TANH) v[i] *= gelu_gate<false>(v[i]);
-        if (EPI == SFM_EPI_GATE_RESIDUAL) v[i] = r[i] + v[i] * g[i];
-    }
+    for (int i = 0; i < 4; ++i) v[i] = l8_tail<E, EPI>(acc[i], b[i], r[i], g[i]);
     uint16_t* o = p.out + row * p.out_stride + c;
     if (full) {
         u32x2 w = {pack2<E>(v[0], v[1]), pack2<E>(v[2], v[3])};
@@ -153,9 +158,336 @@ int launch_direct(const L8Args& a0, hipStream_t st) {
     return launched8("sfm_linear8");
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// Many rows.  A workgroup of four waves owns 256 weight rows x 64 TB activation rows (TB = 4 or 2), a wave 128 x 32 TB of it: 4 x TB
+// matrix instructions 32x32x64 a k step, 64 TB accumulator registers, one wave per SIMD.  A stage is 128 bytes of every row, one
+// block and one cache line; both operands go from memory straight into LDS through a ring of nine 16 KB slots of 128 rows: the
+// weight rows of a stage are two slots, its activation rows two (TB = 4) or one, so that more than a stage is in flight while one is
+// multiplied.  Rows sit two to a 256-byte LDS line with their 16-byte pieces XOR-ed by the line index: the 16 lanes of an
+// operand read hit 64 different banks.  A lane's 32 bytes of a step are pieces 4 s + hf and 4 s + 2 + hf of its row for both operands.
+//
+// Scales: the 64 words of a stage's 256 rows follow the rows into LDS, a lane's word holds those of its row in the four row blocks
+// (rows8.hpp), and the matrix instruction picks the byte; the weight's is one for the wave, through the scalar cache.
+constexpr int kTileN = 256, kSlot = 128 * kBlock8, kRing = 9;
+constexpr int kScaleAt = kRing * kSlot, kScaleSlot = 256, kLdsBytes = kScaleAt + 4 * kScaleSlot;
+constexpr int kGroupM = 8;                   // row tiles per patch of the tile order
+
+template <int BYTES>
+__device__ __forceinline__ void l8_load_lds(const void* base, uint32_t off, uint32_t lds_addr) {
+    static_assert(BYTES == 16 || BYTES == 4, "");
+    if constexpr (BYTES == 16)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_addr), "v"(off), "s"(base) : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_addr), "v"(off), "s"(base) : "memory", "m0");
+}
+// waits until at most N of this wave's loads are outstanding (they complete in order), then the barrier
+template <int N>
+__device__ __forceinline__ void l8_wait_stage() { asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory"); }
+template <int OFF>
+__device__ __forceinline__ u32x4 l8_lds_read16(uint32_t addr) {
+    u32x4 r;
+    asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(r) : "v"(addr), "n"(OFF));
+    return r;
+}
+__device__ __forceinline__ uint32_t l8_lds_read4(uint32_t addr) {
+    uint32_t r;
+    asm volatile("ds_read_b32 %0, %1" : "=v"(r) : "v"(addr));
+    return r;
+}
+template <int NF>
+__device__ __forceinline__ void l8_wait_frags(u32x4 (&f)[NF], uint32_t& xe) {
+    static_assert(NF == 16 || NF == 12, "two pieces of 4 weight blocks + 4 or 2 activation blocks");
+    asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(f[0]), "+v"(f[1]), "+v"(f[2]), "+v"(f[3]), "+v"(f[4]), "+v"(f[5]), "+v"(f[6]), "+v"(f[7]),
+                 "+v"(f[8]), "+v"(f[9]), "+v"(f[10]), "+v"(f[11]), "+v"(xe));
+    if constexpr (NF == 16) asm volatile("" : "+v"(f[12]), "+v"(f[13]), "+v"(f[14]), "+v"(f[15]));
+}
+__device__ __forceinline__ i32x8 l8_join(u32x4 a, u32x4 b) {
+    return __builtin_shufflevector(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// where a wave's loads go: request j of a list of quarter stages (4 requests each), then the scales
+template <int TB>
+struct L8Src {
+    const uint8_t *w, *x, *s;                // stage of the next request
+    uint32_t w_off[8], x_off[2 * TB], s_off;
+    uint32_t lds;                            // LDS address of this wave's first 1 KB in slot 0
+};
+// request j (0 ..) of quarters Q0, Q0 + 1, .. of a stage whose first quarter is in slot `slot`; past the last quarter: the scales
+template <int TB, int Q0, int J>
+__device__ __forceinline__ void l8_request(const L8Src<TB>& src, uint32_t slot, uint32_t scale_addr) {
+    constexpr int q = Q0 + J / 4, j = J % 4, NQ = 2 + TB / 2;
+    if constexpr (q == NQ) {
+        static_assert(j == 0, "one request for the scales");
+        l8_load_lds<4>(src.s, src.s_off, scale_addr);
+    } else {
+        uint32_t at = slot + q;
+        at = at >= kRing ? at - kRing : at;
+        if constexpr (q < 2) l8_load_lds<16>(src.w, src.w_off[4 * q + j], src.lds + at * kSlot + j * 4096);
+        else l8_load_lds<16>(src.x, src.x_off[4 * (q - 2) + j], src.lds + at * kSlot + j * 4096);
+    }
+}
+
+template <int TB, int J>
+__device__ __forceinline__ void l8_fetch(u32x4 (&fn)[8 + 2 * TB], uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1) {
+    if constexpr (J < 8) fn[J] = l8_lds_read16<(J >> 1) * 4096>(J & 1 ? a1 : a0);
+    else if constexpr (J < 8 + 2 * TB) fn[J] = l8_lds_read16<((J - 8) >> 1) * 4096>(J & 1 ? b1 : b0);
+}
+// One k step: 4 TB matrix instructions on the operand set fc (piece pairs of blocks 0..3: weights, 4..: activations).  Behind each
+// of them go some of the LDS reads of the next set fn and of the NLOAD requests (from quarter Q0 on), so that their issue runs
+// under the matrix pipe.
+#define L8_KS(I)                                                                                                              \
+    if constexpr ((I) < 4 * TB) {                                                                                             \
+        constexpr int cb = (I) / TB, tb = (I) % TB;                                                                           \
+        acc[cb][tb] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(l8_join(fc[2 * cb], fc[2 * cb + 1]),                    \
+                                                                      l8_join(fc[8 + 2 * tb], fc[9 + 2 * tb]), acc[cb][tb], 0, 0, 0, we, tb, xe); \
+        __builtin_amdgcn_sched_barrier(0);                                                                                    \
+        if constexpr (FETCH) {                                                                                                \
+            l8_fetch<TB, (I) * kRd>(fn, a0, a1, b0, b1);                                                                      \
+            if constexpr (kRd == 2) l8_fetch<TB, (I) * kRd + 1>(fn, a0, a1, b0, b1);                                          \
+            __builtin_amdgcn_sched_barrier(0);                                                                                \
+        }                                                                                                                     \
+        if constexpr ((I) * kLd < NLOAD) {                                                                                    \
+            l8_request<TB, Q0, (I) * kLd>(src, slot, scale_addr);                                                             \
+            if constexpr (kLd == 2 && (I) * kLd + 1 < NLOAD) l8_request<TB, Q0, (I) * kLd + 1>(src, slot, scale_addr);        \
+            __builtin_amdgcn_sched_barrier(0);                                                                                \
+        }                                                                                                                     \
+    }
+template <int TB, bool FETCH, int NLOAD, int Q0>
+__device__ __forceinline__ void l8_kstep(f32x16 (&acc)[4][TB], const u32x4 (&fc)[8 + 2 * TB], u32x4 (&fn)[8 + 2 * TB], uint32_t a0, uint32_t a1,
+                                         uint32_t b0, uint32_t b1, int we, int xe, const L8Src<TB>& src, uint32_t slot, uint32_t scale_addr) {
+    constexpr int kRd = TB == 4 ? 1 : 2;                       // LDS reads per matrix instruction
+    constexpr int kLd = NLOAD > 4 * TB ? 2 : 1;                // requests per matrix instruction
+    static_assert(NLOAD <= kLd * 4 * TB, "requests fit the step");
+    L8_KS(0) L8_KS(1) L8_KS(2) L8_KS(3) L8_KS(4) L8_KS(5) L8_KS(6) L8_KS(7)
+    L8_KS(8) L8_KS(9) L8_KS(10) L8_KS(11) L8_KS(12) L8_KS(13) L8_KS(14) L8_KS(15)
+}
+#undef L8_KS
+
+template <class E, int EPI, int TB>
+__global__ __launch_bounds__(256) void l8_tile_kernel(L8Args p) {
+    constexpr int kTileM = 64 * TB;
+    constexpr int NQ = 2 + TB / 2, kLoads = 4 * NQ + 1;        // slots and a wave's load instructions of a stage
+    constexpr int kAhead = TB == 4 ? 2 : 3;                    // stage s + kAhead is requested while stage s is multiplied ..
+    constexpr int kEarly = TB == 4 ? 4 : 0;                    // .. so many of its requests before stage s has been read
+    extern __shared__ __attribute__((aligned(256))) uint8_t l8_lds[];
+    const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) uint8_t*)l8_lds;
+    const int tid = threadIdx.x, lane = tid & 63, m = lane & 31, hf = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wn = wave & 1, wm = wave >> 1;
+
+    // every eighth workgroup shares an XCD: each XCD gets a contiguous run of the patch order
+    const int ntiles = p.tm * p.tn, per_xcd = (ntiles + 7) / 8;
+    const int v = (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
+    if (v >= ntiles) return;
+    const int patch = v / (kGroupM * p.tn), first = patch * kGroupM, gsize = min(kGroupM, p.tm - first);
+    const int within = v - patch * kGroupM * p.tn;
+    const int tile_n = __builtin_amdgcn_readfirstlane(within / gsize);
+    const int64_t m0 = (int64_t)__builtin_amdgcn_readfirstlane(first + within - tile_n * gsize) * kTileM;
+    const int n0 = tile_n * kTileN;
+
+    // request j of a wave fills rows 8 (4 j + wave) .. + 7 of a slot; rows past the end repeat the last
+    L8Src<TB> src;
+    src.w = p.w + (int64_t)n0 * p.kp;
+    src.x = p.x + m0 * p.kp;
+    src.s = p.xscale;
+    src.lds = lds0 + (uint32_t)wave * 1024;
+    {
+        const int g_row = lane >> 3, g_c = (lane & 7) ^ ((((wave & 1) << 2) + (lane >> 4)) & 7);
+        const int wlast = p.N - 1 - n0, xlast = (int)min(p.M - 1 - m0, (int64_t)kTileM - 1);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) src.w_off[j] = (uint32_t)min((4 * j + wave) * 8 + g_row, wlast) * (uint32_t)p.kp + g_c * 16;
+#pragma unroll
+        for (int j = 0; j < 2 * TB; ++j) src.x_off[j] = (uint32_t)min((4 * j + wave) * 8 + g_row, xlast) * (uint32_t)p.kp + g_c * 16;
+        src.s += min(m0 >> 7, p.groups - 1) * 128;
+        src.s_off = (uint32_t)(lane * 4 - ((m0 >> 7) + 1 < p.groups ? 0 : 128 * hf));
+    }
+    const int64_t s_step = p.groups * 128;
+    auto advance = [&]() {
+        src.w += kBlock8;
+        src.x += kBlock8;
+        src.s += s_step;
+    };
+    const auto* wsp = (const __attribute__((address_space(4))) uint32_t*)(size_t)(p.wscale + (int64_t)min((n0 >> 7) + wn, (p.N - 1) >> 7) * p.pitch);
+    auto w_exp = [&](int s) { return (int)(wsp[s >> 2] >> (8 * (s & 3))) & 0xff; };
+
+    f32x16 acc[4][TB];
+#pragma unroll
+    for (int cb = 0; cb < 4; ++cb)
+#pragma unroll
+        for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[cb][tb][i] = 0.f;
+
+    // operand read addresses of the pieces of a row, relative to a slot (of the wave's weight rows / activation rows)
+    const int sw = (m >> 1) & 7;
+    uint32_t ka[4], kb[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const uint32_t ko = (uint32_t)(((2 * q + hf) ^ sw) << 4);
+        ka[q] = lds0 + (uint32_t)(m * 128) + ko;
+        kb[q] = lds0 + (uint32_t)(((TB == 4 ? 0 : wm * 64) + m) * 128) + ko;
+    }
+    const uint32_t ks = lds0 + kScaleAt + (uint32_t)(((TB == 4 ? wm : 0) * 32 + m) * 4);
+    const int xsh = TB == 4 ? 0 : 16 * wm;
+
+    // Quarter q of stage s lives in slot (NQ s + q) % 9.  Iteration s multiplies stage s in two k steps; the operands of a step are
+    // read during the step before.  After its first step a wave has read all of stage s: it waits for its own loads of stage
+    // s + 1, meets the others, and requests the next stage into the slots of stage s (TB = 4: the first quarter of stage s + 2 has
+    // a slot already before that).
+    const int nstage = p.nkb;
+    auto wrap = [](uint32_t h) { return h >= kRing ? h - kRing : h; };
+    auto scale_at = [&](int s) { return lds0 + kScaleAt + (uint32_t)(s & 3) * kScaleSlot; };
+    auto whole_stage = [&](int s) {
+        const uint32_t slot = (uint32_t)(NQ * s) % kRing;
+#define L8_RQ(J) if constexpr ((J) < kLoads) l8_request<TB, 0, (J) < kLoads ? (J) : 0>(src, slot, scale_at(s));
+        L8_RQ(0) L8_RQ(1) L8_RQ(2) L8_RQ(3) L8_RQ(4) L8_RQ(5) L8_RQ(6) L8_RQ(7) L8_RQ(8) L8_RQ(9) L8_RQ(10) L8_RQ(11) L8_RQ(12)
+        L8_RQ(13) L8_RQ(14) L8_RQ(15) L8_RQ(16)
+#undef L8_RQ
+        advance();
+    };
+    whole_stage(0);
+    if (nstage > 1) whole_stage(1);
+    if (kAhead == 3 && nstage > 2) whole_stage(2);
+    if (kAhead == 3 && nstage > 2) l8_wait_stage<2 * kLoads>();
+    else if (nstage > 1) l8_wait_stage<kLoads>();
+    else l8_wait_stage<0>();
+    u32x4 f0[8 + 2 * TB], f1[8 + 2 * TB];
+    uint32_t hs = 0;                                           // slot of the first quarter of the stage being multiplied
+    uint32_t xe0, xe1;
+    xe0 = l8_lds_read4(ks);
+    {
+        const uint32_t a = wn * kSlot, b = (2 + (TB == 4 ? wm : 0)) * kSlot;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            f0[0 + c] = l8_lds_read16<0>(ka[c] + a);
+            f0[2 + c] = l8_lds_read16<4096>(ka[c] + a);
+            f0[4 + c] = l8_lds_read16<8192>(ka[c] + a);
+            f0[6 + c] = l8_lds_read16<12288>(ka[c] + a);
+            f0[8 + c] = l8_lds_read16<0>(kb[c] + b);
+            f0[10 + c] = l8_lds_read16<4096>(kb[c] + b);
+            if constexpr (TB == 4) {
+                f0[12 + c] = l8_lds_read16<8192>(kb[c] + b);
+                f0[14 + c] = l8_lds_read16<12288>(kb[c] + b);
+            }
+        }
+    }
+    int s = 0, we = w_exp(0);
+    // LOAD: request stage s + kAhead; WAIT: loads that may stay outstanding at the barrier; LAST: no barrier
+#define L8_ITER(LOAD, WAIT, LAST)                                                                                              \
+    {                                                                                                                          \
+        const uint32_t sa = wrap(hs + wn) * kSlot, sb = wrap(hs + 2 + (TB == 4 ? wm : 0)) * kSlot;                             \
+        const uint32_t ns = wrap(hs + (NQ * kAhead) % kRing);                                                                  \
+        const uint32_t sc = scale_at(s + kAhead);                                                                              \
+        const int wec = we;                                                                                                    \
+        if (!LAST) we = w_exp(s + 1);                                                                                          \
+        l8_wait_frags(f0, xe0);                                                                                                \
+        const int xe = (int)(xe0 >> xsh);                                                                                      \
+        l8_kstep<TB, true, LOAD ? kEarly : 0, 0>(acc, f0, f1, ka[2] + sa, ka[3] + sa, kb[2] + sb, kb[3] + sb, wec, xe, src, ns, sc); \
+        l8_wait_frags(f1, xe0);                                /* this wave has read all of the stage */                       \
+        if (!LAST) {                                                                                                           \
+            l8_wait_stage<WAIT>();                                                                                             \
+            hs = wrap(hs + NQ);                                                                                                \
+            const uint32_t na = wrap(hs + wn) * kSlot, nb = wrap(hs + 2 + (TB == 4 ? wm : 0)) * kSlot;                         \
+            xe1 = l8_lds_read4(ks + (uint32_t)((s + 1) & 3) * kScaleSlot);                                                     \
+            l8_kstep<TB, true, LOAD ? kLoads - kEarly : 0, kEarly / 4>(acc, f1, f0, ka[0] + na, ka[1] + na, kb[0] + nb, kb[1] + nb, wec, xe, src, ns, sc); \
+            if (LOAD) advance();                                                                                               \
+            xe0 = xe1;                                                                                                         \
+            ++s;                                                                                                               \
+        } else {                                                                                                               \
+            l8_kstep<TB, false, 0, 0>(acc, f1, f0, 0, 0, 0, 0, wec, xe, src, 0, 0);                                            \
+        }                                                                                                                      \
+    }
+    if constexpr (TB == 4) {
+        while (s + 2 < nstage) L8_ITER(true, 4, false)
+    } else {
+        while (s + 3 < nstage) L8_ITER(true, kLoads, false)
+        if (nstage >= 3) L8_ITER(false, kLoads, false)
+    }
+    if (nstage >= 2) L8_ITER(false, 0, false)
+    L8_ITER(false, 0, true)
+#undef L8_ITER
+
+    // lane (m, hf) of block (cb, tb) holds row 32 tb + m, channels 8 g + 4 hf + (i & 3), i = 4 g + ..
+    const int64_t row0 = m0 + wm * 32 * TB + m;
+    if (p.vec && n0 + wn * 128 + 128 <= p.N) {                 // whole: 16-byte stores, a block column's operands loaded together
+#pragma unroll
+        for (int cb = 0; cb < 4; ++cb) {
+            const int cbase = n0 + wn * 128 + 32 * cb;
+            float bia[16];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                u32x2 b = {0u, 0u};
+                if (p.bias != nullptr) b = *(const u32x2*)(p.bias + cbase + 8 * g + 4 * hf);
+                l8_unpack4<E>(b, bia + 4 * g);
+            }
+#pragma unroll
+            for (int tb = 0; tb < TB; ++tb) {
+                const int64_t row = row0 + 32 * tb, rc = min(row, p.M - 1);
+                float res[16], gate[16];
+                if (EPI == SFM_EPI_GATE_RESIDUAL) {
+                    const uint16_t *rp = p.res + rc * p.res_stride + cbase + 4 * hf;
+                    const uint16_t *gp = p.gate != nullptr ? p.gate + (rc / p.rows_per_frame) * p.gate_stride + cbase + 4 * hf : nullptr;
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        l8_unpack4<E>(*(const u32x2*)(rp + 8 * g), res + 4 * g);
+                        if (gp != nullptr) {
+                            l8_unpack4<E>(*(const u32x2*)(gp + 8 * g), gate + 4 * g);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) gate[4 * g + i] = 1.f;
+                        }
+                    }
+                }
+                uint32_t w[8];
+#pragma unroll
+                for (int i = 0; i < 16; i += 2)
+                    w[i / 2] = pack2<E>(l8_tail<E, EPI>(acc[cb][tb][i], bia[i], res[i], gate[i]),
+                                        l8_tail<E, EPI>(acc[cb][tb][i + 1], bia[i + 1], res[i + 1], gate[i + 1]));
+#pragma unroll
+                for (int gp = 0; gp < 2; ++gp) {               // the two lanes of a row exchange halves: 16 bytes each
+                    auto rx = __builtin_amdgcn_permlane32_swap(w[4 * gp], w[4 * gp + 2], false, false);
+                    auto ry = __builtin_amdgcn_permlane32_swap(w[4 * gp + 1], w[4 * gp + 3], false, false);
+                    u32x4 o = {(uint32_t)rx[0], (uint32_t)ry[0], (uint32_t)rx[1], (uint32_t)ry[1]};
+                    if (row < p.M) *(u32x4*)(p.out + row * p.out_stride + cbase + 16 * gp + 8 * hf) = o;
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int cb = 0; cb < 4; ++cb)
+#pragma unroll
+            for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const float a4[4] = {acc[cb][tb][4 * g], acc[cb][tb][4 * g + 1], acc[cb][tb][4 * g + 2], acc[cb][tb][4 * g + 3]};
+                    l8_finish4<E, EPI>(p, row0 + 32 * tb, n0 + wn * 128 + 32 * cb + 8 * g + 4 * hf, a4);
+                }
+    }
+}
+
+template <class E, int EPI, int TB>
+int launch_tile(const L8Args& a0, hipStream_t st) {
+    static bool configured = false;          // the attribute belongs to the function; racing callers set the same value
+    if (!configured) {
+        hipError_t e = hipFuncSetAttribute((const void*)l8_tile_kernel<E, EPI, TB>, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes);
+        if (e != hipSuccess) {
+            set_error("sfm_linear8: hipFuncSetAttribute failed: %s", hipGetErrorString(e));
+            return SFM_ERR_HIP;
+        }
+        configured = true;
+    }
+    L8Args a = a0;
+    a.tm = (int)((a.M + 64 * TB - 1) / (64 * TB));
+    a.tn = (a.N + kTileN - 1) / kTileN;
+    hipLaunchKernelGGL((l8_tile_kernel<E, EPI, TB>), dim3((unsigned)((a.tm * a.tn + 7) / 8 * 8)), dim3(256), kLdsBytes, st, a);
+    return launched8("sfm_linear8");
+}
+
 template <class E, int EPI>
 int launch_epi(const L8Args& a, hipStream_t st) {
     if (a.M <= 16) return launch_direct<E, EPI, 1, 1, 8>(a, st);
+    if (a.M >= 1024 && a.N >= 256) return launch_tile<E, EPI, 4>(a, st);
+    if (a.M >= 256 && a.N >= 256) return launch_tile<E, EPI, 2>(a, st);
     return launch_direct<E, EPI, 4, 4, 4>(a, st);
 }
 

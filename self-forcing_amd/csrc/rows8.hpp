@@ -59,6 +59,7 @@ __device__ __forceinline__ float wave_sum(float v) {
 }
 
 
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
 
 template <typename T> constexpr bool kWide = std::is_same<T, float>::value;      // 4-byte elements
@@ -137,11 +138,12 @@ __device__ __forceinline__ float max16(float a) {
 }
 
 // GELU in its tanh form, 0.5 x (1 + tanh(u)) with u = sqrt(2/pi) (x + 0.044715 x^3), as x p with p = 1 / (1 + exp(-2u)): no
-// cancellation where tanh approaches -1.  FULL: expf instead of the hardware's exponential (fp32 tensors).
+// cancellation where tanh approaches -1.  FULL (fp32 tensors): expf and a division; otherwise the hardware's 2^x and reciprocal,
+// good to a unit of fp32 each, with -2 log2(e) in the constants.
 template <bool FULL>
 __device__ __forceinline__ float gelu_gate(float x) {
-    const float u2 = -1.5957691216057308f * (x + 0.044715f * x * x * x);
-    return 1.f / (1.f + (FULL ? expf(u2) : __expf(u2)));
+    if (FULL) return 1.f / (1.f + expf(-1.5957691216057308f * (x + 0.044715f * x * x * x)));
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * (-2.3022082f - 0.10294324f * x * x)));
 }
 // d gelu / dx = p + x p (1 - p) 2 u'(x); past |x| = 16 p is 0 or 1 to fp32
 template <bool FULL>
