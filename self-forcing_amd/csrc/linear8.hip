@@ -14,6 +14,8 @@
 // Weight rows are the A operand and activation rows the B operand, so that a lane ends up with neighbouring channels of
 // one row.
 
+#include <utility>
+
 #include "rows8.hpp"
 
 namespace sfm {
@@ -33,6 +35,7 @@ struct L8Args {
     int64_t out_stride, res_stride, gate_stride;
     int rows_per_frame;
     int tm, tn;              // tiles along M and N
+    int half;                // 1: the last strip of tiles has half the rows
     bool vec;                // rows of out, res, gate and bias allow 8-byte accesses
 };
 
@@ -169,16 +172,18 @@ int launch_direct(const L8Args& a0, hipStream_t st) {
 // Scales: the 64 words of a stage's 256 rows follow the rows into LDS, a lane's word holds those of its row in the four row blocks
 // (rows8.hpp), and the matrix instruction picks the byte; the weight's is one for the wave, through the scalar cache.
 constexpr int kTileN = 256, kSlot = 128 * kBlock8, kRing = 9;
-constexpr int kScaleAt = kRing * kSlot, kScaleSlot = 256, kLdsBytes = kScaleAt + 4 * kScaleSlot;
+constexpr int kScaleAt = kRing * kSlot, kScaleSlot = 256;
+constexpr int kLdsBytes = kScaleAt + 4 * kScaleSlot;
 constexpr int kGroupM = 8;                   // row tiles per patch of the tile order
 
-template <int BYTES>
+// BYTES a lane from base + off to LDS at lds_addr + ADD, lane after lane
+template <int BYTES, int ADD>
 __device__ __forceinline__ void l8_load_lds(const void* base, uint32_t off, uint32_t lds_addr) {
     static_assert(BYTES == 16 || BYTES == 4, "");
     if constexpr (BYTES == 16)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_addr), "v"(off), "s"(base) : "memory", "m0");
+        asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_addr), "v"(off), "s"(base), "n"(ADD) : "memory", "m0", "scc");
     else
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_addr), "v"(off), "s"(base) : "memory", "m0");
+        asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_addr), "v"(off), "s"(base), "n"(ADD) : "memory", "m0", "scc");
 }
 // waits until at most N of this wave's loads are outstanding (they complete in order), then the barrier
 template <int N>
@@ -205,228 +210,96 @@ __device__ __forceinline__ i32x8 l8_join(u32x4 a, u32x4 b) {
     return __builtin_shufflevector(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// where a wave's loads go: request j of a list of quarter stages (4 requests each), then the scales
+// where a wave's requests go: quarter stages of 128 rows (4 requests each), then the scales
 template <int TB>
 struct L8Src {
-    const uint8_t *w, *x, *s;                // stage of the next request
+    const uint8_t *w, *x, *s;                // of the stage to be requested next
     uint32_t w_off[8], x_off[2 * TB], s_off;
     uint32_t lds;                            // LDS address of this wave's first 1 KB in slot 0
 };
-// request j (0 ..) of quarters Q0, Q0 + 1, .. of a stage whose first quarter is in slot `slot`; past the last quarter: the scales
+__device__ __forceinline__ uint32_t l8_wrap(uint32_t slot) { return slot >= kRing ? slot - kRing : slot; }
+// request J of the quarters Q0, Q0 + 1, .. of a stage whose first quarter is in `slot`; past the last quarter: the scales
 template <int TB, int Q0, int J>
 __device__ __forceinline__ void l8_request(const L8Src<TB>& src, uint32_t slot, uint32_t scale_addr) {
     constexpr int q = Q0 + J / 4, j = J % 4, NQ = 2 + TB / 2;
     if constexpr (q == NQ) {
         static_assert(j == 0, "one request for the scales");
-        l8_load_lds<4>(src.s, src.s_off, scale_addr);
+        l8_load_lds<4, 0>(src.s, src.s_off, scale_addr);
     } else {
-        uint32_t at = slot + q;
-        at = at >= kRing ? at - kRing : at;
-        if constexpr (q < 2) l8_load_lds<16>(src.w, src.w_off[4 * q + j], src.lds + at * kSlot + j * 4096);
-        else l8_load_lds<16>(src.x, src.x_off[4 * (q - 2) + j], src.lds + at * kSlot + j * 4096);
+        const uint32_t at = src.lds + l8_wrap(slot + q) * kSlot;
+        if constexpr (q < 2) l8_load_lds<16, j * 4096>(src.w, src.w_off[4 * q + j], at);
+        else l8_load_lds<16, j * 4096>(src.x, src.x_off[4 * (q - 2) + j], at);
     }
 }
-
+// piece J of an operand set: two pieces of each weight block, then of each activation block
 template <int TB, int J>
 __device__ __forceinline__ void l8_fetch(u32x4 (&fn)[8 + 2 * TB], uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1) {
     if constexpr (J < 8) fn[J] = l8_lds_read16<(J >> 1) * 4096>(J & 1 ? a1 : a0);
-    else if constexpr (J < 8 + 2 * TB) fn[J] = l8_lds_read16<((J - 8) >> 1) * 4096>(J & 1 ? b1 : b0);
+    else fn[J] = l8_lds_read16<((J - 8) >> 1) * 4096>(J & 1 ? b1 : b0);
 }
-// One k step: 4 TB matrix instructions on the operand set fc (piece pairs of blocks 0..3: weights, 4..: activations).  Behind each
-// of them go some of the LDS reads of the next set fn and of the NLOAD requests (from quarter Q0 on), so that their issue runs
-// under the matrix pipe.
-#define L8_KS(I)                                                                                                              \
-    if constexpr ((I) < 4 * TB) {                                                                                             \
-        constexpr int cb = (I) / TB, tb = (I) % TB;                                                                           \
-        acc[cb][tb] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(l8_join(fc[2 * cb], fc[2 * cb + 1]),                    \
-                                                                      l8_join(fc[8 + 2 * tb], fc[9 + 2 * tb]), acc[cb][tb], 0, 0, 0, we, tb, xe); \
-        __builtin_amdgcn_sched_barrier(0);                                                                                    \
-        if constexpr (FETCH) {                                                                                                \
-            l8_fetch<TB, (I) * kRd>(fn, a0, a1, b0, b1);                                                                      \
-            if constexpr (kRd == 2) l8_fetch<TB, (I) * kRd + 1>(fn, a0, a1, b0, b1);                                          \
-            __builtin_amdgcn_sched_barrier(0);                                                                                \
-        }                                                                                                                     \
-        if constexpr ((I) * kLd < NLOAD) {                                                                                    \
-            l8_request<TB, Q0, (I) * kLd>(src, slot, scale_addr);                                                             \
-            if constexpr (kLd == 2 && (I) * kLd + 1 < NLOAD) l8_request<TB, Q0, (I) * kLd + 1>(src, slot, scale_addr);        \
-            __builtin_amdgcn_sched_barrier(0);                                                                                \
-        }                                                                                                                     \
-    }
-template <int TB, bool FETCH, int NLOAD, int Q0>
-__device__ __forceinline__ void l8_kstep(f32x16 (&acc)[4][TB], const u32x4 (&fc)[8 + 2 * TB], u32x4 (&fn)[8 + 2 * TB], uint32_t a0, uint32_t a1,
-                                         uint32_t b0, uint32_t b1, int we, int xe, const L8Src<TB>& src, uint32_t slot, uint32_t scale_addr) {
-    constexpr int kRd = TB == 4 ? 1 : 2;                       // LDS reads per matrix instruction
-    constexpr int kLd = NLOAD > 4 * TB ? 2 : 1;                // requests per matrix instruction
-    static_assert(NLOAD <= kLd * 4 * TB, "requests fit the step");
-    L8_KS(0) L8_KS(1) L8_KS(2) L8_KS(3) L8_KS(4) L8_KS(5) L8_KS(6) L8_KS(7)
-    L8_KS(8) L8_KS(9) L8_KS(10) L8_KS(11) L8_KS(12) L8_KS(13) L8_KS(14) L8_KS(15)
+template <int TB, int... J>
+__device__ __forceinline__ void l8_fetch_all(std::integer_sequence<int, J...>, u32x4 (&fn)[8 + 2 * TB], uint32_t a0, uint32_t a1, uint32_t b0,
+                                             uint32_t b1) {
+    (l8_fetch<TB, J>(fn, a0, a1, b0, b1), ...);
 }
-#undef L8_KS
+// One k step: 4 x TB matrix instructions on the operand set fc.  Behind each of them go some of the
+// LDS reads of the next set fn and of NLOAD requests (from quarter Q0 on), so that their issue runs under the matrix pipe.
+template <int TB, bool FETCH, int NLOAD, int Q0, int I>
+__device__ __forceinline__ void l8_kone(f32x16 (&acc)[4][TB], const u32x4 (&fc)[8 + 2 * TB], u32x4 (&fn)[8 + 2 * TB], uint32_t a0, uint32_t a1,
+                                        uint32_t b0, uint32_t b1, int we, int xe, const L8Src<TB>& src, uint32_t slot, uint32_t scale_addr) {
+    // A matrix instruction takes the time of a dozen others.  The reads are done three of them before the end of the step, where
+    // they are waited for; requests go one behind each where there are many, else behind the reads.
+    constexpr int kMM = 4 * TB, kReads = 8 + 2 * TB, kTwo = kMM == 16 ? (NLOAD > 4 ? 4 : 8) : kMM;
+    constexpr int kR0 = I < kTwo ? 2 * I : kTwo + I, kR1 = I < kTwo ? kR0 + 2 : kR0 + 1;
+    constexpr int kLd = NLOAD > kMM ? 2 : 1, kL0 = NLOAD > 4 || kMM < 16 ? kLd * I : I - 8, kL1 = kL0 + kLd;
+    constexpr int cb = I / TB, tb = I % TB;
+    acc[cb][tb] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(l8_join(fc[2 * cb], fc[2 * cb + 1]), l8_join(fc[8 + 2 * tb], fc[9 + 2 * tb]),
+                                                                  acc[cb][tb], 0, 0, 0, we, tb, xe);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (FETCH && kR0 < kReads) l8_fetch<TB, kR0>(fn, a0, a1, b0, b1);
+    if constexpr (FETCH && kR1 == kR0 + 2 && kR0 + 1 < kReads) l8_fetch<TB, kR0 + 1>(fn, a0, a1, b0, b1);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (kL0 >= 0 && kL0 < NLOAD) l8_request<TB, Q0, kL0>(src, slot, scale_addr);
+    if constexpr (kL1 == kL0 + 2 && kL0 + 1 < NLOAD) l8_request<TB, Q0, kL0 + 1>(src, slot, scale_addr);
+    __builtin_amdgcn_sched_barrier(0);
+}
+template <int TB, bool FETCH, int NLOAD, int Q0, int... I>
+__device__ __forceinline__ void l8_kstep(std::integer_sequence<int, I...>, f32x16 (&acc)[4][TB], const u32x4 (&fc)[8 + 2 * TB],
+                                         u32x4 (&fn)[8 + 2 * TB], uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1, int we, int xe,
+                                         const L8Src<TB>& src, uint32_t slot, uint32_t scale_addr) {
+    (l8_kone<TB, FETCH, NLOAD, Q0, I>(acc, fc, fn, a0, a1, b0, b1, we, xe, src, slot, scale_addr), ...);
+}
 
-template <class E, int EPI, int TB>
-__global__ __launch_bounds__(256) void l8_tile_kernel(L8Args p) {
-    constexpr int kTileM = 64 * TB;
-    constexpr int NQ = 2 + TB / 2, kLoads = 4 * NQ + 1;        // slots and a wave's load instructions of a stage
-    constexpr int kAhead = TB == 4 ? 2 : 3;                    // stage s + kAhead is requested while stage s is multiplied ..
-    constexpr int kEarly = TB == 4 ? 4 : 0;                    // .. so many of its requests before stage s has been read
-    extern __shared__ __attribute__((aligned(256))) uint8_t l8_lds[];
-    const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) uint8_t*)l8_lds;
-    const int tid = threadIdx.x, lane = tid & 63, m = lane & 31, hf = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wn = wave & 1, wm = wave >> 1;
-
-    // every eighth workgroup shares an XCD: each XCD gets a contiguous run of the patch order
-    const int ntiles = p.tm * p.tn, per_xcd = (ntiles + 7) / 8;
-    const int v = (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
-    if (v >= ntiles) return;
-    const int patch = v / (kGroupM * p.tn), first = patch * kGroupM, gsize = min(kGroupM, p.tm - first);
-    const int within = v - patch * kGroupM * p.tn;
-    const int tile_n = __builtin_amdgcn_readfirstlane(within / gsize);
-    const int64_t m0 = (int64_t)__builtin_amdgcn_readfirstlane(first + within - tile_n * gsize) * kTileM;
-    const int n0 = tile_n * kTileN;
-
-    // request j of a wave fills rows 8 (4 j + wave) .. + 7 of a slot; rows past the end repeat the last
-    L8Src<TB> src;
-    src.w = p.w + (int64_t)n0 * p.kp;
-    src.x = p.x + m0 * p.kp;
-    src.s = p.xscale;
-    src.lds = lds0 + (uint32_t)wave * 1024;
-    {
-        const int g_row = lane >> 3, g_c = (lane & 7) ^ ((((wave & 1) << 2) + (lane >> 4)) & 7);
-        const int wlast = p.N - 1 - n0, xlast = (int)min(p.M - 1 - m0, (int64_t)kTileM - 1);
+// sums to memory: CB x TB blocks of 32 channels x 32 rows from channel c0, row r0 on.  Lane (m, hf) of block (cb, tb) holds row
+// 32 tb + m, channels 8 g + 4 hf + (i & 3), i = 4 g + ..  One block after the other, each with addresses of its own: formed for all
+// blocks together they would not fit beside the sums.
+template <class E, int EPI, int TB, int CB>
+__device__ __forceinline__ void l8_store(const L8Args& p, const f32x16 (&acc)[4][TB], int c0, int64_t r0, int m, int hf) {
+    if (p.vec && c0 + 32 * CB <= p.N && r0 + 32 * TB <= p.M) { // whole: 16-byte stores
 #pragma unroll
-        for (int j = 0; j < 8; ++j) src.w_off[j] = (uint32_t)min((4 * j + wave) * 8 + g_row, wlast) * (uint32_t)p.kp + g_c * 16;
-#pragma unroll
-        for (int j = 0; j < 2 * TB; ++j) src.x_off[j] = (uint32_t)min((4 * j + wave) * 8 + g_row, xlast) * (uint32_t)p.kp + g_c * 16;
-        src.s += min(m0 >> 7, p.groups - 1) * 128;
-        src.s_off = (uint32_t)(lane * 4 - ((m0 >> 7) + 1 < p.groups ? 0 : 128 * hf));
-    }
-    const int64_t s_step = p.groups * 128;
-    auto advance = [&]() {
-        src.w += kBlock8;
-        src.x += kBlock8;
-        src.s += s_step;
-    };
-    const auto* wsp = (const __attribute__((address_space(4))) uint32_t*)(size_t)(p.wscale + (int64_t)min((n0 >> 7) + wn, (p.N - 1) >> 7) * p.pitch);
-    auto w_exp = [&](int s) { return (int)(wsp[s >> 2] >> (8 * (s & 3))) & 0xff; };
-
-    f32x16 acc[4][TB];
-#pragma unroll
-    for (int cb = 0; cb < 4; ++cb)
-#pragma unroll
-        for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[cb][tb][i] = 0.f;
-
-    // operand read addresses of the pieces of a row, relative to a slot (of the wave's weight rows / activation rows)
-    const int sw = (m >> 1) & 7;
-    uint32_t ka[4], kb[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const uint32_t ko = (uint32_t)(((2 * q + hf) ^ sw) << 4);
-        ka[q] = lds0 + (uint32_t)(m * 128) + ko;
-        kb[q] = lds0 + (uint32_t)(((TB == 4 ? 0 : wm * 64) + m) * 128) + ko;
-    }
-    const uint32_t ks = lds0 + kScaleAt + (uint32_t)(((TB == 4 ? wm : 0) * 32 + m) * 4);
-    const int xsh = TB == 4 ? 0 : 16 * wm;
-
-    // Quarter q of stage s lives in slot (NQ s + q) % 9.  Iteration s multiplies stage s in two k steps; the operands of a step are
-    // read during the step before.  After its first step a wave has read all of stage s: it waits for its own loads of stage
-    // s + 1, meets the others, and requests the next stage into the slots of stage s (TB = 4: the first quarter of stage s + 2 has
-    // a slot already before that).
-    const int nstage = p.nkb;
-    auto wrap = [](uint32_t h) { return h >= kRing ? h - kRing : h; };
-    auto scale_at = [&](int s) { return lds0 + kScaleAt + (uint32_t)(s & 3) * kScaleSlot; };
-    auto whole_stage = [&](int s) {
-        const uint32_t slot = (uint32_t)(NQ * s) % kRing;
-#define L8_RQ(J) if constexpr ((J) < kLoads) l8_request<TB, 0, (J) < kLoads ? (J) : 0>(src, slot, scale_at(s));
-        L8_RQ(0) L8_RQ(1) L8_RQ(2) L8_RQ(3) L8_RQ(4) L8_RQ(5) L8_RQ(6) L8_RQ(7) L8_RQ(8) L8_RQ(9) L8_RQ(10) L8_RQ(11) L8_RQ(12)
-        L8_RQ(13) L8_RQ(14) L8_RQ(15) L8_RQ(16)
-#undef L8_RQ
-        advance();
-    };
-    whole_stage(0);
-    if (nstage > 1) whole_stage(1);
-    if (kAhead == 3 && nstage > 2) whole_stage(2);
-    if (kAhead == 3 && nstage > 2) l8_wait_stage<2 * kLoads>();
-    else if (nstage > 1) l8_wait_stage<kLoads>();
-    else l8_wait_stage<0>();
-    u32x4 f0[8 + 2 * TB], f1[8 + 2 * TB];
-    uint32_t hs = 0;                                           // slot of the first quarter of the stage being multiplied
-    uint32_t xe0, xe1;
-    xe0 = l8_lds_read4(ks);
-    {
-        const uint32_t a = wn * kSlot, b = (2 + (TB == 4 ? wm : 0)) * kSlot;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            f0[0 + c] = l8_lds_read16<0>(ka[c] + a);
-            f0[2 + c] = l8_lds_read16<4096>(ka[c] + a);
-            f0[4 + c] = l8_lds_read16<8192>(ka[c] + a);
-            f0[6 + c] = l8_lds_read16<12288>(ka[c] + a);
-            f0[8 + c] = l8_lds_read16<0>(kb[c] + b);
-            f0[10 + c] = l8_lds_read16<4096>(kb[c] + b);
-            if constexpr (TB == 4) {
-                f0[12 + c] = l8_lds_read16<8192>(kb[c] + b);
-                f0[14 + c] = l8_lds_read16<12288>(kb[c] + b);
-            }
-        }
-    }
-    int s = 0, we = w_exp(0);
-    // LOAD: request stage s + kAhead; WAIT: loads that may stay outstanding at the barrier; LAST: no barrier
-#define L8_ITER(LOAD, WAIT, LAST)                                                                                              \
-    {                                                                                                                          \
-        const uint32_t sa = wrap(hs + wn) * kSlot, sb = wrap(hs + 2 + (TB == 4 ? wm : 0)) * kSlot;                             \
-        const uint32_t ns = wrap(hs + (NQ * kAhead) % kRing);                                                                  \
-        const uint32_t sc = scale_at(s + kAhead);                                                                              \
-        const int wec = we;                                                                                                    \
-        if (!LAST) we = w_exp(s + 1);                                                                                          \
-        l8_wait_frags(f0, xe0);                                                                                                \
-        const int xe = (int)(xe0 >> xsh);                                                                                      \
-        l8_kstep<TB, true, LOAD ? kEarly : 0, 0>(acc, f0, f1, ka[2] + sa, ka[3] + sa, kb[2] + sb, kb[3] + sb, wec, xe, src, ns, sc); \
-        l8_wait_frags(f1, xe0);                                /* this wave has read all of the stage */                       \
-        if (!LAST) {                                                                                                           \
-            l8_wait_stage<WAIT>();                                                                                             \
-            hs = wrap(hs + NQ);                                                                                                \
-            const uint32_t na = wrap(hs + wn) * kSlot, nb = wrap(hs + 2 + (TB == 4 ? wm : 0)) * kSlot;                         \
-            xe1 = l8_lds_read4(ks + (uint32_t)((s + 1) & 3) * kScaleSlot);                                                     \
-            l8_kstep<TB, true, LOAD ? kLoads - kEarly : 0, kEarly / 4>(acc, f1, f0, ka[0] + na, ka[1] + na, kb[0] + nb, kb[1] + nb, wec, xe, src, ns, sc); \
-            if (LOAD) advance();                                                                                               \
-            xe0 = xe1;                                                                                                         \
-            ++s;                                                                                                               \
-        } else {                                                                                                               \
-            l8_kstep<TB, false, 0, 0>(acc, f1, f0, 0, 0, 0, 0, wec, xe, src, 0, 0);                                            \
-        }                                                                                                                      \
-    }
-    if constexpr (TB == 4) {
-        while (s + 2 < nstage) L8_ITER(true, 4, false)
-    } else {
-        while (s + 3 < nstage) L8_ITER(true, kLoads, false)
-        if (nstage >= 3) L8_ITER(false, kLoads, false)
-    }
-    if (nstage >= 2) L8_ITER(false, 0, false)
-    L8_ITER(false, 0, true)
-#undef L8_ITER
-
-    // lane (m, hf) of block (cb, tb) holds row 32 tb + m, channels 8 g + 4 hf + (i & 3), i = 4 g + ..
-    const int64_t row0 = m0 + wm * 32 * TB + m;
-    if (p.vec && n0 + wn * 128 + 128 <= p.N) {                 // whole: 16-byte stores, a block column's operands loaded together
-#pragma unroll
-        for (int cb = 0; cb < 4; ++cb) {
-            const int cbase = n0 + wn * 128 + 32 * cb;
+        for (int cb = 0; cb < CB; ++cb) {
+            const int cbase = c0 + 32 * cb;
             float bia[16];
+            if (p.bias != nullptr) {
+                const auto* bp = (const __attribute__((address_space(4))) uint32_t*)(size_t)(p.bias + cbase);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                u32x2 b = {0u, 0u};
-                if (p.bias != nullptr) b = *(const u32x2*)(p.bias + cbase + 8 * g + 4 * hf);
-                l8_unpack4<E>(b, bia + 4 * g);
+                for (int g = 0; g < 4; ++g) {
+                    const u32x2 b = {hf ? bp[4 * g + 2] : bp[4 * g], hf ? bp[4 * g + 3] : bp[4 * g + 1]};
+                    l8_unpack4<E>(b, bia + 4 * g);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) bia[i] = 0.f;
             }
 #pragma unroll
             for (int tb = 0; tb < TB; ++tb) {
-                const int64_t row = row0 + 32 * tb, rc = min(row, p.M - 1);
+                int own = 32 * tb + m;
+                asm volatile("" : "+v"(own));
+                const int64_t row = r0 + own;
                 float res[16], gate[16];
                 if (EPI == SFM_EPI_GATE_RESIDUAL) {
-                    const uint16_t *rp = p.res + rc * p.res_stride + cbase + 4 * hf;
-                    const uint16_t *gp = p.gate != nullptr ? p.gate + (rc / p.rows_per_frame) * p.gate_stride + cbase + 4 * hf : nullptr;
+                    const uint16_t* rp = p.res + row * p.res_stride + cbase + 4 * hf;
+                    const uint16_t* gp = p.gate != nullptr ? p.gate + (row / p.rows_per_frame) * p.gate_stride + cbase + 4 * hf : nullptr;
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
                         l8_unpack4<E>(*(const u32x2*)(rp + 8 * g), res + 4 * g);
@@ -448,20 +321,157 @@ __global__ __launch_bounds__(256) void l8_tile_kernel(L8Args p) {
                     auto rx = __builtin_amdgcn_permlane32_swap(w[4 * gp], w[4 * gp + 2], false, false);
                     auto ry = __builtin_amdgcn_permlane32_swap(w[4 * gp + 1], w[4 * gp + 3], false, false);
                     u32x4 o = {(uint32_t)rx[0], (uint32_t)ry[0], (uint32_t)rx[1], (uint32_t)ry[1]};
-                    if (row < p.M) *(u32x4*)(p.out + row * p.out_stride + cbase + 16 * gp + 8 * hf) = o;
+                    *(u32x4*)(p.out + row * p.out_stride + cbase + 16 * gp + 8 * hf) = o;
                 }
             }
         }
-    } else {
+        return;
+    }
 #pragma unroll
-        for (int cb = 0; cb < 4; ++cb)
+    for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
-            for (int tb = 0; tb < TB; ++tb)
+        for (int tb = 0; tb < TB; ++tb) {
+            int own = 32 * tb + m;
+            asm volatile("" : "+v"(own));
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const float a4[4] = {acc[cb][tb][4 * g], acc[cb][tb][4 * g + 1], acc[cb][tb][4 * g + 2], acc[cb][tb][4 * g + 3]};
-                    l8_finish4<E, EPI>(p, row0 + 32 * tb, n0 + wn * 128 + 32 * cb + 8 * g + 4 * hf, a4);
-                }
+            for (int g = 0; g < 4; ++g) {
+                const float a4[4] = {acc[cb][tb][4 * g], acc[cb][tb][4 * g + 1], acc[cb][tb][4 * g + 2], acc[cb][tb][4 * g + 3]};
+                l8_finish4<E, EPI>(p, r0 + own, c0 + 32 * cb + 8 * g + 4 * hf, a4);
+            }
+        }
+}
+
+// One tile: strip rows m0 .., channels n0 ..
+template <class E, int EPI, int TB>
+__device__ __forceinline__ void l8_tile(const L8Args& p, int64_t m0, int n0) {
+    constexpr int kTileM = 64 * TB;
+    constexpr int NQ = 2 + TB / 2, kLoads = 4 * NQ + 1;        // slots and a wave's requests of a stage
+    constexpr int kAhead = TB == 4 ? 2 : 3;                    // stage s + kAhead is requested while stage s is multiplied ..
+    constexpr int kEarly = TB == 4 ? 4 : 0;                    // .. so many of its requests before stage s has been read
+    constexpr int kOut = kEarly + (kAhead - 2) * kLoads;       // requests of later stages under way when stage s + 1 is needed
+    extern __shared__ __attribute__((aligned(256))) uint8_t l8_lds[];
+    const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) uint8_t*)l8_lds;
+    const int tid = threadIdx.x, lane = tid & 63, m = lane & 31, hf = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wn = wave & 1, wm = wave >> 1;
+
+    // request j of a wave fills rows 8 (4 j + wave) .. + 7 of a slot; rows past the end repeat the last
+    L8Src<TB> src;
+    src.w = p.w + (int64_t)n0 * p.kp;
+    src.x = p.x + m0 * p.kp;
+    src.s = p.xscale + m0;                                     // 128 bytes of scales per 128 rows
+    src.lds = lds0 + (uint32_t)wave * 1024;
+    {
+        const int g_row = lane >> 3, g_c = (lane & 7) ^ ((((wave & 1) << 2) + (lane >> 4)) & 7);
+        const int wlast = p.N - 1 - n0, xlast = (int)min(p.M - 1 - m0, (int64_t)kTileM - 1);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) src.w_off[j] = (uint32_t)min((4 * j + wave) * 8 + g_row, wlast) * (uint32_t)p.kp + g_c * 16;
+#pragma unroll
+        for (int j = 0; j < 2 * TB; ++j) src.x_off[j] = (uint32_t)min((4 * j + wave) * 8 + g_row, xlast) * (uint32_t)p.kp + g_c * 16;
+        src.s_off = (uint32_t)(lane * 4 - (m0 + 128 < p.M ? 0 : 128 * hf));
+    }
+    const int64_t s_step = p.groups * 128;
+    auto advance = [&]() {
+        src.w += kBlock8;
+        src.x += kBlock8;
+        src.s += s_step;
+    };
+    const auto* wsp = (const __attribute__((address_space(4))) uint32_t*)(size_t)(p.wscale + (int64_t)min((n0 >> 7) + wn, (p.N - 1) >> 7) * p.pitch);
+
+    f32x16 acc[4][TB];
+#pragma unroll
+    for (int cb = 0; cb < 4; ++cb)
+#pragma unroll
+        for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[cb][tb][i] = 0.f;
+
+    // operand read addresses of the pieces of a row, relative to a slot; the wave's weight and activation rows in a stage
+    const int sw = (m >> 1) & 7;
+    uint32_t kp4[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) kp4[q] = lds0 + (uint32_t)(m * 128) + (uint32_t)(((2 * q + hf) ^ sw) << 4);
+    const uint32_t bq = TB == 4 ? 2 + wm : 2, bo = TB == 4 ? 0 : wm * 8192;
+    const uint32_t ks = lds0 + kScaleAt + (uint32_t)(((TB == 4 ? wm : 0) * 32 + m) * 4);
+    const int xsh = TB == 4 ? 0 : 16 * wm;
+
+    // Quarter q of stage s lives in slot (NQ s + q) % 9.  Iteration s multiplies stage s in two k steps; the operands of a step are
+    // read during the step before.  After its first step a wave has read all of stage s: it waits for its own loads of stage
+    // s + 1, meets the others, and requests stage s + kAhead into the slots that are free (TB = 4: its first quarter has a slot
+    // already before that).
+    const int nstage = p.nkb;
+    auto whole_stage = [&](int g) {
+        const uint32_t slot = (uint32_t)(NQ * g) % kRing, sc = lds0 + kScaleAt + g * kScaleSlot;
+#define L8_RQ(J) if constexpr ((J) < kLoads) l8_request<TB, 0, (J) < kLoads ? (J) : 0>(src, slot, sc);
+        L8_RQ(0) L8_RQ(1) L8_RQ(2) L8_RQ(3) L8_RQ(4) L8_RQ(5) L8_RQ(6) L8_RQ(7) L8_RQ(8) L8_RQ(9) L8_RQ(10) L8_RQ(11) L8_RQ(12)
+        L8_RQ(13) L8_RQ(14) L8_RQ(15) L8_RQ(16)
+#undef L8_RQ
+        advance();
+    };
+    whole_stage(0);
+    if (nstage > 1) whole_stage(1);
+    if (kAhead == 3 && nstage > 2) whole_stage(2);
+    if (kAhead == 3 && nstage > 2) l8_wait_stage<2 * kLoads>();
+    else if (nstage > 1) l8_wait_stage<kLoads>();
+    else l8_wait_stage<0>();
+    u32x4 f0[8 + 2 * TB], f1[8 + 2 * TB];
+    uint32_t hs = 0;                                           // slot of the first quarter of the stage being multiplied
+    uint32_t xe0 = l8_lds_read4(ks), xe1;
+    {
+        const uint32_t a = wn * kSlot, b = bq * kSlot + bo;
+        l8_fetch_all<TB>(std::make_integer_sequence<int, 8 + 2 * TB>{}, f0, kp4[0] + a, kp4[1] + a, kp4[0] + b, kp4[1] + b);
+    }
+    int s = 0;
+    uint32_t wword = wsp[0];                                   // the word with the weight scale of the stage
+    // LOAD: request stage s + kAhead; WAIT: requests that may be under way at the barrier; LAST: nothing follows
+#define L8_ITER(LOAD, WAIT, LAST)                                                                                              \
+    {                                                                                                                          \
+        const uint32_t sa = l8_wrap(hs + wn) * kSlot, sb = l8_wrap(hs + bq) * kSlot + bo;                                      \
+        const uint32_t ns = l8_wrap(hs + (NQ * kAhead) % kRing);                                                               \
+        const uint32_t sc = lds0 + kScaleAt + (uint32_t)((s + kAhead) & 3) * kScaleSlot;                                       \
+        l8_wait_frags(f0, xe0);                                                                                                \
+        const int wec = (int)(wword >> (8 * (s & 3))) & 0xff, xe = (int)(xe0 >> xsh);                                          \
+        if (!LAST) wword = wsp[(s + 1) >> 2];                                                                                  \
+        l8_kstep<TB, true, LOAD ? kEarly : 0, 0>(std::make_integer_sequence<int, 4 * TB>{}, acc, f0, f1, kp4[2] + sa, kp4[3] + sa, \
+                                                           kp4[2] + sb, kp4[3] + sb, wec, xe, src, ns, sc);                    \
+        l8_wait_frags(f1, xe0);                                /* this wave has read all of the stage */                       \
+        if (!LAST) {                                                                                                           \
+            l8_wait_stage<WAIT>();                                                                                             \
+            hs = l8_wrap(hs + NQ);                                                                                             \
+            const uint32_t na = l8_wrap(hs + wn) * kSlot, nb = l8_wrap(hs + bq) * kSlot + bo;                                  \
+            xe1 = l8_lds_read4(ks + (uint32_t)((s + 1) & 3) * kScaleSlot);                                                     \
+            l8_kstep<TB, true, LOAD ? kLoads - kEarly : 0, kEarly / 4>(std::make_integer_sequence<int, 4 * TB>{}, acc, f1, f0, \
+                                                                                 kp4[0] + na, kp4[1] + na, kp4[0] + nb, kp4[1] + nb, wec, xe, src, ns, sc); \
+            if (LOAD) advance();                                                                                               \
+            xe0 = xe1;                                                                                                         \
+            ++s;                                                                                                               \
+        } else {                                                                                                               \
+            l8_kstep<TB, false, 0, 0>(std::make_integer_sequence<int, 4 * TB>{}, acc, f1, f0, 0, 0, 0, 0, wec, xe, src, 0, 0); \
+        }                                                                                                                      \
+    }
+    while (s + kAhead < nstage) L8_ITER(true, kOut, false)
+    if (kAhead == 3 && nstage >= 3) L8_ITER(false, kLoads, false)
+    if (nstage >= 2) L8_ITER(false, 0, false)
+    L8_ITER(false, 0, true)
+#undef L8_ITER
+    l8_store<E, EPI, TB, 4>(p, acc, n0 + wn * 128, m0 + wm * 32 * TB, m, hf);
+}
+
+// Every eighth workgroup shares an XCD: each XCD gets a contiguous run of the patch order.  With TB = 4 a last strip of at most 128
+// rows is made of half tiles, which come last and fill the last round of the compute units.
+template <class E, int EPI, int TB>
+__global__ __launch_bounds__(256) void l8_tile_kernel(L8Args p) {
+    const int strips = p.tm - p.half, all = strips * p.tn, per_xcd = (all + 7) / 8, blk = (int)blockIdx.x;
+    if (blk < 8 * per_xcd) {
+        const int v = (blk & 7) * per_xcd + (blk >> 3);
+        if (v >= all) return;
+        const int patch = v / (kGroupM * p.tn), first = patch * kGroupM, gsize = min(kGroupM, strips - first);
+        const int within = v - patch * kGroupM * p.tn;
+        const int tn = __builtin_amdgcn_readfirstlane(within / gsize);
+        l8_tile<E, EPI, TB>(p, (int64_t)__builtin_amdgcn_readfirstlane(first + within - tn * gsize) * (64 * TB), tn * kTileN);
+    } else if (TB == 4) {
+        const int per = (p.tn + 7) / 8, h = blk - 8 * per_xcd, v = (h & 7) * per + (h >> 3);
+        if (v < p.tn) l8_tile<E, EPI, 2>(p, (int64_t)strips * 256, v * kTileN);
     }
 }
 
@@ -479,7 +489,9 @@ int launch_tile(const L8Args& a0, hipStream_t st) {
     L8Args a = a0;
     a.tm = (int)((a.M + 64 * TB - 1) / (64 * TB));
     a.tn = (a.N + kTileN - 1) / kTileN;
-    hipLaunchKernelGGL((l8_tile_kernel<E, EPI, TB>), dim3((unsigned)((a.tm * a.tn + 7) / 8 * 8)), dim3(256), kLdsBytes, st, a);
+    a.half = TB == 4 && a.M % 256 != 0 && a.M % 256 <= 128;
+    const int64_t full = ((int64_t)(a.tm - a.half) * a.tn + 7) / 8 * 8, halves = a.half ? (a.tn + 7) / 8 * 8 : 0;
+    hipLaunchKernelGGL((l8_tile_kernel<E, EPI, TB>), dim3((unsigned)(full + halves)), dim3(256), kLdsBytes, st, a);
     return launched8("sfm_linear8");
 }
 
