@@ -36,7 +36,6 @@ struct L8Args {
     int rows_per_frame;
     int tm, tn;              // tiles along M and N
     int half;                // 1: the last strip of tiles has half the rows
-    bool vec;                // rows of out, res, gate and bias allow 8-byte accesses
 };
 
 template <class E>
@@ -54,11 +53,11 @@ __device__ __forceinline__ float l8_tail(float sum, float bias, float res, float
 template <class E, int EPI>
 __device__ __forceinline__ void l8_finish4(const L8Args& p, int64_t row, int c, const float* acc) {
     if (row >= p.M || c >= p.N) return;
-    const bool full = p.vec && c + 4 <= p.N;
+    const bool full = c + 4 <= p.N;
     float v[4], r[4] = {0.f, 0.f, 0.f, 0.f}, g[4] = {1.f, 1.f, 1.f, 1.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
     auto get4 = [&](const uint16_t* s, float* d) {
         if (full) {
-            l8_unpack4<E>(*(const u32x2*)s, d);
+            l8_unpack4<E>(*(const u32x2_any*)s, d);
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -75,7 +74,7 @@ __device__ __forceinline__ void l8_finish4(const L8Args& p, int64_t row, int c, 
     uint16_t* o = p.out + row * p.out_stride + c;
     if (full) {
         u32x2 w = {pack2<E>(v[0], v[1]), pack2<E>(v[2], v[3])};
-        *(u32x2*)o = w;
+        *(u32x2_any*)o = w;
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -275,21 +274,16 @@ __device__ __forceinline__ void l8_kstep(std::integer_sequence<int, I...>, f32x1
 // blocks together they would not fit beside the sums.
 template <class E, int EPI, int TB, int CB>
 __device__ __forceinline__ void l8_store(const L8Args& p, const f32x16 (&acc)[4][TB], int c0, int64_t r0, int m, int hf) {
-    if (p.vec && c0 + 32 * CB <= p.N && r0 + 32 * TB <= p.M) { // whole: 16-byte stores
+    if (c0 + 32 * CB <= p.N && r0 + 32 * TB <= p.M) {          // whole: 16-byte stores
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
             const int cbase = c0 + 32 * cb;
             float bia[16];
-            if (p.bias != nullptr) {
-                const auto* bp = (const __attribute__((address_space(4))) uint32_t*)(size_t)(p.bias + cbase);
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const u32x2 b = {hf ? bp[4 * g + 2] : bp[4 * g], hf ? bp[4 * g + 3] : bp[4 * g + 1]};
-                    l8_unpack4<E>(b, bia + 4 * g);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) bia[i] = 0.f;
+            for (int g = 0; g < 4; ++g) {
+                u32x2 b = {0u, 0u};
+                if (p.bias != nullptr) b = *(const u32x2_any*)(p.bias + cbase + 8 * g + 4 * hf);
+                l8_unpack4<E>(b, bia + 4 * g);
             }
 #pragma unroll
             for (int tb = 0; tb < TB; ++tb) {
@@ -302,9 +296,9 @@ __device__ __forceinline__ void l8_store(const L8Args& p, const f32x16 (&acc)[4]
                     const uint16_t* gp = p.gate != nullptr ? p.gate + (row / p.rows_per_frame) * p.gate_stride + cbase + 4 * hf : nullptr;
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
-                        l8_unpack4<E>(*(const u32x2*)(rp + 8 * g), res + 4 * g);
+                        l8_unpack4<E>(*(const u32x2_any*)(rp + 8 * g), res + 4 * g);
                         if (gp != nullptr) {
-                            l8_unpack4<E>(*(const u32x2*)(gp + 8 * g), gate + 4 * g);
+                            l8_unpack4<E>(*(const u32x2_any*)(gp + 8 * g), gate + 4 * g);
                         } else {
 #pragma unroll
                             for (int i = 0; i < 4; ++i) gate[4 * g + i] = 1.f;
@@ -321,7 +315,7 @@ __device__ __forceinline__ void l8_store(const L8Args& p, const f32x16 (&acc)[4]
                     auto rx = __builtin_amdgcn_permlane32_swap(w[4 * gp], w[4 * gp + 2], false, false);
                     auto ry = __builtin_amdgcn_permlane32_swap(w[4 * gp + 1], w[4 * gp + 3], false, false);
                     u32x4 o = {(uint32_t)rx[0], (uint32_t)ry[0], (uint32_t)rx[1], (uint32_t)ry[1]};
-                    *(u32x4*)(p.out + row * p.out_stride + cbase + 16 * gp + 8 * hf) = o;
+                    *(u32x4_any*)(p.out + row * p.out_stride + cbase + 16 * gp + 8 * hf) = o;
                 }
             }
         }
@@ -495,12 +489,20 @@ int launch_tile(const L8Args& a0, hipStream_t st) {
     return launched8("sfm_linear8");
 }
 
+// Which kernel.  Times of a round of tiles over the compute units, fitted to measurements from 12 to 70 stages (us): 256 rows 8 + 1.2
+// a stage, 128 rows 7 + 0.9.  Measured on both sides: 4680 x 8960 -> 1536 (114 or 222 tiles, one round) 87 against 67; 4680 x 1536 ->
+// 8960 (665 or 1295) 82 against 99; 1560 x 1536 -> 8960 (245 or 455) 27 against 35.  The kernel without LDS runs at up to 0.5
+// PFLOP/s behind 6 us, and wins where the tiles are few: 512 x 1536 -> 1536 13 against 15, 1111 x 1000 -> 777 12 against 32.
 template <class E, int EPI>
 int launch_epi(const L8Args& a, hipStream_t st) {
     if (a.M <= 16) return launch_direct<E, EPI, 1, 1, 8>(a, st);
-    if (a.M >= 1024 && a.N >= 256) return launch_tile<E, EPI, 4>(a, st);
-    if (a.M >= 256 && a.N >= 256) return launch_tile<E, EPI, 2>(a, st);
-    return launch_direct<E, EPI, 4, 4, 4>(a, st);
+    const double cus = cu_count(), tn = (a.N + kTileN - 1) / kTileN;
+    auto rounds = [&](double tiles) { return tiles < cus ? 1.0 : tiles / cus + 0.3; };
+    const double t4 = rounds(tn * (double)((a.M + 255) / 256)) * (8.0 + 1.2 * a.nkb);
+    const double t2 = rounds(tn * (double)((a.M + 127) / 128)) * (7.0 + 0.9 * a.nkb);
+    const double flops = 2.0 * a.M * a.N * a.kp, direct = 6.0 + 0.35 * a.nkb + flops / 0.5e9;
+    if (direct < t2 && direct < t4) return launch_direct<E, EPI, 4, 2, 8>(a, st);
+    return t2 < t4 ? launch_tile<E, EPI, 2>(a, st) : launch_tile<E, EPI, 4>(a, st);
 }
 
 template <class E>
@@ -533,8 +535,6 @@ int launch_linear8(const sfm_linear8_desc& d, const void* x8, const void* xscale
     a.res_stride = d.res_stride;
     a.gate_stride = d.gate_stride;
     a.rows_per_frame = d.rows_per_frame > 0 ? d.rows_per_frame : 1;
-    auto ok = [](const void* q, int64_t stride) { return q == nullptr || (((uintptr_t)q & 15) == 0 && stride % 8 == 0); };
-    a.vec = ok(out, d.out_stride) && ok(res, d.res_stride) && ok(gate, d.gate_stride) && ok(bias, 0);
     return d.dtype == SFM_BF16 ? launch_dtype<BF16>(a, d.epilogue, stream) : launch_dtype<F16>(a, d.epilogue, stream);
 }
 

@@ -15,8 +15,8 @@ namespace {
 //   GELU: y = gelu_tanh(x) is stored besides.   data NULL: nothing is quantised (only the sums are wanted).
 //   colsum: float [row groups][K], the sums over the group's rows (a bias gradient's first half).
 template <typename T, bool GELU>
-__global__ __launch_bounds__(256) void quantize8_kernel(const void* x, int64_t xs, int64_t rows, int K, bool xvec, uint8_t* data,
-                                                        uint8_t* scale, void* y, int64_t ys, bool yvec, float* colsum) {
+__global__ __launch_bounds__(256) void quantize8_kernel(const void* x, int64_t xs, int64_t rows, int K, uint8_t* data,
+                                                        uint8_t* scale, void* y, int64_t ys, float* colsum) {
     __shared__ uint8_t sc[kBlock8];
     __shared__ float cs[16][kBlock8];
     const int64_t groups = gridDim.x;
@@ -28,7 +28,7 @@ __global__ __launch_bounds__(256) void quantize8_kernel(const void* x, int64_t x
     for (int i = 0; i < 8; ++i) {
         const int64_t r = row0 + r0 + 16 * i;
         if (r < rows) {
-            load_part8<T>(x, r * xs, c, K, xvec, v[i]);
+            load_part8<T>(x, r * xs, c, K, v[i]);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
@@ -68,7 +68,7 @@ __global__ __launch_bounds__(256) void quantize8_kernel(const void* x, int64_t x
             if (r < rows) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[i][e] *= gelu_gate<kWide<T>>(v[i][e]);
-                store_part8<T>(y, r * ys, c, K, yvec, v[i]);
+                store_part8<T>(y, r * ys, c, K, v[i]);
             }
         }
     }
@@ -96,7 +96,7 @@ __device__ __forceinline__ void values8(const uint8_t* data, const uint8_t* scal
 // in fp16 a value past its range (65536 for a 65504 that was rounded up) becomes the largest one
 template <typename T>
 __global__ __launch_bounds__(256) void dequantize8_kernel(const uint8_t* data, const uint8_t* scale, int64_t rows, int K, void* y,
-                                                          int64_t ys, bool vec) {
+                                                          int64_t ys) {
     const int64_t kp = pad8(K), groups = (rows + kBlock8 - 1) / kBlock8;
     const int chunks = (K + 7) / 8;
     const int64_t n = rows * chunks;
@@ -109,15 +109,15 @@ __global__ __launch_bounds__(256) void dequantize8_kernel(const uint8_t* data, c
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = v[e] != v[e] ? v[e] : fminf(fmaxf(v[e], -65504.f), 65504.f);
         }
-        store_part8<T>(y, r * ys, c, K, vec, v);
+        store_part8<T>(y, r * ys, c, K, v);
     }
 }
 
 // dx = dy gelu'(x), x from its 8-bit blocks (KEPT) or as it was
 template <typename T, bool KEPT>
-__global__ __launch_bounds__(256) void gelu_bwd_kernel(const void* x, int64_t xs, bool xvec, const uint8_t* data, const uint8_t* scale,
-                                                       int64_t rows, int K, const void* dy, int64_t dys, bool dyvec, void* dx,
-                                                       int64_t dxs, bool dxvec) {
+__global__ __launch_bounds__(256) void gelu_bwd_kernel(const void* x, int64_t xs, const uint8_t* data, const uint8_t* scale,
+                                                       int64_t rows, int K, const void* dy, int64_t dys, void* dx,
+                                                       int64_t dxs) {
     const int64_t kp = pad8(K), groups = (rows + kBlock8 - 1) / kBlock8;
     const int chunks = (K + 7) / 8;
     const int64_t n = rows * chunks;
@@ -126,18 +126,18 @@ __global__ __launch_bounds__(256) void gelu_bwd_kernel(const void* x, int64_t xs
         const int c = (int)(i - r * chunks) * 8;
         float v[8], g[8];
         if (KEPT) values8(data, scale, r, kp, groups, c, v);
-        else load_part8<T>(x, r * xs, c, K, xvec, v);
-        load_part8<T>(dy, r * dys, c, K, dyvec, g);
+        else load_part8<T>(x, r * xs, c, K, v);
+        load_part8<T>(dy, r * dys, c, K, g);
 #pragma unroll
         for (int e = 0; e < 8; ++e) g[e] *= gelu_slope<kWide<T>>(v[e]);
-        store_part8<T>(dx, r * dxs, c, K, dxvec, g);
+        store_part8<T>(dx, r * dxs, c, K, g);
     }
 }
 
 // One workgroup: a 128 x 128 block of a weight [N, K], one scale.  The block goes out twice, as it lies and transposed (through
 // LDS, a thread turning 4 x 4 bytes at a time), so that the product with the gradient of the output reads it along N.
 template <typename T>
-__global__ __launch_bounds__(256) void pack8_kernel(const void* w, int64_t ws, int N, int K, bool vec, uint8_t* data, uint8_t* scale,
+__global__ __launch_bounds__(256) void pack8_kernel(const void* w, int64_t ws, int N, int K, uint8_t* data, uint8_t* scale,
                                                     uint8_t* data_t, uint8_t* scale_t, int pitch, int pitch_t) {
     __shared__ float top[4];
     __shared__ __attribute__((aligned(16))) uint8_t tile[kBlock8][kBlock8 + 4];
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(256) void pack8_kernel(const void* w, int64_t ws, i
     for (int i = 0; i < 8; ++i) {
         const int64_t r = (int64_t)nb * kBlock8 + r0 + 16 * i;
         if (r < N) {
-            load_part8<T>(w, r * ws, c, K, vec, v[i]);
+            load_part8<T>(w, r * ws, c, K, v[i]);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
@@ -198,20 +198,14 @@ __global__ __launch_bounds__(256) void pack8_kernel(const void* w, int64_t ws, i
 }
 
 template <typename T>
-bool rows_vec(const void* p, int64_t stride) {
-    const int e = kWide<T> ? 4 : 2;
-    return ((uintptr_t)p & 15) == 0 && (stride * e) % 16 == 0;
-}
-
-template <typename T>
 int quantize_t(int64_t rows, int K, const void* x, int64_t xs, void* data, void* scale, void* y, int64_t ys, float* colsum, hipStream_t st) {
     const dim3 grid((unsigned)((rows + kBlock8 - 1) / kBlock8), (unsigned)blocks8(K));
     if (y != nullptr)
-        hipLaunchKernelGGL((quantize8_kernel<T, true>), grid, dim3(256), 0, st, x, xs, rows, K, rows_vec<T>(x, xs), (uint8_t*)data,
-                           (uint8_t*)scale, y, ys, rows_vec<T>(y, ys), colsum);
+        hipLaunchKernelGGL((quantize8_kernel<T, true>), grid, dim3(256), 0, st, x, xs, rows, K, (uint8_t*)data,
+                           (uint8_t*)scale, y, ys, colsum);
     else
-        hipLaunchKernelGGL((quantize8_kernel<T, false>), grid, dim3(256), 0, st, x, xs, rows, K, rows_vec<T>(x, xs), (uint8_t*)data,
-                           (uint8_t*)scale, nullptr, 0, false, colsum);
+        hipLaunchKernelGGL((quantize8_kernel<T, false>), grid, dim3(256), 0, st, x, xs, rows, K, (uint8_t*)data,
+                           (uint8_t*)scale, nullptr, 0, colsum);
     return launched8("sfm_quantize8");
 }
 
@@ -219,7 +213,7 @@ template <typename T>
 int dequantize_t(int64_t rows, int K, const void* data, const void* scale, void* y, int64_t ys, hipStream_t st) {
     const int64_t wgs = (rows * ((K + 7) / 8) + 255) / 256, cap = (int64_t)cu_count() * 16;
     hipLaunchKernelGGL((dequantize8_kernel<T>), dim3((unsigned)(wgs < cap ? wgs : cap)), dim3(256), 0, st, (const uint8_t*)data, (const uint8_t*)scale, rows, K,
-                       y, ys, rows_vec<T>(y, ys));
+                       y, ys);
     return launched8("sfm_dequantize8");
 }
 
@@ -229,17 +223,16 @@ int gelu_bwd_t(int64_t rows, int K, const void* x, int64_t xs, const void* data,
     const int64_t wgs = (rows * ((K + 7) / 8) + 255) / 256, cap = (int64_t)cu_count() * 16;
     const dim3 grid((unsigned)(wgs < cap ? wgs : cap));
     if (data != nullptr)
-        hipLaunchKernelGGL((gelu_bwd_kernel<T, true>), grid, dim3(256), 0, st, nullptr, 0, false, (const uint8_t*)data, (const uint8_t*)scale,
-                           rows, K, dy, dys, rows_vec<T>(dy, dys), dx, dxs, rows_vec<T>(dx, dxs));
+        hipLaunchKernelGGL((gelu_bwd_kernel<T, true>), grid, dim3(256), 0, st, nullptr, 0, (const uint8_t*)data, (const uint8_t*)scale,
+                           rows, K, dy, dys, dx, dxs);
     else
-        hipLaunchKernelGGL((gelu_bwd_kernel<T, false>), grid, dim3(256), 0, st, x, xs, rows_vec<T>(x, xs), nullptr, nullptr, rows, K, dy, dys,
-                           rows_vec<T>(dy, dys), dx, dxs, rows_vec<T>(dx, dxs));
+        hipLaunchKernelGGL((gelu_bwd_kernel<T, false>), grid, dim3(256), 0, st, x, xs, nullptr, nullptr, rows, K, dy, dys, dx, dxs);
     return launched8("sfm_gelu_bwd");
 }
 
 template <typename T>
 int pack_t(int N, int K, const void* w, int64_t ws, void* data, void* scale, void* data_t, void* scale_t, hipStream_t st) {
-    hipLaunchKernelGGL((pack8_kernel<T>), dim3((unsigned)blocks8(K), (unsigned)blocks8(N)), dim3(256), 0, st, w, ws, N, K, rows_vec<T>(w, ws),
+    hipLaunchKernelGGL((pack8_kernel<T>), dim3((unsigned)blocks8(K), (unsigned)blocks8(N)), dim3(256), 0, st, w, ws, N, K,
                        (uint8_t*)data, (uint8_t*)scale, (uint8_t*)data_t, (uint8_t*)scale_t, pitch8(K), pitch8(N));
     return launched8("sfm_pack8");
 }

@@ -101,28 +101,54 @@ __device__ __forceinline__ void unpack_e4m3(uint32_t w, float* v) {
     v[0] = lo[0]; v[1] = lo[1]; v[2] = hi[0]; v[3] = hi[1];
 }
 
-// eight elements of a row of n that may end inside them or start off a 16-byte boundary; zeros past the end
+// Eight elements of a row of n that may end inside them, at any address that suits the elements (gfx950 takes wide accesses off
+// their own alignment); zeros past the end
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 template <typename T> struct Elem {
     static __device__ __forceinline__ float get(const void* p, int64_t e) { return T::to_float(((const uint16_t*)p)[e]); }
     static __device__ __forceinline__ void put(void* p, int64_t e, float v) { ((uint16_t*)p)[e] = T::from_float(v); }
+    static __device__ __forceinline__ void get8(const void* p, int64_t e, float* v) {
+        const u32x4 w = *(const u32x4_any*)((const uint16_t*)p + e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = T::to_float((uint16_t)(w[i] & 0xffffu));
+            v[2 * i + 1] = T::to_float((uint16_t)(w[i] >> 16));
+        }
+    }
+    static __device__ __forceinline__ void put8(void* p, int64_t e, const float* v) {
+        const u32x4 w = {pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7])};
+        *(u32x4_any*)((uint16_t*)p + e) = w;
+    }
 };
 template <> struct Elem<float> {
     static __device__ __forceinline__ float get(const void* p, int64_t e) { return ((const float*)p)[e]; }
     static __device__ __forceinline__ void put(void* p, int64_t e, float v) { ((float*)p)[e] = v; }
+    static __device__ __forceinline__ void get8(const void* p, int64_t e, float* v) {
+        const f32x4_any* s = (const f32x4_any*)((const float*)p + e);
+        const f32x4 a = s[0], b = s[1];
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+    static __device__ __forceinline__ void put8(void* p, int64_t e, const float* v) {
+        f32x4_any* d = (f32x4_any*)((float*)p + e);
+        d[0] = f32x4{v[0], v[1], v[2], v[3]};
+        d[1] = f32x4{v[4], v[5], v[6], v[7]};
+    }
 };
 template <typename T>
-__device__ __forceinline__ void load_part8(const void* p, int64_t row_off, int c, int n, bool vec, float* v) {
-    if (vec && c + 8 <= n) {
-        V8<T>::load(p, row_off + c, v);
+__device__ __forceinline__ void load_part8(const void* p, int64_t row_off, int c, int n, float* v) {
+    if (c + 8 <= n) {
+        Elem<T>::get8(p, row_off + c, v);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = c + i < n ? Elem<T>::get(p, row_off + c + i) : 0.f;
     }
 }
 template <typename T>
-__device__ __forceinline__ void store_part8(void* p, int64_t row_off, int c, int n, bool vec, const float* v) {
-    if (vec && c + 8 <= n) {
-        V8<T>::store(p, row_off + c, v);
+__device__ __forceinline__ void store_part8(void* p, int64_t row_off, int c, int n, const float* v) {
+    if (c + 8 <= n) {
+        Elem<T>::put8(p, row_off + c, v);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
