@@ -367,6 +367,13 @@ typedef struct sfm_linear8_desc {
 int sfm_linear8(const sfm_linear8_desc* desc, const void* x8, const void* xscale, const void* w8, const void* wscale, const void* bias,
                 const void* res, const void* gate, void* out, void* stream);
 
+/* sfm_quantize8 of the rows x (16-bit, x_stride apart) and sfm_linear8 in one call.  data, scale: where the blocks go, as sfm_quantize8
+ * writes them; NULL, both, is allowed for up to SFM_LINEAR8_FEW_ROWS rows, which are quantised inside the product's kernel (with data
+ * given the blocks are written all the same). */
+#define SFM_LINEAR8_FEW_ROWS 16
+int sfm_linear8_fwd(const sfm_linear8_desc* desc, const void* x, int64_t x_stride, void* data, void* scale, const void* w8,
+                    const void* wscale, const void* bias, const void* res, const void* gate, void* out, void* stream);
+
 /* Gradients of a linear layer's weight and bias: dw[n][k] = sum_m dy[m][n] x[m][k] from the rows that the forward kept in 8 bits
  * (dy as it is; [N, K] contiguous), dbias[n] = sum_m dy[m][n]; either may be NULL.  16-bit tensors, fp32 sums in a fixed order, one
  * rounding.  colsum: dy's column sums where sfm_quantize8 has formed them (NULL: formed here, in the workspace). */

@@ -6,7 +6,7 @@ import ctypes
 import torch
 
 from . import lib as _l
-from .monarch_attn import _DT, _stream
+from .monarch_attn import _DT, _on_device, _stream
 
 _HALF = (torch.float16, torch.bfloat16)
 
@@ -94,7 +94,7 @@ def _even(dy):
 def _ln(x, mod, eps):
     rows, C, xs = _rows(x)
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    with torch.cuda.device(x.device):
+    with _on_device(x.device):
         _l.check(_l.load().sfm_ln_modulate(_DT[x.dtype], rows, C, eps, x.data_ptr(), xs, y.data_ptr(), C, *mod, _stream(x)))
     return y
 
@@ -107,7 +107,7 @@ def _ln_keep8(x, mod, eps):
     data = torch.empty((rows, kp), dtype=torch.uint8, device=x.device)
     scale = torch.empty(-(-rows // 128) * kp, dtype=torch.uint8, device=x.device)
     rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
+    with _on_device(x.device):
         _l.check(_l.load().sfm_ln_keep8(_DT[x.dtype], rows, C, eps, x.data_ptr(), xs, y.data_ptr(), C, *mod, data.data_ptr(),
                                         scale.data_ptr(), rstd.data_ptr(), _stream(x)))
     return y, data, scale, rstd
@@ -124,12 +124,19 @@ def _ln_bwd(dy, x, kept, weight, scale, ms, group, eps, want_dx=True):
     _l.check(_l.load().sfm_ln_bwd_workspace_bytes(rows, C, group, ctypes.byref(n)))
     ws = torch.empty(n.value, dtype=torch.uint8, device=dy.device)
     data, sc8, rstd = (None, None, None) if kept is None else (t.data_ptr() for t in kept)
-    with torch.cuda.device(dy.device):
+    with _on_device(dy.device):
         _l.check(_l.load().sfm_ln_bwd(_DT[dy.dtype], rows, C, eps, None if x is None else x.data_ptr(), xs, data, sc8, rstd, dy.data_ptr(),
                                       _row_stride(dy), None if weight is None else weight.data_ptr(), None if scale is None else scale.data_ptr(),
                                       ms, group, None if dx is None else dx.data_ptr(), C, dw.data_ptr(), db.data_ptr(), ws.data_ptr(),
                                       n.value, _stream(dy)))
     return dx, dw, db
+
+
+def _once(backward):
+    """A backward without a derivative of its own: `once_differentiable`, but for calls that build no graph, which it would only
+    slow down (a third of a small call's time)."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+    return lambda ctx, *grads: (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
 
 
 class _LnFn(torch.autograd.Function):
@@ -154,7 +161,7 @@ class _LnFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy):
         modulate, eps, checkpoint8, ms, rpf, a_shape, b_shape = ctx.cfg
         sc, *rest = ctx.saved_tensors
@@ -211,7 +218,7 @@ def _gelu(x, keep8):
         kp = -(-C // 128) * 128
         data = torch.empty((rows, kp), dtype=torch.uint8, device=x.device)
         scale = torch.empty(-(-rows // 128) * kp, dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
+    with _on_device(x.device):
         _l.check(_l.load().sfm_quantize8(_DT[x.dtype], rows, C, x.data_ptr(), xs, data.data_ptr() if keep8 else None,
                                          scale.data_ptr() if keep8 else None, y.data_ptr(), C, None, _stream(x)))
     return y, data, scale
@@ -228,7 +235,7 @@ class _GeluFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy):
         dy = _even(dy)
         B, L, C = dy.shape
@@ -239,7 +246,7 @@ class _GeluFn(torch.autograd.Function):
             x, = ctx.saved_tensors
             xs, x = _row_stride(x), x.data_ptr()
         dx = torch.empty((B, L, C), dtype=dy.dtype, device=dy.device)
-        with torch.cuda.device(dy.device):
+        with _on_device(dy.device):
             _l.check(_l.load().sfm_gelu_bwd(_DT[dy.dtype], B * L, C, x, xs, data, scale, dy.data_ptr(), _row_stride(dy), dx.data_ptr(), C,
                                             _stream(dy)))
         return dx, None

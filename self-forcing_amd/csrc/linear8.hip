@@ -117,24 +117,41 @@ __global__ __launch_bounds__(64 * W) void l8_direct_kernel(L8Args p) {
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int kb = wave; kb < p.nkb; kb += W) {
-        i32x8 xf[MT], wf[NT];
+    struct Ops {
+        i32x8 x[MT], w[NT];
         int xe[MT], we[NT];
+    };
+    auto fetch = [&](Ops& o, int kb) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            wf[j] = l8_load32(wp[j] + (int64_t)kb * kBlock8);
-            we[j] = p.wscale[wsc[j] + kb];
+            o.w[j] = l8_load32(wp[j] + (int64_t)kb * kBlock8);
+            o.we[j] = p.wscale[wsc[j] + kb];
         }
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-            xf[i] = l8_load32(xp[i] + (int64_t)kb * kBlock8);
-            xe[i] = p.xscale[xsc[i] + (int64_t)kb * p.groups * kBlock8];
+            o.x[i] = l8_load32(xp[i] + (int64_t)kb * kBlock8);
+            o.xe[i] = p.xscale[xsc[i] + (int64_t)kb * p.groups * kBlock8];
         }
+    };
+    auto multiply = [&](const Ops& o) {
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int j = 0; j < NT; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[j], xf[i], acc[i][j], 0, 0, 0, we[j], 0, xe[i]);
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(o.w[j], o.x[i], acc[i][j], 0, 0, 0, o.we[j], 0, o.xe[i]);
+    };
+    // the next block column is on its way while one is multiplied (past the last, that one again)
+    Ops a, b;
+    const int last = p.nkb - 1;
+    if (wave <= last) {
+        fetch(a, wave);
+        for (int kb = wave; kb <= last; kb += 2 * W) {
+            fetch(b, min(kb + W, last));
+            multiply(a);
+            if (kb + W > last) break;
+            fetch(a, min(kb + 2 * W, last));
+            multiply(b);
+        }
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -149,6 +166,90 @@ __global__ __launch_bounds__(64 * W) void l8_direct_kernel(L8Args p) {
         const float v[4] = {s.x, s.y, s.z, s.w};
         l8_finish4<E, EPI>(p, m0 + 16 * (t / NT) + l16, n0 + 16 * (t % NT) + 4 * q, v);
     }
+}
+
+// Up to 16 rows, quantised where they are used: lane (l16, q) forms the operand of its row's 32 values from the 16-bit rows, the four
+// lanes of a row agree on the block's scale.  The weights pass once, 16 channels a workgroup, the block columns over its W waves; one
+// launch, no rows in memory.
+template <class E, int EPI, int W>
+__global__ __launch_bounds__(64 * W) void l8_few_kernel(L8Args p, const uint16_t* x, int64_t xstride, int K) {
+    __shared__ f32x4 part[W][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, q = lane >> 4;
+    const int n0 = blockIdx.x * 16, n = min(n0 + l16, p.N - 1);
+    const uint8_t* wp = p.w + (int64_t)n * p.kp + q * 32;
+    const uint8_t* ws = p.wscale + (int64_t)(n >> 7) * p.pitch;
+    const bool live = l16 < p.M;
+    const int64_t row = live ? l16 * xstride : 0;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    struct Ops {
+        i32x8 w;
+        int we;
+        float v[4][8];
+    };
+    auto fetch = [&](Ops& o, int kb) {
+        o.w = l8_load32(wp + (int64_t)kb * kBlock8);
+        o.we = ws[kb];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            if (live) {
+                load_part8<E>(x, row, kb * kBlock8 + q * 32 + 8 * c, K, o.v[c]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o.v[c][e] = 0.f;
+            }
+        }
+    };
+    auto multiply = [&](const Ops& o) {
+        float a = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) a = fmaxf(a, finite_mag(o.v[c][e]));
+        a = fmaxf(a, __shfl_xor(a, 16));
+        const int s = block_exp8(fmaxf(a, __shfl_xor(a, 32)));
+        const float inv = two_to(-s);
+        i32x8 xf;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            xf[2 * c] = (int)pack_e4m3(o.v[c][0] * inv, o.v[c][1] * inv, o.v[c][2] * inv, o.v[c][3] * inv);
+            xf[2 * c + 1] = (int)pack_e4m3(o.v[c][4] * inv, o.v[c][5] * inv, o.v[c][6] * inv, o.v[c][7] * inv);
+        }
+        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(o.w, xf, acc, 0, 0, 0, o.we, 0, s + 127);
+    };
+    Ops a, b;
+    const int last = p.nkb - 1;
+    if (wave <= last) {
+        fetch(a, wave);
+        for (int kb = wave; kb <= last; kb += 2 * W) {
+            fetch(b, min(kb + W, last));
+            multiply(a);
+            if (kb + W > last) break;
+            fetch(a, min(kb + 2 * W, last));
+            multiply(b);
+        }
+    }
+    part[wave][lane] = acc;
+    __syncthreads();
+    if (wave == 0) {
+        f32x4 s = part[0][lane];
+#pragma unroll
+        for (int w = 1; w < W; ++w) s += part[w][lane];
+        const float v[4] = {s.x, s.y, s.z, s.w};
+        l8_finish4<E, EPI>(p, l16, n0 + 4 * q, v);
+    }
+}
+
+// 8 or 16 waves a workgroup for up to 16 rows: 16 where the channels make few workgroups and the rows are long enough to share out
+// (8960 -> 1536: 96 workgroups of 70 blocks)
+bool few_wide(const L8Args& a) { return (a.N + 15) / 16 < 2 * cu_count() && a.nkb >= 16; }
+template <class E, int EPI>
+int launch_few(const L8Args& a, const void* x, int64_t xstride, int K, hipStream_t st) {
+    const unsigned wgs = (unsigned)((a.N + 15) / 16);
+    if (few_wide(a))
+        hipLaunchKernelGGL((l8_few_kernel<E, EPI, 16>), dim3(wgs), dim3(1024), 0, st, a, (const uint16_t*)x, xstride, K);
+    else
+        hipLaunchKernelGGL((l8_few_kernel<E, EPI, 8>), dim3(wgs), dim3(512), 0, st, a, (const uint16_t*)x, xstride, K);
+    return launched8("sfm_linear8_fwd");
 }
 
 template <class E, int EPI, int MT, int NT, int W>
@@ -495,7 +596,7 @@ int launch_tile(const L8Args& a0, hipStream_t st) {
 // PFLOP/s behind 6 us, and wins where the tiles are few: 512 x 1536 -> 1536 13 against 15, 1111 x 1000 -> 777 12 against 32.
 template <class E, int EPI>
 int launch_epi(const L8Args& a, hipStream_t st) {
-    if (a.M <= 16) return launch_direct<E, EPI, 1, 1, 8>(a, st);
+    if (a.M <= 16) return few_wide(a) ? launch_direct<E, EPI, 1, 1, 16>(a, st) : launch_direct<E, EPI, 1, 1, 8>(a, st);
     const double cus = cu_count(), tn = (a.N + kTileN - 1) / kTileN;
     auto rounds = [&](double tiles) { return tiles < cus ? 1.0 : tiles / cus + 0.3; };
     const double t4 = rounds(tn * (double)((a.M + 255) / 256)) * (8.0 + 1.2 * a.nkb);
@@ -512,10 +613,17 @@ int launch_dtype(const L8Args& a, int epilogue, hipStream_t st) {
     return launch_epi<E, SFM_EPI_NONE>(a, st);
 }
 
+template <class E>
+int few_dtype(const L8Args& a, int epilogue, const void* x, int64_t xstride, int K, hipStream_t st) {
+    if (epilogue == SFM_EPI_GELU_TANH) return launch_few<E, SFM_EPI_GELU_TANH>(a, x, xstride, K, st);
+    if (epilogue == SFM_EPI_GATE_RESIDUAL) return launch_few<E, SFM_EPI_GATE_RESIDUAL>(a, x, xstride, K, st);
+    return launch_few<E, SFM_EPI_NONE>(a, x, xstride, K, st);
+}
+
 }  // namespace
 
-int launch_linear8(const sfm_linear8_desc& d, const void* x8, const void* xscale, const void* w8, const void* wscale, const void* bias,
-                   const void* res, const void* gate, void* out, hipStream_t stream) {
+int launch_linear8(const sfm_linear8_desc& d, const void* x, int64_t x_stride, const void* x8, const void* xscale, const void* w8,
+                   const void* wscale, const void* bias, const void* res, const void* gate, void* out, hipStream_t stream) {
     L8Args a;
     a.x = (const uint8_t*)x8;
     a.xscale = (const uint8_t*)xscale;
@@ -535,6 +643,8 @@ int launch_linear8(const sfm_linear8_desc& d, const void* x8, const void* xscale
     a.res_stride = d.res_stride;
     a.gate_stride = d.gate_stride;
     a.rows_per_frame = d.rows_per_frame > 0 ? d.rows_per_frame : 1;
+    if (x != nullptr && d.M <= kFewRows8)
+        return d.dtype == SFM_BF16 ? few_dtype<BF16>(a, d.epilogue, x, x_stride, d.K, stream) : few_dtype<F16>(a, d.epilogue, x, x_stride, d.K, stream);
     return d.dtype == SFM_BF16 ? launch_dtype<BF16>(a, d.epilogue, stream) : launch_dtype<F16>(a, d.epilogue, stream);
 }
 

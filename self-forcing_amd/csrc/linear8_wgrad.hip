@@ -386,8 +386,8 @@ __global__ __launch_bounds__(256) void wgrad8_big_kernel(WgradArgs p) {
     else wgrad8_tile<E, true>(p, n0, kb, s0, s1, split);
 }
 
-// Tiles and parts of the rows.  A round of large tiles takes 0.5 us a step of 32 rows, one of small tiles 0.6 a step of 64, and parts
-// cost what their fp32 sums take to write and read again.
+// Tiles and parts of the rows.  A round of large tiles takes 0.93 us a step of 32 rows, one of small tiles 1.05 a step of 64 (1.6 with
+// two on a compute unit), and parts cost what their fp32 sums take to write and read again.
 struct WgradPlan {
     bool big;
     int splits;
@@ -400,10 +400,10 @@ WgradPlan wgrad_plan(int64_t M, int N, int K) {
         const double tiles = big ? (double)((N + 255) / 256) * ((K + 255) / 256) : (double)blocks8(N) * blocks8(K);
         const int64_t steps = big ? (M + kBR - 1) / kBR : (M + kWR - 1) / kWR;
         for (int s = 1; s <= 16 && (s == 1 || steps >= 4 * s); ++s) {
-            const double wgs = tiles * s, per_cu = big ? 1.0 : 2.0;
+            const double wgs = tiles * s, per_cu = big || wgs <= cus ? 1.0 : 2.0;
             const double rounds = wgs <= cus * per_cu ? 1.0 : wgs / (cus * per_cu) + 0.4;
-            const double t = 6.0 + rounds * ((double)((steps + s - 1) / s) * (big ? 0.5 : 0.8) + (big ? 6.0 : 3.0)) +
-                             (s > 1 ? 4.0 + 8.0 * s * N * K / 4.0e6 : 0.0);
+            const double t = 4.0 + rounds * ((double)((steps + s - 1) / s) * (big ? 0.93 : per_cu > 1.0 ? 1.6 : 1.05) + (big ? 5.0 : 3.0)) +
+                             (s > 1 ? 3.0 + 8.0 * s * N * K / 4.5e6 : 0.0);
             if (t < least) {
                 least = t;
                 best = {big != 0, s};

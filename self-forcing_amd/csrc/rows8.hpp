@@ -194,9 +194,10 @@ int launch_dequantize8(int dtype, int64_t rows, int K, const void* data, const v
 int launch_gelu_bwd(int dtype, int64_t rows, int K, const void* x, int64_t xs, const void* data, const void* scale, const void* dy,
                     int64_t dys, void* dx, int64_t dxs, hipStream_t st);
 int launch_pack8(int dtype, int N, int K, const void* w, int64_t ws, void* data, void* scale, void* data_t, void* scale_t, hipStream_t st);
-// linear8.hip
-int launch_linear8(const sfm_linear8_desc& d, const void* x8, const void* xscale, const void* w8, const void* wscale, const void* bias,
-                   const void* res, const void* gate, void* out, hipStream_t stream);
+// linear8.hip; x: the 16-bit rows, or null.  Up to kFewRows8 of them are quantised in the product's own kernel, which reads no blocks
+constexpr int kFewRows8 = SFM_LINEAR8_FEW_ROWS;
+int launch_linear8(const sfm_linear8_desc& d, const void* x, int64_t x_stride, const void* x8, const void* xscale, const void* w8,
+                   const void* wscale, const void* bias, const void* res, const void* gate, void* out, hipStream_t stream);
 // linear8_wgrad.hip; `colsum`: column sums of dy by groups of 128 rows where a quantisation has formed them, else null
 size_t wgrad8_workspace_bytes(int64_t M, int N, int K, bool bias);
 int launch_wgrad8(int dtype, int64_t M, int N, int K, const void* dy, int64_t dy_stride, const void* x8, const void* xscale, void* dw,

@@ -1483,8 +1483,9 @@ int sfm_pack8(int32_t dtype, int32_t N, int32_t K, const void* w, int64_t w_stri
     return launch_pack8(dtype, N, K, w, w_stride, data, scale, data_t, scale_t, (hipStream_t)stream);
 }
 
-int sfm_linear8(const sfm_linear8_desc* d, const void* x8, const void* xscale, const void* w8, const void* wscale, const void* bias,
-                const void* res, const void* gate, void* out, void* stream) {
+// everything but the rows
+static int check_linear8(const sfm_linear8_desc* d, const void* w8, const void* wscale, const void* bias, const void* res, const void* gate,
+                         const void* out) {
     if (!d || !out) {
         set_error("desc and out must be non-NULL");
         return SFM_ERR_NULL;
@@ -1496,7 +1497,7 @@ int sfm_linear8(const sfm_linear8_desc* d, const void* x8, const void* xscale, c
         set_error("unknown epilogue %d", d->epilogue);
         return SFM_ERR_SHAPE;
     }
-    if ((rc = check_blocks("x8", x8, xscale)) || (rc = check_blocks("w8", w8, wscale))) return rc;
+    if ((rc = check_blocks("w8", w8, wscale))) return rc;
     const bool gr = d->epilogue == SFM_EPI_GATE_RESIDUAL;
     if (gr && !res) {
         set_error("the gated-residual epilogue needs res");
@@ -1508,12 +1509,42 @@ int sfm_linear8(const sfm_linear8_desc* d, const void* x8, const void* xscale, c
         set_error("rows_per_frame >= 1 and gate_stride >= 0 are needed");
         return SFM_ERR_STRIDE;
     }
-    const size_t ob = ((size_t)(d->M - 1) * d->out_stride + d->N) * 2;
-    if (overlap(out, ob, x8, (size_t)d->M * SFM_PAD8(d->K)) || overlap(out, ob, w8, (size_t)d->N * SFM_PAD8(d->K))) {
-        set_error("out overlaps x8 or w8");
-        return SFM_ERR_RANGE;
+    return SFM_OK;
+}
+static int check_out8(const sfm_linear8_desc* d, const void* out, const char* name, const void* p, size_t bytes) {
+    if (!overlap(out, ((size_t)(d->M - 1) * d->out_stride + d->N) * 2, p, bytes)) return SFM_OK;
+    set_error("out overlaps %s", name);
+    return SFM_ERR_RANGE;
+}
+
+int sfm_linear8(const sfm_linear8_desc* d, const void* x8, const void* xscale, const void* w8, const void* wscale, const void* bias,
+                const void* res, const void* gate, void* out, void* stream) {
+    int rc = check_linear8(d, w8, wscale, bias, res, gate, out);
+    if (rc || (rc = check_blocks("x8", x8, xscale))) return rc;
+    if ((rc = check_out8(d, out, "x8", x8, (size_t)d->M * SFM_PAD8(d->K))) || (rc = check_out8(d, out, "w8", w8, (size_t)d->N * SFM_PAD8(d->K)))) return rc;
+    const bool gr = d->epilogue == SFM_EPI_GATE_RESIDUAL;
+    return launch_linear8(*d, nullptr, 0, x8, xscale, w8, wscale, bias, gr ? res : nullptr, gr ? gate : nullptr, out, (hipStream_t)stream);
+}
+
+int sfm_linear8_fwd(const sfm_linear8_desc* d, const void* x, int64_t x_stride, void* data, void* scale, const void* w8,
+                    const void* wscale, const void* bias, const void* res, const void* gate, void* out, void* stream) {
+    int rc = check_linear8(d, w8, wscale, bias, res, gate, out);
+    if (rc) return rc;
+    if (!x) {
+        set_error("x must be non-NULL");
+        return SFM_ERR_NULL;
     }
-    return launch_linear8(*d, x8, xscale, w8, wscale, bias, gr ? res : nullptr, gr ? gate : nullptr, out, (hipStream_t)stream);
+    if ((rc = check_elem("x", x, x_stride, d->K, 2))) return rc;
+    const bool keep = data || scale;
+    if (keep || d->M > SFM_LINEAR8_FEW_ROWS) {
+        if ((rc = check_blocks("x8", data, scale))) return rc;
+        if ((rc = check_out8(d, out, "x8", data, (size_t)d->M * SFM_PAD8(d->K)))) return rc;
+    }
+    if ((rc = check_out8(d, out, "w8", w8, (size_t)d->N * SFM_PAD8(d->K))) ||
+        (rc = check_out8(d, out, "x", x, ((size_t)(d->M - 1) * x_stride + d->K) * 2))) return rc;
+    const bool gr = d->epilogue == SFM_EPI_GATE_RESIDUAL;
+    if (keep && (rc = launch_quantize8(d->dtype, d->M, d->K, x, x_stride, data, scale, nullptr, 0, nullptr, (hipStream_t)stream))) return rc;
+    return launch_linear8(*d, x, x_stride, data, scale, w8, wscale, bias, gr ? res : nullptr, gr ? gate : nullptr, out, (hipStream_t)stream);
 }
 
 int sfm_linear8_wgrad_workspace_bytes(int64_t M, int32_t N, int32_t K, size_t* bytes) {

@@ -16,7 +16,7 @@ import ctypes as C
 import torch
 
 from . import lib as _l
-from .block_ops import _HALF, _like, _mod, _row_stride, _rows, _written
+from .block_ops import _HALF, _like, _mod, _once, _row_stride, _rows, _written
 from .monarch_attn import _DT, _on_device, _stream
 
 _EPI = {"none": _l.EPI_NONE, "gelu_tanh": _l.EPI_GELU_TANH, "gate_residual": _l.EPI_GATE_RESIDUAL}
@@ -119,19 +119,36 @@ def pack(weight, transposed=True):
     return Weight8(data, scale, data_t, scale_t, (N, K), weight.dtype)
 
 
+def _desc(dtype, rows, N, K, out, epi, res, gate):
+    """(descriptor, gate tensor to hold on to or None)."""
+    if res is None:
+        return _l.Linear8Desc(_DT[dtype], epi, rows, N, K, _row_stride(out), 0, 0, 0, 0), None
+    g, gs, rpf = (None, 0, 1) if gate is None else _mod(gate, res)
+    return _l.Linear8Desc(_DT[dtype], epi, rows, N, K, _row_stride(out), _rows(res)[2], gs, rpf, 0), g
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
 def _product(x8, w_data, w_scale, N, bias, out, epi=_l.EPI_NONE, res=None, gate=None):
     B, L, K = x8.shape
-    d = _l.Linear8Desc(_DT[out.dtype], epi, B * L, N, K, _rows(out)[2], 0, 0, 0, 0)
-    g = None
-    if res is not None:
-        d.res_stride = _rows(res)[2]
-        if gate is not None:
-            g, d.gate_stride, d.rows_per_frame = _mod(gate, res)
+    d, g = _desc(out.dtype, B * L, N, K, out, epi, res, gate)
     with _on_device(out.device):
         _l.check(_l.load().sfm_linear8(C.byref(d), x8.data.data_ptr(), x8.scale.data_ptr(), w_data.data_ptr(), w_scale.data_ptr(),
-                                       None if bias is None else bias.data_ptr(), None if res is None else res.data_ptr(),
-                                       None if g is None else g.data_ptr(), out.data_ptr(), _stream(out)))
+                                       _ptr(bias), _ptr(res), _ptr(g), out.data_ptr(), _stream(out)))
     return out
+
+
+def _forward(x, w8, bias, out, keep, epi=_l.EPI_NONE, res=None, gate=None):
+    """Quantisation and product in one call; returns the rows' blocks where they are to be kept (few rows have none otherwise)."""
+    rows, K, xs = _rows(x)
+    d, g = _desc(x.dtype, rows, w8.shape[0], K, out, epi, res, gate)
+    data, scale = _empty_rows(rows, K, x.device) if keep or rows > _l.LINEAR8_FEW_ROWS else (None, None)
+    with _on_device(x.device):
+        _l.check(_l.load().sfm_linear8_fwd(C.byref(d), x.data_ptr(), xs, _ptr(data), _ptr(scale), w8.data.data_ptr(), w8.scale.data_ptr(),
+                                           _ptr(bias), _ptr(res), _ptr(g), out.data_ptr(), _stream(x)))
+    return data, scale
 
 
 def _wgrad(dy, x8, want_dw, want_db, cs=None):
@@ -173,20 +190,24 @@ class _Linear8Fn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, x8, w8):
         need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        if x8 is None:
-            x8 = quantize(x)
         if w8 is None:
             w8 = pack(weight, transposed=need_x)
         if need_x and w8.data_t is None:
             raise ValueError("the weight was packed without its transposed form, which the input's gradient needs")
+        rows = x if x8 is None else x8
         N = w8.shape[0]
-        out = _product(x8, w8.data, w8.scale, N, bias, torch.empty((*x8.shape[:2], N), dtype=x8.dtype, device=x8.device))
-        ctx.cfg = (x8.shape, x8.dtype, w8.shape)
-        ctx.save_for_backward(*((x8.data, x8.scale) if need_w else (None, None)), *((w8.data_t, w8.scale_t) if need_x else (None, None)))
+        out = torch.empty((*rows.shape[:2], N), dtype=rows.dtype, device=rows.device)
+        if x8 is None:
+            data, scale = _forward(x, w8, bias, out, need_w)
+        else:
+            data, scale = x8.data, x8.scale
+            _product(x8, w8.data, w8.scale, N, bias, out)
+        ctx.cfg = (rows.shape, rows.dtype, w8.shape)
+        ctx.save_for_backward(*((data, scale) if need_w else (None, None)), *((w8.data_t, w8.scale_t) if need_x else (None, None)))
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         x_shape, dtype, (N, K) = ctx.cfg
@@ -256,8 +277,10 @@ def linear8(x, weight, bias=None, epilogue="none", res=None, gate=None, out=None
             raise ValueError("out must be [B, L, N]")
         _rows(out)
         _written(out)
-    if x8 is None:
-        x8 = quantize(x)
     if w8 is None:
         w8 = pack(weight, transposed=False)
-    return _product(x8, w8.data, w8.scale, N, bias, out, _EPI[epilogue], res, gate)
+    if x8 is None:
+        _forward(x, w8, bias, out, False, _EPI[epilogue], res, gate)
+    else:
+        _product(x8, w8.data, w8.scale, N, bias, out, _EPI[epilogue], res, gate)
+    return out

@@ -104,7 +104,7 @@ def test_blocks_of_extreme_and_non_finite_values():
 
 
 # ------------------------------------------------------------------------------------------------ product
-SIZES = [(1, 1, 1), (1, 128, 16), (3, 1536, 100), (16, 100, 8), (17, 300, 40), (64, 128, 129), (65, 1000, 77), (128, 256, 256), (129, 513, 300),
+SIZES = [(1, 1, 1), (1, 128, 16), (3, 1536, 100), (16, 100, 8), (5, 2500, 70), (1, 8960, 33), (16, 2176, 130), (17, 300, 40), (64, 128, 129), (65, 1000, 77), (128, 256, 256), (129, 513, 300),
          (200, 2100, 130), (257, 640, 260), (700, 384, 520),
          (300, 100, 300), (300, 200, 260), (300, 390, 256), (300, 512, 264), (1100, 100, 260), (1100, 200, 300), (1100, 384, 256),
          (1030, 520, 257), (1281, 1300, 300), (1420, 513, 264), (2304, 640, 2100), (4300, 520, 5000)]

@@ -79,6 +79,25 @@ def test_product_refusals():
     _rc(f(out=3 * P + 64 * 128 - 2), -4, "overlaps")
 
 
+def test_forward_refusals():
+    lib = L.load()
+
+    def f(d=None, x=P, xs=128, data=2 * P, scale=3 * P, out=6 * P):
+        return lib.sfm_linear8_fwd(C.byref(_desc() if d is None else d), x, xs, data, scale, 4 * P, 5 * P, None, None, None, out, None)
+    _rc(f(x=None), -1, "x must")
+    _rc(f(xs=127), -5, "x: rows")
+    _rc(f(x=P + 1), -7, "x is not")
+    _rc(f(data=None), -1, "x8")
+    _rc(f(scale=None), -1, "x8")
+    _rc(f(_desc(M=17), data=None, scale=None), -1, "x8")
+    _rc(f(_desc(dtype=2)), -2, "dtype")
+    _rc(f(out=P + 64), -4, "overlaps x")
+    _rc(f(out=2 * P + 64), -4, "overlaps x8")
+    _rc(f(data=None, scale=None, out=4 * P + 64), -4, "overlaps w8")
+    text = open(os.path.join(ROOT, "include", "sfm_attn.h")).read()
+    assert f"#define SFM_LINEAR8_FEW_ROWS {L.LINEAR8_FEW_ROWS}\n" in text
+
+
 def test_gradient_refusals():
     lib = L.load()
     n = C.c_size_t(0)
