@@ -12,6 +12,8 @@
 //
 // Calls with few output tiles split the rows; the parts' fp32 sums meet in a fixed order in a second kernel.
 
+#include <type_traits>
+
 #include "rows8.hpp"
 
 namespace sfm {
@@ -218,17 +220,24 @@ __device__ __forceinline__ void wgrad8_tile(const WgradArgs& p, int n0, int kb, 
         off[j] = min(c, p.N - 8);
         down[j] = EDGE ? min(c - off[j], 7) : 0;
     }
-    auto fetch = [&](Raw& w, int64_t st) {
+    struct Rows {                                                       // where a step's row of this thread lies
+        const uint8_t *s, *x;
+        const uint16_t* d;
+    };
+    auto find = [&](int64_t st) {
         const int64_t row = min(st * kBR + r, p.M - 1);
-        const uint8_t* sc = p.xscale + scale_at8(row, kb, p.groups);
-        w.s[0] = sc[0];
-        w.s[1] = sc[kb1 * p.groups * kBlock8];
-        const uint16_t* d = (const uint16_t*)p.dy + row * p.dy_stride;
+        return Rows{p.xscale + scale_at8(row, kb, p.groups), p.x + row * p.kp + (int64_t)kb * kBlock8 + c8 * 16,
+                    (const uint16_t*)p.dy + row * p.dy_stride};
+    };
+    auto load = [&](Raw& w, const Rows& at, int i) {                    // request i of 8
+        if (i < 2) w.s[i] = at.s[i * kb1 * p.groups * kBlock8];
+        else if (i < 4) w.x[i - 2] = *(const u32x4*)(at.x + (i - 2) * kb1 * kBlock8);
+        else w.d[i - 4] = *(const u32x4_any*)(at.d + off[i - 4]);
+    };
+    auto fetch = [&](Raw& w, int64_t st) {
+        const Rows at = find(st);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w.d[j] = *(const u32x4_any*)(d + off[j]);
-        const uint8_t* x = p.x + row * p.kp + (int64_t)kb * kBlock8 + c8 * 16;
-        w.x[0] = *(const u32x4*)x;
-        w.x[1] = *(const u32x4*)(x + kBlock8 * kb1);
+        for (int i = 0; i < 8; ++i) load(w, at, i);
     };
     auto shifted = [&](u32x4 v, int by) {
         if (!EDGE) return v;
@@ -298,34 +307,54 @@ __device__ __forceinline__ void wgrad8_tile(const WgradArgs& p, int n0, int kb, 
     lds_barrier();
 #pragma unroll
     for (int i = 0; i < 8; ++i) f0[i] = operand_at(0, 0, i);
-    // step st from buffer `buf`; the next one's rows are in `w`, which then takes those of step st + 5
-    auto step = [&](int64_t st, Raw& w, int buf) {
-        const bool ok = live(st + 1);
+    // Step st from buffer `buf`; the next one's rows are in `w`, which then takes those of step st + 5.  WHOLE: all rows of the next
+    // step exist.  Behind the 16 matrix instructions of its first half: the reads for the second, the next step's rows into LDS, the
+    // first requests; of its second: the barrier, the reads for the next step (done some instructions before they are waited
+    // for), the other requests.
+    auto step = [&](int64_t st, Raw& w, int buf, auto whole_c) {
+        const bool ok = decltype(whole_c)::value || live(st + 1);
+        Rows rows;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             acc[i >> 2][i & 3] = E::mfma32(f0[i >> 2], f0[4 + (i & 3)], acc[i >> 2][i & 3]);
             __builtin_amdgcn_sched_barrier(0);
-            if (i < 8) f1[i] = operand_at(buf, 1, i);
-            else if (i < 12) put_dy(w, buf ^ 1, i - 8, ok);
-            else put_x(w, buf ^ 1, i - 12, ok);
+            if (i < 4) {
+                f1[2 * i] = operand_at(buf, 1, 2 * i);
+                f1[2 * i + 1] = operand_at(buf, 1, 2 * i + 1);
+            } else if (i < 8) {
+                put_dy(w, buf ^ 1, i - 4, ok);
+            } else if (i < 12) {
+                put_x(w, buf ^ 1, i - 8, ok);
+            } else if (i == 12) {
+                rows = find(last(st + 5));
+            } else {
+                load(w, rows, i - 13);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
-        fetch(w, last(st + 5));
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             acc[i >> 2][i & 3] = E::mfma32(f1[i >> 2], f1[4 + (i & 3)], acc[i >> 2][i & 3]);
             __builtin_amdgcn_sched_barrier(0);
-            if (i == 5) lds_barrier();
-            if (i > 5 && i < 14) f0[i - 6] = operand_at(buf ^ 1, 0, i - 6);
+            if (i == 1) lds_barrier();
+            if (i > 1 && i < 10) f0[i - 2] = operand_at(buf ^ 1, 0, i - 2);
+            if (i > 9 && i < 15) load(w, rows, i - 7);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
+    int64_t st = s0;
+    for (; st + 4 < s1 && (st + 5) * kBR <= p.M; st += 4) {
+        step(st, raw[1], 0, std::true_type{});
+        step(st + 1, raw[2], 1, std::true_type{});
+        step(st + 2, raw[3], 0, std::true_type{});
+        step(st + 3, raw[0], 1, std::true_type{});
+    }
     // rows behind the last step are zeros (`live`): up to three steps of nothing keep the loop whole
-    for (int64_t st = s0; st < s1; st += 4) {
-        step(st, raw[1], 0);
-        step(st + 1, raw[2], 1);
-        step(st + 2, raw[3], 0);
-        step(st + 3, raw[0], 1);
+    for (; st < s1; st += 4) {
+        step(st, raw[1], 0, std::false_type{});
+        step(st + 1, raw[2], 1, std::false_type{});
+        step(st + 2, raw[3], 0, std::false_type{});
+        step(st + 3, raw[0], 1, std::false_type{});
     }
     // lane: channel n = .. + m32, channels k = 8 g + 4 hf + (0..3) of a 32-block
 #pragma unroll
