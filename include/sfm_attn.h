@@ -382,6 +382,13 @@ int sfm_linear8_wgrad(int32_t dtype, int64_t M, int32_t N, int32_t K, const void
                       const void* xscale, void* dw, void* dbias, const float* colsum, void* workspace, size_t workspace_bytes,
                       void* stream);
 
+/* The backward of a linear layer in one call: dx = dy8 w8 (dy quantised here; [M, K] contiguous; data_t and scale_t are the transposed
+ * weight's), dw and dbias as in sfm_linear8_wgrad.  Each of dx, dw, dbias may be NULL, with what it needs; not all of them. */
+int sfm_linear8_bwd_workspace_bytes(int64_t M, int32_t N, int32_t K, size_t* bytes);
+int sfm_linear8_bwd(int32_t dtype, int64_t M, int32_t N, int32_t K, const void* dy, int64_t dy_stride, const void* data_t,
+                    const void* scale_t, const void* x8, const void* xscale, void* dx, void* dw, void* dbias, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
 /* dx = dy * gelu_tanh'(x) from x, or (x NULL) from the 8-bit blocks that sfm_quantize8 kept of it. */
 int sfm_gelu_bwd(int32_t dtype, int64_t rows, int32_t C, const void* x, int64_t x_stride, const void* data, const void* scale,
                  const void* dy, int64_t dy_stride, void* dx, int64_t dx_stride, void* stream);

@@ -50,24 +50,31 @@ __device__ __forceinline__ float l8_tail(float sum, float bias, float res, float
 }
 
 // four neighbouring channels c.. of a row: bias and epilogue on the fp32 sums, rounded once and stored
+template <class E>
+__device__ __forceinline__ void l8_get4(const L8Args& p, const uint16_t* s, int c, float* d) {
+    if (c + 4 <= p.N) {
+        l8_unpack4<E>(*(const u32x2_any*)s, d);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (c + i < p.N) d[i] = E::to_float(s[i]);
+    }
+}
+// the bias of four channels, zeros without one or past the last
+template <class E>
+__device__ __forceinline__ f32x4 l8_bias4(const L8Args& p, int c) {
+    float b[4] = {0.f, 0.f, 0.f, 0.f};
+    if (p.bias != nullptr) l8_get4<E>(p, p.bias + c, c, b);
+    return f32x4{b[0], b[1], b[2], b[3]};
+}
 template <class E, int EPI>
-__device__ __forceinline__ void l8_finish4(const L8Args& p, int64_t row, int c, const float* acc) {
+__device__ __forceinline__ void l8_finish4(const L8Args& p, int64_t row, int c, const float* acc, f32x4 b) {
     if (row >= p.M || c >= p.N) return;
     const bool full = c + 4 <= p.N;
-    float v[4], r[4] = {0.f, 0.f, 0.f, 0.f}, g[4] = {1.f, 1.f, 1.f, 1.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
-    auto get4 = [&](const uint16_t* s, float* d) {
-        if (full) {
-            l8_unpack4<E>(*(const u32x2_any*)s, d);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (c + i < p.N) d[i] = E::to_float(s[i]);
-        }
-    };
-    if (p.bias != nullptr) get4(p.bias + c, b);
+    float v[4], r[4] = {0.f, 0.f, 0.f, 0.f}, g[4] = {1.f, 1.f, 1.f, 1.f};
     if (EPI == SFM_EPI_GATE_RESIDUAL) {
-        get4(p.res + row * p.res_stride + c, r);
-        if (p.gate != nullptr) get4(p.gate + (row / p.rows_per_frame) * p.gate_stride + c, g);
+        l8_get4<E>(p, p.res + row * p.res_stride + c, c, r);
+        if (p.gate != nullptr) l8_get4<E>(p, p.gate + (row / p.rows_per_frame) * p.gate_stride + c, c, g);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = l8_tail<E, EPI>(acc[i], b[i], r[i], g[i]);
@@ -89,7 +96,8 @@ __device__ __forceinline__ i32x8 l8_load32(const uint8_t* p) {
 }
 
 // Any size: a workgroup of W waves owns 16 MT rows x 16 NT channels, its waves share the block columns (wave w takes w,
-// w + W, ...) and their sums meet in LDS in a fixed order.  Operands come from memory straight into registers, 32 bytes a
+// w + W, ...) and their sums meet in LDS in a fixed order.  Many waves hide the loads: with the next block column's operands held besides,
+// 128 x 1536 -> 8960 takes 26 us against 18.  Operands come from memory straight into registers, 32 bytes a
 // lane of one row: 4 lanes take a row's block of 128 bytes, a whole line.
 template <class E, int EPI, int MT, int NT, int W>
 __global__ __launch_bounds__(64 * W) void l8_direct_kernel(L8Args p) {
@@ -117,41 +125,24 @@ __global__ __launch_bounds__(64 * W) void l8_direct_kernel(L8Args p) {
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    struct Ops {
-        i32x8 x[MT], w[NT];
+    for (int kb = wave; kb < p.nkb; kb += W) {
+        i32x8 xf[MT], wf[NT];
         int xe[MT], we[NT];
-    };
-    auto fetch = [&](Ops& o, int kb) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            o.w[j] = l8_load32(wp[j] + (int64_t)kb * kBlock8);
-            o.we[j] = p.wscale[wsc[j] + kb];
+            wf[j] = l8_load32(wp[j] + (int64_t)kb * kBlock8);
+            we[j] = p.wscale[wsc[j] + kb];
         }
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-            o.x[i] = l8_load32(xp[i] + (int64_t)kb * kBlock8);
-            o.xe[i] = p.xscale[xsc[i] + (int64_t)kb * p.groups * kBlock8];
+            xf[i] = l8_load32(xp[i] + (int64_t)kb * kBlock8);
+            xe[i] = p.xscale[xsc[i] + (int64_t)kb * p.groups * kBlock8];
         }
-    };
-    auto multiply = [&](const Ops& o) {
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int j = 0; j < NT; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(o.w[j], o.x[i], acc[i][j], 0, 0, 0, o.we[j], 0, o.xe[i]);
-    };
-    // the next block column is on its way while one is multiplied (past the last, that one again)
-    Ops a, b;
-    const int last = p.nkb - 1;
-    if (wave <= last) {
-        fetch(a, wave);
-        for (int kb = wave; kb <= last; kb += 2 * W) {
-            fetch(b, min(kb + W, last));
-            multiply(a);
-            if (kb + W > last) break;
-            fetch(a, min(kb + 2 * W, last));
-            multiply(b);
-        }
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[j], xf[i], acc[i][j], 0, 0, 0, we[j], 0, xe[i]);
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -164,7 +155,7 @@ __global__ __launch_bounds__(64 * W) void l8_direct_kernel(L8Args p) {
 #pragma unroll
         for (int w = 1; w < W; ++w) s += part[w][t][lane];
         const float v[4] = {s.x, s.y, s.z, s.w};
-        l8_finish4<E, EPI>(p, m0 + 16 * (t / NT) + l16, n0 + 16 * (t % NT) + 4 * q, v);
+        l8_finish4<E, EPI>(p, m0 + 16 * (t / NT) + l16, n0 + 16 * (t % NT) + 4 * q, v, l8_bias4<E>(p, n0 + 16 * (t % NT) + 4 * q));
     }
 }
 
@@ -178,42 +169,50 @@ __global__ __launch_bounds__(64 * W) void l8_few_kernel(L8Args p, const uint16_t
     const int n0 = blockIdx.x * 16, n = min(n0 + l16, p.N - 1);
     const uint8_t* wp = p.w + (int64_t)n * p.kp + q * 32;
     const uint8_t* ws = p.wscale + (int64_t)(n >> 7) * p.pitch;
-    const bool live = l16 < p.M;
-    const int64_t row = live ? l16 * xstride : 0;
+    const uint16_t* xr = x + min((int64_t)l16, p.M - 1) * xstride;       // lanes past the last row form products that nobody stores
+    const f32x4 bias = l8_bias4<E>(p, n0 + 4 * q);                      // on its way from the start
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     struct Ops {
         i32x8 w;
         int we;
-        float v[4][8];
+        u32x4 v[4];
     };
+    const int whole = K / kBlock8;
     auto fetch = [&](Ops& o, int kb) {
         o.w = l8_load32(wp + (int64_t)kb * kBlock8);
         o.we = ws[kb];
+        const int c0 = kb * kBlock8 + q * 32;
+        if (kb < whole) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            if (live) {
-                load_part8<E>(x, row, kb * kBlock8 + q * 32 + 8 * c, K, o.v[c]);
-            } else {
+            for (int c = 0; c < 4; ++c) o.v[c] = *(const u32x4_any*)(xr + c0 + 8 * c);
+        } else {                                                        // the row ends in this block: zeros behind it
 #pragma unroll
-                for (int e = 0; e < 8; ++e) o.v[c][e] = 0.f;
+            for (int c = 0; c < 4; ++c) {
+                o.v[c] = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (c0 + 8 * c + e < K) o.v[c][e >> 1] |= (uint32_t)xr[c0 + 8 * c + e] << (16 * (e & 1));
             }
         }
     };
     auto multiply = [&](const Ops& o) {
-        float a = 0.f;
+        float v[32];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) a = fmaxf(a, finite_mag(o.v[c][e]));
-        a = fmaxf(a, __shfl_xor(a, 16));
-        const int s = block_exp8(fmaxf(a, __shfl_xor(a, 32)));
+        for (int i = 0; i < 16; ++i) {
+            v[2 * i] = E::to_float((uint16_t)(o.v[i >> 2][i & 3] & 0xffffu));
+            v[2 * i + 1] = E::to_float((uint16_t)(o.v[i >> 2][i & 3] >> 16));
+        }
+        auto block_max = [](float m) {
+            m = fmaxf(m, __shfl_xor(m, 16));
+            return fmaxf(m, __shfl_xor(m, 32));
+        };
+        float a = block_max(mag_max<32>(v));
+        if (__builtin_expect(a > 3.402823466e38f, 0)) a = block_max(mag_max_finite<32>(v));
+        const int s = block_exp8(a);
         const float inv = two_to(-s);
         i32x8 xf;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            xf[2 * c] = (int)pack_e4m3(o.v[c][0] * inv, o.v[c][1] * inv, o.v[c][2] * inv, o.v[c][3] * inv);
-            xf[2 * c + 1] = (int)pack_e4m3(o.v[c][4] * inv, o.v[c][5] * inv, o.v[c][6] * inv, o.v[c][7] * inv);
-        }
+        for (int c = 0; c < 8; ++c) xf[c] = (int)pack_e4m3(v[4 * c] * inv, v[4 * c + 1] * inv, v[4 * c + 2] * inv, v[4 * c + 3] * inv);
         acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(o.w, xf, acc, 0, 0, 0, o.we, 0, s + 127);
     };
     Ops a, b;
@@ -222,9 +221,11 @@ __global__ __launch_bounds__(64 * W) void l8_few_kernel(L8Args p, const uint16_t
         fetch(a, wave);
         for (int kb = wave; kb <= last; kb += 2 * W) {
             fetch(b, min(kb + W, last));
+            __builtin_amdgcn_sched_barrier(0);
             multiply(a);
             if (kb + W > last) break;
             fetch(a, min(kb + 2 * W, last));
+            __builtin_amdgcn_sched_barrier(0);
             multiply(b);
         }
     }
@@ -235,7 +236,7 @@ __global__ __launch_bounds__(64 * W) void l8_few_kernel(L8Args p, const uint16_t
 #pragma unroll
         for (int w = 1; w < W; ++w) s += part[w][lane];
         const float v[4] = {s.x, s.y, s.z, s.w};
-        l8_finish4<E, EPI>(p, l16, n0 + 4 * q, v);
+        l8_finish4<E, EPI>(p, l16, n0 + 4 * q, v, bias);
     }
 }
 
@@ -431,7 +432,7 @@ __device__ __forceinline__ void l8_store(const L8Args& p, const f32x16 (&acc)[4]
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const float a4[4] = {acc[cb][tb][4 * g], acc[cb][tb][4 * g + 1], acc[cb][tb][4 * g + 2], acc[cb][tb][4 * g + 3]};
-                l8_finish4<E, EPI>(p, r0 + own, c0 + 32 * cb + 8 * g + 4 * hf, a4);
+                l8_finish4<E, EPI>(p, r0 + own, c0 + 32 * cb + 8 * g + 4 * hf, a4, l8_bias4<E>(p, c0 + 32 * cb + 8 * g + 4 * hf));
             }
         }
 }

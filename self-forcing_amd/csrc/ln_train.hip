@@ -24,7 +24,8 @@ struct LnBwdArgs {
     const void* dy;
     void* dx;                // may be null
     const void* weight;      // [C], or scale rows (MOD) mod_stride apart
-    float* part;             // [groups of rows][splits][2][C]
+    float* part;             // [groups of rows][splits][2][C], unless a group has one workgroup, which stores dw and db itself
+    void *dw, *db;
     int64_t xs, dys, dxs, ms, rows, groups8;
     int C, rpg, splits;      // rows per group (of one weight gradient), workgroups per group
     float eps;
@@ -147,14 +148,17 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(LnBwdArgs p) {
     }
     // column sums of the workgroup
     float* part = p.part + (grp * p.splits + split) * 2 * (int64_t)p.C;
+    const bool alone = p.splits == 1;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
             const int ch = lane + (t * WPR + sub) * 64;
             float* v = which == 0 ? dw[t] : db[t];
+            void* out = which == 0 ? p.dw : p.db;
             if (WPR > 1) {
-                if (ch < nch) V8<float>::store(part, which * (int64_t)p.C + ch * 8, v);
+                if (ch < nch && alone) V::store(out, grp * p.C + ch * 8, v);
+                else if (ch < nch) V8<float>::store(part, which * (int64_t)p.C + ch * 8, v);
             } else {
                 __syncthreads();
 #pragma unroll
@@ -164,27 +168,39 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(LnBwdArgs p) {
                     const int l = e >> 3, i = e & 7;
                     const float s = col[0][i * 64 + l] + col[1][i * 64 + l] + col[2][i * 64 + l] + col[3][i * 64 + l];
                     const int c = (t * 64 + l) * 8 + i;
-                    if (c < p.C) part[which * (int64_t)p.C + c] = s;
+                    if (c < p.C && alone) Elem<T>::put(out, grp * p.C + c, s);
+                    else if (c < p.C) part[which * (int64_t)p.C + c] = s;
                 }
             }
         }
 }
 
-// out[g][c] = sum over s of part[g][s][c], c < n; the first `n1` columns of a group go to out1, the rest to out2.  32
-// columns x 8 slices of the parts per workgroup
-template <typename T>
-__global__ __launch_bounds__(256) void sum_parts_kernel(const float* part, int64_t parts, int64_t n, int64_t n1, void* out1, void* out2) {
-    __shared__ float sl[8][32];
-    const int l = threadIdx.x & 31, s8 = threadIdx.x >> 5;
+// out[g][c] = sum over s of part[g][s][c], c < n; the first `n1` columns of a group go to out1, the rest to out2.  32 columns x SL
+// slices of the parts per workgroup, the slices in a fixed order; SL = 32 where there are parts enough: a thread's loads, eight at a
+// time, are then few one after the other (512 parts of 2 x 1536 columns: 5 us, with 8 slices 20)
+template <typename T, int SL>
+__global__ __launch_bounds__(32 * SL) void sum_parts_kernel(const float* part, int64_t parts, int64_t n, int64_t n1, void* out1, void* out2) {
+    __shared__ float sl[SL][32];
+    const int l = threadIdx.x & 31, sn = threadIdx.x >> 5;
     const int64_t cols = (n + 31) / 32, g = blockIdx.x / cols, c = (blockIdx.x % cols) * 32 + l;
     float s = 0.f;
-    if (c < n)
-        for (int64_t i = s8; i < parts; i += 8) s += part[(g * parts + i) * n + c];
-    sl[s8][l] = s;
-    __syncthreads();
-    if (s8 == 0 && c < n) {
+    if (c < n) {
+        const float* p = part + (g * parts) * n + c;
+        int64_t i = sn;
+        for (; i + 7 * SL < parts; i += 8 * SL) {
+            float v[8];
 #pragma unroll
-        for (int i = 1; i < 8; ++i) s += sl[i][l];
+            for (int e = 0; e < 8; ++e) v[e] = p[(i + e * SL) * n];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s += v[e];
+        }
+        for (; i < parts; i += SL) s += p[i * n];
+    }
+    sl[sn][l] = s;
+    __syncthreads();
+    if (sn == 0 && c < n) {
+#pragma unroll
+        for (int i = 1; i < SL; ++i) s += sl[i][l];
         if (c < n1) Elem<T>::put(out1, g * n1 + c, s);
         else Elem<T>::put(out2, g * (n - n1) + c - n1, s);
     }
@@ -229,18 +245,12 @@ __global__ __launch_bounds__(256) void ln_keep8_kernel(const void* x, int64_t xs
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const int ch = lane + t * 64;
-        float n[8], a = 0.f;
+        float n[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            n[i] = ch < nch ? (v[t][i] - mean) * rstd : 0.f;
-            a = fmaxf(a, finite_mag(n[i]));
-        }
-        const int s = block_exp8(max16(a));
-        const float inv = two_to(-s);
+        for (int i = 0; i < 8; ++i) n[i] = ch < nch ? (v[t][i] - mean) * rstd : 0.f;
+        u32x2 q;
+        const int s = quantize_block8(n, &q);
         if (ch < kp / 8) {
-            u32x2 q;
-            q.x = pack_e4m3(n[0] * inv, n[1] * inv, n[2] * inv, n[3] * inv);
-            q.y = pack_e4m3(n[4] * inv, n[5] * inv, n[6] * inv, n[7] * inv);
             *(u32x2*)(data + row * kp + ch * 8) = q;
             if ((lane & 15) == 0) scale8[scale_at8(row, ch >> 4, groups)] = (uint8_t)(s + 127);
         }
@@ -290,7 +300,9 @@ int ln_bwd_m(const LnBwdArgs& a, bool mod, int64_t groups, hipStream_t st) {
 
 template <typename T>
 int sum_parts_t(int64_t parts, int64_t n, int64_t n1, int64_t groups, const float* part, void* out1, void* out2, hipStream_t st) {
-    hipLaunchKernelGGL((sum_parts_kernel<T>), dim3((unsigned)((n + 31) / 32 * groups)), dim3(256), 0, st, part, parts, n, n1, out1, out2);
+    const dim3 grid((unsigned)((n + 31) / 32 * groups));
+    if (parts >= 64) hipLaunchKernelGGL((sum_parts_kernel<T, 32>), grid, dim3(1024), 0, st, part, parts, n, n1, out1, out2);
+    else hipLaunchKernelGGL((sum_parts_kernel<T, 8>), grid, dim3(256), 0, st, part, parts, n, n1, out1, out2);
     return launched8("sum of partials");
 }
 
@@ -321,6 +333,8 @@ int launch_ln_bwd(int dtype, int64_t rows, int C, float eps, const void* x, int6
     a.dx = dx;
     a.weight = weight;
     a.part = (float*)workspace;
+    a.dw = dw;
+    a.db = db;
     a.xs = xs;
     a.dys = dys;
     a.dxs = dxs;
@@ -332,7 +346,7 @@ int launch_ln_bwd(int dtype, int64_t rows, int C, float eps, const void* x, int6
     a.splits = ln_bwd_splits(groups, rows_per_group, C);
     a.eps = eps;
     int rc = dtype == SFM_BF16 ? ln_bwd_m<BF16>(a, mod, groups, st) : dtype == SFM_F16 ? ln_bwd_m<F16>(a, mod, groups, st) : ln_bwd_m<float>(a, mod, groups, st);
-    if (rc) return rc;
+    if (rc || a.splits == 1) return rc;
     return launch_sum_parts(dtype, a.splits, 2 * (int64_t)C, groups, a.part, dw, db, st);
 }
 

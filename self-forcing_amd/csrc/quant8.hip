@@ -17,8 +17,8 @@ namespace {
 template <typename T, bool GELU>
 __global__ __launch_bounds__(256) void quantize8_kernel(const void* x, int64_t xs, int64_t rows, int K, uint8_t* data,
                                                         uint8_t* scale, void* y, int64_t ys, float* colsum) {
-    __shared__ uint8_t sc[kBlock8];
-    __shared__ float cs[16][kBlock8];
+    __shared__ __attribute__((aligned(16))) uint8_t sc[kBlock8];
+    __shared__ __attribute__((aligned(16))) float cs[16][kBlock8];
     const int64_t groups = gridDim.x;
     const int kb = blockIdx.y, l16 = threadIdx.x & 15, r0 = threadIdx.x >> 4;
     const int c = kb * kBlock8 + l16 * 8;
@@ -41,21 +41,15 @@ __global__ __launch_bounds__(256) void quantize8_kernel(const void* x, int64_t x
             s[e] = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) s[e] += v[i][e];
-            cs[r0][l16 * 8 + e] = s[e];
         }
+        V8<float>::store(&cs[r0][0], l16 * 8, s);
     }
     if (data != nullptr) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int64_t r = row0 + r0 + 16 * i;
-            float a = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) a = fmaxf(a, finite_mag(v[i][e]));
-            const int s = block_exp8(max16(a));
-            const float inv = two_to(-s);
             u32x2 q;
-            q.x = pack_e4m3(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
-            q.y = pack_e4m3(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv);
+            const int s = quantize_block8(v[i], &q);
             if (r < rows) *(u32x2*)(data + r * kp + c) = q;
             const int rr = r0 + 16 * i;
             if (l16 == 0) sc[((rr & 31) << 2) + (rr >> 5)] = (uint8_t)(s + 127);
@@ -154,14 +148,25 @@ __global__ __launch_bounds__(256) void pack8_kernel(const void* w, int64_t ws, i
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) a = fmaxf(a, finite_mag(v[i][e]));
+        a = fmaxf(a, mag_max<8>(v[i]));
     }
+    auto block_max = [&](float m) {
+        m = max16(m);
+        m = fmaxf(m, __shfl_xor(m, 16));
+        m = fmaxf(m, __shfl_xor(m, 32));
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = m;
+        __syncthreads();
+        return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+    };
+    a = block_max(a);
+    if (a > 3.402823466e38f) {                       // the same for the whole workgroup
+        a = 0.f;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o));
-    if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = a;
-    __syncthreads();
-    const int s = block_exp8(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+        for (int i = 0; i < 8; ++i) a = fmaxf(a, mag_max_finite<8>(v[i]));
+        a = block_max(a);
+    }
+    const int s = block_exp8(a);
     const float inv = two_to(-s);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {

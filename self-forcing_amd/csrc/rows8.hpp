@@ -88,11 +88,10 @@ __device__ __forceinline__ float finite_mag(float v) {
     const float a = fabsf(v);
     return a <= 3.402823466e38f ? a : 0.f;
 }
-// four values, already divided by the block's scale, to e4m3
+// four values, already divided by the block's scale, to e4m3: at most 448, or not finite, which the conversion turns into NaN
 __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
-    auto fit = [](float v) { return fabsf(v) <= 448.f ? v : __uint_as_float(0x7fc00000u); };
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(fit(a), fit(b), 0, false);
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(fit(c), fit(d), w, true);
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
     return (uint32_t)w;
 }
 __device__ __forceinline__ void unpack_e4m3(uint32_t w, float* v) {
@@ -156,11 +155,40 @@ __device__ __forceinline__ void store_part8(void* p, int64_t row_off, int c, int
     }
 }
 
-// maximum over the 16 lanes that share a block of 128 values (8 a lane)
+// maximum over the 16 lanes that share a block of 128 values (8 a lane), in all of them: rotations within the row of lanes
 __device__ __forceinline__ float max16(float a) {
+    auto turned = [](float v, auto by) {
+        return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + decltype(by)::value, 0xf, 0xf, true));
+    };
+    a = fmaxf(a, turned(a, std::integral_constant<int, 8>{}));
+    a = fmaxf(a, turned(a, std::integral_constant<int, 4>{}));
+    a = fmaxf(a, turned(a, std::integral_constant<int, 2>{}));
+    return fmaxf(a, turned(a, std::integral_constant<int, 1>{}));
+}
+// largest magnitude of N values, not numbers left out; infinite values are (with their block redone by `finite_mag`) the rare case
+template <int N>
+__device__ __forceinline__ float mag_max(const float* v) {
+    float a = 0.f;
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o));
+    for (int i = 0; i < N; ++i) a = fmaxf(a, fabsf(v[i]));
     return a;
+}
+template <int N>
+__device__ __forceinline__ float mag_max_finite(const float* v) {
+    float a = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) a = fmaxf(a, finite_mag(v[i]));
+    return a;
+}
+// 8 values of each of 16 lanes that make a block: the block's exponent, and the lane's bytes
+__device__ __forceinline__ int quantize_block8(const float* v, u32x2* q) {
+    float a = max16(mag_max<8>(v));
+    if (__builtin_expect(a > 3.402823466e38f, 0)) a = max16(mag_max_finite<8>(v));
+    const int s = block_exp8(a);
+    const float inv = two_to(-s);
+    q->x = pack_e4m3(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+    q->y = pack_e4m3(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+    return s;
 }
 
 // GELU in its tanh form, 0.5 x (1 + tanh(u)) with u = sqrt(2/pi) (x + 0.044715 x^3), as x p with p = 1 / (1 + exp(-2u)): no

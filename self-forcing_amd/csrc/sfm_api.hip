@@ -1579,6 +1579,71 @@ int sfm_linear8_wgrad(int32_t dtype, int64_t M, int32_t N, int32_t K, const void
     return launch_wgrad8(dtype, M, N, K, dy, dy_stride, x8, xscale, dw, dbias, colsum, workspace, (hipStream_t)stream);
 }
 
+// dy's blocks, their scales, its column sums, and what sfm_linear8_wgrad needs besides
+struct Linear8BwdLayout {
+    size_t data, scale, colsum, rest, total;
+};
+static Linear8BwdLayout linear8_bwd_layout(int64_t M, int32_t N, int32_t K) {
+    auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+    Linear8BwdLayout l;
+    l.data = 0;
+    l.scale = up((size_t)M * SFM_PAD8(N));
+    l.colsum = l.scale + up((size_t)SFM_ROWS8_SCALE_BYTES(M, N));
+    l.rest = l.colsum + up((size_t)((M + 127) / 128) * N * sizeof(float));
+    l.total = l.rest + wgrad8_workspace_bytes(M, N, K, false);
+    return l;
+}
+
+int sfm_linear8_bwd_workspace_bytes(int64_t M, int32_t N, int32_t K, size_t* bytes) {
+    if (!bytes) {
+        set_error("bytes must be non-NULL");
+        return SFM_ERR_NULL;
+    }
+    int rc = check_rows8(SFM_BF16, M, K, false);
+    if (!rc) rc = check_rows8(SFM_BF16, M, N, false);
+    if (rc) return rc;
+    *bytes = linear8_bwd_layout(M, N, K).total;
+    return SFM_OK;
+}
+
+int sfm_linear8_bwd(int32_t dtype, int64_t M, int32_t N, int32_t K, const void* dy, int64_t dy_stride, const void* data_t,
+                    const void* scale_t, const void* x8, const void* xscale, void* dx, void* dw, void* dbias, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+    int rc = check_rows8(dtype, M, K, false);
+    if (!rc) rc = check_rows8(dtype, M, N, false);
+    if (rc) return rc;
+    if (!dy || (!dx && !dw && !dbias)) {
+        set_error("dy and one of dx, dw and dbias must be non-NULL");
+        return SFM_ERR_NULL;
+    }
+    if ((rc = check_elem("dy", dy, dy_stride, N, 2)) || (dx && (rc = check_blocks("the transposed weight", data_t, scale_t))) ||
+        (dw && (rc = check_blocks("x8", x8, xscale)))) return rc;
+    if ((dx && (rc = check_elem("dx", dx, K, K, 2))) || (dw && (rc = check_elem("dw", dw, K, K, 2))) ||
+        (dbias && (rc = check_elem("dbias", dbias, N, N, 2)))) return rc;
+    const Linear8BwdLayout l = linear8_bwd_layout(M, N, K);
+    if (!workspace || (((uintptr_t)workspace) & 255) || workspace_bytes < l.total) {
+        set_error("workspace must be non-NULL, 256-byte aligned and hold %zu bytes", l.total);
+        return SFM_ERR_WORKSPACE;
+    }
+    char* ws = (char*)workspace;
+    hipStream_t st = (hipStream_t)stream;
+    float* colsum = dbias ? (float*)(ws + l.colsum) : nullptr;
+    if (dx || dbias) {
+        if ((rc = launch_quantize8(dtype, M, N, dy, dy_stride, dx ? ws + l.data : nullptr, ws + l.scale, nullptr, 0, colsum, st))) return rc;
+    }
+    if (dx) {
+        sfm_linear8_desc d = {};
+        d.dtype = dtype;
+        d.epilogue = SFM_EPI_NONE;
+        d.M = M;
+        d.N = K;
+        d.K = N;
+        d.out_stride = K;
+        if ((rc = launch_linear8(d, nullptr, 0, ws + l.data, ws + l.scale, data_t, scale_t, nullptr, nullptr, nullptr, dx, st))) return rc;
+    }
+    return dw || dbias ? launch_wgrad8(dtype, M, N, K, dy, dy_stride, x8, xscale, dw, dbias, colsum, ws + l.rest, st) : SFM_OK;
+}
+
 int sfm_gelu_bwd(int32_t dtype, int64_t rows, int32_t C, const void* x, int64_t x_stride, const void* data, const void* scale,
                  const void* dy, int64_t dy_stride, void* dx, int64_t dx_stride, void* stream) {
     int rc = check_rows8(dtype, rows, C, true);

@@ -78,20 +78,14 @@ def _empty_rows(rows, K, device):
     return torch.empty((rows, _pad(K)), dtype=torch.uint8, device=device), torch.empty(n, dtype=torch.uint8, device=device)
 
 
-def _quantize(x, want_data=True, colsum=False):
-    """(Rows8 or None, column sums by 128 rows or None) of [B, L, K] rows."""
-    rows, K, xs = _rows(x)
-    data, scale = _empty_rows(rows, K, x.device) if want_data else (None, None)
-    cs = torch.empty((-(-rows // 128), K), dtype=torch.float32, device=x.device) if colsum else None
-    with _on_device(x.device):
-        _l.check(_l.load().sfm_quantize8(_DT[x.dtype], rows, K, x.data_ptr(), xs, data.data_ptr() if want_data else None,
-                                         scale.data_ptr() if want_data else None, None, 0, cs.data_ptr() if colsum else None, _stream(x)))
-    return (Rows8(data, scale, x.shape, x.dtype) if want_data else None), cs
-
-
 def quantize(x):
     """[B, L, K] rows (bf16, fp16 or fp32; any K) in 8-bit blocks.  Not differentiable."""
-    return _quantize(x.detach())[0]
+    x = x.detach()
+    rows, K, xs = _rows(x)
+    data, scale = _empty_rows(rows, K, x.device)
+    with _on_device(x.device):
+        _l.check(_l.load().sfm_quantize8(_DT[x.dtype], rows, K, x.data_ptr(), xs, data.data_ptr(), scale.data_ptr(), None, 0, None, _stream(x)))
+    return Rows8(data, scale, x.shape, x.dtype)
 
 
 def pack(weight, transposed=True):
@@ -151,19 +145,10 @@ def _forward(x, w8, bias, out, keep, epi=_l.EPI_NONE, res=None, gate=None):
     return data, scale
 
 
-def _wgrad(dy, x8, want_dw, want_db, cs=None):
-    rows, N, dys = _rows(dy)
-    K = x8.shape[2]
-    dw = torch.empty((N, K), dtype=dy.dtype, device=dy.device) if want_dw else None
-    db = torch.empty(N, dtype=dy.dtype, device=dy.device) if want_db else None
+def _bytes(query, *sizes):
     n = C.c_size_t(0)
-    _l.check(_l.load().sfm_linear8_wgrad_workspace_bytes(rows, N, K, C.byref(n)))
-    ws = torch.empty(max(n.value, 1), dtype=torch.uint8, device=dy.device)
-    with _on_device(dy.device):
-        _l.check(_l.load().sfm_linear8_wgrad(_DT[dy.dtype], rows, N, K, dy.data_ptr(), dys, x8.data.data_ptr(), x8.scale.data_ptr(),
-                                             dw.data_ptr() if want_dw else None, db.data_ptr() if want_db else None,
-                                             None if cs is None else cs.data_ptr(), ws.data_ptr(), n.value, _stream(dy)))
-    return dw, db
+    _l.check(query(*sizes, C.byref(n)))
+    return n.value
 
 
 def weight_grad(dy, x8):
@@ -175,7 +160,16 @@ def weight_grad(dy, x8):
         raise ValueError("expected dy [B, L, N] and the Rows8 of a [B, L, K] input")
     if dy.device != x8.device:
         raise ValueError(f"dy on {dy.device}, the rows on {x8.device}")
-    return _wgrad(_even(dy), x8, True, True)
+    dy = _even(dy)
+    rows, N, dys = _rows(dy)
+    K = x8.shape[2]
+    dw, db = torch.empty((N, K), dtype=dy.dtype, device=dy.device), torch.empty(N, dtype=dy.dtype, device=dy.device)
+    with _on_device(dy.device):
+        n = _bytes(_l.load().sfm_linear8_wgrad_workspace_bytes, rows, N, K)
+        ws = torch.empty(n, dtype=torch.uint8, device=dy.device)
+        _l.check(_l.load().sfm_linear8_wgrad(_DT[dy.dtype], rows, N, K, dy.data_ptr(), dys, x8.data.data_ptr(), x8.scale.data_ptr(),
+                                             dw.data_ptr(), db.data_ptr(), None, ws.data_ptr(), n, _stream(dy)))
+    return dw, db
 
 
 def _even(dy):
@@ -213,13 +207,15 @@ class _Linear8Fn(torch.autograd.Function):
         x_shape, dtype, (N, K) = ctx.cfg
         xd, xs, wd, ws = ctx.saved_tensors
         dy = _even(dy)
-        dx = dw = db = cs = None
-        if need_x:
-            dy8, cs = _quantize(dy, colsum=need_b)
-            dx = _product(dy8, wd, ws, K, None, torch.empty(x_shape, dtype=dtype, device=dy.device))
-        if need_w or need_b:
-            x8 = Rows8(xd, xs, x_shape, dtype) if need_w else Rows8(dy, dy, x_shape, dtype)     # the bias' gradient reads no rows
-            dw, db = _wgrad(dy, x8, need_w, need_b, cs)
+        rows, dev = x_shape[0] * x_shape[1], dy.device
+        dx = torch.empty(x_shape, dtype=dtype, device=dev) if need_x else None
+        dw = torch.empty((N, K), dtype=dtype, device=dev) if need_w else None
+        db = torch.empty(N, dtype=dtype, device=dev) if need_b else None
+        with _on_device(dev):
+            n = _bytes(_l.load().sfm_linear8_bwd_workspace_bytes, rows, N, K)
+            work = torch.empty(n, dtype=torch.uint8, device=dev)
+            _l.check(_l.load().sfm_linear8_bwd(_DT[dtype], rows, N, K, dy.data_ptr(), _row_stride(dy), _ptr(wd), _ptr(ws), _ptr(xd), _ptr(xs),
+                                               _ptr(dx), _ptr(dw), _ptr(db), work.data_ptr(), n, _stream(dy)))
         return dx, dw, db, None, None
 
 

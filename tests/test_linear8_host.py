@@ -118,6 +118,22 @@ def test_gradient_refusals():
     _rc(f(ws=None), -6, "workspace")
     _rc(f(ws=6 * P + 16), -6, "workspace")
     _rc(f(wb=need - 1), -6, "workspace")
+    assert lib.sfm_linear8_bwd_workspace_bytes(300, 64, 128, C.byref(n)) == 0 and n.value >= 300 * 128 + need
+    all_of = n.value
+    _rc(lib.sfm_linear8_bwd_workspace_bytes(300, 64, 128, None), -1, "bytes")
+    _rc(lib.sfm_linear8_bwd_workspace_bytes(300, 0, 128, C.byref(n)), -3, "rows=")
+
+    def g(dt=0, dy=P, dys=64, wt=7 * P, st=8 * P, x=2 * P, xs=3 * P, dx=9 * P, dw=4 * P, db=5 * P, ws=6 * P, wb=all_of):
+        return lib.sfm_linear8_bwd(dt, 300, 64, 128, dy, dys, wt, st, x, xs, dx, dw, db, ws, wb, None)
+    _rc(g(dt=2), -2, "dtype")
+    _rc(g(dy=None), -1, "dy")
+    _rc(g(dx=None, dw=None, db=None), -1, "one of dx")
+    _rc(g(wt=None), -1, "transposed")
+    _rc(g(x=None), -1, "x8")
+    _rc(g(dys=63), -5, "dy")
+    _rc(g(dx=9 * P + 1), -7, "dx")
+    _rc(g(ws=6 * P + 8), -6, "workspace")
+    _rc(g(wb=all_of - 1), -6, "workspace")
     _rc(lib.sfm_gelu_bwd(0, 4, 128, None, 0, None, P, P, 128, P, 128, None), -1, "gelu_bwd")
     _rc(lib.sfm_gelu_bwd(0, 4, 128, P, 128, None, None, None, 128, P, 128, None), -1, "dy")
     _rc(lib.sfm_gelu_bwd(0, 4, 128, P, 127, None, None, P, 128, P, 128, None), -5, "x: rows")
