@@ -2,6 +2,7 @@
 RMSNorm, GELU); counterparts of the eager chains in wan/modules/causal_model.py:1176-1205 and
 wan/modules/model.py:462-478.  [B, L, C] tensors, modulation rows [B, F, 1, C] (one per latent frame)."""
 import ctypes
+import functools
 
 import torch
 
@@ -113,22 +114,31 @@ def _ln_keep8(x, mod, eps):
     return y, data, scale, rstd
 
 
-def _ln_bwd(dy, x, kept, weight, scale, ms, group, eps, want_dx=True):
-    """(dx, dw, db): dw, db [groups of rows, C].  From x, or from `kept` = (data, scales, 1 / standard deviations)."""
-    dy = _even(dy)
-    B, L, C = dy.shape
-    rows, xs = B * L, 0 if x is None else _rows(x)[2]
-    dx = torch.empty((B, L, C), dtype=dy.dtype, device=dy.device) if want_dx else None
-    dw, db = (torch.empty((rows // group, C), dtype=dy.dtype, device=dy.device) for _ in range(2))
+@functools.lru_cache(maxsize=1024)
+def _ln_bwd_bytes(rows, C, group, device_index):
+    """Workspace of sfm_ln_bwd on a device (its compute units are in the size)."""
     n = ctypes.c_size_t(0)
     _l.check(_l.load().sfm_ln_bwd_workspace_bytes(rows, C, group, ctypes.byref(n)))
-    ws = torch.empty(n.value, dtype=torch.uint8, device=dy.device)
+    return n.value
+
+
+def _ln_bwd(dy, x, kept, weight, scale, ms, group, eps, w_shape, b_shape, want_dx=True):
+    """(dx, dw, db): dw, db hold [groups of rows, C] in the given shapes.  From x, or from `kept` = (data, scales, 1 / standard
+    deviations)."""
+    dy = _even(dy)
+    B, L, C = dy.shape
+    dt, dev = dy.dtype, dy.device
+    rows = B * L
+    dx = torch.empty((B, L, C), dtype=dt, device=dev) if want_dx else None
+    dw, db = torch.empty(w_shape, dtype=dt, device=dev), torch.empty(b_shape, dtype=dt, device=dev)
     data, sc8, rstd = (None, None, None) if kept is None else (t.data_ptr() for t in kept)
-    with _on_device(dy.device):
-        _l.check(_l.load().sfm_ln_bwd(_DT[dy.dtype], rows, C, eps, None if x is None else x.data_ptr(), xs, data, sc8, rstd, dy.data_ptr(),
-                                      _row_stride(dy), None if weight is None else weight.data_ptr(), None if scale is None else scale.data_ptr(),
-                                      ms, group, None if dx is None else dx.data_ptr(), C, dw.data_ptr(), db.data_ptr(), ws.data_ptr(),
-                                      n.value, _stream(dy)))
+    with _on_device(dev):
+        n = _ln_bwd_bytes(rows, C, group, dev.index)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        _l.check(_l.load().sfm_ln_bwd(_DT[dt], rows, C, eps, None if x is None else x.data_ptr(), 0 if x is None else _row_stride(x), data, sc8,
+                                      rstd, dy.data_ptr(), _row_stride(dy), None if weight is None else weight.data_ptr(),
+                                      None if scale is None else scale.data_ptr(), ms, group, dx.data_ptr() if want_dx else None, C,
+                                      dw.data_ptr(), db.data_ptr(), ws.data_ptr(), n, _stream(dy)))
     return dx, dw, db
 
 
@@ -166,8 +176,9 @@ class _LnFn(torch.autograd.Function):
         modulate, eps, checkpoint8, ms, rpf, a_shape, b_shape = ctx.cfg
         sc, *rest = ctx.saved_tensors
         x, kept = (None, rest) if checkpoint8 else (rest[0], None)
-        dx, dw, db = _ln_bwd(dy, x, kept, None if modulate else sc, sc if modulate else None, ms, rpf, eps, ctx.needs_input_grad[0])
-        return dx, dw.view(a_shape), db.view(b_shape), None, None, None
+        dx, dw, db = _ln_bwd(dy, x, kept, None if modulate else sc, sc if modulate else None, ms, rpf, eps, a_shape, b_shape,
+                             ctx.needs_input_grad[0])
+        return dx, dw, db, None, None, None
 
 
 def ln_modulate(x, scale, shift, eps=1e-6, checkpoint8=False):
@@ -197,8 +208,7 @@ def ln_affine_backward(dy, x, weight, eps=1e-6):
     """(dx, dweight, dbias) of ln_affine from its output's gradient."""
     _rows(x)
     _check_dy(dy, x)
-    dx, dw, db = _ln_bwd(dy, x, None, _vec("weight", weight, x), None, 0, x.shape[0] * x.shape[1], eps)
-    return dx, dw[0], db[0]
+    return _ln_bwd(dy, x, None, _vec("weight", weight, x), None, 0, x.shape[0] * x.shape[1], eps, weight.shape, weight.shape)
 
 
 def ln_modulate_backward(dy, x, scale, eps=1e-6):
@@ -206,8 +216,7 @@ def ln_modulate_backward(dy, x, scale, eps=1e-6):
     _rows(x)
     _check_dy(dy, x)
     sc, ms, rpf = _mod(scale, x)
-    dx, dw, db = _ln_bwd(dy, x, None, None, sc, ms, rpf, eps)
-    return dx, dw.view(scale.shape), db.view(scale.shape)
+    return _ln_bwd(dy, x, None, None, sc, ms, rpf, eps, scale.shape, scale.shape)
 
 
 def _gelu(x, keep8):

@@ -12,6 +12,7 @@ finite.
 The gradients are those of the product with the rounding passed through: dx = dy8 w8 (dy in 8-bit blocks too), dw = dy^T x8 with dy
 as it is, dbias = sum of dy."""
 import ctypes as C
+import functools
 
 import torch
 
@@ -145,9 +146,11 @@ def _forward(x, w8, bias, out, keep, epi=_l.EPI_NONE, res=None, gate=None):
     return data, scale
 
 
-def _bytes(query, *sizes):
+@functools.lru_cache(maxsize=1024)
+def _bytes(query, rows, N, K, device_index):
+    """Workspace that the named query asks for on a device (its compute units are in the size)."""
     n = C.c_size_t(0)
-    _l.check(query(*sizes, C.byref(n)))
+    _l.check(getattr(_l.load(), query)(rows, N, K, C.byref(n)))
     return n.value
 
 
@@ -165,7 +168,7 @@ def weight_grad(dy, x8):
     K = x8.shape[2]
     dw, db = torch.empty((N, K), dtype=dy.dtype, device=dy.device), torch.empty(N, dtype=dy.dtype, device=dy.device)
     with _on_device(dy.device):
-        n = _bytes(_l.load().sfm_linear8_wgrad_workspace_bytes, rows, N, K)
+        n = _bytes("sfm_linear8_wgrad_workspace_bytes", rows, N, K, dy.device.index)
         ws = torch.empty(n, dtype=torch.uint8, device=dy.device)
         _l.check(_l.load().sfm_linear8_wgrad(_DT[dy.dtype], rows, N, K, dy.data_ptr(), dys, x8.data.data_ptr(), x8.scale.data_ptr(),
                                              dw.data_ptr(), db.data_ptr(), None, ws.data_ptr(), n, _stream(dy)))
@@ -212,7 +215,7 @@ class _Linear8Fn(torch.autograd.Function):
         dw = torch.empty((N, K), dtype=dtype, device=dev) if need_w else None
         db = torch.empty(N, dtype=dtype, device=dev) if need_b else None
         with _on_device(dev):
-            n = _bytes(_l.load().sfm_linear8_bwd_workspace_bytes, rows, N, K)
+            n = _bytes("sfm_linear8_bwd_workspace_bytes", rows, N, K, dev.index)
             work = torch.empty(n, dtype=torch.uint8, device=dev)
             _l.check(_l.load().sfm_linear8_bwd(_DT[dtype], rows, N, K, dy.data_ptr(), _row_stride(dy), _ptr(wd), _ptr(ws), _ptr(xd), _ptr(xs),
                                                _ptr(dx), _ptr(dw), _ptr(db), work.data_ptr(), n, _stream(dy)))
