@@ -26,6 +26,7 @@ import torch.nn.functional as F
 from . import attention as _attn
 from . import block_ops as _blk
 from . import linear as _lin
+from . import linear8 as _l8
 from . import monarch_attn as _mon
 from . import prologue as _pro
 
@@ -43,14 +44,21 @@ class HipAttentionOps:
     hipBLASLt: False (default) none; "auto" the square projections of the block (attention output, cross-attention q
     and output: N, K <= 2048), where the own kernel's 128 x 256 tiles are level with hipBLASLt in isolation (26 vs
     25-29 us at 4680 x 1536 x 1536) and 0.5 % slower over a rollout; True additionally the FFN with the GELU and the
-    gated residual update in the GEMM's epilogue (10-15 % slower than the tuned hipBLASLt kernels at those shapes)."""
+    gated residual update in the GEMM's epilogue (10-15 % slower than the tuned hipBLASLt kernels at those shapes).
+
+    A layer that `CausalWanModel.pack_linear8` has laid out in 8-bit blocks runs on those (linear8.linear8), whatever own_gemm
+    says; with gradients enabled it is the 16-bit layer."""
 
     def __init__(self, own_gemm=False):
         self.own_gemm = own_gemm is True
         self.own_square = own_gemm is True or own_gemm == "auto"
 
     def linear(self, x, linear):
-        """nn.Linear forward for inference: the own kernel for the block's square projections, else the library."""
+        """nn.Linear forward for inference: 8-bit blocks where the layer has them, the own kernel for the block's square projections,
+        else the library."""
+        w8 = _packed8(linear)
+        if w8 is not None:
+            return _l8.linear8(x, w8, linear.bias)
         w = linear.weight
         if (self.own_square and not torch.is_grad_enabled() and w.shape[0] <= 2048 and w.shape[1] <= 2048 and x.dim() == 3
                 and _lin.supported(x, w)):
@@ -91,6 +99,9 @@ class HipAttentionOps:
         """GELU(tanh)(x W^T + b) with the activation applied in the GEMM's epilogue (hipBLASLt through
         torch's addmm-with-activation); the reference runs Linear and nn.GELU(approximate='tanh') apart
         (model.py:648-650)."""
+        w8 = _packed8(linear)
+        if w8 is not None:
+            return _l8.linear8(x, w8, linear.bias, epilogue="gelu_tanh")
         if self.own_gemm and _lin.supported(x, linear.weight):
             return _lin.linear(x, linear.weight, linear.bias, epilogue="gelu_tanh")
         out = torch._addmm_activation(linear.bias, x.reshape(-1, x.shape[-1]), linear.weight.t(), use_gelu=True)
@@ -99,9 +110,17 @@ class HipAttentionOps:
     def linear_gate_residual(self, x, h, linear, gate):
         """x + linear(h) * gate, in place into x (the FFN's second half and the block's last residual update,
         causal_model.py:1203-1204)."""
+        w8 = _packed8(linear)
+        if w8 is not None:
+            return _l8.linear8(h, w8, linear.bias, epilogue="gate_residual", res=x, gate=gate)
         if self.own_gemm and _lin.supported(h, linear.weight):
             return _lin.linear(h, linear.weight, linear.bias, epilogue="gate_residual", res=x, gate=gate)
         return self.gate_residual(x, linear(h), gate)
+
+
+def _packed8(layer):
+    """The 8-bit form that `CausalWanModel.pack_linear8` has given a layer, None without one or where gradients are wanted."""
+    return None if torch.is_grad_enabled() else getattr(layer, "weight8", None)
 
 
 def _env_int(name, default):
@@ -285,18 +304,22 @@ class CausalWanSelfAttention(nn.Module):
         self.norm_k = WanRMSNorm(dim, eps=eps)
         self._rope = None
         self._qkv = None
+        self.qkv8 = None           # (the three projections' weight in 8-bit blocks, their bias): CausalWanModel.pack_linear8
 
     def _project_qkv(self, x):
         """q, k, v projections as one GEMM over the concatenated weights (the parameters stay the reference's
         three Linear layers; the concatenation is rebuilt when one of them changes).  The three results are
         column slices of one [B, S, 3C] tensor, which the prologue reads through its row stride."""
+        c = self.dim
+        if self.qkv8 is not None:
+            y = _l8.linear8(x, *self.qkv8)
+            return y[..., :c], y[..., c:2 * c], y[..., 2 * c:]
         ws = (self.q.weight, self.k.weight, self.v.weight)
         key = tuple((w.data_ptr(), w._version) for w in ws) + (x.dtype, x.device)
         if self._qkv is None or self._qkv[0] != key:
             with torch.no_grad():
                 self._qkv = (key, torch.cat(ws, 0).contiguous(), torch.cat((self.q.bias, self.k.bias, self.v.bias), 0).contiguous())
         y = torch.nn.functional.linear(x, self._qkv[1], self._qkv[2])
-        c = self.dim
         return y[..., :c], y[..., c:2 * c], y[..., 2 * c:]
 
     def forward(self, x, grid, kv_cache, current_start=0):
@@ -417,7 +440,7 @@ class CausalWanAttentionBlock(nn.Module):
         if getattr(ops, "own_gemm", False):
             x = ops.linear_gate_residual(x, h, self.ffn[2], e[5])
             return x, ops.ln_modulate(x, next_mod[0], next_mod[1], self.eps)
-        return ops.gate_residual_ln(x, self.ffn[2](h), e[5], self.eps, scale=next_mod[0], shift=next_mod[1])
+        return ops.gate_residual_ln(x, ops.linear(h, self.ffn[2]), e[5], self.eps, scale=next_mod[0], shift=next_mod[1])
 
 
 class CausalHead(nn.Module):
@@ -481,6 +504,22 @@ class CausalWanModel(nn.Module):
                     nn.init.normal_(m.weight, std=.02)
         if zero_head:
             nn.init.zeros_(self.head.head.weight)
+
+    @torch.no_grad()
+    def pack_linear8(self, on=True):
+        """Lays the blocks' linear layers out in 8-bit blocks of 128 (linear8.pack): self-attention's q, k, v as one weight, the
+        output projections, cross-attention's q, and the feed-forward.  Passes without gradients then run them on 8-bit products
+        (weights and activations as e4m3, fp32 sums).  The 16-bit weights stay; call it again after they change, `on=False`
+        goes back to them.  Returns the model."""
+        for b in self.blocks:
+            sa, ca = b.self_attn, b.cross_attn
+            sa.qkv8 = None
+            if on:
+                ws = torch.cat((sa.q.weight, sa.k.weight, sa.v.weight), 0)
+                sa.qkv8 = (_l8.pack(ws, transposed=False), torch.cat((sa.q.bias, sa.k.bias, sa.v.bias), 0))
+            for layer in (sa.o, ca.q, ca.o, b.ffn[0], b.ffn[2]):
+                layer.weight8 = _l8.pack(layer.weight, transposed=False) if on else None
+        return self
 
     def _patchify(self, x):
         """[B, C, F, H, W] -> tokens [B, F*h*w, dim]; same arithmetic as the strided Conv3d."""
