@@ -337,8 +337,8 @@ int sfm_linear(const sfm_linear_desc* desc, const void* x, const void* w, const 
  *            transposed weight [K, N] (the same values), for the product with the output's gradient.
  * data and scale are 16-byte aligned.
  *
- * sfm_quantize8: data / scale of x [rows, K] (rows x_stride apart, any alignment).  colsum (NULL or float [ceil(rows / 128)][K])
- *   receives the column sums of each 128 rows; y (NULL or [rows, K]): GELU (tanh) of x, rounded once.
+ * sfm_quantize8: data / scale of x [rows, K] (rows x_stride apart, any alignment).  colsum (NULL or float [ceil(rows / 32)][K])
+ *   receives the column sums of each 32 rows; y (NULL or [rows, K]): GELU (tanh) of x, rounded once.
  *   data NULL: nothing is quantised.
  * sfm_dequantize8: the values, rounded to the dtype (exact in bf16 and fp32 but for fp32-subnormal ones; fp16 saturates at 65504).
  * sfm_pack8: a weight's data and scale, and data_t and scale_t unless both are NULL. */

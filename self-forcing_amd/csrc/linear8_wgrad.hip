@@ -448,7 +448,7 @@ size_t wgrad8_workspace_bytes(int64_t M, int N, int K, bool bias) {
     const int s = wgrad_plan(M, N, K).splits;
     size_t b = s > 1 ? (size_t)s * N * K * sizeof(float) : 0;
     b = (b + 255) / 256 * 256;
-    return b + (bias ? (size_t)((M + kBlock8 - 1) / kBlock8) * N * sizeof(float) : 0);
+    return b + (bias ? (size_t)((M + kColRows8 - 1) / kColRows8) * N * sizeof(float) : 0);
 }
 
 int launch_wgrad8(int dtype, int64_t M, int N, int K, const void* dy, int64_t dy_stride, const void* x8, const void* xscale, void* dw,
@@ -502,7 +502,7 @@ int launch_wgrad8(int dtype, int64_t M, int N, int K, const void* dy, int64_t dy
         if (rc) return rc;
         colsum = cs;
     }
-    return launch_sum_parts(dtype, groups, N, 1, colsum, dbias, nullptr, st);
+    return launch_sum_parts(dtype, (M + kColRows8 - 1) / kColRows8, N, 1, colsum, dbias, nullptr, st);
 }
 
 }  // namespace sfm

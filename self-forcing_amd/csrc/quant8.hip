@@ -9,23 +9,24 @@
 namespace sfm {
 namespace {
 
-// One workgroup: 128 rows of one block column.  A thread holds 8 neighbouring elements of the rows r0 + 16 i, all eight
-// rows' loads in flight together; the 16 lanes of a row find the block's maximum by shuffles.  The 128 scale bytes meet in
-// LDS and leave as 32 words.
-//   GELU: y = gelu_tanh(x) is stored besides.   data NULL: nothing is quantised (only the sums are wanted).
-//   colsum: float [row groups][K], the sums over the group's rows (a bias gradient's first half).
+// One workgroup: 32 rows of one block column.  A thread holds 8 neighbouring elements of the rows r0 and r0 + 16; the 16 lanes of a row
+// find the block's maximum by rotations.  Small workgroups keep more of them on their way: with 128 rows, whose scales would be
+// whole words, 4680 x 5120 takes 22 us (16; 4.5 TB/s) and GELU's forward at 4680 x 8960 48 (39; 5.4 TB/s).
+//   GELU: y = gelu_tanh(x) is stored besides.   data NULL: nothing is quantised.
+//   colsum: float [ceil(rows / 32)][K], the sums over the workgroup's rows (a bias gradient's first half).
 template <typename T, bool GELU>
-__global__ __launch_bounds__(256) void quantize8_kernel(const void* x, int64_t xs, int64_t rows, int K, uint8_t* data,
-                                                        uint8_t* scale, void* y, int64_t ys, float* colsum) {
-    __shared__ __attribute__((aligned(16))) uint8_t sc[kBlock8];
+__global__ __launch_bounds__(256) void quantize8_kernel(const void* x, int64_t xs, int64_t rows, int K, uint8_t* data, uint8_t* scale,
+                                                        void* y, int64_t ys, float* colsum) {
+    constexpr int NR = 2;
+    __shared__ uint8_t sc[kColRows8];
     __shared__ __attribute__((aligned(16))) float cs[16][kBlock8];
-    const int64_t groups = gridDim.x;
+    const int64_t groups = (rows + kBlock8 - 1) / kBlock8;
     const int kb = blockIdx.y, l16 = threadIdx.x & 15, r0 = threadIdx.x >> 4;
     const int c = kb * kBlock8 + l16 * 8;
-    const int64_t kp = pad8(K), row0 = (int64_t)blockIdx.x * kBlock8;
-    float v[8][8];
+    const int64_t kp = pad8(K), row0 = (int64_t)blockIdx.x * kColRows8;
+    float v[NR][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < NR; ++i) {
         const int64_t r = row0 + r0 + 16 * i;
         if (r < rows) {
             load_part8<T>(x, r * xs, c, K, v[i]);
@@ -40,24 +41,23 @@ __global__ __launch_bounds__(256) void quantize8_kernel(const void* x, int64_t x
         for (int e = 0; e < 8; ++e) {
             s[e] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s[e] += v[i][e];
+            for (int i = 0; i < NR; ++i) s[e] += v[i][e];
         }
         V8<float>::store(&cs[r0][0], l16 * 8, s);
     }
     if (data != nullptr) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < NR; ++i) {
             const int64_t r = row0 + r0 + 16 * i;
             u32x2 q;
             const int s = quantize_block8(v[i], &q);
             if (r < rows) *(u32x2*)(data + r * kp + c) = q;
-            const int rr = r0 + 16 * i;
-            if (l16 == 0) sc[((rr & 31) << 2) + (rr >> 5)] = (uint8_t)(s + 127);
+            if (l16 == 0) sc[r0 + 16 * i] = (uint8_t)(s + 127);
         }
     }
     if (GELU) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < NR; ++i) {
             const int64_t r = row0 + r0 + 16 * i;
             if (r < rows) {
 #pragma unroll
@@ -67,8 +67,7 @@ __global__ __launch_bounds__(256) void quantize8_kernel(const void* x, int64_t x
         }
     }
     __syncthreads();
-    if (data != nullptr && threadIdx.x < 32)
-        ((uint32_t*)scale)[(kb * groups + blockIdx.x) * 32 + threadIdx.x] = ((const uint32_t*)sc)[threadIdx.x];
+    if (data != nullptr && threadIdx.x < kColRows8) scale[scale_at8(row0 + threadIdx.x, kb, groups)] = sc[threadIdx.x];
     if (colsum != nullptr && threadIdx.x < kBlock8 && kb * kBlock8 + (int)threadIdx.x < K) {
         float s = 0.f;
 #pragma unroll
@@ -204,13 +203,11 @@ __global__ __launch_bounds__(256) void pack8_kernel(const void* w, int64_t ws, i
 
 template <typename T>
 int quantize_t(int64_t rows, int K, const void* x, int64_t xs, void* data, void* scale, void* y, int64_t ys, float* colsum, hipStream_t st) {
-    const dim3 grid((unsigned)((rows + kBlock8 - 1) / kBlock8), (unsigned)blocks8(K));
+    const dim3 grid((unsigned)((rows + kColRows8 - 1) / kColRows8), (unsigned)blocks8(K));
     if (y != nullptr)
-        hipLaunchKernelGGL((quantize8_kernel<T, true>), grid, dim3(256), 0, st, x, xs, rows, K, (uint8_t*)data,
-                           (uint8_t*)scale, y, ys, colsum);
+        hipLaunchKernelGGL((quantize8_kernel<T, true>), grid, dim3(256), 0, st, x, xs, rows, K, (uint8_t*)data, (uint8_t*)scale, y, ys, colsum);
     else
-        hipLaunchKernelGGL((quantize8_kernel<T, false>), grid, dim3(256), 0, st, x, xs, rows, K, (uint8_t*)data,
-                           (uint8_t*)scale, nullptr, 0, colsum);
+        hipLaunchKernelGGL((quantize8_kernel<T, false>), grid, dim3(256), 0, st, x, xs, rows, K, (uint8_t*)data, (uint8_t*)scale, y, ys, colsum);
     return launched8("sfm_quantize8");
 }
 

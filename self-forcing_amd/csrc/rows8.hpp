@@ -65,6 +65,7 @@ typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
 template <typename T> constexpr bool kWide = std::is_same<T, float>::value;      // 4-byte elements
 
 constexpr int kBlock8 = 128;
+constexpr int kColRows8 = 32;          // rows of one partial column sum (sfm_quantize8)
 
 __host__ __device__ inline int blocks8(int64_t k) { return (int)((k + kBlock8 - 1) / kBlock8); }
 __host__ __device__ inline int64_t pad8(int64_t k) { return (k + kBlock8 - 1) / kBlock8 * kBlock8; }
@@ -226,7 +227,7 @@ int launch_pack8(int dtype, int N, int K, const void* w, int64_t ws, void* data,
 constexpr int kFewRows8 = SFM_LINEAR8_FEW_ROWS;
 int launch_linear8(const sfm_linear8_desc& d, const void* x, int64_t x_stride, const void* x8, const void* xscale, const void* w8,
                    const void* wscale, const void* bias, const void* res, const void* gate, void* out, hipStream_t stream);
-// linear8_wgrad.hip; `colsum`: column sums of dy by groups of 128 rows where a quantisation has formed them, else null
+// linear8_wgrad.hip; `colsum`: column sums of dy by kColRows8 rows where a quantisation has formed them, else null
 size_t wgrad8_workspace_bytes(int64_t M, int N, int K, bool bias);
 int launch_wgrad8(int dtype, int64_t M, int N, int K, const void* dy, int64_t dy_stride, const void* x8, const void* xscale, void* dw,
                   void* dbias, const float* colsum, void* workspace, hipStream_t st);

@@ -1589,7 +1589,7 @@ static Linear8BwdLayout linear8_bwd_layout(int64_t M, int32_t N, int32_t K) {
     l.data = 0;
     l.scale = up((size_t)M * SFM_PAD8(N));
     l.colsum = l.scale + up((size_t)SFM_ROWS8_SCALE_BYTES(M, N));
-    l.rest = l.colsum + up((size_t)((M + 127) / 128) * N * sizeof(float));
+    l.rest = l.colsum + up((size_t)((M + 31) / 32) * N * sizeof(float));
     l.total = l.rest + wgrad8_workspace_bytes(M, N, K, false);
     return l;
 }

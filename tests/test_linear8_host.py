@@ -101,7 +101,7 @@ def test_forward_refusals():
 def test_gradient_refusals():
     lib = L.load()
     n = C.c_size_t(0)
-    assert lib.sfm_linear8_wgrad_workspace_bytes(300, 64, 128, C.byref(n)) == 0 and n.value >= 3 * 64 * 4
+    assert lib.sfm_linear8_wgrad_workspace_bytes(300, 64, 128, C.byref(n)) == 0 and n.value >= 10 * 64 * 4
     need = n.value
     _rc(lib.sfm_linear8_wgrad_workspace_bytes(300, 64, 128, None), -1, "bytes")
     _rc(lib.sfm_linear8_wgrad_workspace_bytes(0, 64, 128, C.byref(n)), -3, "rows=")
