@@ -49,7 +49,7 @@ __device__ __forceinline__ float l8_tail(float sum, float bias, float res, float
     return EPI == SFM_EPI_GELU_TANH ? v * gelu_gate<false>(v) : EPI == SFM_EPI_GATE_RESIDUAL ? res + v * gate : v;
 }
 
-// four neighbouring channels c.. of a row: bias and epilogue on the fp32 sums, rounded once and stored
+// four neighbouring channels c.. of a row of 16-bit values
 template <class E>
 __device__ __forceinline__ void l8_get4(const L8Args& p, const uint16_t* s, int c, float* d) {
     if (c + 4 <= p.N) {
@@ -67,6 +67,7 @@ __device__ __forceinline__ f32x4 l8_bias4(const L8Args& p, int c) {
     if (p.bias != nullptr) l8_get4<E>(p, p.bias + c, c, b);
     return f32x4{b[0], b[1], b[2], b[3]};
 }
+// four neighbouring channels of a row: bias and epilogue on the fp32 sums, rounded once and stored
 template <class E, int EPI>
 __device__ __forceinline__ void l8_finish4(const L8Args& p, int64_t row, int c, const float* acc, f32x4 b) {
     if (row >= p.M || c >= p.N) return;
@@ -96,9 +97,9 @@ __device__ __forceinline__ i32x8 l8_load32(const uint8_t* p) {
 }
 
 // Any size: a workgroup of W waves owns 16 MT rows x 16 NT channels, its waves share the block columns (wave w takes w,
-// w + W, ...) and their sums meet in LDS in a fixed order.  Many waves hide the loads: with the next block column's operands held besides,
-// 128 x 1536 -> 8960 takes 26 us against 18.  Operands come from memory straight into registers, 32 bytes a
-// lane of one row: 4 lanes take a row's block of 128 bytes, a whole line.
+// w + W, ...) and their sums meet in LDS in a fixed order.  Operands come from memory straight into registers, 32 bytes a lane of one
+// row: 4 lanes take a row's block of 128 bytes, a whole line.  Many waves hide the loads: with the next block column's operands held
+// besides, 128 x 1536 -> 8960 takes 26 us against 18.
 template <class E, int EPI, int MT, int NT, int W>
 __global__ __launch_bounds__(64 * W) void l8_direct_kernel(L8Args p) {
     __shared__ f32x4 part[W][MT * NT][64];
@@ -286,27 +287,14 @@ __device__ __forceinline__ void l8_load_lds(const void* base, uint32_t off, uint
     else
         asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_addr), "v"(off), "s"(base), "n"(ADD) : "memory", "m0", "scc");
 }
-// waits until at most N of this wave's loads are outstanding (they complete in order), then the barrier
+// waits until at most N of this wave's requests are outstanding (they complete in order) and its LDS reads are done, then the barrier
 template <int N>
-__device__ __forceinline__ void l8_wait_stage() { asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void l8_wait_stage() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 template <int OFF>
 __device__ __forceinline__ u32x4 l8_lds_read16(uint32_t addr) {
-    u32x4 r;
-    asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(r) : "v"(addr), "n"(OFF));
-    return r;
+    return *(const __attribute__((address_space(3))) u32x4*)(size_t)(addr + OFF);
 }
-__device__ __forceinline__ uint32_t l8_lds_read4(uint32_t addr) {
-    uint32_t r;
-    asm volatile("ds_read_b32 %0, %1" : "=v"(r) : "v"(addr));
-    return r;
-}
-template <int NF>
-__device__ __forceinline__ void l8_wait_frags(u32x4 (&f)[NF], uint32_t& xe) {
-    static_assert(NF == 16 || NF == 12, "two pieces of 4 weight blocks + 4 or 2 activation blocks");
-    asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(f[0]), "+v"(f[1]), "+v"(f[2]), "+v"(f[3]), "+v"(f[4]), "+v"(f[5]), "+v"(f[6]), "+v"(f[7]),
-                 "+v"(f[8]), "+v"(f[9]), "+v"(f[10]), "+v"(f[11]), "+v"(xe));
-    if constexpr (NF == 16) asm volatile("" : "+v"(f[12]), "+v"(f[13]), "+v"(f[14]), "+v"(f[15]));
-}
+__device__ __forceinline__ uint32_t l8_lds_read4(uint32_t addr) { return *(const __attribute__((address_space(3))) uint32_t*)(size_t)addr; }
 __device__ __forceinline__ i32x8 l8_join(u32x4 a, u32x4 b) {
     return __builtin_shufflevector(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), 0, 1, 2, 3, 4, 5, 6, 7);
 }
@@ -343,8 +331,8 @@ __device__ __forceinline__ void l8_fetch_all(std::integer_sequence<int, J...>, u
                                              uint32_t b1) {
     (l8_fetch<TB, J>(fn, a0, a1, b0, b1), ...);
 }
-// One k step: 4 x TB matrix instructions on the operand set fc.  Behind each of them go some of the
-// LDS reads of the next set fn and of NLOAD requests (from quarter Q0 on), so that their issue runs under the matrix pipe.
+// One k step: 4 x TB matrix instructions on the operand set fc.  Behind each of them go some of the LDS reads of the next set fn and of
+// NLOAD requests (from quarter Q0 on), so that their issue runs under the matrix pipe.
 template <int TB, bool FETCH, int NLOAD, int Q0, int I>
 __device__ __forceinline__ void l8_kone(f32x16 (&acc)[4][TB], const u32x4 (&fc)[8 + 2 * TB], u32x4 (&fn)[8 + 2 * TB], uint32_t a0, uint32_t a1,
                                         uint32_t b0, uint32_t b1, int we, int xe, const L8Src<TB>& src, uint32_t slot, uint32_t scale_addr) {
@@ -371,14 +359,14 @@ __device__ __forceinline__ void l8_kstep(std::integer_sequence<int, I...>, f32x1
     (l8_kone<TB, FETCH, NLOAD, Q0, I>(acc, fc, fn, a0, a1, b0, b1, we, xe, src, slot, scale_addr), ...);
 }
 
-// sums to memory: CB x TB blocks of 32 channels x 32 rows from channel c0, row r0 on.  Lane (m, hf) of block (cb, tb) holds row
+// sums to memory: 4 x TB blocks of 32 channels x 32 rows from channel c0, row r0 on.  Lane (m, hf) of block (cb, tb) holds row
 // 32 tb + m, channels 8 g + 4 hf + (i & 3), i = 4 g + ..  One block after the other, each with addresses of its own: formed for all
 // blocks together they would not fit beside the sums.
-template <class E, int EPI, int TB, int CB>
+template <class E, int EPI, int TB>
 __device__ __forceinline__ void l8_store(const L8Args& p, const f32x16 (&acc)[4][TB], int c0, int64_t r0, int m, int hf) {
-    if (c0 + 32 * CB <= p.N && r0 + 32 * TB <= p.M) {          // whole: 16-byte stores
+    if (c0 + 128 <= p.N && r0 + 32 * TB <= p.M) {          // whole: 16-byte stores
 #pragma unroll
-        for (int cb = 0; cb < CB; ++cb) {
+        for (int cb = 0; cb < 4; ++cb) {
             const int cbase = c0 + 32 * cb;
             float bia[16];
 #pragma unroll
@@ -424,7 +412,7 @@ __device__ __forceinline__ void l8_store(const L8Args& p, const f32x16 (&acc)[4]
         return;
     }
 #pragma unroll
-    for (int cb = 0; cb < CB; ++cb)
+    for (int cb = 0; cb < 4; ++cb)
 #pragma unroll
         for (int tb = 0; tb < TB; ++tb) {
             int own = 32 * tb + m;
@@ -492,8 +480,8 @@ __device__ __forceinline__ void l8_tile(const L8Args& p, int64_t m0, int n0) {
     const int xsh = TB == 4 ? 0 : 16 * wm;
 
     // Quarter q of stage s lives in slot (NQ s + q) % 9.  Iteration s multiplies stage s in two k steps; the operands of a step are
-    // read during the step before.  After its first step a wave has read all of stage s: it waits for its own loads of stage
-    // s + 1, meets the others, and requests stage s + kAhead into the slots that are free (TB = 4: its first quarter has a slot
+    // read during the step before.  After its first step a wave has read all of stage s: it waits for that and for its own loads
+    // of stage s + 1, meets the others, and requests stage s + kAhead into the slots that are free (TB = 4: its first quarter has a slot
     // already before that).
     const int nstage = p.nkb;
     auto whole_stage = [&](int g) {
@@ -512,7 +500,7 @@ __device__ __forceinline__ void l8_tile(const L8Args& p, int64_t m0, int n0) {
     else l8_wait_stage<0>();
     u32x4 f0[8 + 2 * TB], f1[8 + 2 * TB];
     uint32_t hs = 0;                                           // slot of the first quarter of the stage being multiplied
-    uint32_t xe0 = l8_lds_read4(ks), xe1;
+    uint32_t xe0 = l8_lds_read4(ks);                           // this lane's scales of the stage
     {
         const uint32_t a = wn * kSlot, b = bq * kSlot + bo;
         l8_fetch_all<TB>(std::make_integer_sequence<int, 8 + 2 * TB>{}, f0, kp4[0] + a, kp4[1] + a, kp4[0] + b, kp4[1] + b);
@@ -525,21 +513,20 @@ __device__ __forceinline__ void l8_tile(const L8Args& p, int64_t m0, int n0) {
         const uint32_t sa = l8_wrap(hs + wn) * kSlot, sb = l8_wrap(hs + bq) * kSlot + bo;                                      \
         const uint32_t ns = l8_wrap(hs + (NQ * kAhead) % kRing);                                                               \
         const uint32_t sc = lds0 + kScaleAt + (uint32_t)((s + kAhead) & 3) * kScaleSlot;                                       \
-        l8_wait_frags(f0, xe0);                                                                                                \
+        __builtin_amdgcn_sched_barrier(0);                                                                                     \
         const int wec = (int)(wword >> (8 * (s & 3))) & 0xff, xe = (int)(xe0 >> xsh);                                          \
         if (!LAST) wword = wsp[(s + 1) >> 2];                                                                                  \
         l8_kstep<TB, true, LOAD ? kEarly : 0, 0>(std::make_integer_sequence<int, 4 * TB>{}, acc, f0, f1, kp4[2] + sa, kp4[3] + sa, \
                                                            kp4[2] + sb, kp4[3] + sb, wec, xe, src, ns, sc);                    \
-        l8_wait_frags(f1, xe0);                                /* this wave has read all of the stage */                       \
+        __builtin_amdgcn_sched_barrier(0);                                                                                     \
         if (!LAST) {                                                                                                           \
             l8_wait_stage<WAIT>();                                                                                             \
             hs = l8_wrap(hs + NQ);                                                                                             \
             const uint32_t na = l8_wrap(hs + wn) * kSlot, nb = l8_wrap(hs + bq) * kSlot + bo;                                  \
-            xe1 = l8_lds_read4(ks + (uint32_t)((s + 1) & 3) * kScaleSlot);                                                     \
+            xe0 = l8_lds_read4(ks + (uint32_t)((s + 1) & 3) * kScaleSlot);                                                     \
             l8_kstep<TB, true, LOAD ? kLoads - kEarly : 0, kEarly / 4>(std::make_integer_sequence<int, 4 * TB>{}, acc, f1, f0, \
                                                                                  kp4[0] + na, kp4[1] + na, kp4[0] + nb, kp4[1] + nb, wec, xe, src, ns, sc); \
             if (LOAD) advance();                                                                                               \
-            xe0 = xe1;                                                                                                         \
             ++s;                                                                                                               \
         } else {                                                                                                               \
             l8_kstep<TB, false, 0, 0>(std::make_integer_sequence<int, 4 * TB>{}, acc, f1, f0, 0, 0, 0, 0, wec, xe, src, 0, 0); \
@@ -550,7 +537,7 @@ __device__ __forceinline__ void l8_tile(const L8Args& p, int64_t m0, int n0) {
     if (nstage >= 2) L8_ITER(false, 0, false)
     L8_ITER(false, 0, true)
 #undef L8_ITER
-    l8_store<E, EPI, TB, 4>(p, acc, n0 + wn * 128, m0 + wm * 32 * TB, m, hf);
+    l8_store<E, EPI, TB>(p, acc, n0 + wn * 128, m0 + wm * 32 * TB, m, hf);
 }
 
 // Every eighth workgroup shares an XCD: each XCD gets a contiguous run of the patch order.  With TB = 4 a last strip of at most 128
