@@ -3,11 +3,13 @@ RMSNorm, GELU); counterparts of the eager chains in wan/modules/causal_model.py:
 wan/modules/model.py:462-478.  [B, L, C] tensors, modulation rows [B, F, 1, C] (one per latent frame)."""
 import ctypes
 import functools
+import threading
+import weakref
 
 import torch
 
 from . import lib as _l
-from .monarch_attn import _DT, _on_device, _stream
+from .monarch_attn import _DT, _on_device, _raw_stream, _stream
 
 _HALF = (torch.float16, torch.bfloat16)
 
@@ -52,7 +54,7 @@ def _mod(e, x):
     """[B, F, 1, C] (or [B, F, C]) modulation tensor -> (tensor, frame stride, rows per frame)."""
     B, L, C = x.shape
     _like("modulation", e, x)
-    if e.numel() == 0 or e.numel() % (B * C):
+    if e.numel() == 0 or x.numel() == 0 or e.numel() % (B * C):
         raise ValueError("modulation: expected [B, F, 1, C] rows")
     e = e.reshape(B, -1, C)
     if e.stride(2) != 1 or (B > 1 and e.stride(0) != e.shape[1] * e.stride(1)):
@@ -142,11 +144,42 @@ def _ln_bwd(dy, x, kept, weight, scale, ms, group, eps, w_shape, b_shape, want_d
     return dx, dw, db
 
 
+_eager_graphs, _eager_lock = weakref.WeakSet(), threading.Lock()
+
+
+def _noted(ctx, device):
+    """Called by the forwards: remembers a graph recorded on the default stream for as long as it lives."""
+    if _raw_stream(device.index) == 0:
+        with _eager_lock:
+            _eager_graphs.add(ctx)
+
+
+def _leaves(ctx):
+    return [n.variable for n, _ in ctx.next_functions if hasattr(n, "variable")]
+
+
+def _check_captured(ctx):
+    """Autograd sums a leaf's gradient on the stream that its oldest living graph was recorded on.  A captured backward whose leaf
+    belongs to a living graph of the default stream would make that stream part of the capture, which HIP does not allow and which
+    ends the process: refused before anything reaches the leaf."""
+    mine = _leaves(ctx)
+    with _eager_lock:
+        others = [o for o in _eager_graphs if o is not ctx]
+    if any(a is b for o in others for a in _leaves(o) for b in mine):
+        raise RuntimeError("a backward cannot be captured while a graph of the same leaves, recorded on the default stream, lives: drop "
+                           "its outputs first, or record it on another stream")
+
+
 def _once(backward):
     """A backward without a derivative of its own: `once_differentiable`, but for calls that build no graph, which it would only
     slow down (a third of a small call's time)."""
     guarded = torch.autograd.function.once_differentiable(backward)
-    return lambda ctx, *grads: (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    def run(ctx, *grads):
+        if torch.cuda.is_current_stream_capturing():
+            _check_captured(ctx)
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return run
 
 
 class _LnFn(torch.autograd.Function):
@@ -162,6 +195,7 @@ class _LnFn(torch.autograd.Function):
             sc, sh, ms, rpf = _vec("weight", a, x), _vec("bias", b, x), 0, x.shape[0] * x.shape[1]
             mod = (None, None, 0, 1, sc.data_ptr(), sh.data_ptr())
         ctx.cfg = (modulate, eps, checkpoint8, ms, rpf, a.shape, b.shape)
+        _noted(ctx, x.device)
         if checkpoint8:
             y, *kept = _ln_keep8(x, mod, eps)
             ctx.save_for_backward(sc, *kept)
@@ -240,6 +274,7 @@ class _GeluFn(torch.autograd.Function):
     def forward(ctx, x, checkpoint8):
         y, data, scale = _gelu(x, checkpoint8)
         ctx.checkpoint8 = checkpoint8
+        _noted(ctx, x.device)
         ctx.save_for_backward(*((data, scale) if checkpoint8 else (x,)))
         return y
 

@@ -196,9 +196,13 @@ __global__ __launch_bounds__(256) void wgrad8_kernel(WgradArgs p) {
 
 // Large tiles: 256 x 256 channels, a wave 128 x 128 (16 matrix instructions 32x32x16 per 16 rows, 256 accumulator registers, one wave
 // per SIMD), 32 rows per step, two LDS buffers.  A thread stages one row: four 16-byte pieces of dy and two of x8, whose 16 values
-// become 32 bytes.  The rows of a step are requested four steps ahead into registers (three sets in turn), written to LDS
+// become 32 bytes.  The rows of a step are requested five steps ahead into registers (four sets in turn), written to LDS
 // a step ahead, behind the matrix instructions of the step's first 16 rows; the operands of the next 16 rows are read behind those
 // of the 16 before.  EDGE: a row of dy ends inside a piece of 8 channels of this tile.
+//
+// Bound by the matrix pipe: 4680 x 1536 x 8960 has 129 GFLOP, 80 us at the 1.6 PFLOP/s of a large bf16 product here, and takes 133 us
+// (0.97 PFLOP/s; a library product of 16-bit operands of this shape 158 us); its 210 tiles leave 46 of 256 compute units idle, which
+// alone makes 80 us 98.  Requests three steps ahead: 150 us.
 template <class E, bool EDGE>
 __device__ __forceinline__ void wgrad8_tile(const WgradArgs& p, int n0, int kb, int64_t s0, int64_t s1, int split) {
     extern __shared__ __attribute__((aligned(256))) char w8_lds[];      // [buffer][dy tile | x tile]

@@ -1516,12 +1516,25 @@ static int check_out8(const sfm_linear8_desc* d, const void* out, const char* na
     set_error("out overlaps %s", name);
     return SFM_ERR_RANGE;
 }
+// The same for 16-bit rows of n, stride apart: out's rows and these may be columns of the same rows.
+static int check_out8(const sfm_linear8_desc* d, const void* out, const char* name, const void* p, int64_t stride, int64_t n) {
+    const int64_t s = stride * 2, ahead = ((const char*)p - (const char*)out) % s, at = ahead < 0 ? ahead + s : ahead;
+    if (stride == d->out_stride && at >= 2 * (int64_t)d->N && at + 2 * n <= s) return SFM_OK;
+    return check_out8(d, out, name, p, ((size_t)(d->M - 1) * stride + n) * 2);
+}
+
+// a value of res is read by the thread that stores it: res is out itself, or apart from it
+static int check_res8(const sfm_linear8_desc* d, const void* res, const void* out) {
+    if (d->epilogue != SFM_EPI_GATE_RESIDUAL || (res == out && (d->res_stride == d->out_stride || d->M == 1))) return SFM_OK;
+    return check_out8(d, out, "res", res, d->res_stride, d->N);
+}
 
 int sfm_linear8(const sfm_linear8_desc* d, const void* x8, const void* xscale, const void* w8, const void* wscale, const void* bias,
                 const void* res, const void* gate, void* out, void* stream) {
     int rc = check_linear8(d, w8, wscale, bias, res, gate, out);
     if (rc || (rc = check_blocks("x8", x8, xscale))) return rc;
-    if ((rc = check_out8(d, out, "x8", x8, (size_t)d->M * SFM_PAD8(d->K))) || (rc = check_out8(d, out, "w8", w8, (size_t)d->N * SFM_PAD8(d->K)))) return rc;
+    if ((rc = check_out8(d, out, "x8", x8, (size_t)d->M * SFM_PAD8(d->K))) || (rc = check_out8(d, out, "w8", w8, (size_t)d->N * SFM_PAD8(d->K))) ||
+        (rc = check_res8(d, res, out))) return rc;
     const bool gr = d->epilogue == SFM_EPI_GATE_RESIDUAL;
     return launch_linear8(*d, nullptr, 0, x8, xscale, w8, wscale, bias, gr ? res : nullptr, gr ? gate : nullptr, out, (hipStream_t)stream);
 }
@@ -1541,7 +1554,7 @@ int sfm_linear8_fwd(const sfm_linear8_desc* d, const void* x, int64_t x_stride, 
         if ((rc = check_out8(d, out, "x8", data, (size_t)d->M * SFM_PAD8(d->K)))) return rc;
     }
     if ((rc = check_out8(d, out, "w8", w8, (size_t)d->N * SFM_PAD8(d->K))) ||
-        (rc = check_out8(d, out, "x", x, ((size_t)(d->M - 1) * x_stride + d->K) * 2))) return rc;
+        (rc = check_out8(d, out, "x", x, x_stride, d->K)) || (rc = check_res8(d, res, out))) return rc;
     const bool gr = d->epilogue == SFM_EPI_GATE_RESIDUAL;
     if (keep && (rc = launch_quantize8(d->dtype, d->M, d->K, x, x_stride, data, scale, nullptr, 0, nullptr, (hipStream_t)stream))) return rc;
     return launch_linear8(*d, x, x_stride, data, scale, w8, wscale, bias, gr ? res : nullptr, gr ? gate : nullptr, out, (hipStream_t)stream);

@@ -17,7 +17,7 @@ import functools
 import torch
 
 from . import lib as _l
-from .block_ops import _HALF, _like, _mod, _once, _row_stride, _rows, _written
+from .block_ops import _HALF, _like, _mod, _noted, _once, _row_stride, _rows, _written
 from .monarch_attn import _DT, _on_device, _stream
 
 _EPI = {"none": _l.EPI_NONE, "gelu_tanh": _l.EPI_GELU_TANH, "gate_residual": _l.EPI_GATE_RESIDUAL}
@@ -200,6 +200,7 @@ class _Linear8Fn(torch.autograd.Function):
             data, scale = x8.data, x8.scale
             _product(x8, w8.data, w8.scale, N, bias, out)
         ctx.cfg = (rows.shape, rows.dtype, w8.shape)
+        _noted(ctx, rows.device)
         ctx.save_for_backward(*((data, scale) if need_w else (None, None)), *((w8.data_t, w8.scale_t) if need_x else (None, None)))
         return out
 

@@ -379,3 +379,51 @@ def test_captured_and_replayed():
         ref = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, r) for a, r in zip(out, ref))
+
+
+@pytest.mark.parametrize("M", [5, 70])
+def test_columns_of_one_buffer(M):
+    """x, res and out side by side in the rows of one buffer are not an overlap; what lies between stays."""
+    buf = randn((1, M, 640), 60, torch.bfloat16).to(DEV)
+    w = l8.pack(randn((96, 256), 61, torch.bfloat16).to(DEV))
+    was = buf.clone()
+    x, res, out = buf[..., :256], buf[..., 256:352], buf[..., 400:496]
+    ref = l8.linear8(x.clone(), w, epilogue="gate_residual", res=res.clone())
+    l8.linear8(x, w, epilogue="gate_residual", res=res, out=out)
+    assert torch.equal(out, ref)
+    assert torch.equal(buf[..., :400], was[..., :400]) and torch.equal(buf[..., 496:], was[..., 496:])
+    l8.linear8(x, w, epilogue="gate_residual", res=res)
+    assert torch.equal(res, ref)
+    for bad in (buf[..., 255:351], buf[..., 257:353]):
+        with pytest.raises(ValueError, match="overlaps"):
+            l8.linear8(x, w, epilogue="gate_residual", res=res, out=bad)
+
+
+def test_a_captured_backward_refuses_leaves_of_a_living_eager_graph():
+    """Refused before a gradient reaches the leaf; with the eager graph dropped the same capture runs and replays."""
+    x, dy = rows((1, 40, 128), 63, torch.bfloat16).to(DEV), randn((1, 40, 64), 64, torch.bfloat16).to(DEV)
+    w = randn((64, 128), 65, torch.bfloat16).to(DEV).requires_grad_()
+
+    def step():
+        return torch.autograd.grad(l8.linear8(x, w), w, dy)[0]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    eager = l8.linear8(x, w)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        y = l8.linear8(x, w)
+        with pytest.raises(RuntimeError, match="same leaves"):
+            torch.autograd.grad(y, w, dy)
+        del y
+    ref = torch.autograd.grad(eager, w, dy)[0]
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ref) and torch.equal(step(), ref)
+        out.zero_()

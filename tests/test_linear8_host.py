@@ -177,3 +177,61 @@ def test_python_entry_points_refuse_before_any_call():
                  lambda: l8.linear8(x, w[0])):
         with pytest.raises(ValueError):
             call()
+
+
+def test_rows_of_one_buffer_overlap_only_where_they_do():
+    """out may be columns of the rows that x or res are columns of; by one column too far, or with other strides, it is refused."""
+    lib = L.load()
+    d = dict(M=8, N=64, K=128, out_stride=256)
+
+    def f(out, xs=256):
+        return lib.sfm_linear8_fwd(C.byref(_desc(**d)), P, xs, None, None, 4 * P, 5 * P, None, None, None, out, None)
+    for out in (P + 2 * 64, P + 2 * 127, P - 2 * 63, P + 2 * (256 - 63), P + 2 * (256 * 7 + 127)):
+        _rc(f(out), -4, "overlaps x")
+    _rc(f(P + 2 * 128, xs=257), -4, "overlaps x")                 # other strides: rows cross
+    for res in (7 * P + 2, 7 * P - 2, 7 * P + 2 * 63, 7 * P + 2 * 256):
+        e = _desc(**d, epilogue=L.EPI_GATE_RESIDUAL, res_stride=256)
+        _rc(lib.sfm_linear8_fwd(C.byref(e), P, 128, None, None, 4 * P, 5 * P, None, res, None, 7 * P, None), -4, "overlaps res")
+    e = _desc(**d, epilogue=L.EPI_GATE_RESIDUAL, res_stride=320)
+    _rc(lib.sfm_linear8_fwd(C.byref(e), P, 128, None, None, 4 * P, 5 * P, None, 7 * P, None, 7 * P, None), -4, "overlaps res")
+
+
+def test_a_captured_backward_refuses_leaves_of_an_eager_graph(monkeypatch):
+    """The rule without a GPU: graphs recorded on the default stream are remembered while they live."""
+    blk = sfa.block_ops
+    stream = [0]
+    monkeypatch.setattr(blk, "_raw_stream", lambda index: stream[0])
+    capturing = [False]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+
+    class Twice(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, w):
+            blk._noted(ctx, x.device)
+            return x * 2 + w
+
+        @staticmethod
+        @blk._once
+        def backward(ctx, dy):
+            return dy * 2, dy
+    w, v = (torch.randn(3, requires_grad=True) for _ in range(2))
+    dy = torch.ones(3)
+    eager = Twice.apply(torch.ones(3), w)
+
+    def captured(leaf):
+        stream[0], capturing[0] = 5, True
+        try:
+            return torch.autograd.grad(Twice.apply(torch.ones(3), leaf), leaf, dy)[0]
+        finally:
+            stream[0], capturing[0] = 0, False
+    with pytest.raises(RuntimeError, match="same leaves"):
+        captured(w)
+    assert torch.equal(captured(v), dy)
+    assert torch.equal(torch.autograd.grad(eager, w, dy, retain_graph=True)[0], dy)      # the eager one still runs
+    with pytest.raises(RuntimeError, match="same leaves"):
+        captured(w)
+    del eager
+    assert torch.equal(captured(w), dy)
+    stream[0] = 3
+    other = Twice.apply(torch.ones(3), w)                         # recorded on a stream of the user's
+    assert torch.equal(captured(w), dy) and other is not None
