@@ -162,7 +162,8 @@ __global__ __launch_bounds__(64 * W) void l8_direct_kernel(L8Args p) {
 
 // Up to 16 rows, quantised where they are used: lane (l16, q) forms the operand of its row's 32 values from the 16-bit rows, the four
 // lanes of a row agree on the block's scale.  The weights pass once, 16 channels a workgroup, the block columns over its W waves; one
-// launch, no rows in memory.
+// launch, no rows in memory.  One token, 1536 -> 8960: 9.7 us, of which the weight's 13.8 MB are 2.8 at the rate of a large copy: the
+// rest is the launch and two trips to memory, one after the other, for the row's blocks and the weights.
 template <class E, int EPI, int W>
 __global__ __launch_bounds__(64 * W) void l8_few_kernel(L8Args p, const uint16_t* x, int64_t xstride, int K) {
     __shared__ f32x4 part[W][64];
@@ -273,6 +274,12 @@ int launch_direct(const L8Args& a0, hipStream_t st) {
 //
 // Scales: the 64 words of a stage's 256 rows follow the rows into LDS, a lane's word holds those of its row in the four row blocks
 // (rows8.hpp), and the matrix instruction picks the byte; the weight's is one for the wave, through the scalar cache.
+//
+// Bound by the matrix pipe, which is busy 53 % of the time at 2.1 GHz, and by the stages' arrival from L2 and the memory-side cache
+// (72 % of the requests hit L2): 8192^3 392 us, 2.80 PFLOP/s; 4680 x 5120 -> 13824 294, 2.25; 4680 x 1536 -> 8960 83-85, 1.5, where a
+// tile has 12 stages and its sums' way out is not hidden.  (A library's product with one scale per tensor: 2.6 PFLOP/s, 259 us, 85.)
+// Patches of 4, 6, 8 or 12 strips: no difference, 19 worse; a workgroup that goes on to further tiles: slower (the operands of the
+// step in flight are copied at each tile's end).
 constexpr int kTileN = 256, kSlot = 128 * kBlock8, kRing = 9;
 constexpr int kScaleAt = kRing * kSlot, kScaleSlot = 256;
 constexpr int kLdsBytes = kScaleAt + 4 * kScaleSlot;
