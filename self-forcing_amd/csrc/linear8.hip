@@ -366,70 +366,108 @@ __device__ __forceinline__ void l8_kstep(std::integer_sequence<int, I...>, f32x1
     (l8_kone<TB, FETCH, NLOAD, Q0, I>(acc, fc, fn, a0, a1, b0, b1, we, xe, src, slot, scale_addr), ...);
 }
 
-// sums to memory: 4 x TB blocks of 32 channels x 32 rows from channel c0, row r0 on.  Lane (m, hf) of block (cb, tb) holds row
-// 32 tb + m, channels 8 g + 4 hf + (i & 3), i = 4 g + ..  One block after the other, each with addresses of its own: formed for all
-// blocks together they would not fit beside the sums.
+// Four neighbouring values of a row, eight of them: zeros past the last channel.
+__device__ __forceinline__ u32x2 l8_raw4(const uint16_t* s, int left) {
+    if (left >= 4) return *(const u32x2_any*)s;
+    u32x2 w = {0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i < left) w[i >> 1] |= (uint32_t)s[i] << (16 * (i & 1));
+    return w;
+}
+__device__ __forceinline__ u32x4 l8_raw8(const uint16_t* s, int left) {
+    if (left >= 8) return *(const u32x4_any*)s;
+    const u32x2 lo = l8_raw4(s, left), hi = l8_raw4(s + 4, left - 4);
+    return u32x4{lo.x, lo.y, hi.x, hi.y};
+}
+// LDS accesses of a wave's lanes before this come before those behind it (a wave's are done in order: nothing to wait for)
+__device__ __forceinline__ void l8_wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Sums to memory: 4 x TB blocks of 32 channels x 32 rows from channel c0, row r0 on.  Lane (m, hf) of block (cb, tb) holds row
+// 32 tb + m, channels 8 g + 4 hf + (i & 3), i = 4 g + ..  32 rows x 128 channels at a time pass through the wave's own `lds`, so that a
+// store takes four rows of 256 bytes, whole cache lines; a residual comes in the same way.  (Stored from the registers, 32 rows
+// of 32 bytes a time, 32760 x 1536 -> 8960 takes 548 us against 464, 4680 x 5120 -> 13824 294 against 283.)
+constexpr int kOutPitch = 256 + 16;                            // the 16-byte pieces of a column of rows sit in different banks
 template <class E, int EPI, int TB>
-__device__ __forceinline__ void l8_store(const L8Args& p, const f32x16 (&acc)[4][TB], int c0, int64_t r0, int m, int hf) {
-    if (c0 + 128 <= p.N && r0 + 32 * TB <= p.M) {          // whole: 16-byte stores
-#pragma unroll
-        for (int cb = 0; cb < 4; ++cb) {
-            const int cbase = c0 + 32 * cb;
-            float bia[16];
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                u32x2 b = {0u, 0u};
-                if (p.bias != nullptr) b = *(const u32x2_any*)(p.bias + cbase + 8 * g + 4 * hf);
-                l8_unpack4<E>(b, bia + 4 * g);
-            }
-#pragma unroll
-            for (int tb = 0; tb < TB; ++tb) {
-                int own = 32 * tb + m;
-                asm volatile("" : "+v"(own));
-                const int64_t row = r0 + own;
-                float res[16], gate[16];
-                if (EPI == SFM_EPI_GATE_RESIDUAL) {
-                    const uint16_t* rp = p.res + row * p.res_stride + cbase + 4 * hf;
-                    const uint16_t* gp = p.gate != nullptr ? p.gate + (row / p.rows_per_frame) * p.gate_stride + cbase + 4 * hf : nullptr;
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        l8_unpack4<E>(*(const u32x2_any*)(rp + 8 * g), res + 4 * g);
-                        if (gp != nullptr) {
-                            l8_unpack4<E>(*(const u32x2_any*)(gp + 8 * g), gate + 4 * g);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) gate[4 * g + i] = 1.f;
-                        }
-                    }
-                }
-                uint32_t w[8];
-#pragma unroll
-                for (int i = 0; i < 16; i += 2)
-                    w[i / 2] = pack2<E>(l8_tail<E, EPI>(acc[cb][tb][i], bia[i], res[i], gate[i]),
-                                        l8_tail<E, EPI>(acc[cb][tb][i + 1], bia[i + 1], res[i + 1], gate[i + 1]));
-#pragma unroll
-                for (int gp = 0; gp < 2; ++gp) {               // the two lanes of a row exchange halves: 16 bytes each
-                    auto rx = __builtin_amdgcn_permlane32_swap(w[4 * gp], w[4 * gp + 2], false, false);
-                    auto ry = __builtin_amdgcn_permlane32_swap(w[4 * gp + 1], w[4 * gp + 3], false, false);
-                    u32x4 o = {(uint32_t)rx[0], (uint32_t)ry[0], (uint32_t)rx[1], (uint32_t)ry[1]};
-                    *(u32x4_any*)(p.out + row * p.out_stride + cbase + 16 * gp + 8 * hf) = o;
-                }
-            }
-        }
-        return;
-    }
+__device__ __forceinline__ void l8_store(const L8Args& p, const f32x16 (&acc)[4][TB], int c0, int64_t r0, int lane, uint8_t* lds) {
+    const int m = lane & 31, hf = lane >> 5, l16 = lane & 15, q = lane >> 4;
+    const int pc = c0 + 8 * l16, left = p.N - pc;              // a lane's piece of a row in memory
+    uint8_t *at_row = lds + q * kOutPitch + l16 * 16, *at_sum = lds + m * kOutPitch + hf * 16;
+    u32x2 bia[4][4];
 #pragma unroll
     for (int cb = 0; cb < 4; ++cb)
 #pragma unroll
-        for (int tb = 0; tb < TB; ++tb) {
-            int own = 32 * tb + m;
-            asm volatile("" : "+v"(own));
+        for (int g = 0; g < 4; ++g) {
+            const int c = c0 + 32 * cb + 8 * g + 4 * hf;
+            bia[cb][g] = p.bias != nullptr ? l8_raw4(p.bias + c, p.N - c) : u32x2{0u, 0u};
+        }
+#pragma unroll
+    for (int tb = 0; tb < TB; ++tb) {
+        const int64_t row0 = r0 + 32 * tb;
+        if (EPI == SFM_EPI_GATE_RESIDUAL) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int64_t row = row0 + 4 * i + q;
+                u32x4 v = {0u, 0u, 0u, 0u};
+                if (row < p.M) v = l8_raw8(p.res + row * p.res_stride + pc, left);
+                *(u32x4*)(at_row + 4 * i * kOutPitch) = v;
+            }
+            l8_wave_sync();
+        }
+        int64_t row = row0 + m;
+        if (row >= p.M) row = p.M - 1;
+        const uint16_t* gp = EPI == SFM_EPI_GATE_RESIDUAL && p.gate != nullptr ? p.gate + (row / p.rows_per_frame) * p.gate_stride : nullptr;
+#pragma unroll
+        for (int cb = 0; cb < 4; ++cb) {
+            float bf[16], res[16], gate[16];
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const float a4[4] = {acc[cb][tb][4 * g], acc[cb][tb][4 * g + 1], acc[cb][tb][4 * g + 2], acc[cb][tb][4 * g + 3]};
-                l8_finish4<E, EPI>(p, r0 + own, c0 + 32 * cb + 8 * g + 4 * hf, a4, l8_bias4<E>(p, c0 + 32 * cb + 8 * g + 4 * hf));
+                l8_unpack4<E>(bia[cb][g], bf + 4 * g);
+                if (EPI == SFM_EPI_GATE_RESIDUAL) {
+                    const int c = c0 + 32 * cb + 8 * g + 4 * hf;
+                    l8_unpack4<E>(*(const u32x2*)(lds + m * kOutPitch + (32 * cb + 8 * g + 4 * hf) * 2), res + 4 * g);
+                    if (gp != nullptr) {
+                        l8_unpack4<E>(l8_raw4(gp + c, p.N - c), gate + 4 * g);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) gate[4 * g + i] = 1.f;
+                    }
+                }
+            }
+            if (EPI == SFM_EPI_GATE_RESIDUAL) l8_wave_sync();
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 16; i += 2)
+                w[i / 2] = pack2<E>(l8_tail<E, EPI>(acc[cb][tb][i], bf[i], res[i], gate[i]),
+                                    l8_tail<E, EPI>(acc[cb][tb][i + 1], bf[i + 1], res[i + 1], gate[i + 1]));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {                      // the two lanes of a row exchange halves: 16 bytes each
+                auto rx = __builtin_amdgcn_permlane32_swap(w[4 * h], w[4 * h + 2], false, false);
+                auto ry = __builtin_amdgcn_permlane32_swap(w[4 * h + 1], w[4 * h + 3], false, false);
+                *(u32x4*)(at_sum + cb * 64 + h * 32) = u32x4{(uint32_t)rx[0], (uint32_t)ry[0], (uint32_t)rx[1], (uint32_t)ry[1]};
             }
         }
+        l8_wave_sync();
+        u32x4 o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = *(const u32x4*)(at_row + 4 * i * kOutPitch);
+        l8_wave_sync();
+        uint16_t* out = p.out + (row0 + q) * p.out_stride + pc;
+        const int64_t rows = p.M - row0 - q;                   // those from this lane's first on
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (4 * i < rows && left >= 8) {
+                *(u32x4_any*)(out + 4 * i * p.out_stride) = o[i];
+            } else if (4 * i < rows) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (e < left) out[4 * i * p.out_stride + e] = (uint16_t)(o[i][e >> 1] >> (16 * (e & 1)));
+            }
+        }
+    }
 }
 
 // One tile: strip rows m0 .., channels n0 ..
@@ -544,7 +582,8 @@ __device__ __forceinline__ void l8_tile(const L8Args& p, int64_t m0, int n0) {
     if (nstage >= 2) L8_ITER(false, 0, false)
     L8_ITER(false, 0, true)
 #undef L8_ITER
-    l8_store<E, EPI, TB>(p, acc, n0 + wn * 128, m0 + wm * 32 * TB, m, hf);
+    __syncthreads();                                           // every wave has read its operands: LDS is free
+    l8_store<E, EPI, TB>(p, acc, n0 + wn * 128, m0 + wm * 32 * TB, lane, l8_lds + wave * 32 * kOutPitch);
 }
 
 // Every eighth workgroup shares an XCD: each XCD gets a contiguous run of the patch order.  With TB = 4 a last strip of at most 128
