@@ -275,9 +275,10 @@ int launch_direct(const L8Args& a0, hipStream_t st) {
 // Scales: the 64 words of a stage's 256 rows follow the rows into LDS, a lane's word holds those of its row in the four row blocks
 // (rows8.hpp), and the matrix instruction picks the byte; the weight's is one for the wave, through the scalar cache.
 //
-// Bound by the matrix pipe, which is busy 53 % of the time at 2.1 GHz, and by the stages' arrival from L2 and the memory-side cache
-// (72 % of the requests hit L2): 8192^3 392 us, 2.80 PFLOP/s; 4680 x 5120 -> 13824 294, 2.25; 4680 x 1536 -> 8960 83-85, 1.5, where a
-// tile has 12 stages and its sums' way out is not hidden.  (A library's product with one scale per tensor: 2.6 PFLOP/s, 259 us, 85.)
+// A stage takes 1.35 us, its matrix instructions 0.98 at the 2.1 GHz of a long run, and a tile 8-10 us besides (launch, first stages,
+// its 128 KB on their way out): 8192^3 386-393 us, 2.8 PFLOP/s; 4680 x 5120 -> 13824 283-290, 2.3; 4680 x 1536 -> 8960, 12 stages a
+// tile, 81, 1.6.  (A library's product with one scale per tensor: 2.6 PFLOP/s, 259 us, 85.)  What the stages wait for is the compute
+// unit's load path, 64 KB a stage, not the misses of L2 (28 %): lines brought into L2 two stages early cost 8 %, their own requests.
 // Patches of 4, 6, 8 or 12 strips: no difference, 19 worse; a workgroup that goes on to further tiles: slower (the operands of the
 // step in flight are copied at each tile's end).
 constexpr int kTileN = 256, kSlot = 128 * kBlock8, kRing = 9;

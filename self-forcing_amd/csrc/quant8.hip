@@ -179,9 +179,15 @@ __global__ __launch_bounds__(256) void pack8_kernel(const void* w, int64_t ws, i
         *(uint32_t*)&tile[rr][l16 * 8] = q.x;
         *(uint32_t*)&tile[rr][l16 * 8 + 4] = q.y;
     }
-    if (threadIdx.x == 0) {
-        scale[(int64_t)nb * pitch + kb] = (uint8_t)(s + 127);
-        if (data_t != nullptr) scale_t[(int64_t)kb * pitch_t + nb] = (uint8_t)(s + 127);
+    if (threadIdx.x == 0) {                          // the last block of a row of scales fills the rest of its last word
+        uint8_t* o = scale + (int64_t)nb * pitch;
+        o[kb] = (uint8_t)(s + 127);
+        for (int i = kb + 1; kb + 1 == (int)gridDim.x && i < pitch; ++i) o[i] = 0;
+        if (data_t != nullptr) {
+            o = scale_t + (int64_t)kb * pitch_t;
+            o[nb] = (uint8_t)(s + 127);
+            for (int i = nb + 1; nb + 1 == (int)gridDim.y && i < pitch_t; ++i) o[i] = 0;
+        }
     }
     if (data_t == nullptr) return;
     __syncthreads();

@@ -105,7 +105,7 @@ def pack(weight, transposed=True):
 
     def blocks(n, k):
         return (torch.empty((n, _pad(k)), dtype=torch.uint8, device=weight.device),
-                torch.zeros((-(-n // 128), -(-k // 512) * 4), dtype=torch.uint8, device=weight.device))
+                torch.empty((-(-n // 128), -(-k // 512) * 4), dtype=torch.uint8, device=weight.device))
     data, scale = blocks(N, K)
     data_t, scale_t = blocks(K, N) if transposed else (None, None)
     with _on_device(weight.device):
@@ -139,9 +139,16 @@ def _forward(x, w8, bias, out, keep, epi=_l.EPI_NONE, res=None, gate=None):
     """Quantisation and product in one call; returns the rows' blocks where they are to be kept (few rows have none otherwise)."""
     rows, K, xs = _rows(x)
     d, g = _desc(x.dtype, rows, w8.shape[0], K, out, epi, res, gate)
-    data, scale = _empty_rows(rows, K, x.device) if keep or rows > _l.LINEAR8_FEW_ROWS else (None, None)
+    data = scale = data_at = scale_at = None
+    if keep:
+        data, scale = _empty_rows(rows, K, x.device)
+        data_at, scale_at = data.data_ptr(), scale.data_ptr()
+    elif rows > _l.LINEAR8_FEW_ROWS:                 # one piece of scratch for both
+        scratch = torch.empty((rows + -(-rows // 128)) * _pad(K), dtype=torch.uint8, device=x.device)
+        data_at = scratch.data_ptr()
+        scale_at = data_at + rows * _pad(K)
     with _on_device(x.device):
-        _l.check(_l.load().sfm_linear8_fwd(C.byref(d), x.data_ptr(), xs, _ptr(data), _ptr(scale), w8.data.data_ptr(), w8.scale.data_ptr(),
+        _l.check(_l.load().sfm_linear8_fwd(C.byref(d), x.data_ptr(), xs, data_at, scale_at, w8.data.data_ptr(), w8.scale.data_ptr(),
                                            _ptr(bias), _ptr(res), _ptr(g), out.data_ptr(), _stream(x)))
     return data, scale
 
@@ -254,7 +261,8 @@ def linear8(x, weight, bias=None, epilogue="none", res=None, gate=None, out=None
         if bias.shape != (N,):
             raise ValueError("bias must be [N]")
         bias = bias.contiguous()
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, weight, bias, res, gate)):
+    if torch.is_grad_enabled() and ((x8 is None and x.requires_grad) or (w8 is None and weight.requires_grad)
+                                    or any(t is not None and t.requires_grad for t in (bias, res, gate))):
         if epilogue != "none" or out is not None:
             raise NotImplementedError("linear8 is differentiable with epilogue 'none' and its own output")
         if res is not None or gate is not None:
