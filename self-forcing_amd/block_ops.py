@@ -124,34 +124,41 @@ def _ln_bwd_bytes(rows, C, group, device_index):
     return n.value
 
 
-def _ln_bwd(dy, x, kept, weight, scale, ms, group, eps, w_shape, b_shape, want_dx=True):
-    """(dx, dw, db): dw, db hold [groups of rows, C] in the given shapes.  From x, or from `kept` = (data, scales, 1 / standard
-    deviations)."""
-    dy = _even(dy)
+def _ln_bwd(dy, x, xs, kept, weight, scale, ms, group, nbytes, eps, w_shape, b_shape, want_dx=True):
+    """(dx, dw, db): dw, db hold [groups of rows, C] in the given shapes.  From x, rows xs apart, or from `kept` = (data, scales,
+    1 / standard deviations).  On the current device."""
     B, L, C = dy.shape
-    dt, dev = dy.dtype, dy.device
-    rows = B * L
-    dx = torch.empty((B, L, C), dtype=dt, device=dev) if want_dx else None
-    dw, db = torch.empty(w_shape, dtype=dt, device=dev), torch.empty(b_shape, dtype=dt, device=dev)
-    data, sc8, rstd = (None, None, None) if kept is None else (t.data_ptr() for t in kept)
-    with _on_device(dev):
-        n = _ln_bwd_bytes(rows, C, group, dev.index)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        _l.check(_l.load().sfm_ln_bwd(_DT[dt], rows, C, eps, None if x is None else x.data_ptr(), 0 if x is None else _row_stride(x), data, sc8,
-                                      rstd, dy.data_ptr(), _row_stride(dy), None if weight is None else weight.data_ptr(),
-                                      None if scale is None else scale.data_ptr(), ms, group, dx.data_ptr() if want_dx else None, C,
-                                      dw.data_ptr(), db.data_ptr(), ws.data_ptr(), n, _stream(dy)))
+    dys = C
+    if not dy.is_contiguous() or dy.data_ptr() & 15:
+        dy = _even(dy)
+        dys = _row_stride(dy)
+    dx = torch.empty_like(dy, memory_format=torch.contiguous_format) if want_dx else None
+    dw, db = dy.new_empty(w_shape), dy.new_empty(b_shape)
+    data = sc8 = rstd = None
+    if kept is not None:
+        data, sc8, rstd = kept[0].data_ptr(), kept[1].data_ptr(), kept[2].data_ptr()
+    ws = dy.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    rc = _l.load().sfm_ln_bwd(_DT[dy.dtype], B * L, C, eps, None if x is None else x.data_ptr(), xs, data, sc8, rstd, dy.data_ptr(), dys,
+                              None if weight is None else weight.data_ptr(), None if scale is None else scale.data_ptr(), ms, group,
+                              dx.data_ptr() if want_dx else None, C, dw.data_ptr(), db.data_ptr(), ws.data_ptr() if nbytes else None, nbytes,
+                              _raw_stream(dy.get_device()))
+    if rc:
+        _l.check(rc)
     return dx, dw, db
 
 
-_eager_graphs, _eager_lock = weakref.WeakSet(), threading.Lock()
+_eager_graphs, _eager_lock, _eager_limit = [], threading.Lock(), 1024
 
 
 def _noted(ctx, device):
-    """Called by the forwards: remembers a graph recorded on the default stream for as long as it lives."""
+    """Called by the forwards: remembers a graph recorded on the default stream while it lives."""
+    global _eager_limit
     if _raw_stream(device.index) == 0:
         with _eager_lock:
-            _eager_graphs.add(ctx)
+            _eager_graphs.append(weakref.ref(ctx))
+            if len(_eager_graphs) > _eager_limit:              # most of them are gone
+                _eager_graphs[:] = [r for r in _eager_graphs if r() is not None]
+                _eager_limit = max(1024, 2 * len(_eager_graphs))
 
 
 def _leaves(ctx):
@@ -162,23 +169,29 @@ def _check_captured(ctx):
     """Autograd sums a leaf's gradient on the stream that its oldest living graph was recorded on.  A captured backward whose leaf
     belongs to a living graph of the default stream would make that stream part of the capture, which HIP does not allow and which
     ends the process: refused before anything reaches the leaf."""
+    if not torch.cuda.is_current_stream_capturing():
+        return
     mine = _leaves(ctx)
     with _eager_lock:
-        others = [o for o in _eager_graphs if o is not ctx]
-    if any(a is b for o in others for a in _leaves(o) for b in mine):
+        others = [r() for r in _eager_graphs]
+    if any(a is b for o in others if o is not None and o is not ctx for a in _leaves(o) for b in mine):
         raise RuntimeError("a backward cannot be captured while a graph of the same leaves, recorded on the default stream, lives: drop "
                            "its outputs first, or record it on another stream")
 
 
 def _once(backward):
     """A backward without a derivative of its own: `once_differentiable`, but for calls that build no graph, which it would only
-    slow down (a third of a small call's time)."""
+    slow down.
+
+    The backwards themselves are short on purpose: autograd's thread, whose current device is the node's, runs them on another core, and every
+    Python object that they touch comes over from the caller's (LayerNorm of three rows, forward and backward: 94 us a call, 41 with
+    both threads on one core, 110 and 47 with checks, sizes and device contexts in the backward)."""
     guarded = torch.autograd.function.once_differentiable(backward)
 
-    def run(ctx, *grads):
-        if torch.cuda.is_current_stream_capturing():
+    def run(ctx, dy):
+        if _raw_stream(dy.get_device()):                       # the default stream is never captured
             _check_captured(ctx)
-        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, dy)
     return run
 
 
@@ -194,23 +207,24 @@ class _LnFn(torch.autograd.Function):
         else:
             sc, sh, ms, rpf = _vec("weight", a, x), _vec("bias", b, x), 0, x.shape[0] * x.shape[1]
             mod = (None, None, 0, 1, sc.data_ptr(), sh.data_ptr())
-        ctx.cfg = (modulate, eps, checkpoint8, ms, rpf, a.shape, b.shape)
-        _noted(ctx, x.device)
         if checkpoint8:
             y, *kept = _ln_keep8(x, mod, eps)
             ctx.save_for_backward(sc, *kept)
         else:
             y = _ln(x, mod, eps)
             ctx.save_for_backward(sc, x)
+        ctx.cfg = (modulate, eps, checkpoint8, ms, rpf, _row_stride(x), _ln_bwd_bytes(x.shape[0] * x.shape[1], x.shape[2], rpf, x.get_device()),
+                   a.shape, b.shape)
+        _noted(ctx, x.device)
         return y
 
     @staticmethod
     @_once
     def backward(ctx, dy):
-        modulate, eps, checkpoint8, ms, rpf, a_shape, b_shape = ctx.cfg
+        modulate, eps, checkpoint8, ms, rpf, xs, nbytes, a_shape, b_shape = ctx.cfg
         sc, *rest = ctx.saved_tensors
         x, kept = (None, rest) if checkpoint8 else (rest[0], None)
-        dx, dw, db = _ln_bwd(dy, x, kept, None if modulate else sc, sc if modulate else None, ms, rpf, eps, a_shape, b_shape,
+        dx, dw, db = _ln_bwd(dy, x, xs, kept, None if modulate else sc, sc if modulate else None, ms, rpf, nbytes, eps, a_shape, b_shape,
                              ctx.needs_input_grad[0])
         return dx, dw, db, None, None, None
 
@@ -240,17 +254,21 @@ def _check_dy(dy, x):
 
 def ln_affine_backward(dy, x, weight, eps=1e-6):
     """(dx, dweight, dbias) of ln_affine from its output's gradient."""
-    _rows(x)
     _check_dy(dy, x)
-    return _ln_bwd(dy, x, None, _vec("weight", weight, x), None, 0, x.shape[0] * x.shape[1], eps, weight.shape, weight.shape)
+    rows, C, xs = _rows(x)
+    with _on_device(x.device):
+        n = _ln_bwd_bytes(rows, C, rows, x.get_device())
+        return _ln_bwd(dy, x, xs, None, _vec("weight", weight, x), None, 0, rows, n, eps, weight.shape, weight.shape)
 
 
 def ln_modulate_backward(dy, x, scale, eps=1e-6):
     """(dx, dscale, dshift) of ln_modulate from its output's gradient; dscale and dshift in scale's shape."""
-    _rows(x)
     _check_dy(dy, x)
     sc, ms, rpf = _mod(scale, x)
-    return _ln_bwd(dy, x, None, None, sc, ms, rpf, eps, scale.shape, scale.shape)
+    rows, C, xs = _rows(x)
+    with _on_device(x.device):
+        n = _ln_bwd_bytes(rows, C, rpf, x.get_device())
+        return _ln_bwd(dy, x, xs, None, None, sc, ms, rpf, n, eps, scale.shape, scale.shape)
 
 
 def _gelu(x, keep8):
@@ -281,18 +299,21 @@ class _GeluFn(torch.autograd.Function):
     @staticmethod
     @_once
     def backward(ctx, dy):
-        dy = _even(dy)
         B, L, C = dy.shape
+        dys = C
+        if not dy.is_contiguous():
+            dy = _even(dy)
+            dys = _row_stride(dy)
         x, xs, data, scale = None, 0, None, None
         if ctx.checkpoint8:
             data, scale = (t.data_ptr() for t in ctx.saved_tensors)
         else:
             x, = ctx.saved_tensors
             xs, x = _row_stride(x), x.data_ptr()
-        dx = torch.empty((B, L, C), dtype=dy.dtype, device=dy.device)
-        with _on_device(dy.device):
-            _l.check(_l.load().sfm_gelu_bwd(_DT[dy.dtype], B * L, C, x, xs, data, scale, dy.data_ptr(), _row_stride(dy), dx.data_ptr(), C,
-                                            _stream(dy)))
+        dx = torch.empty_like(dy, memory_format=torch.contiguous_format)
+        rc = _l.load().sfm_gelu_bwd(_DT[dy.dtype], B * L, C, x, xs, data, scale, dy.data_ptr(), dys, dx.data_ptr(), C, _raw_stream(dy.get_device()))
+        if rc:
+            _l.check(rc)
         return dx, None
 
 

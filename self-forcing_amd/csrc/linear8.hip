@@ -163,7 +163,7 @@ __global__ __launch_bounds__(64 * W) void l8_direct_kernel(L8Args p) {
 // Up to 16 rows, quantised where they are used: lane (l16, q) forms the operand of its row's 32 values from the 16-bit rows, the four
 // lanes of a row agree on the block's scale.  The weights pass once, 16 channels a workgroup, the block columns over its W waves; one
 // launch, no rows in memory.  One token, 1536 -> 8960: 9.7 us, of which the weight's 13.8 MB are 2.8 at the rate of a large copy: the
-// rest is the launch and two trips to memory, one after the other, for the row's blocks and the weights.
+// rest is the launch (3), one trip to memory for a wave's one or two blocks, and the sums' meeting.
 template <class E, int EPI, int W>
 __global__ __launch_bounds__(64 * W) void l8_few_kernel(L8Args p, const uint16_t* x, int64_t xstride, int K) {
     __shared__ f32x4 part[W][64];

@@ -327,7 +327,8 @@ int launch_sum_parts(int dtype, int64_t parts, int64_t n, int64_t groups, const 
 
 size_t ln_bwd_workspace_bytes(int64_t rows, int C, int64_t rows_per_group) {
     const int64_t groups = rows / rows_per_group;
-    return (size_t)groups * ln_bwd_splits(groups, rows_per_group, C) * 2 * C * sizeof(float);
+    const int splits = ln_bwd_splits(groups, rows_per_group, C);
+    return splits > 1 ? (size_t)groups * splits * 2 * C * sizeof(float) : 0;
 }
 
 int launch_ln_bwd(int dtype, int64_t rows, int C, float eps, const void* x, int64_t xs, const void* data, const void* scale8,

@@ -1736,7 +1736,7 @@ int sfm_ln_bwd(int32_t dtype, int64_t rows, int32_t C, float eps, const void* x,
         return SFM_ERR_ALIGN;
     }
     const size_t need = ln_bwd_workspace_bytes(rows, C, rows_per_group);
-    if (!workspace || (((uintptr_t)workspace) & 255) || workspace_bytes < need) {
+    if (need && (!workspace || (((uintptr_t)workspace) & 255) || workspace_bytes < need)) {
         set_error("workspace must be non-NULL, 256-byte aligned and hold %zu bytes", need);
         return SFM_ERR_WORKSPACE;
     }

@@ -18,7 +18,7 @@ import torch
 
 from . import lib as _l
 from .block_ops import _HALF, _like, _mod, _noted, _once, _row_stride, _rows, _written
-from .monarch_attn import _DT, _on_device, _stream
+from .monarch_attn import _DT, _on_device, _raw_stream, _stream
 
 _EPI = {"none": _l.EPI_NONE, "gelu_tanh": _l.EPI_GELU_TANH, "gate_residual": _l.EPI_GATE_RESIDUAL}
 
@@ -206,7 +206,8 @@ class _Linear8Fn(torch.autograd.Function):
         else:
             data, scale = x8.data, x8.scale
             _product(x8, w8.data, w8.scale, N, bias, out)
-        ctx.cfg = (rows.shape, rows.dtype, w8.shape)
+        n = rows.shape[0] * rows.shape[1]
+        ctx.cfg = (rows.shape, rows.dtype, w8.shape, n, _bytes("sfm_linear8_bwd_workspace_bytes", n, N, rows.shape[2], rows.device.index))
         _noted(ctx, rows.device)
         ctx.save_for_backward(*((data, scale) if need_w else (None, None)), *((w8.data_t, w8.scale_t) if need_x else (None, None)))
         return out
@@ -215,18 +216,21 @@ class _Linear8Fn(torch.autograd.Function):
     @_once
     def backward(ctx, dy):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        x_shape, dtype, (N, K) = ctx.cfg
+        x_shape, dtype, w_shape, rows, nbytes = ctx.cfg
         xd, xs, wd, ws = ctx.saved_tensors
-        dy = _even(dy)
-        rows, dev = x_shape[0] * x_shape[1], dy.device
-        dx = torch.empty(x_shape, dtype=dtype, device=dev) if need_x else None
-        dw = torch.empty((N, K), dtype=dtype, device=dev) if need_w else None
-        db = torch.empty(N, dtype=dtype, device=dev) if need_b else None
-        with _on_device(dev):
-            n = _bytes("sfm_linear8_bwd_workspace_bytes", rows, N, K, dev.index)
-            work = torch.empty(n, dtype=torch.uint8, device=dev)
-            _l.check(_l.load().sfm_linear8_bwd(_DT[dtype], rows, N, K, dy.data_ptr(), _row_stride(dy), _ptr(wd), _ptr(ws), _ptr(xd), _ptr(xs),
-                                               _ptr(dx), _ptr(dw), _ptr(db), work.data_ptr(), n, _stream(dy)))
+        N, K = w_shape
+        dys = N
+        if not dy.is_contiguous():
+            dy = _even(dy)
+            dys = _row_stride(dy)
+        dx = dy.new_empty(x_shape) if need_x else None
+        dw = dy.new_empty(w_shape) if need_w else None
+        db = dy.new_empty(N) if need_b else None
+        work = dy.new_empty(nbytes, dtype=torch.uint8)
+        rc = _l.load().sfm_linear8_bwd(_DT[dtype], rows, N, K, dy.data_ptr(), dys, _ptr(wd), _ptr(ws), _ptr(xd), _ptr(xs), _ptr(dx), _ptr(dw), _ptr(db),
+                                       work.data_ptr(), nbytes, _raw_stream(dy.get_device()))
+        if rc:
+            _l.check(rc)
         return dx, dw, db, None, None
 
 
