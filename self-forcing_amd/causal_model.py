@@ -118,9 +118,21 @@ class HipAttentionOps:
         return self.gate_residual(x, linear(h), gate)
 
 
+def _state(*params):
+    return tuple((p.data_ptr(), p._version) for p in params)
+
+
+def _check_packed(was, *params):
+    if was != _state(*params):
+        raise RuntimeError("a layer's parameters have changed since pack_linear8: call it again")
+
+
 def _packed8(layer):
     """The 8-bit form that `CausalWanModel.pack_linear8` has given a layer, None without one or where gradients are wanted."""
-    return None if torch.is_grad_enabled() else getattr(layer, "weight8", None)
+    w8 = None if torch.is_grad_enabled() else getattr(layer, "weight8", None)
+    if w8 is not None:
+        _check_packed(layer.weight8_of, layer.weight)
+    return w8
 
 
 def _env_int(name, default):
@@ -306,12 +318,16 @@ class CausalWanSelfAttention(nn.Module):
         self._qkv = None
         self.qkv8 = None           # (the three projections' weight in 8-bit blocks, their bias): CausalWanModel.pack_linear8
 
+    def _qkv_params(self):
+        return [p for layer in (self.q, self.k, self.v) for p in (layer.weight, layer.bias)]
+
     def _project_qkv(self, x):
         """q, k, v projections as one GEMM over the concatenated weights (the parameters stay the reference's
         three Linear layers; the concatenation is rebuilt when one of them changes).  The three results are
         column slices of one [B, S, 3C] tensor, which the prologue reads through its row stride."""
         c = self.dim
         if self.qkv8 is not None:
+            _check_packed(self.qkv8_of, *self._qkv_params())
             y = _l8.linear8(x, *self.qkv8)
             return y[..., :c], y[..., c:2 * c], y[..., 2 * c:]
         ws = (self.q.weight, self.k.weight, self.v.weight)
@@ -509,16 +525,18 @@ class CausalWanModel(nn.Module):
     def pack_linear8(self, on=True):
         """Lays the blocks' linear layers out in 8-bit blocks of 128 (linear8.pack): self-attention's q, k, v as one weight, the
         output projections, cross-attention's q, and the feed-forward.  Passes without gradients then run them on 8-bit products
-        (weights and activations as e4m3, fp32 sums).  The 16-bit weights stay; call it again after they change, `on=False`
-        goes back to them.  Returns the model."""
+        (weights and activations as e4m3, fp32 sums).  The 16-bit weights stay; call it again after they change or move (a pass before
+        that is refused), `on=False` goes back to them.  Returns the model."""
         for b in self.blocks:
             sa, ca = b.self_attn, b.cross_attn
             sa.qkv8 = None
             if on:
                 ws = torch.cat((sa.q.weight, sa.k.weight, sa.v.weight), 0)
                 sa.qkv8 = (_l8.pack(ws, transposed=False), torch.cat((sa.q.bias, sa.k.bias, sa.v.bias), 0))
+                sa.qkv8_of = _state(*sa._qkv_params())
             for layer in (sa.o, ca.q, ca.o, b.ffn[0], b.ffn[2]):
                 layer.weight8 = _l8.pack(layer.weight, transposed=False) if on else None
+                layer.weight8_of = _state(layer.weight)
         return self
 
     def _patchify(self, x):

@@ -207,3 +207,29 @@ def test_blocks_in_8_bits():
         del b.self_attn._project_qkv
     dev_gen.model.pack_linear8(False)
     assert torch.equal(flow(), plain)
+
+
+def test_packed_layers_refuse_parameters_that_have_changed():
+    """A weight, or a bias that was laid out with its weights, written after pack_linear8: refused until it is called again."""
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(1, 3, 16, 12, 104, generator=g).to(torch.bfloat16).to("cuda:0")
+    cond = {"prompt_embeds": torch.randn(1, 16, 64, generator=g).to(torch.bfloat16).to("cuda:0")}
+    t = torch.full((1, 3), 937.5, device="cuda:0")
+    _, dev_gen = _pair(use_framewise=True)
+
+    def flow():
+        kv = [{"k": torch.zeros(1, 6 * 312, 2, 128, dtype=torch.bfloat16, device="cuda:0"),
+               "v": torch.zeros(1, 6 * 312, 2, 128, dtype=torch.bfloat16, device="cuda:0"),
+               "global_end_index": torch.tensor([0], device="cuda:0"), "local_end_index": torch.tensor([0], device="cuda:0")}
+              for _ in range(2)]
+        return dev_gen(x, cond, t, kv, [{"k": None, "v": None, "is_init": False} for _ in range(2)], 0)[0]
+    dev_gen.model.pack_linear8()
+    block = dev_gen.model.blocks[1]
+    for p in (block.ffn[0].weight, block.self_attn.k.bias):
+        before = flow()
+        with torch.no_grad():
+            p.mul_(2).add_(0.25)
+        with pytest.raises(RuntimeError, match="pack_linear8"):
+            flow()
+        dev_gen.model.pack_linear8()
+        assert not torch.equal(flow(), before)
