@@ -162,7 +162,7 @@ __global__ __launch_bounds__(64 * W) void l8_direct_kernel(L8Args p) {
 
 // Up to 16 rows, quantised where they are used: lane (l16, q) forms the operand of its row's 32 values from the 16-bit rows, the four
 // lanes of a row agree on the block's scale.  The weights pass once, 16 channels a workgroup, the block columns over its W waves; one
-// launch, no rows in memory.  One token, 1536 -> 8960: 9.7 us, of which the weight's 13.8 MB are 2.8 at the rate of a large copy: the
+// launch, no rows in memory.  One token, 1536 -> 8960: 9.4 us, of which the weight's 13.8 MB are 2.8 at the rate of a large copy: the
 // rest is the launch (3), one trip to memory for a wave's one or two blocks, and the sums' meeting.
 template <class E, int EPI, int W>
 __global__ __launch_bounds__(64 * W) void l8_few_kernel(L8Args p, const uint16_t* x, int64_t xstride, int K) {
@@ -276,8 +276,8 @@ int launch_direct(const L8Args& a0, hipStream_t st) {
 // (rows8.hpp), and the matrix instruction picks the byte; the weight's is one for the wave, through the scalar cache.
 //
 // A stage takes 1.35 us, its matrix instructions 0.98 at the 2.1 GHz of a long run, and a tile 8-10 us besides (launch, first stages,
-// its 128 KB on their way out): 8192^3 386-393 us, 2.8 PFLOP/s; 4680 x 5120 -> 13824 283-290, 2.3; 4680 x 1536 -> 8960, 12 stages a
-// tile, 81, 1.6.  (A library's product with one scale per tensor: 2.6 PFLOP/s, 259 us, 85.)  What the stages wait for is the compute
+// its 128 KB on their way out): 8192^3 374-393 us, 2.8-2.9 PFLOP/s; 4680 x 5120 -> 13824 273-285, 2.4; 4680 x 1536 -> 8960, 12 stages a
+// tile, 80, 1.6.  (A library's product with one scale per tensor: 2.6 PFLOP/s, 259 us, 85.)  What the stages wait for is the compute
 // unit's load path, 64 KB a stage, not the misses of L2 (28 %): lines brought into L2 two stages early cost 8 %, their own requests.
 // Patches of 4, 6, 8 or 12 strips: no difference, 19 worse; a workgroup that goes on to further tiles: slower (the operands of the
 // step in flight are copied at each tile's end).

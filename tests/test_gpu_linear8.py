@@ -427,3 +427,33 @@ def test_a_captured_backward_refuses_leaves_of_a_living_eager_graph():
         torch.cuda.synchronize()
         assert torch.equal(out, ref) and torch.equal(step(), ref)
         out.zero_()
+
+
+def test_rows_past_4_gib():
+    """2.2 million rows of 2048, more than 2^32 elements: the same 4400 rows over and over, of -1, 0 and 1, so that every sum is exact
+    in any order (their magnitudes stay under 2^24) and what the last rows give is what the first give."""
+    n, times, K, N = 4400, 500, 2048, 64
+    g = torch.Generator().manual_seed(70)
+    base, dy1 = (torch.randint(-1, 2, (1, n, c), generator=g).to(torch.bfloat16).to(DEV) for c in (K, N))
+    w = torch.randint(-1, 2, (N, K), generator=g).to(torch.bfloat16).to(DEV)
+    x, dy = base.repeat(1, times, 1), dy1.repeat(1, times, 1)
+    assert x.numel() > 1 << 32
+    x8, w8 = l8.quantize(x), l8.pack(w)
+    assert torch.equal(x8.dequantize()[:, -n:], base)
+    ref = torch.nn.functional.linear(base.float(), w.float()).to(torch.bfloat16)
+    for y in (l8.linear8(x8, w8), l8.linear8(x, w8)):
+        assert torch.equal(y[:, -n:], ref) and torch.equal(y[:, :n], ref)
+    dw, db = l8.weight_grad(dy, x8)
+    assert torch.equal(dw, (times * (dy1[0].double().T @ base[0].double())).to(torch.bfloat16))
+    assert torch.equal(db, (times * dy1[0].double().sum(0)).to(torch.bfloat16))
+    del x8, dy, y
+    lw, lb = torch.ones(K, dtype=torch.bfloat16, device=DEV), torch.zeros(K, dtype=torch.bfloat16, device=DEV)
+    for op in (lambda t: blk.gelu_tanh(t, checkpoint8=True), lambda t: blk.ln_affine(t, lw, lb, checkpoint8=True),
+               lambda t: blk.ln_affine(t, lw, lb)):
+        few, many = base.clone().requires_grad_(), x.requires_grad_()
+        a, b = op(few), op(many)
+        assert torch.equal(a, b[:, -n:])
+        da, = torch.autograd.grad(a, few, base)
+        dm, = torch.autograd.grad(b, many, x.detach())
+        assert torch.equal(da, dm[:, -n:])
+        del a, b, dm
