@@ -333,8 +333,8 @@ int sfm_linear(const sfm_linear_desc* desc, const void* x, const void* w, const 
  * that is not finite as NaN.
  *   rows     data: rows x SFM_PAD8(K) bytes, zeros past K.  scale: SFM_ROWS8_SCALE_BYTES(rows, K) bytes of s + 127; row r, block
  *            column kb at ((kb * ceil(rows / 128) + r / 128) * 32 + r % 32) * 4 + r % 128 / 32.
- *   weights  data: N x SFM_PAD8(K) bytes, scale: ceil(N / 128) rows of SFM_PITCH8(K) bytes; data_t, scale_t: the same of the
- *            transposed weight [K, N] (the same values), for the product with the output's gradient.
+ *   weights  data: N x SFM_PAD8(K) bytes, scale: ceil(N / 128) rows of SFM_PITCH8(K) bytes, zeros past the blocks; data_t,
+ *            scale_t: the same of the transposed weight [K, N] (the same values), for the product with the output's gradient.
  * data and scale are 16-byte aligned.
  *
  * sfm_quantize8: data / scale of x [rows, K] (rows x_stride apart, any alignment).  colsum (NULL or float [ceil(rows / 32)][K])
@@ -403,7 +403,8 @@ int sfm_ln_keep8(int32_t dtype, int64_t rows, int32_t C, float eps, const void* 
 /* Backward of sfm_ln_modulate.  Rows in groups of rows_per_group (affine form: all of them; modulated: the rows of a frame); dw, db:
  * [rows / rows_per_group][C], for the affine form the gradients of weight and bias, for the modulated one of scale and shift.
  * Exactly one of weight ([C]) and scale (rows mod_stride apart) is given; dx may be NULL.  From x, or (x NULL) from the blocks and
- * rstd of sfm_ln_keep8.  Statistics and sums in fp32, in a fixed order; one rounding. */
+ * rstd of sfm_ln_keep8.  Statistics and sums in fp32, in a fixed order; one rounding. No workspace (0
+ * bytes) where each group of rows is one workgroup's. */
 int sfm_ln_bwd_workspace_bytes(int64_t rows, int32_t C, int64_t rows_per_group, size_t* bytes);
 int sfm_ln_bwd(int32_t dtype, int64_t rows, int32_t C, float eps, const void* x, int64_t x_stride, const void* data, const void* scale8,
                const float* rstd, const void* dy, int64_t dy_stride, const void* weight, const void* scale, int64_t mod_stride,

@@ -457,3 +457,16 @@ def test_rows_past_4_gib():
         dm, = torch.autograd.grad(b, many, x.detach())
         assert torch.equal(da, dm[:, -n:])
         del a, b, dm
+
+
+@pytest.mark.parametrize("N,K", [(1, 1), (130, 300), (700, 513), (512, 512)])
+def test_a_weights_scales_are_whole_words(N, K):
+    """What lies behind a row's blocks in the scales is written too, whatever was in the memory before."""
+    torch.full((1 << 20,), 255, dtype=torch.uint8, device=DEV)
+    w = randn((N, K), 71, torch.bfloat16).to(DEV)
+    p = l8.pack(w)
+    for s, n, k in ((p.scale, N, K), (p.scale_t, K, N)):
+        assert s.shape == (-(-n // 128), -(-k // 512) * 4)
+        assert bool((s[:, :-(-k // 128)] > 0).all()) and not s[:, -(-k // 128):].any()
+    q = l8.pack(w)
+    assert all(torch.equal(getattr(p, a), getattr(q, a)) for a in ("data", "scale", "data_t", "scale_t"))
