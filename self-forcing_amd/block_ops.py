@@ -214,16 +214,21 @@ class _LnFn(torch.autograd.Function):
             y = _ln(x, mod, eps)
             ctx.save_for_backward(sc, x)
         ctx.cfg = (modulate, eps, checkpoint8, ms, rpf, _row_stride(x), _ln_bwd_bytes(x.shape[0] * x.shape[1], x.shape[2], rpf, x.get_device()),
-                   a.shape, b.shape)
+                   a.shape, b.shape, sc.stride(), x.stride())
         _noted(ctx, x.device)
         return y
 
     @staticmethod
     @_once
     def backward(ctx, dy):
-        modulate, eps, checkpoint8, ms, rpf, xs, nbytes, a_shape, b_shape = ctx.cfg
+        modulate, eps, checkpoint8, ms, rpf, xs, nbytes, a_shape, b_shape, sc_strides, x_strides = ctx.cfg
         sc, *rest = ctx.saved_tensors
-        x, kept = (None, rest) if checkpoint8 else (rest[0], None)
+        x, kept = (None, [t.contiguous() for t in rest]) if checkpoint8 else (rest[0], None)
+        # saved-tensor hooks (save_on_cpu) give the values back, not the layout
+        if sc.stride() != sc_strides:
+            sc, ms = sc.contiguous(), sc.shape[-1] if modulate else 0
+        if x is not None and x.stride() != x_strides:
+            x, xs = x.contiguous(), x.shape[2]
         dx, dw, db = _ln_bwd(dy, x, xs, kept, None if modulate else sc, sc if modulate else None, ms, rpf, nbytes, eps, a_shape, b_shape,
                              ctx.needs_input_grad[0])
         return dx, dw, db, None, None, None

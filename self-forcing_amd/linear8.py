@@ -217,7 +217,7 @@ class _Linear8Fn(torch.autograd.Function):
     def backward(ctx, dy):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         x_shape, dtype, w_shape, rows, nbytes = ctx.cfg
-        xd, xs, wd, ws = ctx.saved_tensors
+        xd, xs, wd, ws = (t if t is None else t.contiguous() for t in ctx.saved_tensors)      # saved-tensor hooks may change the layout
         N, K = w_shape
         dys = N
         if not dy.is_contiguous():
