@@ -310,10 +310,14 @@ class _GeluFn(torch.autograd.Function):
             dy = _even(dy)
             dys = _row_stride(dy)
         x, xs, data, scale = None, 0, None, None
+        saved = ctx.saved_tensors              # held until the call: saved-tensor hooks give tensors that nobody else holds
         if ctx.checkpoint8:
-            data, scale = (t.data_ptr() for t in ctx.saved_tensors)
+            saved = [t.contiguous() for t in saved]
+            data, scale = (t.data_ptr() for t in saved)
         else:
-            x, = ctx.saved_tensors
+            x, = saved
+            if _row_stride(x) is None:
+                saved = x = x.contiguous()
             xs, x = _row_stride(x), x.data_ptr()
         dx = torch.empty_like(dy, memory_format=torch.contiguous_format)
         rc = _l.load().sfm_gelu_bwd(_DT[dy.dtype], B * L, C, x, xs, data, scale, dy.data_ptr(), dys, dx.data_ptr(), C, _raw_stream(dy.get_device()))

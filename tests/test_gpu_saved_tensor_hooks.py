@@ -46,3 +46,9 @@ def test_layer_norms(keep8):
 def test_linear():
     x, w = (randn(s, 6 + i, torch.bfloat16).to(DEV).requires_grad_() for i, s in enumerate(((1, 70, 200), (130, 200))))
     _same(lambda: l8.linear8(x, w), (x, w), randn((1, 70, 130), 8, torch.bfloat16).to(DEV))
+
+
+@pytest.mark.parametrize("keep8", [False, True])
+def test_gelu(keep8):
+    x = randn((1, 300, 1000), 9, torch.bfloat16).to(DEV).requires_grad_()
+    _same(lambda: blk.gelu_tanh(x, checkpoint8=keep8), x, randn((1, 300, 1000), 10, torch.bfloat16).to(DEV))

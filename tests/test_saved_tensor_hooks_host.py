@@ -4,6 +4,7 @@ import contextlib
 
 import pytest
 import torch
+from torch.multiprocessing.reductions import StorageWeakRef
 
 import self_forcing_amd as sfa
 
@@ -95,3 +96,34 @@ def test_blocks_come_as_rows_whatever_the_hooks_give(library, monkeypatch, op):
     torch.autograd.grad(y, x, torch.ones_like(y))
     given = [t for t in hooks.given if t.dtype == torch.uint8 and t.dim() == 2 and not t.is_contiguous()]
     assert given and library.calls[name][at] not in [t.data_ptr() for t in given]
+
+
+@pytest.mark.parametrize("keep8", [False, True])
+def test_gelu_holds_what_the_hooks_give_until_its_call(library, monkeypatch, keep8):
+    """Nobody else holds a tensor that a hook has made: freed before the call, its memory would be the gradient's."""
+    x = torch.randn(1, 40, 256).bfloat16().requires_grad_()
+    given = []
+
+    def unpack(t):
+        t = t.clone()
+        given.append((t.data_ptr(), StorageWeakRef(t.untyped_storage())))
+        return t
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        y = blk.gelu_tanh(x, checkpoint8=keep8)
+
+    def call(*args):
+        library.calls["sfm_gelu_bwd"] = args, [ref.expired() for _, ref in given]
+        return 0
+    monkeypatch.setattr(library, "sfm_gelu_bwd", call, raising=False)
+    torch.autograd.grad(y, x, torch.ones_like(y))
+    args, gone = library.calls["sfm_gelu_bwd"]
+    assert gone == [False] * (2 if keep8 else 1)
+    assert [at for at, _ in given] == list(args[5:7] if keep8 else args[3:4])
+
+
+def test_gelu_takes_rows_whatever_the_hooks_give(library):
+    x = torch.randn(1, 40, 256).bfloat16().requires_grad_()
+    with _Hooks(transposed=True):
+        y = blk.gelu_tanh(x)
+    torch.autograd.grad(y, x, torch.ones_like(y))
+    assert library.calls["sfm_gelu_bwd"][4] == 256
