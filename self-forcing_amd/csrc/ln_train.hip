@@ -48,8 +48,8 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(LnBwdArgs p) {
     const int64_t grp = blockIdx.x / p.splits;
     const int split = blockIdx.x % p.splits;
     const int64_t g0 = grp * p.rpg;
-    const int per = (p.rpg + p.splits - 1) / p.splits;
-    const int64_t r_end = g0 + min((int64_t)p.rpg, (int64_t)(split + 1) * per);
+    const RowRange mine = rows_of_part(p.rpg, p.splits, split);
+    const int64_t r_end = g0 + mine.last;
     int par = 0;
     auto row_sum3 = [&](float& a, float& b, float& c) {
         a = wave_sum(a);
@@ -82,7 +82,7 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(LnBwdArgs p) {
             }
         }
     }
-    for (int64_t base = g0 + (int64_t)split * per; base < r_end; base += RW) {
+    for (int64_t base = g0 + mine.first; base < r_end; base += RW) {
         const int64_t row = base + (WPR == 1 ? wave : 0);
         const bool live = row < r_end;       // with WPR > 1 the same for the whole workgroup
         if (WPR == 1 && !live) break;

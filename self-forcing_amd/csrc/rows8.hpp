@@ -208,6 +208,16 @@ __device__ __forceinline__ float gelu_slope(float x) {
     return p + x * p * (1.f - p) * (1.5957691216057308f + 0.21406445f * x * x);
 }
 
+// Rows first .. last - 1, of a group of `rows`, that workgroup `part` of `parts` takes (LayerNorm's backward); none where the parts
+// before it have all.  Up to 2^31 - 1 rows: in 64 bits, the sums pass 32.
+struct RowRange {
+    int64_t first, last;
+};
+__host__ __device__ inline RowRange rows_of_part(int64_t rows, int parts, int part) {
+    const int64_t per = (rows + parts - 1) / parts, first = part * per;
+    return {first, first + per < rows ? first + per : rows};
+}
+
 // the launch that precedes: SFM_OK, or SFM_ERR_HIP with the runtime's message
 inline int launched8(const char* what) {
     hipError_t e = hipGetLastError();
