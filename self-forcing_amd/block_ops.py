@@ -161,20 +161,30 @@ def _noted(ctx, device):
                 _eager_limit = max(1024, 2 * len(_eager_graphs))
 
 
-def _leaves(ctx):
-    return [n.variable for n, _ in ctx.next_functions if hasattr(n, "variable")]
+def _leaves(*nodes):
+    """The leaves, by identity, that the gradients of these nodes go to, directly or through other operators."""
+    seen, leaves, todo = set(), {}, list(nodes)
+    while todo:
+        node = todo.pop()
+        if hasattr(node, "variable"):
+            leaves[id(node.variable)] = node.variable
+        elif node is not None and node not in seen:
+            seen.add(node)
+            todo.extend(n for n, _ in node.next_functions)
+    return leaves
 
 
 def _check_captured(ctx):
     """Autograd sums a leaf's gradient on the stream that its oldest living graph was recorded on.  A captured backward whose leaf
     belongs to a living graph of the default stream would make that stream part of the capture, which HIP does not allow and which
-    ends the process: refused before anything reaches the leaf."""
+    ends the process: refused before anything reaches the leaf.  Graphs are known by the operators of this module and of linear8 in
+    them."""
     if not torch.cuda.is_current_stream_capturing():
         return
-    mine = _leaves(ctx)
     with _eager_lock:
         others = [r() for r in _eager_graphs]
-    if any(a is b for o in others if o is not None and o is not ctx for a in _leaves(o) for b in mine):
+    others = [o for o in others if o is not None and o is not ctx]
+    if others and _leaves(ctx).keys() & _leaves(*others).keys():
         raise RuntimeError("a backward cannot be captured while a graph of the same leaves, recorded on the default stream, lives: drop "
                            "its outputs first, or record it on another stream")
 
