@@ -118,20 +118,29 @@ class HipAttentionOps:
         return self.gate_residual(x, linear(h), gate)
 
 
-def _state(*params):
-    return tuple((p.data_ptr(), p._version) for p in params)
+class _Snapshot:
+    """The parameters that 8-bit blocks were made from: their memory, held so that no other tensor can come to lie there, and the
+    writes to it that autograd has counted.  Writes through `p.data` are not counted and cannot be seen.  A copy of the model has
+    parameters of its own: its snapshot is empty, and refused."""
+    __slots__ = ("of",)
 
+    def __init__(self, *params):
+        self.of = tuple((p.detach(), p._version) for p in params)
 
-def _check_packed(was, *params):
-    if was != _state(*params):
-        raise RuntimeError("a layer's parameters have changed since pack_linear8: call it again")
+    def __reduce__(self):
+        return _Snapshot, ()
+
+    def check(self, *params):
+        if len(self.of) != len(params) or not all(p._version == version and p.device == t.device and t.is_set_to(p)
+                                                  for (t, version), p in zip(self.of, params)):
+            raise RuntimeError("a layer's parameters have changed since pack_linear8: call it again")
 
 
 def _packed8(layer):
     """The 8-bit form that `CausalWanModel.pack_linear8` has given a layer, None without one or where gradients are wanted."""
     w8 = None if torch.is_grad_enabled() else getattr(layer, "weight8", None)
     if w8 is not None:
-        _check_packed(layer.weight8_of, layer.weight)
+        layer.weight8_of.check(layer.weight)
     return w8
 
 
@@ -316,7 +325,7 @@ class CausalWanSelfAttention(nn.Module):
         self.norm_k = WanRMSNorm(dim, eps=eps)
         self._rope = None
         self._qkv = None
-        self.qkv8 = None           # (the three projections' weight in 8-bit blocks, their bias): CausalWanModel.pack_linear8
+        self.qkv8 = self.qkv8_of = None           # (the three projections' weight in 8-bit blocks, their bias): CausalWanModel.pack_linear8
 
     def _qkv_params(self):
         return [p for layer in (self.q, self.k, self.v) for p in (layer.weight, layer.bias)]
@@ -327,7 +336,7 @@ class CausalWanSelfAttention(nn.Module):
         column slices of one [B, S, 3C] tensor, which the prologue reads through its row stride."""
         c = self.dim
         if self.qkv8 is not None:
-            _check_packed(self.qkv8_of, *self._qkv_params())
+            self.qkv8_of.check(*self._qkv_params())
             y = _l8.linear8(x, *self.qkv8)
             return y[..., :c], y[..., c:2 * c], y[..., 2 * c:]
         ws = (self.q.weight, self.k.weight, self.v.weight)
@@ -525,18 +534,21 @@ class CausalWanModel(nn.Module):
     def pack_linear8(self, on=True):
         """Lays the blocks' linear layers out in 8-bit blocks of 128 (linear8.pack): self-attention's q, k, v as one weight, the
         output projections, cross-attention's q, and the feed-forward.  Passes without gradients then run them on 8-bit products
-        (weights and activations as e4m3, fp32 sums).  The 16-bit weights stay; call it again after they change or move (a pass before
-        that is refused), `on=False` goes back to them.  Returns the model."""
+        (weights and activations as e4m3, fp32 sums).  The 16-bit weights stay, their memory is held until the next call; `on=False` goes
+        back to them.  The blocks are a snapshot: call it again after the weights change or move.  A pass before that is refused where
+        autograd has counted the change (a write under no_grad, an optimiser's step, load_state_dict) or a parameter has other memory
+        (`to`, `p.data = t`); a write through `p.data`, such as `p.data.copy_(t)`, cannot be seen, and passes go on with the snapshot.
+        Returns the model."""
         for b in self.blocks:
             sa, ca = b.self_attn, b.cross_attn
-            sa.qkv8 = None
+            sa.qkv8 = sa.qkv8_of = None
             if on:
                 ws = torch.cat((sa.q.weight, sa.k.weight, sa.v.weight), 0)
                 sa.qkv8 = (_l8.pack(ws, transposed=False), torch.cat((sa.q.bias, sa.k.bias, sa.v.bias), 0))
-                sa.qkv8_of = _state(*sa._qkv_params())
+                sa.qkv8_of = _Snapshot(*sa._qkv_params())
             for layer in (sa.o, ca.q, ca.o, b.ffn[0], b.ffn[2]):
                 layer.weight8 = _l8.pack(layer.weight, transposed=False) if on else None
-                layer.weight8_of = _state(layer.weight)
+                layer.weight8_of = _Snapshot(layer.weight) if on else None
         return self
 
     def _patchify(self, x):
