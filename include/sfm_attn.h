@@ -330,7 +330,7 @@ int sfm_linear(const sfm_linear_desc* desc, const void* x, const void* w, const 
  *
  * A block is 128 consecutive values of a row (of a weight: 128 x 128).  It has the smallest power of two 2^s with max |v| <= 448 *
  * 2^s over its finite values (s = 0 for a block of zeros; s >= -126); a value is kept as e4m3 (OCP) of v * 2^-s, ties to even, one
- * that is not finite as NaN.
+ * that is not finite as NaN, one that would round up to 2^128 (from 248 * 2^120 on) as 240 * 2^120.
  *   rows     data: rows x SFM_PAD8(K) bytes, zeros past K.  scale: SFM_ROWS8_SCALE_BYTES(rows, K) bytes of s + 127; row r, block
  *            column kb at ((kb * ceil(rows / 128) + r / 128) * 32 + r % 32) * 4 + r % 128 / 32.
  *   weights  data: N x SFM_PAD8(K) bytes, scale: ceil(N / 128) rows of SFM_PITCH8(K) bytes, zeros past the blocks; data_t,

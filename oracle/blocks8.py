@@ -24,14 +24,16 @@ def exponents(v, square=False):
 
 
 def values(v, square=False):
-    """What the blocks of v [R, K] hold, in float64 (NaN where v is not finite)."""
+    """What the blocks of v [R, K] hold, in float64 (NaN where v is not finite; 240 * 2^120 where it would round up to 2^128)."""
     v = v.double()
     R, K = v.shape
     s = exponents(v, square).repeat_interleave(128 if square else 1, 0)[:R].repeat_interleave(128, 1)[:, :K]
     a = v / _pow2(s)
     _, e = torch.frexp(a.abs().clamp_min(2.0 ** -6))
     step = _pow2(e - 4)                   # e4m3: 3 bits behind the leading one, subnormals below 2^-6
-    return torch.where(v.isfinite(), torch.round(a / step) * step * _pow2(s), float("nan"))
+    q = torch.round(a / step) * step * _pow2(s)
+    q = torch.where(q.abs() >= 2.0 ** 128, q.sign() * 240 * 2.0 ** 120, q)
+    return torch.where(v.isfinite(), q, float("nan"))
 
 
 def gelu(x):

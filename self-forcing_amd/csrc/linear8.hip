@@ -209,7 +209,7 @@ __global__ __launch_bounds__(64 * W) void l8_few_kernel(L8Args p, const uint16_t
             return fmaxf(m, __shfl_xor(m, 32));
         };
         float a = block_max(mag_max<32>(v));
-        if (__builtin_expect(a > 3.402823466e38f, 0)) a = block_max(mag_max_finite<32>(v));
+        if (__builtin_expect(a >= kTop8, 0)) a = block_max(mag_max_finite<32>(v));
         const int s = block_exp8(a);
         const float inv = two_to(-s);
         i32x8 xf;

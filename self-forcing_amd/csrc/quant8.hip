@@ -160,7 +160,7 @@ __global__ __launch_bounds__(256) void pack8_kernel(const void* w, int64_t ws, i
         return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
     };
     a = block_max(a);
-    if (a > 3.402823466e38f) {                       // the same for the whole workgroup
+    if (a >= kTop8) {                                 // the same for the whole workgroup
         a = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) a = fmaxf(a, mag_max_finite<8>(v[i]));

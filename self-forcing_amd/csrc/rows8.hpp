@@ -3,7 +3,7 @@
 //
 // 8-bit blocks: 128 consecutive values of a row share a power of two 2^s, the smallest with max |v| <= 448 * 2^s over the
 // finite values (s = 0 for a block of zeros, never below -126); a value is kept as e4m3 of v * 2^-s, ties to even, one
-// that is not finite as NaN.  Powers of two cost up to one bit of the e4m3 range against a free scale and nothing of its
+// that is not finite as NaN, and one that would round up to 2^128 (from 248 * 2^120, 3.3e38, on) as 240 * 2^120.  Powers of two cost up to one bit of the e4m3 range against a free scale and nothing of its
 // relative precision (half a step is 2^-4 either way), and the scaled matrix instructions apply them: no product needs a
 // multiplication of its own per block, and the 8-bit value times its scale is exact in bf16.
 //
@@ -89,6 +89,12 @@ __device__ __forceinline__ float finite_mag(float v) {
     const float a = fabsf(v);
     return a <= 3.402823466e38f ? a : 0.f;
 }
+// Blocks with a magnitude from here on hold values that are not finite, or finite ones that e4m3 would round up to 2^128
+constexpr float kTop8 = 0x1.fp127f;                       // 248 * 2^120
+__device__ __forceinline__ float below_top8(float v) {
+    const float a = fabsf(v);
+    return a >= kTop8 && a <= 3.402823466e38f ? copysignf(0x1.ep127f, v) : v;         // 240 * 2^120
+}
 // four values, already divided by the block's scale, to e4m3: at most 448, or not finite, which the conversion turns into NaN
 __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
@@ -166,7 +172,7 @@ __device__ __forceinline__ float max16(float a) {
     a = fmaxf(a, turned(a, std::integral_constant<int, 2>{}));
     return fmaxf(a, turned(a, std::integral_constant<int, 1>{}));
 }
-// largest magnitude of N values, not numbers left out; infinite values are (with their block redone by `finite_mag`) the rare case
+// largest magnitude of N values, not numbers left out; from kTop8 on a block is redone by `mag_max_finite`, the rare case
 template <int N>
 __device__ __forceinline__ float mag_max(const float* v) {
     float a = 0.f;
@@ -174,17 +180,24 @@ __device__ __forceinline__ float mag_max(const float* v) {
     for (int i = 0; i < N; ++i) a = fmaxf(a, fabsf(v[i]));
     return a;
 }
+// of the finite ones, which are brought below kTop8
 template <int N>
-__device__ __forceinline__ float mag_max_finite(const float* v) {
+__device__ __forceinline__ float mag_max_finite(float* v) {
     float a = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) a = fmaxf(a, finite_mag(v[i]));
+    for (int i = 0; i < N; ++i) {
+        v[i] = below_top8(v[i]);
+        a = fmaxf(a, finite_mag(v[i]));
+    }
     return a;
 }
 // 8 values of each of 16 lanes that make a block: the block's exponent, and the lane's bytes
-__device__ __forceinline__ int quantize_block8(const float* v, u32x2* q) {
+__device__ __forceinline__ int quantize_block8(const float* v0, u32x2* q) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = v0[i];
     float a = max16(mag_max<8>(v));
-    if (__builtin_expect(a > 3.402823466e38f, 0)) a = max16(mag_max_finite<8>(v));
+    if (__builtin_expect(a >= kTop8, 0)) a = max16(mag_max_finite<8>(v));
     const int s = block_exp8(a);
     const float inv = two_to(-s);
     q->x = pack_e4m3(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);

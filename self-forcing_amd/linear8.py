@@ -7,7 +7,7 @@ layers are 16 bits (wan/modules/model.py:592-650).
 
 A block is 128 consecutive values of a row (128 x 128 of a weight) with the smallest power of two 2^s such that their largest
 magnitude is at most 448 * 2^s; a value is kept as e4m3 of v / 2^s, ties to even (half a step: 2^-4 of it), NaN where it is not
-finite.
+finite, 240 * 2^120 where it would round up to 2^128.
 
 The gradients are those of the product with the rounding passed through: dx = dy8 w8 (dy in 8-bit blocks too), dw = dy^T x8 with dy
 as it is, dbias = sum of dy."""

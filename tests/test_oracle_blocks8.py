@@ -53,3 +53,9 @@ def test_gradients_against_differences():
     t = torch.linspace(-8, 8, 101, dtype=torch.float64)
     assert ((o.gelu(t + h) - o.gelu(t - h)) / (2 * h) - o.gelu_slope(t)).abs().max() < 1e-8
     assert (o.gelu(t) - torch.nn.functional.gelu(t, approximate="tanh")).abs().max() < 1e-12
+
+
+def test_values_at_the_top_of_the_range_stay_finite():
+    """248 * 2^120 lies half way between 240 and 256 steps of 2^120, of which the latter is 2^128."""
+    v = torch.tensor([[3.39e38, -3.39e38, 248 * 2.0 ** 120, 247.9 * 2.0 ** 120, 3.0e38]], dtype=torch.float64)
+    assert (o.values(v) / 2.0 ** 120).tolist() == [[240.0, -240.0, 240.0, 240.0, 224.0]]
