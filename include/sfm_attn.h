@@ -376,8 +376,9 @@ int sfm_linear8_fwd(const sfm_linear8_desc* desc, const void* x, int64_t x_strid
                     const void* wscale, const void* bias, const void* res, const void* gate, void* out, void* stream);
 
 /* Gradients of a linear layer's weight and bias: dw[n][k] = sum_m dy[m][n] x[m][k] from the rows that the forward kept in 8 bits
- * (dy as it is; [N, K] contiguous), dbias[n] = sum_m dy[m][n]; either may be NULL.  16-bit tensors, fp32 sums in a fixed order, one
- * rounding.  colsum: dy's column sums where sfm_quantize8 has formed them (NULL: formed here, in the workspace). */
+ * (dy as it is; [N, K] contiguous), dbias[n] = sum_m dy[m][n]; either may be NULL.  The rows' values enter in
+ * the dtype: exact in bf16, in fp16 saturated at 65504 (of fp16 rows those that were rounded up to 65536; blocks of other types may pass it by
+ * far).  16-bit tensors, fp32 sums in a fixed order, one rounding.  colsum: dy's column sums where sfm_quantize8 has formed them (NULL: formed here, in the workspace). */
 int sfm_linear8_wgrad_workspace_bytes(int64_t M, int32_t N, int32_t K, size_t* bytes);
 int sfm_linear8_wgrad(int32_t dtype, int64_t M, int32_t N, int32_t K, const void* dy, int64_t dy_stride, const void* x8,
                       const void* xscale, void* dw, void* dbias, const float* colsum, void* workspace, size_t workspace_bytes,

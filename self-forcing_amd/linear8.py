@@ -10,7 +10,7 @@ magnitude is at most 448 * 2^s; a value is kept as e4m3 of v / 2^s, ties to even
 finite, 240 * 2^120 where it would round up to 2^128.
 
 The gradients are those of the product with the rounding passed through: dx = dy8 w8 (dy in 8-bit blocks too), dw = dy^T x8 with dy
-as it is, dbias = sum of dy."""
+as it is, dbias = sum of dy.  (In fp16 dw takes 65504 for a value of x8 that was rounded up to 65536.)"""
 import ctypes as C
 import functools
 
@@ -162,7 +162,8 @@ def _bytes(query, rows, N, K, device_index):
 
 
 def weight_grad(dy, x8):
-    """(dw [N, K], dbias [N]) of a layer from its output's gradient dy [B, L, N] and the rows its forward kept in 8 bits."""
+    """(dw [N, K], dbias [N]) of a layer from its output's gradient dy [B, L, N] and the rows its forward kept in 8 bits (of
+    fp16 rows where dy is fp16; a row's value then counts as 65504 where its block rounded it up to 65536)."""
     dy = dy.detach()
     if dy.dtype not in _HALF:
         raise ValueError("weight_grad takes float16 / bfloat16 gradients")
@@ -170,6 +171,8 @@ def weight_grad(dy, x8):
         raise ValueError("expected dy [B, L, N] and the Rows8 of a [B, L, K] input")
     if dy.device != x8.device:
         raise ValueError(f"dy on {dy.device}, the rows on {x8.device}")
+    if dy.dtype == torch.float16 and x8.dtype != torch.float16:
+        raise ValueError(f"dy: {dy.dtype}, whose range the rows of {x8.dtype} may pass")
     dy = _even(dy)
     rows, N, dys = _rows(dy)
     K = x8.shape[2]
