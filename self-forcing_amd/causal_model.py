@@ -335,7 +335,7 @@ class CausalWanSelfAttention(nn.Module):
         three Linear layers; the concatenation is rebuilt when one of them changes).  The three results are
         column slices of one [B, S, 3C] tensor, which the prologue reads through its row stride."""
         c = self.dim
-        if self.qkv8 is not None:
+        if self.qkv8 is not None and not torch.is_grad_enabled():
             self.qkv8_of.check(*self._qkv_params())
             y = _l8.linear8(x, *self.qkv8)
             return y[..., :c], y[..., c:2 * c], y[..., 2 * c:]

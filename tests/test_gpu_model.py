@@ -233,3 +233,21 @@ def test_packed_layers_refuse_parameters_that_have_changed():
             flow()
         dev_gen.model.pack_linear8()
         assert not torch.equal(flow(), before)
+
+
+def test_layers_of_a_packed_block_with_gradients_enabled_are_the_16_bit_ones():
+    """Bit for bit as before pack_linear8, for an input that wants a gradient or not; without gradients the 8-bit ones.  (The model's own
+    forward runs without.)"""
+    _, dev_gen = _pair(use_framewise=True)
+    block = dev_gen.model.blocks[0]
+    x = torch.randn(1, 312, 256, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).to("cuda:0")
+
+    def layers(t):
+        y = [*block.self_attn._project_qkv(t), block.ops.linear(t, block.self_attn.o), block.ops.linear_gelu(t, block.ffn[0])]
+        return [v.detach() for v in y]
+    plain = layers(x)
+    dev_gen.model.pack_linear8()
+    for t in (x, x.clone().requires_grad_()):
+        assert all(torch.equal(a, b) for a, b in zip(layers(t), plain))
+    with torch.no_grad():
+        assert not any(torch.equal(a, b) for a, b in zip(layers(x), plain))

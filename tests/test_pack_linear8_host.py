@@ -93,3 +93,18 @@ def test_unpacked_layers_hold_nothing(model):
     model.pack_linear8(False)
     for b in model.blocks:
         assert b.self_attn.qkv8 is None and b.self_attn.qkv8_of is None and b.ffn[0].weight8 is None and b.ffn[0].weight8_of is None
+
+
+def test_with_gradients_enabled_every_layer_is_the_16_bit_one(model, monkeypatch):
+    def reached(*args, **kw):
+        raise AssertionError("the 8-bit layer")
+    monkeypatch.setattr(cm._l8, "linear8", reached)
+    sa, ops = model.blocks[0].self_attn, model.blocks[0].ops
+    x = torch.randn(1, 2, 64).to(torch.bfloat16)
+    qkv = [sa.q, sa.k, sa.v]
+    ref = torch.nn.functional.linear(x, torch.cat([m.weight for m in qkv]), torch.cat([m.bias for m in qkv]))
+    assert torch.equal(torch.cat(sa._project_qkv(x), -1), ref)
+    assert torch.equal(ops.linear(x, sa.o), sa.o(x))
+    for call in (lambda: sa._project_qkv(x), lambda: ops.linear(x, sa.o)):
+        with torch.no_grad(), pytest.raises(AssertionError, match="the 8-bit layer"):
+            call()
