@@ -465,7 +465,8 @@ class CausalWanAttentionBlock(nn.Module):
         if getattr(ops, "own_gemm", False):
             x = ops.linear_gate_residual(x, h, self.ffn[2], e[5])
             return x, ops.ln_modulate(x, next_mod[0], next_mod[1], self.eps)
-        return ops.gate_residual_ln(x, ops.linear(h, self.ffn[2]), e[5], self.eps, scale=next_mod[0], shift=next_mod[1])
+        y = self.ffn[2](h) if _packed8(self.ffn[2]) is None else ops.linear(h, self.ffn[2])
+        return ops.gate_residual_ln(x, y, e[5], self.eps, scale=next_mod[0], shift=next_mod[1])
 
 
 class CausalHead(nn.Module):

@@ -108,3 +108,35 @@ def test_with_gradients_enabled_every_layer_is_the_16_bit_one(model, monkeypatch
     for call in (lambda: sa._project_qkv(x), lambda: ops.linear(x, sa.o)):
         with torch.no_grad(), pytest.raises(AssertionError, match="the 8-bit layer"):
             call()
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_the_feed_forwards_second_layer_is_the_librarys_unless_packed(monkeypatch, packed):
+    """own_gemm="auto" is for the block's square projections, however small the feed-forward is."""
+    class Ops(cm.HipAttentionOps):
+        def __init__(self):
+            super().__init__("auto")
+            self.through = []
+
+        def linear(self, x, linear):
+            self.through.append(linear)
+            return linear(x)
+
+        def linear_gelu(self, x, linear):
+            return linear(x)
+
+        def ln_modulate(self, x, scale, shift, eps):
+            return x
+
+        def gate_residual_ln(self, x, y, gate, eps, **kw):
+            return x + y, x + y
+    ops = Ops()
+    block = cm.CausalWanAttentionBlock(64, 128, 2, frame_hw=(2, 3), total_seq_len=36, ops=ops)
+    monkeypatch.setattr(block.self_attn, "forward", lambda x, *a: x)
+    monkeypatch.setattr(block.cross_attn, "forward", lambda x, *a: x)
+    if packed:
+        block.ffn[2].weight8, block.ffn[2].weight8_of = object(), cm._Snapshot(block.ffn[2].weight)
+    x, e = torch.randn(1, 6, 64), torch.randn(1, 1, 6, 64)
+    with torch.no_grad():
+        block(x, e, None, None, None, None, 0, next_mod=(e[:, :, 0], e[:, :, 1]))
+    assert (block.ffn[2] in ops.through) == packed
