@@ -533,21 +533,26 @@ class CausalWanModel(nn.Module):
 
     @torch.no_grad()
     def pack_linear8(self, on=True):
-        """Lays the blocks' linear layers out in 8-bit blocks of 128 (linear8.pack): self-attention's q, k, v as one weight, the
+        """Lays the blocks' linear layers (16 bits) out in 8-bit blocks of 128 (linear8.pack): self-attention's q, k, v as one weight, the
         output projections, cross-attention's q, and the feed-forward.  Passes without gradients then run them on 8-bit products
         (weights and activations as e4m3, fp32 sums).  The 16-bit weights stay, their memory is held until the next call; `on=False` goes
         back to them.  The blocks are a snapshot: call it again after the weights change or move.  A pass before that is refused where
         autograd has counted the change (a write under no_grad, an optimiser's step, load_state_dict) or a parameter has other memory
         (`to`, `p.data = t`); a write through `p.data`, such as `p.data.copy_(t)`, cannot be seen, and passes go on with the snapshot.
         Returns the model."""
+        def layers(b):
+            return b.self_attn.o, b.cross_attn.q, b.cross_attn.o, b.ffn[0], b.ffn[2]
+        if on and any(p.dtype not in _blk._HALF for b in self.blocks
+                      for p in b.self_attn._qkv_params() + [p for m in layers(b) for p in m.parameters()]):
+            raise ValueError("pack_linear8 takes float16 / bfloat16 layers: the rows that reach them are 16 bits")
         for b in self.blocks:
-            sa, ca = b.self_attn, b.cross_attn
+            sa = b.self_attn
             sa.qkv8 = sa.qkv8_of = None
             if on:
                 ws = torch.cat((sa.q.weight, sa.k.weight, sa.v.weight), 0)
                 sa.qkv8 = (_l8.pack(ws, transposed=False), torch.cat((sa.q.bias, sa.k.bias, sa.v.bias), 0))
                 sa.qkv8_of = _Snapshot(*sa._qkv_params())
-            for layer in (sa.o, ca.q, ca.o, b.ffn[0], b.ffn[2]):
+            for layer in layers(b):
                 layer.weight8 = _l8.pack(layer.weight, transposed=False) if on else None
                 layer.weight8_of = _Snapshot(layer.weight) if on else None
         return self

@@ -140,3 +140,14 @@ def test_the_feed_forwards_second_layer_is_the_librarys_unless_packed(monkeypatc
     with torch.no_grad():
         block(x, e, None, None, None, None, 0, next_mod=(e[:, :, 0], e[:, :, 1]))
     assert (block.ffn[2] in ops.through) == packed
+
+
+def test_layers_of_32_bits_are_refused_before_any_is_packed(model):
+    was = [b.self_attn.qkv8_of for b in model.blocks]
+    model.packed.clear()
+    model.blocks[1].ffn[2].float()
+    with pytest.raises(ValueError, match="float16 / bfloat16 layers"):
+        model.pack_linear8()
+    assert not model.packed and was == [b.self_attn.qkv8_of for b in model.blocks]
+    model.pack_linear8(False)
+    model.half().pack_linear8()
