@@ -102,6 +102,7 @@ def pack(weight, transposed=True):
     N, K = weight.shape
     if N < 1 or K < 1:
         raise ValueError("weight is empty")
+    ws = weight.stride(0) if N > 1 else K            # the stride of a dimension of one says nothing
 
     def blocks(n, k):
         return (torch.empty((n, _pad(k)), dtype=torch.uint8, device=weight.device),
@@ -109,7 +110,7 @@ def pack(weight, transposed=True):
     data, scale = blocks(N, K)
     data_t, scale_t = blocks(K, N) if transposed else (None, None)
     with _on_device(weight.device):
-        _l.check(_l.load().sfm_pack8(_DT[weight.dtype], N, K, weight.data_ptr(), weight.stride(0), data.data_ptr(), scale.data_ptr(),
+        _l.check(_l.load().sfm_pack8(_DT[weight.dtype], N, K, weight.data_ptr(), ws, data.data_ptr(), scale.data_ptr(),
                                      data_t.data_ptr() if transposed else None, scale_t.data_ptr() if transposed else None, _stream(weight)))
     return Weight8(data, scale, data_t, scale_t, (N, K), weight.dtype)
 
