@@ -120,7 +120,8 @@ def _ln_keep8(x, mod, eps):
 def _ln_bwd_bytes(rows, C, group, device_index):
     """Workspace of sfm_ln_bwd on a device (its compute units are in the size)."""
     n = ctypes.c_size_t(0)
-    _l.check(_l.load().sfm_ln_bwd_workspace_bytes(rows, C, group, ctypes.byref(n)))
+    with torch.cuda.device(device_index):
+        _l.check(_l.load().sfm_ln_bwd_workspace_bytes(rows, C, group, ctypes.byref(n)))
     return n.value
 
 

@@ -158,7 +158,8 @@ def _forward(x, w8, bias, out, keep, epi=_l.EPI_NONE, res=None, gate=None):
 def _bytes(query, rows, N, K, device_index):
     """Workspace that the named query asks for on a device (its compute units are in the size)."""
     n = C.c_size_t(0)
-    _l.check(getattr(_l.load(), query)(rows, N, K, C.byref(n)))
+    with torch.cuda.device(device_index):
+        _l.check(getattr(_l.load(), query)(rows, N, K, C.byref(n)))
     return n.value
 
 
