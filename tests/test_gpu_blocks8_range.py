@@ -64,3 +64,16 @@ def test_gelu(dtype):
     dx, = torch.autograd.grad(y, leaf, torch.ones_like(leaf))
     assert torch.equal(y[0, 0].cpu(), x[0, 0]) and not y[0, 1].any()
     assert torch.equal(dx.cpu(), (x > 0).to(dtype))
+
+
+def test_a_weights_values_at_every_scale():
+    """The values of a packed weight are the blocks' own, bit for bit, for every exponent a block can have."""
+    e = torch.arange(-126, 120)
+    w = torch.zeros((128 * len(e), 130))
+    w[::128, 0] = torch.pow(2.0, e.double() + 8).float()                # 256 * 2^s: more than 448 * 2^(s - 1)
+    w[1::128] = w[::128, :1] * torch.rand((1, 130), generator=torch.Generator().manual_seed(5))
+    p = l8.pack(w.to(DEV))
+    assert p.scale[:, 0].tolist() == (e + 127).tolist()
+    ref = o.values(w, True)
+    assert torch.equal(p.dequantize(torch.float32).double().cpu(), ref.float().double())
+    assert torch.equal(p.dequantize(torch.bfloat16).double().cpu(), ref.to(torch.bfloat16).double())
