@@ -375,6 +375,12 @@ int sfm_linear8(const sfm_linear8_desc* desc, const void* x8, const void* xscale
 int sfm_linear8_fwd(const sfm_linear8_desc* desc, const void* x, int64_t x_stride, void* data, void* scale, const void* w8,
                     const void* wscale, const void* bias, const void* res, const void* gate, void* out, void* stream);
 
+/* Which kernels these products and the weight's gradient take on the current device, for tests and profiles.  tile_rows: 256 or 128 rows
+ * of an LDS tile, 0 for the kernels without; half_strip: 1 where the last strip of 256-row tiles has half of them.  tile: 256 or 128
+ * channels squared, parts: of the rows, joined behind the product. */
+int sfm_linear8_plan(int64_t M, int32_t N, int32_t K, int32_t* tile_rows, int32_t* half_strip);
+int sfm_linear8_wgrad_plan(int64_t M, int32_t N, int32_t K, int32_t* tile, int32_t* parts);
+
 /* Gradients of a linear layer's weight and bias: dw[n][k] = sum_m dy[m][n] x[m][k] from the rows that the forward kept in 8 bits
  * (dy as it is; [N, K] contiguous), dbias[n] = sum_m dy[m][n]; either may be NULL.  The rows' values enter in
  * the dtype: exact in bf16, in fp16 saturated at 65504 (of fp16 rows those that were rounded up to 65536; blocks of other types may pass it by

@@ -606,7 +606,7 @@ __global__ __launch_bounds__(256) void l8_tile_kernel(L8Args p) {
 }
 
 template <class E, int EPI, int TB>
-int launch_tile(const L8Args& a0, hipStream_t st) {
+int launch_tile(const L8Args& a0, bool half, hipStream_t st) {
     static bool configured = false;          // the attribute belongs to the function; racing callers set the same value
     if (!configured) {
         hipError_t e = hipFuncSetAttribute((const void*)l8_tile_kernel<E, EPI, TB>, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes);
@@ -619,7 +619,7 @@ int launch_tile(const L8Args& a0, hipStream_t st) {
     L8Args a = a0;
     a.tm = (int)((a.M + 64 * TB - 1) / (64 * TB));
     a.tn = (a.N + kTileN - 1) / kTileN;
-    a.half = TB == 4 && a.M % 256 != 0 && a.M % 256 <= 128;
+    a.half = half;
     const int64_t full = ((int64_t)(a.tm - a.half) * a.tn + 7) / 8 * 8, halves = a.half ? (a.tn + 7) / 8 * 8 : 0;
     hipLaunchKernelGGL((l8_tile_kernel<E, EPI, TB>), dim3((unsigned)(full + halves)), dim3(256), kLdsBytes, st, a);
     return launched8("sfm_linear8");
@@ -629,16 +629,26 @@ int launch_tile(const L8Args& a0, hipStream_t st) {
 // a stage, 128 rows 7 + 0.9.  Measured on both sides: 4680 x 8960 -> 1536 (114 or 222 tiles, one round) 87 against 67; 4680 x 1536 ->
 // 8960 (665 or 1295) 82 against 99; 1560 x 1536 -> 8960 (245 or 455) 27 against 35.  The kernel without LDS runs at up to 0.5
 // PFLOP/s behind 6 us, and wins where the tiles are few: 512 x 1536 -> 1536 13 against 15, 1111 x 1000 -> 777 12 against 32.
+struct L8Plan {
+    int rows;                                // of a tile: 256 or 128; 0: the kernels without LDS tiles
+    bool half;                               // the last strip of 256-row tiles is made of half ones
+};
+L8Plan l8_plan(int64_t M, int N, int nkb) {
+    if (M <= 16) return {0, false};
+    const double cus = cu_count(), tn = (N + kTileN - 1) / kTileN;
+    auto rounds = [&](double tiles) { return tiles < cus ? 1.0 : tiles / cus + 0.3; };
+    const double t4 = rounds(tn * (double)((M + 255) / 256)) * (8.0 + 1.2 * nkb);
+    const double t2 = rounds(tn * (double)((M + 127) / 128)) * (7.0 + 0.9 * nkb);
+    const double flops = 2.0 * M * N * nkb * kBlock8, direct = 6.0 + 0.35 * nkb + flops / 0.5e9;
+    if (direct < t2 && direct < t4) return {0, false};
+    return t2 < t4 ? L8Plan{128, false} : L8Plan{256, M % 256 != 0 && M % 256 <= 128};
+}
 template <class E, int EPI>
 int launch_epi(const L8Args& a, hipStream_t st) {
     if (a.M <= 16) return few_wide(a) ? launch_direct<E, EPI, 1, 1, 16>(a, st) : launch_direct<E, EPI, 1, 1, 8>(a, st);
-    const double cus = cu_count(), tn = (a.N + kTileN - 1) / kTileN;
-    auto rounds = [&](double tiles) { return tiles < cus ? 1.0 : tiles / cus + 0.3; };
-    const double t4 = rounds(tn * (double)((a.M + 255) / 256)) * (8.0 + 1.2 * a.nkb);
-    const double t2 = rounds(tn * (double)((a.M + 127) / 128)) * (7.0 + 0.9 * a.nkb);
-    const double flops = 2.0 * a.M * a.N * a.kp, direct = 6.0 + 0.35 * a.nkb + flops / 0.5e9;
-    if (direct < t2 && direct < t4) return launch_direct<E, EPI, 4, 2, 8>(a, st);
-    return t2 < t4 ? launch_tile<E, EPI, 2>(a, st) : launch_tile<E, EPI, 4>(a, st);
+    const L8Plan plan = l8_plan(a.M, a.N, a.nkb);
+    return plan.rows == 0 ? launch_direct<E, EPI, 4, 2, 8>(a, st) : plan.rows == 128 ? launch_tile<E, EPI, 2>(a, false, st)
+                                                                                     : launch_tile<E, EPI, 4>(a, plan.half, st);
 }
 
 template <class E>
@@ -656,6 +666,12 @@ int few_dtype(const L8Args& a, int epilogue, const void* x, int64_t xstride, int
 }
 
 }  // namespace
+
+int tile_rows8(int64_t M, int N, int K, bool* half_strip) {
+    const L8Plan plan = l8_plan(M, N, blocks8(K));
+    *half_strip = plan.half;
+    return plan.rows;
+}
 
 int launch_linear8(const sfm_linear8_desc& d, const void* x, int64_t x_stride, const void* x8, const void* xscale, const void* w8,
                    const void* wscale, const void* bias, const void* res, const void* gate, void* out, hipStream_t stream) {

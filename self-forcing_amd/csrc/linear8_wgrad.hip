@@ -448,6 +448,12 @@ WgradPlan wgrad_plan(int64_t M, int N, int K) {
 
 }  // namespace
 
+int wgrad8_tile_size(int64_t M, int N, int K, int* parts) {
+    const WgradPlan plan = wgrad_plan(M, N, K);
+    *parts = plan.splits;
+    return plan.big ? kBT : kWT;
+}
+
 size_t wgrad8_workspace_bytes(int64_t M, int N, int K, bool bias) {
     const int s = wgrad_plan(M, N, K).splits;
     size_t b = s > 1 ? (size_t)s * N * K * sizeof(float) : 0;

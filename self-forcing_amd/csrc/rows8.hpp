@@ -250,8 +250,10 @@ int launch_pack8(int dtype, int N, int K, const void* w, int64_t ws, void* data,
 constexpr int kFewRows8 = SFM_LINEAR8_FEW_ROWS;
 int launch_linear8(const sfm_linear8_desc& d, const void* x, int64_t x_stride, const void* x8, const void* xscale, const void* w8,
                    const void* wscale, const void* bias, const void* res, const void* gate, void* out, hipStream_t stream);
+int tile_rows8(int64_t M, int N, int K, bool* half_strip);
 // linear8_wgrad.hip; `colsum`: column sums of dy by kColRows8 rows where a quantisation has formed them, else null
 size_t wgrad8_workspace_bytes(int64_t M, int N, int K, bool bias);
+int wgrad8_tile_size(int64_t M, int N, int K, int* parts);
 int launch_wgrad8(int dtype, int64_t M, int N, int K, const void* dy, int64_t dy_stride, const void* x8, const void* xscale, void* dw,
                   void* dbias, const float* colsum, void* workspace, hipStream_t st);
 // ln_train.hip; launch_sum_parts: out[g][c] = sum over s of part[g][s][c], two halves of the columns to out1 and out2 if that is given

@@ -1560,6 +1560,32 @@ int sfm_linear8_fwd(const sfm_linear8_desc* d, const void* x, int64_t x_stride, 
     return launch_linear8(*d, x, x_stride, data, scale, w8, wscale, bias, gr ? res : nullptr, gr ? gate : nullptr, out, (hipStream_t)stream);
 }
 
+int sfm_linear8_plan(int64_t M, int32_t N, int32_t K, int32_t* tile_rows, int32_t* half_strip) {
+    if (!tile_rows || !half_strip) {
+        set_error("tile_rows and half_strip must be non-NULL");
+        return SFM_ERR_NULL;
+    }
+    int rc = check_rows8(SFM_BF16, M, K, false);
+    if (!rc) rc = check_rows8(SFM_BF16, M, N, false);
+    if (rc) return rc;
+    bool half;
+    *tile_rows = tile_rows8(M, N, K, &half);
+    *half_strip = half;
+    return SFM_OK;
+}
+
+int sfm_linear8_wgrad_plan(int64_t M, int32_t N, int32_t K, int32_t* tile, int32_t* parts) {
+    if (!tile || !parts) {
+        set_error("tile and parts must be non-NULL");
+        return SFM_ERR_NULL;
+    }
+    int rc = check_rows8(SFM_BF16, M, K, false);
+    if (!rc) rc = check_rows8(SFM_BF16, M, N, false);
+    if (rc) return rc;
+    *tile = wgrad8_tile_size(M, N, K, parts);
+    return SFM_OK;
+}
+
 int sfm_linear8_wgrad_workspace_bytes(int64_t M, int32_t N, int32_t K, size_t* bytes) {
     if (!bytes) {
         set_error("bytes must be non-NULL");

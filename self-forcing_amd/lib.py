@@ -32,7 +32,7 @@ SYMBOLS = [
     "sfm_monarch_kept_bytes", "sfm_monarch_fwd_kept", "sfm_monarch_bwd_kept_workspace_bytes", "sfm_monarch_bwd_kept",
     "sfm_monarch_attn_with_kv_cache_kept", "sfm_dense_bwd_workspace_bytes", "sfm_dense_bwd", "sfm_probe_mfma_bf16", "sfm_probe_tile_traffic", "sfm_probe_row_stream", "sfm_probe_l2_read", "sfm_conv3d_cl", "sfm_vae_norm_act",
     "sfm_quantize8", "sfm_dequantize8", "sfm_pack8", "sfm_linear8", "sfm_linear8_fwd", "sfm_linear8_wgrad_workspace_bytes", "sfm_linear8_wgrad",
-    "sfm_linear8_bwd_workspace_bytes", "sfm_linear8_bwd",
+    "sfm_linear8_bwd_workspace_bytes", "sfm_linear8_bwd", "sfm_linear8_plan", "sfm_linear8_wgrad_plan",
     "sfm_gelu_bwd", "sfm_ln_keep8", "sfm_ln_bwd_workspace_bytes", "sfm_ln_bwd", "sfm_set_switches", "sfm_get_switches", "sfm_last_error", "sfm_version",
 ]
 
@@ -163,6 +163,7 @@ def load():
     lib.sfm_linear8_wgrad.argtypes = [I32, I64, I32, I32, P, I64, P, P, P, P, P, P, C.c_size_t, P]
     lib.sfm_linear8_bwd_workspace_bytes.argtypes = [I64, I32, I32, C.POINTER(C.c_size_t)]
     lib.sfm_linear8_bwd.argtypes = [I32, I64, I32, I32, P, I64, P, P, P, P, P, P, P, P, C.c_size_t, P]
+    lib.sfm_linear8_plan.argtypes = lib.sfm_linear8_wgrad_plan.argtypes = [I64, I32, I32, C.POINTER(I32), C.POINTER(I32)]
     lib.sfm_gelu_bwd.argtypes = [I32, I64, I32, P, I64, P, P, P, I64, P, I64, P]
     lib.sfm_ln_keep8.argtypes = [I32, I64, I32, C.c_float, P, I64, P, I64, P, P, I64, I32, P, P, P, P, P, P]
     lib.sfm_ln_bwd_workspace_bytes.argtypes = [I64, I32, I64, C.POINTER(C.c_size_t)]
