@@ -535,10 +535,11 @@ class CausalWanModel(nn.Module):
     def pack_linear8(self, on=True):
         """Lays the blocks' linear layers (16 bits) out in 8-bit blocks of 128 (linear8.pack): self-attention's q, k, v as one weight, the
         output projections, cross-attention's q, and the feed-forward.  Passes without gradients then run them on 8-bit products
-        (weights and activations as e4m3, fp32 sums).  The 16-bit weights stay, their memory is held until the next call; `on=False` goes
-        back to them.  The blocks are a snapshot: call it again after the weights change or move.  A pass before that is refused where
-        autograd has counted the change (a write under no_grad, an optimiser's step, load_state_dict) or a parameter has other memory
-        (`to`, `p.data = t`); a write through `p.data`, such as `p.data.copy_(t)`, cannot be seen, and passes go on with the snapshot.
+        (weights and activations as e4m3; linear8 says how they are summed).  The 16-bit weights stay, their memory is held until the next
+        call; `on=False` goes back to them.  The blocks are a snapshot: call it again after the weights change or move.  A pass before
+        that is refused where autograd has counted the change (a write under no_grad, an optimiser's step, load_state_dict) or a
+        parameter has other memory (`to`, `p.data = t`); a write through `p.data`, such as `p.data.copy_(t)`, cannot be seen, and passes
+        go on with the snapshot.
         Returns the model."""
         def layers(b):
             return b.self_attn.o, b.cross_attn.q, b.cross_attn.o, b.ffn[0], b.ffn[2]

@@ -202,7 +202,8 @@ __global__ __launch_bounds__(256) void wgrad8_kernel(WgradArgs p) {
 //
 // Bound by the matrix pipe: 4680 x 1536 x 8960 has 129 GFLOP, 80 us at the 1.6 PFLOP/s of a large bf16 product here, and takes 133 us
 // (0.97 PFLOP/s; a library product of 16-bit operands of this shape 158 us); its 210 tiles leave 46 of 256 compute units idle, which
-// alone makes 80 us 98.  Requests three steps ahead: 150 us.
+// alone makes 80 us 98.  Requests three steps ahead: 150 us.  It does not fit its registers: with both forms of the tile in one kernel
+// the compiler spills 50 vector and some 250 scalar registers (196 bytes of scratch a lane).
 template <class E, bool EDGE>
 __device__ __forceinline__ void wgrad8_tile(const WgradArgs& p, int n0, int kb, int64_t s0, int64_t s1, int split) {
     extern __shared__ __attribute__((aligned(256))) char w8_lds[];      // [buffer][dy tile | x tile]

@@ -6,9 +6,9 @@
 //   dx = r (g - mean(g) - xh mean(g xh))
 //   dw = sum dy xh, db = sum dy   over all rows (affine) or the rows of a frame (scale, shift)
 //
-// A row is read once into registers: its statistics are formed again from the same values in the same order as in the
-// forward (the row is there anyway; kept statistics would be another stream to read), then the sums of g and g (x - mean)
-// in one exchange.  The column sums dw, db stay in registers over all rows of a wave, meet in LDS, and leave as one fp32
+// A row is read once into registers: its statistics are formed again from the same values (the row is there anyway; kept
+// statistics would be another stream to read), up to 1536 channels in the forward's order, above that over four waves where the
+// forward has one, so that their last bits may differ; then the sums of g and g (x - mean) in one exchange.  The column sums dw, db stay in registers over all rows of a wave, meet in LDS, and leave as one fp32
 // partial per workgroup, which a second kernel adds in a fixed order: no atomics, the same result every time.
 //
 // Bound by memory: 21 frames of 1560 x 1536, modulated, 68-70 us and 5 for the partials (302 MB: 4.3 TB/s).  A chunk of 4680 x 1536 from
@@ -30,7 +30,7 @@ struct LnBwdArgs {
     const void* weight;      // [C], or scale rows (MOD) mod_stride apart
     float* part;             // [groups of rows][splits][2][C], unless a group has one workgroup, which stores dw and db itself
     void *dw, *db;
-    int64_t xs, dys, dxs, ms, rows, groups8;
+    int64_t xs, dys, dxs, ms, groups8;
     int C, rpg, splits;      // rows per group (of one weight gradient), workgroups per group
     float eps;
 };
@@ -284,7 +284,7 @@ __global__ __launch_bounds__(256) void ln_keep8_kernel(const void* x, int64_t xs
 
 // Workgroups per group of rows: three on every compute unit, or two, where that comes out nearly whole (a few more than two make
 // some units run three while the others wait: 21 frames of 1560 x 1536, 525 workgroups 76 us, 756 68), and four rows each at least.
-int ln_bwd_splits(int64_t groups, int64_t rpg, int C) {
+int ln_bwd_splits(int64_t groups, int64_t rpg) {
     const int64_t cus = cu_count(), most = (rpg + 3) / 4;
     for (int64_t k = 3; k >= 2; --k) {
         const int64_t s = k * cus / groups;
@@ -327,7 +327,7 @@ int launch_sum_parts(int dtype, int64_t parts, int64_t n, int64_t groups, const 
 
 size_t ln_bwd_workspace_bytes(int64_t rows, int C, int64_t rows_per_group) {
     const int64_t groups = rows / rows_per_group;
-    const int splits = ln_bwd_splits(groups, rows_per_group, C);
+    const int splits = ln_bwd_splits(groups, rows_per_group);
     return splits > 1 ? (size_t)groups * splits * 2 * C * sizeof(float) : 0;
 }
 
@@ -350,11 +350,10 @@ int launch_ln_bwd(int dtype, int64_t rows, int C, float eps, const void* x, int6
     a.dys = dys;
     a.dxs = dxs;
     a.ms = ms;
-    a.rows = rows;
     a.groups8 = (rows + kBlock8 - 1) / kBlock8;
     a.C = C;
     a.rpg = (int)rows_per_group;
-    a.splits = ln_bwd_splits(groups, rows_per_group, C);
+    a.splits = ln_bwd_splits(groups, rows_per_group);
     a.eps = eps;
     int rc = dtype == SFM_BF16 ? ln_bwd_m<BF16>(a, mod, groups, st) : dtype == SFM_F16 ? ln_bwd_m<F16>(a, mod, groups, st) : ln_bwd_m<float>(a, mod, groups, st);
     if (rc || a.splits == 1) return rc;

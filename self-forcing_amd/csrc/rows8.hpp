@@ -69,7 +69,6 @@ constexpr int kColRows8 = 32;          // rows of one partial column sum (sfm_qu
 
 __host__ __device__ inline int blocks8(int64_t k) { return (int)((k + kBlock8 - 1) / kBlock8); }
 __host__ __device__ inline int64_t pad8(int64_t k) { return (k + kBlock8 - 1) / kBlock8 * kBlock8; }
-__host__ __device__ inline int64_t scale_bytes8(int64_t rows, int64_t k) { return (int64_t)blocks8(k) * blocks8(rows) * kBlock8; }
 // bytes between the scales of two block rows of a weight: whole words, which a wave reads through the scalar cache
 __host__ __device__ inline int pitch8(int64_t k) { return (blocks8(k) + 3) & ~3; }
 // byte of row r in block column kb

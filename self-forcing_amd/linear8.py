@@ -2,12 +2,15 @@
 layers are 16 bits (wan/modules/model.py:592-650).
 
     w8 = pack(weight)                    # once, where the weights stay: half their memory
-    y = linear8(x, w8, bias)             # x in 8 bits per call, fp32 sums, one rounding
+    y = linear8(x, w8, bias)             # x in 8 bits per call, sums kept in fp32, one rounding
     y = linear8(x, weight, bias)         # under autograd: weight packed in the call, x kept in 8 bits for the weight's gradient
 
 A block is 128 consecutive values of a row (128 x 128 of a weight) with the smallest power of two 2^s such that their largest
 magnitude is at most 448 * 2^s; a value is kept as e4m3 of v / 2^s, ties to even (half a step: 2^-4 of it), NaN where it is not
 finite, 240 * 2^120 where it would round up to 2^128.
+
+The product runs on e4m3 matrix instructions, which add the products of 8 neighbouring channels before the fp32 sum and drop of them
+what is below 2^-13 of the largest: 1.7e-5 of the result on random rows, where the values' own rounding makes 2.6e-2.
 
 The gradients are those of the product with the rounding passed through: dx = dy8 w8 (dy in 8-bit blocks too), dw = dy^T x8 with dy
 as it is, dbias = sum of dy.  (In fp16 dw takes 65504 for a value of x8 that was rounded up to 65536.)"""

@@ -86,6 +86,24 @@ def test_gated_residual(dtype, size, plan):
     assert all(bool((buf[..., a:z] == 7).all()) for a, z in ((0, 1), (N + 1, N + 4), (2 * N + 4, 2 * N + 7)))
 
 
+@pytest.mark.parametrize("size", [(4, 256, 64), (528, 512, 256), TILE_128[1], next(iter(TILE_256))])
+@pytest.mark.parametrize("apart", [1, 8])
+def test_what_the_sums_of_eight_drop(size, apart):
+    """Two products of 2^16 that cancel, and one of 2^(16 - j), among the same 8 neighbouring channels or in the next 8: exact up to j = 13,
+    and off by less than 2^-13 of the largest beyond; in another 8 exact."""
+    M, K, N = size
+    x, w = torch.zeros((1, M, K), dtype=torch.bfloat16), torch.zeros((N, K), dtype=torch.bfloat16)
+    j = torch.arange(N) % 18                                          # 2^(8 - j) down to e4m3's least, 2^-9
+    x[..., 0] = x[..., 2] = 256
+    w[:, 0], w[:, 2] = 256, -256
+    k = 1 if apart == 1 else 9
+    x[..., k], w[:, k] = 256, torch.pow(2.0, 8.0 - j)
+    y, small = l8.linear8(x.to(DEV), w.to(DEV))[0].double().cpu(), torch.pow(2.0, 16.0 - j.double())
+    exact = (j <= 13) | (apart == 8)
+    assert torch.equal(y[:, exact], small[exact].expand(M, -1))
+    assert ((y - small).abs() < 2 * 2.0 ** 16 * 2.0 ** -13).all()
+
+
 def _wgrad(dy, x):
     d, v = dy.view(-1, dy.shape[-1]).double(), _values(x)
     if dy.dtype == torch.float16:
