@@ -335,7 +335,8 @@ int sfm_linear(const sfm_linear_desc* desc, const void* x, const void* w, const 
  *            column kb at ((kb * ceil(rows / 128) + r / 128) * 32 + r % 32) * 4 + r % 128 / 32.
  *   weights  data: N x SFM_PAD8(K) bytes, scale: ceil(N / 128) rows of SFM_PITCH8(K) bytes, zeros past the blocks; data_t,
  *            scale_t: the same of the transposed weight [K, N] (the same values), for the product with the output's gradient.
- * data and scale are 16-byte aligned.
+ * data and scale are 16-byte aligned.  Rows are counted in 31 bits; grids of 2^32 work-items or more (sfm_quantize8 from 2^29 rows on,
+ * sfm_ln_keep8 from 2^26) are refused by the runtime, SFM_ERR_HIP.
  *
  * sfm_quantize8: data / scale of x [rows, K] (rows x_stride apart, any alignment).  colsum (NULL or float [ceil(rows / 32)][K])
  *   receives the column sums of each 32 rows; y (NULL or [rows, K]): GELU (tanh) of x, rounded once.

@@ -183,10 +183,13 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(LnBwdArgs p) {
 // slices of the parts per workgroup, the slices in a fixed order; SL = 32 where there are parts enough: a thread's loads, eight at a
 // time, are then few one after the other (512 parts of 2 x 1536 columns: 5 us, with 8 slices 20)
 template <typename T, int SL>
-__global__ __launch_bounds__(32 * SL) void sum_parts_kernel(const float* part, int64_t parts, int64_t n, int64_t n1, void* out1, void* out2) {
+__global__ __launch_bounds__(32 * SL) void sum_parts_kernel(const float* part, int64_t parts, int64_t n, int64_t n1, int64_t groups, void* out1,
+                                                            void* out2) {
     __shared__ float sl[SL][32];
     const int l = threadIdx.x & 31, sn = threadIdx.x >> 5;
-    const int64_t cols = (n + 31) / 32, g = blockIdx.x / cols, c = (blockIdx.x % cols) * 32 + l;
+    const int64_t id = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    const int64_t cols = (n + 31) / 32, g = id / cols, c = (id % cols) * 32 + l;
+    if (g >= groups) return;
     float s = 0.f;
     if (c < n) {
         const float* p = part + (g * parts) * n + c;
@@ -310,9 +313,9 @@ int ln_bwd_m(const LnBwdArgs& a, bool mod, int64_t groups, hipStream_t st) {
 
 template <typename T>
 int sum_parts_t(int64_t parts, int64_t n, int64_t n1, int64_t groups, const float* part, void* out1, void* out2, hipStream_t st) {
-    const dim3 grid((unsigned)((n + 31) / 32 * groups));
-    if (parts >= 64) hipLaunchKernelGGL((sum_parts_kernel<T, 32>), grid, dim3(1024), 0, st, part, parts, n, n1, out1, out2);
-    else hipLaunchKernelGGL((sum_parts_kernel<T, 8>), grid, dim3(256), 0, st, part, parts, n, n1, out1, out2);
+    const dim3 grid = wide_grid((n + 31) / 32 * groups);
+    if (parts >= 64) hipLaunchKernelGGL((sum_parts_kernel<T, 32>), grid, dim3(1024), 0, st, part, parts, n, n1, groups, out1, out2);
+    else hipLaunchKernelGGL((sum_parts_kernel<T, 8>), grid, dim3(256), 0, st, part, parts, n, n1, groups, out1, out2);
     return launched8("sum of partials");
 }
 

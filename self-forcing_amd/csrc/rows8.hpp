@@ -230,6 +230,13 @@ __host__ __device__ inline RowRange rows_of_part(int64_t rows, int parts, int pa
     return {first, first + per < rows ? first + per : rows};
 }
 
+// `wgs` workgroups of up to 1024 threads as a grid: the runtime refuses 2^32 work-items or more along one dimension.  A kernel numbers
+// them blockIdx.y * gridDim.x + blockIdx.x, and those from wgs on have nothing to do.
+inline dim3 wide_grid(int64_t wgs) {
+    const int64_t x = wgs < (1 << 21) ? wgs : 1 << 21;
+    return dim3((unsigned)x, (unsigned)((wgs + x - 1) / x));
+}
+
 // the launch that precedes: SFM_OK, or SFM_ERR_HIP with the runtime's message
 inline int launched8(const char* what) {
     hipError_t e = hipGetLastError();

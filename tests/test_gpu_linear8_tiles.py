@@ -153,3 +153,15 @@ def test_weight_gradient_writes_its_channels_only(size):
     want[7], want[N - 1], want[:, 5], want[:, K - 1] = True, True, True, True
     assert torch.equal(bad, want)
     assert (~torch.isfinite(db[:N])).nonzero().flatten().tolist() == [7, N - 1]
+
+
+def test_weight_gradient_in_parts_of_more_than_two_grids_worth():
+    """More sums of parts than one grid dimension's 2^21 workgroups take: 600 rows of -1, 0 and 1 over and over, so that every sum is exact
+    in any order."""
+    n, times, C = 600, 100, 8200
+    assert wgrad_plan(n * times, C, C) == (256, 2) and C * C > 32 << 21
+    g = torch.Generator().manual_seed(41)
+    x, dy = (torch.randint(-1, 2, (1, n, C), generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    dw, db = l8.weight_grad(dy.repeat(1, times, 1), l8.quantize(x.repeat(1, times, 1)))
+    assert torch.equal(dw, (times * (dy[0].double().t() @ x[0].double())).to(torch.bfloat16))
+    assert torch.equal(db, (times * dy[0].double().sum(0)).to(torch.bfloat16))

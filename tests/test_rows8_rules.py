@@ -14,6 +14,11 @@ extern "C" void rows_of_part(int64_t rows, int parts, int part, int64_t* first, 
     *first = r.first;
     *last = r.last;
 }
+extern "C" void wide_grid(int64_t wgs, unsigned* x, unsigned* y) {
+    const dim3 g = sfm::wide_grid(wgs);
+    *x = g.x;
+    *y = g.y;
+}
 """
 
 
@@ -41,3 +46,12 @@ def test_the_parts_of_a_group_are_its_rows_once(rules, rows, parts):
         else:
             assert at == rows                                   # nothing is left
     assert at == rows
+
+
+@pytest.mark.parametrize("wgs", [1, 2, 4680, 2 ** 21 - 1, 2 ** 21, 2 ** 21 + 1, 23200 * 23200 // 32, 2 ** 31])
+def test_grids_stay_within_what_the_runtime_takes(rules, wgs):
+    x, y = C.c_uint(0), C.c_uint(0)
+    rules.wide_grid(C.c_int64(wgs), C.byref(x), C.byref(y))
+    assert x.value * 1024 < 2 ** 32 and y.value * 1024 < 2 ** 32
+    assert wgs <= x.value * y.value < wgs + x.value
+    assert wgs > 2 ** 21 or y.value == 1
