@@ -167,7 +167,7 @@ def _leaves(*nodes):
     seen, leaves, todo = set(), {}, list(nodes)
     while todo:
         node = todo.pop()
-        if hasattr(node, "variable"):
+        if type(node).__name__ == "AccumulateGrad":
             leaves[id(node.variable)] = node.variable
         elif node is not None and node not in seen:
             seen.add(node)

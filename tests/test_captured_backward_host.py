@@ -60,3 +60,20 @@ def test_a_deep_graph_is_walked(captured):
     with pytest.raises(RuntimeError, match="same leaves"):
         captured(lambda: _Twice.apply(torch.ones(4), w), w)
     assert lives is not None
+
+
+def test_an_operators_own_attributes_are_no_leaves(captured):
+    class Named(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, w):
+            ctx.variable = "mine"
+            return w * 2
+
+        @staticmethod
+        def backward(ctx, dy):
+            return dy * 2
+    w = torch.randn(4, requires_grad=True)
+    lives = _Twice.apply(torch.ones(4), Named.apply(w))
+    with pytest.raises(RuntimeError, match="same leaves"):
+        captured(lambda: _Twice.apply(torch.ones(4), w), w)
+    assert lives is not None
