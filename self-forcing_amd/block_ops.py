@@ -190,6 +190,22 @@ def _check_captured(ctx):
                            "its outputs first, or record it on another stream")
 
 
+def _save(ctx, *tensors):
+    """`save_for_backward`, and what `_saved` holds the tensors against."""
+    ctx.save_for_backward(*tensors)
+    ctx.saved_as = [None if t is None else (t.shape, t.dtype) for t in tensors]
+
+
+def _saved(ctx, dy):
+    """The saved tensors.  Saved-tensor hooks (save_on_cpu) may give them back in another layout, which the caller sees to; the kernels
+    take addresses, so that another size, type or device is refused here."""
+    saved, device = ctx.saved_tensors, dy.device
+    for t, was in zip(saved, ctx.saved_as):
+        if was is not None and (t.shape != was[0] or t.dtype != was[1] or t.device != device):
+            raise RuntimeError(f"saved-tensor hooks gave back {tuple(t.shape)} {t.dtype} on {t.device} for {tuple(was[0])} {was[1]} on {device}")
+    return saved
+
+
 def _once(backward):
     """A backward without a derivative of its own: `once_differentiable`, but for calls that build no graph, which it would only
     slow down.
@@ -220,10 +236,10 @@ class _LnFn(torch.autograd.Function):
             mod = (None, None, 0, 1, sc.data_ptr(), sh.data_ptr())
         if checkpoint8:
             y, *kept = _ln_keep8(x, mod, eps)
-            ctx.save_for_backward(sc, *kept)
+            _save(ctx, sc, *kept)
         else:
             y = _ln(x, mod, eps)
-            ctx.save_for_backward(sc, x)
+            _save(ctx, sc, x)
         ctx.cfg = (modulate, eps, checkpoint8, ms, rpf, _row_stride(x), _ln_bwd_bytes(x.shape[0] * x.shape[1], x.shape[2], rpf, x.get_device()),
                    a.shape, b.shape, sc.stride(), x.stride())
         _noted(ctx, x.device)
@@ -233,9 +249,8 @@ class _LnFn(torch.autograd.Function):
     @_once
     def backward(ctx, dy):
         modulate, eps, checkpoint8, ms, rpf, xs, nbytes, a_shape, b_shape, sc_strides, x_strides = ctx.cfg
-        sc, *rest = ctx.saved_tensors
+        sc, *rest = _saved(ctx, dy)
         x, kept = (None, [t.contiguous() for t in rest]) if checkpoint8 else (rest[0], None)
-        # saved-tensor hooks (save_on_cpu) give the values back, not the layout
         if sc.stride() != sc_strides:
             sc, ms = sc.contiguous(), sc.shape[-1] if modulate else 0
         if x is not None and x.stride() != x_strides:
@@ -309,7 +324,7 @@ class _GeluFn(torch.autograd.Function):
         y, data, scale = _gelu(x, checkpoint8)
         ctx.checkpoint8 = checkpoint8
         _noted(ctx, x.device)
-        ctx.save_for_backward(*((data, scale) if checkpoint8 else (x,)))
+        _save(ctx, *((data, scale) if checkpoint8 else (x,)))
         return y
 
     @staticmethod
@@ -321,7 +336,7 @@ class _GeluFn(torch.autograd.Function):
             dy = _even(dy)
             dys = _row_stride(dy)
         x, xs, data, scale = None, 0, None, None
-        saved = ctx.saved_tensors              # held until the call: saved-tensor hooks give tensors that nobody else holds
+        saved = _saved(ctx, dy)                # held until the call: saved-tensor hooks give tensors that nobody else holds
         if ctx.checkpoint8:
             saved = [t.contiguous() for t in saved]
             data, scale = (t.data_ptr() for t in saved)

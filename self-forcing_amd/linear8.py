@@ -20,7 +20,7 @@ import functools
 import torch
 
 from . import lib as _l
-from .block_ops import _HALF, _like, _mod, _noted, _once, _row_stride, _rows, _written
+from .block_ops import _HALF, _like, _mod, _noted, _once, _row_stride, _rows, _save, _saved, _written
 from .monarch_attn import _DT, _on_device, _raw_stream, _stream
 
 _EPI = {"none": _l.EPI_NONE, "gelu_tanh": _l.EPI_GELU_TANH, "gate_residual": _l.EPI_GATE_RESIDUAL}
@@ -217,7 +217,7 @@ class _Linear8Fn(torch.autograd.Function):
         n = rows.shape[0] * rows.shape[1]
         ctx.cfg = (rows.shape, rows.dtype, w8.shape, n, _bytes("sfm_linear8_bwd_workspace_bytes", n, N, rows.shape[2], rows.device.index))
         _noted(ctx, rows.device)
-        ctx.save_for_backward(*((data, scale) if need_w else (None, None)), *((w8.data_t, w8.scale_t) if need_x else (None, None)))
+        _save(ctx, *((data, scale) if need_w else (None, None)), *((w8.data_t, w8.scale_t) if need_x else (None, None)))
         return out
 
     @staticmethod
@@ -225,7 +225,7 @@ class _Linear8Fn(torch.autograd.Function):
     def backward(ctx, dy):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         x_shape, dtype, w_shape, rows, nbytes = ctx.cfg
-        xd, xs, wd, ws = (t if t is None else t.contiguous() for t in ctx.saved_tensors)      # saved-tensor hooks may change the layout
+        xd, xs, wd, ws = (t if t is None else t.contiguous() for t in _saved(ctx, dy))
         N, K = w_shape
         dys = N
         if not dy.is_contiguous():

@@ -127,3 +127,27 @@ def test_gelu_takes_rows_whatever_the_hooks_give(library):
         y = blk.gelu_tanh(x)
     torch.autograd.grad(y, x, torch.ones_like(y))
     assert library.calls["sfm_gelu_bwd"][4] == 256
+
+
+WRONG = {"type": lambda t: t.double(), "size": lambda t: t[..., :-1], "device": lambda t: t.to("meta"), "none": lambda t: t}
+
+
+@pytest.mark.parametrize("how", WRONG)
+@pytest.mark.parametrize("op", ["ln", "ln8", "gelu", "gelu8", "linear8"])
+def test_what_is_not_the_saved_tensor_is_refused(library, monkeypatch, how, op):
+    """Before its address reaches a kernel."""
+    x, w = torch.randn(1, 40, 256).bfloat16().requires_grad_(), torch.randn(256).bfloat16().requires_grad_()
+    blocks = lambda n, k: (torch.zeros(n, k, dtype=torch.uint8), torch.zeros(1, 4, dtype=torch.uint8))
+    monkeypatch.setattr(l8, "pack", lambda w, transposed: l8.Weight8(*blocks(64, 256), *blocks(256, 128), (64, 256), w.dtype))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, WRONG[how]):
+        y = {"ln": lambda: blk.ln_affine(x, w, w), "ln8": lambda: blk.ln_affine(x, w, w, checkpoint8=True), "gelu": lambda: blk.gelu_tanh(x),
+             "gelu8": lambda: blk.gelu_tanh(x, checkpoint8=True),
+             "linear8": lambda: l8._Linear8Fn.apply(x, torch.randn(64, 256).bfloat16().requires_grad_(), None, None, None)}[op]()
+    library.calls.clear()
+    if how == "none":
+        torch.autograd.grad(y, x, torch.ones_like(y))
+        assert library.calls
+    else:
+        with pytest.raises(RuntimeError, match="saved-tensor hooks gave back"):
+            torch.autograd.grad(y, x, torch.ones_like(y))
+        assert not library.calls
