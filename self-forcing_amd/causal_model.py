@@ -539,7 +539,7 @@ class CausalWanModel(nn.Module):
         call; `on=False` goes back to them.  The blocks are a snapshot: call it again after the weights change or move.  A pass before
         that is refused where autograd has counted the change (a write under no_grad, an optimiser's step, load_state_dict) or a
         parameter has other memory (`to`, `p.data = t`); a write through `p.data`, such as `p.data.copy_(t)`, cannot be seen, and passes
-        go on with the snapshot.
+        go on with the snapshot.  A pass captured into a graph reads the blocks that it was captured with, which the next call frees.
         Returns the model."""
         def layers(b):
             return b.self_attn.o, b.cross_attn.q, b.cross_attn.o, b.ffn[0], b.ffn[2]

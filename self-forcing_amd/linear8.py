@@ -83,7 +83,7 @@ def _empty_rows(rows, K, device):
 
 
 def quantize(x):
-    """[B, L, K] rows (bf16, fp16 or fp32; any K) in 8-bit blocks.  Not differentiable."""
+    """[B, L, K] rows (bf16, fp16 or fp32; any K) in 8-bit blocks.  Not differentiable.  linear8 takes blocks of 16-bit rows."""
     x = x.detach()
     rows, K, xs = _rows(x)
     data, scale = _empty_rows(rows, K, x.device)
