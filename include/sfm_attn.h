@@ -355,10 +355,9 @@ int sfm_pack8(int32_t dtype, int32_t N, int32_t K, const void* w, int64_t w_stri
 /* out = x8 w8^T + bias with the epilogues of sfm_linear, on the 8-bit values of both operands; bias, GELU and the gated residual
  * follow on the fp32 sum, and the result is rounded once (sfm_linear rounds after each step).  The e4m3 matrix instructions add the
  * products of 8 neighbouring k before they add to the fp32 sum, and drop of them what is below 2^-13 of the largest of the 8: each of the
- * other 7 is off by less than that (1.7e-5 of the result on random rows).  Any N and K; rows of out, res, gate
- * and bias may have any alignment.  x8 has M rows of K, w8 is a weight [N, K]; the input gradient of a layer is this product of the
- * quantised output gradient with data_t, scale_t.  out must not overlap x8, w8 or, in sfm_linear8_fwd, x; res may be out, or is apart
- * from it. */
+ * other 7 is off by less than that (1.7e-5 of the result on random rows).  Any N and K; rows of out, res, gate and bias may have
+ * any alignment.  x8 has M rows of K, w8 is a weight [N, K]; the input gradient of a layer is this product of the quantised output
+ * gradient with data_t, scale_t.  out must not overlap x8, w8 or, in sfm_linear8_fwd, x; res may be out, or is apart from it. */
 typedef struct sfm_linear8_desc {
     int32_t dtype;            /* SFM_BF16 | SFM_F16 : type of bias, res, gate and out */
     int32_t epilogue;         /* SFM_EPI_* */

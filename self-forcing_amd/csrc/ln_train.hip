@@ -8,8 +8,9 @@
 //
 // A row is read once into registers: its statistics are formed again from the same values (the row is there anyway; kept
 // statistics would be another stream to read), up to 1536 channels in the forward's order, above that over four waves where the
-// forward has one, so that their last bits may differ; then the sums of g and g (x - mean) in one exchange.  The column sums dw, db stay in registers over all rows of a wave, meet in LDS, and leave as one fp32
-// partial per workgroup, which a second kernel adds in a fixed order: no atomics, the same result every time.
+// forward has one, so that their last bits may differ; then the sums of g and g (x - mean) in one exchange.  The column sums
+// dw, db stay in registers over all rows of a wave, meet in LDS, and leave as one fp32 partial per workgroup, which a second
+// kernel adds in a fixed order: no atomics, the same result every time.
 //
 // Bound by memory: 21 frames of 1560 x 1536, modulated, 68-70 us and 5 for the partials (302 MB: 4.3 TB/s).  A chunk of 4680 x 1536 from
 // 8-bit blocks: 16 us and 4 (36 MB, 8 us at that rate): a wave has two rows, waits for the loads of each and then for its sums, and

@@ -3,9 +3,10 @@
 //
 // 8-bit blocks: 128 consecutive values of a row share a power of two 2^s, the smallest with max |v| <= 448 * 2^s over the
 // finite values (s = 0 for a block of zeros, never below -126); a value is kept as e4m3 of v * 2^-s, ties to even, one
-// that is not finite as NaN, and one that would round up to 2^128 (from 248 * 2^120, 3.3e38, on) as 240 * 2^120.  Powers of two cost up to one bit of the e4m3 range against a free scale and nothing of its
-// relative precision (half a step is 2^-4 either way), and the scaled matrix instructions apply them: no product needs a
-// multiplication of its own per block, and the 8-bit value times its scale is exact in bf16.
+// that is not finite as NaN, and one that would round up to 2^128 (from 248 * 2^120, 3.3e38, on) as 240 * 2^120.  Powers of
+// two cost up to one bit of the e4m3 range against a free scale and nothing of its relative precision (half a step is 2^-4
+// either way), and the scaled matrix instructions apply them: no product needs a multiplication of its own per block, and the
+// 8-bit value times its scale is exact in bf16.
 //
 // Memory: `data` [rows][round_up(K, 128)] bytes, zeros past K; `scale` bytes s + 127, one word of four for the rows
 // 128 g + m + 32 t (t = byte) of block column kb at word (kb * groups + g) * 32 + m, groups = ceil(rows / 128): a lane of a
@@ -179,7 +180,7 @@ __device__ __forceinline__ float mag_max(const float* v) {
     for (int i = 0; i < N; ++i) a = fmaxf(a, fabsf(v[i]));
     return a;
 }
-// of the finite ones, which are brought below kTop8
+// the same of the finite ones, which are brought below kTop8
 template <int N>
 __device__ __forceinline__ float mag_max_finite(float* v) {
     float a = 0.f;
