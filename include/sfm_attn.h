@@ -487,6 +487,75 @@ int sfm_probe_row_stream(int32_t waves, int32_t kb_per_block, const void* worksp
  * twice that per compute unit when only an eighth of them ask). */
 int sfm_probe_l2_read(int32_t workgroups, int32_t stages, void* workspace, size_t workspace_bytes, void* stream, float* us);
 
+/* ---- Serving many requests from one paged key-value cache (no counterpart in the reference, whose caches are one
+ * contiguous tensor per batch) -------------------------------------------------------------------------------------------
+ *
+ * A pool holds `pages` pages of `page_size` token rows [kv_heads][D] for K and as many for V.  Request r has past[r] tokens in it
+ * and new ones in the call; token i of those has position past[r] + i.  Entry e of its row of `table` ([requests][width]) is the
+ * page of positions e * page_size and on.  Tensors over new tokens have `tokens` rows: the requests' one after the other, request r's
+ * from q_start[r] on (q_start has requests + 1 entries), and rows that nobody has behind them.
+ *
+ * The arrays are read on the device, where nothing can be refused: lengths below 0 count as 0, and no number in them makes a
+ * kernel read or write outside the tensors.
+ *
+ * sfm_paged_plan: from past, new_tokens and the pages free_pages[*taken ..) (taken NULL: from 0):
+ *   q_start, lengths (past + new), table entries of the pages that the new tokens open, in the order of the requests; slots
+ *   [tokens]: page * page_size + offset of each new token's row, -1 for rows that nobody has and where there is no page (the list is
+ *   used up, the table too narrow, the entry negative); next_free: *taken + the pages wanted, above free_count where they did not
+ *   suffice (their entries are -1).  Of new tokens past `tokens` rows nothing is planned.  The workspace is for more requests than one workgroup
+ *   takes; 0 bytes up to there. */
+int sfm_paged_plan_workspace_bytes(int32_t requests, size_t* bytes);
+int sfm_paged_plan(int32_t requests, int32_t width, int32_t page_size, int64_t tokens, int32_t* table, int64_t table_stride,
+                   const int32_t* past, const int32_t* new_tokens, const int32_t* free_pages, int64_t free_count, const int32_t* taken,
+                   int32_t* q_start, int32_t* lengths, int64_t* slots, int32_t* next_free, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
+typedef struct sfm_paged_desc {
+    int32_t dtype;            /* SFM_BF16 | SFM_F16 | SFM_F32 : type of q, out, k, v and the pools */
+    int32_t H, kv_heads, D;   /* H a multiple of kv_heads: query heads h * H / kv_heads and on belong to key head h; D a multiple of 8 up to 256 */
+    int64_t tokens;           /* rows of q and out (tokens * H < 2^31) */
+    int32_t requests, width;  /* of the table; width * page_size < 2^31 */
+    int32_t pages, page_size; /* of the pools; page_size a multiple of 8, pages * page_size < 2^31 */
+    int64_t table_stride;
+    int64_t pool_stride[3];   /* page, token, head; of both pools */
+    int64_t q_stride[2], o_stride[2];      /* token, head */
+    float sm_scale;
+    int32_t causal;           /* 1: a token's keys end at its own position; 0: at the request's last */
+    int32_t window, sink;     /* window > 0: of those only the last `window` and the first `sink` */
+    int32_t top, group;       /* top > 0: only the pages that `selected` lists for each `group` tokens (sfm_paged_select); no window then */
+    int32_t zero_rest;        /* 1: out rows that nobody has get zeros (lse -inf); 0: they are left as they were */
+    int32_t reserved;
+} sfm_paged_desc;
+
+/* k, v rows [tokens][kv_heads][D] (k_stride: token, head; of both) into the pools at `slots`; of a slot named twice the row is one of the two in
+ * each 16 bytes, others outside the pool are passed over.  means (NULL or fp32 [pages][kv_heads][D]): of every page that got a row, the mean of its
+ * keys up to the request's length; needs past, q_start and table.  Of desc the types, sizes and pool_stride. */
+int sfm_paged_write(const sfm_paged_desc* desc, const void* k, const void* v, const int64_t k_stride[2], void* k_pages, void* v_pages,
+                    const int64_t* slots, const int32_t* table, const int32_t* past, const int32_t* q_start, float* means,
+                    void* stream);
+
+/* out = softmax(sm_scale q K^T) V of each new token over the keys that it sees; zeros where it sees none.  lse (NULL or fp32 [H][tokens]):
+ * natural logarithm of the sum, -inf for no keys.  A request whose keys have positions without a page (a number outside the pool,
+ * positions past the table) gets NaN in the rows that would read one, and may in others of the same 256 rows of a head.  Keys that a
+ * row does not see have no part in it whatever their K and V hold.  Sums and statistics in fp32, a fixed order.
+ * MFMA kernels for 16-bit tensors with D 64 or 128; a workspace lets calls with few rows be split over the keys. */
+int sfm_paged_workspace_bytes(const sfm_paged_desc* desc, size_t* bytes);
+int sfm_paged_attention(const sfm_paged_desc* desc, const void* q, const void* k_pages, const void* v_pages, const int32_t* table,
+                        const int32_t* past, const int32_t* q_start, const int32_t* selected, void* out, float* lse, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* Which pages each `group` new tokens of a request read, per key head: of the pages up to the last one that the group's last token
+ * sees, the first `first`, the last `last` and those with the largest (sum of q over the tokens of the group and the query heads of the
+ * key head) . means[page], `top` in all, the lower of two level ones.  Scores are sums in 64 bits; NaN counts as -inf.
+ * selected: [tokens / group + requests + 1][kv_heads][top], entries of the table in ascending order and -1 behind them; group i of
+ * request r is row q_start[r] / group + r + i, rows that nobody has are -1.  Of desc the types, sizes and strides of q and the table,
+ * causal, top (up to SFM_PAGED_TOP_MAX) and group. */
+#define SFM_PAGED_TOP_MAX 2048
+int sfm_paged_select_workspace_bytes(const sfm_paged_desc* desc, size_t* bytes);
+int sfm_paged_select(const sfm_paged_desc* desc, const void* q, const float* means, const int32_t* table, const int32_t* past,
+                     const int32_t* q_start, int32_t first, int32_t last, int32_t* selected, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
 /* Implementation switches for measurements and tests; no counterpart in the reference.  The environment is read
  * ONCE, when the library is loaded: a variable of the same name as a bit below that is set to anything but "0" turns
  * the bit on (SFM_BWD_SIMT=1 ...), SFM_NO_ROCBLAS makes the library behave as where rocBLAS is absent, and SFM_S1_WGS=n

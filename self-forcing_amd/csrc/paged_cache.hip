@@ -1,0 +1,501 @@
+// The paged cache's bookkeeping: block tables and slots from request lengths, new rows into their pages with the pages' mean
+// keys, and the selection of pages by those.  (The attention over pages is paged_attn.hip's.)
+#include <algorithm>
+
+#include "paged_rules.hpp"
+#include "rows8.hpp"
+
+namespace sfm {
+
+// ------------------------------------------------------------------------------------------------
+// plan
+// ------------------------------------------------------------------------------------------------
+struct PlanArgs {
+    int R, W;
+    FastDiv page8;             // page_size / 8
+    int64_t T, table_stride, free_count;
+    int32_t* table;
+    const int32_t *past, *fresh, *free_pages, *taken;
+    int32_t *q_start, *lengths, *next_free;
+    int64_t* slots;
+    int32_t *ws_tokens, *ws_pages;     // [R + 1] prefix sums, more requests than a workgroup keeps in LDS
+};
+
+// A workgroup keeps this many requests' sums in LDS (8 bytes each): up to here every workgroup forms all the sums for itself,
+// which is one launch and no wait between workgroups; 6000 requests take it 5 us of a call's 13.
+constexpr int kPlanLds = 8192;
+constexpr int kPlanThreads = 256;
+
+// Exclusive sum over the workgroup's threads; *total gets the sum of all.
+__device__ __forceinline__ int64_t plan_scan(int64_t v, int64_t* red, int64_t* total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int64_t x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) red[wave] = x;
+    __syncthreads();
+    int64_t before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 64; ++w) {
+        if (w < wave) before += red[w];
+        all += red[w];
+    }
+    *total = all;
+    return before + x - v;
+}
+
+__device__ __forceinline__ int64_t plan_entries(int64_t pos, const PlanArgs& a) {      // ceil(pos / page), at most W
+    const int64_t cap = (int64_t)a.W * a.page8.d * 8;
+    const uint32_t b = (uint32_t)((pos < cap ? pos : cap) + 7) / 8, e = quot(b, a.page8);
+    return e + (e * a.page8.d < b);
+}
+
+// tokens[r] = first row of request r (at most T), pages[r] = pages that the requests before r open; r = 0 .. R
+__device__ void plan_sums(const PlanArgs& a, int32_t* tokens, int32_t* pages) {
+    __shared__ int64_t red[kPlanThreads / 64];
+    const int per = (a.R + kPlanThreads - 1) / kPlanThreads, r0 = min((int)threadIdx.x * per, a.R), r1 = min(r0 + per, a.R);
+    int64_t n = 0, total;
+    for (int r = r0; r < r1; ++r) n += max(a.fresh[r], 0);
+    int64_t at = plan_scan(n, red, &total);
+    for (int r = r0; r < r1; ++r) {
+        tokens[r] = (int32_t)min(at, a.T);
+        at += max(a.fresh[r], 0);
+    }
+    if (threadIdx.x == 0) tokens[a.R] = (int32_t)min(total, a.T);
+    __syncthreads();
+    n = 0;
+    for (int r = r0; r < r1; ++r) {
+        const int64_t past = max(a.past[r], 0), len = past + tokens[r + 1] - tokens[r];
+        n += plan_entries(len, a) - plan_entries(past, a);
+    }
+    at = plan_scan(n, red, &total);
+    // fewer pages are wanted than tokens planned, T < 2^31
+    for (int r = r0; r < r1; ++r) {
+        pages[r] = (int32_t)at;
+        const int64_t past = max(a.past[r], 0), len = past + tokens[r + 1] - tokens[r];
+        at += plan_entries(len, a) - plan_entries(past, a);
+    }
+    if (threadIdx.x == 0) pages[a.R] = (int32_t)total;
+    __syncthreads();
+}
+
+// the last r in [0, n) with at[r] <= v (at[0] = 0 <= v, ascending)
+__device__ __forceinline__ int plan_find(const int32_t* at, int n, int v) {
+    int lo = 0;
+    while (n - lo > 1) {
+        const int mid = (lo + n) >> 1;
+        if (at[mid] <= v) lo = mid;
+        else n = mid;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ int32_t plan_page(const PlanArgs& a, int64_t i) {      // the i-th page that this call opens
+    const int64_t j = i + (a.taken ? max(a.taken[0], 0) : 0);
+    return j < a.free_count ? a.free_pages[j] : -1;
+}
+
+__device__ void plan_fill(const PlanArgs& a, const int32_t* tokens, const int32_t* pages) {
+    const int64_t tid = (int64_t)blockIdx.x * kPlanThreads + threadIdx.x, step = (int64_t)gridDim.x * kPlanThreads;
+    const int wanted = pages[a.R], planned = tokens[a.R];
+    for (int64_t r = tid; r <= a.R; r += step) {
+        a.q_start[r] = tokens[r];
+        if (r < a.R) a.lengths[r] = (int32_t)min((int64_t)max(a.past[r], 0) + tokens[r + 1] - tokens[r], (int64_t)0x7fffffff);
+        else a.next_free[0] = (int32_t)min((int64_t)wanted + (a.taken ? max(a.taken[0], 0) : 0), (int64_t)0x7fffffff);
+    }
+    for (int64_t i = tid; i < wanted; i += step) {
+        const int r = plan_find(pages, a.R + 1, (int)i);
+        a.table[r * a.table_stride + plan_entries(max(a.past[r], 0), a) + (i - pages[r])] = plan_page(a, i);
+    }
+    const int64_t cap = (int64_t)a.W * a.page8.d * 8;
+    for (int64_t t = tid; t < a.T; t += step) {
+        int64_t slot = -1;
+        if (t < planned) {
+            const int r = plan_find(tokens, a.R + 1, (int)t);
+            const int64_t past = max(a.past[r], 0), pos = past + t - tokens[r];
+            if (pos < cap) {
+                const uint32_t e = quot((uint32_t)pos / 8, a.page8);
+                const int64_t opened = (int64_t)e - plan_entries(past, a);
+                // an entry of this call's is taken from the list, where another workgroup takes it from too
+                const int32_t page = opened >= 0 ? plan_page(a, pages[r] + opened) : a.table[r * a.table_stride + e];
+                if (page >= 0) slot = (int64_t)page * a.page8.d * 8 + (pos - (int64_t)e * a.page8.d * 8);
+            }
+        }
+        a.slots[t] = slot;
+    }
+}
+
+__global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
+    extern __shared__ int32_t plan_lds[];
+    plan_sums(a, plan_lds, plan_lds + a.R + 1);
+    plan_fill(a, plan_lds, plan_lds + a.R + 1);
+}
+__global__ __launch_bounds__(kPlanThreads) void paged_plan_sums_kernel(PlanArgs a) { plan_sums(a, a.ws_tokens, a.ws_pages); }
+__global__ __launch_bounds__(kPlanThreads) void paged_plan_fill_kernel(PlanArgs a) { plan_fill(a, a.ws_tokens, a.ws_pages); }
+
+static int launched() {
+    const hipError_t err = hipGetLastError();
+    if (err == hipSuccess) return SFM_OK;
+    set_error("hip launch failed: %s", hipGetErrorString(err));
+    return SFM_ERR_HIP;
+}
+
+size_t paged_plan_workspace_bytes(int R) { return R <= kPlanLds ? 0 : 2 * ((size_t)R + 1) * sizeof(int32_t); }
+
+int launch_paged_plan(int R, int W, int page_size, int64_t T, int32_t* table, int64_t table_stride, const int32_t* past,
+                      const int32_t* fresh, const int32_t* free_pages, int64_t free_count, const int32_t* taken, int32_t* q_start,
+                      int32_t* lengths, int64_t* slots, int32_t* next_free, void* workspace, hipStream_t stream) {
+    PlanArgs a{R, W, fast_div(page_size / 8), T, table_stride, free_count, table, past, fresh, free_pages, taken, q_start, lengths, next_free, slots,
+               (int32_t*)workspace, (int32_t*)workspace + R + 1};
+    const int64_t items = T > R + 1 ? T : R + 1;
+    const int wgs = (int)std::min<int64_t>(std::max<int64_t>((items + 4 * kPlanThreads - 1) / (4 * kPlanThreads), 1), 1024);
+    if (R <= kPlanLds) {
+        hipLaunchKernelGGL(paged_plan_kernel, dim3(wgs), dim3(kPlanThreads), 2 * ((size_t)R + 1) * sizeof(int32_t), stream, a);
+    } else {
+        hipLaunchKernelGGL(paged_plan_sums_kernel, dim3(1), dim3(kPlanThreads), 0, stream, a);
+        hipLaunchKernelGGL(paged_plan_fill_kernel, dim3(wgs), dim3(kPlanThreads), 0, stream, a);
+    }
+    return launched();
+}
+
+// ------------------------------------------------------------------------------------------------
+// write
+// ------------------------------------------------------------------------------------------------
+struct WriteArgs {
+    int T, R, W, H, chunks, page, pages, per;      // chunks: 16 bytes each, of a row of a head; per: tokens of a workgroup that forms means
+    int64_t table_stride, ps, ts, hs, ks, kh;      // in chunks (the table: in entries)
+    const u32x4 *k, *v;
+    u32x4 *kp, *vp;
+    const int64_t* slots;
+    const int32_t *table, *past, *q_start;
+    float* means;
+    int mean_wgs;
+};
+
+template <typename T> struct Chunk;                // 16 bytes <-> floats
+template <> struct Chunk<float> {
+    static constexpr int kN = 4;
+    static __device__ __forceinline__ void get(u32x4 w, float* x) {
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
+    }
+};
+template <class E> struct Chunk16 {
+    static constexpr int kN = 8;
+    static __device__ __forceinline__ void get(u32x4 w, float* x) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = E::to_float((uint16_t)(w[i] & 0xffffu));
+            x[2 * i + 1] = E::to_float((uint16_t)(w[i] >> 16));
+        }
+    }
+};
+template <> struct Chunk<BF16> : Chunk16<BF16> {};
+template <> struct Chunk<F16> : Chunk16<F16> {};
+
+// The mean keys of the pages that tokens [t0, t1) are the first to reach, of one head.  New rows are taken from k, whatever the
+// copying workgroups have done by then.  A page's rows are summed by groups of lanes, a row each, joined in LDS in a fixed order.
+template <typename E>
+__device__ void write_means(const WriteArgs& a, int t0, int t1, int h) {
+    constexpr int N = Chunk<E>::kN;
+    __shared__ float part[256 * N];
+    const int tid = threadIdx.x, groups = 256 / a.chunks, g = tid / a.chunks, c = tid - g * a.chunks, D = a.chunks * N;
+    int r = find_last(a.R, t0, [&](int i) { return (int64_t)clamp_int(a.q_start[i], 0, a.T); });
+    for (int t = t0; t < t1; ++t) {
+        while (r < a.R && clamp_int(a.q_start[r + 1], 0, a.T) <= t) ++r;
+        if (r >= a.R) return;
+        const Request q = request_of(a.q_start, a.past, r, a.R, a.T);
+        const int64_t pos = (int64_t)q.past + t - q.first;
+        const int64_t e = pos / a.page, off = pos - e * a.page;
+        if ((t != q.first && off != 0) || e >= a.W) continue;
+        const int page = a.table[r * a.table_stride + e];
+        if (page < 0 || page >= a.pages) continue;
+        const int64_t base = e * a.page;
+        const int rows = (int)min((int64_t)q.past + q.n - base, (int64_t)a.page), old = (int)max((int64_t)0, min((int64_t)rows, q.past - base));
+        float sum[N], x[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum[i] = 0.f;
+        if (g < groups) {
+            const u32x4* const in = a.kp + page * a.ps + h * a.hs + c;
+            for (int j = g; j < old; j += groups) {
+                Chunk<E>::get(in[j * a.ts], x);
+#pragma unroll
+                for (int i = 0; i < N; ++i) sum[i] += x[i];
+            }
+            const u32x4* const fresh = a.k + (q.first + (base - q.past)) * a.ks + h * a.kh + c;
+            for (int j = old + (groups - old % groups + g) % groups; j < rows; j += groups) {
+                Chunk<E>::get(fresh[j * a.ks], x);
+#pragma unroll
+                for (int i = 0; i < N; ++i) sum[i] += x[i];
+            }
+        }
+        __syncthreads();
+        if (g < groups)
+#pragma unroll
+            for (int i = 0; i < N; ++i) part[(g * a.chunks + c) * N + i] = sum[i];
+        __syncthreads();
+        if (tid < D) {
+            float s = 0.f;
+            for (int j = 0; j < groups; ++j) s += part[j * D + tid];
+            a.means[((int64_t)page * a.H + h) * D + tid] = s / (float)rows;
+        }
+    }
+}
+
+// The first mean_wgs workgroups form means, the others copy 16 bytes per lane and tensor at a time.  Bound by the rows' bytes.
+template <typename E>
+__global__ __launch_bounds__(256) void paged_write_kernel(WriteArgs a) {
+    if ((int)blockIdx.x < a.mean_wgs) {
+        const int piece = blockIdx.x / a.H, h = blockIdx.x - piece * a.H;
+        write_means<E>(a, piece * a.per, min(a.T, (piece + 1) * a.per), h);
+        return;
+    }
+    const uint32_t row = a.H * a.chunks;
+    const int64_t total = (int64_t)a.T * row, step = (int64_t)(gridDim.x - a.mean_wgs) * 256, all = (int64_t)a.pages * a.page;
+    for (int64_t i = (int64_t)(blockIdx.x - a.mean_wgs) * 256 + threadIdx.x; i < total; i += step) {
+        const int64_t t = i / row;
+        const uint32_t x = (uint32_t)(i - t * row), h = x / a.chunks, c = x - h * a.chunks;
+        const int64_t slot = a.slots[t];
+        if (slot < 0 || slot >= all) continue;
+        const uint32_t page = (uint32_t)slot / a.page;                 // slots are below 2^31
+        const int64_t to = page * a.ps + (slot - (int64_t)page * a.page) * a.ts + h * a.hs + c, from = t * a.ks + h * a.kh + c;
+        a.kp[to] = a.k[from];
+        a.vp[to] = a.v[from];
+    }
+}
+
+int launch_paged_write(const sfm_paged_desc& d, const void* k, const void* v, const int64_t* ks, void* kp, void* vp, const int64_t* slots,
+                       const int32_t* table, const int32_t* past, const int32_t* q_start, float* means, hipStream_t stream) {
+    const int n16 = d.dtype == SFM_F32 ? 4 : 8;
+    WriteArgs a{(int)d.tokens, d.requests, d.width, d.kv_heads, d.D / n16, d.page_size, d.pages, 1, d.table_stride,
+                d.pool_stride[0] / n16, d.pool_stride[1] / n16, d.pool_stride[2] / n16, ks[0] / n16, ks[1] / n16, (const u32x4*)k, (const u32x4*)v,
+                (u32x4*)kp, (u32x4*)vp, slots, table, past, q_start, means, 0};
+    if (means) {
+        // single tokens of many requests reach a page each, long prompts one page in page_size tokens
+        a.per = std::max(1, a.T / 256);
+        a.mean_wgs = (a.T + a.per - 1) / a.per * a.H;
+    }
+    const int64_t total = (int64_t)a.T * a.H * a.chunks;
+    const dim3 grid((unsigned)(a.mean_wgs + std::min<int64_t>((total + 255) / 256, 8192)));
+    auto kern = d.dtype == SFM_BF16 ? paged_write_kernel<BF16> : d.dtype == SFM_F16 ? paged_write_kernel<F16> : paged_write_kernel<float>;
+    hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, a);
+    return launched();
+}
+
+// ------------------------------------------------------------------------------------------------
+// select
+// ------------------------------------------------------------------------------------------------
+struct SelectArgs {
+    sfm_paged_desc d;
+    int first, last;
+};
+
+// A score's bits in the order of the scores: NaN counts as -inf, -0 as 0.
+__device__ __forceinline__ uint64_t select_key(double s) {
+    if (!(s == s)) s = -INFINITY;
+    const uint64_t b = (uint64_t)__double_as_longlong(s + 0.0);
+    return b >> 63 ? ~b : b | ((uint64_t)1 << 63);
+}
+
+constexpr int kSelPages = 2048;                    // scores that are compared at a time, beside the best so far
+
+// A workgroup takes one group of tokens and one key head: the sum of its queries in LDS, a page's score from 16 lanes, kSelPages
+// pages at a time.  The best of them and of the `top` before are found by the scores' bits, eight at a time from the highest: a
+// histogram says in which digit the top-th score lies; level ones are taken in the order of their pages, which is kept throughout.
+// Sums are of 64 bits: two programs that add in another order still agree on which page is ahead.
+template <typename E>
+__global__ __launch_bounds__(256) void paged_select_kernel(SelectArgs s, const void* q, const float* means, const int32_t* table,
+                                                           const int32_t* past, const int32_t* q_start, int32_t* selected) {
+    constexpr int N = Chunk<E>::kN;
+    extern __shared__ __attribute__((aligned(16))) char sel_lds[];
+    const sfm_paged_desc& d = s.d;
+    const int cap = d.top + kSelPages;
+    double* const qsum = (double*)sel_lds;                         // [D]
+    uint64_t* const key = (uint64_t*)(qsum + 256);                 // [cap]
+    int32_t* const entry = (int32_t*)(key + cap);                  // [cap]
+    __shared__ int hist[256];
+    __shared__ int wsum[4][2];
+    __shared__ int pick[2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int row = blockIdx.x / d.kv_heads, kh = blockIdx.x - row * d.kv_heads;
+    int32_t* const out = selected + ((int64_t)row * d.kv_heads + kh) * d.top;
+    const int r = find_last(d.requests, row, [&](int i) { return first_piece(clamp_int(q_start[i], 0, (int)d.tokens), 1, d.group, i); });
+    const Request rq = request_of(q_start, past, r, d.requests, (int)d.tokens);
+    const int64_t t0 = (row - first_piece(rq.first, 1, d.group, r)) * d.group;
+    if (r >= d.requests || t0 < 0 || t0 >= rq.n) {
+        for (int i = tid; i < d.top; i += 256) out[i] = -1;
+        return;
+    }
+    const int n = (int)min((int64_t)d.group, rq.n - t0);
+    const int64_t end = (int64_t)rq.past + (d.causal ? t0 + n : rq.n);
+    const int64_t pages = (end + d.page_size - 1) / d.page_size;
+    const int P = (int)min(pages, (int64_t)d.width);               // entries that the table has
+    if (P <= d.top) {
+        for (int i = tid; i < d.top; i += 256) out[i] = i < P ? i : -1;
+        return;
+    }
+    // sum of the queries: chunk c of the rows g, g + groups, ...
+    {
+        const int G = d.H / d.kv_heads, chunks = d.D / N, groups = 256 / chunks, g = tid / chunks, c = tid - g * chunks;
+        const int rows = n * G;
+        double sum[N];
+        float x[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum[i] = 0.0;
+        const u32x4* const q16 = (const u32x4*)q;
+        if (g < groups)
+            for (int j = g; j < rows; j += groups) {
+                const int t = j / G, h = j - t * G;
+                Chunk<E>::get(q16[((rq.first + t0 + t) * d.q_stride[0] + (int64_t)(kh * G + h) * d.q_stride[1]) / N + c], x);
+#pragma unroll
+                for (int i = 0; i < N; ++i) sum[i] += (double)x[i];
+            }
+        double* const part = (double*)key;                         // [groups][D]: at most 256 * N doubles, which the keys have room for
+        if (g < groups)
+#pragma unroll
+            for (int i = 0; i < N; ++i) part[g * d.D + c * N + i] = sum[i];
+        __syncthreads();
+        if (tid < d.D) {
+            double t = 0.0;
+            for (int j = 0; j < groups; ++j) t += part[j * d.D + tid];
+            qsum[tid] = t;
+        }
+        __syncthreads();
+    }
+    int kept = 0;                                                  // key[0 .. kept): the best so far, in the order of their entries
+    const int sub = tid & 15;
+    for (int p0 = 0; p0 < P; p0 += kSelPages) {
+        const int count = min(kSelPages, P - p0);
+        for (int i = tid >> 4; i < count; i += 16) {
+            const int e = p0 + i;
+            const int page = table[r * d.table_stride + e];
+            double dot = 0.0;
+            if (page >= 0 && page < d.pages) {
+                const float* const m = means + ((int64_t)page * d.kv_heads + kh) * d.D;
+                for (int x = 4 * sub; x < d.D; x += 64) {
+                    const f32x4 w = *(const f32x4*)(m + x);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) dot = fma(qsum[x + k], (double)w[k], dot);
+                }
+            } else {
+                dot = -INFINITY;
+            }
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) dot += __shfl_xor(dot, o);
+            if (e < s.first || e >= pages - s.last) dot = INFINITY;
+            if (sub == 0) {
+                key[kept + i] = select_key(dot);
+                entry[kept + i] = e;
+            }
+        }
+        __syncthreads();
+        const int have = kept + count;
+        if (have <= d.top) {
+            kept = have;
+            continue;
+        }
+        // the top-th largest key: digits from the highest, `need` of those that agree so far
+        uint64_t prefix = 0;
+        int need = d.top;
+        bool whole = false;                                        // all that agree are taken: no level ones to tell apart
+        int shift = 56;
+        for (; shift >= 0; shift -= 8) {
+            hist[tid] = 0;
+            __syncthreads();
+            for (int i = tid; i < have; i += 256)
+                if (shift == 56 || (key[i] >> (shift + 8)) == prefix) atomicAdd(&hist[(key[i] >> shift) & 255], 1);
+            __syncthreads();
+            // number of keys in digits above this thread's
+            int c = hist[tid], above = c;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int y = __shfl_down(above, o);
+                if (lane + o < 64) above += y;
+            }
+            if (lane == 0) wsum[wave][0] = above;
+            __syncthreads();
+            for (int w = wave + 1; w < 4; ++w) above += wsum[w][0];
+            above -= c;
+            if (above < need && above + c >= need) {
+                pick[0] = tid;
+                pick[1] = above;
+            }
+            __syncthreads();
+            prefix = prefix << 8 | (uint32_t)pick[0];
+            need -= pick[1];
+            whole = hist[pick[0]] == need;
+            __syncthreads();
+            if (whole) break;
+        }
+        const int low = whole ? shift : 0;                         // key >> low against prefix
+        // keep them in order: every thread moves a run of the list; the moves go to lower places, after all have been read
+        const int per = (have + 255) / 256, i0 = min(tid * per, have), i1 = min(i0 + per, have);
+        int over = 0, level = 0;
+        for (int i = i0; i < i1; ++i) {
+            const uint64_t k = key[i] >> low;
+            over += k > prefix;
+            level += k == prefix;
+        }
+        int ao = over, al = level;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(ao, o), z = __shfl_up(al, o);
+            if (lane >= o) ao += y, al += z;
+        }
+        if (lane == 63) wsum[wave][0] = ao, wsum[wave][1] = al;
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) ao += wsum[w][0], al += wsum[w][1];
+        ao -= over;
+        al -= level;
+        constexpr int kRun = (SFM_PAGED_TOP_MAX + kSelPages) / 256;
+        uint64_t mk[kRun];
+        int32_t me[kRun];
+#pragma unroll
+        for (int j = 0; j < kRun; ++j)
+            if (i0 + j < i1) mk[j] = key[i0 + j], me[j] = entry[i0 + j];
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) {
+            if (i0 + j >= i1) continue;
+            const uint64_t k = mk[j] >> low;
+            if (k < prefix) continue;
+            const bool take = k > prefix || al < need;
+            if (take) {
+                const int at = ao + min(al, need);
+                key[at] = mk[j];
+                entry[at] = me[j];
+            }
+            ao += k > prefix;
+            al += k == prefix;
+        }
+        kept = d.top;
+        __syncthreads();
+    }
+    for (int i = tid; i < d.top; i += 256) out[i] = entry[i];
+}
+
+size_t paged_select_workspace_bytes(const sfm_paged_desc&) { return 0; }
+
+int launch_paged_select(const sfm_paged_desc& d, const void* q, const float* means, const int32_t* table, const int32_t* past,
+                        const int32_t* q_start, int first, int last, int32_t* selected, void*, hipStream_t stream) {
+    SelectArgs s{d, first, last};
+    const int64_t wgs = pieces(d.tokens, d.group, d.requests) * d.kv_heads;
+    if (wgs >= (1 << 24)) {
+        set_error("%lld groups of tokens and heads are more than a launch takes", (long long)wgs);
+        return SFM_ERR_UNSUPPORTED;
+    }
+    const size_t lds = 256 * sizeof(double) + (size_t)(d.top + kSelPages) * 12;
+    auto kern = d.dtype == SFM_BF16 ? paged_select_kernel<BF16> : d.dtype == SFM_F16 ? paged_select_kernel<F16> : paged_select_kernel<float>;
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) {
+        set_error("hipFuncSetAttribute failed: %s", hipGetErrorString(e));
+        return SFM_ERR_HIP;
+    }
+    hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(256), lds, stream, s, q, means, table, past, q_start, selected);
+    return launched();
+}
+
+}  // namespace sfm

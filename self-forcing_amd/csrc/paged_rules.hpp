@@ -1,0 +1,95 @@
+// Arithmetic of the paged cache that kernels and host share: which request and which rows a work item has, which keys they see,
+// and where a position's row lies.
+//
+// Tensors over new tokens hold the requests one after the other, request r's from q_start[r] on; n of them with G query heads
+// to a key head are n * G rows of that key head, row = token * G + head.  How many there are is known on the device only.  A
+// grid over pieces of `per` rows has floor(rows / per) + requests + 1 of them: request r's begin at piece floor(start / per) + r,
+// which leaves it the ceil(n / per) that it needs and at most one that nobody has.
+#pragma once
+
+#include "sfm_common.hpp"
+
+namespace sfm {
+
+// Quotient by a divisor that the host knows: exact for n < 2^28, with magic = floor(2^k / d) + 1, k = 28 + ceil(log2 d): the
+// product is above n 2^k / d by n (magic - 2^k / d) <= n < 2^28 <= 2^k / d, too little to reach the next quotient.
+struct FastDiv {
+    uint32_t magic, shift, d;
+};
+inline FastDiv fast_div(uint32_t d) {
+    uint32_t log = 0;
+    while (((uint64_t)1 << log) < d) ++log;
+    FastDiv f;
+    f.shift = 28 + log;
+    f.magic = (uint32_t)(((uint64_t)1 << f.shift) / d + 1);
+    f.d = d;
+    return f;
+}
+__host__ __device__ __forceinline__ uint32_t quot(uint32_t n, const FastDiv& f) { return (uint32_t)(((uint64_t)n * f.magic) >> f.shift); }
+
+// A request's new tokens, whatever the tensors say: rows [first, first + n) of T; its keys are positions [0, past + n).
+// Request R stands for the rows behind the last one: no keys.
+struct Request {
+    int first, n, past;
+};
+__host__ __device__ __forceinline__ int clamp_int(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
+__host__ __device__ __forceinline__ Request request_of(const int32_t* q_start, const int32_t* past, int r, int R, int T) {
+    Request q;
+    q.first = clamp_int(q_start[r], 0, T);
+    const int end = r < R ? clamp_int(q_start[r + 1], 0, T) : T;
+    q.n = end > q.first ? end - q.first : 0;
+    q.past = r < R ? (past[r] > 0 ? past[r] : 0) : 0;
+    return q;
+}
+// first piece of request r
+__host__ __device__ __forceinline__ int64_t first_piece(int64_t start, int64_t heads, int64_t per, int r) { return start * heads / per + r; }
+__host__ __device__ __forceinline__ int64_t pieces(int64_t rows, int64_t per, int R) { return rows / per + R + 1; }
+
+// The keys that a piece's tokens [t0, t1] of a request see, in tiles of 64 positions.  A token's keys end at `end`: its own position
+// + 1 (causal) or the request's length; with a window only the last `window` of them and the first `sink` count.  Positions
+// from `cap` on have no entry in the table.  Virtual tiles 0 .. tiles - 1 are tiles 0 .. sinks - 1 and then first, first + 1, ...;
+// of them [fast0, fast1) are seen whole by every token.
+struct KeyTiles {
+    int end_min, end_max, lo_min, lo_max, sinks, first, tiles, fast0, fast1;
+    bool beyond;               // the request has positions that no entry of the table can hold
+};
+__host__ __device__ __forceinline__ KeyTiles key_tiles(const Request& q, bool none, int t0, int t1, bool causal, int window, int sink, int cap) {
+    KeyTiles k;
+    const int64_t len = none ? 0 : (int64_t)q.past + q.n;
+    const int64_t a = causal && !none ? (int64_t)q.past + t0 + 1 : len, b = causal && !none ? (int64_t)q.past + t1 + 1 : len;
+    k.beyond = b > cap;
+    k.end_min = (int)(a < cap ? a : cap);
+    k.end_max = (int)(b < cap ? b : cap);
+    k.lo_min = window && k.end_min > window ? k.end_min - window : 0;
+    k.lo_max = window && k.end_max > window ? k.end_max - window : 0;
+    const int s = window ? (sink < k.end_max ? sink : k.end_max) : 0;
+    k.first = k.lo_min / 64;
+    k.sinks = (s + 63) / 64 < k.first ? (s + 63) / 64 : k.first;
+    const int last = (k.end_max + 63) / 64;
+    k.tiles = k.sinks + (last > k.first ? last - k.first : 0);
+    const int f0 = k.sinks + (k.lo_max + 63) / 64 - k.first, f1 = k.sinks + k.end_min / 64 - k.first;
+    k.fast0 = f0 < f1 ? f0 : 0;
+    k.fast1 = f0 < f1 ? f1 : 0;
+    return k;
+}
+__host__ __device__ __forceinline__ int tile_of(const KeyTiles& k, int v) { return v < k.sinks ? v : v - k.sinks + k.first; }
+
+#if defined(__HIPCC__)
+// The last r in [0, R] with at(r) <= v, R standing for the rows behind the last request: at ascends from at(0) <= v, and a wave looks
+// at 64 of its values at a time.  The same in every lane; some r in [0, R] where the values make no sense.
+template <class F>
+__device__ __forceinline__ int find_last(int R, int64_t v, F at) {
+    int lo = 0, n = R + 1;                         // in [lo, lo + n)
+    const int lane = threadIdx.x & 63;
+    while (n > 1) {
+        const int step = (n + 63) / 64, off = lane * step;
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(off < n && at(lo + off) <= v);
+        const int k = hit ? 63 - __builtin_clzll(hit) : 0;
+        lo += k * step;
+        n = min(step, n - k * step);
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+#endif
+
+}  // namespace sfm

@@ -76,6 +76,20 @@ int launch_gate_residual(int dtype, int64_t rows, int C, void* x, int64_t xs, co
 int launch_rms_norm(int dtype, int64_t rows, int C, float eps, const void* x, int64_t xs, void* y, int64_t ys,
                     const void* weight, hipStream_t stream);
 
+size_t paged_plan_workspace_bytes(int R);
+int launch_paged_plan(int R, int W, int page_size, int64_t T, int32_t* table, int64_t table_stride, const int32_t* past,
+                      const int32_t* fresh, const int32_t* free_pages, int64_t free_count, const int32_t* taken, int32_t* q_start,
+                      int32_t* lengths, int64_t* slots, int32_t* next_free, void* workspace, hipStream_t stream);
+int launch_paged_write(const sfm_paged_desc& d, const void* k, const void* v, const int64_t* ks, void* kp, void* vp, const int64_t* slots,
+                       const int32_t* table, const int32_t* past, const int32_t* q_start, float* means, hipStream_t stream);
+size_t paged_workspace_bytes(const sfm_paged_desc& d);
+int launch_paged_attention(const sfm_paged_desc& d, const void* q, const void* kp, const void* vp, const int32_t* table,
+                           const int32_t* past, const int32_t* q_start, const int32_t* selected, void* out, float* lse, void* workspace,
+                           size_t workspace_bytes, hipStream_t stream);
+size_t paged_select_workspace_bytes(const sfm_paged_desc& d);
+int launch_paged_select(const sfm_paged_desc& d, const void* q, const float* means, const int32_t* table, const int32_t* past,
+                        const int32_t* q_start, int first, int last, int32_t* selected, void* workspace, hipStream_t stream);
+
 static int check_rows(int dtype, int64_t rows, int C, int64_t xs, int64_t ys) {
     if (dtype != SFM_BF16 && dtype != SFM_F16 && dtype != SFM_F32) {
         set_error("unsupported dtype %d", dtype);
@@ -1768,6 +1782,244 @@ int sfm_ln_bwd(int32_t dtype, int64_t rows, int32_t C, float eps, const void* x,
     }
     return launch_ln_bwd(dtype, rows, C, eps, x, x_stride, x ? nullptr : data, scale8, rstd, dy, dy_stride, weight ? weight : scale, mod_stride,
                          rows_per_group, scale != nullptr, dx, dx_stride, dw, db, workspace, (hipStream_t)stream);
+}
+
+static int check_table(int requests, int width, int page_size, int64_t tokens, int64_t table_stride) {
+    if (requests < 1 || requests > (1 << 24) || width < 1 || tokens < 0 || tokens > 0x7fffffff) {
+        set_error("requests=%d, width=%d, tokens=%lld: need 1 <= requests <= 2^24, a width of 1 or more and 0 <= tokens < 2^31", requests, width,
+                  (long long)tokens);
+        return SFM_ERR_SHAPE;
+    }
+    if (page_size < 8 || page_size % 8 || (int64_t)width * page_size > 0x7fffffff) {
+        set_error("page_size=%d, width=%d: need pages of a multiple of 8 rows, and width * page_size < 2^31", page_size, width);
+        return SFM_ERR_SHAPE;
+    }
+    if (table_stride < width) {
+        set_error("table: rows of %d entries, %lld apart", width, (long long)table_stride);
+        return SFM_ERR_STRIDE;
+    }
+    return SFM_OK;
+}
+static bool aligned4(const void* p) { return (((uintptr_t)p) & 3) == 0; }
+
+int sfm_paged_plan_workspace_bytes(int32_t requests, size_t* bytes) {
+    if (!bytes) {
+        set_error("bytes must be non-NULL");
+        return SFM_ERR_NULL;
+    }
+    const int rc = check_table(requests, 1, 8, 0, 1);
+    if (rc) return rc;
+    *bytes = paged_plan_workspace_bytes(requests);
+    return SFM_OK;
+}
+
+int sfm_paged_plan(int32_t requests, int32_t width, int32_t page_size, int64_t tokens, int32_t* table, int64_t table_stride,
+                   const int32_t* past, const int32_t* new_tokens, const int32_t* free_pages, int64_t free_count, const int32_t* taken,
+                   int32_t* q_start, int32_t* lengths, int64_t* slots, int32_t* next_free, void* workspace, size_t workspace_bytes,
+                   void* stream) {
+    const int rc = check_table(requests, width, page_size, tokens, table_stride);
+    if (rc) return rc;
+    if (!table || !past || !new_tokens || (free_count > 0 && !free_pages) || !q_start || !lengths || (tokens > 0 && !slots) || !next_free) {
+        set_error("table, past, new_tokens, free_pages, q_start, lengths, slots and next_free must be non-NULL");
+        return SFM_ERR_NULL;
+    }
+    if (free_count < 0) {
+        set_error("free_count=%lld is negative", (long long)free_count);
+        return SFM_ERR_RANGE;
+    }
+    if (!aligned4(table) || !aligned4(past) || !aligned4(new_tokens) || !aligned4(free_pages) || !aligned4(taken) || !aligned4(q_start) ||
+        !aligned4(lengths) || !aligned4(next_free) || (((uintptr_t)slots) & 7)) {
+        set_error("the arrays must be aligned to their elements");
+        return SFM_ERR_ALIGN;
+    }
+    // workgroups read what others may have written by then
+    const void* in[4] = {past, new_tokens, taken, free_pages};
+    const size_t in_n[4] = {(size_t)requests * 4, (size_t)requests * 4, taken ? 4u : 0u, (size_t)free_count * 4};
+    const void* out[5] = {q_start, lengths, next_free, slots, table};
+    const size_t out_n[5] = {(size_t)(requests + 1) * 4, (size_t)requests * 4, 4, (size_t)tokens * 8, ((size_t)(requests - 1) * table_stride + width) * 4};
+    for (int i = 0; i < 5; ++i) {
+        bool over = false;
+        for (int j = 0; j < 4; ++j) over = over || (in_n[j] && overlap(out[i], out_n[i], in[j], in_n[j]));
+        for (int j = 0; j < i; ++j) over = over || overlap(out[i], out_n[i], out[j], out_n[j]);
+        if (over) {
+            set_error("q_start, lengths, next_free, slots and table must not overlap the inputs or each other");
+            return SFM_ERR_RANGE;
+        }
+    }
+    const size_t need = paged_plan_workspace_bytes(requests);
+    if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need)) {
+        set_error("workspace must be non-NULL, 16-byte aligned and hold %zu bytes", need);
+        return SFM_ERR_WORKSPACE;
+    }
+    return launch_paged_plan(requests, width, page_size, tokens, table, table_stride, past, new_tokens, free_pages, free_count, taken, q_start,
+                             lengths, slots, next_free, workspace, (hipStream_t)stream);
+}
+
+static int check_paged_stride(const char* name, int64_t s, int64_t least, int esz) {
+    if (s < least || (s * esz) % 16 || s > ((int64_t)1 << 40)) {
+        set_error("%s stride %lld: need %lld or more elements and a multiple of 16 bytes", name, (long long)s, (long long)least);
+        return SFM_ERR_STRIDE;
+    }
+    return SFM_OK;
+}
+
+// what all of the entry points read of a descriptor; `pool`: with the pools
+static int check_paged(const sfm_paged_desc* d, bool pool) {
+    if (!d) {
+        set_error("desc is NULL");
+        return SFM_ERR_NULL;
+    }
+    if (d->dtype != SFM_BF16 && d->dtype != SFM_F16 && d->dtype != SFM_F32) {
+        set_error("unsupported dtype %d", d->dtype);
+        return SFM_ERR_DTYPE;
+    }
+    if (d->kv_heads < 1 || d->D < 8 || d->D % 8 || d->D > 256 || d->pages < 1) {
+        set_error("kv_heads=%d, D=%d, pages=%d invalid", d->kv_heads, d->D, d->pages);
+        return SFM_ERR_SHAPE;
+    }
+    int rc = check_table(d->requests, d->width, d->page_size, d->tokens, d->table_stride);
+    if (rc) return rc;
+    if (d->tokens < 1 || (int64_t)d->pages * d->page_size > 0x7fffffff) {
+        set_error("tokens=%lld, pages=%d of %d: need a token, and pages * page_size < 2^31", (long long)d->tokens, d->pages, d->page_size);
+        return SFM_ERR_SHAPE;
+    }
+    if (pool) {
+        const int esz = elem_size(d->dtype);
+        if ((rc = check_paged_stride("pools: page", d->pool_stride[0], d->D, esz))) return rc;
+        if ((rc = check_paged_stride("pools: token", d->pool_stride[1], d->D, esz))) return rc;
+        if ((rc = check_paged_stride("pools: head", d->pool_stride[2], d->D, esz))) return rc;
+        if (d->pool_stride[1] >= (1 << 24)) {
+            set_error("pools: a token stride of %lld elements is more than 2^24", (long long)d->pool_stride[1]);
+            return SFM_ERR_STRIDE;
+        }
+    }
+    return SFM_OK;
+}
+static int check_paged_q(const sfm_paged_desc* d) {
+    if (d->H < d->kv_heads || d->H % d->kv_heads || d->tokens * d->H > 0x7fffffff) {
+        set_error("H=%d, kv_heads=%d, tokens=%lld: need H a multiple of kv_heads, and tokens * H < 2^31", d->H, d->kv_heads, (long long)d->tokens);
+        return SFM_ERR_SHAPE;
+    }
+    const int esz = elem_size(d->dtype);
+    int rc;
+    if ((rc = check_paged_stride("q: token", d->q_stride[0], 0, esz))) return rc;
+    if ((rc = check_paged_stride("q: head", d->q_stride[1], 0, esz))) return rc;
+    if (d->top < 0 || d->top > SFM_PAGED_TOP_MAX || (d->top && d->group < 1)) {
+        set_error("top=%d, group=%d: need 0 <= top <= %d, and groups of a token or more", d->top, d->group, SFM_PAGED_TOP_MAX);
+        return SFM_ERR_SHAPE;
+    }
+    return SFM_OK;
+}
+
+int sfm_paged_write(const sfm_paged_desc* d, const void* k, const void* v, const int64_t k_stride[2], void* k_pages, void* v_pages,
+                    const int64_t* slots, const int32_t* table, const int32_t* past, const int32_t* q_start, float* means,
+                    void* stream) {
+    int rc = check_paged(d, true);
+    if (rc) return rc;
+    if (!k || !v || !k_stride || !k_pages || !v_pages || !slots || (means && (!table || !past || !q_start))) {
+        set_error("k, v, k_stride, the pools, slots and, for means, table, past and q_start must be non-NULL");
+        return SFM_ERR_NULL;
+    }
+    const int esz = elem_size(d->dtype);
+    if ((rc = check_paged_stride("k: token", k_stride[0], 0, esz)) || (rc = check_paged_stride("k: head", k_stride[1], 0, esz))) return rc;
+    if (!aligned16(k) || !aligned16(v) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned4(means) || !aligned4(table) || !aligned4(past) ||
+        !aligned4(q_start) || (((uintptr_t)slots) & 7)) {
+        set_error("rows and pools must be 16-byte aligned, the arrays to their elements");
+        return SFM_ERR_ALIGN;
+    }
+    return launch_paged_write(*d, k, v, k_stride, k_pages, v_pages, slots, table, past, q_start, means, (hipStream_t)stream);
+}
+
+static int check_paged_attention(const sfm_paged_desc* d) {
+    int rc = check_paged(d, true);
+    if (rc || (rc = check_paged_q(d))) return rc;
+    const int esz = elem_size(d->dtype);
+    if ((rc = check_paged_stride("out: token", d->o_stride[0], d->D, esz))) return rc;
+    if ((rc = check_paged_stride("out: head", d->o_stride[1], d->D, esz))) return rc;
+    if (!(d->sm_scale > 0.f) || d->sm_scale > 3.0e38f) {
+        set_error("sm_scale must be a positive number");
+        return SFM_ERR_SHAPE;
+    }
+    if (d->window < 0 || d->sink < 0 || (d->sink && !d->window) || (d->top && d->window)) {
+        set_error("window=%d, sink=%d, top=%d: a sink goes with a window, and neither with selected pages", d->window, d->sink, d->top);
+        return SFM_ERR_RANGE;
+    }
+    return SFM_OK;
+}
+
+int sfm_paged_workspace_bytes(const sfm_paged_desc* desc, size_t* bytes) {
+    if (!bytes) {
+        set_error("bytes is NULL");
+        return SFM_ERR_NULL;
+    }
+    const int rc = check_paged_attention(desc);
+    if (rc) return rc;
+    *bytes = paged_workspace_bytes(*desc);
+    return SFM_OK;
+}
+
+int sfm_paged_attention(const sfm_paged_desc* d, const void* q, const void* k_pages, const void* v_pages, const int32_t* table,
+                        const int32_t* past, const int32_t* q_start, const int32_t* selected, void* out, float* lse, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+    const int rc = check_paged_attention(d);
+    if (rc) return rc;
+    if (!q || !k_pages || !v_pages || !table || !past || !q_start || !out || (d->top && !selected)) {
+        set_error("q, the pools, table, past, q_start, out and, with top, selected must be non-NULL");
+        return SFM_ERR_NULL;
+    }
+    if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) || !aligned4(table) || !aligned4(past) ||
+        !aligned4(q_start) || !aligned4(selected) || !aligned4(lse) || !aligned16(workspace)) {
+        set_error("tensors and workspace must be 16-byte aligned, the arrays to their elements");
+        return SFM_ERR_ALIGN;
+    }
+    return launch_paged_attention(*d, q, k_pages, v_pages, table, past, q_start, selected, out, lse, workspace, workspace_bytes,
+                                  (hipStream_t)stream);
+}
+
+static int check_paged_select(const sfm_paged_desc* d) {
+    int rc = check_paged(d, false);
+    if (rc || (rc = check_paged_q(d))) return rc;
+    if (d->top < 1) {
+        set_error("top=%d: need a page or more", d->top);
+        return SFM_ERR_SHAPE;
+    }
+    return SFM_OK;
+}
+
+int sfm_paged_select_workspace_bytes(const sfm_paged_desc* desc, size_t* bytes) {
+    if (!bytes) {
+        set_error("bytes is NULL");
+        return SFM_ERR_NULL;
+    }
+    const int rc = check_paged_select(desc);
+    if (rc) return rc;
+    *bytes = paged_select_workspace_bytes(*desc);
+    return SFM_OK;
+}
+
+int sfm_paged_select(const sfm_paged_desc* d, const void* q, const float* means, const int32_t* table, const int32_t* past,
+                     const int32_t* q_start, int32_t first, int32_t last, int32_t* selected, void* workspace, size_t workspace_bytes,
+                     void* stream) {
+    const int rc = check_paged_select(d);
+    if (rc) return rc;
+    if (!q || !means || !table || !past || !q_start || !selected) {
+        set_error("q, means, table, past, q_start and selected must be non-NULL");
+        return SFM_ERR_NULL;
+    }
+    if (first < 0 || last < 0 || (int64_t)first + last > d->top) {
+        set_error("first=%d, last=%d: need 0 or more of each, and no more than top=%d together", first, last, d->top);
+        return SFM_ERR_RANGE;
+    }
+    if (!aligned16(q) || !aligned16(means) || !aligned4(table) || !aligned4(past) || !aligned4(q_start) || !aligned4(selected)) {
+        set_error("q and means must be 16-byte aligned, the arrays to their elements");
+        return SFM_ERR_ALIGN;
+    }
+    const size_t need = paged_select_workspace_bytes(*d);
+    if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need)) {
+        set_error("workspace must be non-NULL, 16-byte aligned and hold %zu bytes", need);
+        return SFM_ERR_WORKSPACE;
+    }
+    return launch_paged_select(*d, q, means, table, past, q_start, first, last, selected, workspace, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -33,7 +33,9 @@ SYMBOLS = [
     "sfm_monarch_attn_with_kv_cache_kept", "sfm_dense_bwd_workspace_bytes", "sfm_dense_bwd", "sfm_probe_mfma_bf16", "sfm_probe_tile_traffic", "sfm_probe_row_stream", "sfm_probe_l2_read", "sfm_conv3d_cl", "sfm_vae_norm_act",
     "sfm_quantize8", "sfm_dequantize8", "sfm_pack8", "sfm_linear8", "sfm_linear8_fwd", "sfm_linear8_wgrad_workspace_bytes", "sfm_linear8_wgrad",
     "sfm_linear8_bwd_workspace_bytes", "sfm_linear8_bwd", "sfm_linear8_plan", "sfm_linear8_wgrad_plan",
-    "sfm_gelu_bwd", "sfm_ln_keep8", "sfm_ln_bwd_workspace_bytes", "sfm_ln_bwd", "sfm_set_switches", "sfm_get_switches", "sfm_last_error", "sfm_version",
+    "sfm_gelu_bwd", "sfm_ln_keep8", "sfm_ln_bwd_workspace_bytes", "sfm_ln_bwd",
+    "sfm_paged_plan_workspace_bytes", "sfm_paged_plan", "sfm_paged_write", "sfm_paged_workspace_bytes", "sfm_paged_attention",
+    "sfm_paged_select_workspace_bytes", "sfm_paged_select", "sfm_set_switches", "sfm_get_switches", "sfm_last_error", "sfm_version",
 ]
 
 
@@ -95,6 +97,17 @@ class PrologueDesc(C.Structure):
                 ("F", C.c_int32), ("h", C.c_int32), ("w", C.c_int32), ("start_frame", C.c_int32),
                 ("eps", C.c_float), ("tiling", Tiling), ("x_stride", C.c_int64 * 2), ("q_stride", C.c_int64 * 3),
                 ("cache_stride", C.c_int64 * 3), ("cache_tokens", C.c_int64), ("start_idx", C.c_int64)]
+
+
+PAGED_TOP_MAX = 2048                  # SFM_PAGED_TOP_MAX of include/sfm_attn.h
+
+
+class PagedDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("H", C.c_int32), ("kv_heads", C.c_int32), ("D", C.c_int32), ("tokens", C.c_int64),
+                ("requests", C.c_int32), ("width", C.c_int32), ("pages", C.c_int32), ("page_size", C.c_int32), ("table_stride", C.c_int64),
+                ("pool_stride", C.c_int64 * 3), ("q_stride", C.c_int64 * 2), ("o_stride", C.c_int64 * 2), ("sm_scale", C.c_float),
+                ("causal", C.c_int32), ("window", C.c_int32), ("sink", C.c_int32), ("top", C.c_int32), ("group", C.c_int32),
+                ("zero_rest", C.c_int32), ("reserved", C.c_int32)]
 
 
 _lib = None
@@ -168,6 +181,13 @@ def load():
     lib.sfm_ln_keep8.argtypes = [I32, I64, I32, C.c_float, P, I64, P, I64, P, P, I64, I32, P, P, P, P, P, P]
     lib.sfm_ln_bwd_workspace_bytes.argtypes = [I64, I32, I64, C.POINTER(C.c_size_t)]
     lib.sfm_ln_bwd.argtypes = [I32, I64, I32, C.c_float, P, I64, P, P, P, P, I64, P, P, I64, I64, P, I64, P, P, P, C.c_size_t, P]
+    PD = C.POINTER(PagedDesc)
+    lib.sfm_paged_plan_workspace_bytes.argtypes = [I32, C.POINTER(C.c_size_t)]
+    lib.sfm_paged_plan.argtypes = [I32, I32, I32, I64, P, I64, P, P, P, I64, P, P, P, P, P, P, C.c_size_t, P]
+    lib.sfm_paged_write.argtypes = [PD, P, P, S3, P, P, P, P, P, P, P, P]
+    lib.sfm_paged_workspace_bytes.argtypes = lib.sfm_paged_select_workspace_bytes.argtypes = [PD, C.POINTER(C.c_size_t)]
+    lib.sfm_paged_attention.argtypes = [PD, P, P, P, P, P, P, P, P, P, P, C.c_size_t, P]
+    lib.sfm_paged_select.argtypes = [PD, P, P, P, P, P, I32, I32, P, P, C.c_size_t, P]
     lib.sfm_vae_norm_act.argtypes = [C.c_int32] * 6 + [P, S3, P, P, S3, P]
     lib.sfm_probe_mfma_bf16.argtypes = [C.c_int32, P, C.POINTER(C.c_float)]
     lib.sfm_probe_tile_traffic.argtypes = [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, P, C.c_size_t, P, C.POINTER(C.c_float)]

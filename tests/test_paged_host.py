@@ -1,0 +1,207 @@
+"""What the paged cache's entry points and functions refuse, without a GPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+import self_forcing_amd as sfa
+from self_forcing_amd import lib as L
+
+PA = sfa.paged_attn
+P = 4096                                          # an aligned address that nothing reads: every call here is refused
+
+
+def desc(**change):
+    d = L.PagedDesc(L.SFM_BF16, 8, 2, 128, 10, 3, 5, 40, 16, 5, (16 * 2 * 128, 2 * 128, 128), (8 * 128, 128), (8 * 128, 128), 0.1, 1, 0, 0, 0, 1, 1, 0)
+    for k, v in change.items():
+        setattr(d, k, v)
+    return d
+
+
+def attention(d, **ptr):
+    p = dict(q=P, k=P, v=P, table=P, past=P, q_start=P, selected=None, out=P, lse=None, ws=None)
+    p.update(ptr)
+    return L.load().sfm_paged_attention(C.byref(d), p["q"], p["k"], p["v"], p["table"], p["past"], p["q_start"], p["selected"], p["out"], p["lse"],
+                                        p["ws"], 0, None)
+
+
+def select(d, first=1, last=1, **ptr):
+    p = dict(q=P, means=P, table=P, past=P, q_start=P, selected=P, ws=None)
+    p.update(ptr)
+    return L.load().sfm_paged_select(C.byref(d), p["q"], p["means"], p["table"], p["past"], p["q_start"], first, last, p["selected"], p["ws"], 0, None)
+
+
+def write(d, stride=(256, 128), **ptr):
+    p = dict(k=P, v=P, kp=P, vp=P, slots=P, table=P, past=P, q_start=P, means=P)
+    p.update(ptr)
+    return L.load().sfm_paged_write(C.byref(d), p["k"], p["v"], (C.c_int64 * 2)(*stride), p["kp"], p["vp"], p["slots"], p["table"], p["past"],
+                                    p["q_start"], p["means"], None)
+
+
+def plan(requests=3, width=5, page=16, tokens=10, stride=5, free_count=9, **ptr):
+    # addresses far apart: outputs must not lie in inputs
+    p = dict(table=1 << 20, past=2 << 20, new=3 << 20, free=4 << 20, taken=None, q_start=5 << 20, lengths=6 << 20, slots=7 << 20, next_free=8 << 20)
+    p.update(ptr)
+    return L.load().sfm_paged_plan(requests, width, page, tokens, p["table"], stride, p["past"], p["new"], p["free"], free_count, p["taken"], p["q_start"],
+                                   p["lengths"], p["slots"], p["next_free"], None, 0, None)
+
+
+NULL, DTYPE, SHAPE, RANGE, STRIDE, WORKSPACE, ALIGN = -1, -2, -3, -4, -5, -6, -7
+SHARED = [(dict(dtype=7), DTYPE), (dict(kv_heads=0), SHAPE), (dict(D=12), SHAPE), (dict(D=264), SHAPE), (dict(D=0), SHAPE), (dict(pages=0), SHAPE),
+          (dict(requests=0), SHAPE), (dict(requests=(1 << 24) + 1), SHAPE), (dict(width=0), SHAPE), (dict(page_size=12), SHAPE), (dict(page_size=0), SHAPE),
+          (dict(width=1 << 20, page_size=2048, table_stride=1 << 20), SHAPE), (dict(pages=1 << 20, page_size=2048), SHAPE), (dict(tokens=0), SHAPE),
+          (dict(tokens=-1), SHAPE), (dict(tokens=1 << 31), SHAPE), (dict(table_stride=4), STRIDE)]
+POOL = [(dict(pool_stride=(4096, 256, 120)), STRIDE), (dict(pool_stride=(4096, 256, 132)), STRIDE), (dict(pool_stride=(4096, 64, 128)), STRIDE),
+        (dict(pool_stride=(-4096, 256, 128)), STRIDE), (dict(pool_stride=(4096, 1 << 24, 128)), STRIDE)]
+Q = [(dict(H=7), SHAPE), (dict(H=1), SHAPE), (dict(tokens=1 << 29), SHAPE), (dict(q_stride=(1024, 129)), STRIDE), (dict(q_stride=(-1024, 128)), STRIDE),
+     (dict(top=-1), SHAPE), (dict(top=2049), SHAPE), (dict(top=2, group=0), SHAPE)]
+
+
+@pytest.mark.parametrize("change,code", SHARED + POOL + Q + [
+    (dict(o_stride=(1024, 64)), STRIDE), (dict(o_stride=(1020, 128)), STRIDE), (dict(sm_scale=0.0), SHAPE), (dict(sm_scale=float("nan")), SHAPE),
+    (dict(sm_scale=float("inf")), SHAPE), (dict(window=-1), RANGE), (dict(sink=-1), RANGE), (dict(sink=3), RANGE), (dict(top=4, window=8), RANGE)])
+def test_attention_refuses(change, code):
+    d, n = desc(**change), C.c_size_t(0)
+    assert attention(d, selected=P) == code
+    assert L.load().sfm_paged_workspace_bytes(C.byref(d), C.byref(n)) == code
+
+
+@pytest.mark.parametrize("ptr,code", [(dict(q=None), NULL), (dict(k=None), NULL), (dict(v=None), NULL), (dict(table=None), NULL), (dict(past=None), NULL),
+                                      (dict(q_start=None), NULL), (dict(out=None), NULL), (dict(q=P + 2), ALIGN), (dict(v=P + 8), ALIGN), (dict(out=P + 4), ALIGN),
+                                      (dict(table=P + 2), ALIGN), (dict(lse=P + 2), ALIGN), (dict(ws=P + 8), ALIGN)])
+def test_attention_refuses_pointers(ptr, code):
+    assert attention(desc(), **ptr) == code
+    assert attention(desc(top=4), selected=None) == NULL and attention(desc(top=4), selected=P + 1) == ALIGN
+
+
+@pytest.mark.parametrize("change,code", SHARED + Q + [(dict(top=0), SHAPE)])
+def test_select_refuses(change, code):
+    d, n = desc(**{"top": 4, **change}), C.c_size_t(0)
+    assert select(d) == code
+    assert L.load().sfm_paged_select_workspace_bytes(C.byref(d), C.byref(n)) == code
+
+
+def test_select_refuses_the_rest():
+    d = desc(top=4)
+    for name in ("q", "means", "table", "past", "q_start", "selected"):
+        assert select(d, **{name: None}) == NULL
+        assert select(d, **{name: P + 2}) == ALIGN
+    assert select(d, first=-1) == RANGE and select(d, last=-1) == RANGE and select(d, first=3, last=2) == RANGE
+    assert select(d, first=2 ** 31 - 1, last=2 ** 31 - 1) == RANGE
+
+
+@pytest.mark.parametrize("change,code", SHARED + POOL)
+def test_write_refuses(change, code):
+    assert write(desc(**change)) == code
+
+
+def test_write_refuses_the_rest():
+    for name in ("k", "v", "kp", "vp", "slots", "table", "past", "q_start"):
+        assert write(desc(), **{name: None}) == NULL
+        assert write(desc(), **{name: P + 2}) == ALIGN
+    assert write(desc(), stride=(257, 128)) == STRIDE and write(desc(), stride=(256, -128)) == STRIDE and write(desc(), means=P + 2) == ALIGN
+
+
+def test_plan_refuses():
+    for kw, code in [(dict(requests=0), SHAPE), (dict(width=0), SHAPE), (dict(page=4), SHAPE), (dict(page=20), SHAPE), (dict(tokens=-1), SHAPE),
+                     (dict(tokens=1 << 31), SHAPE), (dict(stride=4), STRIDE), (dict(free_count=-1), RANGE), (dict(width=1 << 28, stride=1 << 28), SHAPE)]:
+        assert plan(**kw) == code, kw
+    for name in ("table", "past", "new", "free", "q_start", "lengths", "slots", "next_free"):
+        assert plan(**{name: None}) == NULL, name
+    for name in ("table", "past", "new", "free", "taken", "q_start", "lengths", "slots", "next_free"):
+        assert plan(**{name: (20 << 20) + 2}) == ALIGN, name
+    assert plan(slots=(7 << 20) + 4) == ALIGN
+    assert plan(q_start=2 << 20) == RANGE and plan(next_free=9 << 20, taken=9 << 20) == RANGE and plan(lengths=2 << 20) == RANGE
+    assert plan(slots=(1 << 20) + 8) == RANGE and plan(table=(4 << 20) + 32) == RANGE
+    assert plan(requests=9000, stride=5, width=5) == WORKSPACE
+    n = C.c_size_t(1)
+    assert L.load().sfm_paged_plan_workspace_bytes(0, C.byref(n)) == SHAPE and L.load().sfm_paged_plan_workspace_bytes(3, None) == NULL
+    assert L.load().sfm_paged_plan_workspace_bytes(3, C.byref(n)) == 0 and n.value == 0
+    assert L.load().sfm_paged_workspace_bytes(C.byref(desc()), None) == NULL and L.load().sfm_paged_select_workspace_bytes(C.byref(desc()), None) == NULL
+    assert L.load().sfm_paged_workspace_bytes(None, C.byref(n)) == NULL
+
+
+# ---------------------------------------------------------------- the functions, with tensors that are not on the GPU
+def cpu_plan(T=4, R=2):
+    i = torch.zeros(R, dtype=torch.int32)
+    return PA.PagePlan(torch.zeros((R, 3), dtype=torch.int32), i, i, torch.zeros(R + 1, dtype=torch.int32), torch.zeros(T, dtype=torch.int64),
+                       torch.zeros(1, dtype=torch.int32), 16)
+
+
+def test_functions_want_the_gpu():
+    pool, q = torch.zeros((4, 16, 2, 64), dtype=torch.bfloat16), torch.zeros((4, 2, 64), dtype=torch.bfloat16)
+    i = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="GPU"):
+        PA.plan_pages(torch.zeros((2, 3), dtype=torch.int32), i, i, i, 4, 16)
+    with pytest.raises(ValueError, match="GPU"):
+        PA.write_pages(q, q, pool, pool, cpu_plan())
+    with pytest.raises(ValueError, match="GPU"):
+        PA.paged_attention(q, pool, pool, cpu_plan())
+    with pytest.raises(ValueError, match="GPU"):
+        PA.select_pages(q, torch.zeros((4, 2, 64)), cpu_plan(), 2)
+
+
+def test_gradients_are_refused():
+    pool, q = torch.zeros((4, 16, 2, 64)), torch.zeros((4, 2, 64), requires_grad=True)
+    for call in (lambda: PA.write_pages(q, q, pool, pool, cpu_plan()), lambda: PA.paged_attention(q, pool, pool, cpu_plan()),
+                 lambda: PA.paged_attention(q.detach(), pool, pool.requires_grad_(), cpu_plan()), lambda: PA.select_pages(q, pool[:, 0], cpu_plan(), 2)):
+        with pytest.raises(NotImplementedError, match="differentiable"):
+            call()
+
+
+def test_tables_and_arrays():
+    for bad in (torch.zeros((2, 3), dtype=torch.int64), torch.zeros(3, dtype=torch.int32), None):
+        with pytest.raises(ValueError, match="table"):
+            PA._table(bad)
+    for bad in (torch.zeros(2, dtype=torch.int64), torch.zeros((2, 1), dtype=torch.int32), [1, 2], torch.zeros(3, dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            PA._ints("past", bad, torch.device("cpu"), 2)
+    assert PA._ints("past", torch.arange(6, dtype=torch.int32)[::3], torch.device("cpu"), 2).tolist() == [0, 3]
+
+
+def test_strides_of_rows_and_pools():
+    x = torch.zeros((5, 3, 2, 8))
+    assert PA._rows("q", x[:, 1], x.dtype, x.device) == (48, 8)
+    assert PA._rows("q", x[:1, 1, 1:], x.dtype, x.device) == (8, 8)          # dimensions of one
+    with pytest.raises(ValueError):
+        PA._rows("q", x[:, 1].transpose(1, 2), x.dtype, x.device)
+    with pytest.raises(ValueError):
+        PA._rows("q", x[:, 1], torch.float16, x.device)
+    assert PA._pool_strides(x) == (48, 16, 8)
+    assert PA._pool_strides(x[:1, :, :1]) == (48, 16, 8)
+    assert PA._pool_strides(x.transpose(1, 2)) == (48, 8, 16)
+
+
+GPU_ONLY = [
+    ("q heads", dict(H=3), "multiple"), ("q size", dict(D=32), "head_dim"), ("q type", dict(dtype=torch.float16), "expected"),
+    ("window", dict(window=0), "window"), ("sink", dict(sink=2), "sink"), ("both", dict(window=4, selected=True), "together"), ("group", dict(group=0, selected=True), "group"),
+    ("lists", dict(group=3, selected=True), "selected must"), ("out", dict(out=(5, 2, 64)), "like q"), ("rows", dict(T=5), "slots"), ("page size", dict(page=8), "rows"),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name,kw,match", GPU_ONLY, ids=[n for n, *_ in GPU_ONLY])
+def test_attention_refuses_tensors(name, kw, match):
+    dev = "cuda:0"
+    kw = dict(kw)
+    plan = PA.PagePlan(*(t.to(dev) if isinstance(t, torch.Tensor) else t for t in cpu_plan()))._replace(page_size=kw.pop("page", 16))
+    pool = torch.zeros((4, 16, 2, 64), dtype=torch.bfloat16, device=dev)
+    q = torch.zeros((kw.pop("T", 4), kw.pop("H", 4), kw.pop("D", 64)), dtype=kw.pop("dtype", torch.bfloat16), device=dev)
+    if "out" in kw:
+        kw["out"] = torch.zeros(kw["out"], dtype=q.dtype, device=dev)
+    if kw.pop("selected", False):
+        kw["selected"] = torch.zeros((PA.selected_rows(4, 2, 1), 2, 3), dtype=torch.int32, device=dev)
+    with pytest.raises(ValueError, match=match):
+        PA.paged_attention(q, pool, pool, plan, **kw)
+
+
+@pytest.mark.gpu
+def test_empty_steps():
+    dev = "cuda:0"
+    plan = PA.plan_pages(torch.zeros((2, 3), dtype=torch.int32, device=dev), *(torch.zeros(2, dtype=torch.int32, device=dev) for _ in range(3)), 0, 16)
+    pool = torch.zeros((4, 16, 2, 64), dtype=torch.bfloat16, device=dev)
+    q, k = pool.new_zeros((0, 4, 64)), pool.new_zeros((0, 2, 64))
+    PA.write_pages(k, k, pool, pool, plan)
+    out, lse = PA.paged_attention(q, pool, pool, plan, return_lse=True)
+    assert out.shape == (0, 4, 64) and lse.shape == (4, 0)
+    assert bool((PA.select_pages(q, torch.zeros((4, 2, 64), device=dev), plan, 2) == -1).all()) and plan.q_start.tolist() == [0, 0, 0]

@@ -1,0 +1,122 @@
+"""Arithmetic of the paged cache's kernels (csrc/paged_rules.hpp), compiled for the host."""
+import ctypes as C
+import os
+import random
+import shutil
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+SOURCE = """
+#include "paged_rules.hpp"
+extern "C" unsigned quotient(unsigned n, unsigned d) { return sfm::quot(n, sfm::fast_div(d)); }
+extern "C" void request(const int* q_start, const int* past, int r, int R, int T, int* out) {
+    const sfm::Request q = sfm::request_of(q_start, past, r, R, T);
+    out[0] = q.first; out[1] = q.n; out[2] = q.past;
+}
+extern "C" long long piece(long long start, long long heads, long long per, int r) { return sfm::first_piece(start, heads, per, r); }
+extern "C" long long all_pieces(long long rows, long long per, int R) { return sfm::pieces(rows, per, R); }
+extern "C" void tiles(int past, int n, int none, int t0, int t1, int causal, int window, int sink, int cap, int* out) {
+    const sfm::Request q{0, n, past};
+    const sfm::KeyTiles k = sfm::key_tiles(q, none, t0, t1, causal, window, sink, cap);
+    const int v[] = {k.end_min, k.end_max, k.lo_min, k.lo_max, k.sinks, k.first, k.tiles, k.fast0, k.fast1, k.beyond};
+    for (int i = 0; i < 10; ++i) out[i] = v[i];
+}
+extern "C" int tile(int past, int n, int t0, int t1, int causal, int window, int sink, int cap, int v) {
+    return sfm::tile_of(sfm::key_tiles(sfm::Request{0, n, past}, false, t0, t1, causal, window, sink, cap), v);
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def rules(tmp_path_factory):
+    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    d = tmp_path_factory.mktemp("rules")
+    (d / "rules.hip").write_text(SOURCE)
+    csrc = os.path.join(ROOT, "self-forcing_amd", "csrc")
+    subprocess.run([hipcc, "--offload-host-only", "-std=c++17", "-shared", "-fPIC", "-I" + csrc, "-I" + os.path.join(ROOT, "include"),
+                    str(d / "rules.hip"), "-o", str(d / "rules.so")], check=True, capture_output=True)
+    lib = C.CDLL(str(d / "rules.so"))
+    lib.quotient.restype = C.c_uint
+    lib.piece.restype = lib.all_pieces.restype = C.c_longlong
+    lib.piece.argtypes = [C.c_longlong] * 3 + [C.c_int]
+    lib.all_pieces.argtypes = [C.c_longlong] * 2 + [C.c_int]
+    return lib
+
+
+def test_quotients(rules):
+    rng = random.Random(1)
+    top = 2 ** 28 - 1
+    for d in [1, 2, 3, 5, 7, 8, 195, 2 ** 14 - 1, 2 ** 20 + 1, 2 ** 27 + 1, 2 ** 28 - 1] + [rng.randint(1, top) for _ in range(300)]:
+        near = [k * d + e for k in (1, 2, 3, top // d) for e in (-1, 0, 1)]
+        for n in [0, 1, d, top, top - 1] + near + [rng.randint(0, top) for _ in range(60)]:
+            if 0 <= n <= top:
+                assert rules.quotient(n, d) == n // d, (n, d)
+
+
+def test_pieces_are_every_row_once(rules):
+    rng = random.Random(2)
+    for _ in range(200):
+        R, per, heads = rng.randint(1, 40), rng.choice([1, 2, 7, 32, 128, 256]), rng.choice([1, 3, 8])
+        n = [rng.choice([0, 1, 1, rng.randint(0, 300)]) for _ in range(R + 1)]          # the last: rows of nobody
+        start, at = [], 0
+        for m in n:
+            start.append(at)
+            at += m
+        taken = set()
+        for r, m in enumerate(n):
+            first = rules.piece(start[r], heads, per, r)
+            own = range(first, first - (-m * heads // per))
+            assert not taken & set(own)
+            taken |= set(own)
+            assert r == R or rules.piece(start[r + 1], heads, per, r + 1) >= first + len(own)
+            assert first + len(own) <= rules.all_pieces(at * heads, per, R)
+
+
+def test_requests_stay_inside_the_rows(rules):
+    rng = random.Random(3)
+    odd = [0, 1, 5, 100, -1, -2 ** 31, 2 ** 31 - 1, 101]
+    for _ in range(500):
+        R, T = 3, 100
+        qs, ps = [rng.choice(odd) for _ in range(R + 1)], [rng.choice(odd) for _ in range(R)]
+        for r in range(R + 1):
+            out = (C.c_int * 3)()
+            rules.request((C.c_int * (R + 1))(*qs), (C.c_int * R)(*ps), r, R, T, out)
+            assert 0 <= out[0] <= T and 0 <= out[1] <= T - out[0] and out[2] >= 0
+
+
+def visible(past, n, t, causal, window, sink, cap):
+    end = past + t + 1 if causal else past + n
+    end = min(end, cap)
+    return {p for p in range(end) if not window or p >= end - window or p < sink}
+
+
+def test_tiles_hold_what_a_piece_sees_and_fast_ones_nothing_else(rules):
+    rng = random.Random(4)
+    for _ in range(3000):
+        past, n, causal = rng.choice([0, 1, 63, 64, 65, 500, rng.randint(0, 900)]), rng.randint(1, 300), rng.randint(0, 1)
+        t0 = rng.randint(0, n - 1)
+        t1 = rng.randint(t0, min(n - 1, t0 + 255))
+        window = rng.choice([0, 1, 64, 100, rng.randint(1, 700), 5000])
+        sink = rng.choice([0, 1, 64, rng.randint(0, 400)]) if window else 0
+        cap = rng.choice([10 ** 6, 8 * rng.randint(1, 100)])
+        out = (C.c_int * 10)()
+        rules.tiles(past, n, 0, t0, t1, causal, window, sink, cap, out)
+        end_min, end_max, lo_min, lo_max, sinks, first, count, fast0, fast1, beyond = out
+        assert bool(beyond) == ((past + t1 + 1 if causal else past + n) > cap)
+        seen = [visible(past, n, t, causal, window, sink, cap) for t in range(t0, t1 + 1)]
+        order = [rules.tile(past, n, t0, t1, causal, window, sink, cap, v) for v in range(count)]
+        assert order == sorted(set(order))
+        covered = {p for i in order for p in range(64 * i, 64 * i + 64)}
+        assert set().union(*seen) <= covered
+        assert 0 <= fast0 <= fast1 <= count
+        for v in range(fast0, fast1):
+            assert all(set(range(64 * order[v], 64 * order[v] + 64)) <= s for s in seen)
+        for t, s in zip(range(t0, t1 + 1), seen):          # the mask that a kernel takes from a row's own end
+            end = min(past + t + 1 if causal else past + n, cap)
+            lo = max(0, end - window) if window else 0
+            assert s == {p for p in covered if p < end and (p >= lo or p < sink)}
+            assert end_min <= end <= end_max and lo_min <= lo <= lo_max
+    rules.tiles(9, 5, 1, 0, 4, 1, 0, 0, 100, out)
+    assert out[6] == 0                                     # rows of nobody
