@@ -1,4 +1,7 @@
 // Attention of the requests' new tokens over their pages of a shared key-value cache.
+#include <algorithm>
+
+#include "attn_tiles.hpp"
 #include "paged_rules.hpp"
 
 namespace sfm {
@@ -66,8 +69,6 @@ __global__ __launch_bounds__(256) void paged_generic_kernel(PagedArgs a) {
                 const int page = e < d.width ? a.table[r * d.table_stride + e] : -1;
                 if (page < 0 || page >= d.pages) bad = true;
                 else row = page * d.pool_stride[0] + (int64_t)(v % P) * d.pool_stride[1] + (int64_t)kh * d.pool_stride[2];
-            } else if (sel && e >= d.width) {
-                bad = true;
             }
         }
         at[tid] = row;
@@ -112,22 +113,580 @@ __global__ __launch_bounds__(256) void paged_generic_kernel(PagedArgs a) {
     if (a.lse != nullptr && tid == 0) a.lse[(int64_t)h * d.tokens + t] = bad ? NAN : seen ? (mrun + log2f(lrun)) * kLn2 : -INFINITY;
 }
 
-size_t paged_workspace_bytes(const sfm_paged_desc&) { return 0; }
+// ------------------------------------------------------------------------------------------------
+// MFMA kernels (16-bit tensors, head sizes 64 and 128)
+//
+// A piece is up to 32 NW rows (token, query head) of one request and one key head.  Its keys come in virtual tiles of 64 positions
+// (KeyTiles), or of the selected pages one after the other; eight positions, a block, never straddle a page.  A lane works out where
+// one block lies, for eight tiles at a time, and a load of K or V rows takes its block's offset from that lane.  The products
+// are those of the dense kernel: S^T[l, q] = K[l,:] . Q[q,:], O^T[d, q] += V^T[d, l] P^T[l, q], a lane holds one row's logits.
+// ------------------------------------------------------------------------------------------------
+struct Piece {
+    Request rq;
+    KeyTiles k;
+    int r, kh, row0, row1;         // rows [row0, row1) of the request's n * G
+    const int32_t* sel;            // selected entries, `count` of them, or NULL
+    int count;
+};
 
-int launch_paged_attention(const sfm_paged_desc& d, const void* q, const void* kp, const void* vp, const int32_t* table,
-                           const int32_t* past, const int32_t* q_start, const int32_t* selected, void* out, float* lse, void*,
-                           size_t, hipStream_t stream) {
-    PagedArgs a{d, fast_div(d.page_size / 8), d.width * d.page_size, q, kp, vp, table, past, q_start, selected, out, lse};
-    auto kern = d.dtype == SFM_BF16 ? paged_generic_kernel<BF16> : d.dtype == SFM_F16 ? paged_generic_kernel<F16> : paged_generic_kernel<float>;
-    if (d.tokens >= (1 << 24) || d.H > 65535) {
-        set_error("tokens=%lld, H=%d are more than a launch takes", (long long)d.tokens, d.H);
-        return SFM_ERR_UNSUPPORTED;
+// Softmax state of a wave's 32 rows, lane (m, hf) row m: O^T accumulators, running maximum (base-2 units) and this half's sum
+template <int D>
+struct RowState {
+    f32x16 o[D / 32];
+    float mrun, lrun;
+    bool seen;
+    __device__ __forceinline__ void init() {
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[dt][v] = 0.f;
+        mrun = -__FLT_MAX__;
+        lrun = 0.f;
+        seen = false;
     }
-    hipLaunchKernelGGL(kern, dim3((unsigned)d.tokens, d.H), dim3(256), 0, stream, a);
+    __device__ __forceinline__ void raise(float mnew) {
+        if (__builtin_amdgcn_ballot_w64(mnew > mrun) != 0) {
+            const float alpha = fast_exp2(mrun - mnew);
+            lrun *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) o[dt][v] *= alpha;
+            mrun = mnew;
+        }
+    }
+};
+
+// What a row sees of a tile: positions below `end` that are at or past `lo` or below `sink`
+struct RowMask {
+    int end, lo, sink;
+    __device__ __forceinline__ bool sees(int pos) const { return pos < end && (pos >= lo || pos < sink); }
+};
+
+// Key that register v of a lane's logits t belongs to
+__device__ __forceinline__ constexpr int key_of(int t, int v) { return 32 * t + 8 * (v >> 2) + (v & 3); }      // + 4 hf
+
+// One tile of LDS against the wave's rows: logits, masks, weights and V's part.  pos: first positions of the tile's eight blocks.
+// The second half waits for V through `v_ready`, so that K's buffer can be refilled meanwhile (`k_done`).
+//
+// A masked weight is 0, and 0 times an infinity or NaN is NaN: in a masked tile V rows that hold such values are left out of the
+// matrix product and added for the rows that see them, one by one.  (Stale rows, and later tokens of the request.)
+template <class E, int D, class KDone, class VReady>
+__device__ __forceinline__ void masked_tile(const char* lds, uint32_t kbuf, uint32_t vbuf, const u32x4* qb, float sc2, RowState<D>& st,
+                                            const RowMask& mask, bool masked, const int* pos, KDone k_done, VReady v_ready) {
+    using L = DnLds<D>;
+    const int lane = threadIdx.x & 63, m = lane & 31, hf = lane >> 5;
+    f32x16 s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[t][v] = 0.f;
+    const uint32_t sA0 = kbuf + (uint32_t)m * L::kPitch + (uint32_t)((hf ^ L::swz(m)) << 4);
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) {
+        const u32x4 a = *(const u32x4*)(lds + (sA0 ^ (uint32_t)((j >> 1) << 5)) + (j & 1) * 32 * L::kPitch);
+        s[j & 1] = E::mfma32(a, qb[j >> 1], s[j & 1]);
+    }
+    k_done();
+    if (masked) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const bool see = mask.sees(pos[4 * t + (v >> 2)] + 4 * hf + (v & 3));
+                st.seen = st.seen || see;
+                s[t][v] = see ? s[t][v] : -INFINITY;
+            }
+    } else {
+        st.seen = true;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) mx = fmaxf(mx, s[i >> 4][i & 15]);
+    st.raise(fmaxf(st.mrun, xhalf_max(mx) * sc2));
+    u32x4 pb[4];
+    float psum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+        const float a = fast_exp2(fmaf(s[i >> 4][i & 15], sc2, -st.mrun)), b = fast_exp2(fmaf(s[i >> 4][(i & 15) + 1], sc2, -st.mrun));
+        psum += a + b;
+        s[i >> 4][i & 15] = a;
+        s[i >> 4][(i & 15) + 1] = b;
+        pb[i >> 3][(i >> 1) & 3] = pack2<E>(a, b);
+    }
+    st.lrun += psum;
+    v_ready();
+    // V rows with values that are not finite, a lane each
+    uint64_t odd = 0;
+    if (masked) {
+        constexpr uint32_t kExp = E::kDtype == SFM_BF16 ? 0x7f807f80u : 0x7c007c00u, kOne = E::kDtype == SFM_BF16 ? 0x00800080u : 0x04000400u;
+        uint32_t acc = 0;
+#pragma unroll 4
+        for (int c = 0; c < L::kCPR; ++c) {
+            const u32x4 w = *(const u32x4*)(lds + vbuf + (uint32_t)lane * L::kPitch + (uint32_t)(((c + lane) % L::kCPR) << 4));
+#pragma unroll
+            for (int x = 0; x < 4; ++x) acc |= (w[x] & kExp) + kOne;       // all ones in the exponent: the sum reaches the sign's place
+        }
+        odd = __builtin_amdgcn_ballot_w64((acc & 0x80008000u) != 0);
+    }
+    uint32_t trA[2];
+    const int s16 = lane & 15, rl = 4 * hf + (s16 >> 2), cl = 2 * ((lane >> 4) & 1) + ((s16 & 3) >> 1);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const int r = rl + 8 * half;
+        trA[half] = vbuf + (uint32_t)r * L::kPitch + (uint32_t)((cl ^ L::swz(r)) << 4) + (uint32_t)(s16 & 1) * 8;
+    }
+    if (odd == 0) {
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) {
+            const u32x2 lo = dn_read_tr(lds + (trA[0] ^ (uint32_t)((j >> 2) << 6)), (j & 3) * 16 * L::kPitch);
+            const u32x2 hi = dn_read_tr(lds + (trA[1] ^ (uint32_t)((j >> 2) << 6)), (j & 3) * 16 * L::kPitch);
+            st.o[j >> 2] = E::mfma32(u32x4{lo.x, lo.y, hi.x, hi.y}, pb[j & 3], st.o[j >> 2]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) {
+        const u32x2 lo = dn_read_tr(lds + (trA[0] ^ (uint32_t)((j >> 2) << 6)), (j & 3) * 16 * L::kPitch);
+        const u32x2 hi = dn_read_tr(lds + (trA[1] ^ (uint32_t)((j >> 2) << 6)), (j & 3) * 16 * L::kPitch);
+        const uint32_t bits = (uint32_t)(odd >> (16 * (j & 3))) >> (4 * hf);           // keys 16 (j % 4) + 4 hf + {0..3, 8..11}
+        const u32x4 keep = {(bits & 1 ? 0u : 0xffffu) | (bits & 2 ? 0u : 0xffff0000u), (bits & 4 ? 0u : 0xffffu) | (bits & 8 ? 0u : 0xffff0000u),
+                            (bits & 0x100 ? 0u : 0xffffu) | (bits & 0x200 ? 0u : 0xffff0000u), (bits & 0x400 ? 0u : 0xffffu) | (bits & 0x800 ? 0u : 0xffff0000u)};
+        st.o[j >> 2] = E::mfma32(u32x4{lo.x, lo.y, hi.x, hi.y} & keep, pb[j & 3], st.o[j >> 2]);
+    }
+    while (odd) {
+        const int l = __builtin_ctzll(odd);
+        odd &= odd - 1;
+        // the weight lies in half (l / 4) % 2, register 16 (l / 32) + 4 (l / 8 % 4) + l % 4
+        float w = 0.f;
+        const int at = 16 * (l >> 5) + 4 * ((l >> 3) & 3) + (l & 3);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) w = i == at ? s[i >> 4][i & 15] : w;
+        w = __shfl(w, m + 32 * ((l >> 2) & 1));
+        int p = kNoPos;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p = i == (l >> 3) ? pos[i] : p;
+        const bool see = !masked || mask.sees(p + (l & 7));
+#pragma unroll
+        for (int c = 0; c < L::kCPR; ++c) {        // channels 8 c + 4 hf + {0..3}
+            const u32x2 x = *(const u32x2*)(lds + vbuf + (uint32_t)l * L::kPitch + (uint32_t)((c ^ L::swz(l)) << 4) + 8 * hf);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float v = E::to_float((uint16_t)(x[i >> 1] >> (16 * (i & 1))));
+                // an infinity counts however small its weight; a weight of NaN makes all of the row NaN
+                const float part = w == w && !(fabsf(v) < INFINITY) ? v : w * v;
+                const float o = st.o[c >> 2][4 * (c & 3) + i];
+                st.o[c >> 2][4 * (c & 3) + i] = see ? o + part : o;
+            }
+        }
+    }
+}
+
+// Partials of split calls: [chunk][row = token * H + head] of D floats, and behind all of them (maximum, sum): a sum of 0 for nothing
+// seen, NaN for rows that are NaN.
+template <class E, int D>
+__device__ __forceinline__ void store_rows(const PagedArgs& a, const Piece& pc, RowState<D>& st, bool bad, int row0, int chunk, int chunks,
+                                           float* part, char* stage) {
+    const sfm_paged_desc& d = a.d;
+    const int lane = threadIdx.x & 63, m = lane & 31, hf = lane >> 5, G = d.H / d.kv_heads;
+    const int row = row0 + m, t = pc.rq.first + row / G, h = pc.kh * G + row % G;
+    const bool mine = row < pc.row1;
+    const float l = xhalf_sum(st.lrun);
+    const bool seen = __shfl_xor((int)st.seen, 32) || st.seen;
+    if (part != nullptr) {
+        const int64_t rows = d.tokens * d.H, at = chunk * rows + (int64_t)t * d.H + h;
+        if (!mine) return;
+        float* const po = part + at * D + 4 * hf;
+        if (seen)
+#pragma unroll
+            for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *(f32x4*)(po + 32 * dt + 8 * g) = f32x4{st.o[dt][4 * g], st.o[dt][4 * g + 1], st.o[dt][4 * g + 2], st.o[dt][4 * g + 3]};
+        if (hf == 0) {
+            float* const ml = part + chunks * rows * D + at * 2;
+            ml[0] = st.mrun;
+            ml[1] = bad || (seen && l == 0.f) ? NAN : seen ? l : 0.f;
+        }
+        return;
+    }
+    const float inv = bad ? NAN : seen ? 1.f / l : 0.f;
+    if (a.lse != nullptr && hf == 0 && mine) a.lse[(int64_t)h * d.tokens + t] = bad ? NAN : seen ? (st.mrun + log2f(l)) * kLn2 : -INFINITY;
+    // through LDS, so that the rows leave in whole lines
+    constexpr int kSP = D + 8;
+    uint16_t* const so = (uint16_t*)stage;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *(u32x2*)(so + m * kSP + 32 * dt + 8 * g + 4 * hf) = u32x2{pack2<E>(st.o[dt][4 * g] * inv, st.o[dt][4 * g + 1] * inv),
+                                                                      pack2<E>(st.o[dt][4 * g + 2] * inv, st.o[dt][4 * g + 3] * inv)};
+    lds_wave_sync();
+    uint16_t* const out = (uint16_t*)a.out;
+    for (int c = lane; c < 32 * (D / 8); c += 64) {
+        const int r = row0 + c / (D / 8), ch = c % (D / 8);
+        if (r < pc.row1)
+            *(u32x4*)(out + (int64_t)(pc.rq.first + r / G) * d.o_stride[0] + (int64_t)(pc.kh * G + r % G) * d.o_stride[1] + ch * 8) =
+                *(const u32x4*)(so + (c / (D / 8)) * kSP + ch * 8);
+    }
+}
+
+// The piece of a work item; false where it has no rows.
+template <int M>
+__device__ __forceinline__ bool find_piece(const PagedArgs& a, int64_t piece, int kh, Piece* p) {
+    const sfm_paged_desc& d = a.d;
+    const int R = d.requests, T = (int)d.tokens, G = d.H / d.kv_heads;
+    int64_t per = M, heads = G, j = 0, unit = piece;
+    if (d.top) {                   // groups, each in pieces of M rows
+        const int64_t each = ((int64_t)d.group * G + M - 1) / M;
+        unit = piece / each;
+        j = piece - unit * each;
+        per = d.group;
+        heads = 1;
+    }
+    const int r = find_last(R, unit, [&](int i) { return first_piece(clamp_int(a.q_start[i], 0, T), heads, per, i); });
+    if (r >= R && !d.zero_rest) return false;
+    p->r = r;
+    p->kh = kh;
+    p->rq = request_of(a.q_start, a.past, r, R, T);
+    const int64_t nth = unit - first_piece(p->rq.first, heads, per, r), rows = (int64_t)p->rq.n * G;
+    int64_t row0 = nth * M, last = rows;
+    if (d.top) {
+        row0 = nth * d.group * G + j * M;
+        last = min(rows, (nth + 1) * d.group * G);
+    }
+    if (nth < 0 || row0 >= last) return false;
+    p->row0 = (int)row0;
+    p->row1 = (int)min(last, row0 + M);
+    p->k = key_tiles(p->rq, r >= R, p->row0 / G, (p->row1 - 1) / G, d.causal, d.window, d.sink, a.cap);
+    p->sel = nullptr;
+    p->count = 0;
+    if (d.top) {
+        KeyTiles& k = p->k;
+        p->sel = a.selected + (unit * d.kv_heads + kh) * d.top;
+        // entries up to the first that is none, and of those the ones that every token of the piece sees whole
+        const int lane = threadIdx.x & 63, whole = k.end_min / d.page_size;
+        int count = d.top, full = d.top;
+        for (int e0 = 0; e0 < d.top; e0 += 64) {
+            const int e = e0 + lane < d.top ? p->sel[e0 + lane] : -1;
+            const uint64_t none = __builtin_amdgcn_ballot_w64(e < 0), part = __builtin_amdgcn_ballot_w64(e < 0 || e >= whole);
+            if (part && full == d.top) full = min(full, e0 + __builtin_ctzll(part));
+            if (none) {
+                count = min(count, e0 + __builtin_ctzll(none));
+                break;
+            }
+        }
+        if (r >= R) count = full = 0;
+        const int64_t keys = (int64_t)count * d.page_size;
+        p->count = count;
+        k.beyond = false;
+        k.sinks = k.first = 0;
+        k.tiles = (int)((keys + 63) / 64);
+        k.fast0 = 0;
+        k.fast1 = (int)((int64_t)full * d.page_size / 64);
+    }
+    return true;
+}
+
+__device__ __forceinline__ BlockMap block_map(const PagedArgs& a, const Piece& p) {
+    const sfm_paged_desc& d = a.d;
+    BlockMap b;
+    b.table = a.table + (int64_t)(p.r < d.requests ? p.r : 0) * d.table_stride;
+    b.sel = p.sel;
+    b.blocks = p.k.tiles * 8;
+    b.count = p.count;
+    b.sinks8 = p.k.sinks * 8;
+    b.skip8 = (p.k.first - p.k.sinks) * 8;
+    b.end_max = p.k.end_max;
+    b.lo_min = p.k.lo_min;
+    b.sink = d.sink;
+    b.width = d.width;
+    b.pages = d.pages;
+    b.page8 = a.page8;
+    b.page_bytes = d.pool_stride[0] * 2;
+    b.block_bytes = d.pool_stride[1] * 16;
+    return b;
+}
+
+// Operands of the rows row0 .. + 31 (those past the piece repeat its last), and what each row sees
+template <class E, int D>
+__device__ __forceinline__ RowMask load_queries(const PagedArgs& a, const Piece& p, int row0, u32x4* qb) {
+    const sfm_paged_desc& d = a.d;
+    const int lane = threadIdx.x & 63, m = lane & 31, hf = lane >> 5, G = d.H / d.kv_heads;
+    const int row = min(row0 + m, p.row1 - 1), t = row / G;
+    const uint16_t* const q = (const uint16_t*)a.q + (int64_t)(p.rq.first + t) * d.q_stride[0] + (int64_t)(p.kh * G + row - t * G) * d.q_stride[1] + 8 * hf;
+#pragma unroll
+    for (int ds = 0; ds < D / 16; ++ds) qb[ds] = *(const u32x4*)(q + 16 * ds);
+#pragma unroll
+    for (int ds = 0; ds < D / 16; ++ds) asm volatile("" : "+v"(qb[ds]));      // loaded before any tile is awaited
+    RowMask k;
+    k.end = d.causal ? (int)min((int64_t)p.rq.past + t + 1, (int64_t)a.cap) : p.k.end_max;
+    k.lo = d.window && k.end > d.window ? k.end - d.window : 0;
+    k.sink = d.sink;
+    return k;
+}
+
+// ---- few rows: a wave takes tiles of its own --------------------------------------------------------------------------------
+//
+// Pieces of up to 32 rows, single tokens above all.  The four waves of a workgroup take its tiles in turn, each with a K and a V buffer that
+// no other wave sees and no barrier: while a wave works on K the V rows are on their way, and the next K's as soon as its last is
+// read.  Bound by reading the cache: of the matrix instructions' 32 columns a single token uses the query heads of its key head,
+// and they take an eighth of the time that the rows do.
+template <int D>
+struct FewLds {
+    static constexpr int kMat = DnLds<D>::kMat, kWave = 2 * kMat, kTotal = 4 * kWave;
+};
+
+template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+template <class E, int D>
+__global__ __launch_bounds__(256) void paged_few_kernel(PagedArgs a, int64_t npieces, int chunks, int chunk_tiles, float* part) {
+    using L = DnLds<D>;
+    constexpr int kLoads = L::kCPR, kRows = 64 / L::kCPR, kVar = D == 128 ? 4 : 2;     // loads of a tile, rows of a load, column orders
+    extern __shared__ __attribute__((aligned(256))) char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) char*)lds, buf = (uint32_t)wave * FewLds<D>::kWave;
+    const sfm_paged_desc& d = a.d;
+    const int total = (int)(npieces * d.kv_heads * chunks);
+    const int item = xcd_item(total);
+    if (item >= total) return;
+    const int kh = item % d.kv_heads, rest = item / d.kv_heads;        // the heads of a token's row side by side
+    const int chunk = rest % chunks;
+    Piece p;
+    if (!find_piece<32>(a, rest / chunks, kh, &p)) return;
+    const int v0 = min(chunk * chunk_tiles, p.k.tiles), v1 = min(v0 + chunk_tiles, p.k.tiles);
+    const BlockMap map = block_map(a, p);
+    u32x4 qb[D / 16];
+    const RowMask mask = load_queries<E, D>(a, p, p.row0, qb);
+    RowState<D> st;
+    st.init();
+    bool bad = p.k.beyond;
+    const float sc2 = d.sm_scale * kLog2e;
+
+    const int n = v0 + wave < v1 ? (v1 - v0 - wave + 3) / 4 : 0;       // this wave's tiles: v0 + wave + 4 i
+    uint32_t off_lo = 0, off_hi = 0;                                    // lane: block lane % 8 of tile i with i % 8 = lane / 8
+    int pos_of = kNoPos;
+    auto blocks = [&](int i0) {
+        const int i = i0 + (lane >> 3);
+        uint32_t off8;
+        const int e = map.entry(i < n ? 8 * (v0 + wave + 4 * i) + (lane & 7) : kNoPos, &off8, &pos_of);
+        const int page = map.page(e);
+        bad = bad || __builtin_amdgcn_ballot_w64(e >= 0 && page < 0) != 0;
+        const int64_t off = map.offset(page, off8);
+        off_lo = (uint32_t)off;
+        off_hi = (uint32_t)(off >> 32);
+    };
+    const char* const kg = (const char*)a.kp + (int64_t)kh * d.pool_stride[2] * 2;
+    const char* const vg = (const char*)a.vp + (int64_t)kh * d.pool_stride[2] * 2;
+    const uint32_t row_bytes = (uint32_t)d.pool_stride[1] * 2;
+    uint32_t voff[kVar];
+#pragma unroll
+    for (int x = 0; x < kVar; ++x) {
+        const int r = x * kRows + lane / L::kCPR;                      // swz repeats after 16 rows
+        voff[x] = (uint32_t)(lane / L::kCPR) * row_bytes + (uint32_t)(((lane % L::kCPR) ^ L::swz(r)) * 16);
+    }
+    auto stage = [&](const char* g, int i, uint32_t dst) {
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const int from = 8 * (i & 7) + j * kRows / 8;
+            const uint64_t off = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(off_hi, from) << 32 | (uint32_t)__builtin_amdgcn_readlane(off_lo, from);
+            dn_load_lds16(g + off + (uint32_t)(j * kRows % 8) * row_bytes, voff[j % kVar], lds0 + dst + (uint32_t)j * 1024);
+        }
+    };
+    if (n > 0) {
+        blocks(0);
+        stage(kg, 0, buf);
+        stage(vg, 0, buf + FewLds<D>::kMat);
+    }
+    for (int i = 0; i < n; ++i) {
+        int pos[8];
+#pragma unroll
+        for (int b = 0; b < 8; ++b) pos[b] = __builtin_amdgcn_readlane(pos_of, 8 * (i & 7) + b);
+        const bool next = i + 1 < n;
+        const int v = v0 + wave + 4 * i;
+        const bool masked = v < p.k.fast0 || v >= p.k.fast1;
+        wait_loads<kLoads>();                                          // K of this tile; V's are behind it
+        masked_tile<E, D>(lds, buf, buf + FewLds<D>::kMat, qb, sc2, st, mask, masked, pos,
+            [&]() {
+                lds_wave_sync();                                       // K is read
+                if (next) {
+                    if (((i + 1) & 7) == 0) blocks(i + 1);
+                    stage(kg, i + 1, buf);
+                }
+            },
+            [&]() {
+                if (next) wait_loads<kLoads>();
+                else wait_loads<0>();
+            });
+        lds_wave_sync();
+        if (next) stage(vg, i + 1, buf + FewLds<D>::kMat);
+    }
+    // the waves' rows joined: O, maximum and sum through LDS, 32 x D floats each
+    float* const wo = (float*)(lds + buf);                             // [D][32] by (channel, row): lanes of a row group apart
+    float* const ml = (float*)(lds + FewLds<D>::kTotal);               // [4 waves][3][32]
+    const int m = lane & 31, hf = lane >> 5;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) wo[(32 * dt + 8 * (v >> 2) + 4 * hf + (v & 3)) * 32 + m] = st.o[dt][v];
+    const float lsum = xhalf_sum(st.lrun);
+    const bool sees = __shfl_xor((int)st.seen, 32) || st.seen;
+    if (hf == 0) {
+        ml[wave * 96 + m] = st.mrun;
+        ml[wave * 96 + 32 + m] = lsum;
+        ml[wave * 96 + 64 + m] = bad ? 2.f : sees ? 1.f : 0.f;
+    }
+    __syncthreads();
+    // wave w takes rows in turn; a lane D / 64 channels
+    const int G = d.H / d.kv_heads;
+    for (int row = wave; row < p.row1 - p.row0; row += 4) {
+        float M = -__FLT_MAX__, sum = 0.f, o[D / 64];
+        bool rbad = false, rseen = false;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            M = fmaxf(M, ml[w * 96 + row]);
+            rbad = rbad || ml[w * 96 + 64 + row] == 2.f;
+            rseen = rseen || ml[w * 96 + 64 + row] == 1.f;
+        }
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) o[c] = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            if (ml[w * 96 + 64 + row] == 0.f) continue;
+            const float f = fast_exp2(ml[w * 96 + row] - M);
+            sum += f * ml[w * 96 + 32 + row];
+            const float* const x = (const float*)(lds + (uint32_t)w * FewLds<D>::kWave);
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) o[c] += f * x[(lane * (D / 64) + c) * 32 + row];
+        }
+        const int rr = p.row0 + row, t = p.rq.first + rr / G, h = kh * G + rr % G;
+        if (part != nullptr) {
+            const int64_t rows = d.tokens * d.H, at = chunk * rows + (int64_t)t * d.H + h;
+            if (rseen)
+#pragma unroll
+                for (int c = 0; c < D / 64; ++c) part[at * D + lane * (D / 64) + c] = o[c];
+            if (lane == 0) {
+                float* const q = part + chunks * rows * D + at * 2;
+                q[0] = M;
+                q[1] = rbad || (rseen && sum == 0.f) ? NAN : rseen ? sum : 0.f;
+            }
+        } else {
+            const float inv = rbad ? NAN : rseen ? 1.f / sum : 0.f;
+            uint16_t* const out = (uint16_t*)a.out + (int64_t)t * d.o_stride[0] + (int64_t)h * d.o_stride[1] + lane * (D / 64);
+            if constexpr (D == 128) *(uint32_t*)out = pack2<E>(o[0] * inv, o[1] * inv);
+            else *out = E::from_float(o[0] * inv);
+            if (a.lse != nullptr && lane == 0) a.lse[(int64_t)h * d.tokens + t] = rbad ? NAN : rseen ? (M + log2f(sum)) * kLn2 : -INFINITY;
+        }
+    }
+}
+
+// Combines the partials of a row: D / 4 lanes hold four channels each.  Bound by reading the partials once.
+template <class E, int D>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a, const float* __restrict__ part, int chunks) {
+    constexpr int CH = D / 4;
+    const sfm_paged_desc& d = a.d;
+    const int64_t rows = d.tokens * d.H, row = (int64_t)blockIdx.x * (256 / CH) + threadIdx.x / CH;
+    const int ch = threadIdx.x % CH;
+    if (row >= rows) return;
+    const int64_t t = row / d.H;
+    const int h = (int)(row - t * d.H);
+    if (!d.zero_rest && t >= clamp_int(a.q_start[d.requests], 0, (int)d.tokens)) return;       // rows of nobody
+    const float* const ml = part + chunks * rows * D + row * 2;
+    float M = -__FLT_MAX__, sum = 0.f;
+    for (int c = 0; c < chunks; ++c) M = ml[c * rows * 2 + 1] == 0.f ? M : fmaxf(M, ml[c * rows * 2]);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    bool seen = false;
+    for (int c = 0; c < chunks; ++c) {
+        const float l = ml[c * rows * 2 + 1];
+        if (l == 0.f) continue;
+        seen = true;
+        const float f = fast_exp2(ml[c * rows * 2] - M);
+        sum += f * l;
+        o += *(const f32x4*)(part + (c * rows + row) * D + 4 * ch) * f;
+    }
+    const float inv = seen ? 1.f / sum : 0.f;                          // NaN sums make the row NaN
+    *(u32x2*)((uint16_t*)a.out + t * d.o_stride[0] + h * d.o_stride[1] + 4 * ch) =
+        u32x2{pack2<E>(o.x * inv, o.y * inv), pack2<E>(o.z * inv, o.w * inv)};
+    if (a.lse != nullptr && ch == 0) a.lse[(int64_t)h * d.tokens + t] = seen ? (M + log2f(sum)) * kLn2 : -INFINITY;
+}
+
+// Which kernel a call takes, and in how many ranges of tiles.
+struct PagedPlan {
+    int rows;                      // of a piece; 0: the shape-generic kernel
+    int64_t pieces;
+    int chunks, chunk_tiles;
+};
+static PagedPlan paged_plan(const sfm_paged_desc& d) {
+    PagedPlan p{0, 0, 1, 0};
+    if (d.dtype == SFM_F32 || (d.D != 64 && d.D != 128)) return p;
+    const int G = d.H / d.kv_heads;
+    p.rows = 32;
+    p.pieces = d.top ? (pieces(d.tokens, d.group, d.requests)) * (((int64_t)d.group * G + p.rows - 1) / p.rows) : pieces(d.tokens * G, p.rows, d.requests);
+    const int64_t cap = (int64_t)d.width * d.page_size, keys = d.top ? std::min<int64_t>((int64_t)d.top * d.page_size, cap) : cap;
+    const int64_t tiles = (keys + 63) / 64;
+    const int64_t items = std::max<int64_t>(p.pieces - d.requests - 1, std::min<int64_t>(d.requests, p.pieces)) * d.kv_heads;
+    int64_t chunks = std::min<int64_t>((4 * cu_count() + items - 1) / items, (tiles + 7) / 8);
+    chunks = std::max<int64_t>(1, std::min<int64_t>(chunks, 64));
+    p.chunk_tiles = (int)((tiles + chunks - 1) / chunks);
+    p.chunks = (int)((tiles + p.chunk_tiles - 1) / p.chunk_tiles);
+    return p;
+}
+
+size_t paged_workspace_bytes(const sfm_paged_desc& d) {
+    const PagedPlan p = paged_plan(d);
+    return p.chunks < 2 ? 0 : (size_t)p.chunks * d.tokens * d.H * (d.D + 2) * sizeof(float);
+}
+
+static int launch_status() {
     const hipError_t err = hipGetLastError();
     if (err == hipSuccess) return SFM_OK;
     set_error("hip launch failed: %s", hipGetErrorString(err));
     return SFM_ERR_HIP;
+}
+
+template <class E, int D>
+static int launch_mfma(const PagedArgs& a, PagedPlan p, float* part, hipStream_t stream) {
+    const sfm_paged_desc& d = a.d;
+    const int64_t total = p.pieces * d.kv_heads * p.chunks;
+    if (total >= (1 << 23)) {
+        set_error("%lld pieces of rows, heads and ranges are more than a launch takes", (long long)total);
+        return SFM_ERR_UNSUPPORTED;
+    }
+    const size_t lds = FewLds<D>::kTotal + 4 * 96 * sizeof(float);
+    const hipError_t e = hipFuncSetAttribute((const void*)paged_few_kernel<E, D>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) {
+        set_error("hipFuncSetAttribute failed: %s", hipGetErrorString(e));
+        return SFM_ERR_HIP;
+    }
+    hipLaunchKernelGGL((paged_few_kernel<E, D>), dim3(xcd_grid((int)total)), dim3(256), lds, stream, a, p.pieces, p.chunks, p.chunk_tiles, part);
+    if (part != nullptr) {
+        const int64_t rows = d.tokens * d.H, per = 1024 / D;
+        hipLaunchKernelGGL((paged_merge_kernel<E, D>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, stream, a, (const float*)part, p.chunks);
+    }
+    return launch_status();
+}
+
+int launch_paged_attention(const sfm_paged_desc& d, const void* q, const void* kp, const void* vp, const int32_t* table,
+                           const int32_t* past, const int32_t* q_start, const int32_t* selected, void* out, float* lse, void* workspace,
+                           size_t workspace_bytes, hipStream_t stream) {
+    PagedArgs a{d, fast_div(d.page_size / 8), d.width * d.page_size, q, kp, vp, table, past, q_start, selected, out, lse};
+    PagedPlan p = paged_plan(d);
+    if (p.rows) {
+        if (p.chunks > 1 && (!workspace || workspace_bytes < paged_workspace_bytes(d))) {      // whole, then
+            p.chunk_tiles *= p.chunks;
+            p.chunks = 1;
+        }
+        float* const part = p.chunks > 1 ? (float*)workspace : nullptr;
+        if (d.dtype == SFM_BF16) return d.D == 128 ? launch_mfma<BF16, 128>(a, p, part, stream) : launch_mfma<BF16, 64>(a, p, part, stream);
+        return d.D == 128 ? launch_mfma<F16, 128>(a, p, part, stream) : launch_mfma<F16, 64>(a, p, part, stream);
+    }
+    if (d.tokens >= (1 << 24) || d.H > 65535) {
+        set_error("tokens=%lld, H=%d are more than a launch takes", (long long)d.tokens, d.H);
+        return SFM_ERR_UNSUPPORTED;
+    }
+    auto kern = d.dtype == SFM_BF16 ? paged_generic_kernel<BF16> : d.dtype == SFM_F16 ? paged_generic_kernel<F16> : paged_generic_kernel<float>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)d.tokens, d.H), dim3(256), 0, stream, a);
+    return launch_status();
 }
 
 }  // namespace sfm

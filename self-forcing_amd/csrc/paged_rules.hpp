@@ -74,6 +74,41 @@ __host__ __device__ __forceinline__ KeyTiles key_tiles(const Request& q, bool no
 }
 __host__ __device__ __forceinline__ int tile_of(const KeyTiles& k, int v) { return v < k.sinks ? v : v - k.sinks + k.first; }
 
+constexpr int kNoPos = 0x7ffffff8;                 // of a block that nobody sees
+
+// Eight positions that one tile and one page hold are a block.  What a lane needs of a piece to find its blocks
+struct BlockMap {
+    const int32_t* table;          // the request's row
+    const int32_t* sel;
+    int blocks, count, sinks8, skip8, end_max, lo_min, sink, width, pages;
+    FastDiv page8;
+    int64_t page_bytes, block_bytes;
+    // entry of the table and first position of virtual block vb; the entry is -1 where no token of the piece sees the block
+    __host__ __device__ __forceinline__ int entry(int vb, uint32_t* off8, int* pos) const {
+        *off8 = 0;
+        *pos = kNoPos;
+        if (vb >= blocks) return -1;
+        const uint32_t pb = sel ? (uint32_t)vb : (uint32_t)(vb < sinks8 ? vb : vb + skip8);
+        const uint32_t e = quot(pb, page8);
+        *off8 = pb - e * page8.d;
+        int en = (int)e;
+        if (sel) {
+            en = (int)e < count ? sel[e] : -1;
+            if (en < 0 || en >= width) return -1;
+        }
+        *pos = (int)(((uint32_t)en * page8.d + *off8) * 8);
+        if (*pos >= end_max || (*pos + 7 < lo_min && *pos >= sink)) return -1;
+        return en;
+    }
+    // the page of an entry, -1 where it is outside the pool
+    __host__ __device__ __forceinline__ int page(int e) const {
+        const int n = e >= 0 ? table[e] : -1;
+        return n >= 0 && n < pages ? n : -1;
+    }
+    // byte offset of the block in a head's rows of the pools; blocks that nobody sees lie in page 0
+    __host__ __device__ __forceinline__ int64_t offset(int page, uint32_t off8) const { return page < 0 ? 0 : page * page_bytes + off8 * block_bytes; }
+};
+
 #if defined(__HIPCC__)
 // The last r in [0, R] with at(r) <= v, R standing for the rows behind the last request: at ascends from at(0) <= v, and a wave looks
 // at 64 of its values at a time.  The same in every lane; some r in [0, R] where the values make no sense.

@@ -1904,8 +1904,8 @@ static int check_paged_q(const sfm_paged_desc* d) {
     int rc;
     if ((rc = check_paged_stride("q: token", d->q_stride[0], 0, esz))) return rc;
     if ((rc = check_paged_stride("q: head", d->q_stride[1], 0, esz))) return rc;
-    if (d->top < 0 || d->top > SFM_PAGED_TOP_MAX || (d->top && d->group < 1)) {
-        set_error("top=%d, group=%d: need 0 <= top <= %d, and groups of a token or more", d->top, d->group, SFM_PAGED_TOP_MAX);
+    if (d->top < 0 || d->top > SFM_PAGED_TOP_MAX || (d->top && d->group < 1) || (int64_t)d->top * d->page_size > 0x7fffffff) {
+        set_error("top=%d, group=%d: need 0 <= top <= %d, top * page_size < 2^31, and groups of a token or more", d->top, d->group, SFM_PAGED_TOP_MAX);
         return SFM_ERR_SHAPE;
     }
     return SFM_OK;

@@ -29,6 +29,21 @@ extern "C" int tile(int past, int n, int t0, int t1, int causal, int window, int
 """
 
 
+SOURCE += """
+extern "C" long long block(int past, int n, int t0, int t1, int causal, int window, int sink, int cap, const int* table, int width, int pages,
+                           int page_size, const int* sel, int count, long long page_bytes, long long row_bytes, int vb, int* pos, int* entry, int* page) {
+    sfm::KeyTiles k = sfm::key_tiles(sfm::Request{0, n, past}, false, t0, t1, causal, window, sink, cap);
+    if (sel) { k.sinks = k.first = 0; k.tiles = (int)(((long long)count * page_size + 63) / 64); }
+    sfm::BlockMap b{table, sel, k.tiles * 8, count, k.sinks * 8, (k.first - k.sinks) * 8, k.end_max, k.lo_min, sink, width, pages, sfm::fast_div(page_size / 8),
+                    page_bytes, 8 * row_bytes};
+    unsigned off8;
+    *entry = b.entry(vb, &off8, pos);
+    *page = b.page(*entry);
+    return b.offset(*page, off8);
+}
+"""
+
+
 @pytest.fixture(scope="module")
 def rules(tmp_path_factory):
     hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
@@ -41,6 +56,8 @@ def rules(tmp_path_factory):
     lib.quotient.restype = C.c_uint
     lib.piece.restype = lib.all_pieces.restype = C.c_longlong
     lib.piece.argtypes = [C.c_longlong] * 3 + [C.c_int]
+    lib.block.restype = C.c_longlong
+    lib.block.argtypes = [C.c_int] * 8 + [C.c_void_p] + [C.c_int] * 3 + [C.c_void_p, C.c_int] + [C.c_longlong] * 2 + [C.c_int] + [C.c_void_p] * 3
     lib.all_pieces.argtypes = [C.c_longlong] * 2 + [C.c_int]
     return lib
 
@@ -120,3 +137,51 @@ def test_tiles_hold_what_a_piece_sees_and_fast_ones_nothing_else(rules):
             assert end_min <= end <= end_max and lo_min <= lo <= lo_max
     rules.tiles(9, 5, 1, 0, 4, 1, 0, 0, 100, out)
     assert out[6] == 0                                     # rows of nobody
+
+
+@pytest.mark.parametrize("listed", [False, True])
+def test_blocks_lie_where_the_table_says_and_always_inside_the_pool(rules, listed):
+    rng = random.Random(5)
+    odd = [-1, -2 ** 31, 2 ** 31 - 1]
+    for _ in range(800):
+        page = 8 * rng.choice([1, 2, 3, 5, 8, 195])
+        past, n, causal = rng.randint(0, 900), rng.randint(1, 200), rng.randint(0, 1)
+        t0 = rng.randint(0, n - 1)
+        t1 = rng.randint(t0, n - 1)
+        window = 0 if listed else rng.choice([0, 1, 64, rng.randint(1, 700)])
+        sink = rng.randint(0, 300) if window else 0
+        need = -(-(past + n) // page)
+        width, pages = max(1, need + rng.choice([0, 1, -1])), rng.randint(1, 2 * need + 2)
+        table = [rng.choice([rng.randrange(pages), rng.randrange(pages), rng.randrange(pages), rng.choice(odd + [pages])]) for _ in range(width)]
+        cap = width * page
+        sel = sorted(rng.sample(range(need), rng.randint(0, need))) if listed else None
+        if listed and rng.random() < 0.3:
+            sel = [rng.choice([rng.randrange(need), rng.randint(0, 2 ** 31 - 1)]) for _ in range(rng.randint(1, 9))]
+        row_bytes = 16 * rng.randint(1, 40)
+        page_bytes = page * row_bytes + 16 * rng.randint(0, 3)
+        ctable, csel = (C.c_int * width)(*table), (C.c_int * max(1, len(sel or [])))(*(sel or [])) if listed else None
+        pos, entry, number = C.c_int(), C.c_int(), C.c_int()
+        out = (C.c_int * 10)()
+        rules.tiles(past, n, 0, t0, t1, causal, window, sink, cap, out)
+        some = {p for t in range(t0, t1 + 1) for p in visible(past, n, t, causal, window, sink, cap)}
+        blocks = 8 * (-(-len(sel) * page // 64) if listed else out[6])
+        met = set()
+        for vb in [*range(blocks + 3), 2 ** 31 - 8]:
+            off = rules.block(past, n, t0, t1, causal, window, sink, cap, ctable, width, pages, page, csel, len(sel or []), page_bytes, row_bytes, vb,
+                              C.byref(pos), C.byref(entry), C.byref(number))
+            assert 0 <= off <= (pages - 1) * page_bytes + (page - 8) * row_bytes      # eight rows from there are a page's
+            own = set(range(pos.value, pos.value + 8)) if pos.value < 2 ** 31 - 8 else set()
+            if entry.value >= 0:
+                assert own and pos.value % 8 == 0 and entry.value == pos.value // page
+                p = table[entry.value]
+                assert number.value == (p if 0 <= p < pages else -1)
+                if number.value >= 0:
+                    assert off == p * page_bytes + pos.value % page * row_bytes
+                assert listed or not own & met
+                met |= own & some
+            elif own:
+                assert not own & some                          # skipped: nobody sees it
+        if not listed:
+            assert met == some
+        elif sel == sorted(set(sel)) and (not sel or sel[-1] < need):
+            assert met == {p for p in some if p // page in sel}
