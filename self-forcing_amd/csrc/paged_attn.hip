@@ -408,9 +408,9 @@ __device__ __forceinline__ BlockMap block_map(const PagedArgs& a, const Piece& p
     return b;
 }
 
-// Operands of the rows row0 .. + 31 (those past the piece repeat its last), and what each row sees
+// Operands of the rows row0 .. + 31 (those past the piece repeat its last)
 template <class E, int D>
-__device__ __forceinline__ RowMask load_queries(const PagedArgs& a, const Piece& p, int row0, u32x4* qb) {
+__device__ __forceinline__ void load_queries(const PagedArgs& a, const Piece& p, int row0, u32x4* qb) {
     const sfm_paged_desc& d = a.d;
     const int lane = threadIdx.x & 63, m = lane & 31, hf = lane >> 5, G = d.H / d.kv_heads;
     const int row = min(row0 + m, p.row1 - 1), t = row / G;
@@ -419,8 +419,14 @@ __device__ __forceinline__ RowMask load_queries(const PagedArgs& a, const Piece&
     for (int ds = 0; ds < D / 16; ++ds) qb[ds] = *(const u32x4*)(q + 16 * ds);
 #pragma unroll
     for (int ds = 0; ds < D / 16; ++ds) asm volatile("" : "+v"(qb[ds]));      // loaded before any tile is awaited
+}
+
+// What each of them sees
+__device__ __forceinline__ RowMask row_mask(const PagedArgs& a, const Piece& p, int row0) {
+    const sfm_paged_desc& d = a.d;
+    const int row = min(row0 + (int)(threadIdx.x & 31), p.row1 - 1);
     RowMask k;
-    k.end = d.causal ? (int)min((int64_t)p.rq.past + t + 1, (int64_t)a.cap) : p.k.end_max;
+    k.end = d.causal ? (int)min((int64_t)p.rq.past + row / (d.H / d.kv_heads) + 1, (int64_t)a.cap) : p.k.end_max;
     k.lo = d.window && k.end > d.window ? k.end - d.window : 0;
     k.sink = d.sink;
     return k;
@@ -457,7 +463,8 @@ __global__ __launch_bounds__(256) void paged_few_kernel(PagedArgs a, int64_t npi
     const int v0 = min(chunk * chunk_tiles, p.k.tiles), v1 = min(v0 + chunk_tiles, p.k.tiles);
     const BlockMap map = block_map(a, p);
     u32x4 qb[D / 16];
-    const RowMask mask = load_queries<E, D>(a, p, p.row0, qb);
+    load_queries<E, D>(a, p, p.row0, qb);
+    const RowMask mask = row_mask(a, p, p.row0);
     RowState<D> st;
     st.init();
     bool bad = p.k.beyond;
@@ -580,6 +587,276 @@ __global__ __launch_bounds__(256) void paged_few_kernel(PagedArgs a, int64_t npi
     }
 }
 
+// ---- many rows: the waves of a workgroup share tiles -------------------------------------------------------------------------
+//
+// Pieces of 32 NW rows.  The tiles that all of them see whole run through the dense kernel's loop (two K and two V buffers, tiles
+// straight from memory into LDS, the logits of tile n + 1 beside the exponentials of tile n, its maximum beside P V of tile n); those that
+// some row sees in part (the request's own new tokens under a causal mask, a window's edge, the last tile) follow in a plain loop.
+// A wave takes the tile's loads with it one block each: the lane that knows the block's offset is read into scalar registers, which
+// the load adds to a fixed offset per lane.  Half of the lanes learn their next blocks every four tiles, three steps before the
+// first is needed, so that no load from the table is waited for.
+template <class E, int D, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_rows_kernel(PagedArgs a, int64_t npieces, int chunks, int chunk_tiles,
+                                                                                                          float* part) {
+    using L = DnLds<D, NW>;
+    constexpr int DS = D / 16, DT = D / 32, NTH = 64 * NW;
+    extern __shared__ __attribute__((aligned(256))) char lds[];
+    const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) char*)lds;
+    const int tid = threadIdx.x, lane = tid & 63, m = lane & 31, hf = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const sfm_paged_desc& d = a.d;
+    const int total = (int)(npieces * d.kv_heads * chunks);
+    const int item = xcd_item(total);
+    if (item >= total) return;
+    const int unit = item / (int)npieces, kh = unit / chunks, chunk = unit - kh * chunks;
+    const int at = item - unit * (int)npieces;
+    Piece p;
+    // the pieces of a head go to one XCD; under a causal mask those with the most keys first
+    if (!find_piece<32 * NW>(a, d.causal ? npieces - 1 - at : at, kh, &p)) return;
+    const int v0 = min(chunk * chunk_tiles, p.k.tiles), v1 = min(v0 + chunk_tiles, p.k.tiles);
+    const int f0 = max(v0, p.k.fast0), nf = max(min(v1, p.k.fast1) - f0, 0) & ~1;      // the loop over whole tiles takes two at a time
+    const BlockMap map = block_map(a, p);
+    bool bad = p.k.beyond;
+
+    // ---- where blocks lie: lane l holds block l % 8 of the tile whose number in its loop is l / 8 modulo 8
+    uint32_t off_lo = 0, off_hi = 0;
+    int pos_of = kNoPos;
+    auto place = [&](int e, int page, uint32_t off8) {
+        bad = bad || __builtin_amdgcn_ballot_w64(e >= 0 && page < 0) != 0;
+        const int64_t off = map.offset(page, off8);
+        off_lo = (uint32_t)off;
+        off_hi = (uint32_t)(off >> 32);
+    };
+    const char* const kg = (const char*)a.kp + (int64_t)kh * d.pool_stride[2] * 2;
+    const char* const vg = (const char*)a.vp + (int64_t)kh * d.pool_stride[2] * 2;
+    const uint32_t row_bytes = (uint32_t)d.pool_stride[1] * 2;
+    // a load moves 64 / kCPR rows of one block; a wave's loads of a tile are kRPC rows apart, a multiple of 16
+    constexpr int kCh = 64 * L::kCPR / NTH, kRPC = NTH / L::kCPR;
+    const int wrow = wave * 64 / L::kCPR, srow = wrow + lane / L::kCPR;
+    const uint32_t voff = (uint32_t)(lane / L::kCPR) * row_bytes + (uint32_t)(((lane % L::kCPR) ^ L::swz(srow)) * 16);
+    const uint32_t in_block = (uint32_t)(wrow % 8) * row_bytes;
+    auto stage = [&](const char* g, int i, uint32_t dst) {
+#pragma unroll
+        for (int j = 0; j < kCh; ++j) {
+            const int from = 8 * (i & 7) + j * (kRPC / 8) + wrow / 8;
+            const uint64_t off = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(off_hi, from) << 32 | (uint32_t)__builtin_amdgcn_readlane(off_lo, from);
+            dn_load_lds16(g + off + in_block, voff, lds0 + dst + (uint32_t)(j * NTH + wave * 64) * 16);
+        }
+    };
+
+    u32x4 qb[DS];
+    load_queries<E, D>(a, p, p.row0 + wave * 32, qb);
+    RowState<D> st;
+    st.init();
+    const float sc2 = d.sm_scale * kLog2e;
+
+    if (nf > 0) {
+        constexpr int NA = 2 * DS, NP = 4 * DT, kVA = 32 / NA, kVP = 32 / NP, kAhead = 3, kRing = kAhead + 1;
+        const uint32_t sA0 = (uint32_t)m * L::kPitch + (uint32_t)((hf ^ L::swz(m)) << 4);
+        uint32_t trA[2];
+        {
+            const int s16 = lane & 15, rl = 4 * hf + (s16 >> 2), cl = 2 * ((lane >> 4) & 1) + ((s16 & 3) >> 1);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int r = rl + 8 * half;
+                trA[half] = (uint32_t)r * L::kPitch + (uint32_t)((cl ^ L::swz(r)) << 4) + (uint32_t)(s16 & 1) * 8;
+            }
+        }
+        auto read_k = [&](uint32_t kbuf, int j) -> u32x4 {
+            return *(const u32x4*)(lds + (sA0 ^ (uint32_t)((j >> 1) << 5)) + kbuf + (j & 1) * 32 * L::kPitch);
+        };
+        auto read_v = [&](uint32_t vbuf, int j) -> u32x4 {
+            const u32x2 lo = dn_read_tr(lds + (trA[0] ^ (uint32_t)((j >> 2) << 6)), vbuf + (j & 3) * 16 * L::kPitch);
+            const u32x2 hi = dn_read_tr(lds + (trA[1] ^ (uint32_t)((j >> 2) << 6)), vbuf + (j & 3) * 16 * L::kPitch);
+            return u32x4{lo.x, lo.y, hi.x, hi.y};
+        };
+#define PG_SVAL(s, i) s[(i) >> 4][(i) & 15]
+        f32x16 sbuf[2][2];
+        u32x4 ring[kRing], pb[4];
+        float mrun = -__FLT_MAX__, lrun = 0.f;
+
+        // A lane's next block in three steps, the entry, its page and the place, in one register: the loops' others are taken.
+        int ahead;
+        auto block_of = [&](int i) { return i < nf ? 8 * (f0 + i) + (lane & 7) : kNoPos; };
+        {
+            uint32_t off8;
+            const int e = map.entry(block_of(lane >> 3), &off8, &pos_of);
+            place(e, map.page(e), off8);
+        }
+        // of tile n + 5 and the three behind it, which the lanes of their half hold from tile n + 2 on
+        auto next_blocks = [&](int n, int step) {
+            uint32_t off8;
+            int pos;
+            if (step == 0) {
+                ahead = map.entry(block_of(n + 5 + ((lane & 31) >> 3)), &off8, &pos);
+            } else if (step == 1) {
+                ahead = ahead < 0 ? -1 : map.page(ahead) < 0 ? -2 : map.page(ahead);
+            } else if ((lane >> 5) == (((n + 3) >> 2) & 1)) {
+                const int64_t off = map.offset(ahead, map.off8(block_of(n + 3 + ((lane & 31) >> 3))));
+                off_lo = (uint32_t)off;
+                off_hi = (uint32_t)(off >> 32);
+            }
+            if (step == 2) bad = bad || __builtin_amdgcn_ballot_w64(ahead == -2) != 0;
+        };
+
+        stage(kg, 0, L::kK);
+        stage(vg, 0, L::kV);
+        stage(kg, 1, L::kK + L::kMat);
+        dn_wait_tiles();
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) sbuf[0][t][v] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NA; ++j) sbuf[0][j & 1] = E::mfma32(read_k(L::kK, j), qb[j >> 1], sbuf[0][j & 1]);
+        {
+            float mx = sbuf[0][0][0];
+#pragma unroll
+            for (int i = 1; i < 32; ++i) mx = fmaxf(mx, PG_SVAL(sbuf[0], i));
+            mrun = fmaxf(xhalf_max(mx) * sc2, -__FLT_MAX__);
+        }
+
+        // tile n; kind 2: two more follow it at least, 1: one, 0: it is the last
+        auto iteration = [&](int n, auto par_c, auto kind_c) {
+            constexpr int PAR = decltype(par_c)::value, kind = decltype(kind_c)::value;
+            constexpr bool has_next = kind != 0;
+            constexpr uint32_t kbuf = L::kK + (uint32_t)(PAR ^ 1) * L::kMat;
+            constexpr uint32_t vbuf = L::kV + (uint32_t)PAR * L::kMat;
+            f32x16* scur = sbuf[PAR];
+            f32x16* snext = sbuf[PAR ^ 1];
+            dn_wait_tiles();
+            if (kind == 2) {
+                // what the last step asked the table for is here: used before new loads go out, so that nothing else is waited for
+                if (PAR == 1) {
+                    if ((n & 3) == 3) {
+                        next_blocks(n, 0);
+                    } else if (n > 1) {
+                        asm volatile("" : "+v"(ahead));
+                        next_blocks(n, 2);
+                    }
+                } else if ((n & 3) == 0 && n > 0) {
+                    asm volatile("" : "+v"(ahead));
+                    next_blocks(n, 1);
+                }
+                stage(kg, n + 2, L::kK + (uint32_t)PAR * L::kMat);
+            }
+            if (has_next) stage(vg, n + 1, L::kV + (uint32_t)(PAR ^ 1) * L::kMat);
+            float psum = 0.f;
+            if (has_next) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) snext[t][v] = 0.f;
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) ring[j % kRing] = read_k(kbuf, j);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) ring[(NA + j) % kRing] = read_v(vbuf, j);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < NA; ++j) {
+                if (has_next) {
+                    const int ja = j + kAhead;
+                    if (ja < NA) ring[ja % kRing] = read_k(kbuf, ja);
+                    else ring[ja % kRing] = read_v(vbuf, ja - NA);
+                    snext[j & 1] = E::mfma32(ring[j % kRing], qb[j >> 1], snext[j & 1]);
+                }
+#pragma unroll
+                for (int i = kVA * j; i < kVA * (j + 1); ++i) {
+                    const float e = fast_exp2(fmaf(PG_SVAL(scur, i), sc2, -mrun));
+                    psum += e;
+                    PG_SVAL(scur, i) = e;
+                }
+#pragma unroll
+                for (int i = kVA * j; i < kVA * (j + 1); i += 2) pb[i >> 3][(i >> 1) & 3] = pack2<E>(PG_SVAL(scur, i), PG_SVAL(scur, i + 1));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            lrun += psum;
+            float mx = has_next ? snext[0][0] : 0.f;
+#pragma unroll
+            for (int j = 0; j < NP; ++j) {
+                if (j + kAhead < NP) ring[(NA + j + kAhead) % kRing] = read_v(vbuf, j + kAhead);
+                st.o[j >> 2] = E::mfma32(ring[(NA + j) % kRing], pb[j & 3], st.o[j >> 2]);
+                if (has_next) {
+#pragma unroll
+                    for (int i = kVP * j; i < kVP * (j + 1); ++i) mx = fmaxf(mx, PG_SVAL(snext, i));
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (has_next) {
+                const float mnew = fmaxf(mrun, xhalf_max(mx) * sc2);
+                if (__builtin_amdgcn_ballot_w64(mnew > mrun) != 0) {
+                    const float alpha = fast_exp2(mrun - mnew);
+                    lrun *= alpha;
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) st.o[dt][v] *= alpha;
+                    mrun = mnew;
+                }
+            }
+        };
+        using c0 = std::integral_constant<int, 0>;
+        using c1 = std::integral_constant<int, 1>;
+        using c2 = std::integral_constant<int, 2>;
+        int n = 0;
+        for (; n + 2 < nf; n += 2) {
+            iteration(n, c0{}, c2{});
+            iteration(n + 1, c1{}, c2{});
+        }
+        iteration(n, c0{}, c1{});
+        iteration(n + 1, c1{}, c0{});
+#undef PG_SVAL
+        st.mrun = mrun;
+        st.lrun = lrun;
+        st.seen = true;
+        lds_barrier();                             // the buffers are everybody's again
+    }
+
+    // ---- tiles seen in part: virtual tiles before the whole ones and behind them
+    const int before = nf > 0 ? f0 - v0 : v1 - v0, rest = nf > 0 ? before + v1 - f0 - nf : before;
+    if (rest > 0) {
+        const int G = d.H / d.kv_heads, w0 = p.row0 + wave * 32, w1 = min(w0 + 31, p.row1 - 1);
+        const bool idle = w0 >= p.row1;
+        // what the wave's rows see at most and at least
+        const int e0 = idle || !d.causal ? p.k.end_max : (int)min((int64_t)p.rq.past + w0 / G + 1, (int64_t)a.cap);
+        const int e1 = idle || !d.causal ? p.k.end_max : (int)min((int64_t)p.rq.past + w1 / G + 1, (int64_t)a.cap);
+        const int lo = d.window && e1 > d.window ? e1 - d.window : 0;
+        auto blocks = [&](int u0) {
+            const int u = u0 + (lane >> 3), v = v0 + (u < before ? u : u + nf);
+            uint32_t off8;
+            const int e = map.entry(u < rest ? 8 * v + (lane & 7) : kNoPos, &off8, &pos_of);
+            place(e, map.page(e), off8);
+        };
+        const RowMask mask = row_mask(a, p, w0);
+        blocks(0);
+        stage(kg, 0, L::kK);
+        stage(vg, 0, L::kV);
+        for (int u = 0; u < rest; ++u) {
+            int pos[8];
+#pragma unroll
+            for (int b = 0; b < 8; ++b) pos[b] = __builtin_amdgcn_readlane(pos_of, 8 * (u & 7) + b);
+            const uint32_t buf = (uint32_t)(u & 1) * L::kMat, other = (uint32_t)(~u & 1) * L::kMat;
+            dn_wait_tiles();
+            if (u + 1 < rest) {
+                if (((u + 1) & 7) == 0) blocks(u + 1);
+                stage(kg, u + 1, L::kK + other);
+                stage(vg, u + 1, L::kV + other);
+            }
+            bool some = false, all = true;
+#pragma unroll
+            for (int b = 0; b < 8; ++b) {
+                some = some || pos[b] < e1;
+                all = all && pos[b] < e0 - 7 && (pos[b] >= lo || pos[b] + 7 < d.sink);
+            }
+            if (!idle && some) masked_tile<E, D>(lds, L::kK + buf, L::kV + buf, qb, sc2, st, mask, !all, pos, [] {}, [] {});
+        }
+    }
+    __syncthreads();                               // the tiles are dead: rows leave through LDS
+    store_rows<E, D>(a, p, st, bad, p.row0 + wave * 32, chunk, chunks, part, lds + wave * 32 * (2 * D + 16));
+}
+
 // Combines the partials of a row: D / 4 lanes hold four channels each.  Bound by reading the partials once.
 template <class E, int D>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a, const float* __restrict__ part, int chunks) {
@@ -619,13 +896,16 @@ struct PagedPlan {
 static PagedPlan paged_plan(const sfm_paged_desc& d) {
     PagedPlan p{0, 0, 1, 0};
     if (d.dtype == SFM_F32 || (d.D != 64 && d.D != 128)) return p;
-    const int G = d.H / d.kv_heads;
-    p.rows = 32;
-    p.pieces = d.top ? (pieces(d.tokens, d.group, d.requests)) * (((int64_t)d.group * G + p.rows - 1) / p.rows) : pieces(d.tokens * G, p.rows, d.requests);
-    const int64_t cap = (int64_t)d.width * d.page_size, keys = d.top ? std::min<int64_t>((int64_t)d.top * d.page_size, cap) : cap;
-    const int64_t tiles = (keys + 63) / 64;
+    const int64_t G = d.H / d.kv_heads;
+    // rows of a request (of a group of tokens) and key head, on average
+    const int64_t mean = std::max<int64_t>(1, d.top ? std::min<int64_t>(d.group, d.tokens) * G : d.tokens * G / d.requests);
+    p.rows = mean <= 32 ? 32 : mean <= 128 ? 128 : 256;
+    p.pieces = d.top ? pieces(d.tokens, d.group, d.requests) * ((d.group * G + p.rows - 1) / p.rows) : pieces(d.tokens * G, p.rows, d.requests);
+    const int64_t cap = (int64_t)d.width * d.page_size, tiles = ((d.top ? (int64_t)d.top * d.page_size : cap) + 63) / 64;
     const int64_t items = std::max<int64_t>(p.pieces - d.requests - 1, std::min<int64_t>(d.requests, p.pieces)) * d.kv_heads;
-    int64_t chunks = std::min<int64_t>((4 * cu_count() + items - 1) / items, (tiles + 7) / 8);
+    int64_t chunks = 1;
+    if (p.rows == 32) chunks = std::min<int64_t>((4 * cu_count() + items - 1) / items, (tiles + 7) / 8);
+    else if (items < cu_count()) chunks = std::min<int64_t>((2 * cu_count() + items - 1) / items, (tiles + 7) / 8);
     chunks = std::max<int64_t>(1, std::min<int64_t>(chunks, 64));
     p.chunk_tiles = (int)((tiles + chunks - 1) / chunks);
     p.chunks = (int)((tiles + p.chunk_tiles - 1) / p.chunk_tiles);
@@ -652,13 +932,18 @@ static int launch_mfma(const PagedArgs& a, PagedPlan p, float* part, hipStream_t
         set_error("%lld pieces of rows, heads and ranges are more than a launch takes", (long long)total);
         return SFM_ERR_UNSUPPORTED;
     }
-    const size_t lds = FewLds<D>::kTotal + 4 * 96 * sizeof(float);
-    const hipError_t e = hipFuncSetAttribute((const void*)paged_few_kernel<E, D>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) {
-        set_error("hipFuncSetAttribute failed: %s", hipGetErrorString(e));
-        return SFM_ERR_HIP;
-    }
-    hipLaunchKernelGGL((paged_few_kernel<E, D>), dim3(xcd_grid((int)total)), dim3(256), lds, stream, a, p.pieces, p.chunks, p.chunk_tiles, part);
+    auto go = [&](auto kern, int nw, size_t lds) -> int {
+        const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) {
+            set_error("hipFuncSetAttribute failed: %s", hipGetErrorString(e));
+            return SFM_ERR_HIP;
+        }
+        hipLaunchKernelGGL(kern, dim3(xcd_grid((int)total)), dim3(64 * nw), lds, stream, a, p.pieces, p.chunks, p.chunk_tiles, part);
+        return SFM_OK;
+    };
+    const int rc = p.rows == 32 ? go(paged_few_kernel<E, D>, 4, FewLds<D>::kTotal + 4 * 96 * sizeof(float))
+                   : p.rows == 128 ? go(paged_rows_kernel<E, D, 4>, 4, DnLds<D, 4>::kTotal) : go(paged_rows_kernel<E, D, 8>, 8, DnLds<D, 8>::kTotal);
+    if (rc) return rc;
     if (part != nullptr) {
         const int64_t rows = d.tokens * d.H, per = 1024 / D;
         hipLaunchKernelGGL((paged_merge_kernel<E, D>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, stream, a, (const float*)part, p.chunks);

@@ -100,6 +100,11 @@ struct BlockMap {
         if (*pos >= end_max || (*pos + 7 < lo_min && *pos >= sink)) return -1;
         return en;
     }
+    // block of its page
+    __host__ __device__ __forceinline__ uint32_t off8(int vb) const {
+        const uint32_t pb = sel || vb < sinks8 ? (uint32_t)vb : (uint32_t)vb + skip8;
+        return vb < blocks ? pb - quot(pb, page8) * page8.d : 0;
+    }
     // the page of an entry, -1 where it is outside the pool
     __host__ __device__ __forceinline__ int page(int e) const {
         const int n = e >= 0 ? table[e] : -1;
