@@ -592,9 +592,17 @@ __global__ __launch_bounds__(256) void paged_few_kernel(PagedArgs a, int64_t npi
 // Pieces of 32 NW rows.  The tiles that all of them see whole run through the dense kernel's loop (two K and two V buffers, tiles
 // straight from memory into LDS, the logits of tile n + 1 beside the exponentials of tile n, its maximum beside P V of tile n); those that
 // some row sees in part (the request's own new tokens under a causal mask, a window's edge, the last tile) follow in a plain loop.
-// A wave takes the tile's loads with it one block each: the lane that knows the block's offset is read into scalar registers, which
-// the load adds to a fixed offset per lane.  Half of the lanes learn their next blocks every four tiles, three steps before the
-// first is needed, so that no load from the table is waited for.
+// Where the whole tiles' blocks lie is worked out by all threads together and kept in LDS, 8 bytes a block, for a stretch of tiles at a
+// time (a request's page table row is read once per workgroup, not once per wave); a step reads one tile's eight offsets, a
+// step before it asks for that tile, and V's rows take the offsets that K's were read with.
+template <int D, int NW>
+struct RowsLds {
+    static constexpr int kPlaces = 4 * DnLds<D, NW>::kMat;                     // behind the tiles
+    static constexpr int kStretch = NW == 8 ? 512 : 240;                       // tiles; two workgroups of four waves share a compute unit's 160 KB
+    static constexpr int kLoop = kPlaces + (kStretch + 1) * 64, kStage = DnLds<D, NW>::kStage;
+    static constexpr int kTotal = kLoop > kStage ? kLoop : kStage;
+};
+
 template <class E, int D, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_rows_kernel(PagedArgs a, int64_t npieces, int chunks, int chunk_tiles,
                                                                                                           float* part) {
@@ -618,30 +626,30 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const BlockMap map = block_map(a, p);
     bool bad = p.k.beyond;
 
-    // ---- where blocks lie: lane l holds block l % 8 of the tile whose number in its loop is l / 8 modulo 8
-    uint32_t off_lo = 0, off_hi = 0;
-    int pos_of = kNoPos;
-    auto place = [&](int e, int page, uint32_t off8) {
-        bad = bad || __builtin_amdgcn_ballot_w64(e >= 0 && page < 0) != 0;
-        const int64_t off = map.offset(page, off8);
-        off_lo = (uint32_t)off;
-        off_hi = (uint32_t)(off >> 32);
-    };
-    const char* const kg = (const char*)a.kp + (int64_t)kh * d.pool_stride[2] * 2;
-    const char* const vg = (const char*)a.vp + (int64_t)kh * d.pool_stride[2] * 2;
     const uint32_t row_bytes = (uint32_t)d.pool_stride[1] * 2;
     // a load moves 64 / kCPR rows of one block; a wave's loads of a tile are kRPC rows apart, a multiple of 16
     constexpr int kCh = 64 * L::kCPR / NTH, kRPC = NTH / L::kCPR;
     const int wrow = wave * 64 / L::kCPR, srow = wrow + lane / L::kCPR;
     const uint32_t voff = (uint32_t)(lane / L::kCPR) * row_bytes + (uint32_t)(((lane % L::kCPR) ^ L::swz(srow)) * 16);
-    const uint32_t in_block = (uint32_t)(wrow % 8) * row_bytes;
-    auto stage = [&](const char* g, int i, uint32_t dst) {
+    const int64_t head = (int64_t)kh * d.pool_stride[2] * 2 + (uint32_t)(wrow % 8) * row_bytes;
+    const char* const kg = (const char*)a.kp + head;
+    const char* const vg = (const char*)a.vp + head;
+    // offsets of this wave's loads of a tile, from the lanes that hold its blocks from `from` on
+    struct Places {
+        uint64_t at[kCh];
+    };
+    auto places = [&](uint32_t lo, uint32_t hi, int from) {
+        Places x;
 #pragma unroll
         for (int j = 0; j < kCh; ++j) {
-            const int from = 8 * (i & 7) + j * (kRPC / 8) + wrow / 8;
-            const uint64_t off = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(off_hi, from) << 32 | (uint32_t)__builtin_amdgcn_readlane(off_lo, from);
-            dn_load_lds16(g + off + in_block, voff, lds0 + dst + (uint32_t)(j * NTH + wave * 64) * 16);
+            const int l = from + j * (kRPC / 8) + wrow / 8;
+            x.at[j] = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, l) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, l);
         }
+        return x;
+    };
+    auto stage = [&](const char* g, const Places& x, uint32_t dst) {
+#pragma unroll
+        for (int j = 0; j < kCh; ++j) dn_load_lds16(g + x.at[j], voff, lds0 + dst + (uint32_t)(j * NTH + wave * 64) * 16);
     };
 
     u32x4 qb[DS];
@@ -650,8 +658,20 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     st.init();
     const float sc2 = d.sm_scale * kLog2e;
 
-    if (nf > 0) {
+    for (int done = 0; done < nf; done += RowsLds<D, NW>::kStretch) {
         constexpr int NA = 2 * DS, NP = 4 * DT, kVA = 32 / NA, kVP = 32 / NP, kAhead = 3, kRing = kAhead + 1;
+        const int here = min(nf - done, RowsLds<D, NW>::kStretch);             // an even number of tiles
+        u32x2* const where = (u32x2*)(lds + RowsLds<D, NW>::kPlaces);
+        for (int b = tid; b < 8 * here; b += NTH) {
+            uint32_t off8;
+            int pos;
+            const int e = map.entry(8 * (f0 + done) + b, &off8, &pos), page = map.page(e);
+            bad = bad || (e >= 0 && page < 0);
+            const uint64_t off = (uint64_t)map.offset(page, off8);
+            where[b] = u32x2{(uint32_t)off, (uint32_t)(off >> 32)};
+        }
+        bad = __syncthreads_or(bad);
+        auto look = [&](int n) { return where[8 * n + (lane & 7)]; };
         const uint32_t sA0 = (uint32_t)m * L::kPitch + (uint32_t)((hf ^ L::swz(m)) << 4);
         uint32_t trA[2];
         {
@@ -673,35 +693,16 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #define PG_SVAL(s, i) s[(i) >> 4][(i) & 15]
         f32x16 sbuf[2][2];
         u32x4 ring[kRing], pb[4];
-        float mrun = -__FLT_MAX__, lrun = 0.f;
+        float lrun = st.lrun;
 
-        // A lane's next block in three steps, the entry, its page and the place, in one register: the loops' others are taken.
-        int ahead;
-        auto block_of = [&](int i) { return i < nf ? 8 * (f0 + i) + (lane & 7) : kNoPos; };
-        {
-            uint32_t off8;
-            const int e = map.entry(block_of(lane >> 3), &off8, &pos_of);
-            place(e, map.page(e), off8);
-        }
-        // of tile n + 5 and the three behind it, which the lanes of their half hold from tile n + 2 on
-        auto next_blocks = [&](int n, int step) {
-            uint32_t off8;
-            int pos;
-            if (step == 0) {
-                ahead = map.entry(block_of(n + 5 + ((lane & 31) >> 3)), &off8, &pos);
-            } else if (step == 1) {
-                ahead = ahead < 0 ? -1 : map.page(ahead) < 0 ? -2 : map.page(ahead);
-            } else if ((lane >> 5) == (((n + 3) >> 2) & 1)) {
-                const int64_t off = map.offset(ahead, map.off8(block_of(n + 3 + ((lane & 31) >> 3))));
-                off_lo = (uint32_t)off;
-                off_hi = (uint32_t)(off >> 32);
-            }
-            if (step == 2) bad = bad || __builtin_amdgcn_ballot_w64(ahead == -2) != 0;
-        };
-
-        stage(kg, 0, L::kK);
-        stage(vg, 0, L::kV);
-        stage(kg, 1, L::kK + L::kMat);
+        u32x2 next = look(0);
+        Places x = places(next.x, next.y, 0);
+        stage(kg, x, L::kK);
+        stage(vg, x, L::kV);
+        next = look(1);
+        x = places(next.x, next.y, 0);                     // of tile n + 1 when tile n begins
+        stage(kg, x, L::kK + L::kMat);
+        next = look(min(2, here - 1));                     // of tile n + 2
         dn_wait_tiles();
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -713,10 +714,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
             float mx = sbuf[0][0][0];
 #pragma unroll
             for (int i = 1; i < 32; ++i) mx = fmaxf(mx, PG_SVAL(sbuf[0], i));
-            mrun = fmaxf(xhalf_max(mx) * sc2, -__FLT_MAX__);
+            st.lrun = lrun;
+            st.raise(fmaxf(st.mrun, xhalf_max(mx) * sc2));
+            lrun = st.lrun;
         }
+        float mrun = st.mrun;
 
-        // tile n; kind 2: two more follow it at least, 1: one, 0: it is the last
+        // tile n of the stretch; kind 2: two more follow it at least, 1: one, 0: it is the last
         auto iteration = [&](int n, auto par_c, auto kind_c) {
             constexpr int PAR = decltype(par_c)::value, kind = decltype(kind_c)::value;
             constexpr bool has_next = kind != 0;
@@ -725,22 +729,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
             f32x16* scur = sbuf[PAR];
             f32x16* snext = sbuf[PAR ^ 1];
             dn_wait_tiles();
+            if (has_next) stage(vg, x, L::kV + (uint32_t)(PAR ^ 1) * L::kMat);
             if (kind == 2) {
-                // what the last step asked the table for is here: used before new loads go out, so that nothing else is waited for
-                if (PAR == 1) {
-                    if ((n & 3) == 3) {
-                        next_blocks(n, 0);
-                    } else if (n > 1) {
-                        asm volatile("" : "+v"(ahead));
-                        next_blocks(n, 2);
-                    }
-                } else if ((n & 3) == 0 && n > 0) {
-                    asm volatile("" : "+v"(ahead));
-                    next_blocks(n, 1);
-                }
-                stage(kg, n + 2, L::kK + (uint32_t)PAR * L::kMat);
+                x = places(next.x, next.y, 0);
+                stage(kg, x, L::kK + (uint32_t)PAR * L::kMat);
+                next = look(n + 3);                        // of the last step: a place behind the stretch's, not used
             }
-            if (has_next) stage(vg, n + 1, L::kV + (uint32_t)(PAR ^ 1) * L::kMat);
             float psum = 0.f;
             if (has_next) {
 #pragma unroll
@@ -801,7 +795,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         using c1 = std::integral_constant<int, 1>;
         using c2 = std::integral_constant<int, 2>;
         int n = 0;
-        for (; n + 2 < nf; n += 2) {
+        for (; n + 2 < here; n += 2) {
             iteration(n, c0{}, c2{});
             iteration(n + 1, c1{}, c2{});
         }
@@ -823,16 +817,22 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         const int e0 = idle || !d.causal ? p.k.end_max : (int)min((int64_t)p.rq.past + w0 / G + 1, (int64_t)a.cap);
         const int e1 = idle || !d.causal ? p.k.end_max : (int)min((int64_t)p.rq.past + w1 / G + 1, (int64_t)a.cap);
         const int lo = d.window && e1 > d.window ? e1 - d.window : 0;
+        // lane l: block l % 8 of tile u with u % 8 = l / 8
+        uint32_t off_lo = 0, off_hi = 0;
+        int pos_of = kNoPos;
         auto blocks = [&](int u0) {
             const int u = u0 + (lane >> 3), v = v0 + (u < before ? u : u + nf);
             uint32_t off8;
-            const int e = map.entry(u < rest ? 8 * v + (lane & 7) : kNoPos, &off8, &pos_of);
-            place(e, map.page(e), off8);
+            const int e = map.entry(u < rest ? 8 * v + (lane & 7) : kNoPos, &off8, &pos_of), page = map.page(e);
+            bad = bad || __builtin_amdgcn_ballot_w64(e >= 0 && page < 0) != 0;
+            const uint64_t off = (uint64_t)map.offset(page, off8);
+            off_lo = (uint32_t)off;
+            off_hi = (uint32_t)(off >> 32);
         };
         const RowMask mask = row_mask(a, p, w0);
         blocks(0);
-        stage(kg, 0, L::kK);
-        stage(vg, 0, L::kV);
+        stage(kg, places(off_lo, off_hi, 0), L::kK);
+        stage(vg, places(off_lo, off_hi, 0), L::kV);
         for (int u = 0; u < rest; ++u) {
             int pos[8];
 #pragma unroll
@@ -841,8 +841,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
             dn_wait_tiles();
             if (u + 1 < rest) {
                 if (((u + 1) & 7) == 0) blocks(u + 1);
-                stage(kg, u + 1, L::kK + other);
-                stage(vg, u + 1, L::kV + other);
+                const Places x = places(off_lo, off_hi, 8 * ((u + 1) & 7));
+                stage(kg, x, L::kK + other);
+                stage(vg, x, L::kV + other);
             }
             bool some = false, all = true;
 #pragma unroll
@@ -896,16 +897,32 @@ struct PagedPlan {
 static PagedPlan paged_plan(const sfm_paged_desc& d) {
     PagedPlan p{0, 0, 1, 0};
     if (d.dtype == SFM_F32 || (d.D != 64 && d.D != 128)) return p;
-    const int64_t G = d.H / d.kv_heads;
-    // rows of a request (of a group of tokens) and key head, on average
+    const int64_t G = d.H / d.kv_heads, cu = cu_count();
+    // rows of a request (of a group of tokens) and key head, on average, and pieces that have rows
     const int64_t mean = std::max<int64_t>(1, d.top ? std::min<int64_t>(d.group, d.tokens) * G : d.tokens * G / d.requests);
-    p.rows = mean <= 32 ? 32 : mean <= 128 ? 128 : 256;
+    const int64_t units = d.top ? (d.tokens + d.group - 1) / d.group : std::min<int64_t>(d.requests, d.tokens);
+    auto items = [&](int64_t rows) { return units * ((mean + rows - 1) / rows) * d.kv_heads; };
+    p.rows = mean <= 32 ? 32 : mean <= 128 || items(256) < cu / 2 ? 128 : 256;
     p.pieces = d.top ? pieces(d.tokens, d.group, d.requests) * ((d.group * G + p.rows - 1) / p.rows) : pieces(d.tokens * G, p.rows, d.requests);
-    const int64_t cap = (int64_t)d.width * d.page_size, tiles = ((d.top ? (int64_t)d.top * d.page_size : cap) + 63) / 64;
-    const int64_t items = std::max<int64_t>(p.pieces - d.requests - 1, std::min<int64_t>(d.requests, p.pieces)) * d.kv_heads;
+    const int64_t cap = (int64_t)d.width * d.page_size, tiles = ((d.top ? (int64_t)d.top * d.page_size : cap) + 63) / 64, n = items(p.rows);
     int64_t chunks = 1;
-    if (p.rows == 32) chunks = std::min<int64_t>((4 * cu_count() + items - 1) / items, (tiles + 7) / 8);
-    else if (items < cu_count()) chunks = std::min<int64_t>((2 * cu_count() + items - 1) / items, (tiles + 7) / 8);
+    if (p.rows == 32) {
+        chunks = std::min<int64_t>((4 * cu + n - 1) / n, (tiles + 7) / 8);
+    } else if (tiles >= 16) {
+        const bool wide = p.rows == 256;
+        const double scale = d.D == 64 ? 0.6 : 1.0, partial_ns = (double)d.H * d.tokens * (d.D + 2) * 8 / 3500;
+        double t1 = 0, best = 0;
+        for (int64_t s = 1; s <= 64 && s <= tiles / 4 && (s == 1 || n * s <= cu * (wide ? 1 : 2)); ++s) {
+            const double tile_ns = wide ? (n * s <= cu / 2 ? 1460 : 1830) : (n * s <= cu ? 1100 : 1900);
+            double t = 5000 + (double)((tiles + s - 1) / s) * tile_ns * scale;
+            if (s == 1) t1 = best = t;
+            else t += 6000 + s * partial_ns;
+            if (t < best && t < 0.9 * t1) {
+                chunks = s;
+                best = t;
+            }
+        }
+    }
     chunks = std::max<int64_t>(1, std::min<int64_t>(chunks, 64));
     p.chunk_tiles = (int)((tiles + chunks - 1) / chunks);
     p.chunks = (int)((tiles + p.chunk_tiles - 1) / p.chunk_tiles);
@@ -942,7 +959,7 @@ static int launch_mfma(const PagedArgs& a, PagedPlan p, float* part, hipStream_t
         return SFM_OK;
     };
     const int rc = p.rows == 32 ? go(paged_few_kernel<E, D>, 4, FewLds<D>::kTotal + 4 * 96 * sizeof(float))
-                   : p.rows == 128 ? go(paged_rows_kernel<E, D, 4>, 4, DnLds<D, 4>::kTotal) : go(paged_rows_kernel<E, D, 8>, 8, DnLds<D, 8>::kTotal);
+                   : p.rows == 128 ? go(paged_rows_kernel<E, D, 4>, 4, RowsLds<D, 4>::kTotal) : go(paged_rows_kernel<E, D, 8>, 8, RowsLds<D, 8>::kTotal);
     if (rc) return rc;
     if (part != nullptr) {
         const int64_t rows = d.tokens * d.H, per = 1024 / D;
