@@ -288,9 +288,19 @@ int launch_paged_write(const sfm_paged_desc& d, const void* k, const void* v, co
 // ------------------------------------------------------------------------------------------------
 // select
 // ------------------------------------------------------------------------------------------------
+// Two steps: scores of every candidate page into a workspace, then the best of a row.  Few rows (single tokens) are spread over the chip by
+// their pages in the first, where the means' bytes are, and the second works from LDS.  Scores are sums of 64 bits: two programs that
+// add in another order still agree on which page is ahead, as long as no two scores are level to 15 digits.
 struct SelectArgs {
     sfm_paged_desc d;
+    const void* q;
+    const float* means;
+    const int32_t *table, *past, *q_start;
+    int32_t* selected;
+    uint64_t* keys;                // [row - row0][kv head][width]: scores as integers in their order
     int first, last;
+    int row0, rows;                // of this pass
+    int chunk;                     // pages that a workgroup scores
 };
 
 // A score's bits in the order of the scores: NaN counts as -inf, -0 as 0.
@@ -300,96 +310,154 @@ __device__ __forceinline__ uint64_t select_key(double s) {
     return b >> 63 ? ~b : b | ((uint64_t)1 << 63);
 }
 
-constexpr int kSelPages = 2048;                    // scores that are compared at a time, beside the best so far
+// The tokens of row `row` of the lists and the pages that they choose from; n = 0: nobody's.
+struct SelectRow {
+    int r, n, candidates;          // entries of the table's row that the last token sees
+    int64_t t0, pages;             // first token; candidates, had the table room for them
+};
+__device__ __forceinline__ SelectRow select_row(const SelectArgs& s, int row) {
+    const sfm_paged_desc& d = s.d;
+    SelectRow x;
+    x.r = find_last(d.requests, row, [&](int i) { return first_piece(clamp_int(s.q_start[i], 0, (int)d.tokens), 1, d.group, i); });
+    const Request rq = request_of(s.q_start, s.past, x.r, d.requests, (int)d.tokens);
+    const int64_t t0 = (row - first_piece(rq.first, 1, d.group, x.r)) * d.group;
+    x.n = x.r < d.requests && t0 >= 0 && t0 < rq.n ? (int)min((int64_t)d.group, rq.n - t0) : 0;
+    x.t0 = rq.first + t0;
+    x.pages = ((int64_t)rq.past + (d.causal ? t0 + x.n : rq.n) + d.page_size - 1) / d.page_size;
+    x.candidates = x.n ? (int)min(x.pages, (int64_t)d.width) : 0;
+    return x;
+}
 
-// A workgroup takes one group of tokens and one key head: the sum of its queries in LDS, a page's score from 16 lanes, kSelPages
-// pages at a time.  The best of them and of the `top` before are found by the scores' bits, eight at a time from the highest: a
-// histogram says in which digit the top-th score lies; level ones are taken in the order of their pages, which is kept throughout.
-// Sums are of 64 bits: two programs that add in another order still agree on which page is ahead.
-template <typename E>
-__global__ __launch_bounds__(256) void paged_select_kernel(SelectArgs s, const void* q, const float* means, const int32_t* table,
-                                                           const int32_t* past, const int32_t* q_start, int32_t* selected) {
+// Scores of `chunk` pages for RT rows of one key head.  Sixteen lanes share a page, 4 of each 64 channels a lane; their queries' sums
+// stay in registers, so that rows of one request (many groups of a prompt) read a mean once.  Bound by the means' bytes for single
+// tokens.
+template <typename E, int NI, int RT>
+__global__ __launch_bounds__(256) void paged_score_kernel(SelectArgs s) {
     constexpr int N = Chunk<E>::kN;
+    __shared__ double part[256 * N];
+    __shared__ double qsum[RT][256];
+    const sfm_paged_desc& d = s.d;
+    const int tid = threadIdx.x, sub = tid & 15;
+    const int kh = blockIdx.y, tile = s.row0 + blockIdx.x * RT, end = min(tile + RT, s.row0 + s.rows), c0 = blockIdx.z * s.chunk;
+    const int G = d.H / d.kv_heads, chunks = d.D / N, groups = 256 / chunks, g = tid / chunks, c = tid - g * chunks;
+    for (int row = tile; row < end;) {
+        const SelectRow x = select_row(s, row);
+        int count = 1;             // rows of the same request from here on
+        SelectRow last = x;
+        int most = x.candidates > d.top ? x.candidates : 0;
+        while (RT > 1 && row + count < end) {
+            const SelectRow y = select_row(s, row + count);
+            if (y.r != x.r || !y.n) break;
+            last = y;
+            most = max(most, y.candidates > d.top ? y.candidates : 0);
+            ++count;
+        }
+        if (c0 < most) {
+            // sums of the queries: chunk c of the rows g, g + groups, ...
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                const int64_t t0 = x.t0 + (int64_t)i * d.group;
+                const int rows = i < count ? (int)(i == count - 1 ? last.n : d.group) * G : 0;
+                double sum[N];
+                float v[N];
+#pragma unroll
+                for (int k = 0; k < N; ++k) sum[k] = 0.0;
+                if (g < groups)
+                    for (int j = g; j < rows; j += groups) {
+                        const int t = j / G, h = j - t * G;
+                        Chunk<E>::get(((const u32x4*)s.q)[((t0 + t) * d.q_stride[0] + (int64_t)(kh * G + h) * d.q_stride[1]) / N + c], v);
+#pragma unroll
+                        for (int k = 0; k < N; ++k) sum[k] += (double)v[k];
+                    }
+                __syncthreads();
+                if (g < groups)
+#pragma unroll
+                    for (int k = 0; k < N; ++k) part[g * d.D + c * N + k] = sum[k];
+                __syncthreads();
+                if (tid < d.D) {
+                    double t = 0.0;
+                    for (int j = 0; j < min(groups, rows); ++j) t += part[j * d.D + tid];
+                    qsum[i][tid] = t;
+                }
+            }
+            __syncthreads();
+            double q[RT][NI * 4];
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int k = 0; k < NI * 4; ++k) {
+                    const int ch = 64 * (k >> 2) + 4 * sub + (k & 3);
+                    q[i][k] = ch < d.D ? qsum[i][ch] : 0.0;
+                }
+            uint64_t* const keys = s.keys + ((int64_t)(row - s.row0) * d.kv_heads + kh) * d.width;
+            const int32_t* const table = s.table + x.r * d.table_stride;
+            const int c1 = min(c0 + s.chunk, most);
+            constexpr int U = 4;                                       // pages on their way at a time
+            for (int e0 = c0 + (tid >> 4); e0 < c1; e0 += 16 * U) {
+                int page[U];
+                f32x4 w[U][NI];
+#pragma unroll
+                for (int u = 0; u < U; ++u) page[u] = e0 + 16 * u < c1 ? table[e0 + 16 * u] : -1;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const bool fine = page[u] >= 0 && page[u] < d.pages;
+                    const float* const m = s.means + ((int64_t)(fine ? page[u] : 0) * d.kv_heads + kh) * d.D;
+#pragma unroll
+                    for (int i = 0; i < NI; ++i) w[u][i] = 64 * i + 4 * sub < d.D ? *(const f32x4*)(m + 64 * i + 4 * sub) : f32x4{0.f, 0.f, 0.f, 0.f};
+                    if (!fine) page[u] = -1;
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int e = e0 + 16 * u;
+#pragma unroll
+                    for (int i = 0; i < RT; ++i) {
+                        double dot = 0.0;
+#pragma unroll
+                        for (int k = 0; k < NI * 4; ++k) dot = fma(q[i][k], (double)w[u][k >> 2][k & 3], dot);
+#pragma unroll
+                        for (int o = 8; o > 0; o >>= 1) dot += __shfl_xor(dot, o);
+                        if (page[u] < 0) dot = -INFINITY;
+                        if (sub == 0 && i < count && e < c1) keys[(int64_t)i * d.kv_heads * d.width + e] = select_key(dot);
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        row += count;
+    }
+}
+
+constexpr int kSelPages = 4096;                    // scores that are compared at a time, beside the best so far
+
+// The best of a row.  Scores are taken kSelPages at a time; the best of them and of the `top` before are found by the keys' bits, eight at
+// a time from the highest: a histogram says in which digit the top-th largest lies.  Level ones are taken in the order of their
+// pages, which is kept throughout.
+__global__ __launch_bounds__(256) void paged_select_kernel(SelectArgs s) {
     extern __shared__ __attribute__((aligned(16))) char sel_lds[];
     const sfm_paged_desc& d = s.d;
     const int cap = d.top + kSelPages;
-    double* const qsum = (double*)sel_lds;                         // [D]
-    uint64_t* const key = (uint64_t*)(qsum + 256);                 // [cap]
+    uint64_t* const key = (uint64_t*)sel_lds;                      // [cap]
     int32_t* const entry = (int32_t*)(key + cap);                  // [cap]
     __shared__ int hist[256];
     __shared__ int wsum[4][2];
     __shared__ int pick[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int row = blockIdx.x / d.kv_heads, kh = blockIdx.x - row * d.kv_heads;
-    int32_t* const out = selected + ((int64_t)row * d.kv_heads + kh) * d.top;
-    const int r = find_last(d.requests, row, [&](int i) { return first_piece(clamp_int(q_start[i], 0, (int)d.tokens), 1, d.group, i); });
-    const Request rq = request_of(q_start, past, r, d.requests, (int)d.tokens);
-    const int64_t t0 = (row - first_piece(rq.first, 1, d.group, r)) * d.group;
-    if (r >= d.requests || t0 < 0 || t0 >= rq.n) {
-        for (int i = tid; i < d.top; i += 256) out[i] = -1;
-        return;
-    }
-    const int n = (int)min((int64_t)d.group, rq.n - t0);
-    const int64_t end = (int64_t)rq.past + (d.causal ? t0 + n : rq.n);
-    const int64_t pages = (end + d.page_size - 1) / d.page_size;
-    const int P = (int)min(pages, (int64_t)d.width);               // entries that the table has
+    const int row = s.row0 + blockIdx.x / d.kv_heads, kh = blockIdx.x % d.kv_heads;
+    int32_t* const out = s.selected + ((int64_t)row * d.kv_heads + kh) * d.top;
+    const SelectRow x = select_row(s, row);
+    const int P = x.candidates;
     if (P <= d.top) {
         for (int i = tid; i < d.top; i += 256) out[i] = i < P ? i : -1;
         return;
     }
-    // sum of the queries: chunk c of the rows g, g + groups, ...
-    {
-        const int G = d.H / d.kv_heads, chunks = d.D / N, groups = 256 / chunks, g = tid / chunks, c = tid - g * chunks;
-        const int rows = n * G;
-        double sum[N];
-        float x[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) sum[i] = 0.0;
-        const u32x4* const q16 = (const u32x4*)q;
-        if (g < groups)
-            for (int j = g; j < rows; j += groups) {
-                const int t = j / G, h = j - t * G;
-                Chunk<E>::get(q16[((rq.first + t0 + t) * d.q_stride[0] + (int64_t)(kh * G + h) * d.q_stride[1]) / N + c], x);
-#pragma unroll
-                for (int i = 0; i < N; ++i) sum[i] += (double)x[i];
-            }
-        double* const part = (double*)key;                         // [groups][D]: at most 256 * N doubles, which the keys have room for
-        if (g < groups)
-#pragma unroll
-            for (int i = 0; i < N; ++i) part[g * d.D + c * N + i] = sum[i];
-        __syncthreads();
-        if (tid < d.D) {
-            double t = 0.0;
-            for (int j = 0; j < groups; ++j) t += part[j * d.D + tid];
-            qsum[tid] = t;
-        }
-        __syncthreads();
-    }
+    const uint64_t* const keys = s.keys + ((int64_t)(row - s.row0) * d.kv_heads + kh) * d.width;
     int kept = 0;                                                  // key[0 .. kept): the best so far, in the order of their entries
-    const int sub = tid & 15;
     for (int p0 = 0; p0 < P; p0 += kSelPages) {
         const int count = min(kSelPages, P - p0);
-        for (int i = tid >> 4; i < count; i += 16) {
+        for (int i = tid; i < count; i += 256) {
             const int e = p0 + i;
-            const int page = table[r * d.table_stride + e];
-            double dot = 0.0;
-            if (page >= 0 && page < d.pages) {
-                const float* const m = means + ((int64_t)page * d.kv_heads + kh) * d.D;
-                for (int x = 4 * sub; x < d.D; x += 64) {
-                    const f32x4 w = *(const f32x4*)(m + x);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) dot = fma(qsum[x + k], (double)w[k], dot);
-                }
-            } else {
-                dot = -INFINITY;
-            }
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) dot += __shfl_xor(dot, o);
-            if (e < s.first || e >= pages - s.last) dot = INFINITY;
-            if (sub == 0) {
-                key[kept + i] = select_key(dot);
-                entry[kept + i] = e;
-            }
+            key[kept + i] = e < s.first || e >= x.pages - s.last ? ~(uint64_t)0 : keys[e];      // above infinity's
+            entry[kept + i] = e;
         }
         __syncthreads();
         const int have = kept + count;
@@ -477,24 +545,49 @@ __global__ __launch_bounds__(256) void paged_select_kernel(SelectArgs s, const v
     for (int i = tid; i < d.top; i += 256) out[i] = entry[i];
 }
 
-size_t paged_select_workspace_bytes(const sfm_paged_desc&) { return 0; }
+// Rows of a pass: their scores take this many bytes at most (a row's always).
+constexpr size_t kSelWorkspace = 256u << 20;
+static int select_pass(const sfm_paged_desc& d) {
+    const size_t row = (size_t)d.kv_heads * d.width * sizeof(uint64_t);
+    const int64_t rows = pieces(d.tokens, d.group, d.requests);
+    return (int)std::max<int64_t>(1, std::min<int64_t>({rows, (int64_t)(kSelWorkspace / row), 65535}));
+}
+size_t paged_select_workspace_bytes(const sfm_paged_desc& d) { return (size_t)select_pass(d) * d.kv_heads * d.width * sizeof(uint64_t); }
+
+template <typename E, int RT>
+static auto score_kernel(int ni) {
+    return ni == 1 ? paged_score_kernel<E, 1, RT> : ni == 2 ? paged_score_kernel<E, 2, RT> : ni == 3 ? paged_score_kernel<E, 3, RT> : paged_score_kernel<E, 4, RT>;
+}
 
 int launch_paged_select(const sfm_paged_desc& d, const void* q, const float* means, const int32_t* table, const int32_t* past,
-                        const int32_t* q_start, int first, int last, int32_t* selected, void*, hipStream_t stream) {
-    SelectArgs s{d, first, last};
-    const int64_t wgs = pieces(d.tokens, d.group, d.requests) * d.kv_heads;
-    if (wgs >= (1 << 24)) {
-        set_error("%lld groups of tokens and heads are more than a launch takes", (long long)wgs);
+                        const int32_t* q_start, int first, int last, int32_t* selected, void* workspace, hipStream_t stream) {
+    const int64_t rows = pieces(d.tokens, d.group, d.requests);
+    if (d.kv_heads > 65535 || (int64_t)select_pass(d) * d.kv_heads >= (1 << 24) || rows / select_pass(d) > 4096) {
+        set_error("%lld groups of tokens with %d key heads are more than a call takes", (long long)rows, d.kv_heads);
         return SFM_ERR_UNSUPPORTED;
     }
-    const size_t lds = 256 * sizeof(double) + (size_t)(d.top + kSelPages) * 12;
-    auto kern = d.dtype == SFM_BF16 ? paged_select_kernel<BF16> : d.dtype == SFM_F16 ? paged_select_kernel<F16> : paged_select_kernel<float>;
-    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    const size_t lds = (size_t)(d.top + kSelPages) * 12;
+    const hipError_t e = hipFuncSetAttribute((const void*)paged_select_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) {
         set_error("hipFuncSetAttribute failed: %s", hipGetErrorString(e));
         return SFM_ERR_HIP;
     }
-    hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(256), lds, stream, s, q, means, table, past, q_start, selected);
+    // four rows share a mean where most requests have that many groups
+    const int rt = d.tokens / d.group >= 4 * (int64_t)d.requests ? 4 : 1, ni = (d.D + 63) / 64;
+    for (int64_t row0 = 0; row0 < rows; row0 += select_pass(d)) {
+        SelectArgs s{d, q, means, table, past, q_start, selected, (uint64_t*)workspace, first, last, (int)row0, (int)std::min<int64_t>(select_pass(d), rows - row0), 0};
+        const int64_t tiles = (s.rows + rt - 1) / rt;
+        // 64 pages are a round of a workgroup's loads; as few rounds as keep the chip busy
+        const int64_t wanted = std::max<int64_t>(1, 8 * cu_count() / (tiles * d.kv_heads));
+        s.chunk = (int)std::max<int64_t>(64, ((d.width + wanted - 1) / wanted + 63) / 64 * 64);
+        s.chunk = (int)std::max<int64_t>(s.chunk, (d.width / 65535 + 64) / 64 * 64);
+        const dim3 grid((unsigned)tiles, d.kv_heads, (d.width + s.chunk - 1) / s.chunk);
+        auto kern = d.dtype == SFM_BF16 ? (rt == 4 ? score_kernel<BF16, 4>(ni) : score_kernel<BF16, 1>(ni))
+                    : d.dtype == SFM_F16 ? (rt == 4 ? score_kernel<F16, 4>(ni) : score_kernel<F16, 1>(ni))
+                                         : (rt == 4 ? score_kernel<float, 4>(ni) : score_kernel<float, 1>(ni));
+        hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, s);
+        hipLaunchKernelGGL(paged_select_kernel, dim3((unsigned)(s.rows * d.kv_heads)), dim3(256), lds, stream, s);
+    }
     return launched();
 }
 
