@@ -22,11 +22,11 @@ struct PlanArgs {
 };
 
 // A workgroup keeps this many requests' sums in LDS (8 bytes each): up to here every workgroup forms all the sums for itself,
-// which is one launch and no wait between workgroups; 6000 requests take it 5 us of a call's 13.
+// which is one launch and no wait between workgroups.
 constexpr int kPlanLds = 8192;
-constexpr int kPlanThreads = 256;
 
 // Exclusive sum over the workgroup's threads; *total gets the sum of all.
+template <int NT>
 __device__ __forceinline__ int64_t plan_scan(int64_t v, int64_t* red, int64_t* total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int64_t x = v;
@@ -40,7 +40,7 @@ __device__ __forceinline__ int64_t plan_scan(int64_t v, int64_t* red, int64_t* t
     __syncthreads();
     int64_t before = 0, all = 0;
 #pragma unroll
-    for (int w = 0; w < kPlanThreads / 64; ++w) {
+    for (int w = 0; w < NT / 64; ++w) {
         if (w < wave) before += red[w];
         all += red[w];
     }
@@ -54,33 +54,38 @@ __device__ __forceinline__ int64_t plan_entries(int64_t pos, const PlanArgs& a) 
     return e + (e * a.page8.d < b);
 }
 
-// tokens[r] = first row of request r (at most T), pages[r] = pages that the requests before r open; r = 0 .. R
+// at[0 .. n) becomes its exclusive sum, at most `most`, and at[n] the whole of it
+template <int NT>
+__device__ __forceinline__ void plan_prefix(int32_t* at, int n, int64_t most, int64_t* red) {
+    const int per = (n + NT - 1) / NT, i0 = min((int)threadIdx.x * per, n), i1 = min(i0 + per, n);
+    int64_t sum = 0, total;
+    for (int i = i0; i < i1; ++i) sum += at[i];
+    int64_t before = plan_scan<NT>(sum, red, &total);
+    for (int i = i0; i < i1; ++i) {
+        const int v = at[i];
+        at[i] = (int32_t)min(before, most);
+        before += v;
+    }
+    if (threadIdx.x == 0) at[n] = (int32_t)min(total, most);
+    __syncthreads();
+}
+
+// tokens[r] = first row of request r (at most T), pages[r] = pages that the requests before r open; r = 0 .. R.  The lengths are
+// read in whole lines and independently of each other; a thread sums a run of them.
+template <int NT>
 __device__ void plan_sums(const PlanArgs& a, int32_t* tokens, int32_t* pages) {
-    __shared__ int64_t red[kPlanThreads / 64];
-    const int per = (a.R + kPlanThreads - 1) / kPlanThreads, r0 = min((int)threadIdx.x * per, a.R), r1 = min(r0 + per, a.R);
-    int64_t n = 0, total;
-    for (int r = r0; r < r1; ++r) n += max(a.fresh[r], 0);
-    int64_t at = plan_scan(n, red, &total);
-    for (int r = r0; r < r1; ++r) {
-        tokens[r] = (int32_t)min(at, a.T);
-        at += max(a.fresh[r], 0);
-    }
-    if (threadIdx.x == 0) tokens[a.R] = (int32_t)min(total, a.T);
+    __shared__ int64_t red[NT / 64];
+#pragma unroll 8
+    for (int r = threadIdx.x; r < a.R; r += NT) tokens[r] = max(a.fresh[r], 0);
     __syncthreads();
-    n = 0;
-    for (int r = r0; r < r1; ++r) {
+    plan_prefix<NT>(tokens, a.R, a.T, red);
+#pragma unroll 8
+    for (int r = threadIdx.x; r < a.R; r += NT) {
         const int64_t past = max(a.past[r], 0), len = past + tokens[r + 1] - tokens[r];
-        n += plan_entries(len, a) - plan_entries(past, a);
+        pages[r] = (int32_t)(plan_entries(len, a) - plan_entries(past, a));
     }
-    at = plan_scan(n, red, &total);
-    // fewer pages are wanted than tokens planned, T < 2^31
-    for (int r = r0; r < r1; ++r) {
-        pages[r] = (int32_t)at;
-        const int64_t past = max(a.past[r], 0), len = past + tokens[r + 1] - tokens[r];
-        at += plan_entries(len, a) - plan_entries(past, a);
-    }
-    if (threadIdx.x == 0) pages[a.R] = (int32_t)total;
     __syncthreads();
+    plan_prefix<NT>(pages, a.R, 0x7fffffff, red);        // fewer pages are wanted than tokens planned, T < 2^31
 }
 
 // the last r in [0, n) with at[r] <= v (at[0] = 0 <= v, ascending)
@@ -100,7 +105,7 @@ __device__ __forceinline__ int32_t plan_page(const PlanArgs& a, int64_t i) {    
 }
 
 __device__ void plan_fill(const PlanArgs& a, const int32_t* tokens, const int32_t* pages) {
-    const int64_t tid = (int64_t)blockIdx.x * kPlanThreads + threadIdx.x, step = (int64_t)gridDim.x * kPlanThreads;
+    const int64_t tid = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * blockDim.x;
     const int wanted = pages[a.R], planned = tokens[a.R];
     for (int64_t r = tid; r <= a.R; r += step) {
         a.q_start[r] = tokens[r];
@@ -129,13 +134,14 @@ __device__ void plan_fill(const PlanArgs& a, const int32_t* tokens, const int32_
     }
 }
 
-__global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
+template <int NT>
+__global__ __launch_bounds__(NT) void paged_plan_kernel(PlanArgs a) {
     extern __shared__ int32_t plan_lds[];
-    plan_sums(a, plan_lds, plan_lds + a.R + 1);
+    plan_sums<NT>(a, plan_lds, plan_lds + a.R + 1);
     plan_fill(a, plan_lds, plan_lds + a.R + 1);
 }
-__global__ __launch_bounds__(kPlanThreads) void paged_plan_sums_kernel(PlanArgs a) { plan_sums(a, a.ws_tokens, a.ws_pages); }
-__global__ __launch_bounds__(kPlanThreads) void paged_plan_fill_kernel(PlanArgs a) { plan_fill(a, a.ws_tokens, a.ws_pages); }
+__global__ __launch_bounds__(1024) void paged_plan_sums_kernel(PlanArgs a) { plan_sums<1024>(a, a.ws_tokens, a.ws_pages); }
+__global__ __launch_bounds__(256) void paged_plan_fill_kernel(PlanArgs a) { plan_fill(a, a.ws_tokens, a.ws_pages); }
 
 static int launched() {
     const hipError_t err = hipGetLastError();
@@ -152,12 +158,15 @@ int launch_paged_plan(int R, int W, int page_size, int64_t T, int32_t* table, in
     PlanArgs a{R, W, fast_div(page_size / 8), T, table_stride, free_count, table, past, fresh, free_pages, taken, q_start, lengths, next_free, slots,
                (int32_t*)workspace, (int32_t*)workspace + R + 1};
     const int64_t items = T > R + 1 ? T : R + 1;
-    const int wgs = (int)std::min<int64_t>(std::max<int64_t>((items + 4 * kPlanThreads - 1) / (4 * kPlanThreads), 1), 1024);
-    if (R <= kPlanLds) {
-        hipLaunchKernelGGL(paged_plan_kernel, dim3(wgs), dim3(kPlanThreads), 2 * ((size_t)R + 1) * sizeof(int32_t), stream, a);
+    auto wgs = [&](int threads) { return dim3((unsigned)std::min<int64_t>(std::max<int64_t>((items + 4 * threads - 1) / (4 * threads), 1), 1024)); };
+    const size_t lds = 2 * ((size_t)R + 1) * sizeof(int32_t);
+    if (R <= 1024) {
+        hipLaunchKernelGGL(paged_plan_kernel<256>, wgs(256), dim3(256), lds, stream, a);
+    } else if (R <= kPlanLds) {
+        hipLaunchKernelGGL(paged_plan_kernel<1024>, wgs(1024), dim3(1024), lds, stream, a);
     } else {
-        hipLaunchKernelGGL(paged_plan_sums_kernel, dim3(1), dim3(kPlanThreads), 0, stream, a);
-        hipLaunchKernelGGL(paged_plan_fill_kernel, dim3(wgs), dim3(kPlanThreads), 0, stream, a);
+        hipLaunchKernelGGL(paged_plan_sums_kernel, dim3(1), dim3(1024), 0, stream, a);
+        hipLaunchKernelGGL(paged_plan_fill_kernel, wgs(256), dim3(256), 0, stream, a);
     }
     return launched();
 }
@@ -167,6 +176,8 @@ int launch_paged_plan(int R, int W, int page_size, int64_t T, int32_t* table, in
 // ------------------------------------------------------------------------------------------------
 struct WriteArgs {
     int T, R, W, H, chunks, page, pages, per;      // chunks: 16 bytes each, of a row of a head; per: tokens of a workgroup that forms means
+    FastDiv row, head;             // by the chunks of a token's row, and of a head's
+    int copy;                      // tokens of a workgroup that copies
     int64_t table_stride, ps, ts, hs, ks, kh;      // in chunks (the table: in entries)
     const u32x4 *k, *v;
     u32x4 *kp, *vp;
@@ -219,18 +230,17 @@ __device__ void write_means(const WriteArgs& a, int t0, int t1, int h) {
 #pragma unroll
         for (int i = 0; i < N; ++i) sum[i] = 0.f;
         if (g < groups) {
-            const u32x4* const in = a.kp + page * a.ps + h * a.hs + c;
-            for (int j = g; j < old; j += groups) {
-                Chunk<E>::get(in[j * a.ts], x);
+            // several rows on their way at a time: a page of 1560 rows is 98 of a lane's
+            auto add = [&](const u32x4* from, int64_t stride, int j, int end) {
+#pragma unroll 8
+                for (; j < end; j += groups) {
+                    Chunk<E>::get(from[j * stride], x);
 #pragma unroll
-                for (int i = 0; i < N; ++i) sum[i] += x[i];
-            }
-            const u32x4* const fresh = a.k + (q.first + (base - q.past)) * a.ks + h * a.kh + c;
-            for (int j = old + (groups - old % groups + g) % groups; j < rows; j += groups) {
-                Chunk<E>::get(fresh[j * a.ks], x);
-#pragma unroll
-                for (int i = 0; i < N; ++i) sum[i] += x[i];
-            }
+                    for (int i = 0; i < N; ++i) sum[i] += x[i];
+                }
+            };
+            add(a.kp + page * a.ps + h * a.hs + c, a.ts, g, old);
+            add(a.k + (q.first + (base - q.past)) * a.ks + h * a.kh + c, a.ks, old + (groups - old % groups + g) % groups, rows);
         }
         __syncthreads();
         if (g < groups)
@@ -253,12 +263,11 @@ __global__ __launch_bounds__(256) void paged_write_kernel(WriteArgs a) {
         write_means<E>(a, piece * a.per, min(a.T, (piece + 1) * a.per), h);
         return;
     }
-    const uint32_t row = a.H * a.chunks;
-    const int64_t total = (int64_t)a.T * row, step = (int64_t)(gridDim.x - a.mean_wgs) * 256, all = (int64_t)a.pages * a.page;
-    for (int64_t i = (int64_t)(blockIdx.x - a.mean_wgs) * 256 + threadIdx.x; i < total; i += step) {
-        const int64_t t = i / row;
-        const uint32_t x = (uint32_t)(i - t * row), h = x / a.chunks, c = x - h * a.chunks;
-        const int64_t slot = a.slots[t];
+    const int t0 = ((int)blockIdx.x - a.mean_wgs) * a.copy, n = min(a.T - t0, a.copy) * (int)a.row.d;
+    const int64_t all = (int64_t)a.pages * a.page;
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const uint32_t tt = quot(i, a.row), x = i - tt * a.row.d, h = quot(x, a.head), c = x - h * a.head.d;
+        const int64_t t = t0 + (int)tt, slot = a.slots[t];
         if (slot < 0 || slot >= all) continue;
         const uint32_t page = (uint32_t)slot / a.page;                 // slots are below 2^31
         const int64_t to = page * a.ps + (slot - (int64_t)page * a.page) * a.ts + h * a.hs + c, from = t * a.ks + h * a.kh + c;
@@ -270,7 +279,7 @@ __global__ __launch_bounds__(256) void paged_write_kernel(WriteArgs a) {
 int launch_paged_write(const sfm_paged_desc& d, const void* k, const void* v, const int64_t* ks, void* kp, void* vp, const int64_t* slots,
                        const int32_t* table, const int32_t* past, const int32_t* q_start, float* means, hipStream_t stream) {
     const int n16 = d.dtype == SFM_F32 ? 4 : 8;
-    WriteArgs a{(int)d.tokens, d.requests, d.width, d.kv_heads, d.D / n16, d.page_size, d.pages, 1, d.table_stride,
+    WriteArgs a{(int)d.tokens, d.requests, d.width, d.kv_heads, d.D / n16, d.page_size, d.pages, 1, fast_div(d.kv_heads * d.D / n16), fast_div(d.D / n16), 1, d.table_stride,
                 d.pool_stride[0] / n16, d.pool_stride[1] / n16, d.pool_stride[2] / n16, ks[0] / n16, ks[1] / n16, (const u32x4*)k, (const u32x4*)v,
                 (u32x4*)kp, (u32x4*)vp, slots, table, past, q_start, means, 0};
     if (means) {
@@ -278,8 +287,13 @@ int launch_paged_write(const sfm_paged_desc& d, const void* k, const void* v, co
         a.per = std::max(1, a.T / 256);
         a.mean_wgs = (a.T + a.per - 1) / a.per * a.H;
     }
-    const int64_t total = (int64_t)a.T * a.H * a.chunks;
-    const dim3 grid((unsigned)(a.mean_wgs + std::min<int64_t>((total + 255) / 256, 8192)));
+    a.copy = std::max(1, 1024 / (int)a.row.d);
+    const int64_t wgs = a.mean_wgs + ((int64_t)a.T + a.copy - 1) / a.copy;
+    if (wgs >= (1 << 24) || a.row.d >= (1 << 24)) {
+        set_error("%lld rows of %d heads are more than a launch takes", (long long)d.tokens, d.kv_heads);
+        return SFM_ERR_UNSUPPORTED;
+    }
+    const dim3 grid((unsigned)wgs);
     auto kern = d.dtype == SFM_BF16 ? paged_write_kernel<BF16> : d.dtype == SFM_F16 ? paged_write_kernel<F16> : paged_write_kernel<float>;
     hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, a);
     return launched();
@@ -301,6 +315,7 @@ struct SelectArgs {
     int first, last;
     int row0, rows;                // of this pass
     int chunk;                     // pages that a workgroup scores
+    double* sums;                  // [row - row0][kv head][D]: the queries' sums, NULL: formed by whom they are for
 };
 
 // A score's bits in the order of the scores: NaN counts as -inf, -0 as 0.
@@ -328,6 +343,47 @@ __device__ __forceinline__ SelectRow select_row(const SelectArgs& s, int row) {
     return x;
 }
 
+// Sum of the queries of `n` tokens from t0 on and of a key head's G query heads, in sum[0 .. D).  Chunk c of the rows g, g + groups, ...
+// to a thread; `part` holds their sums.
+template <typename E>
+__device__ __forceinline__ void sum_queries(const SelectArgs& s, int kh, int64_t t0, int n, double* part, double* sum) {
+    constexpr int N = Chunk<E>::kN;
+    const sfm_paged_desc& d = s.d;
+    const int tid = threadIdx.x, G = d.H / d.kv_heads, chunks = d.D / N, groups = 256 / chunks, g = tid / chunks, c = tid - g * chunks;
+    const int64_t rows = (int64_t)n * G;
+    double mine[N];
+    float v[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) mine[k] = 0.0;
+    if (g < groups)
+#pragma unroll 4
+        for (int64_t j = g; j < rows; j += groups) {
+            const int64_t t = j / G, h = j - t * G;
+            Chunk<E>::get(((const u32x4*)s.q)[((t0 + t) * d.q_stride[0] + (kh * G + h) * d.q_stride[1]) / N + c], v);
+#pragma unroll
+            for (int k = 0; k < N; ++k) mine[k] += (double)v[k];
+        }
+    __syncthreads();
+    if (g < groups)
+#pragma unroll
+        for (int k = 0; k < N; ++k) part[g * d.D + c * N + k] = mine[k];
+    __syncthreads();
+    if (tid < d.D) {
+        double t = 0.0;
+        for (int j = 0; j < min((int64_t)groups, rows); ++j) t += part[j * d.D + tid];
+        sum[tid] = t;
+    }
+}
+
+// The sums of all rows, where many queries make one: the scores' workgroups would each add them up again.
+template <typename E>
+__global__ __launch_bounds__(256) void paged_sums_kernel(SelectArgs s) {
+    __shared__ double part[256 * Chunk<E>::kN];
+    const SelectRow x = select_row(s, s.row0 + blockIdx.x);
+    if (x.candidates > s.d.top)
+        sum_queries<E>(s, blockIdx.y, x.t0, x.n, part, s.sums + ((int64_t)blockIdx.x * s.d.kv_heads + blockIdx.y) * s.d.D);
+}
+
 // Scores of `chunk` pages for RT rows of one key head.  Sixteen lanes share a page, 4 of each 64 channels a lane; their queries' sums
 // stay in registers, so that rows of one request (many groups of a prompt) read a mean once.  Bound by the means' bytes for single
 // tokens.
@@ -339,7 +395,6 @@ __global__ __launch_bounds__(256) void paged_score_kernel(SelectArgs s) {
     const sfm_paged_desc& d = s.d;
     const int tid = threadIdx.x, sub = tid & 15;
     const int kh = blockIdx.y, tile = s.row0 + blockIdx.x * RT, end = min(tile + RT, s.row0 + s.rows), c0 = blockIdx.z * s.chunk;
-    const int G = d.H / d.kv_heads, chunks = d.D / N, groups = 256 / chunks, g = tid / chunks, c = tid - g * chunks;
     for (int row = tile; row < end;) {
         const SelectRow x = select_row(s, row);
         int count = 1;             // rows of the same request from here on
@@ -353,31 +408,12 @@ __global__ __launch_bounds__(256) void paged_score_kernel(SelectArgs s) {
             ++count;
         }
         if (c0 < most) {
-            // sums of the queries: chunk c of the rows g, g + groups, ...
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
-                const int64_t t0 = x.t0 + (int64_t)i * d.group;
-                const int rows = i < count ? (int)(i == count - 1 ? last.n : d.group) * G : 0;
-                double sum[N];
-                float v[N];
-#pragma unroll
-                for (int k = 0; k < N; ++k) sum[k] = 0.0;
-                if (g < groups)
-                    for (int j = g; j < rows; j += groups) {
-                        const int t = j / G, h = j - t * G;
-                        Chunk<E>::get(((const u32x4*)s.q)[((t0 + t) * d.q_stride[0] + (int64_t)(kh * G + h) * d.q_stride[1]) / N + c], v);
-#pragma unroll
-                        for (int k = 0; k < N; ++k) sum[k] += (double)v[k];
-                    }
-                __syncthreads();
-                if (g < groups)
-#pragma unroll
-                    for (int k = 0; k < N; ++k) part[g * d.D + c * N + k] = sum[k];
-                __syncthreads();
-                if (tid < d.D) {
-                    double t = 0.0;
-                    for (int j = 0; j < min(groups, rows); ++j) t += part[j * d.D + tid];
-                    qsum[i][tid] = t;
+                if (s.sums != nullptr) {
+                    if (tid < d.D) qsum[i][tid] = i < count ? s.sums[((int64_t)(row + i - s.row0) * d.kv_heads + kh) * d.D + tid] : 0.0;
+                } else {
+                    sum_queries<E>(s, kh, x.t0 + (int64_t)i * d.group, i < count ? (i == count - 1 ? last.n : d.group) : 0, part, qsum[i]);
                 }
             }
             __syncthreads();
@@ -547,12 +583,13 @@ __global__ __launch_bounds__(256) void paged_select_kernel(SelectArgs s) {
 
 // Rows of a pass: their scores take this many bytes at most (a row's always).
 constexpr size_t kSelWorkspace = 256u << 20;
+static size_t select_row_bytes(const sfm_paged_desc& d) { return (size_t)d.kv_heads * (d.width + d.D) * sizeof(uint64_t); }
 static int select_pass(const sfm_paged_desc& d) {
-    const size_t row = (size_t)d.kv_heads * d.width * sizeof(uint64_t);
+    const size_t row = select_row_bytes(d);
     const int64_t rows = pieces(d.tokens, d.group, d.requests);
     return (int)std::max<int64_t>(1, std::min<int64_t>({rows, (int64_t)(kSelWorkspace / row), 65535}));
 }
-size_t paged_select_workspace_bytes(const sfm_paged_desc& d) { return (size_t)select_pass(d) * d.kv_heads * d.width * sizeof(uint64_t); }
+size_t paged_select_workspace_bytes(const sfm_paged_desc& d) { return select_pass(d) * select_row_bytes(d); }
 
 template <typename E, int RT>
 static auto score_kernel(int ni) {
@@ -573,9 +610,12 @@ int launch_paged_select(const sfm_paged_desc& d, const void* q, const float* mea
         return SFM_ERR_HIP;
     }
     // four rows share a mean where most requests have that many groups
+    // and the sums are formed once where a row's are of more queries than a workgroup reads at once
+    const bool sums = (int64_t)d.group * (d.H / d.kv_heads) > 16;
     const int rt = d.tokens / d.group >= 4 * (int64_t)d.requests ? 4 : 1, ni = (d.D + 63) / 64;
     for (int64_t row0 = 0; row0 < rows; row0 += select_pass(d)) {
-        SelectArgs s{d, q, means, table, past, q_start, selected, (uint64_t*)workspace, first, last, (int)row0, (int)std::min<int64_t>(select_pass(d), rows - row0), 0};
+        SelectArgs s{d, q, means, table, past, q_start, selected, (uint64_t*)workspace, first, last, (int)row0, (int)std::min<int64_t>(select_pass(d), rows - row0), 0, nullptr};
+        if (sums) s.sums = (double*)(s.keys + (size_t)s.rows * d.kv_heads * d.width);
         const int64_t tiles = (s.rows + rt - 1) / rt;
         // 64 pages are a round of a workgroup's loads; as few rounds as keep the chip busy
         const int64_t wanted = std::max<int64_t>(1, 8 * cu_count() / (tiles * d.kv_heads));
@@ -585,6 +625,10 @@ int launch_paged_select(const sfm_paged_desc& d, const void* q, const float* mea
         auto kern = d.dtype == SFM_BF16 ? (rt == 4 ? score_kernel<BF16, 4>(ni) : score_kernel<BF16, 1>(ni))
                     : d.dtype == SFM_F16 ? (rt == 4 ? score_kernel<F16, 4>(ni) : score_kernel<F16, 1>(ni))
                                          : (rt == 4 ? score_kernel<float, 4>(ni) : score_kernel<float, 1>(ni));
+        if (sums) {
+            auto add = d.dtype == SFM_BF16 ? paged_sums_kernel<BF16> : d.dtype == SFM_F16 ? paged_sums_kernel<F16> : paged_sums_kernel<float>;
+            hipLaunchKernelGGL(add, dim3(s.rows, d.kv_heads), dim3(256), 0, stream, s);
+        }
         hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, s);
         hipLaunchKernelGGL(paged_select_kernel, dim3((unsigned)(s.rows * d.kv_heads)), dim3(256), lds, stream, s);
     }
