@@ -175,7 +175,7 @@ int launch_paged_plan(int R, int W, int page_size, int64_t T, int32_t* table, in
 // write
 // ------------------------------------------------------------------------------------------------
 struct WriteArgs {
-    int T, R, W, H, chunks, page, pages, per;      // chunks: 16 bytes each, of a row of a head; per: tokens of a workgroup that forms means
+    int T, R, W, H, chunks, page, pages;           // chunks: 16 bytes each, of a row of a head
     FastDiv row, head;             // by the chunks of a token's row, and of a head's
     int copy;                      // tokens of a workgroup that copies
     int64_t table_stride, ps, ts, hs, ks, kh;      // in chunks (the table: in entries)
@@ -207,65 +207,69 @@ template <class E> struct Chunk16 {
 template <> struct Chunk<BF16> : Chunk16<BF16> {};
 template <> struct Chunk<F16> : Chunk16<F16> {};
 
-// The mean keys of the pages that tokens [t0, t1) are the first to reach, of one head.  New rows are taken from k, whatever the
-// copying workgroups have done by then.  A page's rows are summed by groups of lanes, a row each, joined in LDS in a fixed order.
-template <typename E>
-__device__ void write_means(const WriteArgs& a, int t0, int t1, int h) {
+// The mean key of one page, of one head: the page'th that a step's requests write to.  A request of n tokens writes to at most
+// (n - 1) / page_size + 2 pages; its first has number q_start / page_size + 2 r, which leaves it as many.  New rows are taken from
+// k, whatever the copying workgroups have done by then.  The rows are summed by groups of lanes, a row each, joined in LDS in
+// a fixed order.
+template <typename E, int NT>
+__device__ void write_mean(const WriteArgs& a, int number, int h) {
     constexpr int N = Chunk<E>::kN;
-    __shared__ float part[256 * N];
-    const int tid = threadIdx.x, groups = 256 / a.chunks, g = tid / a.chunks, c = tid - g * a.chunks, D = a.chunks * N;
-    int r = find_last(a.R, t0, [&](int i) { return (int64_t)clamp_int(a.q_start[i], 0, a.T); });
-    for (int t = t0; t < t1; ++t) {
-        while (r < a.R && clamp_int(a.q_start[r + 1], 0, a.T) <= t) ++r;
-        if (r >= a.R) return;
-        const Request q = request_of(a.q_start, a.past, r, a.R, a.T);
-        const int64_t pos = (int64_t)q.past + t - q.first;
-        const int64_t e = pos / a.page, off = pos - e * a.page;
-        if ((t != q.first && off != 0) || e >= a.W) continue;
-        const int page = a.table[r * a.table_stride + e];
-        if (page < 0 || page >= a.pages) continue;
-        const int64_t base = e * a.page;
-        const int rows = (int)min((int64_t)q.past + q.n - base, (int64_t)a.page), old = (int)max((int64_t)0, min((int64_t)rows, q.past - base));
-        float sum[N], x[N];
+    __shared__ float part[NT * N];
+    const int tid = threadIdx.x, groups = NT / a.chunks, g = tid / a.chunks, c = tid - g * a.chunks, D = a.chunks * N;
+    auto first = [&](int i) { return (int64_t)clamp_int(a.q_start[i], 0, a.T) / a.page + 2 * (int64_t)i; };
+    const int r = find_last(a.R, number, first);
+    if (r >= a.R) return;
+    const Request q = request_of(a.q_start, a.past, r, a.R, a.T);
+    const int64_t e = q.past / a.page + (number - first(r));
+    if (q.n == 0 || number < first(r) || e * a.page >= (int64_t)q.past + q.n || e >= a.W) return;
+    const int page = a.table[r * a.table_stride + e];
+    if (page < 0 || page >= a.pages) return;
+    const int64_t base = e * a.page;
+    const int rows = (int)min((int64_t)q.past + q.n - base, (int64_t)a.page), old = (int)max((int64_t)0, min((int64_t)rows, q.past - base));
+    float sum[N], x[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) sum[i] = 0.f;
-        if (g < groups) {
-            // several rows on their way at a time: a page of 1560 rows is 98 of a lane's
-            auto add = [&](const u32x4* from, int64_t stride, int j, int end) {
-#pragma unroll 8
-                for (; j < end; j += groups) {
-                    Chunk<E>::get(from[j * stride], x);
+    for (int i = 0; i < N; ++i) sum[i] = 0.f;
+    if (g < groups) {
+        // eight rows on their way at a time
+        auto add = [&](const u32x4* from, int64_t stride, int j, int end) {
+            for (; j < end; j += 8 * groups) {
+                u32x4 w[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) w[u] = j + u * groups < end ? from[(j + u * groups) * stride] : u32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    Chunk<E>::get(w[u], x);
 #pragma unroll
                     for (int i = 0; i < N; ++i) sum[i] += x[i];
                 }
-            };
-            add(a.kp + page * a.ps + h * a.hs + c, a.ts, g, old);
-            add(a.k + (q.first + (base - q.past)) * a.ks + h * a.kh + c, a.ks, old + (groups - old % groups + g) % groups, rows);
-        }
-        __syncthreads();
-        if (g < groups)
+            }
+        };
+        add(a.kp + page * a.ps + h * a.hs + c, a.ts, g, old);
+        add(a.k + (q.first + (base - q.past)) * a.ks + h * a.kh + c, a.ks, old + (groups - old % groups + g) % groups, rows);
+    }
+    __syncthreads();
+    if (g < groups)
 #pragma unroll
-            for (int i = 0; i < N; ++i) part[(g * a.chunks + c) * N + i] = sum[i];
-        __syncthreads();
-        if (tid < D) {
-            float s = 0.f;
-            for (int j = 0; j < groups; ++j) s += part[j * D + tid];
-            a.means[((int64_t)page * a.H + h) * D + tid] = s / (float)rows;
-        }
+        for (int i = 0; i < N; ++i) part[(g * a.chunks + c) * N + i] = sum[i];
+    __syncthreads();
+    if (tid < D) {
+        float s = 0.f;
+        for (int j = 0; j < groups; ++j) s += part[j * D + tid];
+        a.means[((int64_t)page * a.H + h) * D + tid] = s / (float)rows;
     }
 }
 
 // The first mean_wgs workgroups form means, the others copy 16 bytes per lane and tensor at a time.  Bound by the rows' bytes.
-template <typename E>
-__global__ __launch_bounds__(256) void paged_write_kernel(WriteArgs a) {
+template <typename E, int NT>
+__global__ __launch_bounds__(NT) void paged_write_kernel(WriteArgs a) {
     if ((int)blockIdx.x < a.mean_wgs) {
         const int piece = blockIdx.x / a.H, h = blockIdx.x - piece * a.H;
-        write_means<E>(a, piece * a.per, min(a.T, (piece + 1) * a.per), h);
+        write_mean<E, NT>(a, piece, h);
         return;
     }
     const int t0 = ((int)blockIdx.x - a.mean_wgs) * a.copy, n = min(a.T - t0, a.copy) * (int)a.row.d;
     const int64_t all = (int64_t)a.pages * a.page;
-    for (int i = threadIdx.x; i < n; i += 256) {
+    for (int i = threadIdx.x; i < n; i += NT) {
         const uint32_t tt = quot(i, a.row), x = i - tt * a.row.d, h = quot(x, a.head), c = x - h * a.head.d;
         const int64_t t = t0 + (int)tt, slot = a.slots[t];
         if (slot < 0 || slot >= all) continue;
@@ -279,23 +283,25 @@ __global__ __launch_bounds__(256) void paged_write_kernel(WriteArgs a) {
 int launch_paged_write(const sfm_paged_desc& d, const void* k, const void* v, const int64_t* ks, void* kp, void* vp, const int64_t* slots,
                        const int32_t* table, const int32_t* past, const int32_t* q_start, float* means, hipStream_t stream) {
     const int n16 = d.dtype == SFM_F32 ? 4 : 8;
-    WriteArgs a{(int)d.tokens, d.requests, d.width, d.kv_heads, d.D / n16, d.page_size, d.pages, 1, fast_div(d.kv_heads * d.D / n16), fast_div(d.D / n16), 1, d.table_stride,
+    WriteArgs a{(int)d.tokens, d.requests, d.width, d.kv_heads, d.D / n16, d.page_size, d.pages, fast_div(d.kv_heads * d.D / n16), fast_div(d.D / n16), 1, d.table_stride,
                 d.pool_stride[0] / n16, d.pool_stride[1] / n16, d.pool_stride[2] / n16, ks[0] / n16, ks[1] / n16, (const u32x4*)k, (const u32x4*)v,
                 (u32x4*)kp, (u32x4*)vp, slots, table, past, q_start, means, 0};
-    if (means) {
-        // single tokens of many requests reach a page each, long prompts one page in page_size tokens
-        a.per = std::max(1, a.T / 256);
-        a.mean_wgs = (a.T + a.per - 1) / a.per * a.H;
-    }
-    a.copy = std::max(1, 1024 / (int)a.row.d);
-    const int64_t wgs = a.mean_wgs + ((int64_t)a.T + a.copy - 1) / a.copy;
-    if (wgs >= (1 << 24) || a.row.d >= (1 << 24)) {
+    const int64_t numbers = means ? d.tokens / d.page_size + 2 * (int64_t)d.requests : 0;
+    // a page's mean is one workgroup's: sixteen waves for long pages, whose rows take it 4 rounds of loads instead of 13 (1560 rows)
+    const int nt = means && d.page_size >= 256 ? 1024 : 256;
+    a.copy = std::max(1, 4 * nt / (int)a.row.d);
+    const int64_t wgs = numbers * a.H + ((int64_t)a.T + a.copy - 1) / a.copy;
+    if (wgs * nt >= ((int64_t)1 << 32) || a.row.d >= (1 << 24)) {
         set_error("%lld rows of %d heads are more than a launch takes", (long long)d.tokens, d.kv_heads);
         return SFM_ERR_UNSUPPORTED;
     }
-    const dim3 grid((unsigned)wgs);
-    auto kern = d.dtype == SFM_BF16 ? paged_write_kernel<BF16> : d.dtype == SFM_F16 ? paged_write_kernel<F16> : paged_write_kernel<float>;
-    hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, a);
+    a.mean_wgs = (int)(numbers * a.H);
+    auto pick = [&](auto nt_c) {
+        constexpr int NT = decltype(nt_c)::value;
+        return d.dtype == SFM_BF16 ? paged_write_kernel<BF16, NT> : d.dtype == SFM_F16 ? paged_write_kernel<F16, NT> : paged_write_kernel<float, NT>;
+    };
+    auto kern = nt == 256 ? pick(std::integral_constant<int, 256>{}) : pick(std::integral_constant<int, 1024>{});
+    hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(nt), 0, stream, a);
     return launched();
 }
 
@@ -599,7 +605,7 @@ static auto score_kernel(int ni) {
 int launch_paged_select(const sfm_paged_desc& d, const void* q, const float* means, const int32_t* table, const int32_t* past,
                         const int32_t* q_start, int first, int last, int32_t* selected, void* workspace, hipStream_t stream) {
     const int64_t rows = pieces(d.tokens, d.group, d.requests);
-    if (d.kv_heads > 65535 || (int64_t)select_pass(d) * d.kv_heads >= (1 << 24) || rows / select_pass(d) > 4096) {
+    if ((int64_t)select_pass(d) * d.kv_heads >= (1 << 24) || rows / select_pass(d) > 4096) {
         set_error("%lld groups of tokens with %d key heads are more than a call takes", (long long)rows, d.kv_heads);
         return SFM_ERR_UNSUPPORTED;
     }

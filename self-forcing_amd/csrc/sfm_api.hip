@@ -1873,7 +1873,7 @@ static int check_paged(const sfm_paged_desc* d, bool pool) {
         set_error("unsupported dtype %d", d->dtype);
         return SFM_ERR_DTYPE;
     }
-    if (d->kv_heads < 1 || d->D < 8 || d->D % 8 || d->D > 256 || d->pages < 1) {
+    if (d->kv_heads < 1 || d->kv_heads > 65535 || d->D < 8 || d->D % 8 || d->D > 256 || d->pages < 1) {
         set_error("kv_heads=%d, D=%d, pages=%d invalid", d->kv_heads, d->D, d->pages);
         return SFM_ERR_SHAPE;
     }

@@ -47,7 +47,7 @@ def plan(requests=3, width=5, page=16, tokens=10, stride=5, free_count=9, **ptr)
 
 
 NULL, DTYPE, SHAPE, RANGE, STRIDE, WORKSPACE, ALIGN = -1, -2, -3, -4, -5, -6, -7
-SHARED = [(dict(dtype=7), DTYPE), (dict(kv_heads=0), SHAPE), (dict(D=12), SHAPE), (dict(D=264), SHAPE), (dict(D=0), SHAPE), (dict(pages=0), SHAPE),
+SHARED = [(dict(dtype=7), DTYPE), (dict(kv_heads=0), SHAPE), (dict(kv_heads=65536, H=65536), SHAPE), (dict(D=12), SHAPE), (dict(D=264), SHAPE), (dict(D=0), SHAPE), (dict(pages=0), SHAPE),
           (dict(requests=0), SHAPE), (dict(requests=(1 << 24) + 1), SHAPE), (dict(width=0), SHAPE), (dict(page_size=12), SHAPE), (dict(page_size=0), SHAPE),
           (dict(width=1 << 20, page_size=2048, table_stride=1 << 20), SHAPE), (dict(pages=1 << 20, page_size=2048), SHAPE), (dict(tokens=0), SHAPE),
           (dict(tokens=-1), SHAPE), (dict(tokens=1 << 31), SHAPE), (dict(table_stride=4), STRIDE)]
