@@ -157,14 +157,12 @@ struct RowState {
     }
 };
 
-// What a row sees of a tile: positions below `end` that are at or past `lo` or below `sink`
+// What a row sees of a tile: positions below `end` that, with a window, are at or past `lo` or below `sink`
 struct RowMask {
     int end, lo, sink;
-    __device__ __forceinline__ bool sees(int pos) const { return pos < end && (pos >= lo || pos < sink); }
+    bool window;
+    __device__ __forceinline__ bool sees(int pos) const { return pos < end && (!window || pos >= lo || pos < sink); }
 };
-
-// Key that register v of a lane's logits t belongs to
-__device__ __forceinline__ constexpr int key_of(int t, int v) { return 32 * t + 8 * (v >> 2) + (v & 3); }      // + 4 hf
 
 // One tile of LDS against the wave's rows: logits, masks, weights and V's part.  pos: first positions of the tile's eight blocks.
 // The second half waits for V through `v_ready`, so that K's buffer can be refilled meanwhile (`k_done`).
@@ -189,14 +187,31 @@ __device__ __forceinline__ void masked_tile(const char* lds, uint32_t kbuf, uint
     }
     k_done();
     if (masked) {
+        // key 32 t + 8 g + 4 hf + i is number 4 hf + i of block 4 t + g: the block's first position against limits per i
+        int end[4], lo[4], sink[4];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int i = 0; i < 4; ++i) end[i] = mask.end - 4 * hf - i;
+        if (!mask.window) {
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const bool see = mask.sees(pos[4 * t + (v >> 2)] + 4 * hf + (v & 3));
-                st.seen = st.seen || see;
-                s[t][v] = see ? s[t][v] : -INFINITY;
+            for (int b = 0; b < 8; ++b) {
+                st.seen = st.seen || pos[b] < end[0];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[b >> 2][4 * (b & 3) + i] = pos[b] < end[i] ? s[b >> 2][4 * (b & 3) + i] : -INFINITY;
+                }
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) lo[i] = mask.lo - 4 * hf - i, sink[i] = mask.sink - 4 * hf - i;
+#pragma unroll
+            for (int b = 0; b < 8; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool see = pos[b] < end[i] && (pos[b] >= lo[i] || pos[b] < sink[i]);
+                    st.seen = st.seen || see;
+                    s[b >> 2][4 * (b & 3) + i] = see ? s[b >> 2][4 * (b & 3) + i] : -INFINITY;
+                }
+        }
     } else {
         st.seen = true;
     }
@@ -219,15 +234,16 @@ __device__ __forceinline__ void masked_tile(const char* lds, uint32_t kbuf, uint
     // V rows with values that are not finite, a lane each
     uint64_t odd = 0;
     if (masked) {
-        constexpr uint32_t kExp = E::kDtype == SFM_BF16 ? 0x7f807f80u : 0x7c007c00u, kOne = E::kDtype == SFM_BF16 ? 0x00800080u : 0x04000400u;
-        uint32_t acc = 0;
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+        constexpr uint16_t kInf = E::kDtype == SFM_BF16 ? 0x7f80 : 0x7c00;
+        u16x2 top = {0, 0};                                            // largest magnitude's bits
 #pragma unroll 4
         for (int c = 0; c < L::kCPR; ++c) {
             const u32x4 w = *(const u32x4*)(lds + vbuf + (uint32_t)lane * L::kPitch + (uint32_t)(((c + lane) % L::kCPR) << 4));
 #pragma unroll
-            for (int x = 0; x < 4; ++x) acc |= (w[x] & kExp) + kOne;       // all ones in the exponent: the sum reaches the sign's place
+            for (int x = 0; x < 4; ++x) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[x] & 0x7fff7fffu));
         }
-        odd = __builtin_amdgcn_ballot_w64((acc & 0x80008000u) != 0);
+        odd = __builtin_amdgcn_ballot_w64(max(top.x, top.y) >= kInf);
     }
     uint32_t trA[2];
     const int s16 = lane & 15, rl = 4 * hf + (s16 >> 2), cl = 2 * ((lane >> 4) & 1) + ((s16 & 3) >> 1);
@@ -429,6 +445,7 @@ __device__ __forceinline__ RowMask row_mask(const PagedArgs& a, const Piece& p, 
     k.end = d.causal ? (int)min((int64_t)p.rq.past + row / (d.H / d.kv_heads) + 1, (int64_t)a.cap) : p.k.end_max;
     k.lo = d.window && k.end > d.window ? k.end - d.window : 0;
     k.sink = d.sink;
+    k.window = d.window != 0;
     return k;
 }
 
@@ -453,10 +470,9 @@ __global__ __launch_bounds__(256) void paged_few_kernel(PagedArgs a, int64_t npi
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) char*)lds, buf = (uint32_t)wave * FewLds<D>::kWave;
     const sfm_paged_desc& d = a.d;
-    const int total = (int)(npieces * d.kv_heads * chunks);
-    const int item = xcd_item(total);
-    if (item >= total) return;
-    const int kh = item % d.kv_heads, rest = item / d.kv_heads;        // the heads of a token's row side by side
+    // the heads of a token's row on one XCD, the pieces and ranges in turn on all of them: requests differ in length
+    const int ring = blockIdx.x / 8, kh = ring % d.kv_heads, rest = ring / d.kv_heads * 8 + blockIdx.x % 8;
+    if (rest >= npieces * chunks) return;
     const int chunk = rest % chunks;
     Piece p;
     if (!find_piece<32>(a, rest / chunks, kh, &p)) return;
@@ -955,7 +971,8 @@ static int launch_mfma(const PagedArgs& a, PagedPlan p, float* part, hipStream_t
             set_error("hipFuncSetAttribute failed: %s", hipGetErrorString(e));
             return SFM_ERR_HIP;
         }
-        hipLaunchKernelGGL(kern, dim3(xcd_grid((int)total)), dim3(64 * nw), lds, stream, a, p.pieces, p.chunks, p.chunk_tiles, part);
+        const int64_t grid = p.rows == 32 ? (p.pieces * p.chunks + 7) / 8 * 8 * d.kv_heads : xcd_grid((int)total);
+        hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * nw), lds, stream, a, p.pieces, p.chunks, p.chunk_tiles, part);
         return SFM_OK;
     };
     const int rc = p.rows == 32 ? go(paged_few_kernel<E, D>, 4, FewLds<D>::kTotal + 4 * 96 * sizeof(float))
