@@ -164,26 +164,26 @@ struct RowMask {
     __device__ __forceinline__ bool sees(int pos) const { return pos < end && (!window || pos >= lo || pos < sink); }
 };
 
-// One tile of LDS against the wave's rows: logits, masks, weights and V's part.  pos: first positions of the tile's eight blocks.
+// A tile of 32 NB keys in LDS against the wave's rows: logits, masks, weights and V's part.  pos: first positions of its blocks.
 // The second half waits for V through `v_ready`, so that K's buffer can be refilled meanwhile (`k_done`).
 //
 // A masked weight is 0, and 0 times an infinity or NaN is NaN: in a masked tile V rows that hold such values are left out of the
 // matrix product and added for the rows that see them, one by one.  (Stale rows, and later tokens of the request.)
-template <class E, int D, class KDone, class VReady>
+template <class E, int D, int NB, class KDone, class VReady>
 __device__ __forceinline__ void masked_tile(const char* lds, uint32_t kbuf, uint32_t vbuf, const u32x4* qb, float sc2, RowState<D>& st,
                                             const RowMask& mask, bool masked, const int* pos, KDone k_done, VReady v_ready) {
     using L = DnLds<D>;
     const int lane = threadIdx.x & 63, m = lane & 31, hf = lane >> 5;
-    f32x16 s[2];
+    f32x16 s[NB];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < NB; ++t)
 #pragma unroll
         for (int v = 0; v < 16; ++v) s[t][v] = 0.f;
     const uint32_t sA0 = kbuf + (uint32_t)m * L::kPitch + (uint32_t)((hf ^ L::swz(m)) << 4);
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j) {
-        const u32x4 a = *(const u32x4*)(lds + (sA0 ^ (uint32_t)((j >> 1) << 5)) + (j & 1) * 32 * L::kPitch);
-        s[j & 1] = E::mfma32(a, qb[j >> 1], s[j & 1]);
+    for (int j = 0; j < NB * D / 16; ++j) {
+        const u32x4 a = *(const u32x4*)(lds + (sA0 ^ (uint32_t)((j / NB) << 5)) + (j % NB) * 32 * L::kPitch);
+        s[j % NB] = E::mfma32(a, qb[j / NB], s[j % NB]);
     }
     k_done();
     if (masked) {
@@ -193,8 +193,8 @@ __device__ __forceinline__ void masked_tile(const char* lds, uint32_t kbuf, uint
         for (int i = 0; i < 4; ++i) end[i] = mask.end - 4 * hf - i;
         if (!mask.window) {
 #pragma unroll
-            for (int b = 0; b < 8; ++b) {
-                st.seen = st.seen || pos[b] < end[0];
+            for (int b = 0; b < 4 * NB; ++b) {
+                st.seen = st.seen | (pos[b] < end[0]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     s[b >> 2][4 * (b & 3) + i] = pos[b] < end[i] ? s[b >> 2][4 * (b & 3) + i] : -INFINITY;
@@ -204,11 +204,11 @@ __device__ __forceinline__ void masked_tile(const char* lds, uint32_t kbuf, uint
 #pragma unroll
             for (int i = 0; i < 4; ++i) lo[i] = mask.lo - 4 * hf - i, sink[i] = mask.sink - 4 * hf - i;
 #pragma unroll
-            for (int b = 0; b < 8; ++b)
+            for (int b = 0; b < 4 * NB; ++b)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const bool see = pos[b] < end[i] && (pos[b] >= lo[i] || pos[b] < sink[i]);
-                    st.seen = st.seen || see;
+                    const bool see = (pos[b] < end[i]) & ((pos[b] >= lo[i]) | (pos[b] < sink[i]));
+                    st.seen = st.seen | see;
                     s[b >> 2][4 * (b & 3) + i] = see ? s[b >> 2][4 * (b & 3) + i] : -INFINITY;
                 }
         }
@@ -217,12 +217,12 @@ __device__ __forceinline__ void masked_tile(const char* lds, uint32_t kbuf, uint
     }
     float mx = s[0][0];
 #pragma unroll
-    for (int i = 1; i < 32; ++i) mx = fmaxf(mx, s[i >> 4][i & 15]);
+    for (int i = 1; i < 16 * NB; ++i) mx = fmaxf(mx, s[i >> 4][i & 15]);
     st.raise(fmaxf(st.mrun, xhalf_max(mx) * sc2));
-    u32x4 pb[4];
+    u32x4 pb[2 * NB];
     float psum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) {
+    for (int i = 0; i < 16 * NB; i += 2) {
         const float a = fast_exp2(fmaf(s[i >> 4][i & 15], sc2, -st.mrun)), b = fast_exp2(fmaf(s[i >> 4][(i & 15) + 1], sc2, -st.mrun));
         psum += a + b;
         s[i >> 4][i & 15] = a;
@@ -239,11 +239,11 @@ __device__ __forceinline__ void masked_tile(const char* lds, uint32_t kbuf, uint
         u16x2 top = {0, 0};                                            // largest magnitude's bits
 #pragma unroll 4
         for (int c = 0; c < L::kCPR; ++c) {
-            const u32x4 w = *(const u32x4*)(lds + vbuf + (uint32_t)lane * L::kPitch + (uint32_t)(((c + lane) % L::kCPR) << 4));
+            const u32x4 w = *(const u32x4*)(lds + vbuf + (uint32_t)(lane % (32 * NB)) * L::kPitch + (uint32_t)(((c + lane) % L::kCPR) << 4));
 #pragma unroll
             for (int x = 0; x < 4; ++x) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[x] & 0x7fff7fffu));
         }
-        odd = __builtin_amdgcn_ballot_w64(max(top.x, top.y) >= kInf);
+        odd = __builtin_amdgcn_ballot_w64(max(top.x, top.y) >= kInf) & (NB == 2 ? ~(uint64_t)0 : 0xffffffffu);
     }
     uint32_t trA[2];
     const int s16 = lane & 15, rl = 4 * hf + (s16 >> 2), cl = 2 * ((lane >> 4) & 1) + ((s16 & 3) >> 1);
@@ -254,21 +254,21 @@ __device__ __forceinline__ void masked_tile(const char* lds, uint32_t kbuf, uint
     }
     if (odd == 0) {
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j) {
-            const u32x2 lo = dn_read_tr(lds + (trA[0] ^ (uint32_t)((j >> 2) << 6)), (j & 3) * 16 * L::kPitch);
-            const u32x2 hi = dn_read_tr(lds + (trA[1] ^ (uint32_t)((j >> 2) << 6)), (j & 3) * 16 * L::kPitch);
-            st.o[j >> 2] = E::mfma32(u32x4{lo.x, lo.y, hi.x, hi.y}, pb[j & 3], st.o[j >> 2]);
+        for (int j = 0; j < NB * D / 16; ++j) {
+            const u32x2 lo = dn_read_tr(lds + (trA[0] ^ (uint32_t)((j / (2 * NB)) << 6)), (j % (2 * NB)) * 16 * L::kPitch);
+            const u32x2 hi = dn_read_tr(lds + (trA[1] ^ (uint32_t)((j / (2 * NB)) << 6)), (j % (2 * NB)) * 16 * L::kPitch);
+            st.o[j / (2 * NB)] = E::mfma32(u32x4{lo.x, lo.y, hi.x, hi.y}, pb[j % (2 * NB)], st.o[j / (2 * NB)]);
         }
         return;
     }
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j) {
-        const u32x2 lo = dn_read_tr(lds + (trA[0] ^ (uint32_t)((j >> 2) << 6)), (j & 3) * 16 * L::kPitch);
-        const u32x2 hi = dn_read_tr(lds + (trA[1] ^ (uint32_t)((j >> 2) << 6)), (j & 3) * 16 * L::kPitch);
-        const uint32_t bits = (uint32_t)(odd >> (16 * (j & 3))) >> (4 * hf);           // keys 16 (j % 4) + 4 hf + {0..3, 8..11}
+    for (int j = 0; j < NB * D / 16; ++j) {
+        const u32x2 lo = dn_read_tr(lds + (trA[0] ^ (uint32_t)((j / (2 * NB)) << 6)), (j % (2 * NB)) * 16 * L::kPitch);
+        const u32x2 hi = dn_read_tr(lds + (trA[1] ^ (uint32_t)((j / (2 * NB)) << 6)), (j % (2 * NB)) * 16 * L::kPitch);
+        const uint32_t bits = (uint32_t)(odd >> (16 * (j % (2 * NB)))) >> (4 * hf);   // keys 16 (j % (2 NB)) + 4 hf + {0..3, 8..11}
         const u32x4 keep = {(bits & 1 ? 0u : 0xffffu) | (bits & 2 ? 0u : 0xffff0000u), (bits & 4 ? 0u : 0xffffu) | (bits & 8 ? 0u : 0xffff0000u),
                             (bits & 0x100 ? 0u : 0xffffu) | (bits & 0x200 ? 0u : 0xffff0000u), (bits & 0x400 ? 0u : 0xffffu) | (bits & 0x800 ? 0u : 0xffff0000u)};
-        st.o[j >> 2] = E::mfma32(u32x4{lo.x, lo.y, hi.x, hi.y} & keep, pb[j & 3], st.o[j >> 2]);
+        st.o[j / (2 * NB)] = E::mfma32(u32x4{lo.x, lo.y, hi.x, hi.y} & keep, pb[j % (2 * NB)], st.o[j / (2 * NB)]);
     }
     while (odd) {
         const int l = __builtin_ctzll(odd);
@@ -277,11 +277,11 @@ __device__ __forceinline__ void masked_tile(const char* lds, uint32_t kbuf, uint
         float w = 0.f;
         const int at = 16 * (l >> 5) + 4 * ((l >> 3) & 3) + (l & 3);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) w = i == at ? s[i >> 4][i & 15] : w;
+        for (int i = 0; i < 16 * NB; ++i) w = i == at ? s[i >> 4][i & 15] : w;
         w = __shfl(w, m + 32 * ((l >> 2) & 1));
         int p = kNoPos;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p = i == (l >> 3) ? pos[i] : p;
+        for (int i = 0; i < 4 * NB; ++i) p = i == (l >> 3) ? pos[i] : p;
         const bool see = !masked || mask.sees(p + (l & 7));
 #pragma unroll
         for (int c = 0; c < L::kCPR; ++c) {        // channels 8 c + 4 hf + {0..3}
@@ -451,27 +451,28 @@ __device__ __forceinline__ RowMask row_mask(const PagedArgs& a, const Piece& p, 
 
 // ---- few rows: a wave takes tiles of its own --------------------------------------------------------------------------------
 //
-// Pieces of up to 32 rows, single tokens above all.  The four waves of a workgroup take its tiles in turn, each with a K and a V buffer that
-// no other wave sees and no barrier: while a wave works on K the V rows are on their way, and the next K's as soon as its last is
-// read.  Bound by reading the cache: of the matrix instructions' 32 columns a single token uses the query heads of its key head,
-// and they take an eighth of the time that the rows do.
+// Pieces of up to 32 rows, single tokens above all.  The four waves of a workgroup take its tiles in turn, in halves of 32 keys, each
+// with a K and a V buffer that no other wave sees and no barrier: while a wave works on K the V rows are on their way, and the next
+// K's as soon as its last is read.  Two workgroups share a compute unit, so that the one's start (its piece, table entries, first
+// rows) is behind the other's loads.  Bound by reading the cache: of the matrix instructions' 32 columns a single token uses the
+// query heads of its key head, and they take an eighth of the time that the rows do.
 template <int D>
 struct FewLds {
-    static constexpr int kMat = DnLds<D>::kMat, kWave = 2 * kMat, kTotal = 4 * kWave;
+    static constexpr int kMat = DnLds<D>::kMat / 2, kWave = 2 * kMat, kTotal = 4 * kWave;
 };
 
 template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
 template <class E, int D>
-__global__ __launch_bounds__(256) void paged_few_kernel(PagedArgs a, int64_t npieces, int chunks, int chunk_tiles, float* part) {
+__global__ __launch_bounds__(256, 2) void paged_few_kernel(PagedArgs a, int64_t npieces, int chunks, int chunk_tiles, float* part) {
     using L = DnLds<D>;
-    constexpr int kLoads = L::kCPR, kRows = 64 / L::kCPR, kVar = D == 128 ? 4 : 2;     // loads of a tile, rows of a load, column orders
+    constexpr int kRows = 64 / L::kCPR, kLoads = 32 / kRows, kVar = D == 128 ? 4 : 2;  // rows of a load, loads of half a tile, column orders
     extern __shared__ __attribute__((aligned(256))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) char*)lds, buf = (uint32_t)wave * FewLds<D>::kWave;
     const sfm_paged_desc& d = a.d;
-    // the heads of a token's row on one XCD, the pieces and ranges in turn on all of them: requests differ in length
-    const int ring = blockIdx.x / 8, kh = ring % d.kv_heads, rest = ring / d.kv_heads * 8 + blockIdx.x % 8;
+    // the heads of a token's row side by side
+    const int item = blockIdx.x, kh = item % d.kv_heads, rest = item / d.kv_heads;
     if (rest >= npieces * chunks) return;
     const int chunk = rest % chunks;
     Piece p;
@@ -486,13 +487,13 @@ __global__ __launch_bounds__(256) void paged_few_kernel(PagedArgs a, int64_t npi
     bool bad = p.k.beyond;
     const float sc2 = d.sm_scale * kLog2e;
 
-    const int n = v0 + wave < v1 ? (v1 - v0 - wave + 3) / 4 : 0;       // this wave's tiles: v0 + wave + 4 i
-    uint32_t off_lo = 0, off_hi = 0;                                    // lane: block lane % 8 of tile i with i % 8 = lane / 8
+    const int n = v0 + wave < v1 ? 2 * ((v1 - v0 - wave + 3) / 4) : 0; // this wave's halves: of tiles v0 + wave + 4 (i / 2)
+    uint32_t off_lo = 0, off_hi = 0;                                    // lane: block lane % 8 of the tile i / 2 with i / 2 % 8 = lane / 8
     int pos_of = kNoPos;
-    auto blocks = [&](int i0) {
-        const int i = i0 + (lane >> 3);
+    auto blocks = [&](int t0) {
+        const int t = t0 + (lane >> 3);
         uint32_t off8;
-        const int e = map.entry(i < n ? 8 * (v0 + wave + 4 * i) + (lane & 7) : kNoPos, &off8, &pos_of);
+        const int e = map.entry(2 * t < n ? 8 * (v0 + wave + 4 * t) + (lane & 7) : kNoPos, &off8, &pos_of);
         const int page = map.page(e);
         bad = bad || __builtin_amdgcn_ballot_w64(e >= 0 && page < 0) != 0;
         const int64_t off = map.offset(page, off8);
@@ -511,7 +512,7 @@ __global__ __launch_bounds__(256) void paged_few_kernel(PagedArgs a, int64_t npi
     auto stage = [&](const char* g, int i, uint32_t dst) {
 #pragma unroll
         for (int j = 0; j < kLoads; ++j) {
-            const int from = 8 * (i & 7) + j * kRows / 8;
+            const int from = 4 * (i & 15) + j * kRows / 8;
             const uint64_t off = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(off_hi, from) << 32 | (uint32_t)__builtin_amdgcn_readlane(off_lo, from);
             dn_load_lds16(g + off + (uint32_t)(j * kRows % 8) * row_bytes, voff[j % kVar], lds0 + dst + (uint32_t)j * 1024);
         }
@@ -522,18 +523,18 @@ __global__ __launch_bounds__(256) void paged_few_kernel(PagedArgs a, int64_t npi
         stage(vg, 0, buf + FewLds<D>::kMat);
     }
     for (int i = 0; i < n; ++i) {
-        int pos[8];
+        int pos[4];
 #pragma unroll
-        for (int b = 0; b < 8; ++b) pos[b] = __builtin_amdgcn_readlane(pos_of, 8 * (i & 7) + b);
+        for (int b = 0; b < 4; ++b) pos[b] = __builtin_amdgcn_readlane(pos_of, 4 * (i & 15) + b);
         const bool next = i + 1 < n;
-        const int v = v0 + wave + 4 * i;
+        const int v = v0 + wave + 4 * (i >> 1);
         const bool masked = v < p.k.fast0 || v >= p.k.fast1;
         wait_loads<kLoads>();                                          // K of this tile; V's are behind it
-        masked_tile<E, D>(lds, buf, buf + FewLds<D>::kMat, qb, sc2, st, mask, masked, pos,
+        masked_tile<E, D, 1>(lds, buf, buf + FewLds<D>::kMat, qb, sc2, st, mask, masked, pos,
             [&]() {
                 lds_wave_sync();                                       // K is read
                 if (next) {
-                    if (((i + 1) & 7) == 0) blocks(i + 1);
+                    if (((i + 1) & 15) == 0) blocks((i + 1) / 2);
                     stage(kg, i + 1, buf);
                 }
             },
@@ -674,19 +675,30 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     st.init();
     const float sc2 = d.sm_scale * kLog2e;
 
-    for (int done = 0; done < nf; done += RowsLds<D, NW>::kStretch) {
-        constexpr int NA = 2 * DS, NP = 4 * DT, kVA = 32 / NA, kVP = 32 / NP, kAhead = 3, kRing = kAhead + 1;
-        const int here = min(nf - done, RowsLds<D, NW>::kStretch);             // an even number of tiles
-        u32x2* const where = (u32x2*)(lds + RowsLds<D, NW>::kPlaces);
-        for (int b = tid; b < 8 * here; b += NTH) {
+    // the virtual tiles that are not whole come behind them: `before` of them from v0 on, the others behind the last whole one
+    const int before = nf > 0 ? f0 - v0 : v1 - v0, rest = v1 - v0 - nf;
+    auto tile_at = [&](int i) { return i < nf ? f0 + i : i - nf < before ? v0 + i - nf : v0 + i; };
+    u32x2* const where = (u32x2*)(lds + RowsLds<D, NW>::kPlaces);
+    // places of tiles [i0, i0 + n) in that order
+    auto fill = [&](int i0, int n) {
+        for (int b = tid; b < 8 * n; b += NTH) {
             uint32_t off8;
             int pos;
-            const int e = map.entry(8 * (f0 + done) + b, &off8, &pos), page = map.page(e);
+            const int e = map.entry(8 * tile_at(i0 + b / 8) + b % 8, &off8, &pos), page = map.page(e);
             bad = bad || (e >= 0 && page < 0);
             const uint64_t off = (uint64_t)map.offset(page, off8);
             where[b] = u32x2{(uint32_t)off, (uint32_t)(off >> 32)};
         }
         bad = __syncthreads_or(bad);
+    };
+    bool ready = false;                            // the first of the rest is on its way
+    for (int done = 0; done < nf; done += RowsLds<D, NW>::kStretch) {
+        constexpr int NA = 2 * DS, NP = 4 * DT, kVA = 32 / NA, kVP = 32 / NP, kAhead = 3, kRing = kAhead + 1;
+        const int here = min(nf - done, RowsLds<D, NW>::kStretch);             // an even number of tiles
+        // the last stretch takes as many of the rest with it as there is room for
+        const int filled = min(v1 - v0 - done, RowsLds<D, NW>::kStretch);
+        fill(done, filled);
+        ready = filled > here;
         auto look = [&](int n) { return where[8 * n + (lane & 7)]; };
         const uint32_t sA0 = (uint32_t)m * L::kPitch + (uint32_t)((hf ^ L::swz(m)) << 4);
         uint32_t trA[2];
@@ -718,7 +730,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         next = look(1);
         x = places(next.x, next.y, 0);                     // of tile n + 1 when tile n begins
         stage(kg, x, L::kK + L::kMat);
-        next = look(min(2, here - 1));                     // of tile n + 2
+        next = look(min(2, filled - 1));                   // of tile n + 2
         dn_wait_tiles();
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -745,11 +757,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
             f32x16* scur = sbuf[PAR];
             f32x16* snext = sbuf[PAR ^ 1];
             dn_wait_tiles();
-            if (has_next) stage(vg, x, L::kV + (uint32_t)(PAR ^ 1) * L::kMat);
-            if (kind == 2) {
+            if (has_next || ready) stage(vg, x, L::kV + (uint32_t)(PAR ^ 1) * L::kMat);
+            if (kind == 2 || (kind == 1 && ready)) {
                 x = places(next.x, next.y, 0);
                 stage(kg, x, L::kK + (uint32_t)PAR * L::kMat);
-                next = look(n + 3);                        // of the last step: a place behind the stretch's, not used
+                if (kind == 2) next = look(n + 3);         // of the last step: a place behind the stretch's, not used
             }
             float psum = 0.f;
             if (has_next) {
@@ -821,11 +833,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         st.mrun = mrun;
         st.lrun = lrun;
         st.seen = true;
-        lds_barrier();                             // the buffers are everybody's again
     }
 
-    // ---- tiles seen in part: virtual tiles before the whole ones and behind them
-    const int before = nf > 0 ? f0 - v0 : v1 - v0, rest = nf > 0 ? before + v1 - f0 - nf : before;
+    // ---- tiles seen in part
     if (rest > 0) {
         const int G = d.H / d.kv_heads, w0 = p.row0 + wave * 32, w1 = min(w0 + 31, p.row1 - 1);
         const bool idle = w0 >= p.row1;
@@ -833,31 +843,33 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         const int e0 = idle || !d.causal ? p.k.end_max : (int)min((int64_t)p.rq.past + w0 / G + 1, (int64_t)a.cap);
         const int e1 = idle || !d.causal ? p.k.end_max : (int)min((int64_t)p.rq.past + w1 / G + 1, (int64_t)a.cap);
         const int lo = d.window && e1 > d.window ? e1 - d.window : 0;
-        // lane l: block l % 8 of tile u with u % 8 = l / 8
-        uint32_t off_lo = 0, off_hi = 0;
-        int pos_of = kNoPos;
-        auto blocks = [&](int u0) {
-            const int u = u0 + (lane >> 3), v = v0 + (u < before ? u : u + nf);
-            uint32_t off8;
-            const int e = map.entry(u < rest ? 8 * v + (lane & 7) : kNoPos, &off8, &pos_of), page = map.page(e);
-            bad = bad || __builtin_amdgcn_ballot_w64(e >= 0 && page < 0) != 0;
-            const uint64_t off = (uint64_t)map.offset(page, off8);
-            off_lo = (uint32_t)off;
-            off_hi = (uint32_t)(off >> 32);
-        };
         const RowMask mask = row_mask(a, p, w0);
-        blocks(0);
-        stage(kg, places(off_lo, off_hi, 0), L::kK);
-        stage(vg, places(off_lo, off_hi, 0), L::kV);
+        // places: behind those of the last stretch's whole tiles, as far as they went with it
+        int base = ready ? (nf - 1) % RowsLds<D, NW>::kStretch + 1 : 0, held = ready ? min(rest, RowsLds<D, NW>::kStretch - base) : 0, first = 0;
         for (int u = 0; u < rest; ++u) {
+            if (u == first + held) {               // the next stretch of them; nothing is on its way, and everybody is done with the last
+                first = u;
+                base = 0;
+                held = min(rest - u, RowsLds<D, NW>::kStretch);
+                fill(nf + u, held);
+                const u32x2 w = where[lane & 7];
+                const Places x = places(w.x, w.y, 0);
+                stage(kg, x, L::kK + (uint32_t)(u & 1) * L::kMat);
+                stage(vg, x, L::kV + (uint32_t)(u & 1) * L::kMat);
+            }
             int pos[8];
+            {
+                uint32_t off8;
+                int mine;
+                map.entry(8 * tile_at(nf + u) + (lane & 7), &off8, &mine);
 #pragma unroll
-            for (int b = 0; b < 8; ++b) pos[b] = __builtin_amdgcn_readlane(pos_of, 8 * (u & 7) + b);
+                for (int b = 0; b < 8; ++b) pos[b] = __builtin_amdgcn_readlane(mine, b);
+            }
             const uint32_t buf = (uint32_t)(u & 1) * L::kMat, other = (uint32_t)(~u & 1) * L::kMat;
             dn_wait_tiles();
-            if (u + 1 < rest) {
-                if (((u + 1) & 7) == 0) blocks(u + 1);
-                const Places x = places(off_lo, off_hi, 8 * ((u + 1) & 7));
+            if (u + 1 < first + held) {
+                const u32x2 w = where[8 * (base + u + 1 - first) + (lane & 7)];
+                const Places x = places(w.x, w.y, 0);
                 stage(kg, x, L::kK + other);
                 stage(vg, x, L::kV + other);
             }
@@ -867,7 +879,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
                 some = some || pos[b] < e1;
                 all = all && pos[b] < e0 - 7 && (pos[b] >= lo || pos[b] + 7 < d.sink);
             }
-            if (!idle && some) masked_tile<E, D>(lds, L::kK + buf, L::kV + buf, qb, sc2, st, mask, !all, pos, [] {}, [] {});
+            if (!idle && some) masked_tile<E, D, 2>(lds, L::kK + buf, L::kV + buf, qb, sc2, st, mask, !all, pos, [] {}, [] {});
         }
     }
     __syncthreads();                               // the tiles are dead: rows leave through LDS
@@ -887,12 +899,14 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a, const flo
     if (!d.zero_rest && t >= clamp_int(a.q_start[d.requests], 0, (int)d.tokens)) return;       // rows of nobody
     const float* const ml = part + chunks * rows * D + row * 2;
     float M = -__FLT_MAX__, sum = 0.f;
+#pragma unroll 4
     for (int c = 0; c < chunks; ++c) M = ml[c * rows * 2 + 1] == 0.f ? M : fmaxf(M, ml[c * rows * 2]);
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     bool seen = false;
+#pragma unroll 4
     for (int c = 0; c < chunks; ++c) {
         const float l = ml[c * rows * 2 + 1];
-        if (l == 0.f) continue;
+        if (l == 0.f) continue;                    // nothing was seen, nor written
         seen = true;
         const float f = fast_exp2(ml[c * rows * 2] - M);
         sum += f * l;
@@ -917,19 +931,26 @@ static PagedPlan paged_plan(const sfm_paged_desc& d) {
     // rows of a request (of a group of tokens) and key head, on average, and pieces that have rows
     const int64_t mean = std::max<int64_t>(1, d.top ? std::min<int64_t>(d.group, d.tokens) * G : d.tokens * G / d.requests);
     const int64_t units = d.top ? (d.tokens + d.group - 1) / d.group : std::min<int64_t>(d.requests, d.tokens);
+    // 256 rows a workgroup read every tile once per compute unit, 128 twice, with two of them on it: 4 to 7 % slower where both fill
+    // the chip (4680 x 32760 of 12 heads 937 us and 988), but workgroups of 128 rows fill it better: taken where those of 256 would
+    // leave an eighth of it idle in their last round (four requests of 1024 tokens on 15000, 16 heads on 4: 856 us and 712)
+    auto wide = [&](int64_t n) {
+        const double rounds = n * 1.03 / cu;
+        return mean > 128 && (int64_t)rounds + 1 < 1.15 * rounds;
+    };
     auto items = [&](int64_t rows) { return units * ((mean + rows - 1) / rows) * d.kv_heads; };
-    p.rows = mean <= 32 ? 32 : mean <= 128 || items(256) < cu / 2 ? 128 : 256;
+    p.rows = mean <= 32 ? 32 : wide(items(256)) ? 256 : 128;
     p.pieces = d.top ? pieces(d.tokens, d.group, d.requests) * ((d.group * G + p.rows - 1) / p.rows) : pieces(d.tokens * G, p.rows, d.requests);
     const int64_t cap = (int64_t)d.width * d.page_size, tiles = ((d.top ? (int64_t)d.top * d.page_size : cap) + 63) / 64, n = items(p.rows);
     int64_t chunks = 1;
     if (p.rows == 32) {
-        chunks = std::min<int64_t>((4 * cu + n - 1) / n, (tiles + 7) / 8);
+        chunks = std::min<int64_t>((8 * cu + n - 1) / n, (tiles + 7) / 8);
     } else if (tiles >= 16) {
-        const bool wide = p.rows == 256;
+        const bool broad = p.rows == 256;
         const double scale = d.D == 64 ? 0.6 : 1.0, partial_ns = (double)d.H * d.tokens * (d.D + 2) * 8 / 3500;
         double t1 = 0, best = 0;
-        for (int64_t s = 1; s <= 64 && s <= tiles / 4 && (s == 1 || n * s <= cu * (wide ? 1 : 2)); ++s) {
-            const double tile_ns = wide ? (n * s <= cu / 2 ? 1460 : 1830) : (n * s <= cu ? 1100 : 1900);
+        for (int64_t s = 1; s <= 64 && s <= tiles / 4 && (s == 1 || n * s <= cu * (broad ? 1 : 2)); ++s) {
+            const double tile_ns = broad ? (n * s <= cu / 2 ? 1460 : 1830) : (n * s <= cu ? 1100 : 1900);
             double t = 5000 + (double)((tiles + s - 1) / s) * tile_ns * scale;
             if (s == 1) t1 = best = t;
             else t += 6000 + s * partial_ns;
@@ -971,8 +992,7 @@ static int launch_mfma(const PagedArgs& a, PagedPlan p, float* part, hipStream_t
             set_error("hipFuncSetAttribute failed: %s", hipGetErrorString(e));
             return SFM_ERR_HIP;
         }
-        const int64_t grid = p.rows == 32 ? (p.pieces * p.chunks + 7) / 8 * 8 * d.kv_heads : xcd_grid((int)total);
-        hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * nw), lds, stream, a, p.pieces, p.chunks, p.chunk_tiles, part);
+        hipLaunchKernelGGL(kern, dim3(xcd_grid((int)total)), dim3(64 * nw), lds, stream, a, p.pieces, p.chunks, p.chunk_tiles, part);
         return SFM_OK;
     };
     const int rc = p.rows == 32 ? go(paged_few_kernel<E, D>, 4, FewLds<D>::kTotal + 4 * 96 * sizeof(float))
