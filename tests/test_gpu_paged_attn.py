@@ -405,3 +405,81 @@ def test_pools_past_four_gib(D, n):
     q = randn((T, 2 * Hk, D), 9, torch.bfloat16)
     got, lse = PA.paged_attention(q.to(DEV), kp, vp, far, causal=True, return_lse=True)
     close(got.cpu(), lse.cpu(), oracle.attention(q, wk, wv, table, torch.tensor(past), q_start, causal=True), torch.bfloat16)
+
+
+# ---------------------------------------------------------------- long contexts, against the definition in 64 bits on the GPU
+def long_inputs(past, n, page, H, Hk, D, dtype, seed=0):
+    """Pools on the GPU whose pages lie in no order."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    whole = [-(-(p + m) // page) for p, m in zip(past, n)]
+    pages = sum(whole) + 3
+    order = torch.randperm(pages, generator=g, device=DEV).to(torch.int32)
+    table, at = torch.full((len(past), max(whole)), -1, dtype=torch.int32, device=DEV), 0
+    for r, w in enumerate(whole):
+        table[r, :w] = order[at:at + w]
+        at += w
+    held = table.clone()
+    for r, p in enumerate(past):
+        held[r, -(-p // page):] = -1
+    free = torch.cat([table[r, -(-p // page):w] for r, (p, w) in enumerate(zip(past, whole))] + [order[at:]])
+    plan = PA.plan_pages(held, ints(past), ints(n), free, sum(n), page)
+    assert torch.equal(plan.table, table)
+    kp, vp = (torch.randn((pages, page, Hk, D), generator=g, device=DEV, dtype=torch.float32).to(dtype) for _ in range(2))
+    return plan, torch.randn((sum(n), H, D), generator=g, device=DEV).to(dtype), kp, vp
+
+
+def check_rows(got, lse, plan, q, kp, vp, past, n, tokens, causal, window=None, sink=0, selected=None, group=1):
+    """A few tokens of the output, all heads, within the bound of `close`."""
+    page, Hk, D = kp.shape[1:]
+    G, want, start = q.shape[1] // Hk, [], 0
+    for r, (p, m) in enumerate(zip(past, n)):
+        for t in [t - start for t in tokens if start <= t < start + m]:
+            end = p + t + 1 if causal else p + m
+            pos = torch.arange(end, device=DEV)
+            if window is not None:
+                pos = pos[(pos >= end - window) | (pos < sink)]
+            rows = plan.table[r].long()[pos // page] * page + pos % page
+            k, v = (x.view(-1, Hk, D)[rows].double() for x in (kp, vp))
+            x = torch.einsum("hgd,khd->hgk", q[start + t].double().view(Hk, G, D).cpu(), k.cpu()).to(DEV) * D ** -0.5
+            if selected is not None:
+                e = selected[start // group + r + t // group].long()
+                seen = (e[:, :, None] == (pos // page)[None, None]).any(1)
+                x = x.masked_fill(~seen[:, None], -math.inf)
+            l = torch.logsumexp(x, -1)
+            w = torch.exp(x - l[..., None])
+            y = torch.stack([w[h] @ v[:, h] for h in range(Hk)]).view(-1, D)
+            mag = torch.stack([w[h] @ v[:, h].abs() for h in range(Hk)]).view(-1, D)
+            mass = torch.einsum("hgd,khd->hgk", q[start + t].double().abs().view(Hk, G, D).cpu(), k.abs().cpu()).to(DEV).amax(-1) * D ** -0.5
+            fin = torch.where(x.isfinite(), x, 0.0)
+            slip = (mass * (D + 4) + fin.abs().amax(-1) * 4 + 16).view(-1)
+            want.append((start + t, y, l.view(-1), mag, slip, len(pos), v.abs().amax()))
+        start += m
+    t = torch.tensor([w[0] for w in want], device=DEV)
+    ref = dict(out=torch.stack([w[1] for w in want]), lse=torch.stack([w[2] for w in want]).T, mag=torch.stack([w[3] for w in want]),
+               slip=torch.stack([w[4] for w in want]), keys=torch.tensor([[w[5]] * q.shape[1] for w in want], device=DEV),
+               top=torch.stack([w[6].expand(q.shape[1]) for w in want]))
+    ref["bad"] = torch.zeros_like(ref["slip"], dtype=torch.bool)
+    close(got[t].cpu(), lse[:, t].cpu(), {k: v.cpu() for k, v in ref.items()}, q.dtype)
+
+
+@pytest.mark.parametrize("past,n,page,H,Hk,D,causal,window,sink", [
+    ([40000], [1], 64, 8, 2, 128, True, None, 0), ([33000, 70, 16000], [1, 1, 1], 8, 4, 4, 64, True, None, 0),
+    ([18000], [2048], 16, 16, 16, 64, True, None, 0), ([16500], [2048], 64, 16, 16, 128, False, None, 0),
+    ([34000], [3700], 1560, 16, 16, 64, False, None, 0), ([33000], [3700], 32, 16, 16, 128, True, None, 0),
+    ([18000], [2048], 16, 16, 16, 64, True, 100, 17000), ([34000], [3700], 64, 16, 16, 64, True, 2000, 33000), ([20000, 19000], [40, 2], 40, 12, 2, 128, True, 5000, 64),
+])
+def test_long_contexts(past, n, page, H, Hk, D, causal, window, sink):
+    plan, q, kp, vp = long_inputs(past, n, page, H, Hk, D, torch.bfloat16)
+    got, lse = PA.paged_attention(q, kp, vp, plan, causal=causal, window=window, sink=sink, return_lse=True)
+    T = sum(n)
+    tokens = sorted({0, 1, T // 3, T // 2, T - 2, T - 1} & set(range(T)))
+    check_rows(got, lse, plan, q, kp, vp, past, n, tokens, causal, window, sink)
+
+
+def test_long_contexts_selected():
+    past, n, page, group, top = [30000], [1024], 64, 128, 300
+    plan, q, kp, vp = long_inputs(past, n, page, 16, 16, 64, torch.bfloat16)
+    means = kp.float().mean(1)
+    sel = PA.select_pages(q, means, plan, top, group=group, causal=True)
+    got, lse = PA.paged_attention(q, kp, vp, plan, causal=True, selected=sel, group=group, return_lse=True)
+    check_rows(got, lse, plan, q, kp, vp, past, n, [0, 127, 128, 700, 1023], True, selected=sel, group=group)
