@@ -18,6 +18,7 @@ Lengths, tables and lists of free pages stay on the GPU: nothing here waits for 
 they hold cannot be refused, then: no number in them makes a kernel leave its tensors, and each function says what comes of
 numbers that make no sense.  Nothing here is differentiable."""
 import ctypes as C
+import functools
 import math
 from typing import NamedTuple
 
@@ -64,6 +65,13 @@ def _table(t):
     return R, W, t.stride(0) if R > 1 else W
 
 
+@functools.lru_cache(maxsize=1024)
+def _plan_bytes(requests):
+    n = C.c_size_t(0)
+    _l.check(_l.load().sfm_paged_plan_workspace_bytes(requests, C.byref(n)))
+    return n.value
+
+
 def plan_pages(table, past, new, free, tokens, page_size, next_free=None):
     """Block table, slots and row offsets of a step, on the GPU in one launch.
 
@@ -84,17 +92,15 @@ def plan_pages(table, past, new, free, tokens, page_size, next_free=None):
     if tokens < 0:
         raise ValueError("tokens must not be negative")
     slots = torch.empty(tokens, dtype=torch.int64, device=dev)
-    ints = torch.empty(2 * R + 2, dtype=torch.int32, device=dev)           # one allocation: q_start, lengths, next_free
-    q_start, lengths, taken = ints[:R + 1], ints[R + 1:2 * R + 1], ints[2 * R + 1:]
-    n = C.c_size_t(0)
-    lib = _l.load()
+    q_start, lengths, taken = torch.empty(2 * R + 2, dtype=torch.int32, device=dev).split_with_sizes((R + 1, R, 1))
+    nbytes = _plan_bytes(R)
     with _on_device(dev):
-        _l.check(lib.sfm_paged_plan_workspace_bytes(R, C.byref(n)))
-        ws = torch.empty(n.value, dtype=torch.uint8, device=dev) if n.value else None
-        _l.check(lib.sfm_paged_plan(R, W, page_size, tokens, table.data_ptr(), ts, past.data_ptr(), new.data_ptr(), free.data_ptr(), free.shape[0],
-                                    None if next_free is None else next_free.data_ptr(), q_start.data_ptr(), lengths.data_ptr(),
-                                    slots.data_ptr(), taken.data_ptr(), None if ws is None else ws.data_ptr(), n.value,
-                                    _raw_stream(dev.index)))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        rc = _l.load().sfm_paged_plan(R, W, page_size, tokens, table.data_ptr(), ts, past.data_ptr(), new.data_ptr(), free.data_ptr(), free.shape[0],
+                                      None if next_free is None else next_free.data_ptr(), q_start.data_ptr(), lengths.data_ptr(),
+                                      slots.data_ptr(), taken.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, _raw_stream(dev.index))
+    if rc:
+        _l.check(rc)
     _written(table)
     return PagePlan(table, past, lengths, q_start, slots, taken, page_size)
 
@@ -122,13 +128,14 @@ def _pools(k_pages, v_pages, page_size):
         raise ValueError("k_pages and v_pages must agree in shape, dtype and device")
     if k_pages.dtype not in _DT:
         raise ValueError(f"unsupported dtype {k_pages.dtype}")
-    N, P, H, D = k_pages.shape
-    if P != page_size:
-        raise ValueError(f"the pools' pages have {P} rows, the plan's {page_size}")
-    s = [_pool_strides(t) for t in (k_pages, v_pages)]
-    if s[0] != s[1]:
-        raise ValueError("k_pages and v_pages must share strides")
-    return s[0]
+    if k_pages.shape[1] != page_size:
+        raise ValueError(f"the pools' pages have {k_pages.shape[1]} rows, the plan's {page_size}")
+    s = k_pages.stride()
+    if s != v_pages.stride() or s[3] != 1 or 1 in k_pages.shape:           # a dimension of one may have any stride
+        s = _pool_strides(k_pages)
+        if s != _pool_strides(v_pages):
+            raise ValueError("k_pages and v_pages must share strides")
+    return s[:3]
 
 
 def _pool_strides(t):
@@ -148,7 +155,7 @@ def _plan(plan, tokens, device):
     if plan.table.device != device:
         raise ValueError(f"the plan is on {plan.table.device}, the tensors on {device}")
     for name, t, n, dt in (("past", plan.past, R, torch.int32), ("q_start", plan.q_start, R + 1, torch.int32), ("slots", plan.slots, tokens, torch.int64)):
-        if t.dtype != dt or t.dim() != 1 or t.shape[0] != n or t.device != device or (n > 1 and t.stride(0) != 1):
+        if t.shape != (n,) or t.dtype != dt or t.device != device or not t.is_contiguous():
             raise ValueError(f"the plan's {name} must be {n} contiguous {dt} on {device}")
     return R, W, ts
 
@@ -189,11 +196,11 @@ def write_pages(k, v, k_pages, v_pages, plan, means=None):
         _written(means)
 
 
-def _q_desc(q, kv_heads, plan, pages, pool, out, sm_scale, causal, window, sink, top, group, zero_rest):
+def _q_desc(q, qs, kv_heads, plan, pages, pool, out, sm_scale, causal, window, sink, top, group, zero_rest):
     T, H, D = q.shape
     R, W, ts = _plan(plan, T, q.device)
-    return _l.PagedDesc(_DT[q.dtype], H, kv_heads, D, T, R, W, pages, plan.page_size, ts, pool, _rows("q", q, q.dtype, q.device), out, sm_scale,
-                        causal, window, sink, top, group, zero_rest)
+    return _l.PagedDesc(_DT[q.dtype], H, kv_heads, D, T, R, W, pages, plan.page_size, ts, pool, qs, out, sm_scale, causal, window, sink, top, group,
+                        zero_rest)
 
 
 def selected_rows(tokens, requests, group):
@@ -221,9 +228,9 @@ def paged_attention(q, k_pages, v_pages, plan, sm_scale=None, causal=False, wind
     ps = _pools(k_pages, v_pages, getattr(plan, "page_size", None))
     N, P, Hk, D = k_pages.shape
     dev = k_pages.device
-    _rows("q", q, k_pages.dtype, dev)
-    T, H = q.shape[:2]
-    if q.shape[2] != D or H < Hk or H % Hk:
+    qs = _rows("q", q, k_pages.dtype, dev)
+    T, H, qd = q.shape
+    if qd != D or H < Hk or H % Hk:
         raise ValueError("q must be [tokens, heads, head_dim], heads a multiple of the pools' and head_dim theirs")
     if window is not None and window < 1:
         raise ValueError("window must be a position or more (None: all)")
@@ -251,7 +258,7 @@ def paged_attention(q, k_pages, v_pages, plan, sm_scale=None, causal=False, wind
     if T == 0:
         _plan(plan, 0, dev)
         return (out, lse) if return_lse else out
-    d = _q_desc(q, Hk, plan, N, ps, _rows("out", out, q.dtype, dev), float(D ** -0.5 if sm_scale is None else sm_scale), bool(causal),
+    d = _q_desc(q, qs, Hk, plan, N, ps, (H * D, D) if zero_rest else _rows("out", out, q.dtype, dev), float(D ** -0.5 if sm_scale is None else sm_scale), bool(causal),
                 window or 0, sink, top, group, zero_rest)
     n = C.c_size_t(0)
     lib = _l.load()
@@ -280,7 +287,7 @@ def select_pages(q, means, plan, top, group=1, causal=False, first=1, last=1):
         raise NotImplementedError("select_pages is not differentiable")
     if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dtype not in _DT:
         raise ValueError("q must be a [tokens, heads, head_dim] GPU tensor of bf16, fp16 or fp32")
-    _rows("q", q, q.dtype, q.device)
+    qs = _rows("q", q, q.dtype, q.device)
     T, H, D = q.shape
     if means.dim() != 3 or means.dtype != torch.float32 or means.device != q.device or not means.is_contiguous() or means.shape[2] != D:
         raise ValueError("means must be a contiguous float32 [pages, kv_heads, head_dim] tensor on q's device")
@@ -295,7 +302,7 @@ def select_pages(q, means, plan, top, group=1, causal=False, first=1, last=1):
     selected = torch.empty((selected_rows(T, R, group), Hk, top), dtype=torch.int32, device=q.device)
     if T == 0:
         return selected.fill_(-1)
-    d = _q_desc(q, Hk, plan, N, (0, 0, 0), (0, 0), 1.0, bool(causal), 0, 0, top, group, 0)
+    d = _q_desc(q, qs, Hk, plan, N, (0, 0, 0), (0, 0), 1.0, bool(causal), 0, 0, top, group, 0)
     n = C.c_size_t(0)
     lib = _l.load()
     with _on_device(q.device):
