@@ -158,7 +158,7 @@ int launch_paged_plan(int R, int W, int page_size, int64_t T, int32_t* table, in
     PlanArgs a{R, W, fast_div(page_size / 8), T, table_stride, free_count, table, past, fresh, free_pages, taken, q_start, lengths, next_free, slots,
                (int32_t*)workspace, (int32_t*)workspace + R + 1};
     const int64_t items = T > R + 1 ? T : R + 1;
-    auto wgs = [&](int threads) { return dim3((unsigned)std::min<int64_t>(std::max<int64_t>((items + 4 * threads - 1) / (4 * threads), 1), 1024)); };
+    auto wgs = [&](int threads) { return dim3((unsigned)std::min<int64_t>(std::max<int64_t>((items + threads - 1) / threads, 1), 1024)); };
     const size_t lds = 2 * ((size_t)R + 1) * sizeof(int32_t);
     if (R <= 1024) {
         hipLaunchKernelGGL(paged_plan_kernel<256>, wgs(256), dim3(256), lds, stream, a);
@@ -335,17 +335,33 @@ __device__ __forceinline__ uint64_t select_key(double s) {
 struct SelectRow {
     int r, n, candidates;          // entries of the table's row that the last token sees
     int64_t t0, pages;             // first token; candidates, had the table room for them
+    int left;                      // tokens of the request from t0 on
+    int64_t end;                   // positions up to the first of them
 };
+__device__ __forceinline__ void select_pages_of(const SelectArgs& s, SelectRow& x) {
+    x.n = min(x.left, s.d.group);
+    x.pages = (x.end + (s.d.causal ? x.n : x.left) + s.d.page_size - 1) / s.d.page_size;
+    x.candidates = x.n ? (int)min(x.pages, (int64_t)s.d.width) : 0;
+}
 __device__ __forceinline__ SelectRow select_row(const SelectArgs& s, int row) {
     const sfm_paged_desc& d = s.d;
     SelectRow x;
     x.r = find_last(d.requests, row, [&](int i) { return first_piece(clamp_int(s.q_start[i], 0, (int)d.tokens), 1, d.group, i); });
     const Request rq = request_of(s.q_start, s.past, x.r, d.requests, (int)d.tokens);
     const int64_t t0 = (row - first_piece(rq.first, 1, d.group, x.r)) * d.group;
-    x.n = x.r < d.requests && t0 >= 0 && t0 < rq.n ? (int)min((int64_t)d.group, rq.n - t0) : 0;
+    x.left = x.r < d.requests && t0 >= 0 && t0 < rq.n ? (int)(rq.n - t0) : 0;
     x.t0 = rq.first + t0;
-    x.pages = ((int64_t)rq.past + (d.causal ? t0 + x.n : rq.n) + d.page_size - 1) / d.page_size;
-    x.candidates = x.n ? (int)min(x.pages, (int64_t)d.width) : 0;
+    x.end = (int64_t)rq.past + t0;
+    select_pages_of(s, x);
+    return x;
+}
+// the i-th group after it, of the same request
+__device__ __forceinline__ SelectRow select_row_behind(const SelectArgs& s, SelectRow x, int i) {
+    const int64_t by = (int64_t)i * s.d.group;
+    x.left = by < x.left ? (int)(x.left - by) : 0;
+    x.t0 += by;
+    x.end += by;
+    select_pages_of(s, x);
     return x;
 }
 
@@ -407,8 +423,8 @@ __global__ __launch_bounds__(256) void paged_score_kernel(SelectArgs s) {
         SelectRow last = x;
         int most = x.candidates > d.top ? x.candidates : 0;
         while (RT > 1 && row + count < end) {
-            const SelectRow y = select_row(s, row + count);
-            if (y.r != x.r || !y.n) break;
+            const SelectRow y = select_row_behind(s, x, count);
+            if (!y.n) break;
             last = y;
             most = max(most, y.candidates > d.top ? y.candidates : 0);
             ++count;
@@ -508,9 +524,9 @@ __global__ __launch_bounds__(256) void paged_select_kernel(SelectArgs s) {
             continue;
         }
         // the top-th largest key: digits from the highest, `need` of those that agree so far
-        uint64_t prefix = 0;
         int need = d.top;
         bool whole = false;                                        // all that agree are taken: no level ones to tell apart
+        uint64_t prefix = 0;
         int shift = 56;
         for (; shift >= 0; shift -= 8) {
             hist[tid] = 0;
