@@ -354,17 +354,16 @@ __device__ __forceinline__ bool find_piece(const PagedArgs& a, int64_t piece, in
     const int R = d.requests, T = (int)d.tokens, G = d.H / d.kv_heads;
     int64_t per = M, heads = G, j = 0, unit = piece;
     if (d.top) {                   // groups, each in pieces of M rows
-        const int64_t each = ((int64_t)d.group * G + M - 1) / M;
+        const int64_t each = ((int64_t)min(d.group, T) * G + M - 1) / M;
         unit = piece / each;
         j = piece - unit * each;
         per = d.group;
         heads = 1;
     }
-    const int r = find_last(R, unit, [&](int i) { return first_piece(clamp_int(a.q_start[i], 0, T), heads, per, i); });
+    const int r = find_request(a.q_start, a.past, R, T, unit, heads, per, &p->rq);
     if (r >= R && !d.zero_rest) return false;
     p->r = r;
     p->kh = kh;
-    p->rq = request_of(a.q_start, a.past, r, R, T);
     const int64_t nth = unit - first_piece(p->rq.first, heads, per, r), rows = (int64_t)p->rq.n * G;
     int64_t row0 = nth * M, last = rows;
     if (d.top) {
@@ -424,7 +423,8 @@ __device__ __forceinline__ BlockMap block_map(const PagedArgs& a, const Piece& p
     return b;
 }
 
-// Operands of the rows row0 .. + 31 (those past the piece repeat its last)
+// Operands of the rows row0 .. + 31 (those past the piece repeat its last): asked for here, in front of the table's entries, and waited for
+// behind those (wait_queries), before any tile is
 template <class E, int D>
 __device__ __forceinline__ void load_queries(const PagedArgs& a, const Piece& p, int row0, u32x4* qb) {
     const sfm_paged_desc& d = a.d;
@@ -433,8 +433,12 @@ __device__ __forceinline__ void load_queries(const PagedArgs& a, const Piece& p,
     const uint16_t* const q = (const uint16_t*)a.q + (int64_t)(p.rq.first + t) * d.q_stride[0] + (int64_t)(p.kh * G + row - t * G) * d.q_stride[1] + 8 * hf;
 #pragma unroll
     for (int ds = 0; ds < D / 16; ++ds) qb[ds] = *(const u32x4*)(q + 16 * ds);
+    asm volatile("" ::: "memory");
+}
+template <int D>
+__device__ __forceinline__ void wait_queries(u32x4* qb) {
 #pragma unroll
-    for (int ds = 0; ds < D / 16; ++ds) asm volatile("" : "+v"(qb[ds]));      // loaded before any tile is awaited
+    for (int ds = 0; ds < D / 16; ++ds) asm volatile("" : "+v"(qb[ds]));
 }
 
 // What each of them sees
@@ -519,6 +523,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(PagedArgs a, int64_t 
     };
     if (n > 0) {
         blocks(0);
+        wait_queries<D>(qb);
         stage(kg, 0, buf);
         stage(vg, 0, buf + FewLds<D>::kMat);
     }
@@ -690,6 +695,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
             where[b] = u32x2{(uint32_t)off, (uint32_t)(off >> 32)};
         }
         bad = __syncthreads_or(bad);
+        wait_queries<D>(qb);
     };
     bool ready = false;                            // the first of the rest is on its way
     for (int done = 0; done < nf; done += RowsLds<D, NW>::kStretch) {
@@ -940,7 +946,7 @@ static PagedPlan paged_plan(const sfm_paged_desc& d) {
     };
     auto items = [&](int64_t rows) { return units * ((mean + rows - 1) / rows) * d.kv_heads; };
     p.rows = mean <= 32 ? 32 : wide(items(256)) ? 256 : 128;
-    p.pieces = d.top ? pieces(d.tokens, d.group, d.requests) * ((d.group * G + p.rows - 1) / p.rows) : pieces(d.tokens * G, p.rows, d.requests);
+    p.pieces = d.top ? pieces(d.tokens, d.group, d.requests) * ((std::min<int64_t>(d.group, d.tokens) * G + p.rows - 1) / p.rows) : pieces(d.tokens * G, p.rows, d.requests);
     const int64_t cap = (int64_t)d.width * d.page_size, tiles = ((d.top ? (int64_t)d.top * d.page_size : cap) + 63) / 64, n = items(p.rows);
     int64_t chunks = 1;
     if (p.rows == 32) {

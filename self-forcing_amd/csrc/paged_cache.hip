@@ -346,8 +346,8 @@ __device__ __forceinline__ void select_pages_of(const SelectArgs& s, SelectRow& 
 __device__ __forceinline__ SelectRow select_row(const SelectArgs& s, int row) {
     const sfm_paged_desc& d = s.d;
     SelectRow x;
-    x.r = find_last(d.requests, row, [&](int i) { return first_piece(clamp_int(s.q_start[i], 0, (int)d.tokens), 1, d.group, i); });
-    const Request rq = request_of(s.q_start, s.past, x.r, d.requests, (int)d.tokens);
+    Request rq;
+    x.r = find_request(s.q_start, s.past, d.requests, (int)d.tokens, row, 1, d.group, &rq);
     const int64_t t0 = (row - first_piece(rq.first, 1, d.group, x.r)) * d.group;
     x.left = x.r < d.requests && t0 >= 0 && t0 < rq.n ? (int)(rq.n - t0) : 0;
     x.t0 = rq.first + t0;

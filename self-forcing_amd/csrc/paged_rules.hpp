@@ -130,6 +130,26 @@ __device__ __forceinline__ int find_last(int R, int64_t v, F at) {
     }
     return __builtin_amdgcn_readfirstlane(lo);
 }
+
+// The request that a piece of `per` of its rows belongs to (R: nobody's rows), and what find_last and request_of say of it.  Up to 63
+// requests are read at once, a lane each: one round to memory in place of two.
+__device__ __forceinline__ int find_request(const int32_t* q_start, const int32_t* past, int R, int T, int64_t piece, int64_t heads, int64_t per,
+                                            Request* q) {
+    if (R > 63) {
+        const int r = find_last(R, piece, [&](int i) { return first_piece(clamp_int(q_start[i], 0, T), heads, per, i); });
+        *q = request_of(q_start, past, r, R, T);
+        return r;
+    }
+    const int lane = threadIdx.x & 63;
+    const int mine = clamp_int(lane <= R ? q_start[lane] : T, 0, T), held = lane < R ? past[lane] : 0;
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(lane <= R && first_piece(mine, heads, per, lane) <= piece);
+    const int r = hit ? 63 - __builtin_clzll(hit) : 0;
+    q->first = __builtin_amdgcn_readlane(mine, r);
+    const int end = r < R ? __builtin_amdgcn_readlane(mine, r < 63 ? r + 1 : r) : T, had = __builtin_amdgcn_readlane(held, r);
+    q->n = end > q->first ? end - q->first : 0;
+    q->past = had > 0 ? had : 0;
+    return r;
+}
 #endif
 
 }  // namespace sfm

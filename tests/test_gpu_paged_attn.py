@@ -139,6 +139,74 @@ def test_selected_pages(past, n, page, H, Hk, group, top, causal, D):
     close(got.cpu(), lse.cpu(), oracle.attention(q, kp, vp, table, torch.tensor(past), q_start, causal=causal, selected=sel, group=group), torch.bfloat16)
 
 
+@pytest.mark.parametrize("group", [231, 1000, 2 ** 31 - 1])
+def test_groups_larger_than_the_step(group):
+    past, n, page = [300, 20], [100, 131], 16
+    plan, table, q_start, q, kp, vp = inputs(past, n, page, 4, 2, 64, torch.bfloat16)
+    means = kp.float().mean(1)
+    sel = PA.select_pages(q.to(DEV), means.to(DEV), plan, 6, group=group, causal=True)
+    assert torch.equal(sel.cpu().long(), oracle.select_pages(q, means, table, torch.tensor(past), q_start, page, 6, group, True))
+    got = PA.paged_attention(q.to(DEV), kp.to(DEV), vp.to(DEV), plan, causal=True, selected=sel, group=group)
+    close(got.cpu(), None, oracle.attention(q, kp, vp, table, torch.tensor(past), q_start, causal=True, selected=sel.cpu().long(), group=group), torch.bfloat16)
+
+
+@pytest.mark.parametrize("n", [[1, 1, 1], [40, 150, 3]])
+def test_requests_that_share_pages(n):
+    """A prompt's pages in the tables of several requests: read by all of them."""
+    past, page = [96, 100, 200], 16
+    plan, table, q_start, q, kp, vp = inputs(past, n, page, 4, 2, 128, torch.bfloat16)
+    table = table.clone()
+    table[1, :6] = table[2, :6] = table[0, :6]
+    got = PA.paged_attention(q.to(DEV), kp.to(DEV), vp.to(DEV), plan._replace(table=ints(table.tolist())), causal=True)
+    close(got.cpu(), None, oracle.attention(q, kp, vp, table, torch.tensor(past), q_start, causal=True), torch.bfloat16)
+
+
+def test_without_the_workspace_a_call_runs_whole():
+    """The C entry takes a NULL or too small workspace: the same result within the bound, in one range."""
+    import ctypes as C
+    past, n, page = [5000, 300], [1, 1], 16
+    plan, table, q_start, q, kp, vp = inputs(past, n, page, 4, 2, 128, torch.bfloat16)
+    dq, dk, dv = q.to(DEV), kp.to(DEV), vp.to(DEV)
+    out = torch.zeros_like(dq)
+    d = PA._q_desc(dq, (4 * 128, 128), 2, plan, dk.shape[0], dk.stride()[:3], (4 * 128, 128), 128 ** -0.5, True, 0, 0, 0, 1, 1)
+    size = C.c_size_t(0)
+    sfa.lib.check(sfa.lib.load().sfm_paged_workspace_bytes(C.byref(d), C.byref(size)))
+    assert size.value > 0
+    ws = torch.zeros(size.value - 1, dtype=torch.uint8, device=DEV)
+    want = oracle.attention(q, kp, vp, table, torch.tensor(past), q_start, causal=True)
+    for at, bytes_ in ((None, 0), (ws.data_ptr(), size.value - 1)):
+        sfa.lib.check(sfa.lib.load().sfm_paged_attention(C.byref(d), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), plan.table.data_ptr(), plan.past.data_ptr(),
+                                                         plan.q_start.data_ptr(), None, out.data_ptr(), None, at, bytes_,
+                                                         torch.cuda.current_stream().cuda_stream))
+        close(out.cpu(), None, want, torch.bfloat16)
+    assert not ws.any()
+
+
+def test_workspaces_have_the_size_that_is_asked_for():
+    import ctypes as C
+    lib = sfa.lib.load()
+    past, n, page = [5000, 300], [1, 1], 16
+    plan, table, q_start, q, kp, vp = inputs(past, n, page, 4, 2, 128, torch.bfloat16)
+    dq, dk, dv, means = q.to(DEV), kp.to(DEV), vp.to(DEV), kp.float().mean(1).to(DEV)
+    out, sel = torch.zeros_like(dq), torch.zeros((PA.selected_rows(2, 2, 1), 2, 7), dtype=torch.int32, device=DEV)
+    size, stream = C.c_size_t(0), torch.cuda.current_stream().cuda_stream
+
+    def canary():
+        return torch.full((size.value + 65536,), 0xA5, dtype=torch.uint8, device=DEV)
+    d = PA._q_desc(dq, (4 * 128, 128), 2, plan, dk.shape[0], dk.stride()[:3], (4 * 128, 128), 128 ** -0.5, True, 0, 0, 0, 1, 1)
+    sfa.lib.check(lib.sfm_paged_workspace_bytes(C.byref(d), C.byref(size)))
+    ws = canary()
+    sfa.lib.check(lib.sfm_paged_attention(C.byref(d), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), plan.table.data_ptr(), plan.past.data_ptr(),
+                                          plan.q_start.data_ptr(), None, out.data_ptr(), None, ws.data_ptr(), size.value, stream))
+    assert bool((ws[size.value:] == 0xA5).all()) and torch.equal(out, PA.paged_attention(dq, dk, dv, plan, causal=True))
+    d = PA._q_desc(dq, (4 * 128, 128), 2, plan, dk.shape[0], (0, 0, 0), (0, 0), 1.0, True, 0, 0, 7, 1, 0)
+    sfa.lib.check(lib.sfm_paged_select_workspace_bytes(C.byref(d), C.byref(size)))
+    ws = canary()
+    sfa.lib.check(lib.sfm_paged_select(C.byref(d), dq.data_ptr(), means.data_ptr(), plan.table.data_ptr(), plan.past.data_ptr(), plan.q_start.data_ptr(), 1, 1,
+                                       sel.data_ptr(), ws.data_ptr(), size.value, stream))
+    assert bool((ws[size.value:] == 0xA5).all()) and torch.equal(sel, PA.select_pages(dq, means, plan, 7, causal=True))
+
+
 def test_all_pages_selected_is_the_whole_attention():
     past, n, page = [300, 20], [100, 131], 16
     plan, table, q_start, q, kp, vp = inputs(past, n, page, 4, 2, 64, torch.bfloat16)
