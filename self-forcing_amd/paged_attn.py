@@ -25,7 +25,7 @@ from typing import NamedTuple
 import torch
 
 from . import lib as _l
-from .block_ops import _needs_grad, _written
+from .block_ops import _written
 from .monarch_attn import _DT, _KEPT, _drop_kept, _on_device, _raw_stream
 
 
@@ -51,18 +51,17 @@ def _ints(name, t, device, n=None, dtype=torch.int32):
     return t if t.stride(0) == 1 or t.shape[0] < 2 else t.contiguous()
 
 
-def _table(t):
-    """(rows, columns, row stride)"""
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != 2:
+def _table(layout):
+    """(rows, columns, row stride) of a block table's (dtype, shape, strides)."""
+    dt, shape, stride = layout
+    if dt != torch.int32 or len(shape) != 2:
         raise ValueError("table must be an int32 [requests, width] tensor")
-    if not t.is_cuda:
-        raise ValueError("the paged cache lives on the GPU")
-    R, W = t.shape
+    R, W = shape
     if R < 1 or W < 1:
         raise ValueError("table is empty")
-    if W > 1 and t.stride(1) != 1:
+    if W > 1 and stride[1] != 1:
         raise ValueError("table: a request's entries must be contiguous")
-    return R, W, t.stride(0) if R > 1 else W
+    return R, W, stride[0] if R > 1 else W
 
 
 @functools.lru_cache(maxsize=1024)
@@ -83,8 +82,11 @@ def plan_pages(table, past, new, free, tokens, page_size, next_free=None):
     Where the list runs out, or a request outgrows its row of the table, the tokens without a page get slot -1 (and the
     table's entries -1): write_pages passes them over and paged_attention gives NaN for rows that would read them.  Requests past `tokens`
     rows have as many tokens as fit.  Negative lengths count as 0."""
-    R, W, ts = _table(table)
+    if not isinstance(table, torch.Tensor):
+        raise ValueError("table must be an int32 [requests, width] tensor")
+    R, W, ts = _table(_layout(table))
     dev = table.device
+    _together(dev)
     past, new, free = _ints("past", past, dev, R), _ints("new", new, dev, R), _ints("free", free, dev)
     if next_free is not None:
         next_free = _ints("next_free", next_free, dev, 1)
@@ -105,59 +107,97 @@ def plan_pages(table, past, new, free, tokens, page_size, next_free=None):
     return PagePlan(table, past, lengths, q_start, slots, taken, page_size)
 
 
-def _rows(name, t, dtype, device):
-    """[tokens, heads, head_dim] rows -> (token stride, head stride); the stride of a dimension of one says nothing."""
-    if not isinstance(t, torch.Tensor) or t.dim() != 3:
+# What follows from the tensors' shapes, strides and types (their checks, the descriptor, workspace sizes) is worked out once for each set of
+# them: a single token's call is shorter than these steps.  A layout is (dtype, shape, strides); the stride of a dimension of one says
+# nothing.
+
+def _rows(name, layout, dtype):
+    """(token stride, head stride) of [tokens, heads, head_dim] rows."""
+    dt, shape, stride = layout
+    if len(shape) != 3:
         raise ValueError(f"{name} must be a [tokens, heads, head_dim] tensor")
-    if t.dtype != dtype or t.device != device:
-        raise ValueError(f"{name}: {t.dtype} on {t.device}, expected {dtype} on {device}")
-    T, H, D = t.shape
-    if D > 1 and t.stride(2) != 1:
+    if dt != dtype:
+        raise ValueError(f"{name}: {dt}, expected {dtype} like the pools")
+    T, H, D = shape
+    if D > 1 and stride[2] != 1:
         raise ValueError(f"{name}: head_dim must be contiguous")
-    hs = t.stride(1) if H > 1 else D
-    return t.stride(0) if T > 1 else H * hs, hs
+    hs = stride[1] if H > 1 else D
+    return stride[0] if T > 1 else H * hs, hs
+
+
+def _pool(name, layout):
+    """(page stride, token stride, head stride) of a [pages, page_size, kv_heads, head_dim] pool."""
+    dt, shape, stride = layout
+    if len(shape) != 4:
+        raise ValueError(f"{name} must be a [pages, page_size, kv_heads, head_dim] tensor")
+    if dt not in _DT:
+        raise ValueError(f"unsupported dtype {dt}")
+    N, P, H, D = shape
+    if D > 1 and stride[3] != 1:
+        raise ValueError(f"{name}: head_dim must be contiguous")
+    hs = stride[2] if H > 1 else D
+    ts = stride[1] if P > 1 else H * hs
+    return stride[0] if N > 1 else max(P * ts, P * D), ts, hs
 
 
 def _pools(k_pages, v_pages, page_size):
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if not isinstance(t, torch.Tensor) or t.dim() != 4:
-            raise ValueError(f"{name} must be a [pages, page_size, kv_heads, head_dim] tensor")
-        if not t.is_cuda:
-            raise ValueError("the paged cache lives on the GPU")
-    if v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype or v_pages.device != k_pages.device:
-        raise ValueError("k_pages and v_pages must agree in shape, dtype and device")
-    if k_pages.dtype not in _DT:
-        raise ValueError(f"unsupported dtype {k_pages.dtype}")
-    if k_pages.shape[1] != page_size:
-        raise ValueError(f"the pools' pages have {k_pages.shape[1]} rows, the plan's {page_size}")
-    s = k_pages.stride()
-    if s != v_pages.stride() or s[3] != 1 or 1 in k_pages.shape:           # a dimension of one may have any stride
-        s = _pool_strides(k_pages)
-        if s != _pool_strides(v_pages):
-            raise ValueError("k_pages and v_pages must share strides")
-    return s[:3]
+    ps = _pool("k_pages", k_pages)
+    if v_pages[:2] != k_pages[:2]:
+        raise ValueError("k_pages and v_pages must agree in shape and dtype")
+    if _pool("v_pages", v_pages) != ps:
+        raise ValueError("k_pages and v_pages must share strides")
+    if k_pages[1][1] != page_size:
+        raise ValueError(f"the pools' pages have {k_pages[1][1]} rows, the plan's {page_size}")
+    return ps
 
 
-def _pool_strides(t):
-    N, P, H, D = t.shape
-    if D > 1 and t.stride(3) != 1:
-        raise ValueError("the pools' head_dim must be contiguous")
-    hs = t.stride(2) if H > 1 else D
-    ts = t.stride(1) if P > 1 else H * hs
-    return t.stride(0) if N > 1 else max(P * ts, P * D), ts, hs
+def _planned(plan, tokens):
+    """(requests, width, table stride) of a plan's layout for tensors of so many rows."""
+    table, past, q_start, slots = plan
+    R, W, ts = _table(table)
+    for name, (dt, shape, stride), n, want in (("past", past, R, torch.int32), ("q_start", q_start, R + 1, torch.int32), ("slots", slots, tokens, torch.int64)):
+        if dt != want or tuple(shape) != (n,) or (n > 1 and stride[0] != 1):
+            raise ValueError(f"the plan's {name} must be {n} contiguous {want}")
+    return R, W, ts
 
 
-def _plan(plan, tokens, device):
-    """(requests, width, table stride) of a plan for tensors of so many rows."""
+def _layout(t):
+    return t.dtype, t.shape, t.stride()
+
+
+def _plan_layout(plan):
     if not isinstance(plan, PagePlan):
         raise ValueError("plan must be a PagePlan (plan_pages)")
-    R, W, ts = _table(plan.table)
-    if plan.table.device != device:
-        raise ValueError(f"the plan is on {plan.table.device}, the tensors on {device}")
-    for name, t, n, dt in (("past", plan.past, R, torch.int32), ("q_start", plan.q_start, R + 1, torch.int32), ("slots", plan.slots, tokens, torch.int64)):
-        if t.shape != (n,) or t.dtype != dt or t.device != device or not t.is_contiguous():
-            raise ValueError(f"the plan's {name} must be {n} contiguous {dt} on {device}")
-    return R, W, ts
+    return _layout(plan.table), _layout(plan.past), _layout(plan.q_start), _layout(plan.slots)
+
+
+def _together(device, *tensors):
+    """All on one GPU."""
+    if device.type != "cuda":
+        raise ValueError("the paged cache lives on the GPU")
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors on {t.device} and {device}")
+
+
+_I2 = C.c_int64 * 2
+
+
+@functools.lru_cache(maxsize=4096)
+def _write_call(k, v, k_pages, v_pages, page_size, plan, means):
+    """(descriptor, strides of k and v or None where they need a layout in common)."""
+    ps = _pools(k_pages, v_pages, page_size)
+    N, P, H, D = k_pages[1]
+    ks = _rows("k", k, k_pages[0])
+    if tuple(k[1][1:]) != (H, D):
+        raise ValueError("k must be [tokens, kv_heads, head_dim] of the pools' heads")
+    if v[1] != k[1]:
+        raise ValueError("k and v must have the same shape")
+    same = _rows("v", v, k_pages[0]) == ks
+    R, W, ts = _planned(plan, k[1][0])
+    if means is not None and (means[0] != torch.float32 or tuple(means[1]) != (N, H, D) or tuple(means[2]) != (H * D, D, 1)):
+        raise ValueError("means must be a contiguous float32 [pages, kv_heads, head_dim] tensor beside the pools")
+    return _l.PagedDesc(_DT[k[0]], H, H, D, k[1][0], R, W, N, P, ts, ps), _I2(*ks) if same else None
 
 
 def write_pages(k, v, k_pages, v_pages, plan, means=None):
@@ -165,47 +205,68 @@ def write_pages(k, v, k_pages, v_pages, plan, means=None):
     strides with a contiguous head_dim, pools alike.  With means (fp32 [pages, kv_heads, head_dim], in place): the mean key of every page that got a
     row, over the page's rows up to the request's length.  k and v must not lie in the pools; where a slot is named twice one of
     the rows stays in each 16 bytes."""
-    if _needs_grad(k, v):
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
         raise NotImplementedError("write_pages is not differentiable")
-    ps = _pools(k_pages, v_pages, getattr(plan, "page_size", None))
-    N, P, H, D = k_pages.shape
-    dev = k_pages.device
-    ks = _rows("k", k, k_pages.dtype, dev)
-    if k.shape[1:] != (H, D):
-        raise ValueError("k must be [tokens, kv_heads, head_dim] of the pools' heads")
-    if v.shape != k.shape or _rows("v", v, k.dtype, dev) != ks:
-        if v.shape != k.shape:
-            raise ValueError("k and v must have the same shape")
-        k, v = k.contiguous(), v.contiguous()
-        ks = _rows("k", k, k.dtype, dev)
-    R, W, ts = _plan(plan, k.shape[0], dev)
-    if means is not None and (means.dtype != torch.float32 or means.device != dev or means.shape != (N, H, D) or not means.is_contiguous()):
-        raise ValueError("means must be a contiguous float32 [pages, kv_heads, head_dim] tensor beside the pools")
+    dev, planned = k_pages.device, _plan_layout(plan)
+    _together(dev, k, v, v_pages, means, *plan[:5])
+    desc, ks = _write_call(_layout(k), _layout(v), _layout(k_pages), _layout(v_pages), plan.page_size, planned, None if means is None else _layout(means))
+    if ks is None:
+        return write_pages(k.contiguous(), v.contiguous(), k_pages, v_pages, plan, means)
     if k.shape[0] == 0:
         return
-    d = _l.PagedDesc(_DT[k.dtype], H, H, D, k.shape[0], R, W, N, P, ts, ps)
     if _KEPT:
         _drop_kept(dev.index)
     with _on_device(dev):
-        _l.check(_l.load().sfm_paged_write(C.byref(d), k.data_ptr(), v.data_ptr(), (C.c_int64 * 2)(*ks), k_pages.data_ptr(), v_pages.data_ptr(),
-                                           plan.slots.data_ptr(), plan.table.data_ptr(), plan.past.data_ptr(), plan.q_start.data_ptr(),
-                                           None if means is None else means.data_ptr(), _raw_stream(dev.index)))
+        rc = _l.load().sfm_paged_write(desc, k.data_ptr(), v.data_ptr(), ks, k_pages.data_ptr(), v_pages.data_ptr(), plan.slots.data_ptr(),
+                                       plan.table.data_ptr(), plan.past.data_ptr(), plan.q_start.data_ptr(),
+                                       None if means is None else means.data_ptr(), _raw_stream(dev.index))
+    if rc:
+        _l.check(rc)
     _written(k_pages)
     _written(v_pages)
     if means is not None:
         _written(means)
 
 
-def _q_desc(q, qs, kv_heads, plan, pages, pool, out, sm_scale, causal, window, sink, top, group, zero_rest):
-    T, H, D = q.shape
-    R, W, ts = _plan(plan, T, q.device)
-    return _l.PagedDesc(_DT[q.dtype], H, kv_heads, D, T, R, W, pages, plan.page_size, ts, pool, qs, out, sm_scale, causal, window, sink, top, group,
-                        zero_rest)
-
-
 def selected_rows(tokens, requests, group):
     """Rows of the lists that select_pages gives."""
     return tokens // group + requests + 1
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_call(device, q, k_pages, v_pages, page_size, plan, out, selected, sm_scale, causal, window, sink, group):
+    """(descriptor, workspace bytes on the device, whose compute units are in the size)."""
+    ps = _pools(k_pages, v_pages, page_size)
+    N, P, Hk, D = k_pages[1]
+    qs = _rows("q", q, k_pages[0])
+    T, H, qd = q[1]
+    if qd != D or H < Hk or H % Hk:
+        raise ValueError("q must be [tokens, heads, head_dim], heads a multiple of the pools' and head_dim theirs")
+    if window is not None and window < 1:
+        raise ValueError("window must be a position or more (None: all)")
+    if sink < 0 or (sink and window is None):
+        raise ValueError("sink: positions that stay visible outside a window")
+    R, W, ts = _planned(plan, T)
+    top = 0
+    if selected is not None:
+        if window is not None:
+            raise ValueError("selected pages and a window do not go together")
+        if group < 1:
+            raise ValueError("group must be a token or more")
+        rows, (dt, shape, stride) = selected_rows(T, R, group), selected
+        top = shape[2] if len(shape) == 3 else 0
+        if dt != torch.int32 or top < 1 or tuple(shape[:2]) != (rows, Hk) or tuple(stride) != (Hk * top, top, 1):
+            raise ValueError(f"selected must be a contiguous int32 [{rows}, {Hk}, top] tensor")
+    if out is not None and tuple(out[1]) != tuple(q[1]):
+        raise ValueError("out must be like q")
+    os = (H * D, D) if out is None else _rows("out", out, q[0])
+    desc = _l.PagedDesc(_DT[q[0]], H, Hk, D, T, R, W, N, P, ts, ps, qs, os, D ** -0.5 if sm_scale is None else sm_scale, causal, window or 0, sink,
+                        top, group, out is None)
+    n = C.c_size_t(0)
+    if T:
+        with torch.cuda.device(device):
+            _l.check(_l.load().sfm_paged_workspace_bytes(desc, C.byref(n)))
+    return desc, n.value
 
 
 def paged_attention(q, k_pages, v_pages, plan, sm_scale=None, causal=False, window=None, sink=0, selected=None, group=1, out=None,
@@ -223,55 +284,57 @@ def paged_attention(q, k_pages, v_pages, plan, sm_scale=None, causal=False, wind
     [heads, tokens], -inf for nothing.  Rows that would read a position without a page (-1 or another number outside the pool,
     positions past the table) are NaN, and others of their request may be.  What lies in positions that a row does not see has no part in it,
     NaN or infinite.  table[:, :n] of the columns in use sizes the work."""
-    if _needs_grad(q, k_pages, v_pages):
+    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad or (out is not None and out.requires_grad)):
         raise NotImplementedError("paged_attention is not differentiable")
-    ps = _pools(k_pages, v_pages, getattr(plan, "page_size", None))
-    N, P, Hk, D = k_pages.shape
-    dev = k_pages.device
-    qs = _rows("q", q, k_pages.dtype, dev)
-    T, H, qd = q.shape
-    if qd != D or H < Hk or H % Hk:
-        raise ValueError("q must be [tokens, heads, head_dim], heads a multiple of the pools' and head_dim theirs")
-    if window is not None and window < 1:
-        raise ValueError("window must be a position or more (None: all)")
-    if sink < 0 or (sink and window is None):
-        raise ValueError("sink: positions that stay visible outside a window")
-    top = 0
-    if selected is not None:
-        if window is not None:
-            raise ValueError("selected pages and a window do not go together")
-        if group < 1:
-            raise ValueError("group must be a token or more")
-        rows = selected_rows(T, plan.q_start.shape[0] - 1, group)
-        if (selected.dtype != torch.int32 or selected.device != dev or selected.dim() != 3 or selected.shape[:2] != (rows, Hk)
-                or selected.shape[2] < 1 or not selected.is_contiguous()):
-            raise ValueError(f"selected must be a contiguous int32 [{rows}, {Hk}, top] tensor on {dev}")
-        top = selected.shape[2]
-    zero_rest = out is None
-    if out is None:
-        out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
-    elif out.shape != q.shape:
-        raise ValueError("out must be like q")
+    dev, planned = k_pages.device, _plan_layout(plan)
+    _together(dev, q, v_pages, selected, out, *plan[:5])
+    desc, nbytes = _attention_call(dev, _layout(q), _layout(k_pages), _layout(v_pages), plan.page_size, planned, None if out is None else _layout(out),
+                                   None if selected is None else _layout(selected), None if sm_scale is None else float(sm_scale), bool(causal),
+                                   None if window is None else int(window), int(sink), int(group))
+    T, H, _ = q.shape
+    mine = out is None
+    if mine:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     lse = None
-    if return_lse:
-        lse = torch.full((H, T), -math.inf, dtype=torch.float32, device=dev) if not zero_rest else torch.empty((H, T), dtype=torch.float32, device=dev)
-    if T == 0:
-        _plan(plan, 0, dev)
-        return (out, lse) if return_lse else out
-    d = _q_desc(q, qs, Hk, plan, N, ps, (H * D, D) if zero_rest else _rows("out", out, q.dtype, dev), float(D ** -0.5 if sm_scale is None else sm_scale), bool(causal),
-                window or 0, sink, top, group, zero_rest)
-    n = C.c_size_t(0)
-    lib = _l.load()
-    with _on_device(dev):
-        _l.check(lib.sfm_paged_workspace_bytes(C.byref(d), C.byref(n)))
-        ws = torch.empty(n.value, dtype=torch.uint8, device=dev) if n.value else None
-        _l.check(lib.sfm_paged_attention(C.byref(d), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), plan.table.data_ptr(), plan.past.data_ptr(),
-                                         plan.q_start.data_ptr(), None if selected is None else selected.data_ptr(), out.data_ptr(),
-                                         None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), n.value,
-                                         _raw_stream(dev.index)))
-    if not zero_rest:
-        _written(out)
+    if return_lse:             # rows of nobody that are left as they were have none
+        lse = torch.empty((H, T), dtype=torch.float32, device=dev) if mine else torch.full((H, T), -math.inf, dtype=torch.float32, device=dev)
+    if T:
+        with _on_device(dev):
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+            rc = _l.load().sfm_paged_attention(desc, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), plan.table.data_ptr(), plan.past.data_ptr(),
+                                               plan.q_start.data_ptr(), None if selected is None else selected.data_ptr(), out.data_ptr(),
+                                               None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
+                                               _raw_stream(dev.index))
+        if rc:
+            _l.check(rc)
+        if not mine:
+            _written(out)
     return (out, lse) if return_lse else out
+
+
+@functools.lru_cache(maxsize=4096)
+def _select_call(device, q, means, plan, page_size, top, group, causal, first, last):
+    """(descriptor, rows of the lists, workspace bytes)."""
+    if q[0] not in _DT:
+        raise ValueError("q must be a [tokens, heads, head_dim] tensor of bf16, fp16 or fp32")
+    qs = _rows("q", q, q[0])
+    T, H, D = q[1]
+    if means[0] != torch.float32 or len(means[1]) != 3 or means[1][2] != D or tuple(means[2]) != (means[1][1] * D, D, 1):
+        raise ValueError("means must be a contiguous float32 [pages, kv_heads, head_dim] tensor")
+    N, Hk, _ = means[1]
+    if Hk < 1 or H < Hk or H % Hk:
+        raise ValueError("q's heads must be a multiple of the means'")
+    if group < 1 or not 1 <= top <= _l.PAGED_TOP_MAX:
+        raise ValueError(f"group must be a token or more, top 1 to {_l.PAGED_TOP_MAX} pages")
+    if first < 0 or last < 0 or first + last > top:
+        raise ValueError("first and last must not be negative, nor more than top together")
+    R, W, ts = _planned(plan, T)
+    desc = _l.PagedDesc(_DT[q[0]], H, Hk, D, T, R, W, N, page_size, ts, (0, 0, 0), qs, (0, 0), 1.0, causal, 0, 0, top, group, 0)
+    n = C.c_size_t(0)
+    if T:
+        with torch.cuda.device(device):
+            _l.check(_l.load().sfm_paged_select_workspace_bytes(desc, C.byref(n)))
+    return desc, selected_rows(T, R, group), n.value
 
 
 def select_pages(q, means, plan, top, group=1, causal=False, first=1, last=1):
@@ -283,32 +346,19 @@ def select_pages(q, means, plan, top, group=1, causal=False, first=1, last=1):
     to `top` in all; of level ones the lower.  means: fp32 [pages, kv_heads, head_dim], kept by write_pages.  Scores are sums in 64 bits,
     so that which page is ahead does not hang on the order of an addition; NaN counts as -inf, as does a page outside the pool.  Group i of request r
     is row q_start[r] // group + r + i; rows that nobody has are -1."""
-    if _needs_grad(q, means):
+    if torch.is_grad_enabled() and (q.requires_grad or means.requires_grad):
         raise NotImplementedError("select_pages is not differentiable")
-    if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dtype not in _DT:
-        raise ValueError("q must be a [tokens, heads, head_dim] GPU tensor of bf16, fp16 or fp32")
-    qs = _rows("q", q, q.dtype, q.device)
-    T, H, D = q.shape
-    if means.dim() != 3 or means.dtype != torch.float32 or means.device != q.device or not means.is_contiguous() or means.shape[2] != D:
-        raise ValueError("means must be a contiguous float32 [pages, kv_heads, head_dim] tensor on q's device")
-    N, Hk = means.shape[:2]
-    if H < Hk or H % Hk:
-        raise ValueError("q's heads must be a multiple of the means'")
-    if group < 1 or not 1 <= top <= _l.PAGED_TOP_MAX:
-        raise ValueError(f"group must be a token or more, top 1 to {_l.PAGED_TOP_MAX} pages")
-    if first < 0 or last < 0 or first + last > top:
-        raise ValueError("first and last must not be negative, nor more than top together")
-    R = _plan(plan, T, q.device)[0]
-    selected = torch.empty((selected_rows(T, R, group), Hk, top), dtype=torch.int32, device=q.device)
-    if T == 0:
+    dev, planned = q.device, _plan_layout(plan)
+    _together(dev, means, *plan[:5])
+    top, first, last = int(top), int(first), int(last)
+    desc, rows, nbytes = _select_call(dev, _layout(q), _layout(means), planned, plan.page_size, top, int(group), bool(causal), first, last)
+    selected = torch.empty((rows, means.shape[1], top), dtype=torch.int32, device=dev)
+    if q.shape[0] == 0:
         return selected.fill_(-1)
-    d = _q_desc(q, qs, Hk, plan, N, (0, 0, 0), (0, 0), 1.0, bool(causal), 0, 0, top, group, 0)
-    n = C.c_size_t(0)
-    lib = _l.load()
-    with _on_device(q.device):
-        _l.check(lib.sfm_paged_select_workspace_bytes(C.byref(d), C.byref(n)))
-        ws = torch.empty(n.value, dtype=torch.uint8, device=q.device) if n.value else None
-        _l.check(lib.sfm_paged_select(C.byref(d), q.data_ptr(), means.data_ptr(), plan.table.data_ptr(), plan.past.data_ptr(), plan.q_start.data_ptr(),
-                                      first, last, selected.data_ptr(), None if ws is None else ws.data_ptr(), n.value,
-                                      _raw_stream(q.device.index)))
+    with _on_device(dev):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        rc = _l.load().sfm_paged_select(desc, q.data_ptr(), means.data_ptr(), plan.table.data_ptr(), plan.past.data_ptr(), plan.q_start.data_ptr(), first,
+                                        last, selected.data_ptr(), ws.data_ptr(), nbytes, _raw_stream(dev.index))
+    if rc:
+        _l.check(rc)
     return selected

@@ -168,7 +168,7 @@ def test_without_the_workspace_a_call_runs_whole():
     plan, table, q_start, q, kp, vp = inputs(past, n, page, 4, 2, 128, torch.bfloat16)
     dq, dk, dv = q.to(DEV), kp.to(DEV), vp.to(DEV)
     out = torch.zeros_like(dq)
-    d = PA._q_desc(dq, (4 * 128, 128), 2, plan, dk.shape[0], dk.stride()[:3], (4 * 128, 128), 128 ** -0.5, True, 0, 0, 0, 1, 1)
+    d, _ = PA._attention_call(dq.device, PA._layout(dq), PA._layout(dk), PA._layout(dv), page, PA._plan_layout(plan), None, None, None, True, None, 0, 1)
     size = C.c_size_t(0)
     sfa.lib.check(sfa.lib.load().sfm_paged_workspace_bytes(C.byref(d), C.byref(size)))
     assert size.value > 0
@@ -193,13 +193,13 @@ def test_workspaces_have_the_size_that_is_asked_for():
 
     def canary():
         return torch.full((size.value + 65536,), 0xA5, dtype=torch.uint8, device=DEV)
-    d = PA._q_desc(dq, (4 * 128, 128), 2, plan, dk.shape[0], dk.stride()[:3], (4 * 128, 128), 128 ** -0.5, True, 0, 0, 0, 1, 1)
+    d, _ = PA._attention_call(dq.device, PA._layout(dq), PA._layout(dk), PA._layout(dv), page, PA._plan_layout(plan), None, None, None, True, None, 0, 1)
     sfa.lib.check(lib.sfm_paged_workspace_bytes(C.byref(d), C.byref(size)))
     ws = canary()
     sfa.lib.check(lib.sfm_paged_attention(C.byref(d), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), plan.table.data_ptr(), plan.past.data_ptr(),
                                           plan.q_start.data_ptr(), None, out.data_ptr(), None, ws.data_ptr(), size.value, stream))
     assert bool((ws[size.value:] == 0xA5).all()) and torch.equal(out, PA.paged_attention(dq, dk, dv, plan, causal=True))
-    d = PA._q_desc(dq, (4 * 128, 128), 2, plan, dk.shape[0], (0, 0, 0), (0, 0), 1.0, True, 0, 0, 7, 1, 0)
+    d, _, _ = PA._select_call(dq.device, PA._layout(dq), PA._layout(means), PA._plan_layout(plan), page, 7, 1, True, 1, 1)
     sfa.lib.check(lib.sfm_paged_select_workspace_bytes(C.byref(d), C.byref(size)))
     ws = canary()
     sfa.lib.check(lib.sfm_paged_select(C.byref(d), dq.data_ptr(), means.data_ptr(), plan.table.data_ptr(), plan.past.data_ptr(), plan.q_start.data_ptr(), 1, 1,

@@ -143,16 +143,23 @@ def test_functions_want_the_gpu():
 
 def test_gradients_are_refused():
     pool, q = torch.zeros((4, 16, 2, 64)), torch.zeros((4, 2, 64), requires_grad=True)
-    for call in (lambda: PA.write_pages(q, q, pool, pool, cpu_plan()), lambda: PA.paged_attention(q, pool, pool, cpu_plan()),
+    leaf = torch.zeros((4, 16, 2, 64), requires_grad=True)
+    for call in (lambda: PA.write_pages(q.detach(), q.detach(), leaf, pool, cpu_plan()), lambda: PA.paged_attention(q.detach(), pool, pool, cpu_plan(), out=q),
+                 lambda: PA.write_pages(q, q, pool, pool, cpu_plan()), lambda: PA.paged_attention(q, pool, pool, cpu_plan()),
                  lambda: PA.paged_attention(q.detach(), pool, pool.requires_grad_(), cpu_plan()), lambda: PA.select_pages(q, pool[:, 0], cpu_plan(), 2)):
         with pytest.raises(NotImplementedError, match="differentiable"):
             call()
 
 
 def test_tables_and_arrays():
-    for bad in (torch.zeros((2, 3), dtype=torch.int64), torch.zeros(3, dtype=torch.int32), None):
+    for bad in (torch.zeros((2, 3), dtype=torch.int64), torch.zeros(3, dtype=torch.int32), torch.zeros((0, 3), dtype=torch.int32),
+                torch.zeros((3, 2), dtype=torch.int32).T):
         with pytest.raises(ValueError, match="table"):
-            PA._table(bad)
+            PA._table(PA._layout(bad))
+    with pytest.raises(ValueError, match="table"):
+        PA.plan_pages(None, None, None, None, 4, 16)
+    assert PA._table(PA._layout(torch.zeros((4, 9), dtype=torch.int32)[::2, 3:5])) == (2, 2, 18)
+    assert PA._table(PA._layout(torch.zeros((4, 9), dtype=torch.int32)[:1, 3:5])) == (1, 2, 2)
     for bad in (torch.zeros(2, dtype=torch.int64), torch.zeros((2, 1), dtype=torch.int32), [1, 2], torch.zeros(3, dtype=torch.int32)):
         with pytest.raises(ValueError):
             PA._ints("past", bad, torch.device("cpu"), 2)
@@ -161,15 +168,36 @@ def test_tables_and_arrays():
 
 def test_strides_of_rows_and_pools():
     x = torch.zeros((5, 3, 2, 8))
-    assert PA._rows("q", x[:, 1], x.dtype, x.device) == (48, 8)
-    assert PA._rows("q", x[:1, 1, 1:], x.dtype, x.device) == (8, 8)          # dimensions of one
+    assert PA._rows("q", PA._layout(x[:, 1]), x.dtype) == (48, 8)
+    assert PA._rows("q", PA._layout(x[:1, 1, 1:]), x.dtype) == (8, 8)        # dimensions of one
     with pytest.raises(ValueError):
-        PA._rows("q", x[:, 1].transpose(1, 2), x.dtype, x.device)
+        PA._rows("q", PA._layout(x[:, 1].transpose(1, 2)), x.dtype)
     with pytest.raises(ValueError):
-        PA._rows("q", x[:, 1], torch.float16, x.device)
-    assert PA._pool_strides(x) == (48, 16, 8)
-    assert PA._pool_strides(x[:1, :, :1]) == (48, 16, 8)
-    assert PA._pool_strides(x.transpose(1, 2)) == (48, 8, 16)
+        PA._rows("q", PA._layout(x[:, 1]), torch.float16)
+    with pytest.raises(ValueError):
+        PA._rows("q", PA._layout(x), x.dtype)
+    assert PA._pool("k", PA._layout(x)) == (48, 16, 8)
+    assert PA._pool("k", PA._layout(x[:1, :, :1])) == (48, 16, 8)
+    assert PA._pool("k", PA._layout(x.transpose(1, 2))) == (48, 8, 16)
+    with pytest.raises(ValueError):
+        PA._pool("k", PA._layout(x.transpose(2, 3)))
+    assert PA._pools(PA._layout(x), PA._layout(x.clone()), 3) == (48, 16, 8)
+    for other, page in ((x.half(), 3), (x[:4], 3), (x.transpose(1, 2).contiguous().transpose(1, 2), 3), (x, 16)):
+        with pytest.raises(ValueError):
+            PA._pools(PA._layout(x), PA._layout(other), page)
+
+
+def test_layouts_of_plans():
+    layout = PA._plan_layout(cpu_plan())
+    assert PA._planned(layout, 4) == (2, 3, 3)
+    with pytest.raises(ValueError, match="slots"):
+        PA._planned(layout, 5)
+    with pytest.raises(ValueError, match="q_start"):
+        PA._planned(PA._plan_layout(cpu_plan()._replace(q_start=torch.zeros(2, dtype=torch.int32))), 4)
+    with pytest.raises(ValueError, match="past"):
+        PA._planned(PA._plan_layout(cpu_plan()._replace(past=torch.zeros(4, dtype=torch.int32)[::2])), 4)
+    with pytest.raises(ValueError, match="PagePlan"):
+        PA._plan_layout(tuple(cpu_plan()))
 
 
 GPU_ONLY = [
