@@ -467,7 +467,7 @@ struct FewLds {
 
 template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
-template <class E, int D>
+template <class E, int D, bool ONCE>
 __global__ __launch_bounds__(256, 2) void paged_few_kernel(PagedArgs a, int64_t npieces, int chunks, int chunk_tiles, float* part) {
     using L = DnLds<D>;
     constexpr int kRows = 64 / L::kCPR, kLoads = 32 / kRows, kVar = D == 128 ? 4 : 2;  // rows of a load, loads of half a tile, column orders
@@ -518,7 +518,9 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(PagedArgs a, int64_t 
         for (int j = 0; j < kLoads; ++j) {
             const int from = 4 * (i & 15) + j * kRows / 8;
             const uint64_t off = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(off_hi, from) << 32 | (uint32_t)__builtin_amdgcn_readlane(off_lo, from);
-            dn_load_lds16(g + off + (uint32_t)(j * kRows % 8) * row_bytes, voff[j % kVar], lds0 + dst + (uint32_t)j * 1024);
+            const char* const from_block = g + off + (uint32_t)(j * kRows % 8) * row_bytes;
+            if (ONCE) dn_load_lds16_nt(from_block, voff[j % kVar], lds0 + dst + (uint32_t)j * 1024);
+            else dn_load_lds16(from_block, voff[j % kVar], lds0 + dst + (uint32_t)j * 1024);
         }
     };
     if (n > 0) {
@@ -929,9 +931,10 @@ struct PagedPlan {
     int rows;                      // of a piece; 0: the shape-generic kernel
     int64_t pieces;
     int chunks, chunk_tiles;
+    bool once;                     // few rows: the cache is read past the caches
 };
 static PagedPlan paged_plan(const sfm_paged_desc& d) {
-    PagedPlan p{0, 0, 1, 0};
+    PagedPlan p{0, 0, 1, 0, false};
     if (d.dtype == SFM_F32 || (d.D != 64 && d.D != 128)) return p;
     const int64_t G = d.H / d.kv_heads, cu = cu_count();
     // rows of a request (of a group of tokens) and key head, on average, and pieces that have rows
@@ -951,6 +954,9 @@ static PagedPlan paged_plan(const sfm_paged_desc& d) {
     int64_t chunks = 1;
     if (p.rows == 32) {
         chunks = std::min<int64_t>((8 * cu + n - 1) / n, (tiles + 7) / 8);
+        // More rows than twice the memory-side cache (256 MB) holds, and each read once: past it, 848 MB (up to 2 GB by the table's width)
+        // 193 -> 175 us; 134 MB that lie in it 38 -> 44
+        p.once = n * tiles * 64.0 * d.D * 4 > 512e6;
         // Selected pages make rows equally long: where a range of all of them (5.5 us, and 2.9 per tile of each of the four waves) takes
         // no longer than their bytes do, nothing is split and joined: 16 tokens, 8 heads, 64 pages of 32 rows 51 us instead of 55
         const double whole_us = 5.5 + 2.9 * ((tiles + 3) / 4), bytes_us = n * tiles * 64.0 * d.D * 4 / 4.8e6;
@@ -1005,7 +1011,7 @@ static int launch_mfma(const PagedArgs& a, PagedPlan p, float* part, hipStream_t
         hipLaunchKernelGGL(kern, dim3(xcd_grid((int)total)), dim3(64 * nw), lds, stream, a, p.pieces, p.chunks, p.chunk_tiles, part);
         return SFM_OK;
     };
-    const int rc = p.rows == 32 ? go(paged_few_kernel<E, D>, 4, FewLds<D>::kTotal + 4 * 96 * sizeof(float))
+    const int rc = p.rows == 32 ? go(p.once ? paged_few_kernel<E, D, true> : paged_few_kernel<E, D, false>, 4, FewLds<D>::kTotal + 4 * 96 * sizeof(float))
                    : p.rows == 128 ? go(paged_rows_kernel<E, D, 4>, 4, RowsLds<D, 4>::kTotal) : go(paged_rows_kernel<E, D, 8>, 8, RowsLds<D, 8>::kTotal);
     if (rc) return rc;
     if (part != nullptr) {

@@ -161,6 +161,18 @@ def test_requests_that_share_pages(n):
     close(got.cpu(), None, oracle.attention(q, kp, vp, table, torch.tensor(past), q_start, causal=True), torch.bfloat16)
 
 
+@pytest.mark.parametrize("D,dtype", [(128, torch.bfloat16), (64, torch.float16)], ids=str)
+def test_tables_wider_than_the_requests(D, dtype):
+    """A table for 40000 positions: sizes follow from its width (many ranges, the cache read past the caches), results from the lengths."""
+    g = torch.Generator().manual_seed(4)
+    past, n, page = torch.randint(0, 300, (9,), generator=g).tolist(), [1] * 8 + [2], 16
+    plan, table, q_start, q, kp, vp = inputs(past, n, page, 16, 8, D, dtype)
+    wide = torch.full((9, 2500), -1, dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = plan.table
+    got, lse = PA.paged_attention(q.to(DEV), kp.to(DEV), vp.to(DEV), plan._replace(table=wide), causal=True, return_lse=True)
+    close(got.cpu(), lse.cpu(), oracle.attention(q, kp, vp, table, torch.tensor(past), q_start, causal=True), dtype)
+
+
 def test_without_the_workspace_a_call_runs_whole():
     """The C entry takes a NULL or too small workspace: the same result within the bound, in one range."""
     import ctypes as C
