@@ -540,6 +540,11 @@ int sfm_paged_write(const sfm_paged_desc* desc, const void* k, const void* v, co
  * row does not see have no part in it whatever their K and V hold.  Sums and statistics in fp32, a fixed order.
  * MFMA kernels for 16-bit tensors with D 64 or 128; a workspace lets calls with few rows be split over the keys. */
 int sfm_paged_workspace_bytes(const sfm_paged_desc* desc, size_t* bytes);
+
+/* Which kernel such a call takes on the current device with its workspace, for tests and profiles.  rows: of a workgroup's piece, 32 (a
+ * wave's), 128 or 256, 0 for the shape-generic kernel; ranges: of the keys, joined behind it; past_caches: 1 where the cache is read past the
+ * caches. */
+int sfm_paged_attention_plan(const sfm_paged_desc* desc, int32_t* rows, int32_t* ranges, int32_t* past_caches);
 int sfm_paged_attention(const sfm_paged_desc* desc, const void* q, const void* k_pages, const void* v_pages, const int32_t* table,
                         const int32_t* past, const int32_t* q_start, const int32_t* selected, void* out, float* lse, void* workspace,
                         size_t workspace_bytes, void* stream);

@@ -39,5 +39,8 @@ prologue.rope_*       closed form x*e^{i theta}; norm preservation; start_frame
 cache.KVCacheState    hand-traced index sequences (7 chunks x 5 passes; a
                       window/sink eviction trace)
 sched.*               closed form sigma(t); warped step list
+paged.*               scaled_dot_product_attention on a cache in order, pages
+                      moved with their table, windows, lists, plans and writes
+                      in scalar loops
 ====================  ========================================================
 """

@@ -987,6 +987,13 @@ size_t paged_workspace_bytes(const sfm_paged_desc& d) {
     return p.chunks < 2 ? 0 : (size_t)p.chunks * d.tokens * d.H * (d.D + 2) * sizeof(float);
 }
 
+void paged_attention_plan(const sfm_paged_desc& d, int32_t* rows, int32_t* ranges, int32_t* past_caches) {
+    const PagedPlan p = paged_plan(d);
+    *rows = p.rows;
+    *ranges = p.chunks;
+    *past_caches = p.once;
+}
+
 static int launch_status() {
     const hipError_t err = hipGetLastError();
     if (err == hipSuccess) return SFM_OK;

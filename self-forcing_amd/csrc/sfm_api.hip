@@ -83,6 +83,7 @@ int launch_paged_plan(int R, int W, int page_size, int64_t T, int32_t* table, in
 int launch_paged_write(const sfm_paged_desc& d, const void* k, const void* v, const int64_t* ks, void* kp, void* vp, const int64_t* slots,
                        const int32_t* table, const int32_t* past, const int32_t* q_start, float* means, hipStream_t stream);
 size_t paged_workspace_bytes(const sfm_paged_desc& d);
+void paged_attention_plan(const sfm_paged_desc& d, int32_t* rows, int32_t* ranges, int32_t* past_caches);
 int launch_paged_attention(const sfm_paged_desc& d, const void* q, const void* kp, const void* vp, const int32_t* table,
                            const int32_t* past, const int32_t* q_start, const int32_t* selected, void* out, float* lse, void* workspace,
                            size_t workspace_bytes, hipStream_t stream);
@@ -1955,6 +1956,17 @@ int sfm_paged_workspace_bytes(const sfm_paged_desc* desc, size_t* bytes) {
     const int rc = check_paged_attention(desc);
     if (rc) return rc;
     *bytes = paged_workspace_bytes(*desc);
+    return SFM_OK;
+}
+
+int sfm_paged_attention_plan(const sfm_paged_desc* desc, int32_t* rows, int32_t* ranges, int32_t* past_caches) {
+    if (!rows || !ranges || !past_caches) {
+        set_error("rows, ranges and past_caches must be non-NULL");
+        return SFM_ERR_NULL;
+    }
+    const int rc = check_paged_attention(desc);
+    if (rc) return rc;
+    paged_attention_plan(*desc, rows, ranges, past_caches);
     return SFM_OK;
 }
 

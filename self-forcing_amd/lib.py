@@ -34,7 +34,7 @@ SYMBOLS = [
     "sfm_quantize8", "sfm_dequantize8", "sfm_pack8", "sfm_linear8", "sfm_linear8_fwd", "sfm_linear8_wgrad_workspace_bytes", "sfm_linear8_wgrad",
     "sfm_linear8_bwd_workspace_bytes", "sfm_linear8_bwd", "sfm_linear8_plan", "sfm_linear8_wgrad_plan",
     "sfm_gelu_bwd", "sfm_ln_keep8", "sfm_ln_bwd_workspace_bytes", "sfm_ln_bwd",
-    "sfm_paged_plan_workspace_bytes", "sfm_paged_plan", "sfm_paged_write", "sfm_paged_workspace_bytes", "sfm_paged_attention",
+    "sfm_paged_plan_workspace_bytes", "sfm_paged_plan", "sfm_paged_write", "sfm_paged_workspace_bytes", "sfm_paged_attention_plan", "sfm_paged_attention",
     "sfm_paged_select_workspace_bytes", "sfm_paged_select", "sfm_set_switches", "sfm_get_switches", "sfm_last_error", "sfm_version",
 ]
 
@@ -186,6 +186,7 @@ def load():
     lib.sfm_paged_plan.argtypes = [I32, I32, I32, I64, P, I64, P, P, P, I64, P, P, P, P, P, P, C.c_size_t, P]
     lib.sfm_paged_write.argtypes = [PD, P, P, S3, P, P, P, P, P, P, P, P]
     lib.sfm_paged_workspace_bytes.argtypes = lib.sfm_paged_select_workspace_bytes.argtypes = [PD, C.POINTER(C.c_size_t)]
+    lib.sfm_paged_attention_plan.argtypes = [PD, C.POINTER(I32), C.POINTER(I32), C.POINTER(I32)]
     lib.sfm_paged_attention.argtypes = [PD, P, P, P, P, P, P, P, P, P, P, C.c_size_t, P]
     lib.sfm_paged_select.argtypes = [PD, P, P, P, P, P, I32, I32, P, P, C.c_size_t, P]
     lib.sfm_vae_norm_act.argtypes = [C.c_int32] * 6 + [P, S3, P, P, S3, P]

@@ -487,6 +487,44 @@ def test_pools_past_four_gib(D, n):
     close(got.cpu(), lse.cpu(), oracle.attention(q, wk, wv, table, torch.tensor(past), q_start, causal=True), torch.bfloat16)
 
 
+# ---------------------------------------------------------------- which kernel a call takes
+def kernel(plan, q, kp, causal=True, window=None, selected=None, group=1):
+    """(rows of a piece, ranges of the keys, whether the cache is read past the caches)."""
+    import ctypes as C
+    out = [C.c_int32() for _ in range(3)]
+    d, _ = PA._attention_call(kp.device, PA._layout(q), PA._layout(kp), PA._layout(kp), kp.shape[1], PA._plan_layout(plan), None,
+                              None if selected is None else PA._layout(selected), None, causal, window, 0, group)
+    sfa.lib.check(sfa.lib.load().sfm_paged_attention_plan(d, *map(C.byref, out)))
+    return tuple(x.value for x in out)
+
+
+def test_every_kernel_is_reached_by_the_tests_above():
+    def of(past, n, page, H, Hk, D=128, dtype=torch.bfloat16, width=None):
+        plan, _, _, q, kp, _ = inputs(past, n, page, H, Hk, D, dtype)
+        if width:
+            plan = plan._replace(table=torch.full((len(past), width), -1, dtype=torch.int32, device=DEV))
+        return kernel(plan, q.to(DEV), kp.to(DEV))
+    assert of([63], [1], 64, 2, 2) == (32, 1, 0)                               # test_against_the_oracle
+    assert of([700], [1], 8, 8, 1)[:2] == (32, 2)
+    rows, ranges, once = of([0] * 9, [1] * 8 + [2], 16, 16, 8, width=2500)     # test_tables_wider_than_the_requests
+    assert rows == 32 and ranges > 1 and once == 1
+    assert of([100], [300], 40, 2, 2) == (128, 1, 0)
+    assert of([300, 10], [70, 129], 8, 5, 1)[0] == 128
+    assert of([63], [1], 64, 2, 2, 40)[0] == 0 and of([63], [1], 64, 2, 2, 64, torch.float32)[0] == 0
+
+
+def test_every_kernel_is_reached_by_long_contexts():
+    def of(past, n, page, H, Hk, D):
+        plan, q, kp, _ = long_inputs(past, n, page, H, Hk, D, torch.bfloat16)
+        return kernel(plan, q, kp)
+    rows, ranges, _ = of([40000], [1], 64, 8, 2, 128)
+    assert rows == 32 and ranges > 8
+    assert of([18000], [2048], 16, 16, 16, 64) == (128, 1, 0)                  # more tiles than a stretch of places holds
+    assert of([34000], [3700], 1560, 16, 16, 64) == (256, 1, 0)
+    rows, ranges, _ = of([20000, 19000], [40, 2], 40, 12, 2, 128)
+    assert rows == 128 and ranges > 1
+
+
 # ---------------------------------------------------------------- long contexts, against the definition in 64 bits on the GPU
 def long_inputs(past, n, page, H, Hk, D, dtype, seed=0):
     """Pools on the GPU whose pages lie in no order."""

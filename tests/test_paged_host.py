@@ -64,6 +64,9 @@ def test_attention_refuses(change, code):
     d, n = desc(**change), C.c_size_t(0)
     assert attention(d, selected=P) == code
     assert L.load().sfm_paged_workspace_bytes(C.byref(d), C.byref(n)) == code
+    out = [C.c_int32() for _ in range(3)]
+    assert L.load().sfm_paged_attention_plan(C.byref(d), *map(C.byref, out)) == code
+    assert L.load().sfm_paged_attention_plan(C.byref(desc()), None, C.byref(out[0]), C.byref(out[1])) == NULL
 
 
 @pytest.mark.parametrize("ptr,code", [(dict(q=None), NULL), (dict(k=None), NULL), (dict(v=None), NULL), (dict(table=None), NULL), (dict(past=None), NULL),
