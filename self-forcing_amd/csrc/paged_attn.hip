@@ -468,7 +468,7 @@ struct FewLds {
 template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
 template <class E, int D, bool ONCE>
-__global__ __launch_bounds__(256, 2) void paged_few_kernel(PagedArgs a, int64_t npieces, int chunks, int chunk_tiles, float* part) {
+__global__ __launch_bounds__(256, 2) void paged_few_kernel(PagedArgs a, int64_t npieces, int chunks, int chunk_tiles, float* part, bool) {
     using L = DnLds<D>;
     constexpr int kRows = 64 / L::kCPR, kLoads = 32 / kRows, kVar = D == 128 ? 4 : 2;  // rows of a load, loads of half a tile, column orders
     extern __shared__ __attribute__((aligned(256))) char lds[];
@@ -629,7 +629,7 @@ struct RowsLds {
 
 template <class E, int D, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_rows_kernel(PagedArgs a, int64_t npieces, int chunks, int chunk_tiles,
-                                                                                                          float* part) {
+                                                                                                          float* part, bool paired) {
     using L = DnLds<D, NW>;
     constexpr int DS = D / 16, DT = D / 32, NTH = 64 * NW;
     extern __shared__ __attribute__((aligned(256))) char lds[];
@@ -637,14 +637,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const int tid = threadIdx.x, lane = tid & 63, m = lane & 31, hf = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const sfm_paged_desc& d = a.d;
-    const int total = (int)(npieces * d.kv_heads * chunks);
-    const int item = xcd_item(total);
+    const int total = (int)(npieces * d.kv_heads * chunks), per = (total + 7) / 8;
+    // the pieces of a head go to one XCD, under a causal mask those with the most keys first, or a long and a short one in turn
+    const int item = (int)(blockIdx.x % 8) * per + (paired ? paired_place(blockIdx.x / 8, per) : (int)blockIdx.x / 8);
     if (item >= total) return;
     const int unit = item / (int)npieces, kh = unit / chunks, chunk = unit - kh * chunks;
     const int at = item - unit * (int)npieces;
     Piece p;
-    // the pieces of a head go to one XCD; under a causal mask those with the most keys first
-    if (!find_piece<32 * NW>(a, d.causal ? npieces - 1 - at : at, kh, &p)) return;
+    if (!find_piece<32 * NW>(a, !d.causal ? at : paired ? paired_piece(at, (int)npieces) : npieces - 1 - at, kh, &p)) return;
     const int v0 = min(chunk * chunk_tiles, p.k.tiles), v1 = min(v0 + chunk_tiles, p.k.tiles);
     const int f0 = max(v0, p.k.fast0), nf = max(min(v1, p.k.fast1) - f0, 0) & ~1;      // the loop over whole tiles takes two at a time
     const BlockMap map = block_map(a, p);
@@ -932,9 +932,10 @@ struct PagedPlan {
     int64_t pieces;
     int chunks, chunk_tiles;
     bool once;                     // few rows: the cache is read past the caches
+    bool paired;                   // many rows, causal: long and short pieces share a compute unit
 };
 static PagedPlan paged_plan(const sfm_paged_desc& d) {
-    PagedPlan p{0, 0, 1, 0, false};
+    PagedPlan p{0, 0, 1, 0, false, false};
     if (d.dtype == SFM_F32 || (d.D != 64 && d.D != 128)) return p;
     const int64_t G = d.H / d.kv_heads, cu = cu_count();
     // rows of a request (of a group of tokens) and key head, on average, and pieces that have rows
@@ -948,9 +949,16 @@ static PagedPlan paged_plan(const sfm_paged_desc& d) {
         return mean > 128 && (int64_t)rounds + 1 < 1.15 * rounds;
     };
     auto items = [&](int64_t rows) { return units * ((mean + rows - 1) / rows) * d.kv_heads; };
-    p.rows = mean <= 32 ? 32 : wide(items(256)) ? 256 : 128;
+    // Causal prompts without much before them: a head's last piece has twice the mean's keys, and where all pieces are on the chip at once it
+    // alone sets the time.  Two pieces of 128 rows to a compute unit can be a long and a short one (4680 tokens, 12 heads, 142 us -> 127; four
+    // requests of 1024 on 1024, 92 -> 79); with more pieces than that the order of their lengths balances them better (8192 tokens, 32 heads
+    // on 8, 556 us and 586), and behind a long cache they are much alike.
+    const int64_t cap = (int64_t)d.width * d.page_size;
+    const bool prompts = d.causal && !d.top && mean > 128 && items(128) <= 2 * cu;
+    p.rows = mean <= 32 ? 32 : wide(items(256)) && !(prompts && cap <= 4 * d.tokens / d.requests) ? 256 : 128;
+    p.paired = prompts && p.rows == 128;
     p.pieces = d.top ? pieces(d.tokens, d.group, d.requests) * ((std::min<int64_t>(d.group, d.tokens) * G + p.rows - 1) / p.rows) : pieces(d.tokens * G, p.rows, d.requests);
-    const int64_t cap = (int64_t)d.width * d.page_size, tiles = ((d.top ? (int64_t)d.top * d.page_size : cap) + 63) / 64, n = items(p.rows);
+    const int64_t tiles = ((d.top ? (int64_t)d.top * d.page_size : cap) + 63) / 64, n = items(p.rows);
     int64_t chunks = 1;
     if (p.rows == 32) {
         chunks = std::min<int64_t>((8 * cu + n - 1) / n, (tiles + 7) / 8);
@@ -1015,7 +1023,7 @@ static int launch_mfma(const PagedArgs& a, PagedPlan p, float* part, hipStream_t
             set_error("hipFuncSetAttribute failed: %s", hipGetErrorString(e));
             return SFM_ERR_HIP;
         }
-        hipLaunchKernelGGL(kern, dim3(xcd_grid((int)total)), dim3(64 * nw), lds, stream, a, p.pieces, p.chunks, p.chunk_tiles, part);
+        hipLaunchKernelGGL(kern, dim3(xcd_grid((int)total)), dim3(64 * nw), lds, stream, a, p.pieces, p.chunks, p.chunk_tiles, part, p.paired);
         return SFM_OK;
     };
     const int rc = p.rows == 32 ? go(p.once ? paged_few_kernel<E, D, true> : paged_few_kernel<E, D, false>, 4, FewLds<D>::kTotal + 4 * 96 * sizeof(float))

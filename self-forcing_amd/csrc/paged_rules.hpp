@@ -74,6 +74,12 @@ __host__ __device__ __forceinline__ KeyTiles key_tiles(const Request& q, bool no
 }
 __host__ __device__ __forceinline__ int tile_of(const KeyTiles& k, int v) { return v < k.sinks ? v : v - k.sinks + k.first; }
 
+// Pieces of a causal prompt whose workgroups are on the chip all at once, two to a compute unit.  A head's last pieces have the most keys.  In
+// its list they alternate with its first, so that every XCD's share of the list is as much work; an XCD takes the even places of its
+// share (the long pieces) first, one per compute unit, and then the odd ones, which join them.
+__host__ __device__ __forceinline__ int paired_piece(int at, int pieces) { return at & 1 ? at / 2 : pieces - 1 - at / 2; }
+__host__ __device__ __forceinline__ int paired_place(int i, int share) { return i < (share + 1) / 2 ? 2 * i : 2 * (i - (share + 1) / 2) + 1; }
+
 constexpr int kNoPos = 0x7ffffff8;                 // of a block that nobody sees
 
 // Eight positions that one tile and one page hold are a block.  What a lane needs of a piece to find its blocks

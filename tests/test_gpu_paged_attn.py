@@ -585,9 +585,11 @@ def check_rows(got, lse, plan, q, kp, vp, past, n, tokens, causal, window=None, 
     ([18000], [2048], 16, 16, 16, 64, True, None, 0), ([16500], [2048], 64, 16, 16, 128, False, None, 0),
     ([34000], [3700], 1560, 16, 16, 64, False, None, 0), ([33000], [3700], 32, 16, 16, 128, True, None, 0),
     ([18000], [2048], 16, 16, 16, 64, True, 100, 17000), ([34000], [3700], 64, 16, 16, 64, True, 2000, 33000), ([20000, 19000], [40, 2], 40, 12, 2, 128, True, 5000, 64),
+    ([0], [4680], 64, 12, 12, 64, True, None, 0), ([0, 1000, 5], [1000, 1024, 700], 40, 16, 4, 128, True, None, 0), ([0], [6000], 16, 32, 8, 64, True, None, 0),
 ])
-def test_long_contexts(past, n, page, H, Hk, D, causal, window, sink):
-    plan, q, kp, vp = long_inputs(past, n, page, H, Hk, D, torch.bfloat16)
+@pytest.mark.parametrize("dtype", HALF, ids=str)
+def test_long_contexts(past, n, page, H, Hk, D, causal, window, sink, dtype):
+    plan, q, kp, vp = long_inputs(past, n, page, H, Hk, D, dtype)
     got, lse = PA.paged_attention(q, kp, vp, plan, causal=causal, window=window, sink=sink, return_lse=True)
     T = sum(n)
     tokens = sorted({0, 1, T // 3, T // 2, T - 2, T - 1} & set(range(T)))

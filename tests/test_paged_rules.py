@@ -23,6 +23,7 @@ extern "C" void tiles(int past, int n, int none, int t0, int t1, int causal, int
     const int v[] = {k.end_min, k.end_max, k.lo_min, k.lo_max, k.sinks, k.first, k.tiles, k.fast0, k.fast1, k.beyond};
     for (int i = 0; i < 10; ++i) out[i] = v[i];
 }
+extern "C" int paired(int i, int n, int place) { return place ? sfm::paired_place(i, n) : sfm::paired_piece(i, n); }
 extern "C" int tile(int past, int n, int t0, int t1, int causal, int window, int sink, int cap, int v) {
     return sfm::tile_of(sfm::key_tiles(sfm::Request{0, n, past}, false, t0, t1, causal, window, sink, cap), v);
 }
@@ -101,6 +102,14 @@ def test_requests_stay_inside_the_rows(rules):
             out = (C.c_int * 3)()
             rules.request((C.c_int * (R + 1))(*qs), (C.c_int * R)(*ps), r, R, T, out)
             assert 0 <= out[0] <= T and 0 <= out[1] <= T - out[0] and out[2] >= 0
+
+
+@pytest.mark.parametrize("n", [1, 2, 3, 7, 8, 55, 56, 64, 1001])
+def test_paired_pieces_are_every_piece_once(rules, n):
+    pieces = [rules.paired(i, n, 0) for i in range(n)]
+    assert sorted(pieces) == list(range(n)) and pieces[:3] == [n - 1, 0, n - 2][:n]
+    places = [rules.paired(i, n, 1) for i in range(n)]
+    assert sorted(places) == list(range(n)) and places == sorted(range(n), key=lambda i: (i % 2, i))
 
 
 def visible(past, n, t, causal, window, sink, cap):
