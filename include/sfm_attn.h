@@ -514,7 +514,7 @@ typedef struct sfm_paged_desc {
     int32_t dtype;            /* SFM_BF16 | SFM_F16 | SFM_F32 : type of q, out, k, v and the pools */
     int32_t H, kv_heads, D;   /* H a multiple of kv_heads (up to 65535): query heads h * H / kv_heads and on belong to key head h; D a multiple of 8 up to 256 */
     int64_t tokens;           /* rows of q and out (tokens * H < 2^31) */
-    int32_t requests, width;  /* of the table; width * page_size < 2^31 */
+    int32_t requests, width;  /* of the table; width * page_size <= 2^30, top * page_size as well */
     int32_t pages, page_size; /* of the pools; page_size a multiple of 8, pages * page_size < 2^31 */
     int64_t table_stride;
     int64_t pool_stride[3];   /* page, token, head; of both pools */

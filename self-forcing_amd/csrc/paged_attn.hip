@@ -298,8 +298,15 @@ __device__ __forceinline__ void masked_tile(const char* lds, uint32_t kbuf, uint
     }
 }
 
-// Partials of split calls: [chunk][row = token * H + head] of D floats, and behind all of them (maximum, sum): a sum of 0 for nothing
-// seen, NaN for rows that are NaN.
+// Partials of split calls: [chunk][row = token * H + head] of D floats, and behind all of them (maximum, sum).  Of a range whose keys a row
+// sees, but all with a logit of -infinity, the sum is 0 as of one where it sees none, for which nothing is joined.  The row is NaN then only
+// if that holds of all of its ranges: such a range's maximum is -infinity and its sum 1, so that it counts, with a factor of 0.
+__device__ __forceinline__ void store_partial(float* ml, float mrun, float sum, bool seen, bool bad) {
+    const bool none = seen && sum == 0.f;
+    ml[0] = none ? -INFINITY : mrun;
+    ml[1] = bad ? NAN : !seen ? 0.f : none ? 1.f : sum;
+}
+
 template <class E, int D>
 __device__ __forceinline__ void store_rows(const PagedArgs& a, const Piece& pc, RowState<D>& st, bool bad, int row0, int chunk, int chunks,
                                            float* part, char* stage) {
@@ -319,11 +326,7 @@ __device__ __forceinline__ void store_rows(const PagedArgs& a, const Piece& pc, 
 #pragma unroll
                 for (int g = 0; g < 4; ++g)
                     *(f32x4*)(po + 32 * dt + 8 * g) = f32x4{st.o[dt][4 * g], st.o[dt][4 * g + 1], st.o[dt][4 * g + 2], st.o[dt][4 * g + 3]};
-        if (hf == 0) {
-            float* const ml = part + chunks * rows * D + at * 2;
-            ml[0] = st.mrun;
-            ml[1] = bad || (seen && l == 0.f) ? NAN : seen ? l : 0.f;
-        }
+        if (hf == 0) store_partial(part + chunks * rows * D + at * 2, st.mrun, l, seen, bad);
         return;
     }
     const float inv = bad ? NAN : seen ? 1.f / l : 0.f;
@@ -596,11 +599,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(PagedArgs a, int64_t 
             if (rseen)
 #pragma unroll
                 for (int c = 0; c < D / 64; ++c) part[at * D + lane * (D / 64) + c] = o[c];
-            if (lane == 0) {
-                float* const q = part + chunks * rows * D + at * 2;
-                q[0] = M;
-                q[1] = rbad || (rseen && sum == 0.f) ? NAN : rseen ? sum : 0.f;
-            }
+            if (lane == 0) store_partial(part + chunks * rows * D + at * 2, M, sum, rseen, rbad);
         } else {
             const float inv = rbad ? NAN : rseen ? 1.f / sum : 0.f;
             uint16_t* const out = (uint16_t*)a.out + (int64_t)t * d.o_stride[0] + (int64_t)h * d.o_stride[1] + lane * (D / 64);

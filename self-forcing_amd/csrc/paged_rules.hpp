@@ -72,7 +72,6 @@ __host__ __device__ __forceinline__ KeyTiles key_tiles(const Request& q, bool no
     k.fast1 = f0 < f1 ? f1 : 0;
     return k;
 }
-__host__ __device__ __forceinline__ int tile_of(const KeyTiles& k, int v) { return v < k.sinks ? v : v - k.sinks + k.first; }
 
 // Pieces of a causal prompt whose workgroups are on the chip all at once, two to a compute unit.  A head's last pieces have the most keys.  In
 // its list they alternate with its first, so that every XCD's share of the list is as much work; an XCD takes the even places of its
@@ -105,11 +104,6 @@ struct BlockMap {
         *pos = (int)(((uint32_t)en * page8.d + *off8) * 8);
         if (*pos >= end_max || (*pos + 7 < lo_min && *pos >= sink)) return -1;
         return en;
-    }
-    // block of its page
-    __host__ __device__ __forceinline__ uint32_t off8(int vb) const {
-        const uint32_t pb = sel || vb < sinks8 ? (uint32_t)vb : (uint32_t)vb + skip8;
-        return vb < blocks ? pb - quot(pb, page8) * page8.d : 0;
     }
     // the page of an entry, -1 where it is outside the pool
     __host__ __device__ __forceinline__ int page(int e) const {

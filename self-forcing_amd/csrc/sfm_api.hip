@@ -1791,8 +1791,8 @@ static int check_table(int requests, int width, int page_size, int64_t tokens, i
                   (long long)tokens);
         return SFM_ERR_SHAPE;
     }
-    if (page_size < 8 || page_size % 8 || (int64_t)width * page_size > 0x7fffffff) {
-        set_error("page_size=%d, width=%d: need pages of a multiple of 8 rows, and width * page_size < 2^31", page_size, width);
+    if (page_size < 8 || page_size % 8 || (int64_t)width * page_size > (1 << 30)) {
+        set_error("page_size=%d, width=%d: need pages of a multiple of 8 rows, and width * page_size <= 2^30", page_size, width);
         return SFM_ERR_SHAPE;
     }
     if (table_stride < width) {
@@ -1905,8 +1905,8 @@ static int check_paged_q(const sfm_paged_desc* d) {
     int rc;
     if ((rc = check_paged_stride("q: token", d->q_stride[0], 0, esz))) return rc;
     if ((rc = check_paged_stride("q: head", d->q_stride[1], 0, esz))) return rc;
-    if (d->top < 0 || d->top > SFM_PAGED_TOP_MAX || (d->top && d->group < 1) || (int64_t)d->top * d->page_size > 0x7fffffff) {
-        set_error("top=%d, group=%d: need 0 <= top <= %d, top * page_size < 2^31, and groups of a token or more", d->top, d->group, SFM_PAGED_TOP_MAX);
+    if (d->top < 0 || d->top > SFM_PAGED_TOP_MAX || (d->top && d->group < 1) || (int64_t)d->top * d->page_size > (1 << 30)) {
+        set_error("top=%d, group=%d: need 0 <= top <= %d, top * page_size <= 2^30, and groups of a token or more", d->top, d->group, SFM_PAGED_TOP_MAX);
         return SFM_ERR_SHAPE;
     }
     return SFM_OK;
@@ -1937,7 +1937,7 @@ static int check_paged_attention(const sfm_paged_desc* d) {
     const int esz = elem_size(d->dtype);
     if ((rc = check_paged_stride("out: token", d->o_stride[0], d->D, esz))) return rc;
     if ((rc = check_paged_stride("out: head", d->o_stride[1], d->D, esz))) return rc;
-    if (!(d->sm_scale > 0.f) || d->sm_scale > 3.0e38f) {
+    if (!(d->sm_scale > 0.f) || d->sm_scale > 2.0e38f) {
         set_error("sm_scale must be a positive number");
         return SFM_ERR_SHAPE;
     }

@@ -33,7 +33,7 @@ class PagePlan(NamedTuple):
     """A step of requests.  table int32 [requests, width], past and lengths int32 [requests] (tokens in the cache before and after the
     step), q_start int32 [requests + 1] (first row of each request), slots int64 [tokens] (row of the pools, page * page_size + offset,
     of each new token; -1 for none), next_free int32 [1] (how far the list of free pages is used; above its length where it did not
-    suffice)."""
+    suffice).  table and past are the caller's tensors: they stay as they are until the step's calls are done."""
     table: torch.Tensor
     past: torch.Tensor
     lengths: torch.Tensor
@@ -93,6 +93,8 @@ def plan_pages(table, past, new, free, tokens, page_size, next_free=None):
     tokens, page_size = int(tokens), int(page_size)
     if tokens < 0:
         raise ValueError("tokens must not be negative")
+    if not 8 <= page_size <= _MOST:
+        raise ValueError(f"page_size: {page_size}, expected a multiple of 8")
     slots = torch.empty(tokens, dtype=torch.int64, device=dev)
     q_start, lengths, taken = torch.empty(2 * R + 2, dtype=torch.int32, device=dev).split_with_sizes((R + 1, R, 1))
     nbytes = _plan_bytes(R)
@@ -181,6 +183,7 @@ def _together(device, *tensors):
 
 
 _I2 = C.c_int64 * 2
+_MOST = 2 ** 31 - 1            # a window, sink or group past it is one of everything: there are fewer positions and tokens
 
 
 @functools.lru_cache(maxsize=4096)
@@ -290,7 +293,8 @@ def paged_attention(q, k_pages, v_pages, plan, sm_scale=None, causal=False, wind
     _together(dev, q, v_pages, selected, out, *plan[:5])
     desc, nbytes = _attention_call(dev, _layout(q), _layout(k_pages), _layout(v_pages), plan.page_size, planned, None if out is None else _layout(out),
                                    None if selected is None else _layout(selected), None if sm_scale is None else float(sm_scale), bool(causal),
-                                   None if window is None else int(window), int(sink), int(group))
+                                   None if window is None else min(int(window), _MOST), min(int(sink), _MOST),
+                                   min(int(group), _MOST))
     T, H, _ = q.shape
     mine = out is None
     if mine:
@@ -351,7 +355,7 @@ def select_pages(q, means, plan, top, group=1, causal=False, first=1, last=1):
     dev, planned = q.device, _plan_layout(plan)
     _together(dev, means, *plan[:5])
     top, first, last = int(top), int(first), int(last)
-    desc, rows, nbytes = _select_call(dev, _layout(q), _layout(means), planned, plan.page_size, top, int(group), bool(causal), first, last)
+    desc, rows, nbytes = _select_call(dev, _layout(q), _layout(means), planned, plan.page_size, top, min(int(group), _MOST), bool(causal), first, last)
     selected = torch.empty((rows, means.shape[1], top), dtype=torch.int32, device=dev)
     if q.shape[0] == 0:
         return selected.fill_(-1)

@@ -150,6 +150,20 @@ def test_groups_larger_than_the_step(group):
     close(got.cpu(), None, oracle.attention(q, kp, vp, table, torch.tensor(past), q_start, causal=True, selected=sel.cpu().long(), group=group), torch.bfloat16)
 
 
+def test_counts_past_32_bits_are_one_of_everything():
+    past, n, page, far = [300, 20], [100, 131], 16, 2 ** 32
+    plan, table, q_start, q, kp, vp = inputs(past, n, page, 4, 2, 64, torch.bfloat16)
+    q, kp, vp = q.to(DEV), kp.to(DEV), vp.to(DEV)
+    whole = PA.paged_attention(q, kp, vp, plan, causal=True)
+    assert torch.equal(PA.paged_attention(q, kp, vp, plan, causal=True, window=far + 5), whole)
+    got = PA.paged_attention(q, kp, vp, plan, causal=True, window=5, sink=far + 3)
+    close(got.cpu(), None, oracle.attention(q.cpu(), kp.cpu(), vp.cpu(), table, torch.tensor(past), q_start, causal=True), torch.bfloat16)
+    means = kp.float().mean(1)
+    sel = PA.select_pages(q, means, plan, 6, group=far + 1, causal=True)
+    assert torch.equal(sel, PA.select_pages(q, means, plan, 6, group=1000, causal=True))
+    assert torch.equal(PA.paged_attention(q, kp, vp, plan, selected=sel, group=far + 1), PA.paged_attention(q, kp, vp, plan, selected=sel, group=1000))
+
+
 @pytest.mark.parametrize("n", [[1, 1, 1], [40, 150, 3]])
 def test_requests_that_share_pages(n):
     """A prompt's pages in the tables of several requests: read by all of them."""
@@ -279,6 +293,26 @@ def test_infinite_values_reach_the_rows_that_see_them(dtype, D):
     want = oracle.attention(q, kp, vp, table, torch.tensor(past), q_start, causal=True)
     want["out"], want["mag"] = want["out"][..., rest], want["mag"][..., rest]
     close(got[..., rest], None, want, dtype)
+
+
+@pytest.mark.parametrize("past,n,H,D,dtype", [([9000, 700], [1, 1], 2, 128, torch.bfloat16), ([9000], [1], 8, 64, torch.float16), ([9000], [40], 1, 128, torch.bfloat16),
+                                              ([700], [150], 2, 64, torch.bfloat16), ([9000], [1], 2, 40, torch.bfloat16)], ids=str)
+def test_logits_of_minus_infinity(past, n, H, D, dtype):
+    """Keys that a row sees with a logit of -infinity weigh nothing, a whole range of them too; a row that sees no others is NaN, as 0 / 0."""
+    page = 16
+    plan, table, q_start, q, kp, vp = inputs(past, n, page, H, 1, D, dtype)
+    q[..., 0] = 1.0
+    far = 60000.0 if dtype == torch.float16 else 1e6              # a logit of -6e3 and less: the weight is 0 in 64 bits
+    for r, p in enumerate(past):
+        pos = torch.arange(p // 2)
+        kp[table[r, pos // page], pos % page, 0, 0] = -far
+    want = oracle.attention(q, kp, vp, table, torch.tensor(past), q_start, causal=True)
+    kp[kp == -far] = -math.inf
+    got, lse = PA.paged_attention(q.to(DEV), kp.to(DEV), vp.to(DEV), plan, causal=True, return_lse=True)
+    close(got.cpu(), lse.cpu(), want, dtype)
+    kp[..., 0] = -math.inf
+    got, lse = PA.paged_attention(q.to(DEV), kp.to(DEV), vp.to(DEV), plan, causal=True, return_lse=True)
+    assert got.isnan().all() and (lse == -math.inf).all()
 
 
 def test_a_window_hides_what_has_left_it():

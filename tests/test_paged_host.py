@@ -49,7 +49,7 @@ def plan(requests=3, width=5, page=16, tokens=10, stride=5, free_count=9, **ptr)
 NULL, DTYPE, SHAPE, RANGE, STRIDE, WORKSPACE, ALIGN = -1, -2, -3, -4, -5, -6, -7
 SHARED = [(dict(dtype=7), DTYPE), (dict(kv_heads=0), SHAPE), (dict(kv_heads=65536, H=65536), SHAPE), (dict(D=12), SHAPE), (dict(D=264), SHAPE), (dict(D=0), SHAPE), (dict(pages=0), SHAPE),
           (dict(requests=0), SHAPE), (dict(requests=(1 << 24) + 1), SHAPE), (dict(width=0), SHAPE), (dict(page_size=12), SHAPE), (dict(page_size=0), SHAPE),
-          (dict(width=1 << 20, page_size=2048, table_stride=1 << 20), SHAPE), (dict(pages=1 << 20, page_size=2048), SHAPE), (dict(tokens=0), SHAPE),
+          (dict(width=1 << 20, page_size=2048, table_stride=1 << 20), SHAPE), (dict(width=(1 << 20) + 1, page_size=1024, table_stride=1 << 21), SHAPE), (dict(pages=1 << 20, page_size=2048), SHAPE), (dict(tokens=0), SHAPE),
           (dict(tokens=-1), SHAPE), (dict(tokens=1 << 31), SHAPE), (dict(table_stride=4), STRIDE)]
 POOL = [(dict(pool_stride=(4096, 256, 120)), STRIDE), (dict(pool_stride=(4096, 256, 132)), STRIDE), (dict(pool_stride=(4096, 64, 128)), STRIDE),
         (dict(pool_stride=(-4096, 256, 128)), STRIDE), (dict(pool_stride=(4096, 1 << 24, 128)), STRIDE)]
@@ -59,7 +59,7 @@ Q = [(dict(H=7), SHAPE), (dict(H=1), SHAPE), (dict(tokens=1 << 29), SHAPE), (dic
 
 @pytest.mark.parametrize("change,code", SHARED + POOL + Q + [
     (dict(o_stride=(1024, 64)), STRIDE), (dict(o_stride=(1020, 128)), STRIDE), (dict(sm_scale=0.0), SHAPE), (dict(sm_scale=float("nan")), SHAPE),
-    (dict(sm_scale=float("inf")), SHAPE), (dict(window=-1), RANGE), (dict(sink=-1), RANGE), (dict(sink=3), RANGE), (dict(top=4, window=8), RANGE)])
+    (dict(sm_scale=float("inf")), SHAPE), (dict(sm_scale=3.0e38), SHAPE), (dict(top=2048, page_size=1 << 20, width=1, pages=1), SHAPE), (dict(window=-1), RANGE), (dict(sink=-1), RANGE), (dict(sink=3), RANGE), (dict(top=4, window=8), RANGE)])
 def test_attention_refuses(change, code):
     d, n = desc(**change), C.c_size_t(0)
     assert attention(d, selected=P) == code
@@ -224,6 +224,14 @@ def test_attention_refuses_tensors(name, kw, match):
         kw["selected"] = torch.zeros((PA.selected_rows(4, 2, 1), 2, 3), dtype=torch.int32, device=dev)
     with pytest.raises(ValueError, match=match):
         PA.paged_attention(q, pool, pool, plan, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [0, -16, 12, 2 ** 32 + 16])
+def test_plan_refuses_pages(page):
+    i = torch.zeros(2, dtype=torch.int32, device="cuda:0")
+    with pytest.raises(ValueError, match="page_size"):
+        PA.plan_pages(torch.zeros((2, 3), dtype=torch.int32, device="cuda:0"), i, i, i, 4, page)
 
 
 @pytest.mark.gpu

@@ -24,9 +24,6 @@ extern "C" void tiles(int past, int n, int none, int t0, int t1, int causal, int
     for (int i = 0; i < 10; ++i) out[i] = v[i];
 }
 extern "C" int paired(int i, int n, int place) { return place ? sfm::paired_place(i, n) : sfm::paired_piece(i, n); }
-extern "C" int tile(int past, int n, int t0, int t1, int causal, int window, int sink, int cap, int v) {
-    return sfm::tile_of(sfm::key_tiles(sfm::Request{0, n, past}, false, t0, t1, causal, window, sink, cap), v);
-}
 """
 
 
@@ -132,7 +129,7 @@ def test_tiles_hold_what_a_piece_sees_and_fast_ones_nothing_else(rules):
         end_min, end_max, lo_min, lo_max, sinks, first, count, fast0, fast1, beyond = out
         assert bool(beyond) == ((past + t1 + 1 if causal else past + n) > cap)
         seen = [visible(past, n, t, causal, window, sink, cap) for t in range(t0, t1 + 1)]
-        order = [rules.tile(past, n, t0, t1, causal, window, sink, cap, v) for v in range(count)]
+        order = [v if v < sinks else v - sinks + first for v in range(count)]
         assert order == sorted(set(order))
         covered = {p for i in order for p in range(64 * i, 64 * i + 64)}
         assert set().union(*seen) <= covered
