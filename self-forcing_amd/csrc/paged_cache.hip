@@ -366,24 +366,31 @@ __device__ __forceinline__ SelectRow select_row_behind(const SelectArgs& s, Sele
 }
 
 // Sum of the queries of `n` tokens from t0 on and of a key head's G query heads, in sum[0 .. D).  Chunk c of the rows g, g + groups, ...
-// to a thread; `part` holds their sums.
-template <typename E>
+// to a thread, U of them on their way at a time; `part` holds their sums.
+template <typename E, int U>
 __device__ __forceinline__ void sum_queries(const SelectArgs& s, int kh, int64_t t0, int n, double* part, double* sum) {
     constexpr int N = Chunk<E>::kN;
     const sfm_paged_desc& d = s.d;
     const int tid = threadIdx.x, G = d.H / d.kv_heads, chunks = d.D / N, groups = 256 / chunks, g = tid / chunks, c = tid - g * chunks;
-    const int64_t rows = (int64_t)n * G;
+    const uint32_t rows = (uint32_t)n * G;         // at most tokens * H, below 2^31
     double mine[N];
     float v[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) mine[k] = 0.0;
     if (g < groups)
-#pragma unroll 4
-        for (int64_t j = g; j < rows; j += groups) {
-            const int64_t t = j / G, h = j - t * G;
-            Chunk<E>::get(((const u32x4*)s.q)[((t0 + t) * d.q_stride[0] + (kh * G + h) * d.q_stride[1]) / N + c], v);
+        for (uint32_t j0 = g; j0 < rows; j0 += U * groups) {
+            u32x4 w[U];
 #pragma unroll
-            for (int k = 0; k < N; ++k) mine[k] += (double)v[k];
+            for (int u = 0; u < U; ++u) {
+                const uint32_t j = min(j0 + u * groups, rows - 1), t = j / (uint32_t)G, h = j - t * G;
+                w[u] = ((const u32x4*)s.q)[((t0 + t) * d.q_stride[0] + (kh * G + (int64_t)h) * d.q_stride[1]) / N + c];
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                Chunk<E>::get(w[u], v);
+#pragma unroll
+                for (int k = 0; k < N; ++k) mine[k] += j0 + u * groups < rows ? (double)v[k] : 0.0;
+            }
         }
     __syncthreads();
     if (g < groups)
@@ -392,7 +399,7 @@ __device__ __forceinline__ void sum_queries(const SelectArgs& s, int kh, int64_t
     __syncthreads();
     if (tid < d.D) {
         double t = 0.0;
-        for (int j = 0; j < min((int64_t)groups, rows); ++j) t += part[j * d.D + tid];
+        for (int j = 0; j < (int)min((uint32_t)groups, rows); ++j) t += part[j * d.D + tid];
         sum[tid] = t;
     }
 }
@@ -403,7 +410,40 @@ __global__ __launch_bounds__(256) void paged_sums_kernel(SelectArgs s) {
     __shared__ double part[256 * Chunk<E>::kN];
     const SelectRow x = select_row(s, s.row0 + blockIdx.x);
     if (x.candidates > s.d.top)
-        sum_queries<E>(s, blockIdx.y, x.t0, x.n, part, s.sums + ((int64_t)blockIdx.x * s.d.kv_heads + blockIdx.y) * s.d.D);
+        sum_queries<E, 8>(s, blockIdx.y, x.t0, x.n, part, s.sums + ((int64_t)blockIdx.x * s.d.kv_heads + blockIdx.y) * s.d.D);
+}
+
+// The other lane's value, of the 16 of a DPP row
+template <int CTRL>
+__device__ __forceinline__ double row_lane(double x) {
+    const uint64_t b = (uint64_t)__double_as_longlong(x);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xf, 0xf, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, true);
+    return __longlong_as_double((int64_t)((uint64_t)hi << 32 | lo));
+}
+// Sums over the 16 lanes of a DPP row, lane `sub` of them, of N = 4 or 16 values: lane l gets the sum of value l N / 16.  As long as there
+// are values left to share out, two lanes exchange the half that the other keeps: 15 exchanges for 16 values in place of 64.  The lanes
+// meet at distances 8, 7, 2 and 1 (by exclusive or), which every pair of lanes is a sum of once.
+template <int N>
+__device__ __forceinline__ double row_sums(double* x, int sub) {
+    auto step = [&](auto ctrl_c, auto left_c, int bit) {
+        constexpr int CTRL = decltype(ctrl_c)::value, LEFT = decltype(left_c)::value;
+        if constexpr (LEFT > 1) {
+#pragma unroll
+            for (int j = 0; j < LEFT / 2; ++j) {
+                const double a = x[j], b = x[j + LEFT / 2];
+                x[j] = (sub & bit ? b : a) + row_lane<CTRL>(sub & bit ? a : b);
+            }
+        } else {
+            x[0] += row_lane<CTRL>(x[0]);
+        }
+    };
+    using std::integral_constant;
+    step(integral_constant<int, 0x128>{}, integral_constant<int, N>{}, 8);                         // rotated by 8
+    step(integral_constant<int, 0x141>{}, integral_constant<int, N / 2>{}, 4);                     // mirrored in each 8
+    step(integral_constant<int, 0x4e>{}, integral_constant<int, (N > 4 ? N / 4 : 1)>{}, 2);        // two on, of four
+    step(integral_constant<int, 0xb1>{}, integral_constant<int, (N > 8 ? N / 8 : 1)>{}, 1);
+    return x[0];
 }
 
 // Scores of `chunk` pages for RT rows of one key head.  Sixteen lanes share a page, 4 of each 64 channels a lane; their queries' sums
@@ -435,7 +475,7 @@ __global__ __launch_bounds__(256) void paged_score_kernel(SelectArgs s) {
                 if (s.sums != nullptr) {
                     if (tid < d.D) qsum[i][tid] = i < count ? s.sums[((int64_t)(row + i - s.row0) * d.kv_heads + kh) * d.D + tid] : 0.0;
                 } else {
-                    sum_queries<E>(s, kh, x.t0 + (int64_t)i * d.group, i < count ? (i == count - 1 ? last.n : d.group) : 0, part, qsum[i]);
+                    sum_queries<E, 1>(s, kh, x.t0 + (int64_t)i * d.group, i < count ? (i == count - 1 ? last.n : d.group) : 0, part, qsum[i]);
                 }
             }
             __syncthreads();
@@ -464,20 +504,22 @@ __global__ __launch_bounds__(256) void paged_score_kernel(SelectArgs s) {
                     for (int i = 0; i < NI; ++i) w[u][i] = 64 * i + 4 * sub < d.D ? *(const f32x4*)(m + 64 * i + 4 * sub) : f32x4{0.f, 0.f, 0.f, 0.f};
                     if (!fine) page[u] = -1;
                 }
+                double dot[U * RT];
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int e = e0 + 16 * u;
+                for (int u = 0; u < U; ++u)
 #pragma unroll
                     for (int i = 0; i < RT; ++i) {
-                        double dot = 0.0;
+                        double t = 0.0;
 #pragma unroll
-                        for (int k = 0; k < NI * 4; ++k) dot = fma(q[i][k], (double)w[u][k >> 2][k & 3], dot);
-#pragma unroll
-                        for (int o = 8; o > 0; o >>= 1) dot += __shfl_xor(dot, o);
-                        if (page[u] < 0) dot = -INFINITY;
-                        if (sub == 0 && i < count && e < c1) keys[(int64_t)i * d.kv_heads * d.width + e] = select_key(dot);
+                        for (int k = 0; k < NI * 4; ++k) t = fma(q[i][k], (double)w[u][k >> 2][k & 3], t);
+                        dot[u * RT + i] = t;
                     }
-                }
+                const double score = row_sums<U * RT>(dot, sub);       // of this lane's page and row
+                const int at = sub / (16 / (U * RT)), u = at / RT, i = at % RT, e = e0 + 16 * u;
+                bool fine = false;
+#pragma unroll
+                for (int x = 0; x < U; ++x) fine = x == u ? page[x] >= 0 : fine;
+                if (sub % (16 / (U * RT)) == 0 && i < count && e < c1) keys[(int64_t)i * d.kv_heads * d.width + e] = select_key(fine ? score : -INFINITY);
             }
             __syncthreads();
         }
