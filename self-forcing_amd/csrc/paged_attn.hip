@@ -16,102 +16,20 @@ struct PagedArgs {
     float* lse;
 };
 
-// ------------------------------------------------------------------------------------------------
-// shape-generic kernel (fp32 tensors, head sizes other than 64 and 128): a workgroup takes one query row, 256 positions at a time
-// ------------------------------------------------------------------------------------------------
+// One value of a tensor, four of a row
 template <typename T> struct PElem;
 template <> struct PElem<float> {
     static __device__ __forceinline__ float get(const void* p, int64_t i) { return ((const float*)p)[i]; }
     static __device__ __forceinline__ void put(void* p, int64_t i, float x) { ((float*)p)[i] = x; }
+    static __device__ __forceinline__ void put4(void* p, int64_t i, f32x4 x) { *(f32x4*)((float*)p + i) = x; }
 };
 template <class E> struct PElem16 {
     static __device__ __forceinline__ float get(const void* p, int64_t i) { return E::to_float(((const uint16_t*)p)[i]); }
     static __device__ __forceinline__ void put(void* p, int64_t i, float x) { ((uint16_t*)p)[i] = E::from_float(x); }
+    static __device__ __forceinline__ void put4(void* p, int64_t i, f32x4 x) { *(u32x2*)((uint16_t*)p + i) = u32x2{pack2<E>(x.x, x.y), pack2<E>(x.z, x.w)}; }
 };
 template <> struct PElem<BF16> : PElem16<BF16> {};
 template <> struct PElem<F16> : PElem16<F16> {};
-
-template <typename T>
-__global__ __launch_bounds__(256) void paged_generic_kernel(PagedArgs a) {
-    __shared__ float qs[256];
-    __shared__ float ws[256];
-    __shared__ float red[256];
-    __shared__ int64_t at[256];                    // a position's row in the pools, -1 where the query does not see it
-    const sfm_paged_desc& d = a.d;
-    const int tid = threadIdx.x, t = blockIdx.x, h = blockIdx.y, D = d.D, P = d.page_size;
-    const int r = find_last(d.requests, t, [&](int i) { return (int64_t)clamp_int(a.q_start[i], 0, (int)d.tokens); });
-    if (r >= d.requests && !d.zero_rest) return;
-    const Request rq = request_of(a.q_start, a.past, r, d.requests, (int)d.tokens);
-    const int i = t - rq.first;
-    if (i < 0 || i >= rq.n) return;
-    const KeyTiles k = key_tiles(rq, r >= d.requests, i, i, d.causal, d.window, d.sink, a.cap);
-    const int kh = h / (d.H / d.kv_heads);
-    const int32_t* sel = nullptr;
-    int positions = k.end_max;                     // of the request, or of the selected pages one after the other
-    bool bad = k.beyond && !d.top;
-    if (d.top && r < d.requests) {
-        sel = a.selected + ((first_piece(rq.first, 1, d.group, r) + i / d.group) * d.kv_heads + kh) * d.top;
-        int n = 0;
-        while (n < d.top && sel[n] >= 0) ++n;
-        positions = (int)min((int64_t)n * P, (int64_t)0x7fffffff - 512);
-    }
-    if (tid < D) qs[tid] = PElem<T>::get(a.q, (int64_t)t * d.q_stride[0] + (int64_t)h * d.q_stride[1] + tid);
-    const float sc2 = d.sm_scale * kLog2e;
-    float mrun = -__FLT_MAX__, lrun = 0.f, acc = 0.f;
-    bool seen = false;
-    for (int p0 = 0; p0 < positions; p0 += 256) {
-        const int v = p0 + tid;
-        int64_t row = -1;
-        if (v < positions) {
-            const int e = sel ? sel[v / P] : v / P;
-            const int64_t pos = (int64_t)e * P + v % P;
-            if (pos < k.end_max && (pos >= k.lo_min || pos < d.sink)) {
-                const int page = e < d.width ? a.table[r * d.table_stride + e] : -1;
-                if (page < 0 || page >= d.pages) bad = true;
-                else row = page * d.pool_stride[0] + (int64_t)(v % P) * d.pool_stride[1] + (int64_t)kh * d.pool_stride[2];
-            }
-        }
-        at[tid] = row;
-        __syncthreads();
-        float z = -INFINITY;
-        if (row >= 0) {
-            float s = 0.f;
-            for (int x = 0; x < D; ++x) s += qs[x] * PElem<T>::get(a.kp, row + x);
-            z = s * sc2;
-        }
-        red[tid] = z;
-        const int any = __syncthreads_count(row >= 0);
-        seen = seen || any;
-        for (int s = 128; s > 0; s >>= 1) {
-            if (tid < s) red[tid] = fmaxf(red[tid], red[tid + s]);
-            __syncthreads();
-        }
-        const float mnew = fmaxf(mrun, red[0]);
-        __syncthreads();
-        const float e = row >= 0 ? exp2f(z - mnew) : 0.f;
-        ws[tid] = e;
-        red[tid] = e;
-        __syncthreads();
-        for (int s = 128; s > 0; s >>= 1) {
-            if (tid < s) red[tid] += red[tid + s];
-            __syncthreads();
-        }
-        const float alpha = exp2f(mrun - mnew);
-        lrun = lrun * alpha + red[0];
-        mrun = mnew;
-        if (tid < D) {
-            acc *= alpha;
-            const int cnt = min(256, positions - p0);
-            for (int x = 0; x < cnt; ++x)
-                if (at[x] >= 0) acc += ws[x] * PElem<T>::get(a.vp, at[x] + tid);
-        }
-        __syncthreads();
-    }
-    bad = __syncthreads_or(bad);
-    const float inv = bad ? NAN : seen ? 1.f / lrun : 0.f;
-    if (tid < D) PElem<T>::put(a.out, (int64_t)t * d.o_stride[0] + (int64_t)h * d.o_stride[1] + tid, acc * inv);
-    if (a.lse != nullptr && tid == 0) a.lse[(int64_t)h * d.tokens + t] = bad ? NAN : seen ? (mrun + log2f(lrun)) * kLn2 : -INFINITY;
-}
 
 // ------------------------------------------------------------------------------------------------
 // MFMA kernels (16-bit tensors, head sizes 64 and 128)
@@ -406,7 +324,7 @@ __device__ __forceinline__ bool find_piece(const PagedArgs& a, int64_t piece, in
     return true;
 }
 
-__device__ __forceinline__ BlockMap block_map(const PagedArgs& a, const Piece& p) {
+__device__ __forceinline__ BlockMap block_map(const PagedArgs& a, const Piece& p, int esz) {
     const sfm_paged_desc& d = a.d;
     BlockMap b;
     b.table = a.table + (int64_t)(p.r < d.requests ? p.r : 0) * d.table_stride;
@@ -421,8 +339,8 @@ __device__ __forceinline__ BlockMap block_map(const PagedArgs& a, const Piece& p
     b.width = d.width;
     b.pages = d.pages;
     b.page8 = a.page8;
-    b.page_bytes = d.pool_stride[0] * 2;
-    b.block_bytes = d.pool_stride[1] * 16;
+    b.page_bytes = d.pool_stride[0] * esz;
+    b.block_bytes = d.pool_stride[1] * 8 * esz;
     return b;
 }
 
@@ -444,16 +362,18 @@ __device__ __forceinline__ void wait_queries(u32x4* qb) {
     for (int ds = 0; ds < D / 16; ++ds) asm volatile("" : "+v"(qb[ds]));
 }
 
-// What each of them sees
-__device__ __forceinline__ RowMask row_mask(const PagedArgs& a, const Piece& p, int row0) {
+// What a row sees; of a wave's rows row0 .. + 31, the lane's
+__device__ __forceinline__ RowMask row_mask(const PagedArgs& a, const Piece& p, int row) {
     const sfm_paged_desc& d = a.d;
-    const int row = min(row0 + (int)(threadIdx.x & 31), p.row1 - 1);
     RowMask k;
     k.end = d.causal ? (int)min((int64_t)p.rq.past + row / (d.H / d.kv_heads) + 1, (int64_t)a.cap) : p.k.end_max;
     k.lo = d.window && k.end > d.window ? k.end - d.window : 0;
     k.sink = d.sink;
     k.window = d.window != 0;
     return k;
+}
+__device__ __forceinline__ RowMask lane_mask(const PagedArgs& a, const Piece& p, int row0) {
+    return row_mask(a, p, min(row0 + (int)(threadIdx.x & 31), p.row1 - 1));
 }
 
 // ---- few rows: a wave takes tiles of its own --------------------------------------------------------------------------------
@@ -485,10 +405,10 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(PagedArgs a, int64_t 
     Piece p;
     if (!find_piece<32>(a, rest / chunks, kh, &p)) return;
     const int v0 = min(chunk * chunk_tiles, p.k.tiles), v1 = min(v0 + chunk_tiles, p.k.tiles);
-    const BlockMap map = block_map(a, p);
+    const BlockMap map = block_map(a, p, 2);
     u32x4 qb[D / 16];
     load_queries<E, D>(a, p, p.row0, qb);
-    const RowMask mask = row_mask(a, p, p.row0);
+    const RowMask mask = lane_mask(a, p, p.row0);
     RowState<D> st;
     st.init();
     bool bad = p.k.beyond;
@@ -646,7 +566,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     if (!find_piece<32 * NW>(a, !d.causal ? at : paired ? paired_piece(at, (int)npieces) : npieces - 1 - at, kh, &p)) return;
     const int v0 = min(chunk * chunk_tiles, p.k.tiles), v1 = min(v0 + chunk_tiles, p.k.tiles);
     const int f0 = max(v0, p.k.fast0), nf = max(min(v1, p.k.fast1) - f0, 0) & ~1;      // the loop over whole tiles takes two at a time
-    const BlockMap map = block_map(a, p);
+    const BlockMap map = block_map(a, p, 2);
     bool bad = p.k.beyond;
 
     const uint32_t row_bytes = (uint32_t)d.pool_stride[1] * 2;
@@ -850,7 +770,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         const int e0 = idle || !d.causal ? p.k.end_max : (int)min((int64_t)p.rq.past + w0 / G + 1, (int64_t)a.cap);
         const int e1 = idle || !d.causal ? p.k.end_max : (int)min((int64_t)p.rq.past + w1 / G + 1, (int64_t)a.cap);
         const int lo = d.window && e1 > d.window ? e1 - d.window : 0;
-        const RowMask mask = row_mask(a, p, w0);
+        const RowMask mask = lane_mask(a, p, w0);
         // places: behind those of the last stretch's whole tiles, as far as they went with it
         int base = ready ? (nf - 1) % RowsLds<D, NW>::kStretch + 1 : 0, held = ready ? min(rest, RowsLds<D, NW>::kStretch - base) : 0, first = 0;
         for (int u = 0; u < rest; ++u) {
@@ -893,14 +813,154 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     store_rows<E, D>(a, p, st, bad, p.row0 + wave * 32, chunk, chunks, part, lds + wave * 32 * (2 * D + 16));
 }
 
-// Combines the partials of a row: D / 4 lanes hold four channels each.  Bound by reading the partials once.
-template <class E, int D>
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a, const float* __restrict__ part, int chunks) {
-    constexpr int CH = D / 4;
+// ---- other types and head sizes --------------------------------------------------------------------------------------------------
+//
+// fp32 tensors, head sizes other than 64 and 128, without matrix instructions.  A workgroup takes a piece of 4 rows and 256 positions at a
+// time: a thread one position's logits of the four rows, then 16 bytes of every so many V rows, so that each K and V row is read once
+// per piece.  32 tokens on 4000 positions, 16 heads of 256 on 4, bf16: 193 us, 2.7 TB/s, the threads' loads of whole K rows (lines that 16
+// loads of a thread share) ahead of the arithmetic; 1000 tokens on 4000 before them, 12 heads of 96: 790 us, fp32 multiplications.
+constexpr int kAnyRows = 4;
+
+template <typename T>
+__global__ __launch_bounds__(256) void paged_generic_kernel(PagedArgs a, int64_t npieces, int chunks, int chunk_tiles, float* part) {
+    constexpr int N = Chunk<T>::kN, M = kAnyRows, kEsz = 16 / N;
+    __shared__ float qs[M][256];
+    __shared__ f32x4 ws[256];                      // a position's weights, -1 in rows that do not see it
+    __shared__ int64_t at[256];                    // a position's row in a head's rows of the pools, in bytes; -1 where nobody sees it
+    __shared__ float red[4][M], sums[4][M];
+    __shared__ float sum[256 * N];
     const sfm_paged_desc& d = a.d;
-    const int64_t rows = d.tokens * d.H, row = (int64_t)blockIdx.x * (256 / CH) + threadIdx.x / CH;
-    const int ch = threadIdx.x % CH;
-    if (row >= rows) return;
+    const int tid = threadIdx.x, wave = tid >> 6, D = d.D, G = d.H / d.kv_heads;
+    const int kh = blockIdx.x % d.kv_heads, rest = blockIdx.x / d.kv_heads, chunk = rest % chunks;
+    Piece p;
+    if (!find_piece<M>(a, rest / chunks, kh, &p)) return;
+    const int v0 = min(chunk * chunk_tiles, p.k.tiles) * 64, v1 = min(chunk * chunk_tiles + chunk_tiles, p.k.tiles) * 64;
+    const BlockMap map = block_map(a, p, kEsz);
+    RowMask mask[M];
+#pragma unroll
+    for (int r = 0; r < M; ++r) mask[r] = row_mask(a, p, min(p.row0 + r, p.row1 - 1));
+    for (int i = tid; i < M * D; i += 256) {
+        const int r = i / D, x = i - r * D, row = min(p.row0 + r, p.row1 - 1), t = row / G;
+        qs[r][x] = PElem<T>::get(a.q, (int64_t)(p.rq.first + t) * d.q_stride[0] + (int64_t)(kh * G + row - t * G) * d.q_stride[1] + x);
+    }
+    const char* const kg = (const char*)a.kp + (int64_t)kh * d.pool_stride[2] * kEsz;
+    const char* const vg = (const char*)a.vp + (int64_t)kh * d.pool_stride[2] * kEsz;
+    const int nc = D / N, groups = 256 / nc, g = tid / nc, c = tid - g * nc;           // of V: 16 bytes c of positions g, g + groups, ...
+    const float sc2 = d.sm_scale * kLog2e;
+    float mrun[M], lrun[M], acc[M][N];
+    bool seen[M], bad = p.k.beyond;
+#pragma unroll
+    for (int r = 0; r < M; ++r) {
+        mrun[r] = -__FLT_MAX__;
+        lrun[r] = 0.f;
+        seen[r] = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[r][i] = 0.f;
+    }
+    for (int p0 = v0; p0 < v1; p0 += 256) {
+        const int v = p0 + tid;
+        int64_t row = -1;
+        int pos = kNoPos;
+        if (v < v1) {
+            uint32_t off8;
+            const int e = map.entry(v >> 3, &off8, &pos), page = map.page(e);
+            bad = bad || (e >= 0 && page < 0);
+            if (page >= 0) row = map.offset(page, off8) + (v & 7) * (d.pool_stride[1] * kEsz);
+            pos += v & 7;
+        }
+        __syncthreads();                           // the last step's weights are used; the queries are there
+        float z[M] = {0.f, 0.f, 0.f, 0.f};
+        if (row >= 0) {
+#pragma unroll 4
+            for (int x = 0; x < nc; ++x) {
+                float k[N];
+                Chunk<T>::get(*(const u32x4*)(kg + row + 16 * x), k);
+#pragma unroll
+                for (int r = 0; r < M; ++r)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) z[r] = fmaf(qs[r][x * N + i], k[i], z[r]);
+            }
+        }
+        bool see[M];
+#pragma unroll
+        for (int r = 0; r < M; ++r) {
+            see[r] = row >= 0 && mask[r].sees(pos);
+            seen[r] = seen[r] || see[r];
+            z[r] = see[r] ? z[r] * sc2 : -INFINITY;
+            float m = z[r];
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+            if ((tid & 63) == 0) red[wave][r] = m;
+        }
+        at[tid] = row;
+        __syncthreads();
+        f32x4 w;
+#pragma unroll
+        for (int r = 0; r < M; ++r) {
+            const float mnew = fmaxf(fmaxf(mrun[r], fmaxf(red[0][r], red[1][r])), fmaxf(red[2][r], red[3][r]));
+            const float e = see[r] ? exp2f(z[r] - mnew) : 0.f, alpha = exp2f(mrun[r] - mnew);
+            w[r] = see[r] ? e : -1.f;
+            lrun[r] = lrun[r] * alpha + e;
+            mrun[r] = mnew;
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[r][i] *= alpha;
+        }
+        ws[tid] = w;
+        __syncthreads();
+        const int count = min(256, v1 - p0);
+        if (g < groups)
+#pragma unroll 4
+            for (int x = g; x < count; x += groups) {
+                if (at[x] < 0) continue;
+                const f32x4 wx = ws[x];
+                float val[N];
+                Chunk<T>::get(*(const u32x4*)(vg + at[x] + 16 * c), val);
+#pragma unroll
+                for (int r = 0; r < M; ++r)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) acc[r][i] = wx[r] < 0.f ? acc[r][i] : fmaf(wx[r], val[i], acc[r][i]);
+            }
+    }
+    bad = __syncthreads_or(bad);
+#pragma unroll
+    for (int r = 0; r < M; ++r) {
+        float l = lrun[r];
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+        if ((tid & 63) == 0) sums[wave][r] = l;
+    }
+#pragma unroll
+    for (int r = 0; r < M; ++r) {
+        if (g < groups)
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum[(g * nc + c) * N + i] = acc[r][i];
+        const bool any = __syncthreads_or(seen[r]);
+        const int row = p.row0 + r, t = p.rq.first + row / G, h = kh * G + row % G;
+        if (row < p.row1) {
+            const float l = sums[0][r] + sums[1][r] + sums[2][r] + sums[3][r];
+            const int64_t rows = d.tokens * d.H, to = chunk * rows + (int64_t)t * d.H + h;
+            float o = 0.f;
+            if (tid < D)
+                for (int j = 0; j < groups; ++j) o += sum[j * D + tid];
+            if (part != nullptr) {
+                if (any && tid < D) part[to * D + tid] = o;
+                if (tid == 0) store_partial(part + chunks * rows * D + to * 2, mrun[r], l, any, bad);
+            } else {
+                if (tid < D) PElem<T>::put(a.out, (int64_t)t * d.o_stride[0] + (int64_t)h * d.o_stride[1] + tid, bad ? NAN : any ? o / l : 0.f);
+                if (a.lse != nullptr && tid == 0) a.lse[(int64_t)h * d.tokens + t] = bad ? NAN : any ? (mrun[r] + log2f(l)) * kLn2 : -INFINITY;
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Combines the partials of a row: D / 4 lanes hold four channels each.  Bound by reading the partials once.  SIZE 0: any head size
+template <class T, int SIZE>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a, const float* __restrict__ part, int chunks) {
+    const sfm_paged_desc& d = a.d;
+    const int D = SIZE ? SIZE : d.D, CH = D / 4, per = 256 / CH, mine = threadIdx.x / CH, ch = threadIdx.x - mine * CH;
+    const int64_t rows = d.tokens * d.H, row = (int64_t)blockIdx.x * per + mine;
+    if (mine >= per || row >= rows) return;
     const int64_t t = row / d.H;
     const int h = (int)(row - t * d.H);
     if (!d.zero_rest && t >= clamp_int(a.q_start[d.requests], 0, (int)d.tokens)) return;       // rows of nobody
@@ -920,8 +980,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a, const flo
         o += *(const f32x4*)(part + (c * rows + row) * D + 4 * ch) * f;
     }
     const float inv = seen ? 1.f / sum : 0.f;                          // NaN sums make the row NaN
-    *(u32x2*)((uint16_t*)a.out + t * d.o_stride[0] + h * d.o_stride[1] + 4 * ch) =
-        u32x2{pack2<E>(o.x * inv, o.y * inv), pack2<E>(o.z * inv, o.w * inv)};
+    PElem<T>::put4(a.out, t * d.o_stride[0] + h * d.o_stride[1] + 4 * ch, o * inv);
     if (a.lse != nullptr && ch == 0) a.lse[(int64_t)h * d.tokens + t] = seen ? (M + log2f(sum)) * kLn2 : -INFINITY;
 }
 
@@ -935,7 +994,6 @@ struct PagedPlan {
 };
 static PagedPlan paged_plan(const sfm_paged_desc& d) {
     PagedPlan p{0, 0, 1, 0, false, false};
-    if (d.dtype == SFM_F32 || (d.D != 64 && d.D != 128)) return p;
     const int64_t G = d.H / d.kv_heads, cu = cu_count();
     // rows of a request (of a group of tokens) and key head, on average, and pieces that have rows
     const int64_t mean = std::max<int64_t>(1, d.top ? std::min<int64_t>(d.group, d.tokens) * G : d.tokens * G / d.requests);
@@ -953,13 +1011,16 @@ static PagedPlan paged_plan(const sfm_paged_desc& d) {
     // requests of 1024 on 1024, 92 -> 79); with more pieces than that the order of their lengths balances them better (8192 tokens, 32 heads
     // on 8, 556 us and 586), and behind a long cache they are much alike.
     const int64_t cap = (int64_t)d.width * d.page_size;
-    const bool prompts = d.causal && !d.top && mean > 128 && items(128) <= 2 * cu;
-    p.rows = mean <= 32 ? 32 : wide(items(256)) && !(prompts && cap <= 4 * d.tokens / d.requests) ? 256 : 128;
+    const bool prompts = d.causal && !d.top && mean > 128 && items(128) <= 2 * cu, mfma = d.dtype != SFM_F32 && (d.D == 64 || d.D == 128);
+    p.rows = !mfma ? 0 : mean <= 32 ? 32 : wide(items(256)) && !(prompts && cap <= 4 * d.tokens / d.requests) ? 256 : 128;
     p.paired = prompts && p.rows == 128;
-    p.pieces = d.top ? pieces(d.tokens, d.group, d.requests) * ((std::min<int64_t>(d.group, d.tokens) * G + p.rows - 1) / p.rows) : pieces(d.tokens * G, p.rows, d.requests);
-    const int64_t tiles = ((d.top ? (int64_t)d.top * d.page_size : cap) + 63) / 64, n = items(p.rows);
+    const int64_t per = mfma ? p.rows : kAnyRows;
+    p.pieces = d.top ? pieces(d.tokens, d.group, d.requests) * ((std::min<int64_t>(d.group, d.tokens) * G + per - 1) / per) : pieces(d.tokens * G, per, d.requests);
+    const int64_t tiles = ((d.top ? (int64_t)d.top * d.page_size : cap) + 63) / 64, n = items(per);
     int64_t chunks = 1;
-    if (p.rows == 32) {
+    if (!mfma) {               // a step is 256 positions; one token on 1560, 12 heads of 128 fp32: in 7 ranges 33 us, in 2 76
+        chunks = std::min<int64_t>((4 * cu + n - 1) / n, (tiles + 3) / 4);
+    } else if (p.rows == 32) {
         chunks = std::min<int64_t>((8 * cu + n - 1) / n, (tiles + 7) / 8);
         // More rows than twice the memory-side cache (256 MB) holds, and each read once: past it, 848 MB (up to 2 GB by the table's width)
         // 193 -> 175 us; 134 MB that lie in it 38 -> 44
@@ -985,6 +1046,7 @@ static PagedPlan paged_plan(const sfm_paged_desc& d) {
     }
     chunks = std::max<int64_t>(1, std::min<int64_t>(chunks, 64));
     p.chunk_tiles = (int)((tiles + chunks - 1) / chunks);
+    if (!mfma) p.chunk_tiles = (p.chunk_tiles + 3) / 4 * 4;            // whole steps
     p.chunks = (int)((tiles + p.chunk_tiles - 1) / p.chunk_tiles);
     return p;
 }
@@ -1008,14 +1070,23 @@ static int launch_status() {
     return SFM_ERR_HIP;
 }
 
+template <class T, int SIZE>
+static int launch_merge(const PagedArgs& a, const PagedPlan& p, const float* part, hipStream_t stream) {
+    const int64_t rows = a.d.tokens * a.d.H, per = 1024 / a.d.D;
+    if (part != nullptr) hipLaunchKernelGGL((paged_merge_kernel<T, SIZE>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, stream, a, part, p.chunks);
+    return launch_status();
+}
+
+template <class T>
+static int launch_generic(const PagedArgs& a, const PagedPlan& p, float* part, hipStream_t stream) {
+    hipLaunchKernelGGL(paged_generic_kernel<T>, dim3((unsigned)(p.pieces * a.d.kv_heads * p.chunks)), dim3(256), 0, stream, a, p.pieces, p.chunks, p.chunk_tiles, part);
+    return launch_merge<T, 0>(a, p, part, stream);
+}
+
 template <class E, int D>
-static int launch_mfma(const PagedArgs& a, PagedPlan p, float* part, hipStream_t stream) {
+static int launch_mfma(const PagedArgs& a, const PagedPlan& p, float* part, hipStream_t stream) {
     const sfm_paged_desc& d = a.d;
     const int64_t total = p.pieces * d.kv_heads * p.chunks;
-    if (total >= (1 << 23)) {
-        set_error("%lld pieces of rows, heads and ranges are more than a launch takes", (long long)total);
-        return SFM_ERR_UNSUPPORTED;
-    }
     auto go = [&](auto kern, int nw, size_t lds) -> int {
         const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) {
@@ -1027,12 +1098,7 @@ static int launch_mfma(const PagedArgs& a, PagedPlan p, float* part, hipStream_t
     };
     const int rc = p.rows == 32 ? go(p.once ? paged_few_kernel<E, D, true> : paged_few_kernel<E, D, false>, 4, FewLds<D>::kTotal + 4 * 96 * sizeof(float))
                    : p.rows == 128 ? go(paged_rows_kernel<E, D, 4>, 4, RowsLds<D, 4>::kTotal) : go(paged_rows_kernel<E, D, 8>, 8, RowsLds<D, 8>::kTotal);
-    if (rc) return rc;
-    if (part != nullptr) {
-        const int64_t rows = d.tokens * d.H, per = 1024 / D;
-        hipLaunchKernelGGL((paged_merge_kernel<E, D>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, stream, a, (const float*)part, p.chunks);
-    }
-    return launch_status();
+    return rc ? rc : launch_merge<E, D>(a, p, part, stream);
 }
 
 int launch_paged_attention(const sfm_paged_desc& d, const void* q, const void* kp, const void* vp, const int32_t* table,
@@ -1040,22 +1106,19 @@ int launch_paged_attention(const sfm_paged_desc& d, const void* q, const void* k
                            size_t workspace_bytes, hipStream_t stream) {
     PagedArgs a{d, fast_div(d.page_size / 8), d.width * d.page_size, q, kp, vp, table, past, q_start, selected, out, lse};
     PagedPlan p = paged_plan(d);
-    if (p.rows) {
-        if (p.chunks > 1 && (!workspace || workspace_bytes < paged_workspace_bytes(d))) {      // whole, then
-            p.chunk_tiles *= p.chunks;
-            p.chunks = 1;
-        }
-        float* const part = p.chunks > 1 ? (float*)workspace : nullptr;
-        if (d.dtype == SFM_BF16) return d.D == 128 ? launch_mfma<BF16, 128>(a, p, part, stream) : launch_mfma<BF16, 64>(a, p, part, stream);
-        return d.D == 128 ? launch_mfma<F16, 128>(a, p, part, stream) : launch_mfma<F16, 64>(a, p, part, stream);
+    if (p.chunks > 1 && (!workspace || workspace_bytes < paged_workspace_bytes(d))) {          // whole, then
+        p.chunk_tiles *= p.chunks;
+        p.chunks = 1;
     }
-    if (d.tokens >= (1 << 24) || d.H > 65535) {
-        set_error("tokens=%lld, H=%d are more than a launch takes", (long long)d.tokens, d.H);
+    const int64_t total = p.pieces * d.kv_heads * p.chunks;
+    if (total >= (1 << 23)) {
+        set_error("%lld pieces of rows, heads and ranges are more than a launch takes", (long long)total);
         return SFM_ERR_UNSUPPORTED;
     }
-    auto kern = d.dtype == SFM_BF16 ? paged_generic_kernel<BF16> : d.dtype == SFM_F16 ? paged_generic_kernel<F16> : paged_generic_kernel<float>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)d.tokens, d.H), dim3(256), 0, stream, a);
-    return launch_status();
+    float* const part = p.chunks > 1 ? (float*)workspace : nullptr;
+    if (!p.rows) return d.dtype == SFM_BF16 ? launch_generic<BF16>(a, p, part, stream) : d.dtype == SFM_F16 ? launch_generic<F16>(a, p, part, stream) : launch_generic<float>(a, p, part, stream);
+    if (d.dtype == SFM_BF16) return d.D == 128 ? launch_mfma<BF16, 128>(a, p, part, stream) : launch_mfma<BF16, 64>(a, p, part, stream);
+    return d.D == 128 ? launch_mfma<F16, 128>(a, p, part, stream) : launch_mfma<F16, 64>(a, p, part, stream);
 }
 
 }  // namespace sfm

@@ -187,26 +187,6 @@ struct WriteArgs {
     int mean_wgs;
 };
 
-template <typename T> struct Chunk;                // 16 bytes <-> floats
-template <> struct Chunk<float> {
-    static constexpr int kN = 4;
-    static __device__ __forceinline__ void get(u32x4 w, float* x) {
-        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
-    }
-};
-template <class E> struct Chunk16 {
-    static constexpr int kN = 8;
-    static __device__ __forceinline__ void get(u32x4 w, float* x) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = E::to_float((uint16_t)(w[i] & 0xffffu));
-            x[2 * i + 1] = E::to_float((uint16_t)(w[i] >> 16));
-        }
-    }
-};
-template <> struct Chunk<BF16> : Chunk16<BF16> {};
-template <> struct Chunk<F16> : Chunk16<F16> {};
-
 // The mean key of one page, of one head: the page'th that a step's requests write to.  A request of n tokens writes to at most
 // (n - 1) / page_size + 2 pages; its first has number q_start / page_size + 2 r, which leaves it as many.  New rows are taken from
 // k, whatever the copying workgroups have done by then.  The rows are summed by groups of lanes, a row each, joined in LDS in

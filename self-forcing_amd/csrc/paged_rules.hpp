@@ -115,6 +115,26 @@ struct BlockMap {
 };
 
 #if defined(__HIPCC__)
+template <typename T> struct Chunk;                // 16 bytes <-> floats
+template <> struct Chunk<float> {
+    static constexpr int kN = 4;
+    static __device__ __forceinline__ void get(u32x4 w, float* x) {
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
+    }
+};
+template <class E> struct Chunk16 {
+    static constexpr int kN = 8;
+    static __device__ __forceinline__ void get(u32x4 w, float* x) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = E::to_float((uint16_t)(w[i] & 0xffffu));
+            x[2 * i + 1] = E::to_float((uint16_t)(w[i] >> 16));
+        }
+    }
+};
+template <> struct Chunk<BF16> : Chunk16<BF16> {};
+template <> struct Chunk<F16> : Chunk16<F16> {};
+
 // The last r in [0, R] with at(r) <= v, R standing for the rows behind the last request: at ascends from at(0) <= v, and a wave looks
 // at 64 of its values at a time.  The same in every lane; some r in [0, R] where the values make no sense.
 template <class F>

@@ -72,6 +72,25 @@ def test_other_types_and_head_sizes(past, n, page, H, Hk, pad, causal, D, dtype)
     check(past, n, page, H, Hk, D, dtype, pad, causal=causal)
 
 
+OTHER = [(torch.float32, 64, 4, 2), (torch.bfloat16, 256, 5, 1), (torch.float16, 96, 2, 2), (torch.bfloat16, 8, 12, 1)]
+
+
+@pytest.mark.parametrize("dtype,D,H,Hk", OTHER, ids=str)
+@pytest.mark.parametrize("window,sink", [(None, 0), (1000, 0), (1000, 70), (3, 1)])
+@pytest.mark.parametrize("past,n,page", [([9000, 100], [1, 1], 16), ([700, 5], [9, 30], 40)])
+def test_other_types_and_head_sizes_with_windows(past, n, page, window, sink, dtype, D, H, Hk):
+    check(past, n, page, H, Hk, D, dtype, 3, causal=True, window=window, sink=sink)
+
+
+@pytest.mark.parametrize("dtype,D,H,Hk", OTHER, ids=str)
+@pytest.mark.parametrize("past,n,page,group,top", [([9000, 100], [1, 1], 16, 1, 200), ([700, 5], [9, 30], 8, 7, 9)])
+def test_other_types_and_head_sizes_of_selected_pages(past, n, page, group, top, dtype, D, H, Hk):
+    plan, table, q_start, q, kp, vp = inputs(past, n, page, H, Hk, D, dtype, pad=3)
+    sel = lists(past, n, page, Hk, top, group, True, q.shape[0], q_start, 5, first=False)
+    got, lse = PA.paged_attention(q.to(DEV), kp.to(DEV), vp.to(DEV), plan, causal=True, selected=ints(sel.tolist()), group=group, return_lse=True)
+    close(got.cpu(), lse.cpu(), oracle.attention(q, kp, vp, table, torch.tensor(past), q_start, causal=True, selected=sel, group=group), dtype)
+
+
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("window,sink", [(1, 0), (1, 1), (64, 0), (100, 3), (100, 70), (128, 200), (5000, 9), (65, 64), (37, 500)])
 @pytest.mark.parametrize("causal", [False, True])
@@ -585,6 +604,7 @@ def test_every_kernel_is_reached_by_the_tests_above():
     assert rows == 32 and ranges > 1 and once == 1
     assert of([100], [300], 40, 2, 2) == (128, 1, 0)
     assert of([300, 10], [70, 129], 8, 5, 1)[0] == 128
+    assert of([9000, 100], [1, 1], 16, 5, 1, 256)[1] > 1                         # test_other_types_and_head_sizes_with_windows
     assert of([63], [1], 64, 2, 2, 40)[0] == 0 and of([63], [1], 64, 2, 2, 64, torch.float32)[0] == 0
 
 
