@@ -382,7 +382,9 @@ __device__ __forceinline__ RowMask lane_mask(const PagedArgs& a, const Piece& p,
 // with a K and a V buffer that no other wave sees and no barrier: while a wave works on K the V rows are on their way, and the next
 // K's as soon as its last is read.  Two workgroups share a compute unit, so that the one's start (its piece, table entries, first
 // rows) is behind the other's loads.  Bound by reading the cache: of the matrix instructions' 32 columns a single token uses the
-// query heads of its key head, and they take an eighth of the time that the rows do.
+// query heads of its key head, and they take a tenth of the time that the rows do.  32 tokens on 100 to 16000 positions, 32 heads on 8 of 128, pages
+// of 16: 848 MB in 167 us, 5.1 TB/s (a bare read 5.8).  One token on 1560 positions, 12 heads: 11 us, of which its bytes take 2: launch, the request, its
+// table, first rows and the last tile are waited for one after the other.
 template <int D>
 struct FewLds {
     static constexpr int kMat = DnLds<D>::kMat / 2, kWave = 2 * kMat, kTotal = 4 * kWave;
@@ -537,7 +539,13 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(PagedArgs a, int64_t 
 // some row sees in part (the request's own new tokens under a causal mask, a window's edge, the last tile) follow in a plain loop.
 // Where the whole tiles' blocks lie is worked out by all threads together and kept in LDS, 8 bytes a block, for a stretch of tiles at a
 // time (a request's page table row is read once per workgroup, not once per wave); a step reads one tile's eight offsets, a
-// step before it asks for that tile, and V's rows take the offsets that K's were read with.
+// step before it asks for that tile, and V's rows take the offsets that K's were read with.  (Looked up by each wave as it went, eight tiles at a
+// time, they took scalar registers and a branch from the loop: 4680 x 32760 of 12 heads 1185 us, with places in LDS and better chosen ranges 918.)
+// Masking inside that loop would save the plain one, and spills.
+//
+// Bound at D = 128 by the matrix pipes and the clock that they leave (58 % of the cycles busy; 4680 x 32760 of 12 heads 902 us, 1.04 PFLOP/s,
+// the dense kernel on a contiguous cache 887), at D = 64 by the vector pipes: 32 exponentials of 16 cycles and some 100 instructions of 4
+// per tile and wave.  A tile of the plain loop takes two to three times as long as one of the other.
 template <int D, int NW>
 struct RowsLds {
     static constexpr int kPlaces = 4 * DnLds<D, NW>::kMat;                     // behind the tiles
