@@ -509,6 +509,47 @@ def test_another_stream_and_a_graph(n):
             assert torch.equal(a, b), i
 
 
+@pytest.mark.parametrize("D,dtype", [(128, torch.bfloat16), (64, torch.float16), (96, torch.bfloat16)], ids=str)
+def test_decoding_steps_of_one_graph(D, dtype):
+    """A step that moves its own lengths and list of free pages on, replayed: every step the bits of the eager one, over pages' and tiles' ends."""
+    page, H, Hk, R, W, steps = 16, 8, 2, 3, 40, 40
+    g = torch.Generator().manual_seed(3)
+    pages = R * W
+    free = ints(torch.randperm(pages, generator=g).tolist())
+    new, (q, k, v) = ints([1, 0, 1]), (torch.zeros((3, h, D), dtype=dtype, device=DEV) for h in (H, Hk, Hk))
+
+    def state():
+        prompt = PA.plan_pages(torch.full((R, W), -1, dtype=torch.int32, device=DEV), ints([0] * R), ints([250, 9, 30]), free, 289, page)
+        kp, vp = (torch.full((pages, page, Hk, D), math.nan, dtype=dtype, device=DEV) for _ in range(2))
+        means = torch.zeros((pages, Hk, D), device=DEV)
+        PA.write_pages(*(randn((289, Hk, D), s, dtype).to(DEV) for s in (1, 2)), kp, vp, prompt, means=means)
+        return prompt.table, prompt.lengths.clone(), prompt.next_free.clone(), kp, vp, means
+
+    def run(table, past, taken, kp, vp, means):
+        plan = PA.plan_pages(table, past, new, free, 3, page, next_free=taken)
+        PA.write_pages(k, v, kp, vp, plan, means=means)
+        out, lse = PA.paged_attention(q, kp, vp, plan, causal=True, return_lse=True)
+        sel = PA.select_pages(q, means, plan, 5, causal=True)
+        some = PA.paged_attention(q, kp, vp, plan, causal=True, selected=sel)
+        torch.add(plan.lengths, 0, out=past)
+        torch.add(plan.next_free, 0, out=taken)
+        return plan.slots, out, lse, sel, some
+    eager, replayed = state(), state()
+    run(*state())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(*replayed)
+    for i in range(steps):
+        for t, s in ((q, 100), (k, 200), (v, 300)):
+            t.copy_(randn(t.shape, s + i, dtype).to(DEV))
+        want = run(*eager)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a.nan_to_num(7), b.nan_to_num(7)) if a.is_floating_point() else torch.equal(a, b) for a, b in zip(got, want)), i
+        assert want[1][:2].isfinite().all() and not want[1][2].any()           # two rows, and one of nobody
+    assert replayed[1].tolist() == [250 + steps, 9, 30 + steps] and torch.equal(replayed[0], eager[0]) and torch.equal(replayed[2], eager[2])
+
+
 def test_calls_at_once_on_two_streams():
     """Each call has a workspace of its own (ranges of keys, scores): the same bits as one after the other."""
     def make(seed):
