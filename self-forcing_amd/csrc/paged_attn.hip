@@ -82,11 +82,30 @@ struct RowMask {
     __device__ __forceinline__ bool sees(int pos) const { return pos < end && (!window || pos >= lo || pos < sink); }
 };
 
+// Which V rows of a tile hold values that are not finite, a bit each: of rows r0 + lane / LPR, LPR lanes to a row.
+template <class E, int D, int LPR>
+__device__ __forceinline__ uint64_t odd_rows(const char* lds, uint32_t vbuf, int r0) {
+    using L = DnLds<D>;
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    constexpr uint16_t kInf = E::kDtype == SFM_BF16 ? 0x7f80 : 0x7c00;
+    const int lane = threadIdx.x & 63, r = r0 + lane / LPR, c0 = lane % LPR;
+    u16x2 top = {0, 0};                                                // largest magnitude's bits
+#pragma unroll 4
+    for (int c = 0; c < L::kCPR / LPR; ++c) {                          // neighbouring rows begin at different chunks: apart in the banks
+        const u32x4 w = *(const u32x4*)(lds + vbuf + (uint32_t)r * L::kPitch + (uint32_t)((c0 + LPR * ((c + r) % (L::kCPR / LPR))) << 4));
+#pragma unroll
+        for (int x = 0; x < 4; ++x) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[x] & 0x7fff7fffu));
+    }
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(max(top.x, top.y) >= kInf);
+    if (LPR == 1) return hit;
+    return __builtin_amdgcn_ballot_w64(lane < 64 / LPR && ((hit >> (lane * LPR & 63)) & ((1u << LPR) - 1)) != 0);
+}
+
 // A tile of 32 NB keys in LDS against the wave's rows: logits, masks, weights and V's part.  pos: first positions of its blocks.
 // The second half waits for V through `v_ready`, so that K's buffer can be refilled meanwhile (`k_done`).
 //
-// A masked weight is 0, and 0 times an infinity or NaN is NaN: in a masked tile V rows that hold such values are left out of the
-// matrix product and added for the rows that see them, one by one.  (Stale rows, and later tokens of the request.)
+// A masked weight is 0, and 0 times an infinity or NaN is NaN: in a masked tile V rows that hold such values (`v_ready` tells which) are left out
+// of the matrix product and added for the rows that see them, one by one.  (Stale rows, and later tokens of the request.)
 template <class E, int D, int NB, class KDone, class VReady>
 __device__ __forceinline__ void masked_tile(const char* lds, uint32_t kbuf, uint32_t vbuf, const u32x4* qb, float sc2, RowState<D>& st,
                                             const RowMask& mask, bool masked, const int* pos, KDone k_done, VReady v_ready) {
@@ -148,21 +167,8 @@ __device__ __forceinline__ void masked_tile(const char* lds, uint32_t kbuf, uint
         pb[i >> 3][(i >> 1) & 3] = pack2<E>(a, b);
     }
     st.lrun += psum;
-    v_ready();
-    // V rows with values that are not finite, a lane each
-    uint64_t odd = 0;
-    if (masked) {
-        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-        constexpr uint16_t kInf = E::kDtype == SFM_BF16 ? 0x7f80 : 0x7c00;
-        u16x2 top = {0, 0};                                            // largest magnitude's bits
-#pragma unroll 4
-        for (int c = 0; c < L::kCPR; ++c) {
-            const u32x4 w = *(const u32x4*)(lds + vbuf + (uint32_t)(lane % (32 * NB)) * L::kPitch + (uint32_t)(((c + lane) % L::kCPR) << 4));
-#pragma unroll
-            for (int x = 0; x < 4; ++x) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[x] & 0x7fff7fffu));
-        }
-        odd = __builtin_amdgcn_ballot_w64(max(top.x, top.y) >= kInf) & (NB == 2 ? ~(uint64_t)0 : 0xffffffffu);
-    }
+    uint64_t odd = v_ready();
+    if (!masked) odd = 0;
     uint32_t trA[2];
     const int s16 = lane & 15, rl = 4 * hf + (s16 >> 2), cl = 2 * ((lane >> 4) & 1) + ((s16 & 3) >> 1);
 #pragma unroll
@@ -191,12 +197,12 @@ __device__ __forceinline__ void masked_tile(const char* lds, uint32_t kbuf, uint
     while (odd) {
         const int l = __builtin_ctzll(odd);
         odd &= odd - 1;
-        // the weight lies in half (l / 4) % 2, register 16 (l / 32) + 4 (l / 8 % 4) + l % 4
-        float w = 0.f;
+        // the weight, rounded as the matrix product takes it, lies in half (l / 4) % 2, number 16 (l / 32) + 4 (l / 8 % 4) + l % 4
+        uint32_t both = 0;
         const int at = 16 * (l >> 5) + 4 * ((l >> 3) & 3) + (l & 3);
 #pragma unroll
-        for (int i = 0; i < 16 * NB; ++i) w = i == at ? s[i >> 4][i & 15] : w;
-        w = __shfl(w, m + 32 * ((l >> 2) & 1));
+        for (int i = 0; i < 8 * NB; ++i) both = i == at >> 1 ? pb[i >> 2][i & 3] : both;
+        const float w = __shfl(E::to_float((uint16_t)(both >> (16 * (at & 1)))), m + 32 * ((l >> 2) & 1));
         int p = kNoPos;
 #pragma unroll
         for (int i = 0; i < 4 * NB; ++i) p = i == (l >> 3) ? pos[i] : p;
@@ -473,6 +479,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(PagedArgs a, int64_t 
             [&]() {
                 if (next) wait_loads<kLoads>();
                 else wait_loads<0>();
+                return masked ? odd_rows<E, D, 2>(lds, buf + FewLds<D>::kMat, 0) : (uint64_t)0;
             });
         lds_wave_sync();
         if (next) stage(vg, i + 1, buf + FewLds<D>::kMat);
@@ -814,7 +821,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
                 some = some || pos[b] < e1;
                 all = all && pos[b] < e0 - 7 && (pos[b] >= lo || pos[b] + 7 < d.sink);
             }
-            if (!idle && some) masked_tile<E, D, 2>(lds, L::kK + buf, L::kV + buf, qb, sc2, st, mask, !all, pos, [] {}, [] {});
+            if (!idle && some)
+                masked_tile<E, D, 2>(lds, L::kK + buf, L::kV + buf, qb, sc2, st, mask, !all, pos, [] {}, [&]() { return all ? (uint64_t)0 : odd_rows<E, D, 1>(lds, L::kV + buf, 0); });
         }
     }
     __syncthreads();                               // the tiles are dead: rows leave through LDS
