@@ -32,12 +32,14 @@ template <> struct PElem<BF16> : PElem16<BF16> {};
 template <> struct PElem<F16> : PElem16<F16> {};
 
 // ------------------------------------------------------------------------------------------------
-// MFMA kernels (16-bit tensors, head sizes 64 and 128)
+// out = softmax(sm_scale q K^T) V in one pass over the keys: with m the running maximum of a row's logits, l = sum exp(x - m) and
+// O = sum exp(x - m) v, both scaled by exp(m_old - m) where m grows; out = O / l, and m + log l beside it.  Logits are in units of log 2.
 //
-// A piece is up to 32 NW rows (token, query head) of one request and one key head.  Its keys come in virtual tiles of 64 positions
-// (KeyTiles), or of the selected pages one after the other; eight positions, a block, never straddle a page.  A lane works out where
-// one block lies, for eight tiles at a time, and a load of K or V rows takes its block's offset from that lane.  The products
-// are those of the dense kernel: S^T[l, q] = K[l,:] . Q[q,:], O^T[d, q] += V^T[d, l] P^T[l, q], a lane holds one row's logits.
+// A piece is up to M rows (token, query head) of one request and one key head.  Its keys come in virtual tiles of 64 positions
+// (KeyTiles), or of the selected pages one after the other; eight positions, a block, never straddle a page, and a lane works out where
+// one block lies (BlockMap).  The matrix kernels' products (16-bit tensors, head sizes 64 and 128) are those of the dense kernel:
+// S^T[l, q] = K[l,:] . Q[q,:], O^T[d, q] += V^T[d, l] P^T[l, q], a lane holds one row's logits; the weights are rounded to the tensors' type for the
+// second (half a step of theirs, with signs that average out), their sum is not.
 // ------------------------------------------------------------------------------------------------
 struct Piece {
     Request rq;
