@@ -203,7 +203,7 @@ def _write_call(k, v, k_pages, v_pages, page_size, plan, means):
         raise ValueError("k must be [tokens, kv_heads, head_dim] of the pools' heads")
     if v[1] != k[1]:
         raise ValueError("k and v must have the same shape")
-    same = _rows("v", v, k_pages[0]) == ks
+    same = _rows("v", v, k_pages[0]) == ks or 0 in k[1]         # nothing to write has every layout, and contiguous() leaves it as it is
     R, W, ts = _planned(plan, k[1][0])
     if means is not None and (means[0] != torch.float32 or tuple(means[1]) != (N, H, D) or tuple(means[2]) != (H * D, D, 1)):
         raise ValueError("means must be a contiguous float32 [pages, kv_heads, head_dim] tensor beside the pools")

@@ -244,3 +244,26 @@ def test_empty_steps():
     out, lse = PA.paged_attention(q, pool, pool, plan, return_lse=True)
     assert out.shape == (0, 4, 64) and lse.shape == (4, 0)
     assert bool((PA.select_pages(q, torch.zeros((4, 2, 64), device=dev), plan, 2) == -1).all()) and plan.q_start.tolist() == [0, 0, 0]
+
+
+def empty_rows(dev="cpu"):
+    """k and v of no tokens whose strides differ, both contiguous as any tensor without elements is."""
+    k, v = torch.zeros((2, 3, 64), dtype=torch.bfloat16, device=dev).transpose(0, 1)[:0], torch.zeros((0, 2, 64), dtype=torch.bfloat16, device=dev)
+    assert k.stride() != v.stride() and k.is_contiguous() and v.is_contiguous()
+    return k, v
+
+
+def test_empty_rows_need_no_layout_in_common():
+    k, v = empty_rows()
+    pool, plan = PA._layout(torch.zeros((4, 16, 2, 64), dtype=torch.bfloat16)), PA._plan_layout(cpu_plan(0))
+    assert PA._write_call(PA._layout(k), PA._layout(v), pool, pool, 16, plan, None)[1] is not None
+    k, v = k.new_zeros((3, 2, 64))[:2], v.new_zeros((2, 2, 128))[..., :64]
+    assert PA._write_call(PA._layout(k), PA._layout(v), pool, pool, 16, PA._plan_layout(cpu_plan(2)), None)[1] is None
+
+
+@pytest.mark.gpu
+def test_empty_steps_in_layouts_of_their_own():
+    plan = PA.PagePlan(*(t.to("cuda:0") if isinstance(t, torch.Tensor) else t for t in cpu_plan(0)))
+    pools = torch.ones((2, 4, 16, 2, 64), dtype=torch.bfloat16, device="cuda:0")
+    PA.write_pages(*empty_rows("cuda:0"), *pools, plan)
+    assert bool((pools == 1).all())
