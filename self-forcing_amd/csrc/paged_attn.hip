@@ -1034,7 +1034,7 @@ static PagedPlan paged_plan(const sfm_paged_desc& d) {
     p.paired = prompts && p.rows == 128;
     const int64_t per = mfma ? p.rows : kAnyRows;
     p.pieces = d.top ? pieces(d.tokens, d.group, d.requests) * ((std::min<int64_t>(d.group, d.tokens) * G + per - 1) / per) : pieces(d.tokens * G, per, d.requests);
-    const int64_t tiles = ((d.top ? (int64_t)d.top * d.page_size : cap) + 63) / 64, n = items(per);
+    const int64_t tiles = d.top ? ((int64_t)d.top * d.page_size + 63) / 64 : most_tiles(per, G, d.tokens, d.causal, d.window, d.sink, cap), n = items(per);
     int64_t chunks = 1;
     if (!mfma) {               // a step is 256 positions; one token on 1560, 12 heads of 128 fp32: in 7 ranges 33 us, in 2 76
         chunks = std::min<int64_t>((4 * cu + n - 1) / n, (tiles + 3) / 4);

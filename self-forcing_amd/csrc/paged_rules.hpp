@@ -73,6 +73,14 @@ __host__ __device__ __forceinline__ KeyTiles key_tiles(const Request& q, bool no
     return k;
 }
 
+// How many virtual tiles a piece of `rows` rows, `heads` query heads to a token, has at most.  With a window: those of the first positions, and
+// those that [lo_min, end_max) touches, at most window + span positions, where the last positions of the piece's tokens are `span` apart.
+inline int64_t most_tiles(int64_t rows, int64_t heads, int64_t tokens, bool causal, int64_t window, int64_t sink, int64_t cap) {
+    const int64_t all = (cap + 63) / 64, last = (rows + heads - 2) / heads, span = !causal ? 0 : last < tokens - 1 ? last : tokens - 1;
+    const int64_t seen = (sink + 63) / 64 + (window + span + 126) / 64;
+    return window && seen < all ? seen : all;
+}
+
 // Pieces of a causal prompt whose workgroups are on the chip all at once, two to a compute unit.  A head's last pieces have the most keys.  In
 // its list they alternate with its first, so that every XCD's share of the list is as much work; an XCD takes the even places of its
 // share (the long pieces) first, one per compute unit, and then the odd ones, which join them.

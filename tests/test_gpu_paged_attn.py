@@ -739,3 +739,21 @@ def test_long_contexts_selected():
     sel = PA.select_pages(q, means, plan, top, group=group, causal=True)
     got, lse = PA.paged_attention(q, kp, vp, plan, causal=True, selected=sel, group=group, return_lse=True)
     check_rows(got, lse, plan, q, kp, vp, past, n, [0, 127, 128, 700, 1023], True, selected=sel, group=group)
+
+
+@pytest.mark.parametrize("past,n,H,Hk,D,window,sink,rows", [
+    ([9000, 100, 0], [1, 1, 1], 4, 2, 128, 3000, 70, 32), ([9000, 2037], [30, 1], 2, 2, 64, 2000, 0, 32), ([3000, 700], [300, 2], 2, 2, 128, 1500, 1, 128),
+    ([9000], [40], 4, 1, 64, 4000, 200, 128), ([9000, 100], [1, 3], 4, 2, 96, 2000, 9, 0)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_ranges_of_a_window(past, n, H, Hk, D, window, sink, rows, causal):
+    """Ranges hold the most tiles that a piece can have, in a table of any width."""
+    plan, table, q_start, q, kp, vp = inputs(past, n, 8, H, Hk, D, torch.bfloat16)
+    want = oracle.attention(q, kp, vp, table, torch.tensor(past), q_start, causal=causal, window=window, sink=sink)
+    q, kp, vp = q.to(DEV), kp.to(DEV), vp.to(DEV)
+    for width in (plan.table.shape[1], 5000):
+        wide = torch.full((len(past), width), -1, dtype=torch.int32, device=DEV)
+        wide[:, :plan.table.shape[1]] = plan.table
+        p = plan._replace(table=wide)
+        assert kernel(p, q, kp, causal, window)[0] == rows and kernel(p, q, kp, causal, window)[1] > 1
+        got, lse = PA.paged_attention(q, kp, vp, p, causal=causal, window=window, sink=sink, return_lse=True)
+        close(got.cpu(), lse.cpu(), want, torch.bfloat16)

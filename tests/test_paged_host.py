@@ -267,3 +267,25 @@ def test_empty_steps_in_layouts_of_their_own():
     pools = torch.ones((2, 4, 16, 2, 64), dtype=torch.bfloat16, device="cuda:0")
     PA.write_pages(*empty_rows("cuda:0"), *pools, plan)
     assert bool((pools == 1).all())
+
+
+# ---------------------------------------------------------------- which kernel a call takes, and in how many ranges (of 256 compute units, the GPU's and the default)
+def kernel(**change):
+    out = [C.c_int32() for _ in range(3)]
+    assert L.load().sfm_paged_attention_plan(C.byref(desc(**change)), *map(C.byref, out)) == 0
+    return tuple(x.value for x in out)
+
+
+def test_ranges_follow_the_window():
+    """A window's keys are a few tiles of a table for 30000 positions: ranges are of those, and what lies in the caches is read from them."""
+    tokens = dict(tokens=16, requests=16, H=32, kv_heads=8, width=1875, table_stride=1875, pages=40000)
+    rows, ranges, once = kernel(**tokens)
+    assert rows == 32 and ranges > 8 and once
+    for window, sink, most in ((500, 0, 9), (1, 0, 2), (500, 100, 11), (64, 0, 3)):
+        rows, ranges, once = kernel(**tokens, window=window, sink=sink)
+        assert rows == 32 and ranges <= -(-most // 4) and not once, (window, sink)
+    prompt = dict(tokens=512, requests=1, H=8, kv_heads=8, width=1900, table_stride=1900, pages=2000)
+    assert kernel(**prompt)[1] > 4 and kernel(**prompt, window=1000)[1] <= 4
+    other = dict(tokens, D=96)
+    assert kernel(**other)[1] > 4 and kernel(**other, window=500)[1] <= 3
+    assert kernel(**tokens, window=40000) == kernel(**tokens) == kernel(**tokens, window=30000, sink=9)

@@ -23,6 +23,9 @@ extern "C" void tiles(int past, int n, int none, int t0, int t1, int causal, int
     const int v[] = {k.end_min, k.end_max, k.lo_min, k.lo_max, k.sinks, k.first, k.tiles, k.fast0, k.fast1, k.beyond};
     for (int i = 0; i < 10; ++i) out[i] = v[i];
 }
+extern "C" long long most(long long rows, long long heads, long long tokens, int causal, long long window, long long sink, long long cap) {
+    return sfm::most_tiles(rows, heads, tokens, causal, window, sink, cap);
+}
 extern "C" int paired(int i, int n, int place) { return place ? sfm::paired_place(i, n) : sfm::paired_piece(i, n); }
 """
 
@@ -57,6 +60,8 @@ def rules(tmp_path_factory):
     lib.block.restype = C.c_longlong
     lib.block.argtypes = [C.c_int] * 8 + [C.c_void_p] + [C.c_int] * 3 + [C.c_void_p, C.c_int] + [C.c_longlong] * 2 + [C.c_int] + [C.c_void_p] * 3
     lib.all_pieces.argtypes = [C.c_longlong] * 2 + [C.c_int]
+    lib.most.restype = C.c_longlong
+    lib.most.argtypes = [C.c_longlong] * 3 + [C.c_int] + [C.c_longlong] * 3
     return lib
 
 
@@ -191,3 +196,23 @@ def test_blocks_lie_where_the_table_says_and_always_inside_the_pool(rules, liste
             assert met == some
         elif sel == sorted(set(sel)) and (not sel or sel[-1] < need):
             assert met == {p for p in some if p // page in sel}
+
+
+def test_no_piece_has_more_tiles_than_the_ranges_are_made_for(rules):
+    rng = random.Random(6)
+    reached = 0
+    for _ in range(4000):
+        heads, rows = rng.choice([1, 2, 3, 5, 8, 40]), rng.choice([4, 32, 128, 256])
+        past, n, causal = rng.choice([0, 1, 63, 64, 65, 500, rng.randint(0, 5000)]), rng.choice([1, 2, rng.randint(1, 700)]), rng.randint(0, 1)
+        window = rng.choice([0, 1, 2, 63, 64, 65, 66, rng.randint(1, 900), 2 ** 31 - 1])
+        sink = rng.choice([0, 1, 64, 65, rng.randint(0, 900), 2 ** 31 - 1]) if window else 0
+        cap = rng.choice([past + n, 10 ** 6, 2 ** 30, 8 * rng.randint(1, 600)])
+        most = rules.most(rows, heads, n + rng.choice([0, 0, 100]), causal, window, sink, cap)
+        assert most <= -(-cap // 64) and (window or most == -(-cap // 64))
+        row0 = rng.randint(0, n * heads - 1)                # a piece may begin at any row of a token
+        row1 = min(n * heads, row0 + rows)
+        out = (C.c_int * 10)()
+        rules.tiles(past, n, 0, row0 // heads, (row1 - 1) // heads, causal, window, sink, cap, out)
+        assert out[6] <= most
+        reached += window > 0 and out[6] == most
+    assert reached > 100                                   # and some have as many
