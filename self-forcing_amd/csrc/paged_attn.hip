@@ -1047,12 +1047,11 @@ static PagedPlan paged_plan(const sfm_paged_desc& d) {
         // no longer than their bytes do, nothing is split and joined: 16 tokens, 8 heads, 64 pages of 32 rows 51 us instead of 55
         const double whole_us = 5.5 + 2.9 * ((tiles + 3) / 4), bytes_us = n * tiles * 64.0 * d.D * 4 / 4.8e6;
         if (d.top && n >= cu / 2 && whole_us <= 1.1 * bytes_us) chunks = 1;
-    } else if (tiles >= 16) {
-        const bool broad = p.rows == 256;
+    } else if (p.rows == 128 && tiles >= 16) {                        // 256 rows are taken only where their pieces fill the chip
         const double scale = d.D == 64 ? 0.6 : 1.0, partial_ns = (double)d.H * d.tokens * (d.D + 2) * 8 / 3500;
         double t1 = 0, best = 0;
-        for (int64_t s = 1; s <= 64 && s <= tiles / 4 && (s == 1 || n * s <= cu * (broad ? 1 : 2)); ++s) {
-            const double tile_ns = broad ? (n * s <= cu / 2 ? 1460 : 1830) : (n * s <= cu ? 1100 : 1900);
+        for (int64_t s = 1; s <= 64 && s <= tiles / 4 && (s == 1 || n * s <= 2 * cu); ++s) {
+            const double tile_ns = n * s <= cu ? 1100 : 1900;
             double t = 5000 + (double)((tiles + s - 1) / s) * tile_ns * scale;
             if (s == 1) t1 = best = t;
             else t += 6000 + s * partial_ns;

@@ -1,5 +1,6 @@
 """What the paged cache's entry points and functions refuse, without a GPU."""
 import ctypes as C
+import random
 
 import pytest
 import torch
@@ -289,3 +290,15 @@ def test_ranges_follow_the_window():
     other = dict(tokens, D=96)
     assert kernel(**other)[1] > 4 and kernel(**other, window=500)[1] <= 3
     assert kernel(**tokens, window=40000) == kernel(**tokens) == kernel(**tokens, window=30000, sink=9)
+
+
+def test_pieces_of_256_rows_fill_the_chip_in_one_range():
+    rng, wide = random.Random(7), 0
+    for _ in range(20000):
+        kv, tokens, width = rng.choice([1, 2, 3, 4, 8, 12, 16, 40]), rng.choice([rng.randint(1, 300), rng.randint(1, 40000)]), rng.choice([3, 40, 500, 3000, 60000])
+        window = rng.choice([0, 0, rng.randint(1, 5000)])
+        rows, ranges, _ = kernel(tokens=tokens, requests=rng.choice([1, 1, 2, 5, 40]), kv_heads=kv, H=kv * rng.choice([1, 2, 4, 8]), width=width, table_stride=width,
+                                 pages=width, D=rng.choice([64, 128]), causal=rng.randint(0, 1), window=window)
+        assert rows in (32, 128, 256) and 1 <= ranges <= 64 and (rows < 256 or ranges == 1)
+        wide += rows == 256
+    assert wide > 100
