@@ -538,6 +538,7 @@ int sfm_paged_write(const sfm_paged_desc* desc, const void* k, const void* v, co
  * natural logarithm of the sum, -inf for no keys.  A request whose keys have positions without a page (a number outside the pool,
  * positions past the table) gets NaN in the rows that would read one, and may in others of the same 256 rows of a head.  Keys that a
  * row does not see have no part in it whatever their K and V hold.  Sums and statistics in fp32, a fixed order.
+ * out and lse must share no byte with each other, the workspace or the inputs' rows (refused; they may be columns of the same buffer).
  * MFMA kernels for 16-bit tensors with D 64 or 128; a workspace lets calls with few rows be split over the keys. */
 int sfm_paged_workspace_bytes(const sfm_paged_desc* desc, size_t* bytes);
 

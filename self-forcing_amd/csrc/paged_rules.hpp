@@ -81,6 +81,62 @@ inline int64_t most_tiles(int64_t rows, int64_t heads, int64_t tokens, bool caus
     return window && seen < all ? seen : all;
 }
 
+// Rows of `bytes`, n[0] n[1] n[2] of them at strides of bytes.
+struct Rows3 {
+    const void* at;
+    int64_t bytes;
+    int64_t n[3] = {1, 1, 1}, stride[3] = {0, 0, 0};
+    int64_t extent() const {
+        int64_t e = bytes;
+        for (int i = 0; i < 3; ++i) e += (n[i] - 1) * stride[i];
+        return e;
+    }
+    int64_t largest_stride() const {
+        int64_t s = 0;
+        for (int i = 0; i < 3; ++i) s = n[i] > 1 && stride[i] > s ? stride[i] : s;
+        return s;
+    }
+    // one repetition of the rows at stride s, and how many there are
+    Rows3 without(int64_t s, int64_t* count) const {
+        Rows3 r = *this;
+        *count = 1;
+        for (int i = 0; i < 3; ++i)
+            if (n[i] > 1 && stride[i] == s) {
+                *count = n[i];
+                r.n[i] = 1;
+                break;
+            }
+        return r;
+    }
+};
+// Whether rows of b, which lies x bytes behind a, share a byte with rows of a: columns, heads or pages of one buffer may lie between each
+// other.  The largest stride S of both is taken apart: repetition j of b's lies x + (j - i) S behind repetition i of a's, and few of those
+// distances are short enough to meet.  Where there are many the strides do not nest, and that is taken for a yes.
+inline bool meet(const Rows3& a, const Rows3& b, int64_t x) {
+    if (x >= a.extent() || -x >= b.extent()) return false;
+    const int64_t sa = a.largest_stride(), sb = b.largest_stride(), S = sa > sb ? sa : sb;
+    if (S == 0) return true;
+    int64_t na, nb;
+    const Rows3 ai = a.without(S, &na), bi = b.without(S, &nb);
+    auto floor_div = [](int64_t v, int64_t d) { return v >= 0 ? v / d : -((-v + d - 1) / d); };
+    const int64_t lo = -floor_div(bi.extent() - 1 + x, S), hi = floor_div(ai.extent() - 1 - x, S);
+    const int64_t k0 = lo > 1 - na ? lo : 1 - na, k1 = hi < nb - 1 ? hi : nb - 1;
+    if (k1 - k0 >= 4) return true;
+    for (int64_t k = k0; k <= k1; ++k)
+        if (meet(ai, bi, x + k * S)) return true;
+    return false;
+}
+// Whether two rows of r share a byte
+inline bool folds(const Rows3& r) {
+    const int64_t S = r.largest_stride();
+    if (S == 0) return false;
+    int64_t n;
+    const Rows3 one = r.without(S, &n);
+    for (int64_t k = 1; k < n && k * S < one.extent(); ++k)
+        if (k == 4 || meet(one, one, k * S)) return true;
+    return folds(one);
+}
+
 // Pieces of a causal prompt whose workgroups are on the chip all at once, two to a compute unit.  A head's last pieces have the most keys.  In
 // its list they alternate with its first, so that every XCD's share of the list is as much work; an XCD takes the even places of its
 // share (the long pieces) first, one per compute unit, and then the odd ones, which join them.

@@ -6,6 +6,8 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <algorithm>
+#include "paged_rules.hpp"
 #include "rows8.hpp"
 
 namespace sfm {
@@ -1864,6 +1866,20 @@ static int check_paged_stride(const char* name, int64_t s, int64_t least, int es
     return SFM_OK;
 }
 
+static int check_apart(const char* a_name, const Rows3& a, const char* b_name, const Rows3& b) {
+    if (!a.at || !b.at || a.bytes < 1 || b.bytes < 1 || !meet(a, b, (const char*)b.at - (const char*)a.at)) return SFM_OK;
+    set_error("%s overlaps %s", a_name, b_name);
+    return SFM_ERR_RANGE;
+}
+static Rows3 token_rows(const sfm_paged_desc* d, const void* p, int heads, const int64_t* stride) {
+    const int64_t e = elem_size(d->dtype);
+    return {p, d->D * e, {d->tokens, heads, 1}, {stride[0] * e, stride[1] * e, 0}};
+}
+static Rows3 pool_rows(const sfm_paged_desc* d, const void* p) {
+    const int64_t e = elem_size(d->dtype);
+    return {p, d->D * e, {d->pages, d->page_size, d->kv_heads}, {d->pool_stride[0] * e, d->pool_stride[1] * e, d->pool_stride[2] * e}};
+}
+
 // what all of the entry points read of a descriptor; `pool`: with the pools
 static int check_paged(const sfm_paged_desc* d, bool pool) {
     if (!d) {
@@ -1984,6 +2000,19 @@ int sfm_paged_attention(const sfm_paged_desc* d, const void* q, const void* k_pa
         set_error("tensors and workspace must be 16-byte aligned, the arrays to their elements");
         return SFM_ERR_ALIGN;
     }
+    // other workgroups read the inputs while the first rows are stored
+    const Rows3 to[2] = {token_rows(d, out, d->H, d->o_stride), {lse, (int64_t)4 * d->H * d->tokens}};
+    const int64_t lists = (d->tokens / std::max(d->group, 1) + d->requests + 1) * d->kv_heads * d->top;
+    const Rows3 from[8] = {token_rows(d, q, d->H, d->q_stride), pool_rows(d, k_pages), pool_rows(d, v_pages), {table, (int64_t)4 * d->width, {d->requests, 1, 1}, {4 * d->table_stride, 0, 0}},
+                           {past, (int64_t)4 * d->requests}, {q_start, (int64_t)4 * (d->requests + 1)}, {d->top ? selected : nullptr, 4 * lists}, {workspace, (int64_t)workspace_bytes}};
+    const char* const names[8] = {"q", "k_pages", "v_pages", "table", "past", "q_start", "selected", "the workspace"};
+    if (folds(to[0])) {
+        set_error("rows of out overlap each other");
+        return SFM_ERR_RANGE;
+    }
+    int apart = check_apart("out", to[0], "lse", to[1]);
+    for (int i = 0; i < 16 && !apart; ++i) apart = check_apart(i & 1 ? "lse" : "out", to[i & 1], names[i / 2], from[i / 2]);
+    if (apart) return apart;
     return launch_paged_attention(*d, q, k_pages, v_pages, table, past, q_start, selected, out, lse, workspace, workspace_bytes,
                                   (hipStream_t)stream);
 }

@@ -288,7 +288,7 @@ def paged_attention(q, k_pages, v_pages, plan, sm_scale=None, causal=False, wind
     for each `group` tokens (int32 [selected_rows(tokens, requests, group), kv_heads, top], ascending, each page once; no window then).
 
     -> [tokens, heads, head_dim] in q's dtype, zeros for a token that sees nothing and for rows that nobody has (with out, rows that nobody
-    has stay as they were; out must not overlap the other tensors); with return_lse also the natural logarithm of the sums, fp32
+    has stay as they were; out in q, the pools or the plan is refused); with return_lse also the natural logarithm of the sums, fp32
     [heads, tokens], -inf for nothing.  Rows that would read a position without a page (-1 or another number outside the pool,
     positions past the table) are NaN, and others of their request may be.  What lies in positions that a row does not see has no part in it,
     NaN or infinite.  table[:, :n] of the columns in use sizes the work."""

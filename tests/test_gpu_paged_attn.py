@@ -757,3 +757,27 @@ def test_ranges_of_a_window(past, n, H, Hk, D, window, sink, rows, causal):
         assert kernel(p, q, kp, causal, window)[0] == rows and kernel(p, q, kp, causal, window)[1] > 1
         got, lse = PA.paged_attention(q, kp, vp, p, causal=causal, window=window, sink=sink, return_lse=True)
         close(got.cpu(), lse.cpu(), want, torch.bfloat16)
+
+
+@pytest.mark.parametrize("n", [[150, 3], [1, 1]])
+def test_columns_of_one_buffer(n):
+    """q, out, k and v as columns of the same rows, K's and V's pools as halves of one: nothing is shared, nothing refused."""
+    past, page, H, Hk, D = [70, 30], 16, 4, 2, 64
+    plan, table, q_start, q, kp, vp = inputs(past, n, page, H, Hk, D, torch.bfloat16)
+    T = sum(n)
+    rows = torch.zeros((T, 2 * H + 2 * Hk, D), dtype=torch.bfloat16, device=DEV)
+    rows[:, :H] = q.to(DEV)
+    pool = torch.stack([kp, vp], 1).to(DEV)
+    k, v = (randn((T, Hk, D), s, torch.bfloat16) for s in (5, 6))
+    rows[:, 2 * H:2 * H + Hk], rows[:, 2 * H + Hk:] = k.to(DEV), v.to(DEV)
+    PA.write_pages(rows[:, 2 * H:2 * H + Hk], rows[:, 2 * H + Hk:], pool[:, 0], pool[:, 1], plan)
+    out = rows[:, H:2 * H]
+    assert PA.paged_attention(rows[:, :H], pool[:, 0], pool[:, 1], plan, causal=True, out=out) is out
+    kp, vp, _ = oracle.write(k, v, kp, vp, plan.slots.cpu(), table, torch.tensor(past), q_start)
+    assert torch.equal(pool[:, 0].cpu(), kp) and torch.equal(pool[:, 1].cpu(), vp)
+    close(out.cpu(), None, oracle.attention(q, kp, vp, table, torch.tensor(past), q_start, causal=True), torch.bfloat16)
+    assert torch.equal(rows[:, :H].cpu(), q)
+    for taken in (rows[:, :H], rows[:, 1:H + 1], rows[:, H - 1:2 * H - 1]):
+        with pytest.raises(sfa.lib.SfmError, match="out overlaps q"):
+            PA.paged_attention(rows[:, :H], pool[:, 0], pool[:, 1], plan, causal=True, out=taken)
+    assert torch.equal(pool[:, 0].cpu(), kp) and torch.equal(rows[:, :H].cpu(), q)

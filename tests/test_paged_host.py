@@ -270,6 +270,24 @@ def test_empty_steps_in_layouts_of_their_own():
     assert bool((pools == 1).all())
 
 
+M = 1 << 20
+APART = dict(q=16 * M, k=17 * M, v=18 * M, table=19 * M, past=20 * M, q_start=21 * M, out=22 * M, lse=23 * M, ws=24 * M)      # every call with them is refused
+
+
+@pytest.mark.parametrize("name,at", [(n, p) for n, p in APART.items() if n not in ("out", "lse", "ws")] + [("selected", 25 * M)])
+def test_out_and_lse_in_inputs_are_refused(name, at):
+    d = desc(top=4, group=2)
+    apart = dict(APART, selected=25 * M)
+    for to in ("out", "lse"):
+        assert attention(d, **dict(apart, **{to: at})) == RANGE
+        assert L.load().sfm_last_error().decode() == f"{to} overlaps {dict(k='k_pages', v='v_pages').get(name, name)}"
+    assert attention(d, **dict(apart, lse=APART["out"])) == RANGE and attention(d, **dict(apart, lse=APART["out"] + 9 * 8 * 128 * 2)) == RANGE
+    # the last row of q, a column of q's rows, rows that overlap each other
+    assert attention(d, **dict(apart, out=APART["q"] + 10 * 8 * 128 * 2 - 16)) == RANGE
+    assert attention(desc(q_stride=(4096, 128), o_stride=(4096, 128)), **dict(APART, out=APART["q"] + 2048 - 16)) == RANGE
+    assert attention(desc(o_stride=(128, 128)), **APART) == RANGE and attention(desc(o_stride=(960, 128)), **APART) == RANGE
+
+
 # ---------------------------------------------------------------- which kernel a call takes, and in how many ranges (of 256 compute units, the GPU's and the default)
 def kernel(**change):
     out = [C.c_int32() for _ in range(3)]

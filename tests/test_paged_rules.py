@@ -26,6 +26,13 @@ extern "C" void tiles(int past, int n, int none, int t0, int t1, int causal, int
 extern "C" long long most(long long rows, long long heads, long long tokens, int causal, long long window, long long sink, long long cap) {
     return sfm::most_tiles(rows, heads, tokens, causal, window, sink, cap);
 }
+static sfm::Rows3 rows3(long long bytes, const long long* n, const long long* stride) {
+    return {nullptr, bytes, {n[0], n[1], n[2]}, {stride[0], stride[1], stride[2]}};
+}
+extern "C" int meets(long long ab, const long long* an, const long long* as, long long bb, const long long* bn, const long long* bs, long long x) {
+    return sfm::meet(rows3(ab, an, as), rows3(bb, bn, bs), x);
+}
+extern "C" int folded(long long bytes, const long long* n, const long long* stride) { return sfm::folds(rows3(bytes, n, stride)); }
 extern "C" int paired(int i, int n, int place) { return place ? sfm::paired_place(i, n) : sfm::paired_piece(i, n); }
 """
 
@@ -61,6 +68,8 @@ def rules(tmp_path_factory):
     lib.block.argtypes = [C.c_int] * 8 + [C.c_void_p] + [C.c_int] * 3 + [C.c_void_p, C.c_int] + [C.c_longlong] * 2 + [C.c_int] + [C.c_void_p] * 3
     lib.all_pieces.argtypes = [C.c_longlong] * 2 + [C.c_int]
     lib.most.restype = C.c_longlong
+    lib.meets.argtypes = [C.c_longlong, C.c_void_p, C.c_void_p] * 2 + [C.c_longlong]
+    lib.folded.argtypes = [C.c_longlong, C.c_void_p, C.c_void_p]
     lib.most.argtypes = [C.c_longlong] * 3 + [C.c_int] + [C.c_longlong] * 3
     return lib
 
@@ -216,3 +225,46 @@ def test_no_piece_has_more_tiles_than_the_ranges_are_made_for(rules):
         assert out[6] <= most
         reached += window > 0 and out[6] == most
     assert reached > 100                                   # and some have as many
+
+
+def test_rows_that_share_bytes(rules):
+    """Never missed; and rows whose strides nest, as those of tensors and of their slices do, are told apart exactly."""
+    rng = random.Random(8)
+
+    def where(n, stride, w):
+        return [a * stride[0] + b * stride[1] + c * stride[2] for a in range(n[0]) for b in range(n[1]) for c in range(n[2])]
+
+    def nested(fused):
+        """A slice of a buffer: counts, strides and offset of its rows, in any order of the dimensions."""
+        n, stride, at, size = [], [], 0, fused["w"]
+        for most in fused["n"]:
+            m = rng.randint(1, most)
+            at += rng.randint(0, most - m) * size
+            n.append(m)
+            stride.append(size)
+            size *= most
+        order = rng.sample(range(3), 3)
+        return [n[i] for i in order], [stride[i] for i in order], at
+    ll3 = C.c_longlong * 3
+    seen = [0, 0]
+    for i in range(4000):
+        if i % 2:
+            fused = dict(w=rng.randint(1, 5), n=[rng.randint(1, 4) for _ in range(3)])
+            (an, as_, a), (bn, bs, b), w = nested(fused), nested(fused), fused["w"]
+            bw, x = w, b - a
+        else:
+            an, bn = ([rng.randint(1, 4) for _ in range(3)] for _ in range(2))
+            as_, bs = ([rng.randint(0, 40) for _ in range(3)] for _ in range(2))
+            w, bw, x = rng.randint(1, 5), rng.randint(1, 5), rng.randint(-200, 200)
+        mine = {p + k for p in where(an, as_, w) for k in range(w)}
+        share = bool(mine & {x + p + k for p in where(bn, bs, bw) for k in range(bw)})
+        got = bool(rules.meets(w, ll3(*an), ll3(*as_), bw, ll3(*bn), ll3(*bs), x))
+        assert got or not share
+        if i % 2:
+            assert got == share
+            seen[share] += 1
+        if all(s >= w for s in as_):
+            twice = len(mine) < w * an[0] * an[1] * an[2]
+            assert rules.folded(w, ll3(*an), ll3(*as_)) or not twice
+            assert not i % 2 or not rules.folded(w, ll3(*an), ll3(*as_))
+    assert min(seen) > 300
