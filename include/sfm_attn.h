@@ -529,7 +529,8 @@ typedef struct sfm_paged_desc {
 
 /* k, v rows [tokens][kv_heads][D] (k_stride: token, head; of both) into the pools at `slots`; of a slot named twice the row is one of the two in
  * each 16 bytes, others outside the pool are passed over.  means (NULL or fp32 [pages][kv_heads][D]): of every page that got a row, the mean of its
- * keys up to the request's length; needs past, q_start and table.  Of desc the types, sizes and pool_stride. */
+ * keys up to the request's length; needs past, q_start and table.  k and v must share no byte with the pools' rows (refused).  Of desc the types,
+ * sizes and pool_stride. */
 int sfm_paged_write(const sfm_paged_desc* desc, const void* k, const void* v, const int64_t k_stride[2], void* k_pages, void* v_pages,
                     const int64_t* slots, const int32_t* table, const int32_t* past, const int32_t* q_start, float* means,
                     void* stream);

@@ -1944,6 +1944,11 @@ int sfm_paged_write(const sfm_paged_desc* d, const void* k, const void* v, const
         set_error("rows and pools must be 16-byte aligned, the arrays to their elements");
         return SFM_ERR_ALIGN;
     }
+    // a row could be written before it is read
+    const Rows3 kr = token_rows(d, k, d->kv_heads, k_stride), vr = token_rows(d, v, d->kv_heads, k_stride), kpr = pool_rows(d, k_pages), vpr = pool_rows(d, v_pages);
+    if ((rc = check_apart("k", kr, "k_pages", kpr)) || (rc = check_apart("k", kr, "v_pages", vpr)) || (rc = check_apart("v", vr, "k_pages", kpr)) ||
+        (rc = check_apart("v", vr, "v_pages", vpr)))
+        return rc;
     return launch_paged_write(*d, k, v, k_stride, k_pages, v_pages, slots, table, past, q_start, means, (hipStream_t)stream);
 }
 

@@ -213,7 +213,7 @@ def _write_call(k, v, k_pages, v_pages, page_size, plan, means):
 def write_pages(k, v, k_pages, v_pages, plan, means=None):
     """k_pages / v_pages[slot] = k / v rows ([tokens, kv_heads, head_dim]), in place at the plan's slots; rows without one are passed over.  Any
     strides of whole 16 bytes with a contiguous head_dim, pools alike.  With means (fp32 [pages, kv_heads, head_dim], in place): the mean key of every page that got a
-    row, over the page's rows up to the request's length.  k and v must not lie in the pools; where a slot is named twice one of
+    row, over the page's rows up to the request's length.  k and v must not lie in the pools (refused); where a slot is named twice one of
     the rows stays in each 16 bytes."""
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
         raise NotImplementedError("write_pages is not differentiable")

@@ -780,4 +780,7 @@ def test_columns_of_one_buffer(n):
     for taken in (rows[:, :H], rows[:, 1:H + 1], rows[:, H - 1:2 * H - 1]):
         with pytest.raises(sfa.lib.SfmError, match="out overlaps q"):
             PA.paged_attention(rows[:, :H], pool[:, 0], pool[:, 1], plan, causal=True, out=taken)
+    inside = pool[0, 0].expand(T, page, Hk, D)[:, 0]
+    with pytest.raises(sfa.lib.SfmError, match="k overlaps k_pages"):
+        PA.write_pages(inside, inside, pool[:, 0], pool[:, 1], plan)
     assert torch.equal(pool[:, 0].cpu(), kp) and torch.equal(rows[:, :H].cpu(), q)

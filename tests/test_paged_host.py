@@ -288,6 +288,15 @@ def test_out_and_lse_in_inputs_are_refused(name, at):
     assert attention(desc(o_stride=(128, 128)), **APART) == RANGE and attention(desc(o_stride=(960, 128)), **APART) == RANGE
 
 
+def test_rows_to_write_in_the_pools_are_refused():
+    far = dict(k=16 * M, v=17 * M, kp=18 * M, vp=19 * M, slots=20 * M, table=21 * M, past=22 * M, q_start=23 * M, means=24 * M)
+    for name in ("k", "v"):
+        for pool in ("kp", "vp"):
+            assert write(desc(), **dict(far, **{name: far[pool] + 256})) == RANGE
+            assert write(desc(), **dict(far, **{name: far[pool] + 40 * 16 * 2 * 128 * 2 - 16})) == RANGE
+            assert write(desc(), **dict(far, **{name: far[pool] - 10 * 256 * 2 + 16})) == RANGE
+
+
 # ---------------------------------------------------------------- which kernel a call takes, and in how many ranges (of 256 compute units, the GPU's and the default)
 def kernel(**change):
     out = [C.c_int32() for _ in range(3)]
