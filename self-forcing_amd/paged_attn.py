@@ -16,13 +16,15 @@ scores highest, and paged_attention reads only those (`selected=`).
 
 Lengths, tables and lists of free pages stay on the GPU: nothing here waits for it, and a step can be recorded into a HIP graph.  What
 they hold cannot be refused, then: no number in them makes a kernel leave its tensors, and each function says what comes of
-numbers that make no sense.  Nothing here is differentiable."""
+numbers that make no sense.  Nothing here is differentiable,
+in either mode."""
 import ctypes as C
 import functools
 import math
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from . import lib as _l
@@ -189,6 +191,11 @@ def _gpu(plan):
     return gpu if gpu == plan.past.get_device() == plan.q_start.get_device() == plan.slots.get_device() else -1
 
 
+def _tangents(*tensors):
+    """Whether a tensor carries a tangent of forward-mode differentiation.  (Outside of its levels, as here all but always, none does.)"""
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 _I2 = C.c_int64 * 2
 _MOST = 2 ** 31 - 1            # a window, sink or group past it is one of everything: there are fewer positions and tokens
 
@@ -215,7 +222,8 @@ def write_pages(k, v, k_pages, v_pages, plan, means=None):
     strides of whole 16 bytes with a contiguous head_dim, pools alike.  With means (fp32 [pages, kv_heads, head_dim], in place): the mean key of every page that got a
     row, over the page's rows up to the request's length.  k and v must not lie in the pools (refused); where a slot is named twice one of
     the rows stays in each 16 bytes."""
-    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
+    if (torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad or (
+            means is not None and means.requires_grad))) or _tangents(k, v, k_pages, v_pages, means):
         raise NotImplementedError("write_pages is not differentiable")
     dev, planned, gpu = k_pages.device, _plan_layout(plan), k_pages.get_device()
     if gpu < 0 or not (gpu == k.get_device() == v.get_device() == v_pages.get_device() == _gpu(plan)) or (means is not None and means.get_device() != gpu):
@@ -292,7 +300,8 @@ def paged_attention(q, k_pages, v_pages, plan, sm_scale=None, causal=False, wind
     [heads, tokens], -inf for nothing.  Rows that would read a position without a page (-1 or another number outside the pool,
     positions past the table) are NaN, and others of their request may be.  What lies in positions that a row does not see has no part in it,
     NaN or infinite.  table[:, :n] of the columns in use sizes the work."""
-    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad or (out is not None and out.requires_grad)):
+    if (torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad or (
+            out is not None and out.requires_grad))) or _tangents(q, k_pages, v_pages, out):
         raise NotImplementedError("paged_attention is not differentiable")
     dev, planned, gpu = k_pages.device, _plan_layout(plan), k_pages.get_device()
     if gpu < 0 or not (gpu == q.get_device() == v_pages.get_device() == _gpu(plan)) or (selected is not None and selected.get_device() != gpu) or (
@@ -357,7 +366,7 @@ def select_pages(q, means, plan, top, group=1, causal=False, first=1, last=1):
     to `top` in all; of level ones the lower.  means: fp32 [pages, kv_heads, head_dim], kept by write_pages.  Scores are sums in 64 bits,
     so that which page is ahead does not hang on the order of an addition; NaN counts as -inf, as does a page outside the pool.  Group i of request r
     is row q_start[r] // group + r + i; rows that nobody has are -1."""
-    if torch.is_grad_enabled() and (q.requires_grad or means.requires_grad):
+    if (torch.is_grad_enabled() and (q.requires_grad or means.requires_grad)) or _tangents(q, means):
         raise NotImplementedError("select_pages is not differentiable")
     dev, planned, gpu = q.device, _plan_layout(plan), q.get_device()
     if gpu < 0 or not (gpu == means.get_device() == _gpu(plan)):

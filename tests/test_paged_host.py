@@ -155,6 +155,25 @@ def test_gradients_are_refused():
             call()
 
 
+def test_tangents_are_refused():
+    pool, q, means, plan = torch.zeros((4, 16, 2, 64)), torch.zeros((4, 2, 64)), torch.zeros((4, 2, 64)), cpu_plan()
+    calls = {"k": lambda t: PA.write_pages(t(q), q, pool, pool, plan), "v": lambda t: PA.write_pages(q, t(q), pool, pool, plan),
+             "k_pages": lambda t: PA.write_pages(q, q, t(pool), pool, plan), "v_pages": lambda t: PA.write_pages(q, q, pool, t(pool), plan),
+             "means": lambda t: PA.write_pages(q, q, pool, pool, plan, means=t(means)), "q": lambda t: PA.paged_attention(t(q), pool, pool, plan),
+             "keys": lambda t: PA.paged_attention(q, t(pool), pool, plan), "values": lambda t: PA.paged_attention(q, pool, t(pool), plan),
+             "out": lambda t: PA.paged_attention(q, pool, pool, plan, out=t(q)), "queries": lambda t: PA.select_pages(t(q), means, plan, 2),
+             "scores": lambda t: PA.select_pages(q, t(means), plan, 2)}
+    with torch.autograd.forward_ad.dual_level():
+        for name, call in calls.items():
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises(NotImplementedError, match="differentiable"):
+                    call(lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)))
+            with pytest.raises(ValueError, match="GPU"):          # none: only the device is wrong
+                call(lambda t: t)
+    with pytest.raises(NotImplementedError, match="differentiable"):
+        calls["means"](lambda t: t.clone().requires_grad_())
+
+
 def test_tables_and_arrays():
     for bad in (torch.zeros((2, 3), dtype=torch.int64), torch.zeros(3, dtype=torch.int32), torch.zeros((0, 3), dtype=torch.int32),
                 torch.zeros((3, 2), dtype=torch.int32).T):
