@@ -261,3 +261,47 @@ def test_select_strided_queries_and_table():
     big[:, 1] = q.to(DEV)
     got = PA.select_pages(big[:, 1], means.to(DEV), plan._replace(table=wide[:, :-3]), 6, group=2, causal=True)
     assert torch.equal(got.cpu().long(), oracle.select_pages(q, means, table, torch.tensor([300, 70]), q_start, 8, 6, 2, True, 1, 1))
+
+
+def passes(rows, Hk, W, D):
+    """Scores of so many rows are formed at a time in 256 MB."""
+    return -(-rows // max(1, min(2 ** 28 // (8 * Hk * (W + D)), 65535)))
+
+
+@pytest.mark.parametrize("H,group,width,least", [(2, 1, 60000, 4), (4, 20, 2 ** 20, 4), (2, 7, 400000, 4)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_select_in_several_passes(H, group, width, least, causal):
+    """More rows than a pass holds, by a table wide with entries of nobody: tiles of four rows and requests go on in the next pass, queries
+    summed by whom they are for (group * heads to a key head up to 16) and beforehand."""
+    past, n, page, Hk, D, pad = [90, 300, 4], [3, 700, 500], 8, 2, 16, 41
+    plan, pages, table, q_start, q, means = select_inputs(past, n, page, H, Hk, D, pad, torch.bfloat16)
+    rows = PA.selected_rows(sum(n) + pad, 3, group)
+    assert passes(rows, Hk, width, D) >= least and passes(rows, Hk, table.shape[1], D) == 1
+    wide = torch.full((3, width), -1, dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = plan.table
+    got = PA.select_pages(q.to(DEV), means.to(DEV), plan._replace(table=wide), 9, group=group, causal=causal)
+    assert torch.equal(got, PA.select_pages(q.to(DEV), means.to(DEV), plan, 9, group=group, causal=causal))
+    assert torch.equal(got.cpu().long(), oracle.select_pages(q, means, table, torch.tensor(past), q_start, page, 9, group, causal, 1, 1))
+
+
+def test_select_for_more_rows_than_a_pass_takes():
+    """A pass ends at 65535 rows too: 50000 requests of a token, against themselves in parts of one pass."""
+    R, page, D = 50000, 8, 8
+    g = torch.Generator().manual_seed(5)
+    past, order = torch.randint(0, 150, (R,), generator=g), torch.randint(0, 997, (R, 19), generator=g).int()
+    plan = PA.plan_pages(order.to(DEV), ints(past.tolist()), ints([1] * R), ints(list(range(997)) * 30), R, page)
+    q, means = randn((R, 2, D), 1, torch.bfloat16).to(DEV), randn((997, 2, D), 2, torch.float32).to(DEV)
+    assert passes(PA.selected_rows(R, R, 1), 2, 19, D) == 2
+    got = PA.select_pages(q, means, plan, 4, causal=True)
+    assert got.shape[0] == 2 * R + 1
+    for at in range(0, R, 12500):
+        part = slice(at, at + 12500)
+        own = PA.PagePlan(plan.table[part], plan.past[part], plan.lengths[part], torch.arange(12501, dtype=torch.int32, device=DEV), plan.slots[part],
+                          plan.next_free, page)
+        want = PA.select_pages(q[part], means, own, 4, causal=True)
+        assert torch.equal(got[2 * at:2 * (at + 12500)], want[:-1])
+    few = torch.arange(0, R, 5003)                         # and a few of them against the oracle
+    for r in few.tolist():
+        want = oracle.select_pages(q[r:r + 1].cpu(), means.cpu(), plan.table[r:r + 1].cpu(), past[r:r + 1], torch.tensor([0, 1]), page, 4, 1, True, 1, 1)
+        assert torch.equal(got[2 * r].cpu().long(), want[0])
+    assert bool((got[1::2] == -1).all())                   # rows that nobody has
