@@ -1043,10 +1043,11 @@ static PagedPlan paged_plan(const sfm_paged_desc& d) {
         // More rows than twice the memory-side cache (256 MB) holds, and each read once: past it, 848 MB (up to 2 GB by the table's width)
         // 193 -> 175 us; 134 MB that lie in it 38 -> 44
         p.once = n * tiles * 64.0 * d.D * 4 > 512e6;
-        // Selected pages make rows equally long: where a range of all of them (5.5 us, and 2.9 per tile of each of the four waves) takes
-        // no longer than their bytes do, nothing is split and joined: 16 tokens, 8 heads, 64 pages of 32 rows 51 us instead of 55
-        const double whole_us = 5.5 + 2.9 * ((tiles + 3) / 4), bytes_us = n * tiles * 64.0 * d.D * 4 / 4.8e6;
-        if (d.top && n >= cu / 2 && whole_us <= 1.1 * bytes_us) chunks = 1;
+        // Selected pages make rows equally long.  Where those of half the chip's compute units or more are few and lie in the memory-side cache,
+        // one range of all of them is faster than ranges that are joined: 16 tokens, 8 key heads of 128, 2048 positions each, 29.5 us
+        // and 34.1; 32 tokens of 64 28.4 and 35.8.  Past the cache, where loads take longer, and past 3200 positions, where the
+        // longest chain sets the time, ranges win: 64 tokens, 4096 positions each, 128: 238 us and 191, 64: 157 and 115.
+        if (d.top && n >= cu / 2 && tiles <= 50 && n * tiles * 64.0 * d.D * 4 <= 256e6) chunks = 1;
     } else if (p.rows == 128 && tiles >= 16) {                        // 256 rows are taken only where their pieces fill the chip
         const double scale = d.D == 64 ? 0.6 : 1.0, partial_ns = (double)d.H * d.tokens * (d.D + 2) * 8 / 3500;
         double t1 = 0, best = 0;

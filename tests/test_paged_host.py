@@ -348,3 +348,12 @@ def test_pieces_of_256_rows_fill_the_chip_in_one_range():
         assert rows in (32, 128, 256) and 1 <= ranges <= 64 and (rows < 256 or ranges == 1)
         wide += rows == 256
     assert wide > 100
+
+
+def test_ranges_of_selected_pages():
+    """One range where half the compute units or more have few pages that lie in the memory-side cache, whatever the head size."""
+    def ranges(tokens, D, top, kv_heads=8, page_size=32):
+        return kernel(tokens=tokens, requests=tokens, D=D, H=4 * kv_heads, kv_heads=kv_heads, width=1000, table_stride=1000, page_size=page_size, top=top, group=1)[1]
+    assert ranges(16, 128, 64) == 1 and ranges(32, 64, 64) == 1 and ranges(64, 128, 16) == 1 and ranges(48, 64, 32) == 1
+    assert ranges(16, 128, 160) > 1 and ranges(64, 128, 64) > 1 and ranges(64, 64, 64) > 1 and ranges(64, 64, 128) > 1 and ranges(32, 128, 128) > 1
+    assert ranges(8, 128, 64) > 1 and ranges(24, 128, 64, 4) > 1
