@@ -1040,9 +1040,12 @@ static PagedPlan paged_plan(const sfm_paged_desc& d) {
         chunks = std::min<int64_t>((4 * cu + n - 1) / n, (tiles + 3) / 4);
     } else if (p.rows == 32) {
         chunks = std::min<int64_t>((8 * cu + n - 1) / n, (tiles + 7) / 8);
-        // More rows than twice the memory-side cache (256 MB) holds, and each read once: past it, 848 MB (up to 2 GB by the table's width)
-        // 193 -> 175 us; 134 MB that lie in it 38 -> 44
-        p.once = n * tiles * 64.0 * d.D * 4 > 512e6;
+        // More rows than twice the memory-side cache (256 MB) holds, most of them read once: past it, 848 MB (up to 2 GB by the table's width)
+        // 193 -> 175 us; 134 MB that lie in it 38 -> 44.  A request's second piece reads its rows again.  Lengths are not known here, but the
+        // further apart they are the more of the rows are in such pieces: 32 requests on 15000 positions, 8 key heads, with 4 rows each 340 us
+        // in place of 376, with the same number but 97 in one request 356 (382); with 16 rows 376 (402), with 481 in one 493 (458);
+        // with 31 rows 406 (435), with 961 in one 656 (542).
+        p.once = (mean <= 16 || d.tokens <= d.requests) && n * tiles * 64.0 * d.D * 4 > 512e6;
         // Selected pages make rows equally long.  Where those of half the chip's compute units or more are few and lie in the memory-side cache,
         // one range of all of them is faster than ranges that are joined: 16 tokens, 8 key heads of 128, 2048 positions each, 29.5 us
         // and 34.1; 32 tokens of 64 28.4 and 35.8.  Past the cache, where loads take longer, and past 3200 positions, where the

@@ -357,3 +357,13 @@ def test_ranges_of_selected_pages():
     assert ranges(16, 128, 64) == 1 and ranges(32, 64, 64) == 1 and ranges(64, 128, 16) == 1 and ranges(48, 64, 32) == 1
     assert ranges(16, 128, 160) > 1 and ranges(64, 128, 64) > 1 and ranges(64, 64, 64) > 1 and ranges(64, 64, 128) > 1 and ranges(32, 128, 128) > 1
     assert ranges(8, 128, 64) > 1 and ranges(24, 128, 64, 4) > 1
+
+
+def test_what_may_be_read_again_is_read_through_the_caches():
+    """Past the caches only single tokens go, and few rows to a request, of which only few can be in a second piece of one."""
+    def once(tokens, requests, G, **more):
+        return kernel(tokens=tokens, requests=requests, kv_heads=8, H=8 * G, width=1000, table_stride=1000, pages=40000, **more)
+    assert once(32, 32, 1)[2] and once(32, 32, 32)[2] and once(128, 32, 1)[2] and once(128, 32, 4)[2] and once(20, 32, 4)[2]
+    for tokens, G in ((931, 1), (32 * 20, 1), (32 * 5, 4)):
+        assert once(tokens, 32, G)[0] == 32 and not once(tokens, 32, G)[2]
+    assert not once(32, 32, 4, window=500)[2]
