@@ -215,7 +215,8 @@ __device__ __forceinline__ void masked_tile(const char* lds, uint32_t kbuf, uint
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float v = E::to_float((uint16_t)(x[i >> 1] >> (16 * (i & 1))));
-                // an infinity counts however small its weight; a weight of NaN makes all of the row NaN
+                // an infinity with a weight that went to 0 stays one here; rescaled or joined by a factor of 0 it becomes NaN, as it does in a
+                // tile without masks: which of the two a row gets hangs on where its tiles and ranges end
                 const float part = w == w && !(fabsf(v) < INFINITY) ? v : w * v;
                 const float o = st.o[c >> 2][4 * (c & 3) + i];
                 st.o[c >> 2][4 * (c & 3) + i] = see ? o + part : o;

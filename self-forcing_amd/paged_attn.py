@@ -299,7 +299,7 @@ def paged_attention(q, k_pages, v_pages, plan, sm_scale=None, causal=False, wind
     has stay as they were; out in q, the pools or the plan is refused); with return_lse also the natural logarithm of the sums, fp32
     [heads, tokens], -inf for nothing.  Rows that would read a position without a page (-1 or another number outside the pool,
     positions past the table) are NaN, and others of their request may be.  What lies in positions that a row does not see has no part in it,
-    NaN or infinite.  table[:, :n] of the columns in use sizes the work."""
+    NaN or infinite; an infinity in a channel of V that it does see makes that channel infinite, or NaN if its weight is too small for the type.  table[:, :n] of the columns in use sizes the work."""
     if (torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad or (
             out is not None and out.requires_grad))) or _tangents(q, k_pages, v_pages, out):
         raise NotImplementedError("paged_attention is not differentiable")

@@ -784,3 +784,31 @@ def test_columns_of_one_buffer(n):
     with pytest.raises(sfa.lib.SfmError, match="k overlaps k_pages"):
         PA.write_pages(inside, inside, pool[:, 0], pool[:, 1], plan)
     assert torch.equal(pool[:, 0].cpu(), kp) and torch.equal(rows[:, :H].cpu(), q)
+
+
+@pytest.mark.parametrize("past,n,H,Hk,D,dtype,rows", [
+    ([9000], [1], 4, 1, 128, torch.bfloat16, 32), ([700], [5], 2, 2, 64, torch.float16, 32), ([700], [300], 1, 1, 128, torch.bfloat16, 128),
+    ([9000], [40], 1, 1, 64, torch.float16, 128), ([700], [9], 2, 1, 96, torch.bfloat16, 0), ([3000], [2], 1, 1, 64, torch.float32, 0)], ids=str)
+@pytest.mark.parametrize("weight", [0, 1])
+def test_infinite_values_with_any_weight(past, n, H, Hk, D, dtype, rows, weight):
+    """Infinities in whole tiles, in early ranges and in the last tile, whose weights go to 0 or do not: never a finite number in that channel of
+    a row that sees them, infinite where the weight is a plain number, and nothing in the others."""
+    page, total = 16, past[0] + n[0]
+    plan, table, q_start, q, kp, vp = inputs(past, n, page, H, Hk, D, dtype)
+    q[..., 0] = 1.0
+    at = {3: 1, 70: 2, past[0] // 2: 3, past[0] - 1: 4, total - 1: 5}              # position: channel
+    for pos in at:
+        kp[table[0, pos // page], pos % page, :, 0] = 0.0 if weight else -8000.0        # a logit of -700 and less: exp is 0 in 32 bits
+    want = oracle.attention(q, kp, torch.where(vp.isfinite(), vp, 0.0), table, torch.tensor(past), q_start, causal=True)
+    for pos, channel in at.items():
+        vp[table[0, pos // page], pos % page, :, channel] = math.inf
+    assert kernel(plan, q.to(DEV), kp.to(DEV))[0] == rows
+    got = PA.paged_attention(q.to(DEV), kp.to(DEV), vp.to(DEV), plan, causal=True).cpu()
+    end = torch.arange(n[0]) + past[0] + 1
+    for pos, channel in at.items():
+        assert not got[end > pos][:, :, channel].isfinite().any() and got[end <= pos][:, :, channel].isfinite().all()
+        assert not weight or (got[end > pos][:, :, channel] == math.inf).all()
+    rest = torch.ones(D, dtype=torch.bool)
+    rest[list(at.values())] = False
+    want["out"], want["mag"] = want["out"][..., rest], want["mag"][..., rest]
+    close(got[..., rest], None, want, dtype)
