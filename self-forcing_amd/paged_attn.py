@@ -75,7 +75,7 @@ def _plan_bytes(requests):
 
 
 def plan_pages(table, past, new, free, tokens, page_size, next_free=None):
-    """Block table, slots and row offsets of a step, on the GPU in one launch.
+    """Block table, slots and row offsets of a step, on the GPU in one launch (two for more than 8192 requests).
 
     table int32 [requests, width], whose entries for the tokens before the step are read and whose entries for the pages that the new tokens
     open are written in place; past, new int32 [requests]; free int32 list of free pages, taken from the front, or from
@@ -299,7 +299,14 @@ def paged_attention(q, k_pages, v_pages, plan, sm_scale=None, causal=False, wind
     has stay as they were; out in q, the pools or the plan is refused); with return_lse also the natural logarithm of the sums, fp32
     [heads, tokens], -inf for nothing.  Rows that would read a position without a page (-1 or another number outside the pool,
     positions past the table) are NaN, and others of their request may be.  What lies in positions that a row does not see has no part in it,
-    NaN or infinite; an infinity in a channel of V that it does see makes that channel infinite, or NaN if its weight is too small for the type.  table[:, :n] of the columns in use sizes the work."""
+    NaN or infinite; an infinity in a channel of V that it does see makes that channel infinite, or NaN if its weight is too small for the type.
+
+    Sums and softmax statistics are fp32; 16-bit tensors with head sizes 64 and 128 take the weights rounded to their type into the product
+    with V, as attention.attention does (off 64 bits by 1.2 to 1.4 times as much as a result that is only rounded itself).
+
+    Which kernel a call takes, and into how many ranges its keys are cut, follows what the host knows: rows and requests on average, and the table's
+    width.  table[:, :n] of the columns in use, few rows of nobody, few waiting requests, and prompts and single tokens in calls of their own cost less
+    time; results do not depend on it but for the order of sums."""
     if (torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad or (
             out is not None and out.requires_grad))) or _tangents(q, k_pages, v_pages, out):
         raise NotImplementedError("paged_attention is not differentiable")
@@ -363,7 +370,9 @@ def select_pages(q, means, plan, top, group=1, causal=False, first=1, last=1):
 
     Candidates are the pages up to the last one that the group's last token sees (causal: its own).  The first `first` and the last `last` of
     them are taken, and then those with the largest (sum of q over the group's tokens and the key head's query heads) . mean key, up
-    to `top` in all; of level ones the lower.  means: fp32 [pages, kv_heads, head_dim], kept by write_pages.  Scores are sums in 64 bits,
+    to `top` in all; of level ones the lower.  A group's tokens share that choice, the earlier ones with what the later ones ask for, and where a group
+    crosses a page the forced last page is not every token's own: last = (group + page_size - 2) // page_size + 1 forces all of those; with
+    less a token of a causal group may find none of its pages taken, and gets zeros.  means: fp32 [pages, kv_heads, head_dim], kept by write_pages.  Scores are sums in 64 bits,
     so that which page is ahead does not hang on the order of an addition; NaN counts as -inf, as does a page outside the pool.  Group i of request r
     is row q_start[r] // group + r + i; rows that nobody has are -1."""
     if (torch.is_grad_enabled() and (q.requires_grad or means.requires_grad)) or _tangents(q, means):

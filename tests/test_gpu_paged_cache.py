@@ -305,3 +305,19 @@ def test_select_for_more_rows_than_a_pass_takes():
         want = oracle.select_pages(q[r:r + 1].cpu(), means.cpu(), plan.table[r:r + 1].cpu(), past[r:r + 1], torch.tensor([0, 1]), page, 4, 1, True, 1, 1)
         assert torch.equal(got[2 * r].cpu().long(), want[0])
     assert bool((got[1::2] == -1).all())                   # rows that nobody has
+
+
+@pytest.mark.parametrize("group,page", [(1, 8), (7, 8), (8, 8), (9, 8), (10, 8), (40, 16), (128, 64), (33, 1560)])
+def test_last_pages_of_a_group_hold_every_tokens_own(group, page):
+    past, n, Hk = [3 * page - 1, 5], [2 * group + 3, group], 2
+    plan, pages, table, q_start, q, means = select_inputs(past, n, page, 2, Hk, 64, 0, torch.bfloat16)
+    last = (group + page - 2) // page + 1
+    for more in (0, -1):
+        got = PA.select_pages(q.to(DEV), means.to(DEV), plan, last + 1, group=group, causal=True, first=0, last=last + more)
+        assert torch.equal(got.cpu().long(), oracle.select_pages(q, means, table, torch.tensor(past), q_start, page, last + 1, group, True, 0, last + more))
+    got, own = PA.select_pages(q.to(DEV), means.to(DEV), plan, last, group=group, causal=True, first=0, last=last).cpu(), []
+    for r in range(2):
+        for t in range(n[r]):
+            row = got[int(q_start[r]) // group + r + t // group]
+            own.append(bool((row == (past[r] + t) // page).any(1).all()))
+    assert all(own)
