@@ -547,6 +547,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(PagedArgs a, int64_t 
 // Pieces of 32 NW rows.  The tiles that all of them see whole run through the dense kernel's loop (two K and two V buffers, tiles
 // straight from memory into LDS, the logits of tile n + 1 beside the exponentials of tile n, its maximum beside P V of tile n); those that
 // some row sees in part (the request's own new tokens under a causal mask, a window's edge, the last tile) follow in a plain loop.
+// (The loop is written out here again, since its loads differ: what is changed in the one is to be measured in the other.)
 // Where the whole tiles' blocks lie is worked out by all threads together and kept in LDS, 8 bytes a block, for a stretch of tiles at a
 // time (a request's page table row is read once per workgroup, not once per wave); a step reads one tile's eight offsets, a
 // step before it asks for that tile, and V's rows take the offsets that K's were read with.  (Looked up by each wave as it went, eight tiles at a
