@@ -1048,11 +1048,11 @@ static PagedPlan paged_plan(const sfm_paged_desc& d) {
         // in place of 376, with the same number but 97 in one request 356 (382); with 16 rows 376 (402), with 481 in one 493 (458);
         // with 31 rows 406 (435), with 961 in one 656 (542).
         p.once = (mean <= 16 || d.tokens <= d.requests) && n * tiles * 64.0 * d.D * 4 > 512e6;
-        // Selected pages make rows equally long.  Where those of half the chip's compute units or more are few and lie in the memory-side cache,
-        // one range of all of them is faster than ranges that are joined: 16 tokens, 8 key heads of 128, 2048 positions each, 29.5 us
-        // and 34.1; 32 tokens of 64 28.4 and 35.8.  Past the cache, where loads take longer, and past 3200 positions, where the
-        // longest chain sets the time, ranges win: 64 tokens, 4096 positions each, 128: 238 us and 191, 64: 157 and 115.
-        if (d.top && n >= cu / 2 && tiles <= 50 && n * tiles * 64.0 * d.D * 4 <= 256e6) chunks = 1;
+        // Selected pages make rows equally long.  Where those of half the chip's compute units or more are few and fit the memory-side cache, one
+        // range of all of them is as fast as ranges that are joined, or faster: 32 tokens, 8 key heads of 64, 1024 positions each, pages from
+        // memory, 26.5 us and 33.2 (pages from the caches 18.4 and 26.4); 16 tokens, 128, 2048 each 42.9 and 42.5 (29.5 and 34.1).  Beyond, the longest
+        // chain of loads sets the time: 64 tokens, 4096 positions each, 128: 249 and 209 (238 and 191), 64: 170 and 128 (157 and 115).
+        if (d.top && n >= cu / 2 && tiles <= 40 && n * tiles * 64.0 * d.D * 4 <= 256e6) chunks = 1;
     } else if (p.rows == 128 && tiles >= 16) {                        // 256 rows are taken only where their pieces fill the chip
         const double scale = d.D == 64 ? 0.6 : 1.0, partial_ns = (double)d.H * d.tokens * (d.D + 2) * 8 / 3500;
         double t1 = 0, best = 0;
